@@ -120,6 +120,15 @@ SIGNATURES = {
     "atlas_hip_kv_append_f32": [CTX, P, P, P, U32, U32, P, U32, c_int, F],
     "atlas_hip_kv_append_q8_0": [CTX, P, P, P, U32, U32, P, U32, c_int, F],
     "atlas_hip_kv_append_q4_0": [CTX, P, P, P, U32, U32, P, U32, c_int, F],
+    "atlas_hip_prefix_attention_workspace": [CTX, c_int, U32, U32, U32, U32, U32, U32, U32, c_int, POINTER(c_uint64)],
+    "atlas_hip_prefix_attention_f32": [CTX, P, P, U32, U32, P, P, U32, P, P, P, U32, U32, U32, U32, U32, F, P, U64],
+    "atlas_hip_prefix_attention_q8_0": [CTX, P, P, U32, U32, P, P, U32, P, P, P, U32, U32, U32, U32, U32, F, P, U64],
+    "atlas_hip_prefix_attention_q4_0": [CTX, P, P, U32, U32, P, P, U32, P, P, P, U32, U32, U32, U32, U32, F, P, U64],
+    "atlas_hip_kv_evict_f32": [CTX, P, P, P, P, P, P, P, U32, U32, U32, U32, U32],
+    "atlas_hip_kv_evict_q8_0": [CTX, P, P, P, P, P, P, P, U32, U32, U32, U32, U32],
+    "atlas_hip_kv_evict_q4_0": [CTX, P, P, P, P, P, P, P, U32, U32, U32, U32, U32],
+    "atlas_hip_verify_draft_workspace": [CTX, U32, U32, U32, POINTER(c_uint64)],
+    "atlas_hip_verify_draft_f32": [CTX, P, P, P, P, P, P, P, P, U32, U32, U32, c_double, P, U64],
     "atlas_hip_softcap_f32": [CTX, P, P, U64, F],
     "atlas_hip_argmax_f32": [CTX, P, P, U32, U32],
     "atlas_hip_softcap_argmax_f32": [CTX, P, P, P, U32, U32, F],

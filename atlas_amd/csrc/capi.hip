@@ -5,6 +5,7 @@
 // (crates/atlas-ops/src/lib.rs:20-147) over MetalRuntime's wrappers
 // (crates/atlas-metal/src/lib.rs:1323-1733, 1897-1926).
 #include "../../include/atlas_hip_ops.h"
+#include "decode_checks.hpp"
 #include "launch.hpp"
 
 #include <hip/hip_runtime.h>
@@ -869,6 +870,135 @@ int atlas_hip_kv_append_q4_0(atlas_hip_ctx* ctx, const float* key, const float* 
                              int vnorm, float epsilon) {
     return kv_append(ctx, atlas::kKvQ4_0, key, value, cache, kv_width, capacity, positions, tokens, vnorm, epsilon,
                      "kv_append_q4_0");
+}
+
+// ---------------------------------------------------------------------------
+// decoding a batch behind a shared prompt
+// ---------------------------------------------------------------------------
+
+static int checked(atlas_hip_ctx* ctx, const char* error) { return error ? invalid(ctx, error) : ATLAS_OK; }
+
+int atlas_hip_prefix_attention_workspace(atlas_hip_ctx* ctx, int format, uint32_t sequences, uint32_t tokens,
+                                         uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                                         uint32_t prefix_length, uint32_t capacity, int weights, uint64_t* bytes) {
+    if (!ctx) return ATLAS_ERR_INVALID_INPUT;
+    if (!bytes) return invalid(ctx, "null output pointer");
+    *bytes = 0;
+    float any = 0.0f;  // only whether weights_out is null counts
+    atlas::PrefixAttentionArgs a{};
+    a.format = format;
+    a.sequences = sequences;
+    a.tokens = tokens;
+    a.q_heads = q_heads;
+    a.kv_heads = kv_heads;
+    a.head_dim = head_dim;
+    a.prefix_length = prefix_length;
+    a.capacity = capacity;
+    a.weights_out = weights ? &any : nullptr;
+    if (int rc = checked(ctx, atlas::prefix_attention_sizes_error(a))) return rc;
+    *bytes = atlas::prefix_attention_workspace(a);
+    return ATLAS_OK;
+}
+
+static int prefix_attention(atlas_hip_ctx* ctx, const atlas::PrefixAttentionArgs& a, uint64_t workspace_bytes, const char* op) {
+    int rc = enter(ctx);
+    if (rc) return rc;
+    if ((rc = checked(ctx, atlas::prefix_attention_error(a)))) return rc;
+    if (workspace_bytes < atlas::prefix_attention_workspace(a)) return invalid(ctx, "prefix attention workspace is too small");
+    return launched(ctx, atlas::launch_prefix_attention(ctx->stream, a), op);
+}
+
+int atlas_hip_prefix_attention_f32(atlas_hip_ctx* ctx, const float* q, const float* prefix, uint32_t prefix_length,
+                                   uint32_t prefix_capacity, const float* cache, const uint32_t* lengths,
+                                   uint32_t capacity, float* output, const float* weights_in, float* weights_out,
+                                   uint32_t sequences, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                                   uint32_t head_dim, float scale, void* workspace, uint64_t workspace_bytes) {
+    const atlas::PrefixAttentionArgs a{atlas::kKvF32, q, reinterpret_cast<const uint8_t*>(prefix), prefix_length,
+                                       prefix_capacity, reinterpret_cast<const uint8_t*>(cache), lengths, capacity,
+                                       output, weights_in, weights_out, sequences, tokens, q_heads, kv_heads, head_dim,
+                                       scale, workspace};
+    return prefix_attention(ctx, a, workspace_bytes, "prefix_attention_f32");
+}
+
+int atlas_hip_prefix_attention_q8_0(atlas_hip_ctx* ctx, const float* q, const uint8_t* prefix, uint32_t prefix_length,
+                                    uint32_t prefix_capacity, const uint8_t* cache, const uint32_t* lengths,
+                                    uint32_t capacity, float* output, const float* weights_in, float* weights_out,
+                                    uint32_t sequences, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                                    uint32_t head_dim, float scale, void* workspace, uint64_t workspace_bytes) {
+    const atlas::PrefixAttentionArgs a{atlas::kKvQ8_0, q, prefix, prefix_length, prefix_capacity, cache, lengths, capacity,
+                                       output, weights_in, weights_out, sequences, tokens, q_heads, kv_heads, head_dim,
+                                       scale, workspace};
+    return prefix_attention(ctx, a, workspace_bytes, "prefix_attention_q8_0");
+}
+
+int atlas_hip_prefix_attention_q4_0(atlas_hip_ctx* ctx, const float* q, const uint8_t* prefix, uint32_t prefix_length,
+                                    uint32_t prefix_capacity, const uint8_t* cache, const uint32_t* lengths,
+                                    uint32_t capacity, float* output, const float* weights_in, float* weights_out,
+                                    uint32_t sequences, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                                    uint32_t head_dim, float scale, void* workspace, uint64_t workspace_bytes) {
+    const atlas::PrefixAttentionArgs a{atlas::kKvQ4_0, q, prefix, prefix_length, prefix_capacity, cache, lengths, capacity,
+                                       output, weights_in, weights_out, sequences, tokens, q_heads, kv_heads, head_dim,
+                                       scale, workspace};
+    return prefix_attention(ctx, a, workspace_bytes, "prefix_attention_q4_0");
+}
+
+static int kv_evict(atlas_hip_ctx* ctx, int format, const void* cache, void* cache_out, const float* weights,
+                    float* weights_out, const uint32_t* lengths, uint32_t* lengths_out, uint32_t* kept,
+                    uint32_t sequences, uint32_t capacity, uint32_t kv_width, uint32_t budget, uint32_t recent,
+                    const char* op) {
+    int rc = enter(ctx);
+    if (rc) return rc;
+    atlas::KvEvictArgs a{static_cast<const uint8_t*>(cache), static_cast<uint8_t*>(cache_out), weights, weights_out, lengths,
+                         lengths_out, kept, sequences, capacity, 0, budget, recent};
+    if ((rc = checked(ctx, atlas::kv_evict_error(a, format, kv_width)))) return rc;
+    a.row_bytes = static_cast<uint32_t>(atlas::kv_row_bytes(format, kv_width));
+    return launched(ctx, atlas::launch_kv_evict(ctx->stream, a), op);
+}
+
+int atlas_hip_kv_evict_f32(atlas_hip_ctx* ctx, const float* cache, float* cache_out, const float* weights,
+                           float* weights_out, const uint32_t* lengths, uint32_t* lengths_out, uint32_t* kept,
+                           uint32_t sequences, uint32_t capacity, uint32_t kv_width, uint32_t budget, uint32_t recent) {
+    return kv_evict(ctx, atlas::kKvF32, cache, cache_out, weights, weights_out, lengths, lengths_out, kept, sequences,
+                    capacity, kv_width, budget, recent, "kv_evict_f32");
+}
+
+int atlas_hip_kv_evict_q8_0(atlas_hip_ctx* ctx, const uint8_t* cache, uint8_t* cache_out, const float* weights,
+                            float* weights_out, const uint32_t* lengths, uint32_t* lengths_out, uint32_t* kept,
+                            uint32_t sequences, uint32_t capacity, uint32_t kv_width, uint32_t budget, uint32_t recent) {
+    return kv_evict(ctx, atlas::kKvQ8_0, cache, cache_out, weights, weights_out, lengths, lengths_out, kept, sequences,
+                    capacity, kv_width, budget, recent, "kv_evict_q8_0");
+}
+
+int atlas_hip_kv_evict_q4_0(atlas_hip_ctx* ctx, const uint8_t* cache, uint8_t* cache_out, const float* weights,
+                            float* weights_out, const uint32_t* lengths, uint32_t* lengths_out, uint32_t* kept,
+                            uint32_t sequences, uint32_t capacity, uint32_t kv_width, uint32_t budget, uint32_t recent) {
+    return kv_evict(ctx, atlas::kKvQ4_0, cache, cache_out, weights, weights_out, lengths, lengths_out, kept, sequences,
+                    capacity, kv_width, budget, recent, "kv_evict_q4_0");
+}
+
+int atlas_hip_verify_draft_workspace(atlas_hip_ctx* ctx, uint32_t sequences, uint32_t drafts, uint32_t vocab,
+                                     uint64_t* bytes) {
+    if (!ctx) return ATLAS_ERR_INVALID_INPUT;
+    if (!bytes) return invalid(ctx, "null output pointer");
+    *bytes = 0;
+    if (int rc = checked(ctx, atlas::verify_draft_sizes_error(sequences, drafts, vocab))) return rc;
+    *bytes = atlas::verify_draft_workspace(sequences, drafts, vocab);
+    return ATLAS_OK;
+}
+
+int atlas_hip_verify_draft_f32(atlas_hip_ctx* ctx, const float* target_logits, const float* draft_logits,
+                               const uint32_t* draft_tokens, const uint32_t* draft_lengths,
+                               const float* accept_uniform, const float* sample_uniform, uint32_t* accepted,
+                               uint32_t* tokens, uint32_t sequences, uint32_t drafts, uint32_t vocab,
+                               double inv_temperature, void* workspace, uint64_t workspace_bytes) {
+    int rc = enter(ctx);
+    if (rc) return rc;
+    const atlas::VerifyDraftArgs a{target_logits, draft_logits, draft_tokens, draft_lengths, accept_uniform, sample_uniform,
+                                   accepted, tokens, sequences, drafts, vocab, inv_temperature, workspace};
+    if ((rc = checked(ctx, atlas::verify_draft_error(a)))) return rc;
+    if (workspace_bytes < atlas::verify_draft_workspace(sequences, drafts, vocab))
+        return invalid(ctx, "draft verification workspace is too small");
+    return launched(ctx, atlas::launch_verify_draft(ctx->stream, a), "verify_draft_f32");
 }
 
 // ---------------------------------------------------------------------------

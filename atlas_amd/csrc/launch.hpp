@@ -170,6 +170,59 @@ struct KvAppendArgs {
 };
 hipError_t launch_kv_append(hipStream_t stream, int format, bool vnorm, const KvAppendArgs& a);
 
+// Attention over a shared prompt's cache and the sequences' own
+// (prefix_attention_kernels.hip).  Caches as kv_append writes them: the shared
+// one [K | V][prefix_capacity][kv_heads * head_dim], the own ones together
+// [K | V][sequences * capacity][kv_heads * head_dim].
+struct PrefixAttentionArgs {
+    int format;               // KvFormat of both caches
+    const float* q;           // [sequences, tokens, q_heads, head_dim]
+    const uint8_t* prefix;    // null when prefix_length is 0
+    uint32_t prefix_length, prefix_capacity;
+    const uint8_t* cache;     // null when capacity is 0
+    const uint32_t* lengths;  // [sequences], device
+    uint32_t capacity;
+    float* output;            // as q
+    const float* weights_in;  // [sequences, capacity], or null: zeros
+    float* weights_out;       // or null
+    uint32_t sequences, tokens, q_heads, kv_heads, head_dim;
+    float scale;
+    void* workspace;
+};
+// Bytes of workspace (weights_out null or not matters, no pointer is read).
+uint64_t prefix_attention_workspace(const PrefixAttentionArgs& a);
+hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs& a);
+
+// Cutting caches to a budget by added-up weight (kv_evict_kernels.hip).
+struct KvEvictArgs {
+    const uint8_t* cache;    // [K | V][sequences * capacity][row_bytes]
+    uint8_t* cache_out;      // may be cache
+    const float* weights;    // [sequences, capacity]
+    float* weights_out;      // may be weights
+    const uint32_t* lengths; // [sequences], device
+    uint32_t* lengths_out;   // may be lengths
+    uint32_t* kept;          // [sequences, budget]
+    uint32_t sequences, capacity, row_bytes, budget, recent;
+};
+hipError_t launch_kv_evict(hipStream_t stream, const KvEvictArgs& a);
+
+// Verification of drafted tokens (verify_kernels.hip).
+struct VerifyDraftArgs {
+    const float* target;            // [sequences, drafts + 1, vocab]
+    const float* draft;             // [sequences, drafts, vocab], or null: proposed with certainty
+    const uint32_t* draft_tokens;   // [sequences, drafts]
+    const uint32_t* draft_lengths;  // [sequences], or null: all drafts
+    const float* accept_uniform;    // [sequences, drafts]
+    const float* sample_uniform;    // [sequences]
+    uint32_t* accepted;             // [sequences]
+    uint32_t* tokens;               // [sequences, drafts + 1]
+    uint32_t sequences, drafts, vocab;
+    double inv_temperature;
+    void* workspace;
+};
+uint64_t verify_draft_workspace(uint32_t sequences, uint32_t drafts, uint32_t vocab);
+hipError_t launch_verify_draft(hipStream_t stream, const VerifyDraftArgs& a);
+
 // Logit soft cap and argmax (logits_kernels.hip).  The argmax of a row split
 // over several workgroups goes through a workspace owned by the context:
 // one 64-bit slot per workgroup (at most kArgmaxSlotsPerRow per row), written

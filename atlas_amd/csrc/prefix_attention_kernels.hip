@@ -1,0 +1,531 @@
+// prefix_attention_kernels.hip -- attention of a batch's new tokens over a
+// prompt that all sequences share and over each sequence's own cache, reading
+// the caches that the KV append writes ([K | V][position][row]; f32, Q8_0 or
+// Q4_0 rows).  No counterpart in the reference, whose executors decode one
+// sequence.
+//
+// For query head h of token t of sequence b, with KV head h / group:
+//   x_j = scale * (q . k_j) over the prompt's rows and own rows
+//         j < len_b - (tokens - 1 - t),
+//   out = sum_j e^{x_j} v_j / sum_j e^{x_j}, zero where nothing is seen.
+// The sum over j is split into segments (parts of the prompt, parts of the
+// sequence's own rows); a segment leaves its maximum m, its sum l of 2^{x - m}
+// and its sum O of 2^{x - m} v, and a second launch joins a row's segments:
+// out = sum_s 2^{m_s - M} O_s / sum_s 2^{m_s - M} l_s.  The prompt's segments
+// hold the rows of all sequences, so its cache is read once for the batch.
+#include "device_common.hpp"
+#include "launch.hpp"
+
+namespace atlas {
+namespace {
+
+constexpr int kAttnThreads = 256;
+constexpr int kAttnWaves = kAttnThreads / kWave;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+typedef f32x4 f32x4_b4 __attribute__((aligned(4)));
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// ---------------------------------------------------------------------------
+// Rows of a cache as MFMA operands.  A product over dims may take them in any
+// order that both operands share, and so may the rows of a result, so each
+// format has the order in which a lane's values are contiguous in memory.
+//   key_dim:   dims 32 blk + ... of lane group a = lane / 16, j < 8
+//   value_dim: dims 64 g + ... of lane m = lane % 16, j < 4
+// ---------------------------------------------------------------------------
+template <int FMT>
+__device__ __forceinline__ uint32_t key_dim(uint32_t blk, uint32_t a, uint32_t j) {
+    if (FMT == kKvQ4_0) return 32 * blk + 4 * a + (j & 3) + 16 * (j >> 2);
+    return 32 * blk + 8 * a + j;
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t value_dim(uint32_t g, uint32_t m, uint32_t j) {
+    if (FMT == kKvQ4_0) return 64 * g + 32 * (m >> 3) + 2 * (m & 7) + (j & 1) + 16 * (j >> 1);
+    return 64 * g + 4 * m + j;
+}
+
+template <int FMT>
+__device__ __forceinline__ uint64_t head_offset(uint32_t head, uint32_t head_dim) {
+    if (FMT == kKvF32) return static_cast<uint64_t>(head) * head_dim * 4;
+    return static_cast<uint64_t>(head) * (head_dim / 32) * (FMT == kKvQ8_0 ? 34 : 18);
+}
+
+typedef uint32_t u32_a2 __attribute__((aligned(2)));
+typedef u32x2_t u32x2_a2 __attribute__((aligned(2)));
+
+// The 8 values of block `blk` of a key row's head that lane group `a` holds.
+template <int FMT>
+__device__ __forceinline__ void load_key8(const uint8_t* head, uint32_t blk, uint32_t a, uint32_t head_dim, float* v) {
+    if constexpr (FMT == kKvF32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t dim = 32 * blk + 8 * a + 4 * h;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (dim < head_dim) x = *reinterpret_cast<const f32x4*>(head + dim * 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * h + j] = x[j];
+        }
+    } else if (32 * blk >= head_dim) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    } else if constexpr (FMT == kKvQ8_0) {
+        const uint8_t* p = head + blk * 34;
+        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
+        const u32x2_t c = *reinterpret_cast<const u32x2_a2*>(p + 2 + 8 * a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? c.x : c.y) >> (8 * (j & 3)))) * d;
+    } else {
+        const uint8_t* p = head + blk * 18;
+        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
+        const uint32_t c = *reinterpret_cast<const u32_a2*>(p + 2 + 4 * a);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 3) + 4 * (j >> 2))) & 15u) - 8) * d;
+    }
+}
+
+// The 4 values of group `g` of a value row's head that lane m holds.
+template <int FMT>
+__device__ __forceinline__ void load_value4(const uint8_t* head, uint32_t g, uint32_t m, uint32_t head_dim, float* v) {
+    const uint32_t dim = value_dim<FMT>(g, m, 0);
+    if (dim >= head_dim) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = 0.0f;
+    } else if constexpr (FMT == kKvF32) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(head + dim * 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = x[j];
+    } else if constexpr (FMT == kKvQ8_0) {
+        const uint8_t* p = head + (dim / 32) * 34;
+        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
+        const uint32_t c = *reinterpret_cast<const u32_a2*>(p + 2 + dim % 32);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(static_cast<int8_t>(c >> (8 * j))) * d;
+    } else {
+        const uint8_t* p = head + (dim / 32) * 18;
+        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
+        const uint32_t c = *reinterpret_cast<const uint16_t*>(p + 2 + 2 * (m & 7));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 1) + 4 * (j >> 1))) & 15u) - 8) * d;
+    }
+}
+
+struct AttnParams {
+    const float* q;
+    const uint8_t* prefix;       // K plane; V plane prefix_plane bytes on
+    const uint8_t* cache;        // K plane; V plane cache_plane bytes on
+    const uint32_t* lengths;
+    float* partial_out;          // [slot][kv head][row][head_dim]
+    float2* partial_ml;          // [slot][kv head][row]
+    float* scores;               // [sequence][kv head][row][score_pitch], or null
+    uint64_t prefix_plane, cache_plane;
+    uint32_t row_bytes, prefix_length, capacity, score_pitch;
+    uint32_t tokens, q_heads, kv_heads, group, head_dim;
+    uint32_t rows;               // of one KV head: sequences * tokens * group
+    uint32_t seq_rows;           // tokens * group
+    uint32_t prefix_tiles, prefix_slots, own_tiles, own_slots, prefix_items;
+    float scale;                 // with log2(e)
+};
+
+// out += the products of the keys that a row sees, key by key: for the tiles
+// where a key that only some rows see holds values that are no numbers.
+template <int NG>
+__device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const float (&p)[4], uint32_t key0, uint32_t seen,
+                                      f32x4 (&out)[NG * 4]) {
+    const uint32_t lane = threadIdx.x % kWave, n = lane % 16, quarter = lane / 16;
+    for (uint32_t from = 0; from < 4; ++from)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool sees = key0 + 4 * from + r < seen;
+            const float weight = __shfl(p[r], static_cast<int>(n + 16 * from), kWave);
+#pragma unroll
+            for (int g = 0; g < NG * 4; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = __shfl(v[r][g], static_cast<int>(4 * quarter + i + 16 * from), kWave);
+                    out[g][i] = sees ? out[g][i] + weight * x : out[g][i];
+                }
+        }
+}
+
+// One workgroup: 16 * NR query rows of one KV head against one segment.  The
+// wavefronts take its keys 16 at a time in turn, each with a running maximum,
+// sum and accumulator of its own, and join through LDS at the end.  Products
+// are v_mfma_f32_16x16x4: S^T = K Q^T leaves lane l with query row l % 16 and
+// keys 4 (l / 16) + r, which is the operand that O^T = V^T P^T wants, so P
+// never leaves its registers; the row's statistics are a lane's own.
+template <int FMT, int NB, int NR>
+__global__ __launch_bounds__(kAttnThreads) void attn_rows_kernel(AttnParams a) {
+    constexpr int NG = (NB + 1) / 2;  // groups of 64 dims
+    constexpr int kDims = 64 * NG;
+    __shared__ float2 wave_ml[kAttnWaves][16];
+    __shared__ float wave_out[kAttnWaves][16][kDims + 4];
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+    const uint32_t n = lane % 16, quarter = lane / 16;
+
+    // which rows, which keys
+    uint32_t item = blockIdx.x;
+    const bool shared = item < a.prefix_items;
+    uint32_t kv_head, row0, row_end, slot, key_begin, key_end, length = 0, seq = 0;
+    const uint8_t *keys, *values;
+    if (shared) {
+        const uint32_t tile = item % a.prefix_tiles;
+        item /= a.prefix_tiles;
+        slot = item % a.prefix_slots;
+        kv_head = item / a.prefix_slots;
+        row0 = tile * 16 * NR;
+        row_end = a.rows;
+        const uint32_t part = ((a.prefix_length + a.prefix_slots - 1) / a.prefix_slots + 63) / 64 * 64;
+        key_begin = min(slot * part, a.prefix_length);
+        key_end = min(key_begin + part, a.prefix_length);
+        keys = a.prefix;
+        values = a.prefix + a.prefix_plane;
+    } else {
+        item -= a.prefix_items;
+        const uint32_t tile = item % a.own_tiles;
+        item /= a.own_tiles;
+        const uint32_t part_index = item % a.own_slots;
+        item /= a.own_slots;
+        kv_head = item % a.kv_heads;
+        seq = item / a.kv_heads;
+        slot = a.prefix_slots + part_index;
+        row0 = seq * a.seq_rows + tile * 16 * NR;
+        row_end = (seq + 1) * a.seq_rows;
+        length = min(a.lengths[seq], a.capacity);
+        const uint32_t part = ((length + a.own_slots - 1) / a.own_slots + 63) / 64 * 64;
+        key_begin = min(part_index * part, length);
+        key_end = min(key_begin + part, length);
+        const uint64_t base = static_cast<uint64_t>(seq) * a.capacity * a.row_bytes;
+        keys = a.cache + base;
+        values = a.cache + a.cache_plane + base;
+    }
+    keys += head_offset<FMT>(kv_head, a.head_dim);
+    values += head_offset<FMT>(kv_head, a.head_dim);
+
+    float q[NR][NB * 8];
+    uint32_t seen[NR];  // keys below it are seen by the lane's row
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+        const uint32_t row = row0 + 16 * t + n;
+        const bool there = row < row_end;
+        const uint32_t at = there ? row : row_end - 1;
+        const float* p = a.q + (static_cast<uint64_t>(at / a.group) * a.q_heads + kv_head * a.group + at % a.group) * a.head_dim;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t dim = key_dim<FMT>(b, quarter, j);
+                q[t][8 * b + j] = dim < a.head_dim ? p[dim] * a.scale : 0.0f;
+            }
+        if (shared) {
+            seen[t] = key_end;
+        } else {
+            const uint32_t behind = a.tokens - 1 - (at - seq * a.seq_rows) / a.group;
+            seen[t] = min(length > behind ? length - behind : 0u, key_end);
+        }
+        if (!there) seen[t] = 0;
+    }
+
+    float m[NR], l[NR];
+    f32x4 out[NR][NG * 4];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+        m[t] = neg_inf();
+        l[t] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NG * 4; ++i) out[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    for (uint32_t key0 = key_begin + wave * 16; key0 < key_end; key0 += kAttnWaves * 16) {
+        float k[NB * 8], v[4][NG * 4];
+        {
+            const uint8_t* row = keys + static_cast<uint64_t>(min(key0 + n, key_end - 1)) * a.row_bytes;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) load_key8<FMT>(row, b, quarter, a.head_dim, k + 8 * b);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint8_t* row = values + static_cast<uint64_t>(min(key0 + 4 * quarter + r, key_end - 1)) * a.row_bytes;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) load_value4<FMT>(row, g, n, a.head_dim, v[r] + 4 * g);
+        }
+        // keys that some rows see and others do not: a value there that is no
+        // number must not reach the others as 0 * v
+        bool stained = false;
+        if (!shared && a.tokens > 1 && key0 + 16 + a.tokens > length + 1) {
+            float any = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < NG * 4; ++i) any = __builtin_fmaf(v[r][i], 0.0f, any);
+            stained = __builtin_amdgcn_ballot_w64(any != 0.0f) != 0;
+        }
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < NB * 8; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i], q[t][i], s, 0, 0, 0);
+            float top = neg_inf();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[r] = key0 + 4 * quarter + r < seen[t] ? s[r] : neg_inf();
+                top = fmaxf(top, s[r]);
+            }
+            if (!shared && a.scores) {
+                const uint32_t row = row0 + 16 * t + n;
+                if (row < row_end && key0 + 4 * quarter < key_end) {
+                    const uint64_t line = (static_cast<uint64_t>(seq) * a.kv_heads + kv_head) * a.seq_rows + row - seq * a.seq_rows;
+                    *reinterpret_cast<f32x4*>(a.scores + line * a.score_pitch + key0 + 4 * quarter) = s;
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, kWave));
+            top = fmaxf(top, __shfl_xor(top, 32, kWave));
+            const float m_new = fmaxf(m[t], top);
+            const float base = m_new == neg_inf() ? 0.0f : m_new;
+            const float fade = __builtin_amdgcn_exp2f(m[t] - base);
+            m[t] = m_new;
+            float p[4];
+            l[t] *= fade;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(s[r] - base);
+                l[t] += p[r];
+            }
+#pragma unroll
+            for (int i = 0; i < NG * 4; ++i) out[t][i] *= fade;
+            if (stained) {
+                add_seen<NG>(v, p, key0, seen[t], out[t]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < NG * 4; ++i)
+                        out[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i], p[r], out[t][i], 0, 0, 0);
+            }
+        }
+    }
+
+    // join the wavefronts
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+        l[t] += __shfl_xor(l[t], 16, kWave);
+        l[t] += __shfl_xor(l[t], 32, kWave);
+        if (t) __syncthreads();
+        if (quarter == 0) wave_ml[wave][n] = make_float2(m[t], l[t]);
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    wave_out[wave][n][value_dim<FMT>(g, 4 * quarter + i, j)] = out[t][4 * g + j][i];
+        __syncthreads();
+        const uint32_t per_row = a.head_dim / 4;
+        for (uint32_t i = threadIdx.x; i < 16 * per_row; i += kAttnThreads) {
+            const uint32_t r = i / per_row, d = 4 * (i % per_row);
+            const uint32_t row = row0 + 16 * t + r;
+            if (row >= row_end) break;
+            float top = wave_ml[0][r].x;
+#pragma unroll
+            for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, wave_ml[w][r].x);
+            const float base = top == neg_inf() ? 0.0f : top;
+            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kAttnWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(wave_ml[w][r].x - base);
+                sum += f * wave_ml[w][r].y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] += f * wave_out[w][r][d + j];
+            }
+            const uint64_t at = (static_cast<uint64_t>(slot) * a.kv_heads + kv_head) * a.rows + row;
+            if (d == 0) a.partial_ml[at] = make_float2(top, sum);
+            *reinterpret_cast<f32x4*>(a.partial_out + at * a.head_dim + d) = o;
+        }
+    }
+}
+
+// One wavefront a row: its segments joined, and the base-2 logarithm of its
+// sum (+inf where it saw nothing) for the weights.
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, float* output, float* log_sum) {
+    const uint64_t all = static_cast<uint64_t>(a.rows) * a.kv_heads;
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kAttnWaves + threadIdx.x / kWave;
+    if (row >= all) return;
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t slots = a.prefix_slots + a.own_slots;
+    float top = neg_inf();
+    for (uint32_t s = 0; s < slots; ++s) top = fmaxf(top, a.partial_ml[s * all + row].x);
+    const float base = top == neg_inf() ? 0.0f : top;
+    float sum = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t s = 0; s < slots; ++s) {
+        const float2 ml = a.partial_ml[s * all + row];
+        const float f = __builtin_amdgcn_exp2f(ml.x - base);
+        sum += f * ml.y;
+        if (4 * lane < a.head_dim) {
+            const f32x4 part = *reinterpret_cast<const f32x4*>(a.partial_out + (s * all + row) * a.head_dim + 4 * lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] += f * part[j];
+        }
+    }
+    const uint32_t kv_head = static_cast<uint32_t>(row / a.rows), r = static_cast<uint32_t>(row % a.rows);
+    if (4 * lane < a.head_dim) {
+        f32x4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = sum == 0.0f ? 0.0f : o[j] / sum;
+        float* p = output + (static_cast<uint64_t>(r / a.group) * a.q_heads + kv_head * a.group + r % a.group) * a.head_dim;
+        *reinterpret_cast<f32x4*>(p + 4 * lane) = y;
+    }
+    if (log_sum && lane == 0) {
+        const uint64_t seq = r / a.seq_rows;
+        log_sum[(seq * a.kv_heads + kv_head) * a.seq_rows + r % a.seq_rows] =
+            sum == 0.0f ? __builtin_inff() : base + __builtin_log2f(sum);
+    }
+}
+
+// A thread a position: the weight it got from every row of its sequence, in
+// row order.
+__global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a, const float* log_sum, const float* in,
+                                                                    float* out) {
+    const uint32_t blocks = (a.capacity + kAttnThreads - 1) / kAttnThreads;
+    const uint32_t seq = blockIdx.x / blocks;
+    const uint32_t length = min(a.lengths[seq], a.capacity);
+    const uint32_t key = blockIdx.x % blocks * kAttnThreads + threadIdx.x;
+    if (key >= length) return;
+    const uint32_t lines = a.kv_heads * a.seq_rows;
+    const uint64_t first = static_cast<uint64_t>(seq) * lines;
+    float sum = 0.0f;
+    for (uint32_t i = 0; i < lines; ++i)
+        sum += __builtin_amdgcn_exp2f(a.scores[(first + i) * a.score_pitch + key] - log_sum[first + i]);
+    const uint64_t at = static_cast<uint64_t>(seq) * a.capacity + key;
+    out[at] = in ? in[at] + sum : sum;
+}
+
+// How the work is laid out, and what of the workspace it takes.
+struct AttnPlan {
+    uint32_t row_tiles;  // of 16 rows a workgroup
+    uint32_t prefix_tiles, prefix_slots, own_tiles, own_slots;
+    uint64_t out_bytes, ml_bytes, score_bytes, log_bytes;
+    uint32_t score_pitch;
+    uint64_t total() const { return out_bytes + ml_bytes + score_bytes + log_bytes; }
+};
+
+uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
+
+AttnPlan attn_plan(const PrefixAttentionArgs& s) {
+    AttnPlan p{};
+    const uint32_t seq_rows = s.tokens * (s.q_heads / s.kv_heads);
+    const uint64_t rows = static_cast<uint64_t>(s.sequences) * seq_rows;
+    p.row_tiles = rows > 16 ? 2 : 1;
+    const uint32_t step = 16 * p.row_tiles;
+    const uint32_t wanted = 1024;  // workgroups
+    if (s.prefix_length) {
+        p.prefix_tiles = static_cast<uint32_t>((rows + step - 1) / step);
+        const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
+        const uint32_t most = (s.prefix_length + 255) / 256;
+        const uint64_t want = (wanted + units - 1) / units;
+        p.prefix_slots = static_cast<uint32_t>(want < most ? want : most);
+        if (p.prefix_slots > 64) p.prefix_slots = 64;
+    }
+    if (s.capacity) {
+        p.own_tiles = (seq_rows + step - 1) / step;
+        const uint64_t units = static_cast<uint64_t>(p.own_tiles) * s.kv_heads * s.sequences;
+        const uint32_t most = (s.capacity + 255) / 256;
+        const uint64_t want = (wanted + units - 1) / units;
+        p.own_slots = static_cast<uint32_t>(want < most ? want : most);
+        if (p.own_slots > 64) p.own_slots = 64;
+    }
+    const uint64_t lines = rows * s.kv_heads, parts = lines * (p.prefix_slots + p.own_slots);
+    p.out_bytes = round256(parts * s.head_dim * 4);
+    p.ml_bytes = round256(parts * 8);
+    if (s.weights_out) {
+        p.score_pitch = (s.capacity + 3) / 4 * 4;
+        p.score_bytes = round256(lines * p.score_pitch * 4);
+        p.log_bytes = round256(lines * 4);
+    }
+    return p;
+}
+
+template <int FMT, int NB, int NR>
+void launch_rows(hipStream_t stream, uint32_t items, const AttnParams& a) {
+    hipLaunchKernelGGL((attn_rows_kernel<FMT, NB, NR>), dim3(items), dim3(kAttnThreads), 0, stream, a);
+}
+
+template <int FMT, int NB>
+void launch_rows(hipStream_t stream, uint32_t items, uint32_t row_tiles, const AttnParams& a) {
+    if (row_tiles == 1)
+        launch_rows<FMT, NB, 1>(stream, items, a);
+    else
+        launch_rows<FMT, NB, 2>(stream, items, a);
+}
+
+template <int FMT>
+void launch_rows(hipStream_t stream, uint32_t items, uint32_t row_tiles, const AttnParams& a) {
+    if (a.head_dim <= 64)
+        launch_rows<FMT, 2>(stream, items, row_tiles, a);
+    else if (a.head_dim <= 128)
+        launch_rows<FMT, 4>(stream, items, row_tiles, a);
+    else
+        launch_rows<FMT, 8>(stream, items, row_tiles, a);
+}
+
+}  // namespace
+
+uint64_t prefix_attention_workspace(const PrefixAttentionArgs& s) { return attn_plan(s).total(); }
+
+hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs& s) {
+    const AttnPlan p = attn_plan(s);
+    uint8_t* ws = static_cast<uint8_t*>(s.workspace);
+    AttnParams a{};
+    a.q = s.q;
+    a.prefix = s.prefix;
+    a.cache = s.cache;
+    a.lengths = s.lengths;
+    a.partial_out = reinterpret_cast<float*>(ws);
+    a.partial_ml = reinterpret_cast<float2*>(ws + p.out_bytes);
+    a.scores = s.weights_out ? reinterpret_cast<float*>(ws + p.out_bytes + p.ml_bytes) : nullptr;
+    float* log_sum = s.weights_out ? reinterpret_cast<float*>(ws + p.out_bytes + p.ml_bytes + p.score_bytes) : nullptr;
+    const uint32_t width = s.kv_heads * s.head_dim;
+    a.row_bytes = s.format == kKvF32 ? width * 4 : width / 32 * (s.format == kKvQ8_0 ? 34 : 18);
+    a.prefix_plane = static_cast<uint64_t>(s.prefix_capacity) * a.row_bytes;
+    a.cache_plane = static_cast<uint64_t>(s.sequences) * s.capacity * a.row_bytes;
+    a.prefix_length = s.prefix_length;
+    a.capacity = s.capacity;
+    a.score_pitch = p.score_pitch;
+    a.tokens = s.tokens;
+    a.q_heads = s.q_heads;
+    a.kv_heads = s.kv_heads;
+    a.group = s.q_heads / s.kv_heads;
+    a.head_dim = s.head_dim;
+    a.seq_rows = s.tokens * a.group;
+    a.rows = s.sequences * a.seq_rows;
+    a.prefix_tiles = p.prefix_tiles;
+    a.prefix_slots = p.prefix_slots;
+    a.own_tiles = p.own_tiles;
+    a.own_slots = p.own_slots;
+    a.prefix_items = p.prefix_tiles * p.prefix_slots * s.kv_heads;
+    a.scale = s.scale * kLog2e;
+    const uint32_t items = a.prefix_items + s.sequences * s.kv_heads * p.own_slots * p.own_tiles;
+    if (s.format == kKvF32)
+        launch_rows<kKvF32>(stream, items, p.row_tiles, a);
+    else if (s.format == kKvQ8_0)
+        launch_rows<kKvQ8_0>(stream, items, p.row_tiles, a);
+    else
+        launch_rows<kKvQ4_0>(stream, items, p.row_tiles, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const uint64_t all = static_cast<uint64_t>(a.rows) * a.kv_heads;
+    hipLaunchKernelGGL(attn_join_kernel, dim3(static_cast<uint32_t>((all + kAttnWaves - 1) / kAttnWaves)),
+                       dim3(kAttnThreads), 0, stream, a, s.output, log_sum);
+    e = hipGetLastError();
+    if (e != hipSuccess || !s.weights_out) return e;
+    hipLaunchKernelGGL(attn_weights_kernel, dim3((s.capacity + kAttnThreads - 1) / kAttnThreads * s.sequences),
+                       dim3(kAttnThreads), 0, stream, a, log_sum, s.weights_in, s.weights_out);
+    return hipGetLastError();
+}
+
+}  // namespace atlas

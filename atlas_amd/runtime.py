@@ -10,7 +10,7 @@ errors raised as `OperatorError` carrying the reference's MetalError kind.
 from __future__ import annotations
 
 import ctypes
-from ctypes import byref, c_float, c_int, c_void_p
+from ctypes import byref, c_float, c_int, c_uint64, c_void_p
 from dataclasses import dataclass
 
 import numpy as np
@@ -307,6 +307,46 @@ class HipRuntime:
               "q4_0": self.lib.atlas_hip_kv_append_q4_0}[fmt]
         self._check(fn(self.ctx, _ptr(key), _ptr(value), _ptr(cache), kv_width, capacity, _ptr(positions), tokens,
                        1 if vnorm else 0, eps))
+
+    # Decoding a batch behind a shared prompt (no counterpart in the reference).  The own caches are one
+    # kv_append cache of sequences * capacity positions, sequence b at b * capacity.
+    _CACHE_FORMATS = {"f32": 0, "q8_0": 1, "q4_0": 2}
+
+    def prefix_attention_workspace(self, fmt, sequences, tokens, q_heads, kv_heads, head_dim, prefix_length, capacity,
+                                   weights=False) -> int:
+        """Workspace bytes of prefix_attention at these sizes (weights: with weights_out)."""
+        n = c_uint64()
+        self._check(self.lib.atlas_hip_prefix_attention_workspace(
+            self.ctx, self._CACHE_FORMATS[fmt], sequences, tokens, q_heads, kv_heads, head_dim, prefix_length, capacity,
+            1 if weights else 0, byref(n)))
+        return n.value
+
+    def prefix_attention(self, fmt, q, prefix, prefix_length, prefix_capacity, cache, lengths, capacity, out, weights_in,
+                         weights_out, sequences, tokens, q_heads, kv_heads, head_dim, scale, workspace, workspace_bytes):
+        fn = {"f32": self.lib.atlas_hip_prefix_attention_f32, "q8_0": self.lib.atlas_hip_prefix_attention_q8_0,
+              "q4_0": self.lib.atlas_hip_prefix_attention_q4_0}[fmt]
+        self._check(fn(self.ctx, _ptr(q), _ptr(prefix), prefix_length, prefix_capacity, _ptr(cache), _ptr(lengths),
+                       capacity, _ptr(out), _ptr(weights_in), _ptr(weights_out), sequences, tokens, q_heads, kv_heads,
+                       head_dim, scale, _ptr(workspace), workspace_bytes))
+
+    def kv_evict(self, fmt, cache, cache_out, weights, weights_out, lengths, lengths_out, kept, sequences, capacity,
+                 kv_width, budget, recent):
+        fn = {"f32": self.lib.atlas_hip_kv_evict_f32, "q8_0": self.lib.atlas_hip_kv_evict_q8_0,
+              "q4_0": self.lib.atlas_hip_kv_evict_q4_0}[fmt]
+        self._check(fn(self.ctx, _ptr(cache), _ptr(cache_out), _ptr(weights), _ptr(weights_out), _ptr(lengths),
+                       _ptr(lengths_out), _ptr(kept), sequences, capacity, kv_width, budget, recent))
+
+    def verify_draft_workspace(self, sequences, drafts, vocab) -> int:
+        n = c_uint64()
+        self._check(self.lib.atlas_hip_verify_draft_workspace(self.ctx, sequences, drafts, vocab, byref(n)))
+        return n.value
+
+    def verify_draft(self, target_logits, draft_logits, draft_tokens, draft_lengths, accept_uniform, sample_uniform,
+                     accepted, tokens, sequences, drafts, vocab, inv_temperature, workspace, workspace_bytes):
+        self._check(self.lib.atlas_hip_verify_draft_f32(
+            self.ctx, _ptr(target_logits), _ptr(draft_logits), _ptr(draft_tokens), _ptr(draft_lengths),
+            _ptr(accept_uniform), _ptr(sample_uniform), _ptr(accepted), _ptr(tokens), sequences, drafts, vocab,
+            inv_temperature, _ptr(workspace), workspace_bytes))
 
     # Decode tail: softcap_f32 / argmax_f32 (kernels.metal:931-934, 2033-2066)
     def softcap(self, x, y, n, cap):

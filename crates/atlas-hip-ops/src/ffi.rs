@@ -130,10 +130,19 @@ extern "C" {
     pub fn atlas_hip_kv_append_f32(ctx: *mut AtlasHipCtx, key: *const f32, value: *const f32, cache: *mut f32, kv_width: u32, capacity: u32, positions: *const u32, tokens: u32, vnorm: c_int, epsilon: f32) -> c_int;
     pub fn atlas_hip_kv_append_q8_0(ctx: *mut AtlasHipCtx, key: *const f32, value: *const f32, cache: *mut u8, kv_width: u32, capacity: u32, positions: *const u32, tokens: u32, vnorm: c_int, epsilon: f32) -> c_int;
     pub fn atlas_hip_kv_append_q4_0(ctx: *mut AtlasHipCtx, key: *const f32, value: *const f32, cache: *mut u8, kv_width: u32, capacity: u32, positions: *const u32, tokens: u32, vnorm: c_int, epsilon: f32) -> c_int;
+    pub fn atlas_hip_prefix_attention_workspace(ctx: *mut AtlasHipCtx, format: c_int, sequences: u32, tokens: u32, q_heads: u32, kv_heads: u32, head_dim: u32, prefix_length: u32, capacity: u32, weights: c_int, bytes: *mut u64) -> c_int;
+    pub fn atlas_hip_prefix_attention_f32(ctx: *mut AtlasHipCtx, q: *const f32, prefix: *const f32, prefix_length: u32, prefix_capacity: u32, cache: *const f32, lengths: *const u32, capacity: u32, output: *mut f32, weights_in: *const f32, weights_out: *mut f32, sequences: u32, tokens: u32, q_heads: u32, kv_heads: u32, head_dim: u32, scale: f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn atlas_hip_prefix_attention_q8_0(ctx: *mut AtlasHipCtx, q: *const f32, prefix: *const u8, prefix_length: u32, prefix_capacity: u32, cache: *const u8, lengths: *const u32, capacity: u32, output: *mut f32, weights_in: *const f32, weights_out: *mut f32, sequences: u32, tokens: u32, q_heads: u32, kv_heads: u32, head_dim: u32, scale: f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn atlas_hip_prefix_attention_q4_0(ctx: *mut AtlasHipCtx, q: *const f32, prefix: *const u8, prefix_length: u32, prefix_capacity: u32, cache: *const u8, lengths: *const u32, capacity: u32, output: *mut f32, weights_in: *const f32, weights_out: *mut f32, sequences: u32, tokens: u32, q_heads: u32, kv_heads: u32, head_dim: u32, scale: f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn atlas_hip_kv_evict_f32(ctx: *mut AtlasHipCtx, cache: *const f32, cache_out: *mut f32, weights: *const f32, weights_out: *mut f32, lengths: *const u32, lengths_out: *mut u32, kept: *mut u32, sequences: u32, capacity: u32, kv_width: u32, budget: u32, recent: u32) -> c_int;
+    pub fn atlas_hip_kv_evict_q8_0(ctx: *mut AtlasHipCtx, cache: *const u8, cache_out: *mut u8, weights: *const f32, weights_out: *mut f32, lengths: *const u32, lengths_out: *mut u32, kept: *mut u32, sequences: u32, capacity: u32, kv_width: u32, budget: u32, recent: u32) -> c_int;
+    pub fn atlas_hip_kv_evict_q4_0(ctx: *mut AtlasHipCtx, cache: *const u8, cache_out: *mut u8, weights: *const f32, weights_out: *mut f32, lengths: *const u32, lengths_out: *mut u32, kept: *mut u32, sequences: u32, capacity: u32, kv_width: u32, budget: u32, recent: u32) -> c_int;
     pub fn atlas_hip_softcap_f32(ctx: *mut AtlasHipCtx, input: *const f32, output: *mut f32, count: u64, cap: f32) -> c_int;
     pub fn atlas_hip_argmax_f32(ctx: *mut AtlasHipCtx, values: *const f32, selected: *mut u32, rows: u32, count: u32) -> c_int;
     pub fn atlas_hip_softcap_argmax_f32(ctx: *mut AtlasHipCtx, logits: *const f32, capped: *mut f32, selected: *mut u32, rows: u32, count: u32, cap: f32) -> c_int;
     pub fn atlas_hip_softcap_argmax_f32_noalloc(ctx: *mut AtlasHipCtx, logits: *const f32, capped: *mut f32, selected: *mut u32, rows: u32, count: u32, cap: f32) -> c_int;
+    pub fn atlas_hip_verify_draft_workspace(ctx: *mut AtlasHipCtx, sequences: u32, drafts: u32, vocab: u32, bytes: *mut u64) -> c_int;
+    pub fn atlas_hip_verify_draft_f32(ctx: *mut AtlasHipCtx, target_logits: *const f32, draft_logits: *const f32, draft_tokens: *const u32, draft_lengths: *const u32, accept_uniform: *const f32, sample_uniform: *const f32, accepted: *mut u32, tokens: *mut u32, sequences: u32, drafts: u32, vocab: u32, inv_temperature: f64, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
     pub fn atlas_ops_embedding(ctx: *mut AtlasHipCtx, table: *const f32, table_len: usize, vocabulary: usize, hidden: usize, token_ids: *const u32, token_count: usize, output: *mut f32, output_len: usize, timing: *mut AtlasDispatchTiming) -> c_int;
     pub fn atlas_ops_embedding_q6_k(ctx: *mut AtlasHipCtx, weights: *const u8, weights_len: usize, vocabulary: usize, hidden: usize, token_ids: *const u32, token_count: usize, output: *mut f32, output_len: usize, timing: *mut AtlasDispatchTiming) -> c_int;
     pub fn atlas_ops_add(ctx: *mut AtlasHipCtx, lhs: *const f32, lhs_len: usize, rhs: *const f32, rhs_len: usize, output: *mut f32, output_len: usize, timing: *mut AtlasDispatchTiming) -> c_int;

@@ -386,6 +386,88 @@ int atlas_hip_kv_append_q4_0(atlas_hip_ctx *ctx, const float *key, const float *
                              uint32_t kv_width, uint32_t capacity, const uint32_t *positions,
                              uint32_t tokens, int vnorm, float epsilon);
 
+/* ---- decoding a batch behind a shared prompt ----------------------------- */
+
+/* No counterpart in the reference, whose executors decode one sequence.
+ *
+ * Attention of `tokens` new tokens of each of `sequences` sequences over a
+ * prompt that all of them share and over each sequence's own cache:
+ *   x_j    = scale * (q . k_j)  for the prompt's rows j < prefix_length and
+ *            own rows j < len_b - (tokens - 1 - t),  len_b =
+ *            min(lengths[b], capacity): the sequence's last `tokens` rows are
+ *            the new tokens' own (append them first), each seen from its
+ *            token on
+ *   output = sum_j e^{x_j} v_j / sum_j e^{x_j};  zero where nothing is seen
+ * q and output [sequences, tokens, q_heads, head_dim] f32; query head h reads
+ * KV head h / (q_heads / kv_heads).  The caches have kv_append's layout with
+ * kv_width = kv_heads * head_dim: the prompt's is [K | V][prefix_capacity][row],
+ * read once for the batch; the own ones are one cache [K | V][sequences *
+ * capacity][row], sequence b's row j at b * capacity + j (append to it with
+ * capacity = sequences * capacity and positions[b] = b * capacity + j).
+ * prefix_length or capacity may be 0, not both; that cache (and lengths) may
+ * then be NULL.
+ *
+ * weights_out (NULL: none; [sequences, capacity]) is weights_in (NULL: zeros;
+ * may be the same buffer) plus the attention that own row j got, summed over
+ * tokens and heads; rows from len_b on are left untouched.
+ *
+ * head_dim is at most 256 and a multiple of 4 (f32) or 32 (Q8_0, Q4_0);
+ * kv_heads divides q_heads; q, output, f32 caches and the workspace are
+ * 16-byte aligned, quantised caches 2-byte; output does not overlap q.  What a row does not see never
+ * reaches it, whatever it holds.  Scores, sums and accumulators are f32
+ * (within 1e-5 of float64 normwise); a call's result does not depend on
+ * timing.  The workspace (atlas_hip_prefix_attention_workspace bytes) is
+ * overwritten by every call and holds nothing between calls: calls that can
+ * overlap, and graphs whose replays can, need one each.  weights != 0 asks
+ * for the size with weights_out. */
+int atlas_hip_prefix_attention_workspace(atlas_hip_ctx *ctx, int format, uint32_t sequences, uint32_t tokens,
+                                         uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                                         uint32_t prefix_length, uint32_t capacity, int weights, uint64_t *bytes);
+int atlas_hip_prefix_attention_f32(atlas_hip_ctx *ctx, const float *q, const float *prefix, uint32_t prefix_length,
+                                   uint32_t prefix_capacity, const float *cache, const uint32_t *lengths,
+                                   uint32_t capacity, float *output, const float *weights_in, float *weights_out,
+                                   uint32_t sequences, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                                   uint32_t head_dim, float scale, void *workspace, uint64_t workspace_bytes);
+int atlas_hip_prefix_attention_q8_0(atlas_hip_ctx *ctx, const float *q, const uint8_t *prefix, uint32_t prefix_length,
+                                    uint32_t prefix_capacity, const uint8_t *cache, const uint32_t *lengths,
+                                    uint32_t capacity, float *output, const float *weights_in, float *weights_out,
+                                    uint32_t sequences, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                                    uint32_t head_dim, float scale, void *workspace, uint64_t workspace_bytes);
+int atlas_hip_prefix_attention_q4_0(atlas_hip_ctx *ctx, const float *q, const uint8_t *prefix, uint32_t prefix_length,
+                                    uint32_t prefix_capacity, const uint8_t *cache, const uint32_t *lengths,
+                                    uint32_t capacity, float *output, const float *weights_in, float *weights_out,
+                                    uint32_t sequences, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
+                                    uint32_t head_dim, float scale, void *workspace, uint64_t workspace_bytes);
+
+/* `format` of the workspace query. */
+#define ATLAS_CACHE_F32 0
+#define ATLAS_CACHE_Q8_0 1
+#define ATLAS_CACHE_Q4_0 2
+
+/* No counterpart in the reference.  A batch's own caches (layout as above, a
+ * row of kv_width values) cut to `budget` rows by the weights that
+ * prefix_attention adds up.  With n = min(lengths[b], capacity): n <= budget
+ * keeps every row; otherwise the last `recent` rows stay (recent <= budget <=
+ * capacity) and, of the first n - recent, the budget - recent with the largest
+ * weights -- of equal weights the lowest row, NaN below every number, -0 equal
+ * to +0.  Kept rows of both planes and their weights move to the front in
+ * their order; lengths_out[b] = min(n, budget); kept[b, i] is the row that row
+ * i was ([sequences, budget], 0xffffffff behind the last).  Rows and weights
+ * behind the kept ones are left as they were.  cache_out, weights_out and
+ * lengths_out may each be the input buffer (an in-place cut, which leaves the
+ * rows in front of the first evicted one alone); otherwise they must not
+ * overlap it.  kv_width is a multiple of 32 for Q8_0 and Q4_0; f32 caches are
+ * 4-byte aligned, quantised ones 2-byte. */
+int atlas_hip_kv_evict_f32(atlas_hip_ctx *ctx, const float *cache, float *cache_out, const float *weights,
+                           float *weights_out, const uint32_t *lengths, uint32_t *lengths_out, uint32_t *kept,
+                           uint32_t sequences, uint32_t capacity, uint32_t kv_width, uint32_t budget, uint32_t recent);
+int atlas_hip_kv_evict_q8_0(atlas_hip_ctx *ctx, const uint8_t *cache, uint8_t *cache_out, const float *weights,
+                            float *weights_out, const uint32_t *lengths, uint32_t *lengths_out, uint32_t *kept,
+                            uint32_t sequences, uint32_t capacity, uint32_t kv_width, uint32_t budget, uint32_t recent);
+int atlas_hip_kv_evict_q4_0(atlas_hip_ctx *ctx, const uint8_t *cache, uint8_t *cache_out, const float *weights,
+                            float *weights_out, const uint32_t *lengths, uint32_t *lengths_out, uint32_t *kept,
+                            uint32_t sequences, uint32_t capacity, uint32_t kv_width, uint32_t budget, uint32_t recent);
+
 /* ---- logits: soft cap and greedy argmax (decode tail) -------------------- */
 
 /* softcap_f32 (kernels.metal:931-934; callers gemma4_executor.rs:3673-3676,
@@ -433,6 +515,34 @@ int atlas_hip_softcap_argmax_f32(atlas_hip_ctx *ctx, const float *logits, float 
  * streams or contexts) race. */
 int atlas_hip_softcap_argmax_f32_noalloc(atlas_hip_ctx *ctx, const float *logits, float *capped,
                                          uint32_t *selected, uint32_t rows, uint32_t count, float cap);
+
+/* No counterpart in the reference, which decodes greedily.  Drafted tokens
+ * verified against the target's probabilities with given random numbers
+ * (speculative sampling).  p_t = softmax(target_logits[b, t] * inv_temperature)
+ * over `vocab` logits, q_t the same of draft_logits; draft_logits NULL: the
+ * drafts were proposed with certainty (q_t = 1 at the drafted token).  Draft t
+ * < len_b = min(draft_lengths[b], drafts) (draft_lengths NULL: drafts) of
+ * sequence b is accepted while
+ *     accept_uniform[b, t] * q_t(x_t) < p_t(x_t).
+ * At the first rejection a token is drawn from r = max(p_t - q_t, 0) (from p_t
+ * where that has no mass), after none from r = p of row len_b: the first i
+ * with r_0 + .. + r_i > sample_uniform[b] * (r_0 + .. + r_{vocab-1}).
+ * accepted[b] = accepted drafts; tokens[b] = those, the drawn one, 0xffffffff
+ * behind it.  Uniforms lie in [0, 1).  target_logits [sequences, drafts + 1,
+ * vocab], draft_logits [sequences, drafts, vocab]; drafts may be 0 (sampling).
+ * NaN and -inf logits have no mass, all of a row's mass lies on its +inf; a
+ * row without mass rejects its draft and draws 0xffffffff; a drafted token >=
+ * vocab is rejected.  Probabilities and sums are float64, so that the drawn
+ * token does not depend on how the sums are split.  Workspace as for
+ * prefix_attention (16-byte aligned, one for each of overlapping calls).
+ * accepted and tokens must not overlap the inputs. */
+int atlas_hip_verify_draft_workspace(atlas_hip_ctx *ctx, uint32_t sequences, uint32_t drafts, uint32_t vocab,
+                                     uint64_t *bytes);
+int atlas_hip_verify_draft_f32(atlas_hip_ctx *ctx, const float *target_logits, const float *draft_logits,
+                               const uint32_t *draft_tokens, const uint32_t *draft_lengths,
+                               const float *accept_uniform, const float *sample_uniform, uint32_t *accepted,
+                               uint32_t *tokens, uint32_t sequences, uint32_t drafts, uint32_t vocab,
+                               double inv_temperature, void *workspace, uint64_t workspace_bytes);
 
 /* ---- host-slice operator API (atlas_ops::NeuralOps) --------------------- */
 
