@@ -13,122 +13,10 @@
 // and its sum O of 2^{x - m} v, and a second launch joins a row's segments:
 // out = sum_s 2^{m_s - M} O_s / sum_s 2^{m_s - M} l_s.  The prompt's segments
 // hold the rows of all sequences, so its cache is read once for the batch.
-#include "device_common.hpp"
-#include "launch.hpp"
+#include "prefix_attention.hpp"
 
 namespace atlas {
 namespace {
-
-constexpr int kAttnThreads = 256;
-constexpr int kAttnWaves = kAttnThreads / kWave;
-constexpr float kLog2e = 1.44269504088896340736f;
-
-typedef f32x4 f32x4_b4 __attribute__((aligned(4)));
-
-__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
-
-// ---------------------------------------------------------------------------
-// Rows of a cache as MFMA operands.  A product over dims may take them in any
-// order that both operands share, and so may the rows of a result, so each
-// format has the order in which a lane's values are contiguous in memory.
-//   key_dim:   dims 32 blk + ... of lane group a = lane / 16, j < 8
-//   value_dim: dims 64 g + ... of lane m = lane % 16, j < 4
-// ---------------------------------------------------------------------------
-template <int FMT>
-__device__ __forceinline__ uint32_t key_dim(uint32_t blk, uint32_t a, uint32_t j) {
-    if (FMT == kKvQ4_0) return 32 * blk + 4 * a + (j & 3) + 16 * (j >> 2);
-    return 32 * blk + 8 * a + j;
-}
-template <int FMT>
-__device__ __forceinline__ uint32_t value_dim(uint32_t g, uint32_t m, uint32_t j) {
-    if (FMT == kKvQ4_0) return 64 * g + 32 * (m >> 3) + 2 * (m & 7) + (j & 1) + 16 * (j >> 1);
-    return 64 * g + 4 * m + j;
-}
-
-template <int FMT>
-__device__ __forceinline__ uint64_t head_offset(uint32_t head, uint32_t head_dim) {
-    if (FMT == kKvF32) return static_cast<uint64_t>(head) * head_dim * 4;
-    return static_cast<uint64_t>(head) * (head_dim / 32) * (FMT == kKvQ8_0 ? 34 : 18);
-}
-
-typedef uint32_t u32_a2 __attribute__((aligned(2)));
-typedef u32x2_t u32x2_a2 __attribute__((aligned(2)));
-
-// The 8 values of block `blk` of a key row's head that lane group `a` holds.
-template <int FMT>
-__device__ __forceinline__ void load_key8(const uint8_t* head, uint32_t blk, uint32_t a, uint32_t head_dim, float* v) {
-    if constexpr (FMT == kKvF32) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t dim = 32 * blk + 8 * a + 4 * h;
-            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (dim < head_dim) x = *reinterpret_cast<const f32x4*>(head + dim * 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * h + j] = x[j];
-        }
-    } else if (32 * blk >= head_dim) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    } else if constexpr (FMT == kKvQ8_0) {
-        const uint8_t* p = head + blk * 34;
-        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
-        const u32x2_t c = *reinterpret_cast<const u32x2_a2*>(p + 2 + 8 * a);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? c.x : c.y) >> (8 * (j & 3)))) * d;
-    } else {
-        const uint8_t* p = head + blk * 18;
-        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
-        const uint32_t c = *reinterpret_cast<const u32_a2*>(p + 2 + 4 * a);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 3) + 4 * (j >> 2))) & 15u) - 8) * d;
-    }
-}
-
-// The 4 values of group `g` of a value row's head that lane m holds.
-template <int FMT>
-__device__ __forceinline__ void load_value4(const uint8_t* head, uint32_t g, uint32_t m, uint32_t head_dim, float* v) {
-    const uint32_t dim = value_dim<FMT>(g, m, 0);
-    if (dim >= head_dim) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = 0.0f;
-    } else if constexpr (FMT == kKvF32) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(head + dim * 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = x[j];
-    } else if constexpr (FMT == kKvQ8_0) {
-        const uint8_t* p = head + (dim / 32) * 34;
-        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
-        const uint32_t c = *reinterpret_cast<const u32_a2*>(p + 2 + dim % 32);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(static_cast<int8_t>(c >> (8 * j))) * d;
-    } else {
-        const uint8_t* p = head + (dim / 32) * 18;
-        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
-        const uint32_t c = *reinterpret_cast<const uint16_t*>(p + 2 + 2 * (m & 7));
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 1) + 4 * (j >> 1))) & 15u) - 8) * d;
-    }
-}
-
-struct AttnParams {
-    const float* q;
-    const uint8_t* prefix;       // K plane; V plane prefix_plane bytes on
-    const uint8_t* cache;        // K plane; V plane cache_plane bytes on
-    const uint32_t* lengths;
-    float* partial_out;          // [slot][kv head][row][head_dim]
-    float2* partial_ml;          // [slot][kv head][row]
-    float* scores;               // [sequence][kv head][row][score_pitch], or null
-    uint64_t prefix_plane, cache_plane;
-    uint32_t row_bytes, prefix_length, capacity, score_pitch;
-    uint32_t tokens, q_heads, kv_heads, group, head_dim;
-    uint32_t rows;               // of one KV head: sequences * tokens * group
-    uint32_t seq_rows;           // tokens * group
-    uint32_t prefix_tiles, prefix_slots, own_tiles, own_slots, prefix_items;
-    float scale;                 // with log2(e)
-};
 
 // out += the products of the keys that a row sees, key by key: for the tiles
 // where a key that only some rows see holds values that are no numbers.
@@ -408,6 +296,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a
 // How the work is laid out, and what of the workspace it takes.
 struct AttnPlan {
     uint32_t row_tiles;  // of 16 rows a workgroup
+    uint32_t wide;       // row tiles of 32 of the prompt's f16 kernel; 0: the prompt goes with the own rows
     uint32_t prefix_tiles, prefix_slots, own_tiles, own_slots;
     uint64_t out_bytes, ml_bytes, score_bytes, log_bytes;
     uint32_t score_pitch;
@@ -423,7 +312,19 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     p.row_tiles = rows > 16 ? 2 : 1;
     const uint32_t step = 16 * p.row_tiles;
     const uint32_t wanted = 1024;  // workgroups
-    if (s.prefix_length) {
+    if (s.prefix_length && rows > 16) {
+        p.wide = rows > 64 ? 4 : 2;
+        p.prefix_tiles = static_cast<uint32_t>((rows + 32 * p.wide - 1) / (32 * p.wide));
+        const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
+        const uint32_t pad = s.head_dim <= 64 ? 64 : (s.head_dim <= 128 ? 128 : 256);
+        const uint32_t tile = (p.wide == 4 ? 32 : 64) * 256 / pad;
+        const uint32_t most = (s.prefix_length + tile - 1) / tile;
+        // one workgroup fills a CU; whole rounds of 256
+        uint64_t want = units >= 256 ? 1 : 256 / units;
+        if (want > most) want = most;
+        if (want > 8) want = want / 8 * 8;
+        p.prefix_slots = static_cast<uint32_t>(want);
+    } else if (s.prefix_length) {
         p.prefix_tiles = static_cast<uint32_t>((rows + step - 1) / step);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         const uint32_t most = (s.prefix_length + 255) / 256;
@@ -507,17 +408,21 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
     a.prefix_slots = p.prefix_slots;
     a.own_tiles = p.own_tiles;
     a.own_slots = p.own_slots;
-    a.prefix_items = p.prefix_tiles * p.prefix_slots * s.kv_heads;
     a.scale = s.scale * kLog2e;
+    const uint32_t prefix_items = p.prefix_tiles * p.prefix_slots * s.kv_heads;
+    if (!p.wide) a.prefix_items = prefix_items;
     const uint32_t items = a.prefix_items + s.sequences * s.kv_heads * p.own_slots * p.own_tiles;
-    if (s.format == kKvF32)
-        launch_rows<kKvF32>(stream, items, p.row_tiles, a);
-    else if (s.format == kKvQ8_0)
-        launch_rows<kKvQ8_0>(stream, items, p.row_tiles, a);
-    else
-        launch_rows<kKvQ4_0>(stream, items, p.row_tiles, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    hipError_t e = hipSuccess;
+    if (p.wide && (e = launch_attn_wide(stream, s.format, prefix_items, p.wide, a)) != hipSuccess) return e;
+    if (items) {
+        if (s.format == kKvF32)
+            launch_rows<kKvF32>(stream, items, p.row_tiles, a);
+        else if (s.format == kKvQ8_0)
+            launch_rows<kKvQ8_0>(stream, items, p.row_tiles, a);
+        else
+            launch_rows<kKvQ4_0>(stream, items, p.row_tiles, a);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
     const uint64_t all = static_cast<uint64_t>(a.rows) * a.kv_heads;
     hipLaunchKernelGGL(attn_join_kernel, dim3(static_cast<uint32_t>((all + kAttnWaves - 1) / kAttnWaves)),
                        dim3(kAttnThreads), 0, stream, a, s.output, log_sum);
