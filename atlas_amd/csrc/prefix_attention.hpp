@@ -118,8 +118,8 @@ struct AttnParams {
     float scale;                 // with log2(e)
 };
 
-// The prompt by f16 pieces (prefix_attention_wide.hip): row_waves 2 or 4 row
-// tiles of 32 to a workgroup, items = prefix_tiles * prefix_slots * kv_heads.
-hipError_t launch_attn_wide(hipStream_t stream, int format, uint32_t items, uint32_t row_waves, const AttnParams& a);
+// The prompt by f16 pieces (prefix_attention_wide.hip): 64 rows to a workgroup,
+// items = prefix_tiles * prefix_slots * kv_heads.
+hipError_t launch_attn_wide(hipStream_t stream, int format, uint32_t items, const AttnParams& a);
 
 }  // namespace atlas

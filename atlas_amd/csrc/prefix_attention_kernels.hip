@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a
 // How the work is laid out, and what of the workspace it takes.
 struct AttnPlan {
     uint32_t row_tiles;  // of 16 rows a workgroup
-    uint32_t wide;       // row tiles of 32 of the prompt's f16 kernel; 0: the prompt goes with the own rows
+    bool wide;           // the prompt goes by f16 pieces, not with the own rows
     uint32_t prefix_tiles, prefix_slots, own_tiles, own_slots;
     uint64_t out_bytes, ml_bytes, score_bytes, log_bytes;
     uint32_t score_pitch;
@@ -313,14 +313,14 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     const uint32_t step = 16 * p.row_tiles;
     const uint32_t wanted = 1024;  // workgroups
     if (s.prefix_length && rows > 16) {
-        p.wide = rows > 64 ? 4 : 2;
-        p.prefix_tiles = static_cast<uint32_t>((rows + 32 * p.wide - 1) / (32 * p.wide));
+        p.wide = true;
+        p.prefix_tiles = static_cast<uint32_t>((rows + 63) / 64);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         const uint32_t pad = s.head_dim <= 64 ? 64 : (s.head_dim <= 128 ? 128 : 256);
-        const uint32_t tile = (p.wide == 4 ? 32 : 64) * 256 / pad;
+        const uint32_t tile = 32 * 256 / pad;
         const uint32_t most = (s.prefix_length + tile - 1) / tile;
-        // one workgroup fills a CU; whole rounds of 256
-        uint64_t want = units >= 256 ? 1 : 256 / units;
+        // two workgroups to a CU
+        uint64_t want = units >= 512 ? 1 : 512 / units;
         if (want > most) want = most;
         if (want > 8) want = want / 8 * 8;
         p.prefix_slots = static_cast<uint32_t>(want);
@@ -413,7 +413,7 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
     if (!p.wide) a.prefix_items = prefix_items;
     const uint32_t items = a.prefix_items + s.sequences * s.kv_heads * p.own_slots * p.own_tiles;
     hipError_t e = hipSuccess;
-    if (p.wide && (e = launch_attn_wide(stream, s.format, prefix_items, p.wide, a)) != hipSuccess) return e;
+    if (p.wide && (e = launch_attn_wide(stream, s.format, prefix_items, a)) != hipSuccess) return e;
     if (items) {
         if (s.format == kKvF32)
             launch_rows<kKvF32>(stream, items, p.row_tiles, a);
