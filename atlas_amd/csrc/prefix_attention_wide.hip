@@ -391,6 +391,73 @@ __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// The products read their fragments two steps of four ahead: left to itself
+// the compiler saves the registers and waits for every read (LDS latency, not
+// its rate, then set the time: 32768 x 2048 rows 343 us).
+template <int D>
+__device__ __forceinline__ void score_pair(const WideTile<D>& tile, int t, uint32_t lane, const half8 (&q_hi)[Wide<D>::KS],
+                                           const half8 (&q_lo)[Wide<D>::KS], f32x4& s0, f32x4& s1) {
+    constexpr int kSteps = Wide<D>::KS;
+    half8 f[2][4];
+    auto read = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[k % 2][i] = tile.key[((t + i / 2) * kSteps + k) * 2 + i % 2][lane];
+    };
+    s0 = s1 = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    __builtin_amdgcn_sched_barrier(0);
+    read(0);
+    read(1);
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        half8(&g)[4] = f[k % 2];
+        s0 = mfma(g[1], q_hi[k], s0);
+        s1 = mfma(g[3], q_hi[k], s1);
+        s0 = mfma(g[0], q_lo[k], s0);
+        s1 = mfma(g[2], q_lo[k], s1);
+        s0 = mfma(g[0], q_hi[k], s0);
+        s1 = mfma(g[2], q_hi[k], s1);
+        __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+        if (k + 2 < kSteps) {
+            read(k + 2);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int D>
+__device__ __forceinline__ void add_values(const WideTile<D>& tile, int b, uint32_t lane, const Pieces& p,
+                                           f32x4 (&out)[Wide<D>::DT]) {
+    constexpr int kSteps = Wide<D>::DT / 2;
+    half8 f[2][4];
+    auto read = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[k % 2][i] = tile.value[(b * 2 * kSteps + 2 * k + i / 2) * 2 + i % 2][lane];
+    };
+    __builtin_amdgcn_sched_barrier(0);
+    read(0);
+    read(1);
+    __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        half8(&g)[4] = f[k % 2];
+        f32x4 &o0 = out[2 * k], &o1 = out[2 * k + 1];
+        o0 = mfma(g[1], p.hi, o0);
+        o1 = mfma(g[3], p.hi, o1);
+        o0 = mfma(g[0], p.lo, o0);
+        o1 = mfma(g[2], p.lo, o1);
+        o0 = mfma(g[0], p.hi, o0);
+        o1 = mfma(g[2], p.hi, o1);
+        __builtin_amdgcn_sched_group_barrier(0x008, 6, 0);
+        if (k + 2 < kSteps) {
+            read(k + 2);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 template <int FMT, int D>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_wide_kernel(AttnParams a) {
     using W = Wide<D>;
@@ -465,30 +532,29 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_wide_kernel(AttnParams a
 
     // Two barriers a tile: the first stands between its keys' conversion and
     // their use (and between the last tile's values' use and this one's
-    // conversion), the second likewise for its values.
+    // conversion), the second likewise for its values.  Rows are loaded a whole
+    // tile ahead, or half a one where they would not fit the registers.
+    constexpr bool kAhead = FMT != kKvF32 || D < 256;
     load_keys(raw_keys, mine, tile_rows<W::KT>(keys, begin, end, a.row_bytes, head_off), a.row_bytes);
+    if (kAhead) load_values(raw_values, mine, tile_rows<W::KT>(values, begin, end, a.row_bytes, head_off), a.row_bytes);
     for (uint32_t first = begin; first < end; first += W::KT) {
         const uint32_t left = end - first;
         convert_keys(raw_keys, tile, lane, wave);
-        load_values(raw_values, mine, tile_rows<W::KT>(values, first, end, a.row_bytes, head_off), a.row_bytes);
+        if (kAhead)
+            load_keys(raw_keys, mine, tile_rows<W::KT>(keys, first + W::KT, end, a.row_bytes, head_off), a.row_bytes);
+        else
+            load_values(raw_values, mine, tile_rows<W::KT>(values, first, end, a.row_bytes, head_off), a.row_bytes);
         __syncthreads();
         f32x4 scores[W::KT / 16];
         if (busy) {
 #pragma unroll
-            for (int t = 0; t < W::KT / 16; ++t) {
-                f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int k = 0; k < W::KS; ++k) {
-                    const half8 hi = tile.key[(t * W::KS + k) * 2][lane], lo = tile.key[(t * W::KS + k) * 2 + 1][lane];
-                    s = mfma(lo, q_hi[k], s);
-                    s = mfma(hi, q_lo[k], s);
-                    s = mfma(hi, q_hi[k], s);
-                }
-                scores[t] = s;
-            }
+            for (int t = 0; t < W::KT / 16; t += 2) score_pair<D>(tile, t, lane, q_hi, q_lo, scores[t], scores[t + 1]);
         }
         convert_values(raw_values, tile, lane, wave);
-        load_keys(raw_keys, mine, tile_rows<W::KT>(keys, first + W::KT, end, a.row_bytes, head_off), a.row_bytes);
+        if (kAhead)
+            load_values(raw_values, mine, tile_rows<W::KT>(values, first + W::KT, end, a.row_bytes, head_off), a.row_bytes);
+        else
+            load_keys(raw_keys, mine, tile_rows<W::KT>(keys, first + W::KT, end, a.row_bytes, head_off), a.row_bytes);
         __syncthreads();
         if (!busy) continue;
 #pragma unroll
@@ -532,13 +598,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_wide_kernel(AttnParams a
                 s[j] = __builtin_ldexpf(w, ev[j / 4][j % 4] + shift);
             }
             const Pieces p = pieces(s);
-#pragma unroll
-            for (int d = 0; d < W::DT; ++d) {
-                const half8 hi = tile.value[(b * W::DT + d) * 2][lane], lo = tile.value[(b * W::DT + d) * 2 + 1][lane];
-                out[d] = mfma(lo, p.hi, out[d]);
-                out[d] = mfma(hi, p.lo, out[d]);
-                out[d] = mfma(hi, p.hi, out[d]);
-            }
+            add_values<D>(tile, b, lane, p, out);
         }
     }
 
