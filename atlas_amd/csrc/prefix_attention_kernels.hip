@@ -298,9 +298,9 @@ struct AttnPlan {
     uint32_t row_tiles;  // of 16 rows a workgroup
     bool wide;           // the prompt goes by f16 pieces, not with the own rows
     uint32_t prefix_tiles, prefix_slots, own_tiles, own_slots;
-    uint64_t out_bytes, ml_bytes, score_bytes, log_bytes;
+    uint64_t out_bytes, ml_bytes, score_bytes, log_bytes, packed_bytes;
     uint32_t score_pitch;
-    uint64_t total() const { return out_bytes + ml_bytes + score_bytes + log_bytes; }
+    uint64_t total() const { return out_bytes + ml_bytes + score_bytes + log_bytes + packed_bytes; }
 };
 
 uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
@@ -314,13 +314,16 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     const uint32_t wanted = 1024;  // workgroups
     if (s.prefix_length && rows > 16) {
         p.wide = true;
-        p.prefix_tiles = static_cast<uint32_t>((rows + 63) / 64);
+        const bool packed = rows >= 512;
+        if (packed) p.packed_bytes = round256(attn_packed_bytes(s.head_dim, s.kv_heads, s.prefix_length));
+        p.prefix_tiles = static_cast<uint32_t>(packed ? (rows + 127) / 128 : (rows + 63) / 64);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         const uint32_t pad = s.head_dim <= 64 ? 64 : (s.head_dim <= 128 ? 128 : 256);
         const uint32_t tile = 32 * 256 / pad;
         const uint32_t most = (s.prefix_length + tile - 1) / tile;
-        // two workgroups to a CU
-        uint64_t want = units >= 512 ? 1 : 512 / units;
+        // two workgroups to a CU, or one of eight wavefronts
+        const uint64_t whole = packed ? 256 : 512;
+        uint64_t want = units >= whole ? 1 : whole / units;
         if (want > most) want = most;
         if (want > 8) want = want / 8 * 8;
         p.prefix_slots = static_cast<uint32_t>(want);
@@ -413,7 +416,8 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
     if (!p.wide) a.prefix_items = prefix_items;
     const uint32_t items = a.prefix_items + s.sequences * s.kv_heads * p.own_slots * p.own_tiles;
     hipError_t e = hipSuccess;
-    if (p.wide && (e = launch_attn_wide(stream, s.format, prefix_items, a)) != hipSuccess) return e;
+    void* packed = p.packed_bytes ? ws + p.out_bytes + p.ml_bytes + p.score_bytes + p.log_bytes : nullptr;
+    if (p.wide && (e = launch_attn_wide(stream, s.format, prefix_items, a, packed)) != hipSuccess) return e;
     if (items) {
         if (s.format == kKvF32)
             launch_rows<kKvF32>(stream, items, p.row_tiles, a);

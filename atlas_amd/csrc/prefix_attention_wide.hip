@@ -95,9 +95,52 @@ __device__ __forceinline__ uint32_t quad_dim(uint32_t q, uint32_t e) {
     return 4 * q + e;
 }
 
-// Raw bytes of 8 key dims (unit c = 4 blk + a, the dims of key_dim) and of 4
-// value dims, through a buffer whose end is the last key's: what lies past it
-// is zero.
+// The rows of a plane that a tile covers, from `first` on: `rows` of them are
+// there (0: none, `first` is then some row that is), and what a lane asks for past them, or past the head's
+// dims (offset kNowhere), is zero.  f32 rows come through a buffer that ends
+// with them.  Quantised rows lie on 2-byte boundaries, where buffer loads of
+// more than 2 bytes have returned zeros inside the buffer: they come by plain
+// loads from the last row there, with a block scale of zero.
+template <int FMT>
+struct TileRows;
+template <>
+struct TileRows<kKvF32> {
+    __amdgpu_buffer_rsrc_t rs;
+    uint32_t row_bytes;
+    __device__ TileRows(const uint8_t* plane, uint32_t first, uint32_t rows, uint32_t row_bytes, uint32_t head_off)
+        : rs(span_rsrc(plane + static_cast<uint64_t>(first) * row_bytes, rows ? rows * row_bytes - head_off : 0u)),
+          row_bytes(row_bytes) {}
+    __device__ f32x4 quad(uint32_t row, uint32_t off) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, row * row_bytes + off, 0, 0));
+    }
+};
+struct QuantTileRows {
+    const uint8_t* base;
+    uint32_t row_bytes, rows;
+    __device__ QuantTileRows(const uint8_t* plane, uint32_t first, uint32_t rows, uint32_t row_bytes)
+        : base(plane + static_cast<uint64_t>(first) * row_bytes), row_bytes(row_bytes), rows(rows) {}
+    __device__ const uint8_t* at(uint32_t row, uint32_t off) const {
+        const uint32_t last = rows ? rows - 1 : 0u;
+        return base + (__umul24(min(row, last), row_bytes) + (off == kNowhere ? 0u : off));
+    }
+    __device__ uint16_t scale(uint32_t row, uint32_t off) const {
+        const uint16_t d = *reinterpret_cast<const uint16_t*>(at(row, off));
+        return row < rows && off != kNowhere ? d : static_cast<uint16_t>(0);
+    }
+};
+template <>
+struct TileRows<kKvQ8_0> : QuantTileRows {
+    __device__ TileRows(const uint8_t* plane, uint32_t first, uint32_t rows, uint32_t row_bytes, uint32_t)
+        : QuantTileRows(plane, first, rows, row_bytes) {}
+};
+template <>
+struct TileRows<kKvQ4_0> : QuantTileRows {
+    __device__ TileRows(const uint8_t* plane, uint32_t first, uint32_t rows, uint32_t row_bytes, uint32_t)
+        : QuantTileRows(plane, first, rows, row_bytes) {}
+};
+
+// 8 key dims as stored (unit c = 4 blk + a, the dims of key_dim); offset is
+// the first of them, for a quantised row its block's scale.
 template <int FMT>
 struct RawKey;
 template <>
@@ -107,10 +150,9 @@ struct RawKey<kKvF32> {
         const uint32_t dim = 8 * unit + 4 * part;
         return dim < head_dim ? dim * 4 : kNowhere;
     }
-    __device__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row, const uint32_t (&o)[2]) {
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-            x[p] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, row + o[p], 0, 0));
+    __device__ void load(const TileRows<kKvF32>& t, uint32_t row, uint32_t, const uint32_t (&o)[2]) {
+        x[0] = t.quad(row, o[0]);
+        x[1] = t.quad(row, o[1]);
     }
     __device__ void values(float (&v)[8]) const {
 #pragma unroll
@@ -121,13 +163,12 @@ template <>
 struct RawKey<kKvQ8_0> {
     u32x2_t c;
     uint16_t d;
-    static __device__ uint32_t offset(uint32_t unit, uint32_t head_dim, uint32_t part) {
-        if (8 * unit >= head_dim) return kNowhere;
-        return (unit >> 2) * 34 + (part ? 0 : 2 + 8 * (unit & 3));
+    static __device__ uint32_t offset(uint32_t unit, uint32_t head_dim, uint32_t) {
+        return 8 * unit < head_dim ? (unit >> 2) * 34 : kNowhere;
     }
-    __device__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row, const uint32_t (&o)[2]) {
-        c = __builtin_amdgcn_raw_buffer_load_b64(rs, row + o[0], 0, 0);
-        d = __builtin_amdgcn_raw_buffer_load_b16(rs, row + o[1], 0, 0);
+    __device__ void load(const TileRows<kKvQ8_0>& t, uint32_t row, uint32_t unit, const uint32_t (&o)[2]) {
+        c = *reinterpret_cast<const u32x2_a2*>(t.at(row, o[0]) + 2 + 8 * (unit & 3));
+        d = t.scale(row, o[0]);
     }
     __device__ void values(float (&v)[8]) const {
         const float s = h2f(d);
@@ -139,13 +180,12 @@ template <>
 struct RawKey<kKvQ4_0> {
     uint32_t c;
     uint16_t d;
-    static __device__ uint32_t offset(uint32_t unit, uint32_t head_dim, uint32_t part) {
-        if (8 * unit >= head_dim) return kNowhere;
-        return (unit >> 2) * 18 + (part ? 0 : 2 + 4 * (unit & 3));
+    static __device__ uint32_t offset(uint32_t unit, uint32_t head_dim, uint32_t) {
+        return 8 * unit < head_dim ? (unit >> 2) * 18 : kNowhere;
     }
-    __device__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row, const uint32_t (&o)[2]) {
-        c = __builtin_amdgcn_raw_buffer_load_b32(rs, row + o[0], 0, 0);
-        d = __builtin_amdgcn_raw_buffer_load_b16(rs, row + o[1], 0, 0);
+    __device__ void load(const TileRows<kKvQ4_0>& t, uint32_t row, uint32_t unit, const uint32_t (&o)[2]) {
+        c = *reinterpret_cast<const u32_a2*>(t.at(row, o[0]) + 2 + 4 * (unit & 3));
+        d = t.scale(row, o[0]);
     }
     __device__ void values(float (&v)[8]) const {
         const float s = h2f(d);
@@ -153,17 +193,14 @@ struct RawKey<kKvQ4_0> {
         for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 3) + 4 * (j >> 2))) & 15u) - 8) * s;
     }
 };
+// 4 value dims as stored.
 template <int FMT>
 struct RawValue;
 template <>
 struct RawValue<kKvF32> {
     f32x4 x;
-    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim, uint32_t part) {
-        return 4 * quad < head_dim ? quad * 16 : kNowhere;
-    }
-    __device__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row, const uint32_t (&o)[2]) {
-        x = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, row + o[0], 0, 0));
-    }
+    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim) { return 4 * quad < head_dim ? quad * 16 : kNowhere; }
+    __device__ void load(const TileRows<kKvF32>& t, uint32_t row, uint32_t, uint32_t o) { x = t.quad(row, o); }
     __device__ void values(float (&v)[4]) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = x[j];
@@ -173,13 +210,12 @@ template <>
 struct RawValue<kKvQ8_0> {
     uint32_t c;
     uint16_t d;
-    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim, uint32_t part) {
-        if (4 * quad >= head_dim) return kNowhere;
-        return (quad >> 3) * 34 + (part ? 0 : 2 + 4 * (quad & 7));
+    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim) {
+        return 4 * quad < head_dim ? (quad >> 3) * 34 : kNowhere;
     }
-    __device__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row, const uint32_t (&o)[2]) {
-        c = __builtin_amdgcn_raw_buffer_load_b32(rs, row + o[0], 0, 0);
-        d = __builtin_amdgcn_raw_buffer_load_b16(rs, row + o[1], 0, 0);
+    __device__ void load(const TileRows<kKvQ8_0>& t, uint32_t row, uint32_t quad, uint32_t o) {
+        c = *reinterpret_cast<const u32_a2*>(t.at(row, o) + 2 + 4 * (quad & 7));
+        d = t.scale(row, o);
     }
     __device__ void values(float (&v)[4]) const {
         const float s = h2f(d);
@@ -190,13 +226,12 @@ struct RawValue<kKvQ8_0> {
 template <>
 struct RawValue<kKvQ4_0> {
     uint16_t c, d;
-    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim, uint32_t part) {
-        if (4 * quad >= head_dim) return kNowhere;
-        return (quad >> 3) * 18 + (part ? 0 : 2 + 2 * (quad & 7));
+    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim) {
+        return 4 * quad < head_dim ? (quad >> 3) * 18 : kNowhere;
     }
-    __device__ void load(__amdgpu_buffer_rsrc_t rs, uint32_t row, const uint32_t (&o)[2]) {
-        c = __builtin_amdgcn_raw_buffer_load_b16(rs, row + o[0], 0, 0);
-        d = __builtin_amdgcn_raw_buffer_load_b16(rs, row + o[1], 0, 0);
+    __device__ void load(const TileRows<kKvQ4_0>& t, uint32_t row, uint32_t quad, uint32_t o) {
+        c = *reinterpret_cast<const uint16_t*>(t.at(row, o) + 2 + 2 * (quad & 7));
+        d = t.scale(row, o);
     }
     __device__ void values(float (&v)[4]) const {
         const float s = h2f(d);
@@ -237,6 +272,7 @@ struct WideTile {
     int value_exp[Wide<D>::KT];      // of the value row, also as a float
     float value_expf[Wide<D>::KT];
     float value_scale[Wide<D>::KT];  // 2^-value_exp
+    float pad[D == 256 ? 128 : 0];       // to whole KiB, for the copies of packed tiles
 };
 
 // A lane's part of a tile as loaded: KI * KU key units, 8 keys' value quads.
@@ -252,7 +288,7 @@ struct RawValues {
 // Where this lane's part of a tile lies.
 template <int FMT, int D>
 struct WideLane {
-    uint32_t key_off[Wide<D>::KU][2], value_off[2];
+    uint32_t key_off[Wide<D>::KU][2], value_off;
     uint32_t key_row, value_row;  // first key of each; the others a constant on
     static constexpr uint32_t kQuads = D / 4;
     __device__ WideLane(uint32_t lane, uint32_t wave, uint32_t head_dim) {
@@ -265,33 +301,24 @@ struct WideLane {
         // keys, group q has 4 q + {0..3} and 16 more
         const uint32_t group = wave * (kWave / kQuads) + lane / kQuads;
         value_row = 32 * (group / 4) + 4 * (group % 4);
-#pragma unroll
-        for (uint32_t p = 0; p < 2; ++p) value_off[p] = RawValue<FMT>::offset(lane % kQuads, head_dim, p);
+        value_off = RawValue<FMT>::offset(lane % kQuads, head_dim);
     }
 };
 
-// A plane's rows from `first` on, up to `end`, as a buffer.
-template <int KT>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rows(const uint8_t* plane, uint32_t first, uint32_t end,
-                                                            uint32_t row_bytes, uint32_t head_off) {
-    const uint32_t rows = first < end ? min(end - first, static_cast<uint32_t>(KT)) : 0u;
-    return span_rsrc(plane + static_cast<uint64_t>(first) * row_bytes, rows ? rows * row_bytes - head_off : 0u);
-}
-
 template <int FMT, int D>
-__device__ __forceinline__ void load_keys(RawKeys<FMT, D>& raw, const WideLane<FMT, D>& lane, __amdgpu_buffer_rsrc_t rs,
-                                          uint32_t row_bytes) {
+__device__ __forceinline__ void load_keys(RawKeys<FMT, D>& raw, const WideLane<FMT, D>& at, const TileRows<FMT>& t) {
 #pragma unroll
     for (int i = 0; i < Wide<D>::KI; ++i)
 #pragma unroll
-        for (int u = 0; u < Wide<D>::KU; ++u) raw.at[i][u].load(rs, (lane.key_row + 32 * i) * row_bytes, lane.key_off[u]);
+        for (int u = 0; u < Wide<D>::KU; ++u)
+            raw.at[i][u].load(t, at.key_row + 32 * i, threadIdx.x % kWave / 8 + 8 * u, at.key_off[u]);
 }
 
 template <int FMT, int D>
-__device__ __forceinline__ void load_values(RawValues<FMT>& raw, const WideLane<FMT, D>& lane, __amdgpu_buffer_rsrc_t rs,
-                                            uint32_t row_bytes) {
+__device__ __forceinline__ void load_values(RawValues<FMT>& raw, const WideLane<FMT, D>& at, const TileRows<FMT>& t) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) raw.at[j].load(rs, (lane.value_row + 16 * (j >> 2) + (j & 3)) * row_bytes, lane.value_off);
+    for (int j = 0; j < 8; ++j)
+        raw.at[j].load(t, at.value_row + 16 * (j >> 2) + (j & 3), threadIdx.x % (D / 4), at.value_off);
 }
 
 template <int FMT, int D>
@@ -396,7 +423,7 @@ __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
 // its rate, then set the time: 32768 x 2048 rows 343 us).
 template <int D>
 __device__ __forceinline__ void score_pair(const WideTile<D>& tile, int t, uint32_t lane, const half8 (&q_hi)[Wide<D>::KS],
-                                           const half8 (&q_lo)[Wide<D>::KS], f32x4& s0, f32x4& s1) {
+                                           const half8 (&q_lo)[Wide<D>::KS], int q_exp, f32x4& s0, f32x4& s1) {
     constexpr int kSteps = Wide<D>::KS;
     half8 f[2][4];
     auto read = [&](int k) {
@@ -424,6 +451,15 @@ __device__ __forceinline__ void score_pair(const WideTile<D>& tile, int t, uint3
         }
     }
     __builtin_amdgcn_sched_barrier(0);
+    // the key rows' exponents belong to the keys: read before the barrier
+    // behind which the next tile's may be written
+    const i32x4 e0 = *reinterpret_cast<const i32x4*>(&tile.key_exp[16 * t + lane / 16 * 4]);
+    const i32x4 e1 = *reinterpret_cast<const i32x4*>(&tile.key_exp[16 * t + 16 + lane / 16 * 4]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        s0[j] = __builtin_ldexpf(s0[j], e0[j] + q_exp);
+        s1[j] = __builtin_ldexpf(s1[j], e1[j] + q_exp);
+    }
 }
 
 template <int D>
@@ -458,51 +494,54 @@ __device__ __forceinline__ void add_values(const WideTile<D>& tile, int b, uint3
     __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int FMT, int D>
-__global__ __launch_bounds__(kAttnThreads, 2) void attn_wide_kernel(AttnParams a) {
-    using W = Wide<D>;
-    __shared__ WideTile<D> tile;
-    const uint32_t lane = threadIdx.x % kWave, n = lane % 16, quarter = lane / 16;
-    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
-
-    // workgroups of one segment on one XCD, whose L2 then reads it once
-    uint32_t item = blockIdx.x, slot, tile_index, kv_head;
-    if (a.prefix_slots % 8 == 0) {
-        const uint32_t xcd = item % 8;
-        item /= 8;
-        tile_index = item % a.prefix_tiles;
-        item /= a.prefix_tiles;
-        slot = item % (a.prefix_slots / 8) * 8 + xcd;
-        kv_head = item / (a.prefix_slots / 8);
-    } else {
-        tile_index = item % a.prefix_tiles;
-        item /= a.prefix_tiles;
-        slot = item % a.prefix_slots;
-        kv_head = item / a.prefix_slots;
+// Which rows and which part of the prompt a workgroup takes.
+struct WideItem {
+    uint32_t slot, tile, kv_head, begin, end;
+    // Workgroups of one segment lie on one XCD, whose L2 then reads it once.
+    __device__ WideItem(const AttnParams& a, uint32_t kt) {
+        uint32_t item = blockIdx.x;
+        if (a.prefix_slots % 8 == 0) {
+            const uint32_t xcd = item % 8;
+            item /= 8;
+            tile = item % a.prefix_tiles;
+            item /= a.prefix_tiles;
+            slot = item % (a.prefix_slots / 8) * 8 + xcd;
+            kv_head = item / (a.prefix_slots / 8);
+        } else {
+            tile = item % a.prefix_tiles;
+            item /= a.prefix_tiles;
+            slot = item % a.prefix_slots;
+            kv_head = item / a.prefix_slots;
+        }
+        // the divisions leave them in vector registers; buffers' bases hang on them
+        slot = __builtin_amdgcn_readfirstlane(slot);
+        tile = __builtin_amdgcn_readfirstlane(tile);
+        kv_head = __builtin_amdgcn_readfirstlane(kv_head);
+        const uint32_t part = ((a.prefix_length + a.prefix_slots - 1) / a.prefix_slots + kt - 1) / kt * kt;
+        begin = min(slot * part, a.prefix_length);
+        end = min(begin + part, a.prefix_length);
     }
-    // the divisions leave them in vector registers; the buffers' bases hang on them
-    slot = __builtin_amdgcn_readfirstlane(slot);
-    tile_index = __builtin_amdgcn_readfirstlane(tile_index);
-    kv_head = __builtin_amdgcn_readfirstlane(kv_head);
-    const uint32_t part = ((a.prefix_length + a.prefix_slots - 1) / a.prefix_slots + W::KT - 1) / W::KT * W::KT;
-    const uint32_t begin = min(slot * part, a.prefix_length), end = min(begin + part, a.prefix_length);
-    const uint32_t head_off = static_cast<uint32_t>(head_offset<FMT>(kv_head, a.head_dim));
-    const uint8_t* keys = a.prefix + head_off;
-    const uint8_t* values = a.prefix + a.prefix_plane + head_off;
+};
 
-    // 16 query rows as operands: lane (row n, quarter) holds the dims of units 4 s + quarter
-    const uint32_t row0 = tile_index * 64 + wave * 16, row = row0 + n;
-    const bool busy = row0 < a.rows;  // the wavefront has rows
-    half8 q_hi[W::KS], q_lo[W::KS];
+// 16 query rows of a wavefront as operands, lane (row n, quarter) holding the
+// dims of units 4 s + quarter, and what they have summed.
+template <int FMT, int D>
+struct WideRows {
+    half8 q_hi[Wide<D>::KS], q_lo[Wide<D>::KS];
     int q_exp;
-    {
+    f32x4 out[Wide<D>::DT];
+    // whole numbers; every x <= m + 8 and x + ev <= mv + 8, so a weight
+    // 2^(x - m) is at most 2^8 and p' = 2^(x + ev - mv + 6) at most 2^14
+    float m, mv, l;
+
+    __device__ __forceinline__ WideRows(const AttnParams& a, uint32_t kv_head, uint32_t row, uint32_t quarter) {
         const uint32_t at = min(row, a.rows - 1);
         const float* q_row =
             a.q + (static_cast<uint64_t>(at / a.group) * a.q_heads + kv_head * a.group + at % a.group) * a.head_dim;
-        float x[W::KS][8];
+        float x[Wide<D>::KS][8];
         float top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < W::KS; ++s) {
+        for (int s = 0; s < Wide<D>::KS; ++s) {
             load_query8<FMT>(q_row, 4 * s + quarter, a.head_dim, a.scale, x[s]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = max_mag(top, x[s][j]);
@@ -511,135 +550,253 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_wide_kernel(AttnParams a
         q_exp = row_exponent(top, 100);
         const float scale = pow2i(-q_exp);
 #pragma unroll
-        for (int s = 0; s < W::KS; ++s) {
+        for (int s = 0; s < Wide<D>::KS; ++s) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[s][j] *= scale;
             const Pieces p = pieces(x[s]);
             q_hi[s] = p.hi;
             q_lo[s] = p.lo;
         }
+#pragma unroll
+        for (int d = 0; d < Wide<D>::DT; ++d) out[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m = mv = neg_inf();
+        l = 0.0f;
     }
 
+    // Block b of 32 keys: scores to weights, and their values added.  Register
+    // j of a score: key 32 b + 16 (j / 4) + 4 quarter + j % 4 of the tile, of
+    // which `left` are there.
+    __device__ __forceinline__ void add(const WideTile<D>& tile, int b, const f32x4& s0, const f32x4& s1, uint32_t left,
+                                        uint32_t lane) {
+        const uint32_t quarter = lane / 16;
+        float s[8];
+        i32x4 ev[2];
+        float top = neg_inf(), top_v = neg_inf();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t key = 32 * b + 16 * t + 4 * quarter;
+            const f32x4 evf = *reinterpret_cast<const f32x4*>(&tile.value_expf[key]);
+            ev[t] = *reinterpret_cast<const i32x4*>(&tile.value_exp[key]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x = t ? s1[j] : s0[j];
+                if (left < Wide<D>::KT) x = key + j < left ? x : neg_inf();
+                s[4 * t + j] = x;
+                top = fmaxf(top, x);
+                top_v = fmaxf(top_v, x + evf[j]);
+            }
+        }
+        top = max_xor32(max_xor16(top));
+        top_v = max_xor32(max_xor16(top_v));
+        if (__builtin_amdgcn_ballot_w64(top > m + 8.0f || top_v > mv + 8.0f) != 0) {
+            const float m_new = fmaxf(m, __builtin_ceilf(top)), mv_new = fmaxf(mv, __builtin_ceilf(top_v));
+            l *= m == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+            const float fade = mv == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(mv - mv_new);
+            m = m_new;
+            mv = mv_new;
+#pragma unroll
+            for (int d = 0; d < Wide<D>::DT; ++d) out[d] *= fade;
+        }
+        const float base = m == neg_inf() ? 0.0f : m;
+        const int shift = m == neg_inf() ? 0 : static_cast<int>(m - mv) + 6;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float w = __builtin_amdgcn_exp2f(s[j] - base);
+            l += w;
+            s[j] = __builtin_ldexpf(w, ev[j / 4][j % 4] + shift);
+        }
+        add_values<D>(tile, b, lane, pieces(s), out);
+    }
+
+    // The segment's sums, relative to 2^m.
+    __device__ __forceinline__ void finish(const AttnParams& a, const WideItem& item, uint32_t row, uint32_t quarter) {
+        if (row >= a.rows) return;
+        const float all = sum_xor32(sum_xor16(l));
+        const int back = m == neg_inf() ? 0 : static_cast<int>(mv - m) - 6;
+        const uint64_t to = (static_cast<uint64_t>(item.slot) * a.kv_heads + item.kv_head) * a.rows + row;
+        if (quarter == 0) a.partial_ml[to] = make_float2(m, all);
+        float* p = a.partial_out + to * a.head_dim;
+#pragma unroll
+        for (int d = 0; d < Wide<D>::DT; d += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(out[d + e][i], back);
+                store_quad<FMT>(p, 4 * d + 4 * quarter + i, a.head_dim, v);
+            }
+    }
+};
+
+template <int FMT, int D>
+__global__ __launch_bounds__(kAttnThreads, 2) void attn_wide_kernel(AttnParams a) {
+    using W = Wide<D>;
+    __shared__ WideTile<D> tile;
+    const uint32_t lane = threadIdx.x % kWave, n = lane % 16, quarter = lane / 16;
+    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+    const WideItem item(a, W::KT);
+    const uint32_t head_off = static_cast<uint32_t>(head_offset<FMT>(item.kv_head, a.head_dim));
+    const uint8_t* keys = a.prefix + head_off;
+    const uint8_t* values = a.prefix + a.prefix_plane + head_off;
+    const uint32_t row0 = item.tile * 64 + wave * 16, row = row0 + n, end = item.end;
+    const bool busy = row0 < a.rows;  // the wavefront has rows
+    WideRows<FMT, D> rows(a, item.kv_head, row, quarter);
     const WideLane<FMT, D> mine(lane, wave, a.head_dim);
     RawKeys<FMT, D> raw_keys;
     RawValues<FMT> raw_values;
-    f32x4 out[W::DT];
-#pragma unroll
-    for (int d = 0; d < W::DT; ++d) out[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    // whole numbers; every x <= m + 8 and x + ev <= mv + 8, so a weight
-    // 2^(x - m) is at most 2^8 and p' = 2^(x + ev - mv + 6) at most 2^14
-    float m = neg_inf(), mv = neg_inf(), l = 0.0f;
 
     // Two barriers a tile: the first stands between its keys' conversion and
     // their use (and between the last tile's values' use and this one's
     // conversion), the second likewise for its values.  Rows are loaded a whole
     // tile ahead, or half a one where they would not fit the registers.
+    const auto rows_of = [&](const uint8_t* plane, uint32_t first) {
+        const uint32_t there = first < end ? min(end - first, static_cast<uint32_t>(W::KT)) : 0u;
+        return TileRows<FMT>(plane, there ? first : end - 1, there, a.row_bytes, head_off);
+    };
     constexpr bool kAhead = FMT != kKvF32 || D < 256;
-    load_keys(raw_keys, mine, tile_rows<W::KT>(keys, begin, end, a.row_bytes, head_off), a.row_bytes);
-    if (kAhead) load_values(raw_values, mine, tile_rows<W::KT>(values, begin, end, a.row_bytes, head_off), a.row_bytes);
-    for (uint32_t first = begin; first < end; first += W::KT) {
+    load_keys(raw_keys, mine, rows_of(keys, item.begin));
+    if (kAhead) load_values(raw_values, mine, rows_of(values, item.begin));
+    for (uint32_t first = item.begin; first < end; first += W::KT) {
         const uint32_t left = end - first;
         convert_keys(raw_keys, tile, lane, wave);
         if (kAhead)
-            load_keys(raw_keys, mine, tile_rows<W::KT>(keys, first + W::KT, end, a.row_bytes, head_off), a.row_bytes);
+            load_keys(raw_keys, mine, rows_of(keys, first + W::KT));
         else
-            load_values(raw_values, mine, tile_rows<W::KT>(values, first, end, a.row_bytes, head_off), a.row_bytes);
+            load_values(raw_values, mine, rows_of(values, first));
         __syncthreads();
         f32x4 scores[W::KT / 16];
         if (busy) {
 #pragma unroll
-            for (int t = 0; t < W::KT / 16; t += 2) score_pair<D>(tile, t, lane, q_hi, q_lo, scores[t], scores[t + 1]);
+            for (int t = 0; t < W::KT / 16; t += 2)
+                score_pair<D>(tile, t, lane, rows.q_hi, rows.q_lo, rows.q_exp, scores[t], scores[t + 1]);
         }
         convert_values(raw_values, tile, lane, wave);
         if (kAhead)
-            load_values(raw_values, mine, tile_rows<W::KT>(values, first + W::KT, end, a.row_bytes, head_off), a.row_bytes);
+            load_values(raw_values, mine, rows_of(values, first + W::KT));
         else
-            load_keys(raw_keys, mine, tile_rows<W::KT>(keys, first + W::KT, end, a.row_bytes, head_off), a.row_bytes);
+            load_keys(raw_keys, mine, rows_of(keys, first + W::KT));
         __syncthreads();
         if (!busy) continue;
 #pragma unroll
-        for (int b = 0; b < W::KT / 32; ++b) {
-            // register j: key 32 b + 16 (j / 4) + 4 quarter + j % 4 of the tile
-            float s[8];
-            i32x4 ev[2];
-            float top = neg_inf(), top_v = neg_inf();
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const uint32_t key = 32 * b + 16 * t + 4 * quarter;
-                const i32x4 e = *reinterpret_cast<const i32x4*>(&tile.key_exp[key]);
-                const f32x4 evf = *reinterpret_cast<const f32x4*>(&tile.value_expf[key]);
-                ev[t] = *reinterpret_cast<const i32x4*>(&tile.value_exp[key]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float x = __builtin_ldexpf(scores[2 * b + t][j], e[j] + q_exp);
-                    if (left < W::KT) x = key + j < left ? x : neg_inf();
-                    s[4 * t + j] = x;
-                    top = fmaxf(top, x);
-                    top_v = fmaxf(top_v, x + evf[j]);
-                }
-            }
-            top = max_xor32(max_xor16(top));
-            top_v = max_xor32(max_xor16(top_v));
-            if (__builtin_amdgcn_ballot_w64(top > m + 8.0f || top_v > mv + 8.0f) != 0) {
-                const float m_new = fmaxf(m, __builtin_ceilf(top)), mv_new = fmaxf(mv, __builtin_ceilf(top_v));
-                l *= m == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-                const float fade = mv == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(mv - mv_new);
-                m = m_new;
-                mv = mv_new;
-#pragma unroll
-                for (int d = 0; d < W::DT; ++d) out[d] *= fade;
-            }
-            const float base = m == neg_inf() ? 0.0f : m;
-            const int shift = m == neg_inf() ? 0 : static_cast<int>(m - mv) + 6;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float w = __builtin_amdgcn_exp2f(s[j] - base);
-                l += w;
-                s[j] = __builtin_ldexpf(w, ev[j / 4][j % 4] + shift);
-            }
-            const Pieces p = pieces(s);
-            add_values<D>(tile, b, lane, p, out);
-        }
+        for (int b = 0; b < W::KT / 32; ++b) rows.add(tile, b, scores[2 * b], scores[2 * b + 1], left, lane);
     }
+    rows.finish(a, item, row, quarter);
+}
 
-    if (row >= a.rows) return;
-    // out relative to 2^m, as l is
-    l = sum_xor32(sum_xor16(l));
-    const int back = m == neg_inf() ? 0 : static_cast<int>(mv - m) - 6;
-    const uint64_t to = (static_cast<uint64_t>(slot) * a.kv_heads + kv_head) * a.rows + row;
-    if (quarter == 0) a.partial_ml[to] = make_float2(m, l);
-    float* p = a.partial_out + to * a.head_dim;
+// The prompt's tiles converted once, for batches whose rows would have every
+// one converted many times: a workgroup a tile of a KV head.
+template <int FMT, int D>
+__global__ __launch_bounds__(kAttnThreads) void attn_pack_kernel(AttnParams a, WideTile<D>* packed, uint32_t tiles) {
+    using W = Wide<D>;
+    __shared__ WideTile<D> tile;
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+    const uint32_t kv_head = __builtin_amdgcn_readfirstlane(blockIdx.x / tiles);
+    const uint32_t first = __builtin_amdgcn_readfirstlane(blockIdx.x % tiles) * W::KT;
+    const uint32_t head_off = static_cast<uint32_t>(head_offset<FMT>(kv_head, a.head_dim));
+    const WideLane<FMT, D> mine(lane, wave, a.head_dim);
+    RawKeys<FMT, D> raw_keys;
+    RawValues<FMT> raw_values;
+    const uint32_t there = min(a.prefix_length - first, static_cast<uint32_t>(W::KT));
+    load_keys(raw_keys, mine, TileRows<FMT>(a.prefix + head_off, first, there, a.row_bytes, head_off));
+    load_values(raw_values, mine, TileRows<FMT>(a.prefix + a.prefix_plane + head_off, first, there, a.row_bytes, head_off));
+    convert_keys(raw_keys, tile, lane, wave);
+    convert_values(raw_values, tile, lane, wave);
+    __syncthreads();
+    const f32x4* from = reinterpret_cast<const f32x4*>(&tile);
+    f32x4* to = reinterpret_cast<f32x4*>(packed + blockIdx.x);
+    for (uint32_t i = threadIdx.x; i < sizeof(tile) / 16; i += kAttnThreads) to[i] = from[i];
+}
+
+// Packed tiles: eight wavefronts of 16 rows, tiles copied to LDS one ahead
+// (no registers, no conversion), one barrier a tile.
+constexpr int kPackedThreads = 512;
+
+template <int FMT, int D>
+__global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnParams a, const WideTile<D>* packed, uint32_t tiles) {
+    using W = Wide<D>;
+    static_assert(sizeof(WideTile<D>) % 1024 == 0, "copied by whole KiB");
+    constexpr uint32_t kChunks = sizeof(WideTile<D>) / 1024;
+    __shared__ WideTile<D> buffers[2];
+    const uint32_t lane = threadIdx.x % kWave, n = lane % 16, quarter = lane / 16;
+    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+    const WideItem item(a, W::KT);
+    const uint32_t row0 = item.tile * 128 + wave * 16, row = row0 + n, end = item.end;
+    const bool busy = row0 < a.rows;
+    const WideTile<D>* source = packed + static_cast<uint64_t>(item.kv_head) * tiles;
+    const uint32_t lds = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)(&buffers[0])));
+    auto copy = [&](uint32_t first, uint32_t buffer) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(source + first / W::KT);
 #pragma unroll
-    for (int d = 0; d < W::DT; d += 4)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(out[d + e][i], back);
-            store_quad<FMT>(p, 4 * d + 4 * quarter + i, a.head_dim, v);
+        for (uint32_t c = 0; c < (kChunks + 7) / 8; ++c) {
+            const uint32_t chunk = c * 8 + wave;
+            // 64 lanes of 16 bytes to LDS at M0; nothing comes back to a register
+            if (chunk < kChunks)
+                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                             :
+                             : "s"(lds + buffer * static_cast<uint32_t>(sizeof(WideTile<D>)) + chunk * 1024),
+                               "v"(lane * 16), "s"(from + chunk * 1024)
+                             : "memory", "m0");
         }
+    };
+    if (item.begin < end) copy(item.begin, 0);
+    WideRows<FMT, D> rows(a, item.kv_head, row, quarter);
+    uint32_t buffer = 0;
+    for (uint32_t first = item.begin; first < end; first += W::KT, buffer ^= 1) {
+        // this tile has arrived, and every wavefront is done with the one before
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (first + W::KT < end) copy(first + W::KT, buffer ^ 1);
+        if (!busy) continue;
+        const uint32_t left = end - first;
+        const WideTile<D>& tile = buffers[buffer];
+        f32x4 scores[W::KT / 16];
+#pragma unroll
+        for (int t = 0; t < W::KT / 16; t += 2)
+            score_pair<D>(tile, t, lane, rows.q_hi, rows.q_lo, rows.q_exp, scores[t], scores[t + 1]);
+#pragma unroll
+        for (int b = 0; b < W::KT / 32; ++b) rows.add(tile, b, scores[2 * b], scores[2 * b + 1], left, lane);
+    }
+    rows.finish(a, item, row, quarter);
+}
+
+template <int FMT, int D>
+hipError_t launch_wide(hipStream_t stream, uint32_t items, const AttnParams& a, void* room) {
+    if (!room) {
+        hipLaunchKernelGGL((attn_wide_kernel<FMT, D>), dim3(items), dim3(kAttnThreads), 0, stream, a);
+        return hipGetLastError();
+    }
+    WideTile<D>* packed = static_cast<WideTile<D>*>(room);
+    const uint32_t tiles = (a.prefix_length + Wide<D>::KT - 1) / Wide<D>::KT;
+    hipLaunchKernelGGL((attn_pack_kernel<FMT, D>), dim3(tiles * a.kv_heads), dim3(kAttnThreads), 0, stream, a, packed, tiles);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    // packed tiles of f32 and Q8_0 rows have one order of dims
+    constexpr int kOrder = FMT == kKvQ4_0 ? kKvQ4_0 : kKvF32;
+    hipLaunchKernelGGL((attn_packed_kernel<kOrder, D>), dim3(items), dim3(kPackedThreads), 0, stream, a, packed, tiles);
+    return hipGetLastError();
 }
 
 template <int FMT>
-void launch_wide(hipStream_t stream, uint32_t items, const AttnParams& a) {
-    if (a.head_dim <= 64)
-        hipLaunchKernelGGL((attn_wide_kernel<FMT, 64>), dim3(items), dim3(kAttnThreads), 0, stream, a);
-    else if (a.head_dim <= 128)
-        hipLaunchKernelGGL((attn_wide_kernel<FMT, 128>), dim3(items), dim3(kAttnThreads), 0, stream, a);
-    else
-        hipLaunchKernelGGL((attn_wide_kernel<FMT, 256>), dim3(items), dim3(kAttnThreads), 0, stream, a);
+hipError_t launch_wide(hipStream_t stream, uint32_t items, const AttnParams& a, void* room) {
+    if (a.head_dim <= 64) return launch_wide<FMT, 64>(stream, items, a, room);
+    if (a.head_dim <= 128) return launch_wide<FMT, 128>(stream, items, a, room);
+    return launch_wide<FMT, 256>(stream, items, a, room);
 }
 
 }  // namespace
 
-hipError_t launch_attn_wide(hipStream_t stream, int format, uint32_t items, const AttnParams& a) {
-    if (format == kKvF32)
-        launch_wide<kKvF32>(stream, items, a);
-    else if (format == kKvQ8_0)
-        launch_wide<kKvQ8_0>(stream, items, a);
-    else
-        launch_wide<kKvQ4_0>(stream, items, a);
-    return hipGetLastError();
+uint64_t attn_packed_bytes(uint32_t head_dim, uint32_t kv_heads, uint32_t prefix_length) {
+    const uint32_t d = head_dim <= 64 ? 64 : (head_dim <= 128 ? 128 : 256), kt = 32 * 256 / d;
+    const uint64_t tile = d == 64 ? sizeof(WideTile<64>) : (d == 128 ? sizeof(WideTile<128>) : sizeof(WideTile<256>));
+    return (static_cast<uint64_t>(prefix_length) + kt - 1) / kt * kv_heads * tile;
+}
+
+hipError_t launch_attn_wide(hipStream_t stream, int format, uint32_t items, const AttnParams& a, void* room) {
+    if (format == kKvF32) return launch_wide<kKvF32>(stream, items, a, room);
+    if (format == kKvQ8_0) return launch_wide<kKvQ8_0>(stream, items, a, room);
+    return launch_wide<kKvQ4_0>(stream, items, a, room);
 }
 
 }  // namespace atlas

@@ -85,6 +85,10 @@ SHAPES = {
     "no_groups": (2, 1, 32, 32, 64, 33, 40, 31, [31, 2]),
     "wide_heads": (2, 2, 6, 2, 160, 129, 129, 66, [66, 30]),
     "batch": (70, 1, 8, 1, 256, 1000, 1024, 64, [(7 * i) % 65 for i in range(70)]),
+    "batch_128": (33, 2, 32, 4, 128, 333, 333, 16, [(5 * i) % 17 for i in range(33)]),
+    "batch_64": (90, 1, 12, 2, 64, 700, 700, 9, [(5 * i) % 10 for i in range(90)]),
+    "batch_96": (110, 1, 10, 2, 96, 65, 65, 9, [(5 * i) % 10 for i in range(110)]),
+    "batch_160": (35, 2, 16, 2, 160, 129, 129, 40, [(5 * i) % 41 for i in range(35)]),
     "long": (2, 1, 8, 1, 256, 9001, 9001, 5000, [4999, 700]),
 }
 
