@@ -15,22 +15,44 @@ typedef f32x4 f32x4_b4 __attribute__((aligned(4)));
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
+// The maximum over lanes that differ in bit 3 / 4 / 5 of their number.
+__device__ __forceinline__ float max_xor8(float x) { return fmaxf(x, dpp_f32<0x128, 0xf, false>(x)); }  // row_ror:8
+__device__ __forceinline__ float max_xor16(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float max_xor32(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float sum_xor16(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float sum_xor32(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
 // ---------------------------------------------------------------------------
 // Rows of a cache as MFMA operands.  A product over dims may take them in any
 // order that both operands share, and so may the rows of a result, so each
-// format has the order in which a lane's values are contiguous in memory.
-//   key_dim:   dims 32 blk + ... of lane group a = lane / 16, j < 8
-//   value_dim: dims 64 g + ... of lane m = lane % 16, j < 4
+// format has the order in which a lane's values are contiguous in memory:
+// units of 8 key dims and quads of 4 value dims.
 // ---------------------------------------------------------------------------
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32_a2 __attribute__((aligned(2)));
+typedef u32x2_t u32x2_a2 __attribute__((aligned(2)));
+
+// The dims of unit 4 blk + a, j < 8.
 template <int FMT>
 __device__ __forceinline__ uint32_t key_dim(uint32_t blk, uint32_t a, uint32_t j) {
     if (FMT == kKvQ4_0) return 32 * blk + 4 * a + (j & 3) + 16 * (j >> 2);
     return 32 * blk + 8 * a + j;
-}
-template <int FMT>
-__device__ __forceinline__ uint32_t value_dim(uint32_t g, uint32_t m, uint32_t j) {
-    if (FMT == kKvQ4_0) return 64 * g + 32 * (m >> 3) + 2 * (m & 7) + (j & 1) + 16 * (j >> 1);
-    return 64 * g + 4 * m + j;
 }
 
 template <int FMT>
@@ -39,65 +61,184 @@ __device__ __forceinline__ uint64_t head_offset(uint32_t head, uint32_t head_dim
     return static_cast<uint64_t>(head) * (head_dim / 32) * (FMT == kKvQ8_0 ? 34 : 18);
 }
 
-typedef uint32_t u32_a2 __attribute__((aligned(2)));
-typedef u32x2_t u32x2_a2 __attribute__((aligned(2)));
+constexpr uint32_t kNowhere = 0x7ffffff0u;  // a buffer offset past every span: reads as zero
 
-// The 8 values of block `blk` of a key row's head that lane group `a` holds.
+
+// The dims that value quad q (of head_dim / 4) holds, e < 4.
 template <int FMT>
-__device__ __forceinline__ void load_key8(const uint8_t* head, uint32_t blk, uint32_t a, uint32_t head_dim, float* v) {
-    if constexpr (FMT == kKvF32) {
+__device__ __forceinline__ uint32_t quad_dim(uint32_t q, uint32_t e) {
+    if (FMT == kKvQ4_0) return 32 * (q >> 3) + 2 * (q & 7) + (e & 1) + 16 * (e >> 1);
+    return 4 * q + e;
+}
+
+// The rows of a plane that a tile covers, from `first` on: `rows` of them are
+// there (0: none, `first` is then some row that is), and what a lane asks for past them, or past the head's
+// dims (offset kNowhere), is zero.  f32 rows come through a buffer that ends
+// with them.  Quantised rows lie on 2-byte boundaries, where buffer loads of
+// more than 2 bytes have returned zeros inside the buffer: they come by plain
+// loads from the last row there, with a block scale of zero.
+template <int FMT>
+struct TileRows;
+template <>
+struct TileRows<kKvF32> {
+    __amdgpu_buffer_rsrc_t rs;
+    uint32_t row_bytes;
+    __device__ TileRows(const uint8_t* plane, uint32_t first, uint32_t rows, uint32_t row_bytes, uint32_t head_off)
+        : rs(span_rsrc(plane + static_cast<uint64_t>(first) * row_bytes, rows ? rows * row_bytes - head_off : 0u)),
+          row_bytes(row_bytes) {}
+    __device__ f32x4 quad(uint32_t row, uint32_t off) const {
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, row * row_bytes + off, 0, 0));
+    }
+};
+struct QuantTileRows {
+    const uint8_t* base;
+    uint32_t row_bytes, rows;
+    __device__ QuantTileRows(const uint8_t* plane, uint32_t first, uint32_t rows, uint32_t row_bytes)
+        : base(plane + static_cast<uint64_t>(first) * row_bytes), row_bytes(row_bytes), rows(rows) {}
+    __device__ const uint8_t* at(uint32_t row, uint32_t off) const {
+        const uint32_t last = rows ? rows - 1 : 0u;
+        return base + (__umul24(min(row, last), row_bytes) + (off == kNowhere ? 0u : off));
+    }
+    __device__ uint16_t scale(uint32_t row, uint32_t off) const {
+        const uint16_t d = *reinterpret_cast<const uint16_t*>(at(row, off));
+        return row < rows && off != kNowhere ? d : static_cast<uint16_t>(0);
+    }
+};
+template <>
+struct TileRows<kKvQ8_0> : QuantTileRows {
+    __device__ TileRows(const uint8_t* plane, uint32_t first, uint32_t rows, uint32_t row_bytes, uint32_t)
+        : QuantTileRows(plane, first, rows, row_bytes) {}
+};
+template <>
+struct TileRows<kKvQ4_0> : QuantTileRows {
+    __device__ TileRows(const uint8_t* plane, uint32_t first, uint32_t rows, uint32_t row_bytes, uint32_t)
+        : QuantTileRows(plane, first, rows, row_bytes) {}
+};
+
+// 8 key dims as stored (unit c = 4 blk + a, the dims of key_dim); offset is
+// the first of them, for a quantised row its block's scale.
+template <int FMT>
+struct RawKey;
+template <>
+struct RawKey<kKvF32> {
+    f32x4 x[2];
+    static __device__ uint32_t offset(uint32_t unit, uint32_t head_dim, uint32_t part) {
+        const uint32_t dim = 8 * unit + 4 * part;
+        return dim < head_dim ? dim * 4 : kNowhere;
+    }
+    __device__ void load(const TileRows<kKvF32>& t, uint32_t row, uint32_t, const uint32_t (&o)[2]) {
+        x[0] = t.quad(row, o[0]);
+        x[1] = t.quad(row, o[1]);
+    }
+    __device__ void values(float (&v)[8]) const {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t dim = 32 * blk + 8 * a + 4 * h;
-            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (dim < head_dim) x = *reinterpret_cast<const f32x4*>(head + dim * 4);
+        for (int j = 0; j < 8; ++j) v[j] = x[j >> 2][j & 3];
+    }
+};
+template <>
+struct RawKey<kKvQ8_0> {
+    u32x2_t c;
+    uint16_t d;
+    static __device__ uint32_t offset(uint32_t unit, uint32_t head_dim, uint32_t) {
+        return 8 * unit < head_dim ? (unit >> 2) * 34 : kNowhere;
+    }
+    __device__ void load(const TileRows<kKvQ8_0>& t, uint32_t row, uint32_t unit, const uint32_t (&o)[2]) {
+        c = *reinterpret_cast<const u32x2_a2*>(t.at(row, o[0]) + 2 + 8 * (unit & 3));
+        d = t.scale(row, o[0]);
+    }
+    __device__ void values(float (&v)[8]) const {
+        const float s = h2f(d);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * h + j] = x[j];
-        }
-    } else if (32 * blk >= head_dim) {
+        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? c.x : c.y) >> (8 * (j & 3)))) * s;
+    }
+};
+template <>
+struct RawKey<kKvQ4_0> {
+    uint32_t c;
+    uint16_t d;
+    static __device__ uint32_t offset(uint32_t unit, uint32_t head_dim, uint32_t) {
+        return 8 * unit < head_dim ? (unit >> 2) * 18 : kNowhere;
+    }
+    __device__ void load(const TileRows<kKvQ4_0>& t, uint32_t row, uint32_t unit, const uint32_t (&o)[2]) {
+        c = *reinterpret_cast<const u32_a2*>(t.at(row, o[0]) + 2 + 4 * (unit & 3));
+        d = t.scale(row, o[0]);
+    }
+    __device__ void values(float (&v)[8]) const {
+        const float s = h2f(d);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    } else if constexpr (FMT == kKvQ8_0) {
-        const uint8_t* p = head + blk * 34;
-        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
-        const u32x2_t c = *reinterpret_cast<const u32x2_a2*>(p + 2 + 8 * a);
+        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 3) + 4 * (j >> 2))) & 15u) - 8) * s;
+    }
+};
+// 4 value dims as stored.
+template <int FMT>
+struct RawValue;
+template <>
+struct RawValue<kKvF32> {
+    f32x4 x;
+    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim) { return 4 * quad < head_dim ? quad * 16 : kNowhere; }
+    __device__ void load(const TileRows<kKvF32>& t, uint32_t row, uint32_t, uint32_t o) { x = t.quad(row, o); }
+    __device__ void values(float (&v)[4]) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? c.x : c.y) >> (8 * (j & 3)))) * d;
-    } else {
-        const uint8_t* p = head + blk * 18;
-        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
-        const uint32_t c = *reinterpret_cast<const u32_a2*>(p + 2 + 4 * a);
+        for (int j = 0; j < 4; ++j) v[j] = x[j];
+    }
+};
+template <>
+struct RawValue<kKvQ8_0> {
+    uint32_t c;
+    uint16_t d;
+    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim) {
+        return 4 * quad < head_dim ? (quad >> 3) * 34 : kNowhere;
+    }
+    __device__ void load(const TileRows<kKvQ8_0>& t, uint32_t row, uint32_t quad, uint32_t o) {
+        c = *reinterpret_cast<const u32_a2*>(t.at(row, o) + 2 + 4 * (quad & 7));
+        d = t.scale(row, o);
+    }
+    __device__ void values(float (&v)[4]) const {
+        const float s = h2f(d);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 3) + 4 * (j >> 2))) & 15u) - 8) * d;
+        for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(static_cast<int8_t>(c >> (8 * j))) * s;
+    }
+};
+template <>
+struct RawValue<kKvQ4_0> {
+    uint16_t c, d;
+    static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim) {
+        return 4 * quad < head_dim ? (quad >> 3) * 18 : kNowhere;
+    }
+    __device__ void load(const TileRows<kKvQ4_0>& t, uint32_t row, uint32_t quad, uint32_t o) {
+        c = *reinterpret_cast<const uint16_t*>(t.at(row, o) + 2 + 2 * (quad & 7));
+        d = t.scale(row, o);
+    }
+    __device__ void values(float (&v)[4]) const {
+        const float s = h2f(d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            v[j] = static_cast<float>((c >> (8 * (j & 1) + 4 * (j >> 1)) & 15) - 8) * s;
+    }
+};
+
+// The dims of unit `unit` of a query row, scaled.
+template <int FMT>
+__device__ __forceinline__ void load_query8(const float* q, uint32_t unit, uint32_t head_dim, float scale, float (&x)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t dim = key_dim<FMT>(unit / 4, unit % 4, 4 * h);
+        const bool there = dim < head_dim;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(q + (there ? dim : 0));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * h + j] = there ? v[j] * scale : 0.0f;
     }
 }
 
-// The 4 values of group `g` of a value row's head that lane m holds.
+// The four values of quad q of an output row.
 template <int FMT>
-__device__ __forceinline__ void load_value4(const uint8_t* head, uint32_t g, uint32_t m, uint32_t head_dim, float* v) {
-    const uint32_t dim = value_dim<FMT>(g, m, 0);
-    if (dim >= head_dim) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = 0.0f;
-    } else if constexpr (FMT == kKvF32) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(head + dim * 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = x[j];
-    } else if constexpr (FMT == kKvQ8_0) {
-        const uint8_t* p = head + (dim / 32) * 34;
-        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
-        const uint32_t c = *reinterpret_cast<const u32_a2*>(p + 2 + dim % 32);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(static_cast<int8_t>(c >> (8 * j))) * d;
+__device__ __forceinline__ void store_quad(float* row, uint32_t q, uint32_t head_dim, f32x4 v) {
+    if (4 * q >= head_dim) return;
+    if constexpr (FMT == kKvQ4_0) {
+        *reinterpret_cast<f32x2_t*>(row + quad_dim<FMT>(q, 0)) = f32x2_t{v.x, v.y};
+        *reinterpret_cast<f32x2_t*>(row + quad_dim<FMT>(q, 2)) = f32x2_t{v.z, v.w};
     } else {
-        const uint8_t* p = head + (dim / 32) * 18;
-        const float d = h2f(*reinterpret_cast<const uint16_t*>(p));
-        const uint32_t c = *reinterpret_cast<const uint16_t*>(p + 2 + 2 * (m & 7));
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 1) + 4 * (j >> 1))) & 15u) - 8) * d;
+        *reinterpret_cast<f32x4*>(row + 4 * q) = v;
     }
 }
 

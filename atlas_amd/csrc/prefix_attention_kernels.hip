@@ -35,22 +35,25 @@ __device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const floa
                 for (int i = 0; i < 4; ++i) {
                     const float x = __shfl(v[r][g], static_cast<int>(4 * quarter + i + 16 * from), kWave);
                     out[g][i] = sees ? out[g][i] + weight * x : out[g][i];
+                    __builtin_amdgcn_sched_barrier(0);
                 }
         }
 }
 
-// One workgroup: 16 * NR query rows of one KV head against one segment.  The
-// wavefronts take its keys 16 at a time in turn, each with a running maximum,
-// sum and accumulator of its own, and join through LDS at the end.  Products
-// are v_mfma_f32_16x16x4: S^T = K Q^T leaves lane l with query row l % 16 and
-// keys 4 (l / 16) + r, which is the operand that O^T = V^T P^T wants, so P
-// never leaves its registers; the row's statistics are a lane's own.
+// One workgroup: 16 * NR query rows of one KV head against one segment of a
+// sequence's own rows (or of the prompt, for batches of up to 16 rows).  Its
+// bytes bound it: the wavefronts take its keys 16 at a time in turn, straight
+// from the cache into the operands' registers, with the next 16 loading while
+// these are used.  Products are v_mfma_f32_16x16x4 (f32 throughout): S^T = K Q^T
+// leaves lane l with query row l % 16 and keys 4 (l / 16) + r, which is the
+// operand that O^T = V^T P^T wants, so P never leaves its registers and a
+// row's statistics are the lane's own.  Queries wait in LDS.
 template <int FMT, int NB, int NR>
-__global__ __launch_bounds__(kAttnThreads) void attn_rows_kernel(AttnParams a) {
+__global__ __launch_bounds__(kAttnThreads, NR == 1 && NB < 8 ? 2 : 1) void attn_rows_kernel(AttnParams a) {
     constexpr int NG = (NB + 1) / 2;  // groups of 64 dims
-    constexpr int kDims = 64 * NG;
-    __shared__ float2 wave_ml[kAttnWaves][16];
-    __shared__ float wave_out[kAttnWaves][16][kDims + 4];
+    constexpr int kRoom = NR * NB * 2 > 2 * (NG * 4 + 1) ? NR * NB * 2 : 2 * (NG * 4 + 1);
+    // queries [row tile][step][half]; at the end two wavefronts' sums
+    __shared__ f32x4 room[kRoom][kWave];
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
     const uint32_t n = lane % 16, quarter = lane / 16;
@@ -64,7 +67,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows_kernel(AttnParams a) {
         const uint32_t tile = item % a.prefix_tiles;
         item /= a.prefix_tiles;
         slot = item % a.prefix_slots;
-        kv_head = item / a.prefix_slots;
+        kv_head = __builtin_amdgcn_readfirstlane(item / a.prefix_slots);
         row0 = tile * 16 * NR;
         row_end = a.rows;
         const uint32_t part = ((a.prefix_length + a.prefix_slots - 1) / a.prefix_slots + 63) / 64 * 64;
@@ -78,8 +81,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows_kernel(AttnParams a) {
         item /= a.own_tiles;
         const uint32_t part_index = item % a.own_slots;
         item /= a.own_slots;
-        kv_head = item % a.kv_heads;
-        seq = item / a.kv_heads;
+        kv_head = __builtin_amdgcn_readfirstlane(item % a.kv_heads);
+        seq = __builtin_amdgcn_readfirstlane(item / a.kv_heads);
         slot = a.prefix_slots + part_index;
         row0 = seq * a.seq_rows + tile * 16 * NR;
         row_end = (seq + 1) * a.seq_rows;
@@ -91,56 +94,103 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows_kernel(AttnParams a) {
         keys = a.cache + base;
         values = a.cache + a.cache_plane + base;
     }
-    keys += head_offset<FMT>(kv_head, a.head_dim);
-    values += head_offset<FMT>(kv_head, a.head_dim);
+    key_begin = __builtin_amdgcn_readfirstlane(key_begin);
+    key_end = __builtin_amdgcn_readfirstlane(key_end);
+    row0 = __builtin_amdgcn_readfirstlane(row0);
+    const uint32_t head_off = static_cast<uint32_t>(head_offset<FMT>(kv_head, a.head_dim));
+    keys += head_off;
+    values += head_off;
 
-    float q[NR][NB * 8];
-    uint32_t seen[NR];  // keys below it are seen by the lane's row
-#pragma unroll
-    for (int t = 0; t < NR; ++t) {
-        const uint32_t row = row0 + 16 * t + n;
-        const bool there = row < row_end;
-        const uint32_t at = there ? row : row_end - 1;
-        const float* p = a.q + (static_cast<uint64_t>(at / a.group) * a.q_heads + kv_head * a.group + at % a.group) * a.head_dim;
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t dim = key_dim<FMT>(b, quarter, j);
-                q[t][8 * b + j] = dim < a.head_dim ? p[dim] * a.scale : 0.0f;
-            }
-        if (shared) {
-            seen[t] = key_end;
-        } else {
-            const uint32_t behind = a.tokens - 1 - (at - seq * a.seq_rows) / a.group;
-            seen[t] = min(length > behind ? length - behind : 0u, key_end);
-        }
-        if (!there) seen[t] = 0;
+    for (uint32_t i = wave; i < NR * NB; i += kAttnWaves) {
+        const uint32_t at = min(row0 + 16 * (i / NB) + n, row_end - 1);
+        float x[8];
+        load_query8<FMT>(a.q + (static_cast<uint64_t>(at / a.group) * a.q_heads + kv_head * a.group + at % a.group) * a.head_dim,
+                         4 * (i % NB) + quarter, a.head_dim, a.scale, x);
+        room[2 * i][lane] = f32x4{x[0], x[1], x[2], x[3]};
+        room[2 * i + 1][lane] = f32x4{x[4], x[5], x[6], x[7]};
     }
-
+    uint32_t seen[NR];  // keys below it are seen by the lane's row
     float m[NR], l[NR];
     f32x4 out[NR][NG * 4];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
+        const uint32_t row = row0 + 16 * t + n;
+        seen[t] = key_end;
+        if (!shared) {
+            const uint32_t behind = a.tokens - 1 - (min(row, row_end - 1) - seq * a.seq_rows) / a.group;
+            seen[t] = min(length > behind ? length - behind : 0u, key_end);
+        }
+        if (row >= row_end) seen[t] = 0;
         m[t] = neg_inf();
         l[t] = 0.0f;
 #pragma unroll
         for (int i = 0; i < NG * 4; ++i) out[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    uint32_t key_off[NB][2], value_off[NG];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) key_off[b][p] = RawKey<FMT>::offset(4 * b + quarter, a.head_dim, p);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) value_off[g] = RawValue<FMT>::offset(16 * g + n, a.head_dim);
+    RawKey<FMT> k[NB];
+    RawValue<FMT> raw_v[4][NG];
+    const auto rows_of = [&](const uint8_t* plane, uint32_t first) {
+        const uint32_t there = first < key_end ? min(key_end - first, 16u) : 0u;
+        return TileRows<FMT>(plane, there ? first : key_end - 1, there, a.row_bytes, head_off);
+    };
+    const auto load_k = [&](uint32_t first) {
+        const TileRows<FMT> rows = rows_of(keys, first);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) k[b].load(rows, n, 4 * b + quarter, key_off[b]);
+    };
+    const auto load_v = [&](uint32_t first) {
+        const TileRows<FMT> rows = rows_of(values, first);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int g = 0; g < NG; ++g) raw_v[r][g].load(rows, 4 * quarter + r, 16 * g + n, value_off[g]);
+    };
+    const uint32_t first = key_begin + wave * 16;
+    if (first < key_end) {
+        load_k(first);
+        load_v(first);
+    }
+    __syncthreads();
 
-    for (uint32_t key0 = key_begin + wave * 16; key0 < key_end; key0 += kAttnWaves * 16) {
-        float k[NB * 8], v[4][NG * 4];
-        {
-            const uint8_t* row = keys + static_cast<uint64_t>(min(key0 + n, key_end - 1)) * a.row_bytes;
+    for (uint32_t key0 = first; key0 < key_end; key0 += kAttnWaves * 16) {
+        f32x4 s[NR][2];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) load_key8<FMT>(row, b, quarter, a.head_dim, k + 8 * b);
+        for (int t = 0; t < NR; ++t) s[t][0] = s[t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            float x[8];
+            k[b].values(x);
+#pragma unroll
+            for (int t = 0; t < NR; ++t) {
+                const f32x4 q0 = room[2 * (t * NB + b)][lane], q1 = room[2 * (t * NB + b) + 1][lane];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[t][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], q0[j], s[t][0], 0, 0, 0);
+                    s[t][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[4 + j], q1[j], s[t][1], 0, 0, 0);
+                }
+            }
+            // or every query read is moved up here and the loads in flight to memory
+            if (b % 2) __builtin_amdgcn_sched_barrier(0);
         }
+        const uint32_t next = key0 + kAttnWaves * 16;
+        load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+        float v[4][NG * 4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint8_t* row = values + static_cast<uint64_t>(min(key0 + 4 * quarter + r, key_end - 1)) * a.row_bytes;
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int g = 0; g < NG; ++g) load_value4<FMT>(row, g, n, a.head_dim, v[r] + 4 * g);
-        }
+            for (int g = 0; g < NG; ++g) {
+                float x[4];
+                raw_v[r][g].values(x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[r][4 * g + j] = x[j];
+            }
         // keys that some rows see and others do not: a value there that is no
         // number must not reach the others as 0 * v
         bool stained = false;
@@ -154,37 +204,35 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows_kernel(AttnParams a) {
         }
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
-            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < NB * 8; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i], q[t][i], s, 0, 0, 0);
+            float p[4];
             float top = neg_inf();
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[r] = key0 + 4 * quarter + r < seen[t] ? s[r] : neg_inf();
-                top = fmaxf(top, s[r]);
+                p[r] = key0 + 4 * quarter + r < seen[t] ? s[t][0][r] + s[t][1][r] : neg_inf();
+                top = fmaxf(top, p[r]);
             }
             if (!shared && a.scores) {
                 const uint32_t row = row0 + 16 * t + n;
                 if (row < row_end && key0 + 4 * quarter < key_end) {
                     const uint64_t line = (static_cast<uint64_t>(seq) * a.kv_heads + kv_head) * a.seq_rows + row - seq * a.seq_rows;
-                    *reinterpret_cast<f32x4*>(a.scores + line * a.score_pitch + key0 + 4 * quarter) = s;
+                    *reinterpret_cast<f32x4*>(a.scores + line * a.score_pitch + key0 + 4 * quarter) = f32x4{p[0], p[1], p[2], p[3]};
                 }
             }
-            top = fmaxf(top, __shfl_xor(top, 16, kWave));
-            top = fmaxf(top, __shfl_xor(top, 32, kWave));
-            const float m_new = fmaxf(m[t], top);
-            const float base = m_new == neg_inf() ? 0.0f : m_new;
-            const float fade = __builtin_amdgcn_exp2f(m[t] - base);
-            m[t] = m_new;
-            float p[4];
-            l[t] *= fade;
+            top = max_xor32(max_xor16(top));
+            if (__builtin_amdgcn_ballot_w64(top > m[t]) != 0) {
+                const float m_new = fmaxf(m[t], top);
+                const float fade = m[t] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m[t] - m_new);
+                m[t] = m_new;
+                l[t] *= fade;
+#pragma unroll
+                for (int i = 0; i < NG * 4; ++i) out[t][i] *= fade;
+            }
+            const float base = m[t] == neg_inf() ? 0.0f : m[t];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                p[r] = __builtin_amdgcn_exp2f(s[r] - base);
+                p[r] = __builtin_amdgcn_exp2f(p[r] - base);
                 l[t] += p[r];
             }
-#pragma unroll
-            for (int i = 0; i < NG * 4; ++i) out[t][i] *= fade;
             if (stained) {
                 add_seen<NG>(v, p, key0, seen[t], out[t]);
             } else {
@@ -195,44 +243,45 @@ __global__ __launch_bounds__(kAttnThreads) void attn_rows_kernel(AttnParams a) {
                         out[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i], p[r], out[t][i], 0, 0, 0);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(next);
     }
 
-    // join the wavefronts
+    // join the wavefronts, two to two and one to one
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
-        l[t] += __shfl_xor(l[t], 16, kWave);
-        l[t] += __shfl_xor(l[t], 32, kWave);
-        if (t) __syncthreads();
-        if (quarter == 0) wave_ml[wave][n] = make_float2(m[t], l[t]);
+        l[t] = sum_xor32(sum_xor16(l[t]));
 #pragma unroll
-        for (int g = 0; g < NG; ++g)
+        for (uint32_t half = kAttnWaves / 2; half > 0; half /= 2) {
+            __syncthreads();
+            f32x4(*mine)[kWave] = room + (wave % half) * (NG * 4 + 1);
+            if (wave >= half && wave < 2 * half) {
+                mine[NG * 4][lane] = f32x4{m[t], l[t], 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+                for (int i = 0; i < NG * 4; ++i) mine[i][lane] = out[t][i];
+            }
+            __syncthreads();
+            if (wave < half) {
+                const float m2 = mine[NG * 4][lane].x, l2 = mine[NG * 4][lane].y;
+                const float both = fmaxf(m[t], m2);
+                const float f1 = m[t] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m[t] - both);
+                const float f2 = m2 == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m2 - both);
+                m[t] = both;
+                l[t] = l[t] * f1 + l2 * f2;
+#pragma unroll
+                for (int i = 0; i < NG * 4; ++i) out[t][i] = out[t][i] * f1 + mine[i][lane] * f2;
+            }
+        }
+        const uint32_t row = row0 + 16 * t + n;
+        if (wave == 0 && row < row_end) {
+            const uint64_t at = (static_cast<uint64_t>(slot) * a.kv_heads + kv_head) * a.rows + row;
+            if (quarter == 0) a.partial_ml[at] = make_float2(m[t], l[t]);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    wave_out[wave][n][value_dim<FMT>(g, 4 * quarter + i, j)] = out[t][4 * g + j][i];
-        __syncthreads();
-        const uint32_t per_row = a.head_dim / 4;
-        for (uint32_t i = threadIdx.x; i < 16 * per_row; i += kAttnThreads) {
-            const uint32_t r = i / per_row, d = 4 * (i % per_row);
-            const uint32_t row = row0 + 16 * t + r;
-            if (row >= row_end) break;
-            float top = wave_ml[0][r].x;
-#pragma unroll
-            for (int w = 1; w < kAttnWaves; ++w) top = fmaxf(top, wave_ml[w][r].x);
-            const float base = top == neg_inf() ? 0.0f : top;
-            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-            float sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kAttnWaves; ++w) {
-                const float f = __builtin_amdgcn_exp2f(wave_ml[w][r].x - base);
-                sum += f * wave_ml[w][r].y;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] += f * wave_out[w][r][d + j];
-            }
-            const uint64_t at = (static_cast<uint64_t>(slot) * a.kv_heads + kv_head) * a.rows + row;
-            if (d == 0) a.partial_ml[at] = make_float2(top, sum);
-            *reinterpret_cast<f32x4*>(a.partial_out + at * a.head_dim + d) = o;
+                    store_quad<FMT>(a.partial_out + at * a.head_dim, 16 * g + 4 * quarter + i, a.head_dim,
+                                    f32x4{out[t][4 * g][i], out[t][4 * g + 1][i], out[t][4 * g + 2][i], out[t][4 * g + 3][i]});
         }
     }
 }
@@ -309,7 +358,7 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     AttnPlan p{};
     const uint32_t seq_rows = s.tokens * (s.q_heads / s.kv_heads);
     const uint64_t rows = static_cast<uint64_t>(s.sequences) * seq_rows;
-    p.row_tiles = rows > 16 ? 2 : 1;
+    p.row_tiles = seq_rows > 16 ? 2 : 1;
     const uint32_t step = 16 * p.row_tiles;
     const uint32_t wanted = 1024;  // workgroups
     if (s.prefix_length && rows > 16) {
