@@ -286,31 +286,54 @@ __global__ __launch_bounds__(kAttnThreads, NR == 1 && NB < 8 ? 2 : 1) void attn_
     }
 }
 
-// One wavefront a row: its segments joined, and the base-2 logarithm of its
-// sum (+inf where it saw nothing) for the weights.
+// One workgroup a row: its segments joined, and the base-2 logarithm of its
+// sum (+inf where it saw nothing) for the weights.  LANES lanes hold a
+// segment's dims; as many segments as fit the workgroup are taken at once, and
+// their sums meet in LDS in the segments' order.
+template <int LANES>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, float* output, float* log_sum) {
+    constexpr uint32_t kGroups = kAttnThreads / LANES;
+    __shared__ float wave_top[kAttnWaves];
+    __shared__ f32x4 sums[kGroups][LANES];
+    __shared__ float group_l[kGroups];
     const uint64_t all = static_cast<uint64_t>(a.rows) * a.kv_heads;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kAttnWaves + threadIdx.x / kWave;
-    if (row >= all) return;
-    const uint32_t lane = threadIdx.x % kWave;
+    const uint64_t row = blockIdx.x;
     const uint32_t slots = a.prefix_slots + a.own_slots;
+    const float2* ml = a.partial_ml + row;
     float top = neg_inf();
-    for (uint32_t s = 0; s < slots; ++s) top = fmaxf(top, a.partial_ml[s * all + row].x);
+    for (uint32_t s = threadIdx.x; s < slots; s += kAttnThreads) top = fmaxf(top, ml[s * all].x);
+    top = wave_max_tree_f32(top);
+    if (threadIdx.x % kWave == 0) wave_top[threadIdx.x / kWave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
     const float base = top == neg_inf() ? 0.0f : top;
+    const uint32_t group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const bool holds = 4 * lane < a.head_dim;
+    const float* parts = a.partial_out + row * a.head_dim + (holds ? 4 * lane : 0);
     float sum = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t s = 0; s < slots; ++s) {
-        const float2 ml = a.partial_ml[s * all + row];
-        const float f = __builtin_amdgcn_exp2f(ml.x - base);
-        sum += f * ml.y;
-        if (4 * lane < a.head_dim) {
-            const f32x4 part = *reinterpret_cast<const f32x4*>(a.partial_out + (s * all + row) * a.head_dim + 4 * lane);
+#pragma unroll 4
+    for (uint32_t s = group; s < slots; s += kGroups) {
+        const float2 x = ml[s * all];
+        const f32x4 part = *reinterpret_cast<const f32x4*>(parts + s * all * a.head_dim);
+        const float f = __builtin_amdgcn_exp2f(x.x - base);
+        sum += f * x.y;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] += f * part[j];
-        }
+        for (int j = 0; j < 4; ++j) o[j] += f * part[j];
+    }
+    sums[group][lane] = o;
+    if (lane == 0) group_l[group] = sum;
+    __syncthreads();
+    if (group) return;
+    sum = 0.0f;
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t g = 0; g < kGroups; ++g) {
+        sum += group_l[g];
+        o += sums[g][lane];
     }
     const uint32_t kv_head = static_cast<uint32_t>(row / a.rows), r = static_cast<uint32_t>(row % a.rows);
-    if (4 * lane < a.head_dim) {
+    if (holds) {
         f32x4 y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = sum == 0.0f ? 0.0f : o[j] / sum;
@@ -324,20 +347,30 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, f
     }
 }
 
-// A thread a position: the weight it got from every row of its sequence, in
-// row order.
+// A lane a position: the weight it got from every row of its sequence.  A
+// workgroup's wavefronts take a quarter of the rows each, in row order, and
+// their sums meet in order.
 __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a, const float* log_sum, const float* in,
                                                                     float* out) {
-    const uint32_t blocks = (a.capacity + kAttnThreads - 1) / kAttnThreads;
+    __shared__ float sums[kAttnWaves][kWave];
+    const uint32_t blocks = (a.capacity + kWave - 1) / kWave;
     const uint32_t seq = blockIdx.x / blocks;
     const uint32_t length = min(a.lengths[seq], a.capacity);
-    const uint32_t key = blockIdx.x % blocks * kAttnThreads + threadIdx.x;
-    if (key >= length) return;
-    const uint32_t lines = a.kv_heads * a.seq_rows;
-    const uint64_t first = static_cast<uint64_t>(seq) * lines;
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t key = blockIdx.x % blocks * kWave + lane;
+    if (blockIdx.x % blocks * kWave >= length) return;
+    const uint32_t lines = a.kv_heads * a.seq_rows, part = (lines + kAttnWaves - 1) / kAttnWaves;
+    const uint32_t begin = min(wave * part, lines), end = min(begin + part, lines);
+    const float* logs = log_sum + static_cast<uint64_t>(seq) * lines;
+    const float* scores = a.scores + static_cast<uint64_t>(seq) * lines * a.score_pitch + min(key, length - 1);
     float sum = 0.0f;
-    for (uint32_t i = 0; i < lines; ++i)
-        sum += __builtin_amdgcn_exp2f(a.scores[(first + i) * a.score_pitch + key] - log_sum[first + i]);
+#pragma unroll 8
+    for (uint32_t i = begin; i < end; ++i)
+        sum += __builtin_amdgcn_exp2f(scores[static_cast<uint64_t>(i) * a.score_pitch] - logs[i]);
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave || key >= length) return;
+    sum = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
     const uint64_t at = static_cast<uint64_t>(seq) * a.capacity + key;
     out[at] = in ? in[at] + sum : sum;
 }
@@ -360,7 +393,11 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     const uint64_t rows = static_cast<uint64_t>(s.sequences) * seq_rows;
     p.row_tiles = seq_rows > 16 ? 2 : 1;
     const uint32_t step = 16 * p.row_tiles;
-    const uint32_t wanted = 1024;  // workgroups
+    // Workgroups of a launch: more parts cost their starts and their joins, fewer
+    // leave CUs idle.  256 x 512 own rows, 64 x 8192, 24 x 1024 with 5 drafts, us:
+    //   128  38 / 215 / 38    256  38 / 158 / 35    512  44 / 152 / 40
+    //   1024  59 / 152 / 49   2048  88 / 168 / 63
+    const uint32_t wanted = 512;
     if (s.prefix_length && rows > 16) {
         p.wide = true;
         const bool packed = rows >= 512;
@@ -379,7 +416,7 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     } else if (s.prefix_length) {
         p.prefix_tiles = static_cast<uint32_t>((rows + step - 1) / step);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
-        const uint32_t most = (s.prefix_length + 255) / 256;
+        const uint32_t most = (s.prefix_length + 63) / 64;
         const uint64_t want = (wanted + units - 1) / units;
         p.prefix_slots = static_cast<uint32_t>(want < most ? want : most);
         if (p.prefix_slots > 64) p.prefix_slots = 64;
@@ -387,7 +424,7 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     if (s.capacity) {
         p.own_tiles = (seq_rows + step - 1) / step;
         const uint64_t units = static_cast<uint64_t>(p.own_tiles) * s.kv_heads * s.sequences;
-        const uint32_t most = (s.capacity + 255) / 256;
+        const uint32_t most = (s.capacity + 63) / 64;
         const uint64_t want = (wanted + units - 1) / units;
         p.own_slots = static_cast<uint32_t>(want < most ? want : most);
         if (p.own_slots > 64) p.own_slots = 64;
@@ -477,11 +514,16 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     const uint64_t all = static_cast<uint64_t>(a.rows) * a.kv_heads;
-    hipLaunchKernelGGL(attn_join_kernel, dim3(static_cast<uint32_t>((all + kAttnWaves - 1) / kAttnWaves)),
-                       dim3(kAttnThreads), 0, stream, a, s.output, log_sum);
+    const dim3 join_grid(static_cast<uint32_t>(all)), join_block(kAttnThreads);
+    if (s.head_dim <= 64)
+        hipLaunchKernelGGL(attn_join_kernel<16>, join_grid, join_block, 0, stream, a, s.output, log_sum);
+    else if (s.head_dim <= 128)
+        hipLaunchKernelGGL(attn_join_kernel<32>, join_grid, join_block, 0, stream, a, s.output, log_sum);
+    else
+        hipLaunchKernelGGL(attn_join_kernel<64>, join_grid, join_block, 0, stream, a, s.output, log_sum);
     e = hipGetLastError();
     if (e != hipSuccess || !s.weights_out) return e;
-    hipLaunchKernelGGL(attn_weights_kernel, dim3((s.capacity + kAttnThreads - 1) / kAttnThreads * s.sequences),
+    hipLaunchKernelGGL(attn_weights_kernel, dim3((s.capacity + kWave - 1) / kWave * s.sequences),
                        dim3(kAttnThreads), 0, stream, a, log_sum, s.weights_in, s.weights_out);
     return hipGetLastError();
 }
