@@ -14,10 +14,12 @@
 // terms, which 32-bit sums move by far more than one term; probabilities and
 // sums are in 64 bits throughout.
 //
-// Four launches: every row's maximum and sum per slice of 4096 logits; one
-// wavefront a sequence that accepts and rejects; the residual's sum per slice of the
-// row that was rejected; one workgroup a sequence that finds the slice and
-// the token in it.
+// Launches: every row's maximum and sum per slice of 4096 logits; with a draft
+// model, the residual's sum per slice of the row that was rejected; one
+// workgroup a sequence that finds the slice and the token in it.  The second
+// and third decide for themselves what was accepted (of more than kFusedDrafts
+// drafts a launch of its own does).  Where nothing is taken off p but the drafted token,
+// the slices' sums are the first launch's.
 #include "device_common.hpp"
 #include "launch.hpp"
 
@@ -27,22 +29,57 @@ namespace {
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWaves = kVerifyThreads / kWave;
 constexpr uint32_t kSlice = 4096;
+constexpr int kEach = kSlice / kVerifyThreads;
 constexpr uint32_t kNoToken = 0xffffffffu;
+constexpr uint32_t kFusedDrafts = 16;
 
 typedef f32x4 f32x4_row __attribute__((aligned(4)));
 
 __device__ __forceinline__ float number_or_none(float x) { return x != x ? -__builtin_inff() : x; }
 
-// e^{(x - top) * inv}: 1 at the top (also of an infinite one), 0 in a row
-// that has none.
-__device__ __forceinline__ double mass(float x, float top, double inv) {
-    const double e = exp((static_cast<double>(x) - static_cast<double>(top)) * inv);
+// 2^y, y <= 0, by 2^(j / 32) from a table in LDS and the Taylor polynomial of
+// 2^r to the sixth degree, |r| <= 1 / 64: (r ln 2)^7 / 7! is below 2^-58.  With
+// the rounding of y and of the products, within 2^-51 (|y| + 2) of the true value.
+// About half the operations of the library's exp, whose time the first launch
+// then took: see verify_stats_kernel.
+__device__ __forceinline__ void exp_table(double* table) {
+    if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32.0));
+}
+__device__ __forceinline__ double exp2_table(double y, const double* table) {
+    const double yc = fmax(y, -1200.0);  // 0 there, and what is no number ends there too
+    const double n = __builtin_rint(yc * 32.0);
+    const double r = __builtin_fma(n, -1.0 / 32.0, yc);
+    const int k = static_cast<int>(n);
+    double p = 0x1.430912f86c787p-13;               // ln2^6 / 720
+    p = __builtin_fma(p, r, 0x1.5d87fe78a6731p-10);  // ln2^5 / 120
+    p = __builtin_fma(p, r, 0x1.3b2ab6fba4e77p-7);   // ln2^4 / 24
+    p = __builtin_fma(p, r, 0x1.c6b08d704a0c0p-5);   // ln2^3 / 6
+    p = __builtin_fma(p, r, 0x1.ebfbdff82c58fp-3);   // ln2^2 / 2
+    p = __builtin_fma(p, r, 0x1.62e42fefa39efp-1);   // ln2
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_ldexp(p * table[k & 31], k >> 5);
+}
+
+// e^{(x - top) * inv}, `scale` = inv log2(e): 1 at the top (also of an infinite
+// one), 0 in a row that has none.
+__device__ __forceinline__ double mass(float x, float top, double scale, const double* table) {
+    const double e = exp2_table((static_cast<double>(x) - static_cast<double>(top)) * scale, table);
     return top == -__builtin_inff() ? 0.0 : (x == top ? 1.0 : e);
 }
 
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
     for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+    return v;
+}
+
+__device__ __forceinline__ double wave_inclusive_scan_f64(double v) {
+    const uint32_t lane = threadIdx.x % kWave;
+#pragma unroll
+    for (uint32_t off = 1; off < kWave; off *= 2) {
+        const double u = __shfl_up(v, off, kWave);
+        v += lane >= off ? u : 0.0;
+    }
     return v;
 }
 
@@ -53,9 +90,9 @@ struct SliceStat {
     float unused;
 };
 
-// What the first two launches leave for the others.
+// What was accepted, and the row that is drawn from.
 struct Decision {
-    double target_sum, draft_sum;  // of the row that is drawn from
+    double target_sum, draft_sum;
     float target_top, draft_top;
     uint32_t row;       // accepted drafts = the row of the target
     uint32_t rejected;  // a draft was rejected there
@@ -63,10 +100,11 @@ struct Decision {
 
 struct VerifyParams {
     VerifyDraftArgs s;
+    double scale;             // inv_temperature log2(e)
     SliceStat* target_stats;  // [sequence][drafts + 1][slices]
     SliceStat* draft_stats;   // [sequence][drafts][slices]
     double* slice_sums;       // [sequence][slices]
-    Decision* decisions;      // [sequence]
+    Decision* decisions;      // [sequence], of launches that decide apart
     uint32_t slices;
 };
 
@@ -74,9 +112,32 @@ __device__ __forceinline__ uint32_t drafts_of(const VerifyDraftArgs& s, uint32_t
     return s.draft_lengths ? min(s.draft_lengths[seq], s.drafts) : s.drafts;
 }
 
-// blockIdx.x: slice, blockIdx.y: row in a sequence (targets, then drafts),
-// blockIdx.z: sequence.
+// 16 logits of a slice a thread: four of them at a time, thread by thread
+// (WALK: 16 in a row, for running sums).
+template <bool WALK>
+__device__ __forceinline__ void load_slice(const float* logits, uint32_t first, uint32_t vocab, float (&x)[kEach]) {
+    if (first + kSlice <= vocab) {
+#pragma unroll
+        for (int i = 0; i < kEach / 4; ++i) {
+            const uint32_t at = WALK ? threadIdx.x * kEach + 4 * i : (i * kVerifyThreads + threadIdx.x) * 4;
+            const f32x4 y = *reinterpret_cast<const f32x4_row*>(logits + first + at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = number_or_none(y[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint32_t at = first + (WALK ? threadIdx.x * kEach + i : (i / 4 * kVerifyThreads + threadIdx.x) * 4 + i % 4);
+            x[i] = at < vocab ? number_or_none(logits[at]) : -__builtin_inff();
+        }
+    }
+}
+
+// A workgroup a slice of a row; rows of a sequence: targets, then drafts.  Its
+// bytes bound it, once the exponentials are short: 576 rows of 262144 logits
+// take 120 us with the library's exp.
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyParams v) {
+    __shared__ double table[32];
     __shared__ float wave_top[kVerifyWaves];
     __shared__ double wave_sum[kVerifyWaves];
     const VerifyDraftArgs& s = v.s;
@@ -91,38 +152,20 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyPara
     if (row > count || (!of_target && row == count)) return;
     const float* logits = of_target ? s.target + (static_cast<uint64_t>(seq) * (s.drafts + 1) + row) * s.vocab
                                     : s.draft + (static_cast<uint64_t>(seq) * s.drafts + row) * s.vocab;
-    const uint32_t first = slice * kSlice;
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    constexpr int kEach = kSlice / kVerifyThreads;
     float x[kEach];
-    if (first + kSlice <= s.vocab) {
-#pragma unroll
-        for (int i = 0; i < kEach / 4; ++i) {
-            const f32x4 y = __builtin_nontemporal_load(
-                reinterpret_cast<const f32x4_row*>(logits + first + (i * kVerifyThreads + threadIdx.x) * 4));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[4 * i + j] = y[j];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const uint32_t at = first + i * kVerifyThreads + threadIdx.x;
-            x[i] = at < s.vocab ? logits[at] : -__builtin_inff();
-        }
-    }
+    load_slice<false>(logits, slice * kSlice, s.vocab, x);
+    exp_table(table);
     float top = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        x[i] = number_or_none(x[i]);
-        top = fmaxf(top, x[i]);
-    }
+    for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
     top = wave_max_tree_f32(top);
     if (lane == 0) wave_top[wave] = top;
     __syncthreads();
     top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += mass(x[i], top, s.inv_temperature);
+    for (int i = 0; i < kEach; ++i) sum += mass(x[i], top, v.scale, table);
     sum = wave_sum_f64(sum);
     if (lane == 0) wave_sum[wave] = sum;
     __syncthreads();
@@ -133,56 +176,80 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyPara
 }
 
 // A row's maximum and sum from its slices, by one wavefront.
-__device__ __forceinline__ void row_stat(const SliceStat* slices, uint32_t count, double inv, float& top, double& sum) {
+__device__ __forceinline__ void row_stat(const SliceStat* slices, uint32_t count, double scale, const double* table,
+                                         float& top, double& sum) {
     const uint32_t lane = threadIdx.x % kWave;
-    top = -__builtin_inff();
-    for (uint32_t i = lane; i < count; i += kWave) top = fmaxf(top, slices[i].top);
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
-    sum = 0.0;
-    for (uint32_t i = lane; i < count; i += kWave) sum += slices[i].sum * mass(slices[i].top, top, inv);
+    SliceStat first{0.0, -__builtin_inff(), 0.0f};
+    if (lane < count) first = slices[lane];
+    top = first.top;
+    for (uint32_t i = lane + kWave; i < count; i += kWave) top = fmaxf(top, slices[i].top);
+    top = wave_max_tree_f32(top);
+    sum = first.sum * mass(first.top, top, scale, table);
+    for (uint32_t i = lane + kWave; i < count; i += kWave) sum += slices[i].sum * mass(slices[i].top, top, scale, table);
     sum = wave_sum_f64(sum);
 }
 
-// One wavefront a sequence.
-__global__ __launch_bounds__(kWave) void verify_decide_kernel(VerifyParams v) {
+// The decision of a sequence by a workgroup: the rows' sums by its wavefronts
+// in turn, the drafts' tests by its threads.  The table is filled, and `d` can
+// be read, behind the barriers here.
+template <uint32_t MOST>
+__device__ void decide(const VerifyParams& v, uint32_t seq, const double* table, Decision& d) {
+    __shared__ double sums[2][MOST + 1];
+    __shared__ float tops[2][MOST + 1];
+    __shared__ uint32_t first_rejected;
     const VerifyDraftArgs& s = v.s;
-    const uint32_t seq = blockIdx.x;
-    const uint32_t count = drafts_of(s, seq);
-    Decision d{};
-    uint32_t t = 0;
-    for (;; ++t) {
-        row_stat(v.target_stats + (static_cast<uint64_t>(seq) * (s.drafts + 1) + t) * v.slices, v.slices, s.inv_temperature,
-                 d.target_top, d.target_sum);
-        if (t == count) break;
+    const uint32_t count = drafts_of(s, seq), rows = count + 1 + (s.draft ? count : 0);
+    if (threadIdx.x == 0) first_rejected = count;
+    __syncthreads();
+    for (uint32_t r = threadIdx.x / kWave; r < rows; r += kVerifyWaves) {
+        const bool of_target = r <= count;
+        const uint32_t row = of_target ? r : r - count - 1;
+        const SliceStat* stats = of_target ? v.target_stats + (static_cast<uint64_t>(seq) * (s.drafts + 1) + row) * v.slices
+                                           : v.draft_stats + (static_cast<uint64_t>(seq) * s.drafts + row) * v.slices;
+        float top;
+        double sum;
+        row_stat(stats, v.slices, v.scale, table, top, sum);
+        if (threadIdx.x % kWave == 0) {
+            sums[!of_target][row] = sum;
+            tops[!of_target][row] = top;
+        }
+    }
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < count; t += kVerifyThreads) {
         const uint64_t at = static_cast<uint64_t>(seq) * s.drafts + t;
         const uint32_t token = s.draft_tokens[at];
         double p = 0.0, q = s.draft ? 0.0 : 1.0;
-        if (s.draft) row_stat(v.draft_stats + at * v.slices, v.slices, s.inv_temperature, d.draft_top, d.draft_sum);
         if (token < s.vocab) {
             const float x = number_or_none(s.target[(static_cast<uint64_t>(seq) * (s.drafts + 1) + t) * s.vocab + token]);
-            if (d.target_sum > 0.0) p = mass(x, d.target_top, s.inv_temperature) / d.target_sum;
-            if (s.draft && d.draft_sum > 0.0)
-                q = mass(number_or_none(s.draft[at * s.vocab + token]), d.draft_top, s.inv_temperature) / d.draft_sum;
+            if (sums[0][t] > 0.0) p = mass(x, tops[0][t], v.scale, table) / sums[0][t];
+            if (s.draft && sums[1][t] > 0.0)
+                q = mass(number_or_none(s.draft[at * s.vocab + token]), tops[1][t], v.scale, table) / sums[1][t];
         }
-        if (!(static_cast<double>(s.accept_uniform[at]) * q < p)) {
-            d.rejected = 1;
-            break;
-        }
+        if (!(static_cast<double>(s.accept_uniform[at]) * q < p)) atomicMin(&first_rejected, t);
     }
-    d.row = t;
-    if (threadIdx.x == 0) {
-        v.decisions[seq] = d;
-        s.accepted[seq] = t;
-    }
+    __syncthreads();
+    d.row = first_rejected;
+    d.rejected = d.row < count;
+    d.target_sum = sums[0][d.row];
+    d.target_top = tops[0][d.row];
+    d.draft_sum = s.draft && d.rejected ? sums[1][d.row] : 0.0;
+    d.draft_top = s.draft && d.rejected ? tops[1][d.row] : 0.0f;
 }
 
-// What a draw's terms are, of the row that the decision names.
+__global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(VerifyParams v) {
+    __shared__ double table[32];
+    exp_table(table);
+    Decision d;
+    decide<1024>(v, blockIdx.x, table, d);
+    if (threadIdx.x == 0) v.decisions[blockIdx.x] = d;
+}
+
+// The terms of a draw, of the row that the decision names.
 struct Terms {
     const float* target;
     const float* draft;  // null: none, or certainty at `token`
     uint32_t token;
-    double inv, target_scale, draft_scale;  // 1 / sum, or 0
+    double scale, target_scale, draft_scale;  // 1 / sum, or 0
     float target_top, draft_top;
 
     __device__ Terms(const VerifyParams& v, uint32_t seq, const Decision& d, bool residual) {
@@ -192,31 +259,54 @@ struct Terms {
         const uint64_t at = static_cast<uint64_t>(seq) * s.drafts + d.row;
         draft = minus && s.draft ? s.draft + at * s.vocab : nullptr;
         token = minus && !s.draft ? s.draft_tokens[at] : kNoToken;
-        inv = s.inv_temperature;
+        scale = v.scale;
         target_top = d.target_top;
         draft_top = d.draft_top;
         target_scale = d.target_sum > 0.0 ? 1.0 / d.target_sum : 0.0;
         draft_scale = d.draft_sum > 0.0 ? 1.0 / d.draft_sum : 0.0;
     }
-    __device__ double term(uint32_t i) const {
-        const double p = mass(number_or_none(target[i]), target_top, inv) * target_scale;
-        if (draft) {
-            const double q = mass(number_or_none(draft[i]), draft_top, inv) * draft_scale;
-            return p > q ? p - q : 0.0;
+    // A thread's 16 terms of a slice, as load_slice orders them.
+    template <bool WALK>
+    __device__ void of_slice(uint32_t slice, uint32_t vocab, const double* table, double (&term)[kEach]) const {
+        float x[kEach], y[kEach];
+        load_slice<WALK>(target, slice * kSlice, vocab, x);
+        if (draft) load_slice<WALK>(draft, slice * kSlice, vocab, y);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            double p = mass(x[i], target_top, scale, table) * target_scale;
+            if (draft) {
+                const double q = mass(y[i], draft_top, scale, table) * draft_scale;
+                p = p > q ? p - q : 0.0;
+            } else {
+                const uint32_t at = slice * kSlice + (WALK ? threadIdx.x * kEach + i : (i / 4 * kVerifyThreads + threadIdx.x) * 4 + i % 4);
+                p = at == token ? 0.0 : p;
+            }
+            term[i] = p;
         }
-        return i == token ? 0.0 : p;
     }
 };
 
-// blockIdx.x: slice of sequence blockIdx.x / slices; the sums of the residual.
+// A workgroup a slice: the residual's sum there, of a sequence with a draft
+// rejected (of others the slices' own sums serve).
+template <bool FUSED>
 __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyParams v) {
+    __shared__ double table[32];
     __shared__ double wave_sum[kVerifyWaves];
     const uint32_t seq = blockIdx.x / v.slices, slice = blockIdx.x % v.slices;
-    const Decision d = v.decisions[seq];
-    const Terms terms(v, seq, d, true);
-    const uint32_t first = slice * kSlice, last = min(first + kSlice, v.s.vocab);
+    exp_table(table);
+    Decision d;
+    if (FUSED) {
+        decide<kFusedDrafts>(v, seq, table, d);
+    } else {
+        d = v.decisions[seq];
+        __syncthreads();
+    }
+    if (!d.rejected) return;
+    double term[kEach];
+    Terms(v, seq, d, true).of_slice<false>(slice, v.s.vocab, table, term);
     double sum = 0.0;
-    for (uint32_t i = first + threadIdx.x; i < last; i += kVerifyThreads) sum += terms.term(i);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum += term[i];
     sum = wave_sum_f64(sum);
     if (threadIdx.x % kWave == 0) wave_sum[threadIdx.x / kWave] = sum;
     __syncthreads();
@@ -224,80 +314,134 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyP
         v.slice_sums[static_cast<uint64_t>(seq) * v.slices + slice] = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
 }
 
-// One workgroup a sequence: the token, and the row of results.
+// Of each thread's value, the sum of those before it and of all.
+__device__ __forceinline__ double block_before_f64(double v, double& all) {
+    __shared__ double wave_all[kVerifyWaves];
+    const double upto = wave_inclusive_scan_f64(v);
+    const uint32_t wave = threadIdx.x / kWave;
+    __syncthreads();  // wave_all may still be read from a call before
+    if (threadIdx.x % kWave == kWave - 1) wave_all[wave] = upto;
+    __syncthreads();
+    double before = 0.0;
+#pragma unroll
+    for (uint32_t w = 0; w < kVerifyWaves; ++w) before += w < wave ? wave_all[w] : 0.0;
+    all = (wave_all[0] + wave_all[1]) + (wave_all[2] + wave_all[3]);
+    const double own = __shfl_up(upto, 1, kWave);
+    return before + (threadIdx.x % kWave ? own : 0.0);
+}
+
+// One workgroup a sequence: the slice that holds the draw, the token in it,
+// and the row of results.  Rounding may leave the goal just past the last
+// running sum: the last item with mass is then the one.
+template <bool FUSED>
 __global__ __launch_bounds__(kVerifyThreads) void verify_pick_kernel(VerifyParams v) {
-    __shared__ double before[kVerifyThreads];
-    __shared__ uint32_t shared_slice;
-    __shared__ double shared_goal;
-    __shared__ int shared_residual;
-    __shared__ uint32_t first_hit, last_positive;
+    __shared__ double table[32];
+    __shared__ uint32_t first_hit, last_mass;
+    __shared__ double shared_before;
     const VerifyDraftArgs& s = v.s;
     const uint32_t seq = blockIdx.x, tid = threadIdx.x;
-    const Decision d = v.decisions[seq];
+    exp_table(table);
+    Decision d;
+    if (FUSED) {
+        decide<kFusedDrafts>(v, seq, table, d);
+    } else {
+        d = v.decisions[seq];
+        __syncthreads();
+    }
     const double* sums = v.slice_sums + static_cast<uint64_t>(seq) * v.slices;
     const SliceStat* stats = v.target_stats + (static_cast<uint64_t>(seq) * (s.drafts + 1) + d.row) * v.slices;
-    const double scale = d.target_sum > 0.0 ? 1.0 / d.target_sum : 0.0;
-    if (tid == 0) {
-        double total = 0.0;
-        for (uint32_t i = 0; i < v.slices; ++i) total += sums[i];
-        const bool residual = total > 0.0;
-        if (!residual)
-            for (uint32_t i = 0; i < v.slices; ++i) total += stats[i].sum * mass(stats[i].top, d.target_top, s.inv_temperature) * scale;
-        const double goal = static_cast<double>(s.sample_uniform[seq]) * total;
-        double run = 0.0, at_last = 0.0;
-        uint32_t slice = kNoToken;
-        for (uint32_t i = 0; i < v.slices; ++i) {
-            const double part = residual ? sums[i] : stats[i].sum * mass(stats[i].top, d.target_top, s.inv_temperature) * scale;
-            if (part > 0.0) {
-                slice = i;
-                at_last = run;
-                if (run + part > goal) break;
-            }
-            run += part;
+    const double target_scale = d.target_sum > 0.0 ? 1.0 / d.target_sum : 0.0;
+
+    // the slice that lost the token that was proposed with certainty
+    uint32_t short_slice = kNoToken;
+    double short_sum = 0.0;
+    if (d.rejected && !s.draft) {
+        const uint32_t token = s.draft_tokens[static_cast<uint64_t>(seq) * s.drafts + d.row];
+        if (token < s.vocab) {
+            short_slice = token / kSlice;
+            double term[kEach], sum = 0.0;
+            Terms(v, seq, d, true).of_slice<false>(short_slice, s.vocab, table, term);
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) sum += term[i];
+            (void)block_before_f64(sum, short_sum);
         }
-        shared_slice = slice;
-        shared_goal = goal - at_last;
-        shared_residual = residual;
+    }
+    bool residual = true;
+    const auto part = [&](uint32_t i) {
+        if (residual && d.rejected && s.draft) return sums[i];
+        if (residual && i == short_slice) return short_sum;
+        return stats[i].sum * mass(stats[i].top, d.target_top, v.scale, table) * target_scale;
+    };
+    // slices [begin, end) are this thread's
+    const uint32_t each = (v.slices + kVerifyThreads - 1) / kVerifyThreads;
+    const uint32_t begin = min(tid * each, v.slices), end = min(begin + each, v.slices);
+    double total = 0.0, run = 0.0;
+    for (;;) {
+        double sum = 0.0;
+        for (uint32_t i = begin; i < end; ++i) sum += part(i);
+        run = block_before_f64(sum, total);
+        if (total > 0.0 || !residual) break;
+        residual = false;  // nothing is left of p: draw from p itself
+    }
+    const double goal = static_cast<double>(s.sample_uniform[seq]) * total;
+    if (tid == 0) {
         first_hit = kNoToken;
-        last_positive = 0;
+        last_mass = 0;
     }
     __syncthreads();
-    const uint32_t slice = shared_slice;
-    if (slice != kNoToken) {
-        const Terms terms(v, seq, d, shared_residual != 0);
-        constexpr int kEach = kSlice / kVerifyThreads;
-        const uint32_t first = slice * kSlice + tid * kEach;
-        double run[kEach];
-        double sum = 0.0;
-        uint32_t last = 0;
-        bool any = false;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const double x = first + i < s.vocab ? terms.term(first + i) : 0.0;
-            sum += x;
-            run[i] = x > 0.0 ? sum : -1.0;
-            if (x > 0.0) {
-                last = first + i;
-                any = true;
+    uint32_t mine = kNoToken, last = kNoToken;
+    double mine_before = 0.0, last_before = 0.0;
+    for (uint32_t i = begin; i < end; ++i) {
+        const double x = part(i);
+        if (x > 0.0) {
+            last = i;
+            last_before = run;
+            if (mine == kNoToken && run + x > goal) {
+                mine = i;
+                mine_before = run;
             }
         }
-        before[tid] = sum;
-        __syncthreads();
-        double offset = 0.0;
-        for (uint32_t i = 0; i < tid; ++i) offset += before[i];
-        if (any) atomicMax(&last_positive, last);
-        for (int i = kEach - 1; i >= 0; --i)
-            if (run[i] >= 0.0 && offset + run[i] > shared_goal) atomicMin(&first_hit, first + i);
-        __syncthreads();
+        run += x;
     }
-    const uint64_t at = static_cast<uint64_t>(seq) * (s.drafts + 1);
-    for (uint32_t i = tid; i <= s.drafts; i += kVerifyThreads) {
-        uint32_t token = kNoToken;
-        if (i < d.row) token = s.draft_tokens[static_cast<uint64_t>(seq) * s.drafts + i];
-        // rounding may leave the goal just past the slice's own running sum
-        if (i == d.row && slice != kNoToken) token = first_hit != kNoToken ? first_hit : last_positive;
-        s.tokens[at + i] = token;
+    if (mine != kNoToken) atomicMin(&first_hit, mine);
+    if (last != kNoToken) atomicMax(&last_mass, last);
+    __syncthreads();
+    const bool hit = first_hit != kNoToken;
+    const uint32_t slice = hit ? first_hit : last_mass;
+    if (hit ? mine == slice : last == slice) shared_before = hit ? mine_before : last_before;
+    __syncthreads();
+    uint32_t drawn = kNoToken;
+    if (total > 0.0) {
+        const double rest = goal - shared_before;
+        double term[kEach], sum = 0.0, all;
+        Terms(v, seq, d, residual).of_slice<true>(slice, s.vocab, table, term);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sum += term[i];
+        double upto = block_before_f64(sum, all);  // its barriers stand between the uses of first_hit
+        if (tid == 0) {
+            first_hit = kNoToken;
+            last_mass = 0;
+        }
+        __syncthreads();
+        const uint32_t at = slice * kSlice + tid * kEach;
+        uint32_t found = kNoToken, with_mass = kNoToken;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            upto += term[i];
+            if (term[i] > 0.0) {
+                with_mass = at + i;
+                if (found == kNoToken && upto > rest) found = at + i;
+            }
+        }
+        if (found != kNoToken) atomicMin(&first_hit, found);
+        if (with_mass != kNoToken) atomicMax(&last_mass, with_mass);
+        __syncthreads();
+        drawn = first_hit != kNoToken ? first_hit : last_mass;
     }
+    const uint64_t to = static_cast<uint64_t>(seq) * (s.drafts + 1);
+    for (uint32_t i = tid; i <= s.drafts; i += kVerifyThreads)
+        s.tokens[to + i] = i < d.row ? s.draft_tokens[static_cast<uint64_t>(seq) * s.drafts + i] : (i == d.row ? drawn : kNoToken);
+    if (tid == 0) s.accepted[seq] = d.row;
 }
 
 uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
@@ -319,6 +463,17 @@ VerifyPlan verify_plan(uint32_t sequences, uint32_t drafts, uint32_t vocab) {
     return p;
 }
 
+template <bool FUSED>
+hipError_t launch_draws(hipStream_t stream, const VerifyParams& v) {
+    if (v.s.draft) {
+        hipLaunchKernelGGL(verify_residual_kernel<FUSED>, dim3(v.slices * v.s.sequences), dim3(kVerifyThreads), 0, stream, v);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(verify_pick_kernel<FUSED>, dim3(v.s.sequences), dim3(kVerifyThreads), 0, stream, v);
+    return hipGetLastError();
+}
+
 }  // namespace
 
 uint64_t verify_draft_workspace(uint32_t sequences, uint32_t drafts, uint32_t vocab) {
@@ -329,21 +484,21 @@ hipError_t launch_verify_draft(hipStream_t stream, const VerifyDraftArgs& s) {
     const VerifyPlan p = verify_plan(s.sequences, s.drafts, s.vocab);
     uint8_t* ws = static_cast<uint8_t*>(s.workspace);
     VerifyParams v{s,
+                   s.inv_temperature * 0x1.71547652b82fep+0,
                    reinterpret_cast<SliceStat*>(ws),
                    reinterpret_cast<SliceStat*>(ws + p.target_bytes),
                    reinterpret_cast<double*>(ws + p.target_bytes + p.draft_bytes),
                    reinterpret_cast<Decision*>(ws + p.target_bytes + p.draft_bytes + p.sum_bytes),
                    p.slices};
-    const uint32_t rows = s.drafts + 1 + (s.draft ? s.drafts : 0);
+    if (s.drafts == 0) v.s.draft = nullptr;
+    const uint32_t rows = s.drafts + 1 + (v.s.draft ? s.drafts : 0);
     hipLaunchKernelGGL(verify_stats_kernel, dim3(p.slices * rows * s.sequences), dim3(kVerifyThreads), 0, stream, v);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(verify_decide_kernel, dim3(s.sequences), dim3(kWave), 0, stream, v);
+    if (s.drafts <= kFusedDrafts) return launch_draws<true>(stream, v);
+    hipLaunchKernelGGL(verify_decide_kernel, dim3(s.sequences), dim3(kVerifyThreads), 0, stream, v);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL(verify_residual_kernel, dim3(p.slices * s.sequences), dim3(kVerifyThreads), 0, stream, v);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    hipLaunchKernelGGL(verify_pick_kernel, dim3(s.sequences), dim3(kVerifyThreads), 0, stream, v);
-    return hipGetLastError();
+    return launch_draws<false>(stream, v);
 }
 
 }  // namespace atlas
