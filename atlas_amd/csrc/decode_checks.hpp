@@ -89,7 +89,7 @@ inline const char* verify_draft_sizes_error(uint32_t sequences, uint32_t drafts,
     if (sequences == 0 || vocab == 0) return "draft verification needs sequences and a vocabulary";
     if (drafts > 1024 || vocab > kMostPositions || sequences > (1u << 20))
         return "draft verification is limited to 1024 drafts, 2^30 logits a row and 2^20 sequences";
-    const uint64_t slices = (static_cast<uint64_t>(vocab) + 4095) / 4096;
+    const uint64_t slices = (static_cast<uint64_t>(vocab) + 1023) / 1024;
     if (slices * (2ull * drafts + 1) * sequences > kMostPositions) return "draft verification has too many logits";
     return nullptr;
 }

@@ -14,7 +14,7 @@
 // terms, which 32-bit sums move by far more than one term; probabilities and
 // sums are in 64 bits throughout.
 //
-// Launches: every row's maximum and sum per slice of 4096 logits; with a draft
+// Launches: every row's maximum and sum per slice of 1024 logits; with a draft
 // model, the residual's sum per slice of the row that was rejected; one
 // workgroup a sequence that finds the slice and the token in it.  The second
 // and third decide for themselves what was accepted (of more than kFusedDrafts
@@ -28,8 +28,9 @@ namespace {
 
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWaves = kVerifyThreads / kWave;
-constexpr uint32_t kSlice = 4096;
-constexpr int kEach = kSlice / kVerifyThreads;
+// the draw itself is one workgroup's: its latency counts
+constexpr int kPickThreads = 1024;
+constexpr uint32_t kSlice = 1024;  // a wavefront's, 16 logits a lane
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr uint32_t kFusedDrafts = 16;
 
@@ -67,19 +68,30 @@ __device__ __forceinline__ double mass(float x, float top, double scale, const d
     return top == -__builtin_inff() ? 0.0 : (x == top ? 1.0 : e);
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-    for (int off = kWave / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
-    return v;
+template <int CTRL, int ROW_MASK, bool BOUND>
+__device__ __forceinline__ double dpp_f64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROW_MASK, 0xf, BOUND);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROW_MASK, 0xf, BOUND);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
-
+// Sum over the wavefront in a fixed tree, the result in every lane (the
+// steps of wave_sum_tree_f32).
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v += dpp_f64<0xb1, 0xf, false>(v);
+    v += dpp_f64<0x4e, 0xf, false>(v);
+    v += dpp_f64<0x141, 0xf, false>(v);
+    v += dpp_f64<0x140, 0xf, false>(v);
+    v += __shfl_xor(v, 16, kWave);
+    return v + __shfl_xor(v, 32, kWave);
+}
 __device__ __forceinline__ double wave_inclusive_scan_f64(double v) {
-    const uint32_t lane = threadIdx.x % kWave;
-#pragma unroll
-    for (uint32_t off = 1; off < kWave; off *= 2) {
-        const double u = __shfl_up(v, off, kWave);
-        v += lane >= off ? u : 0.0;
-    }
+    v += dpp_f64<0x111, 0xf, true>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_f64<0x112, 0xf, true>(v);
+    v += dpp_f64<0x114, 0xf, true>(v);
+    v += dpp_f64<0x118, 0xf, true>(v);
+    v += dpp_f64<0x142, 0xa, false>(v);  // the rows before
+    v += dpp_f64<0x143, 0xc, false>(v);
     return v;
 }
 
@@ -105,82 +117,77 @@ struct VerifyParams {
     SliceStat* draft_stats;   // [sequence][drafts][slices]
     double* slice_sums;       // [sequence][slices]
     Decision* decisions;      // [sequence], of launches that decide apart
-    uint32_t slices;
+    uint32_t slices, blocks;  // of a row; blocks of kVerifyWaves slices
 };
 
 __device__ __forceinline__ uint32_t drafts_of(const VerifyDraftArgs& s, uint32_t seq) {
     return s.draft_lengths ? min(s.draft_lengths[seq], s.drafts) : s.drafts;
 }
 
-// 16 logits of a slice a thread: four of them at a time, thread by thread
-// (WALK: 16 in a row, for running sums).
-template <bool WALK>
+// A lane's logits of a wavefront's slice, four at a time.
+constexpr int kEach = kSlice / kWave;
+__device__ __forceinline__ uint32_t slice_at(int i) { return (i / 4 * kWave + threadIdx.x % kWave) * 4 + i % 4; }
 __device__ __forceinline__ void load_slice(const float* logits, uint32_t first, uint32_t vocab, float (&x)[kEach]) {
     if (first + kSlice <= vocab) {
 #pragma unroll
         for (int i = 0; i < kEach / 4; ++i) {
-            const uint32_t at = WALK ? threadIdx.x * kEach + 4 * i : (i * kVerifyThreads + threadIdx.x) * 4;
-            const f32x4 y = *reinterpret_cast<const f32x4_row*>(logits + first + at);
+            const f32x4 y = *reinterpret_cast<const f32x4_row*>(logits + first + slice_at(4 * i));
 #pragma unroll
             for (int j = 0; j < 4; ++j) x[4 * i + j] = number_or_none(y[j]);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const uint32_t at = first + (WALK ? threadIdx.x * kEach + i : (i / 4 * kVerifyThreads + threadIdx.x) * 4 + i % 4);
+            const uint32_t at = first + slice_at(i);
             x[i] = at < vocab ? number_or_none(logits[at]) : -__builtin_inff();
         }
     }
 }
 
-// A workgroup a slice of a row; rows of a sequence: targets, then drafts.  Its
+// A wavefront a slice of a row; rows of a sequence: targets, then drafts.  Its
 // bytes bound it, once the exponentials are short: 576 rows of 262144 logits
 // take 120 us with the library's exp.
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyParams v) {
     __shared__ double table[32];
-    __shared__ float wave_top[kVerifyWaves];
-    __shared__ double wave_sum[kVerifyWaves];
     const VerifyDraftArgs& s = v.s;
     const uint32_t rows = s.drafts + 1 + (s.draft ? s.drafts : 0);
-    const uint32_t seq = blockIdx.x / (v.slices * rows);
-    const uint32_t rest = blockIdx.x % (v.slices * rows);
-    uint32_t row = rest / v.slices;
-    const uint32_t slice = rest % v.slices;
+    const uint32_t seq = blockIdx.x / (v.blocks * rows);
+    const uint32_t rest = blockIdx.x % (v.blocks * rows);
+    uint32_t row = rest / v.blocks;
+    const uint32_t slice = rest % v.blocks * kVerifyWaves + threadIdx.x / kWave;
     const uint32_t count = drafts_of(s, seq);
     const bool of_target = row <= s.drafts;
     if (!of_target) row -= s.drafts + 1;
     if (row > count || (!of_target && row == count)) return;
     const float* logits = of_target ? s.target + (static_cast<uint64_t>(seq) * (s.drafts + 1) + row) * s.vocab
                                     : s.draft + (static_cast<uint64_t>(seq) * s.drafts + row) * s.vocab;
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     float x[kEach];
-    load_slice<false>(logits, slice * kSlice, s.vocab, x);
+    load_slice(logits, min(slice, v.slices - 1) * kSlice, s.vocab, x);
     exp_table(table);
+    __syncthreads();
+    if (slice >= v.slices) return;
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
     top = wave_max_tree_f32(top);
-    if (lane == 0) wave_top[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
     double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) sum += mass(x[i], top, v.scale, table);
     sum = wave_sum_f64(sum);
-    if (lane == 0) wave_sum[wave] = sum;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
     SliceStat* out = of_target ? v.target_stats + (static_cast<uint64_t>(seq) * (s.drafts + 1) + row) * v.slices
                                : v.draft_stats + (static_cast<uint64_t>(seq) * s.drafts + row) * v.slices;
-    out[slice] = SliceStat{(wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]), top, 0.0f};
+    if (threadIdx.x % kWave == 0) out[slice] = SliceStat{sum, top, 0.0f};
 }
 
-// A row's maximum and sum from its slices, by one wavefront.
-__device__ __forceinline__ void row_stat(const SliceStat* slices, uint32_t count, double scale, const double* table,
-                                         float& top, double& sum) {
+// A row's maximum and sum from its slices, by one wavefront; `first`: the
+// lane's first of them, loaded before.
+__device__ __forceinline__ SliceStat first_stat(const SliceStat* slices, uint32_t count) {
     const uint32_t lane = threadIdx.x % kWave;
-    SliceStat first{0.0, -__builtin_inff(), 0.0f};
-    if (lane < count) first = slices[lane];
+    return lane < count ? slices[lane] : SliceStat{0.0, -__builtin_inff(), 0.0f};
+}
+__device__ __forceinline__ void row_stat(const SliceStat& first, const SliceStat* slices, uint32_t count, double scale,
+                                         const double* table, float& top, double& sum) {
+    const uint32_t lane = threadIdx.x % kWave;
     top = first.top;
     for (uint32_t i = lane + kWave; i < count; i += kWave) top = fmaxf(top, slices[i].top);
     top = wave_max_tree_f32(top);
@@ -192,8 +199,9 @@ __device__ __forceinline__ void row_stat(const SliceStat* slices, uint32_t count
 // The decision of a sequence by a workgroup: the rows' sums by its wavefronts
 // in turn, the drafts' tests by its threads.  The table is filled, and `d` can
 // be read, behind the barriers here.
-template <uint32_t MOST>
+template <int THREADS, uint32_t MOST>
 __device__ void decide(const VerifyParams& v, uint32_t seq, const double* table, Decision& d) {
+    constexpr uint32_t kWaves = THREADS / kWave;
     __shared__ double sums[2][MOST + 1];
     __shared__ float tops[2][MOST + 1];
     __shared__ uint32_t first_rejected;
@@ -201,21 +209,32 @@ __device__ void decide(const VerifyParams& v, uint32_t seq, const double* table,
     const uint32_t count = drafts_of(s, seq), rows = count + 1 + (s.draft ? count : 0);
     if (threadIdx.x == 0) first_rejected = count;
     __syncthreads();
-    for (uint32_t r = threadIdx.x / kWave; r < rows; r += kVerifyWaves) {
-        const bool of_target = r <= count;
-        const uint32_t row = of_target ? r : r - count - 1;
-        const SliceStat* stats = of_target ? v.target_stats + (static_cast<uint64_t>(seq) * (s.drafts + 1) + row) * v.slices
-                                           : v.draft_stats + (static_cast<uint64_t>(seq) * s.drafts + row) * v.slices;
-        float top;
-        double sum;
-        row_stat(stats, v.slices, v.scale, table, top, sum);
-        if (threadIdx.x % kWave == 0) {
-            sums[!of_target][row] = sum;
-            tops[!of_target][row] = top;
+    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+    const auto stats_of = [&](uint32_t r) {
+        return r <= count ? v.target_stats + (static_cast<uint64_t>(seq) * (s.drafts + 1) + r) * v.slices
+                          : v.draft_stats + (static_cast<uint64_t>(seq) * s.drafts + r - count - 1) * v.slices;
+    };
+    // three rows' loads at a time: one after another their latency is most of
+    // a small call
+    for (uint32_t r0 = wave; r0 < rows; r0 += 3 * kWaves) {
+        SliceStat first[3];
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i) first[i] = first_stat(stats_of(min(r0 + i * kWaves, rows - 1)), v.slices);
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i) {
+            const uint32_t r = r0 + i * kWaves;
+            if (r >= rows) break;
+            float top;
+            double sum;
+            row_stat(first[i], stats_of(r), v.slices, v.scale, table, top, sum);
+            if (threadIdx.x % kWave == 0) {
+                sums[r > count][r <= count ? r : r - count - 1] = sum;
+                tops[r > count][r <= count ? r : r - count - 1] = top;
+            }
         }
     }
     __syncthreads();
-    for (uint32_t t = threadIdx.x; t < count; t += kVerifyThreads) {
+    for (uint32_t t = threadIdx.x; t < count; t += THREADS) {
         const uint64_t at = static_cast<uint64_t>(seq) * s.drafts + t;
         const uint32_t token = s.draft_tokens[at];
         double p = 0.0, q = s.draft ? 0.0 : 1.0;
@@ -236,11 +255,11 @@ __device__ void decide(const VerifyParams& v, uint32_t seq, const double* table,
     d.draft_top = s.draft && d.rejected ? tops[1][d.row] : 0.0f;
 }
 
-__global__ __launch_bounds__(kVerifyThreads) void verify_decide_kernel(VerifyParams v) {
+__global__ __launch_bounds__(kPickThreads) void verify_decide_kernel(VerifyParams v) {
     __shared__ double table[32];
     exp_table(table);
     Decision d;
-    decide<1024>(v, blockIdx.x, table, d);
+    decide<kPickThreads, 1024>(v, blockIdx.x, table, d);
     if (threadIdx.x == 0) v.decisions[blockIdx.x] = d;
 }
 
@@ -265,67 +284,60 @@ struct Terms {
         target_scale = d.target_sum > 0.0 ? 1.0 / d.target_sum : 0.0;
         draft_scale = d.draft_sum > 0.0 ? 1.0 / d.draft_sum : 0.0;
     }
-    // A thread's 16 terms of a slice, as load_slice orders them.
-    template <bool WALK>
-    __device__ void of_slice(uint32_t slice, uint32_t vocab, const double* table, double (&term)[kEach]) const {
-        float x[kEach], y[kEach];
-        load_slice<WALK>(target, slice * kSlice, vocab, x);
-        if (draft) load_slice<WALK>(draft, slice * kSlice, vocab, y);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            double p = mass(x[i], target_top, scale, table) * target_scale;
-            if (draft) {
-                const double q = mass(y[i], draft_top, scale, table) * draft_scale;
-                p = p > q ? p - q : 0.0;
-            } else {
-                const uint32_t at = slice * kSlice + (WALK ? threadIdx.x * kEach + i : (i / 4 * kVerifyThreads + threadIdx.x) * 4 + i % 4);
-                p = at == token ? 0.0 : p;
-            }
-            term[i] = p;
-        }
+    __device__ double term(float x, float y, uint32_t at, const double* table) const {
+        const double p = mass(x, target_top, scale, table) * target_scale;
+        if (!draft) return at == token ? 0.0 : p;
+        const double q = mass(y, draft_top, scale, table) * draft_scale;
+        return p > q ? p - q : 0.0;
     }
 };
 
-// A workgroup a slice: the residual's sum there, of a sequence with a draft
-// rejected (of others the slices' own sums serve).
+// A wavefront a slice: the residual's sum there, of a sequence with a draft
+// rejected (of others the slices' own sums serve).  FUSED: every workgroup
+// decides for itself, and the first leaves the decision for the next launch.
 template <bool FUSED>
 __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyParams v) {
     __shared__ double table[32];
-    __shared__ double wave_sum[kVerifyWaves];
-    const uint32_t seq = blockIdx.x / v.slices, slice = blockIdx.x % v.slices;
+    const uint32_t seq = blockIdx.x / v.blocks, block = blockIdx.x % v.blocks;
+    const uint32_t slice = block * kVerifyWaves + threadIdx.x / kWave;
     exp_table(table);
     Decision d;
     if (FUSED) {
-        decide<kFusedDrafts>(v, seq, table, d);
+        decide<kVerifyThreads, kFusedDrafts>(v, seq, table, d);
+        if (block == 0 && threadIdx.x == 0) v.decisions[seq] = d;
     } else {
         d = v.decisions[seq];
         __syncthreads();
     }
-    if (!d.rejected) return;
-    double term[kEach];
-    Terms(v, seq, d, true).of_slice<false>(slice, v.s.vocab, table, term);
+    if (!d.rejected || slice >= v.slices) return;
+    const Terms terms(v, seq, d, true);
+    float x[kEach], y[kEach];
+    load_slice(terms.target, slice * kSlice, v.s.vocab, x);
+    load_slice(terms.draft, slice * kSlice, v.s.vocab, y);
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += term[i];
+    for (int i = 0; i < kEach; ++i) sum += terms.term(x[i], y[i], slice * kSlice + slice_at(i), table);
     sum = wave_sum_f64(sum);
-    if (threadIdx.x % kWave == 0) wave_sum[threadIdx.x / kWave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0)
-        v.slice_sums[static_cast<uint64_t>(seq) * v.slices + slice] = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
+    if (threadIdx.x % kWave == 0) v.slice_sums[static_cast<uint64_t>(seq) * v.slices + slice] = sum;
 }
 
 // Of each thread's value, the sum of those before it and of all.
+template <int THREADS>
 __device__ __forceinline__ double block_before_f64(double v, double& all) {
-    __shared__ double wave_all[kVerifyWaves];
+    constexpr uint32_t kWaves = THREADS / kWave;
+    __shared__ double wave_all[kWaves];
     const double upto = wave_inclusive_scan_f64(v);
     const uint32_t wave = threadIdx.x / kWave;
     __syncthreads();  // wave_all may still be read from a call before
     if (threadIdx.x % kWave == kWave - 1) wave_all[wave] = upto;
     __syncthreads();
     double before = 0.0;
+    all = 0.0;
 #pragma unroll
-    for (uint32_t w = 0; w < kVerifyWaves; ++w) before += w < wave ? wave_all[w] : 0.0;
-    all = (wave_all[0] + wave_all[1]) + (wave_all[2] + wave_all[3]);
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        if (w == wave) before = all;
+        all += wave_all[w];
+    }
     const double own = __shfl_up(upto, 1, kWave);
     return before + (threadIdx.x % kWave ? own : 0.0);
 }
@@ -334,24 +346,35 @@ __device__ __forceinline__ double block_before_f64(double v, double& all) {
 // and the row of results.  Rounding may leave the goal just past the last
 // running sum: the last item with mass is then the one.
 template <bool FUSED>
-__global__ __launch_bounds__(kVerifyThreads) void verify_pick_kernel(VerifyParams v) {
+__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams v) {
     __shared__ double table[32];
     __shared__ uint32_t first_hit, last_mass;
     __shared__ double shared_before;
     const VerifyDraftArgs& s = v.s;
     const uint32_t seq = blockIdx.x, tid = threadIdx.x;
+    // what does not hang on the decision is asked for before it
+    const double* sums = v.slice_sums + static_cast<uint64_t>(seq) * v.slices;
+    const double my_sum = s.draft && tid < v.slices ? sums[tid] : 0.0;
+    const uint32_t my_token = tid < s.drafts ? s.draft_tokens[static_cast<uint64_t>(seq) * s.drafts + tid] : kNoToken;
+    const double uniform = s.sample_uniform[seq];
     exp_table(table);
     Decision d;
     if (FUSED) {
-        decide<kFusedDrafts>(v, seq, table, d);
+        decide<kPickThreads, kFusedDrafts>(v, seq, table, d);
     } else {
         d = v.decisions[seq];
         __syncthreads();
     }
-    const double* sums = v.slice_sums + static_cast<uint64_t>(seq) * v.slices;
     const SliceStat* stats = v.target_stats + (static_cast<uint64_t>(seq) * (s.drafts + 1) + d.row) * v.slices;
     const double target_scale = d.target_sum > 0.0 ? 1.0 / d.target_sum : 0.0;
 
+    // this thread's term of a slice
+    static_assert(kPickThreads == kSlice, "a logit a thread");
+    const auto term_of = [&](const Terms& terms, uint32_t slice) {
+        const uint32_t at = slice * kSlice + tid;
+        if (at >= s.vocab) return 0.0;
+        return terms.term(number_or_none(terms.target[at]), terms.draft ? number_or_none(terms.draft[at]) : 0.0f, at, table);
+    };
     // the slice that lost the token that was proposed with certainty
     uint32_t short_slice = kNoToken;
     double short_sum = 0.0;
@@ -359,31 +382,27 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_pick_kernel(VerifyParam
         const uint32_t token = s.draft_tokens[static_cast<uint64_t>(seq) * s.drafts + d.row];
         if (token < s.vocab) {
             short_slice = token / kSlice;
-            double term[kEach], sum = 0.0;
-            Terms(v, seq, d, true).of_slice<false>(short_slice, s.vocab, table, term);
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) sum += term[i];
-            (void)block_before_f64(sum, short_sum);
+            (void)block_before_f64<kPickThreads>(term_of(Terms(v, seq, d, true), short_slice), short_sum);
         }
     }
     bool residual = true;
     const auto part = [&](uint32_t i) {
-        if (residual && d.rejected && s.draft) return sums[i];
+        if (residual && d.rejected && s.draft) return i == tid ? my_sum : sums[i];
         if (residual && i == short_slice) return short_sum;
         return stats[i].sum * mass(stats[i].top, d.target_top, v.scale, table) * target_scale;
     };
     // slices [begin, end) are this thread's
-    const uint32_t each = (v.slices + kVerifyThreads - 1) / kVerifyThreads;
+    const uint32_t each = (v.slices + kPickThreads - 1) / kPickThreads;
     const uint32_t begin = min(tid * each, v.slices), end = min(begin + each, v.slices);
-    double total = 0.0, run = 0.0;
+    double total = 0.0, run = 0.0, one = 0.0;
     for (;;) {
         double sum = 0.0;
-        for (uint32_t i = begin; i < end; ++i) sum += part(i);
-        run = block_before_f64(sum, total);
+        for (uint32_t i = begin; i < end; ++i) sum += one = part(i);
+        run = block_before_f64<kPickThreads>(sum, total);
         if (total > 0.0 || !residual) break;
         residual = false;  // nothing is left of p: draw from p itself
     }
-    const double goal = static_cast<double>(s.sample_uniform[seq]) * total;
+    const double goal = uniform * total;
     if (tid == 0) {
         first_hit = kNoToken;
         last_mass = 0;
@@ -392,7 +411,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_pick_kernel(VerifyParam
     uint32_t mine = kNoToken, last = kNoToken;
     double mine_before = 0.0, last_before = 0.0;
     for (uint32_t i = begin; i < end; ++i) {
-        const double x = part(i);
+        const double x = each == 1 ? one : part(i);
         if (x > 0.0) {
             last = i;
             last_before = run;
@@ -413,35 +432,27 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_pick_kernel(VerifyParam
     uint32_t drawn = kNoToken;
     if (total > 0.0) {
         const double rest = goal - shared_before;
-        double term[kEach], sum = 0.0, all;
-        Terms(v, seq, d, residual).of_slice<true>(slice, s.vocab, table, term);
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) sum += term[i];
-        double upto = block_before_f64(sum, all);  // its barriers stand between the uses of first_hit
+        const double term = term_of(Terms(v, seq, d, residual), slice);
+        double all;
+        const double upto = block_before_f64<kPickThreads>(term, all) + term;  // its barriers stand between the uses of first_hit
         if (tid == 0) {
             first_hit = kNoToken;
             last_mass = 0;
         }
         __syncthreads();
-        const uint32_t at = slice * kSlice + tid * kEach;
-        uint32_t found = kNoToken, with_mass = kNoToken;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            upto += term[i];
-            if (term[i] > 0.0) {
-                with_mass = at + i;
-                if (found == kNoToken && upto > rest) found = at + i;
-            }
-        }
-        if (found != kNoToken) atomicMin(&first_hit, found);
-        if (with_mass != kNoToken) atomicMax(&last_mass, with_mass);
+        const uint32_t at = slice * kSlice + tid;
+        if (term > 0.0 && upto > rest) atomicMin(&first_hit, at);
+        if (term > 0.0) atomicMax(&last_mass, at);
         __syncthreads();
         drawn = first_hit != kNoToken ? first_hit : last_mass;
     }
     const uint64_t to = static_cast<uint64_t>(seq) * (s.drafts + 1);
-    for (uint32_t i = tid; i <= s.drafts; i += kVerifyThreads)
-        s.tokens[to + i] = i < d.row ? s.draft_tokens[static_cast<uint64_t>(seq) * s.drafts + i] : (i == d.row ? drawn : kNoToken);
-    if (tid == 0) s.accepted[seq] = d.row;
+    // at most as many drafts as threads, and one token more
+    if (tid < s.drafts) s.tokens[to + tid] = tid < d.row ? my_token : (tid == d.row ? drawn : kNoToken);
+    if (tid == 0) {
+        s.tokens[to + s.drafts] = d.row == s.drafts ? drawn : kNoToken;
+        s.accepted[seq] = d.row;
+    }
 }
 
 uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
@@ -463,14 +474,9 @@ VerifyPlan verify_plan(uint32_t sequences, uint32_t drafts, uint32_t vocab) {
     return p;
 }
 
-template <bool FUSED>
-hipError_t launch_draws(hipStream_t stream, const VerifyParams& v) {
-    if (v.s.draft) {
-        hipLaunchKernelGGL(verify_residual_kernel<FUSED>, dim3(v.slices * v.s.sequences), dim3(kVerifyThreads), 0, stream, v);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    hipLaunchKernelGGL(verify_pick_kernel<FUSED>, dim3(v.s.sequences), dim3(kVerifyThreads), 0, stream, v);
+template <typename K>
+hipError_t launch(hipStream_t stream, K kernel, uint32_t blocks, const VerifyParams& v, uint32_t threads = kVerifyThreads) {
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, stream, v);
     return hipGetLastError();
 }
 
@@ -489,16 +495,24 @@ hipError_t launch_verify_draft(hipStream_t stream, const VerifyDraftArgs& s) {
                    reinterpret_cast<SliceStat*>(ws + p.target_bytes),
                    reinterpret_cast<double*>(ws + p.target_bytes + p.draft_bytes),
                    reinterpret_cast<Decision*>(ws + p.target_bytes + p.draft_bytes + p.sum_bytes),
-                   p.slices};
+                   p.slices,
+                   (p.slices + kVerifyWaves - 1) / kVerifyWaves};
     if (s.drafts == 0) v.s.draft = nullptr;
     const uint32_t rows = s.drafts + 1 + (v.s.draft ? s.drafts : 0);
-    hipLaunchKernelGGL(verify_stats_kernel, dim3(p.slices * rows * s.sequences), dim3(kVerifyThreads), 0, stream, v);
-    hipError_t e = hipGetLastError();
+    hipError_t e = launch(stream, verify_stats_kernel, v.blocks * rows * s.sequences, v);
     if (e != hipSuccess) return e;
-    if (s.drafts <= kFusedDrafts) return launch_draws<true>(stream, v);
-    hipLaunchKernelGGL(verify_decide_kernel, dim3(s.sequences), dim3(kVerifyThreads), 0, stream, v);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    return launch_draws<false>(stream, v);
+    // Deciding in the launches that need it saves one; where those are many
+    // workgroups, deciding so often costs more.  Residual of 1 x 12 slices fused
+    // 7 us, apart 5 + 5; of 64 x 64 slices fused 41, apart 5 + 27.
+    const uint32_t blocks = v.blocks * s.sequences;
+    const bool fused = s.drafts <= kFusedDrafts && (v.s.draft ? blocks : s.sequences) <= 256;
+    if (!fused && (e = launch(stream, verify_decide_kernel, s.sequences, v, kPickThreads)) != hipSuccess) return e;
+    if (v.s.draft) {
+        e = fused ? launch(stream, verify_residual_kernel<true>, blocks, v) : launch(stream, verify_residual_kernel<false>, blocks, v);
+        if (e != hipSuccess) return e;
+    }
+    return fused && !v.s.draft ? launch(stream, verify_pick_kernel<true>, s.sequences, v, kPickThreads)
+                               : launch(stream, verify_pick_kernel<false>, s.sequences, v, kPickThreads);
 }
 
 }  // namespace atlas
