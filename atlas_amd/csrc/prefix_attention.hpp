@@ -116,7 +116,8 @@ struct TileRows<kKvQ4_0> : QuantTileRows {
 };
 
 // 8 key dims as stored (unit c = 4 blk + a, the dims of key_dim); offset is
-// the first of them, for a quantised row its block's scale.
+// the first of them, for a quantised row its block's scale.  codes() leaves
+// the stored numbers and returns what they are times.
 template <int FMT>
 struct RawKey;
 template <>
@@ -130,9 +131,10 @@ struct RawKey<kKvF32> {
         x[0] = t.quad(row, o[0]);
         x[1] = t.quad(row, o[1]);
     }
-    __device__ void values(float (&v)[8]) const {
+    __device__ float codes(float (&v)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = x[j >> 2][j & 3];
+        return 1.0f;
     }
 };
 template <>
@@ -146,10 +148,10 @@ struct RawKey<kKvQ8_0> {
         c = *reinterpret_cast<const u32x2_a2*>(t.at(row, o[0]) + 2 + 8 * (unit & 3));
         d = t.scale(row, o[0]);
     }
-    __device__ void values(float (&v)[8]) const {
-        const float s = h2f(d);
+    __device__ float codes(float (&v)[8]) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? c.x : c.y) >> (8 * (j & 3)))) * s;
+        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? c.x : c.y) >> (8 * (j & 3))));
+        return h2f(d);
     }
 };
 template <>
@@ -163,10 +165,10 @@ struct RawKey<kKvQ4_0> {
         c = *reinterpret_cast<const u32_a2*>(t.at(row, o[0]) + 2 + 4 * (unit & 3));
         d = t.scale(row, o[0]);
     }
-    __device__ void values(float (&v)[8]) const {
-        const float s = h2f(d);
+    __device__ float codes(float (&v)[8]) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 3) + 4 * (j >> 2))) & 15u) - 8) * s;
+        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((c >> (8 * (j & 3) + 4 * (j >> 2))) & 15u) - 8);
+        return h2f(d);
     }
 };
 // 4 value dims as stored.
@@ -177,9 +179,10 @@ struct RawValue<kKvF32> {
     f32x4 x;
     static __device__ uint32_t offset(uint32_t quad, uint32_t head_dim) { return 4 * quad < head_dim ? quad * 16 : kNowhere; }
     __device__ void load(const TileRows<kKvF32>& t, uint32_t row, uint32_t, uint32_t o) { x = t.quad(row, o); }
-    __device__ void values(float (&v)[4]) const {
+    __device__ float codes(float (&v)[4]) const {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = x[j];
+        return 1.0f;
     }
 };
 template <>
@@ -193,10 +196,10 @@ struct RawValue<kKvQ8_0> {
         c = *reinterpret_cast<const u32_a2*>(t.at(row, o) + 2 + 4 * (quad & 7));
         d = t.scale(row, o);
     }
-    __device__ void values(float (&v)[4]) const {
-        const float s = h2f(d);
+    __device__ float codes(float (&v)[4]) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(static_cast<int8_t>(c >> (8 * j))) * s;
+        for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(static_cast<int8_t>(c >> (8 * j)));
+        return h2f(d);
     }
 };
 template <>
@@ -209,13 +212,20 @@ struct RawValue<kKvQ4_0> {
         c = *reinterpret_cast<const uint16_t*>(t.at(row, o) + 2 + 2 * (quad & 7));
         d = t.scale(row, o);
     }
-    __device__ void values(float (&v)[4]) const {
-        const float s = h2f(d);
+    __device__ float codes(float (&v)[4]) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            v[j] = static_cast<float>((c >> (8 * (j & 1) + 4 * (j >> 1)) & 15) - 8) * s;
+        for (int j = 0; j < 4; ++j) v[j] = static_cast<float>((c >> (8 * (j & 1) + 4 * (j >> 1)) & 15) - 8);
+        return h2f(d);
     }
 };
+
+// The numbers themselves: f32 holds a code times a block's scale exactly.
+template <class Raw, int N>
+__device__ __forceinline__ void raw_values(const Raw& raw, float (&v)[N]) {
+    const float s = raw.codes(v);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] *= s;
+}
 
 // The dims of unit `unit` of a query row, scaled.
 template <int FMT>

@@ -49,7 +49,7 @@ __device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const floa
 // operand that O^T = V^T P^T wants, so P never leaves its registers and a
 // row's statistics are the lane's own.  Queries wait in LDS.
 template <int FMT, int NB, int NR>
-__global__ __launch_bounds__(kAttnThreads, NR == 1 && NB < 8 ? 2 : 1) void attn_rows_kernel(AttnParams a) {
+__global__ __launch_bounds__(kAttnThreads, NB < 8 ? 2 : 1) void attn_rows_kernel(AttnParams a) {
     constexpr int NG = (NB + 1) / 2;  // groups of 64 dims
     constexpr int kRoom = NR * NB * 2 > 2 * (NG * 4 + 1) ? NR * NB * 2 : 2 * (NG * 4 + 1);
     // queries [row tile][step][half]; at the end two wavefronts' sums
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kAttnThreads, NR == 1 && NB < 8 ? 2 : 1) void attn_
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float x[8];
-            k[b].values(x);
+            raw_values(k[b], x);
 #pragma unroll
             for (int t = 0; t < NR; ++t) {
                 const f32x4 q0 = room[2 * (t * NB + b)][lane], q1 = room[2 * (t * NB + b) + 1][lane];
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kAttnThreads, NR == 1 && NB < 8 ? 2 : 1) void attn_
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 float x[4];
-                raw_v[r][g].values(x);
+                raw_values(raw_v[r][g], x);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[r][4 * g + j] = x[j];
             }
@@ -286,10 +286,10 @@ __global__ __launch_bounds__(kAttnThreads, NR == 1 && NB < 8 ? 2 : 1) void attn_
     }
 }
 
-// One workgroup a row: its segments joined, and the base-2 logarithm of its
-// sum (+inf where it saw nothing) for the weights.  LANES lanes hold a
-// segment's dims; as many segments as fit the workgroup are taken at once, and
-// their sums meet in LDS in the segments' order.
+// One workgroup a row, or 4 LANES dims of one: its segments joined, and the
+// base-2 logarithm of its sum (+inf where it saw nothing) for the weights.
+// LANES lanes hold a segment's dims; as many segments as fit the workgroup are
+// taken at once, and their sums meet in LDS in the segments' order.
 template <int LANES>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, float* output, float* log_sum) {
     constexpr uint32_t kGroups = kAttnThreads / LANES;
@@ -308,8 +308,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, f
     top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
     const float base = top == neg_inf() ? 0.0f : top;
     const uint32_t group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
-    const bool holds = 4 * lane < a.head_dim;
-    const float* parts = a.partial_out + row * a.head_dim + (holds ? 4 * lane : 0);
+    const uint32_t dim = 4 * (blockIdx.y * LANES + lane);
+    const bool holds = dim < a.head_dim;
+    const float* parts = a.partial_out + row * a.head_dim + (holds ? dim : 0);
     float sum = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -338,9 +339,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, f
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = sum == 0.0f ? 0.0f : o[j] / sum;
         float* p = output + (static_cast<uint64_t>(r / a.group) * a.q_heads + kv_head * a.group + r % a.group) * a.head_dim;
-        *reinterpret_cast<f32x4*>(p + 4 * lane) = y;
+        *reinterpret_cast<f32x4*>(p + dim) = y;
     }
-    if (log_sum && lane == 0) {
+    if (log_sum && dim == 0) {
         const uint64_t seq = r / a.seq_rows;
         log_sum[(seq * a.kv_heads + kv_head) * a.seq_rows + r % a.seq_rows] =
             sum == 0.0f ? __builtin_inff() : base + __builtin_log2f(sum);
@@ -400,13 +401,21 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     const uint32_t wanted = 512;
     if (s.prefix_length && rows > 16) {
         p.wide = true;
-        const bool packed = rows >= 512;
-        if (packed) p.packed_bytes = round256(attn_packed_bytes(s.head_dim, s.kv_heads, s.prefix_length));
-        p.prefix_tiles = static_cast<uint32_t>(packed ? (rows + 127) / 128 : (rows + 63) / 64);
-        const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         const uint32_t pad = s.head_dim <= 64 ? 64 : (s.head_dim <= 128 ? 128 : 256);
         const uint32_t tile = 32 * 256 / pad;
         const uint32_t most = (s.prefix_length + tile - 1) / tile;
+        // Packing converts a tile of keys once, not once for every 64 rows, for a
+        // launch and a copy of the tiles: it pays from eight such row tiles and
+        // three tiles of keys a workgroup on.  Whole calls without and with it,
+        // us, rows x prompt, one KV head of 256 and four of 128:
+        //   256 x 4097   43 / 45   45 / 42     480 x 4097    48 / 49   (512) 56 / 50
+        //   256 x 32768  71 / 80  108 / 105    512 x 32768  100 / 100
+        //   512 x 1000   37 / 42   37 / 39     2048 x 4097   77 / 70   (1024) 82 / 70
+        const uint64_t row_tiles = (rows + 63) / 64;
+        const bool packed = row_tiles >= 8 && row_tiles * most * s.kv_heads >= 3 * 512;
+        if (packed) p.packed_bytes = round256(attn_packed_bytes(s.head_dim, s.kv_heads, s.prefix_length));
+        p.prefix_tiles = static_cast<uint32_t>(packed ? (rows + 127) / 128 : row_tiles);
+        const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         // two workgroups to a CU, or one of eight wavefronts
         const uint64_t whole = packed ? 256 : 512;
         uint64_t want = units >= whole ? 1 : whole / units;
@@ -514,8 +523,11 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     const uint64_t all = static_cast<uint64_t>(a.rows) * a.kv_heads;
-    const dim3 join_grid(static_cast<uint32_t>(all)), join_block(kAttnThreads);
-    if (s.head_dim <= 64)
+    // Few rows have many segments, and a workgroup for every 64 dims of one reads
+    // them sooner: 64 rows of 256 with 520 segments 18.9 -> 8.6 us.
+    const uint32_t pieces = all < 512 ? (s.head_dim + 63) / 64 : 1;
+    const dim3 join_grid(static_cast<uint32_t>(all), pieces), join_block(kAttnThreads);
+    if (s.head_dim <= 64 * pieces)
         hipLaunchKernelGGL(attn_join_kernel<16>, join_grid, join_block, 0, stream, a, s.output, log_sum);
     else if (s.head_dim <= 128)
         hipLaunchKernelGGL(attn_join_kernel<32>, join_grid, join_block, 0, stream, a, s.output, log_sum);

@@ -52,7 +52,10 @@ __device__ __forceinline__ Pieces pieces(const float (&x)[8]) {
     for (int i = 0; i < 4; ++i) {
         const f32x2_t y = {x[2 * i], x[2 * i + 1]};
         const half2_t h = __builtin_convertvector(y, half2_t);
-        const f32x2_t rest = {y.x - static_cast<float>(h.x), y.y - static_cast<float>(h.y)};
+        // y - h in one instruction each, exactly
+        f32x2_t rest;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest.x) : "v"(h), "v"(y.x));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rest.y) : "v"(h), "v"(y.y));
         const half2_t l = __builtin_convertvector(rest, half2_t);
         p.hi[2 * i] = h.x;
         p.hi[2 * i + 1] = h.y;
@@ -134,13 +137,15 @@ __device__ __forceinline__ void convert_keys(const RawKeys<FMT, D>& raw, WideTil
     using W = Wide<D>;
 #pragma unroll
     for (int i = 0; i < W::KI; ++i) {
-        float x[W::KU][8];
+        float x[W::KU][8], times[W::KU];
         float top = 0.0f;
 #pragma unroll
         for (int u = 0; u < W::KU; ++u) {
-            raw.at[i][u].values(x[u]);
+            times[u] = raw.at[i][u].codes(x[u]);
+            float most = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = max_mag(top, x[u][j]);
+            for (int j = 0; j < 8; ++j) most = max_mag(most, x[u][j]);
+            top = max_mag(top, most * times[u]);
         }
         top = max_xor32(max_xor16(max_xor8(top)));
         const int e = row_exponent(top, 100);
@@ -150,7 +155,7 @@ __device__ __forceinline__ void convert_keys(const RawKeys<FMT, D>& raw, WideTil
 #pragma unroll
         for (int u = 0; u < W::KU; ++u) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[u][j] *= scale;
+            for (int j = 0; j < 8; ++j) x[u][j] *= times[u] * scale;
             const Pieces p = pieces(x[u]);
             const uint32_t unit = lane / 8 + 8 * u;
             const uint32_t frag = (key / 16 * W::KS + unit / 4) * 2, to = unit % 4 * 16 + key % 16;
@@ -166,12 +171,12 @@ __device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTi
     constexpr uint32_t kQuads = D / 4;
     const uint32_t group = wave * (kWave / kQuads) + lane / kQuads, quad = lane % kQuads;
     const uint32_t key0 = 32 * (group / 4) + 4 * (group % 4);
-    float x[8][4];  // [key][dim]
+    float x[8][4], times[8];  // [key][dim]
     float top[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        raw.at[j].values(x[j]);
-        top[j] = fmaxf(max_mag(x[j][0], x[j][1]), max_mag(x[j][2], x[j][3]));
+        times[j] = raw.at[j].codes(x[j]);
+        top[j] = __builtin_fabsf(fmaxf(max_mag(x[j][0], x[j][1]), max_mag(x[j][2], x[j][3])) * times[j]);
     }
     // eight maxima over the group's lanes: each step halves what a lane keeps,
     // ending with key lane % 8
@@ -198,10 +203,12 @@ __device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTi
     const f32x4 s0 = *reinterpret_cast<const f32x4*>(&tile.value_scale[key0]);
     const f32x4 s1 = *reinterpret_cast<const f32x4*>(&tile.value_scale[key0 + 16]);
 #pragma unroll
+    for (int j = 0; j < 8; ++j) times[j] *= j < 4 ? s0[j & 3] : s1[j & 3];
+#pragma unroll
     for (int e = 0; e < 4; ++e) {
         float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[j][e] * (j < 4 ? s0[j & 3] : s1[j & 3]);
+        for (int j = 0; j < 8; ++j) y[j] = x[j][e] * times[j];
         const Pieces p = pieces(y);
         // dim e of quad q: row q % 16 of block 4 (q / 16) + e
         const uint32_t frag = (group / 4 * W::DT + 4 * (quad / 16) + e) * 2, to = group % 4 * 16 + quad % 16;
@@ -527,13 +534,14 @@ __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnPara
 #pragma unroll
         for (uint32_t c = 0; c < (kChunks + 7) / 8; ++c) {
             const uint32_t chunk = c * 8 + wave;
-            // 64 lanes of 16 bytes to LDS at M0; nothing comes back to a register
+            // 64 lanes of 16 bytes to LDS at M0, which the compiler keeps nothing
+            // in; nothing comes back to a register
             if (chunk < kChunks)
                 asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                              :
                              : "s"(lds + buffer * static_cast<uint32_t>(sizeof(WideTile<D>)) + chunk * 1024),
                                "v"(lane * 16), "s"(from + chunk * 1024)
-                             : "memory", "m0");
+                             : "memory");
         }
     };
     if (item.begin < end) copy(item.begin, 0);
