@@ -22,7 +22,10 @@ inline bool overlaps(const void* a, const void* b, uint64_t bytes) {
 
 inline bool misaligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
-constexpr uint32_t kMostPositions = 1u << 30;  // of one cache row, token row or logit index
+constexpr uint32_t kMostPositions = 1u << 29;  // of one cache, or logits of a row
+constexpr uint32_t kMostSequences = 1u << 20;
+// A launch has less than 2^32 threads: 256 of them to each of these.
+constexpr uint32_t kMostGroups = 1u << 23;
 
 inline const char* prefix_attention_sizes_error(const PrefixAttentionArgs& a) {
     if (a.format != kKvF32 && a.format != kKvQ8_0 && a.format != kKvQ4_0) return "unknown cache format";
@@ -35,7 +38,7 @@ inline const char* prefix_attention_sizes_error(const PrefixAttentionArgs& a) {
         static_cast<uint64_t>(a.sequences) * a.capacity > std::numeric_limits<uint32_t>::max())
         return "prefix attention cache positions overflow";
     const uint64_t rows = static_cast<uint64_t>(a.sequences) * a.tokens;
-    if (rows > kMostPositions || rows * a.q_heads > kMostPositions) return "prefix attention has more than 2^30 query rows";
+    if (rows > kMostGroups || rows * a.q_heads > kMostGroups) return "prefix attention has more than 2^23 query rows";
     if (static_cast<uint64_t>(a.kv_heads) * a.head_dim > 32768) return "prefix attention cache rows are limited to 32768 values";
     return nullptr;
 }
@@ -66,10 +69,10 @@ inline const char* prefix_attention_error(const PrefixAttentionArgs& a) {
 inline const char* kv_evict_error(const KvEvictArgs& a, int format, uint32_t kv_width) {
     if (!a.cache || !a.cache_out || !a.weights || !a.weights_out || !a.lengths || !a.lengths_out || !a.kept)
         return "KV evict buffer is null";
-    if (a.sequences == 0 || a.capacity == 0 || kv_width == 0 || kv_width > 32768 || a.sequences > kMostPositions ||
+    if (a.sequences == 0 || a.capacity == 0 || kv_width == 0 || kv_width > 32768 || a.sequences > kMostSequences ||
         a.capacity > kMostPositions ||
         static_cast<uint64_t>(a.sequences) * a.capacity > std::numeric_limits<uint32_t>::max())
-        return "KV evict dimensions are invalid (sequences * capacity below 2^32, kv_width 1..32768)";
+        return "KV evict dimensions are invalid (sequences * capacity below 2^32, at most 2^20 sequences, kv_width 1..32768)";
     if (a.budget == 0 || a.budget > a.capacity || a.recent > a.budget)
         return "KV evict needs recent <= budget and 1 <= budget <= capacity";
     if (format != kKvF32 && kv_width % 32 != 0) return "quantized KV rows need kv_width % 32 == 0";
@@ -87,10 +90,10 @@ inline const char* kv_evict_error(const KvEvictArgs& a, int format, uint32_t kv_
 
 inline const char* verify_draft_sizes_error(uint32_t sequences, uint32_t drafts, uint32_t vocab) {
     if (sequences == 0 || vocab == 0) return "draft verification needs sequences and a vocabulary";
-    if (drafts > 1024 || vocab > kMostPositions || sequences > (1u << 20))
-        return "draft verification is limited to 1024 drafts, 2^30 logits a row and 2^20 sequences";
-    const uint64_t slices = (static_cast<uint64_t>(vocab) + 1023) / 1024;
-    if (slices * (2ull * drafts + 1) * sequences > kMostPositions) return "draft verification has too many logits";
+    if (drafts > 1024 || vocab > kMostPositions || sequences > kMostSequences)
+        return "draft verification is limited to 1024 drafts, 2^29 logits a row and 2^20 sequences";
+    const uint64_t groups = (static_cast<uint64_t>(vocab) + 4095) / 4096;  // a wavefront 1024 logits
+    if (groups * (2ull * drafts + 1) * sequences > kMostGroups) return "draft verification has too many logits";
     return nullptr;
 }
 

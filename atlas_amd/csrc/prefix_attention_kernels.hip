@@ -354,26 +354,29 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, f
 __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a, const float* log_sum, const float* in,
                                                                     float* out) {
     __shared__ float sums[kAttnWaves][kWave];
-    const uint32_t blocks = (a.capacity + kWave - 1) / kWave;
-    const uint32_t seq = blockIdx.x / blocks;
-    const uint32_t length = min(a.lengths[seq], a.capacity);
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const uint32_t key = blockIdx.x % blocks * kWave + lane;
-    if (blockIdx.x % blocks * kWave >= length) return;
+    const uint32_t key = blockIdx.x * kWave + lane;
     const uint32_t lines = a.kv_heads * a.seq_rows, part = (lines + kAttnWaves - 1) / kAttnWaves;
     const uint32_t begin = min(wave * part, lines), end = min(begin + part, lines);
-    const float* logs = log_sum + static_cast<uint64_t>(seq) * lines;
-    const float* scores = a.scores + static_cast<uint64_t>(seq) * lines * a.score_pitch + min(key, length - 1);
-    float sum = 0.0f;
+    // launches have at most 65535 workgroups in y
+    for (uint32_t seq = blockIdx.y; seq < a.rows / a.seq_rows; seq += gridDim.y) {
+        const uint32_t length = min(a.lengths[seq], a.capacity);
+        if (blockIdx.x * kWave >= length) continue;
+        const float* logs = log_sum + static_cast<uint64_t>(seq) * lines;
+        const float* scores = a.scores + static_cast<uint64_t>(seq) * lines * a.score_pitch + min(key, length - 1);
+        float sum = 0.0f;
 #pragma unroll 8
-    for (uint32_t i = begin; i < end; ++i)
-        sum += __builtin_amdgcn_exp2f(scores[static_cast<uint64_t>(i) * a.score_pitch] - logs[i]);
-    sums[wave][lane] = sum;
-    __syncthreads();
-    if (wave || key >= length) return;
-    sum = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
-    const uint64_t at = static_cast<uint64_t>(seq) * a.capacity + key;
-    out[at] = in ? in[at] + sum : sum;
+        for (uint32_t i = begin; i < end; ++i)
+            sum += __builtin_amdgcn_exp2f(scores[static_cast<uint64_t>(i) * a.score_pitch] - logs[i]);
+        sums[wave][lane] = sum;
+        __syncthreads();
+        if (wave == 0 && key < length) {
+            sum = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+            const uint64_t at = static_cast<uint64_t>(seq) * a.capacity + key;
+            out[at] = in ? in[at] + sum : sum;
+        }
+        __syncthreads();
+    }
 }
 
 // How the work is laid out, and what of the workspace it takes.
@@ -411,9 +414,11 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         //   256 x 4097   43 / 45   45 / 42     480 x 4097    48 / 49   (512) 56 / 50
         //   256 x 32768  71 / 80  108 / 105    512 x 32768  100 / 100
         //   512 x 1000   37 / 42   37 / 39     2048 x 4097   77 / 70   (1024) 82 / 70
-        const uint64_t row_tiles = (rows + 63) / 64;
-        const bool packed = row_tiles >= 8 && row_tiles * most * s.kv_heads >= 3 * 512;
-        if (packed) p.packed_bytes = round256(attn_packed_bytes(s.head_dim, s.kv_heads, s.prefix_length));
+        // Tiles take as much as the prompt in f32, of which a caller may have none to
+        // spare beside a very long one: 4 GiB at most.
+        const uint64_t row_tiles = (rows + 63) / 64, packed_bytes = attn_packed_bytes(s.head_dim, s.kv_heads, s.prefix_length);
+        const bool packed = row_tiles >= 8 && row_tiles * most * s.kv_heads >= 3 * 512 && packed_bytes <= 1ull << 32;
+        if (packed) p.packed_bytes = round256(packed_bytes);
         p.prefix_tiles = static_cast<uint32_t>(packed ? (rows + 127) / 128 : row_tiles);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         // two workgroups to a CU, or one of eight wavefronts
@@ -535,7 +540,7 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
         hipLaunchKernelGGL(attn_join_kernel<64>, join_grid, join_block, 0, stream, a, s.output, log_sum);
     e = hipGetLastError();
     if (e != hipSuccess || !s.weights_out) return e;
-    hipLaunchKernelGGL(attn_weights_kernel, dim3((s.capacity + kWave - 1) / kWave * s.sequences),
+    hipLaunchKernelGGL(attn_weights_kernel, dim3((s.capacity + kWave - 1) / kWave, s.sequences < 65535 ? s.sequences : 65535),
                        dim3(kAttnThreads), 0, stream, a, log_sum, s.weights_in, s.weights_out);
     return hipGetLastError();
 }

@@ -195,7 +195,8 @@ __device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTi
         const int e = row_exponent(m, 76);
         tile.value_exp[key] = e;
         tile.value_expf[key] = static_cast<float>(e);
-        tile.value_scale[key] = pow2i(-e);
+        // an infinity would leave the row's other values no bits: NaN, not a wrong number
+        tile.value_scale[key] = m == __builtin_inff() ? __builtin_nanf("") : pow2i(-e);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();

@@ -413,13 +413,18 @@ int atlas_hip_kv_append_q4_0(atlas_hip_ctx *ctx, const float *key, const float *
  *
  * head_dim is at most 256 and a multiple of 4 (f32) or 32 (Q8_0, Q4_0);
  * kv_heads divides q_heads; q, output, f32 caches and the workspace are
- * 16-byte aligned, quantised caches 2-byte; output does not overlap q.  What a row does not see never
- * reaches it, whatever it holds.  Scores, sums and accumulators are f32
- * (within 1e-5 of float64 normwise); a call's result does not depend on
- * timing.  The workspace (atlas_hip_prefix_attention_workspace bytes) is
- * overwritten by every call and holds nothing between calls: calls that can
- * overlap, and graphs whose replays can, need one each.  weights != 0 asks
- * for the size with weights_out. */
+ * 16-byte aligned, quantised caches 2-byte; output does not overlap q.
+ * sequences * tokens * q_heads <= 2^23, prefix_length and capacity <= 2^29,
+ * sequences * capacity < 2^32, kv_heads * head_dim <= 32768.  What a row does
+ * not see never reaches it, whatever it holds; what it sees has to be finite,
+ * with sums of values below 2^119 (a row that sees anything else may be NaN in
+ * every dim).  Scores, sums and accumulators are f32 (within 1e-5 of float64
+ * normwise); a call's result does not depend on timing.  The workspace
+ * (atlas_hip_prefix_attention_workspace bytes at the call's own sizes; smaller
+ * sizes can need more) is overwritten by every call and holds nothing between
+ * calls: calls that can overlap, and graphs whose replays can, need one each.
+ * For large batches it holds the prompt's rows once more, in 4 bytes a value
+ * and at most 4 GiB.  weights != 0 asks for the size with weights_out. */
 int atlas_hip_prefix_attention_workspace(atlas_hip_ctx *ctx, int format, uint32_t sequences, uint32_t tokens,
                                          uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
                                          uint32_t prefix_length, uint32_t capacity, int weights, uint64_t *bytes);
@@ -453,7 +458,7 @@ int atlas_hip_prefix_attention_q4_0(atlas_hip_ctx *ctx, const float *q, const ui
  * to +0.  Kept rows of both planes and their weights move to the front in
  * their order; lengths_out[b] = min(n, budget); kept[b, i] is the row that row
  * i was ([sequences, budget], 0xffffffff behind the last).  Rows and weights
- * behind the kept ones are left as they were.  cache_out, weights_out and
+ * behind the kept ones are left as they were.  At most 2^20 sequences.  cache_out, weights_out and
  * lengths_out may each be the input buffer (an in-place cut, which leaves the
  * rows in front of the first evicted one alone); otherwise they must not
  * overlap it.  kv_width is a multiple of 32 for Q8_0 and Q4_0; f32 caches are
@@ -532,7 +537,8 @@ int atlas_hip_softcap_argmax_f32_noalloc(atlas_hip_ctx *ctx, const float *logits
  * vocab], draft_logits [sequences, drafts, vocab]; drafts may be 0 (sampling).
  * NaN and -inf logits have no mass, all of a row's mass lies on its +inf; a
  * row without mass rejects its draft and draws 0xffffffff; a drafted token >=
- * vocab is rejected.  Probabilities and sums are float64, so that the drawn
+ * vocab is rejected.  At most 1024 drafts, 2^29 logits a row and 2^20
+ * sequences.  Probabilities and sums are float64, so that the drawn
  * token does not depend on how the sums are split.  Workspace as for
  * prefix_attention (16-byte aligned, one for each of overlapping calls).
  * accepted and tokens must not overlap the inputs. */

@@ -43,34 +43,45 @@ def attention(q, prefix, prefix_length, cache, lengths, capacity, kv_heads, scal
     out, mass = np.zeros(q.shape), np.zeros(q.shape)
     dot = np.zeros((B, T, H))
     got = np.zeros((B, capacity))
-    if prefix_length:
-        pk, pv = cache_values(prefix[:, :prefix_length], fmt).reshape(2, prefix_length, kv_heads, D)
+    own = {}
     for b in range(B):
         n = min(int(lengths[b]), capacity) if capacity else 0
         if n:
-            own = cache_values(cache[:, b * capacity:b * capacity + n], fmt).reshape(2, n, kv_heads, D)
-        for t in range(T):
-            see = max(0, n - (T - 1 - t))
-            for h in range(H):
-                kh = h // G
-                keys = [pk[:, kh]] if prefix_length else []
-                vals = [pv[:, kh]] if prefix_length else []
-                if see:
-                    keys.append(own[0, :see, kh])
-                    vals.append(own[1, :see, kh])
-                if not keys:
+            own[b] = cache_values(cache[:, b * capacity:b * capacity + n], fmt).reshape(2, n, kv_heads, D)
+    if prefix_length:
+        pk, pv = cache_values(prefix[:, :prefix_length], fmt).reshape(2, prefix_length, kv_heads, D)
+    with np.errstate(invalid="ignore", over="ignore"):
+        for kh in range(kv_heads):
+            rows = q[:, :, kh * G:(kh + 1) * G].astype(np.float64).reshape(B * T * G, D)
+            if prefix_length:  # every row sees the prompt
+                k, v = np.ascontiguousarray(pk[:, kh]), np.ascontiguousarray(pv[:, kh])
+                x = rows @ k.T * scale
+                dots = (np.abs(rows) @ np.abs(k).T).max(1) * abs(scale)
+            for i, row in enumerate(rows):
+                b, t, h = i // (T * G), i // G % T, kh * G + i % G
+                n = own[b].shape[1] if b in own else 0
+                see = max(0, n - (T - 1 - t))
+                if not see and not prefix_length:
                     continue
-                k, v = np.concatenate(keys), np.concatenate(vals)
-                qq = q[b, t, h].astype(np.float64)
-                with np.errstate(invalid="ignore", over="ignore"):
-                    x = k @ qq * scale
-                    p = np.exp(x - x.max())
-                    p /= p.sum()
-                    out[b, t, h] = p @ v
-                    mass[b, t, h] = p @ np.abs(v)
-                    dot[b, t, h] = (np.abs(k) @ np.abs(qq)).max() * abs(scale)
+                xs = [x[i]] if prefix_length else []
                 if see:
-                    got[b, :see] += p[prefix_length:]
+                    ok, ov = own[b][0, :see, kh], own[b][1, :see, kh]
+                    xs.append(ok @ row * scale)
+                    dot[b, t, h] = (np.abs(ok) @ np.abs(row)).max() * abs(scale)
+                if prefix_length:
+                    dot[b, t, h] = max(dot[b, t, h], dots[i])
+                p = np.concatenate(xs)
+                p = np.exp(p - p.max())
+                p /= p.sum()
+                if prefix_length:
+                    x[i] = p[:prefix_length]
+                if see:
+                    mine = p[prefix_length:]
+                    out[b, t, h], mass[b, t, h] = mine @ ov, mine @ np.abs(ov)
+                    got[b, :see] += mine
+            if prefix_length:
+                out[:, :, kh * G:(kh + 1) * G] += (x @ v).reshape(B, T, G, D)
+                mass[:, :, kh * G:(kh + 1) * G] += (x @ np.abs(v)).reshape(B, T, G, D)
     return out, got, (mass, dot)
 
 

@@ -47,7 +47,7 @@ def call(fn, base, change):
     dict(weights_in=0), dict(weights_in=0, weights_out=0), dict(weights_in=9 * M), dict(head_dim=4), dict(head_dim=256),
     dict(format=1, cache=4 * M + 2, prefix=2 * M + 2), dict(format=2, head_dim=96), dict(scale=-1.0), dict(scale=0.0),
     dict(sequences=1, tokens=1, q_heads=1, kv_heads=1), dict(tokens=4097), dict(prefix_length=128),
-    dict(prefix_length=1 << 30, prefix_capacity=1 << 31), dict(sequences=3, capacity=1 << 30, weights_in=0), dict(kv_heads=128, q_heads=128, head_dim=256),
+    dict(prefix_length=1 << 29, prefix_capacity=1 << 31), dict(sequences=7, capacity=1 << 29, weights_in=0), dict(kv_heads=128, q_heads=128, head_dim=256),
 ])
 def test_attention_calls_that_are_allowed(checks, change):
     assert call(checks.check_prefix_attention, ATTEND, change) is None
@@ -61,7 +61,8 @@ def test_attention_calls_that_are_allowed(checks, change):
     dict(weights_out=0), dict(weights_in=9 * M + 16), dict(scale=math.nan), dict(scale=math.inf), dict(q=M + 4),
     dict(output=7 * M + 8), dict(workspace=10 * M + 4), dict(prefix=2 * M + 4), dict(cache=4 * M + 8),
     dict(format=1, cache=4 * M + 1), dict(weights_out=9 * M + 2), dict(lengths=6 * M + 1), dict(output=M), dict(output=M + 16),
-    dict(output=M - 16), dict(sequences=4, capacity=1 << 30), dict(prefix_length=(1 << 30) + 1, prefix_capacity=1 << 31),
+    dict(output=M - 16), dict(sequences=8, capacity=1 << 29), dict(prefix_length=(1 << 29) + 1, prefix_capacity=1 << 31),
+    dict(sequences=1 << 20, tokens=1, q_heads=9, kv_heads=3),
     dict(sequences=1 << 31, capacity=1), dict(tokens=1 << 28), dict(kv_heads=256, q_heads=256, head_dim=256),
 ])
 def test_attention_calls_that_are_refused(checks, change):
@@ -71,7 +72,7 @@ def test_attention_calls_that_are_refused(checks, change):
 @pytest.mark.parametrize("change", [
     {}, dict(cache_out=M), dict(weights_out=16 * M), dict(lengths_out=18 * M), dict(budget=1000, recent=1000), dict(budget=1, recent=0),
     dict(kv_width=1), dict(kv_width=32768), dict(format=1, cache=M + 2), dict(format=2, kv_width=32),
-    dict(cache_out=M + 2 * 4000 * 96 * 4), dict(sequences=3, capacity=1 << 30, cache_out=1 << 50, weights_out=16 * M)])
+    dict(cache_out=M + 2 * 4000 * 96 * 4), dict(sequences=7, capacity=1 << 29, cache_out=1 << 50, weights_out=16 * M)])
 def test_evict_calls_that_are_allowed(checks, change):
     assert call(checks.check_kv_evict, EVICT, change) is None
 
@@ -81,21 +82,21 @@ def test_evict_calls_that_are_allowed(checks, change):
     dict(sequences=0), dict(capacity=0), dict(kv_width=0), dict(kv_width=32769), dict(budget=0), dict(budget=1001), dict(recent=501),
     dict(format=1, kv_width=48), dict(format=2, kv_width=100), dict(cache=M + 2), dict(format=1, cache=M + 1), dict(kept=20 * M + 2),
     dict(cache_out=M + 16), dict(cache_out=M + 2 * 4000 * 96 * 4 - 4), dict(cache_out=M - 4), dict(weights_out=16 * M + 4),
-    dict(lengths_out=18 * M + 4), dict(sequences=4, capacity=1 << 30), dict(sequences=1 << 31, capacity=1, budget=1, recent=0)])
+    dict(lengths_out=18 * M + 4), dict(sequences=8, capacity=1 << 29), dict(sequences=(1 << 20) + 1, capacity=1, budget=1, recent=0)])
 def test_evict_calls_that_are_refused(checks, change):
     assert call(checks.check_kv_evict, EVICT, change)
 
 
 @pytest.mark.parametrize("change", [
     {}, dict(draft=0), dict(draft_lengths=0), dict(drafts=0, draft=0, draft_tokens=0, accept=0), dict(vocab=1), dict(drafts=1024),
-    dict(inv_temperature=1e-3), dict(vocab=1 << 30, drafts=1, sequences=1)])
+    dict(inv_temperature=1e-3), dict(vocab=1 << 29, drafts=1, sequences=1)])
 def test_verify_calls_that_are_allowed(checks, change):
     assert call(checks.check_verify_draft, VERIFY, change) is None
 
 
 @pytest.mark.parametrize("change", [
     dict(target=0), dict(draft_tokens=0), dict(accept=0), dict(sample=0), dict(accepted=0), dict(tokens=0), dict(workspace=0),
-    dict(sequences=0), dict(vocab=0), dict(drafts=1025), dict(vocab=(1 << 30) + 1), dict(sequences=(1 << 20) + 1),
+    dict(sequences=0), dict(vocab=0), dict(drafts=1025), dict(vocab=(1 << 29) + 1), dict(sequences=(1 << 20) + 1),
     dict(inv_temperature=0.0), dict(inv_temperature=-1.0), dict(inv_temperature=math.nan), dict(inv_temperature=math.inf),
     dict(target=M + 2), dict(draft=2 * M + 1), dict(tokens=8 * M + 2), dict(workspace=9 * M + 8),
     dict(sequences=1 << 20, drafts=1024, vocab=4096)])

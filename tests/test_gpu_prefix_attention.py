@@ -89,6 +89,12 @@ SHAPES = {
     "batch_64": (90, 1, 12, 2, 64, 700, 700, 9, [(5 * i) % 10 for i in range(90)]),
     "batch_96": (110, 1, 10, 2, 96, 65, 65, 9, [(5 * i) % 10 for i in range(110)]),
     "batch_160": (35, 2, 16, 2, 160, 129, 129, 40, [(5 * i) % 41 for i in range(35)]),
+    "batch_256": (9, 1, 8, 1, 256, 300, 300, 40, [(5 * i) % 41 for i in range(9)]),
+    "packed_64": (90, 1, 12, 2, 64, 10900, 10900, 9, [(5 * i) % 10 for i in range(90)]),
+    "packed_96": (110, 1, 10, 2, 96, 5441, 5441, 9, [(5 * i) % 10 for i in range(110)]),
+    "packed_128": (33, 2, 32, 4, 128, 2701, 2702, 16, [(5 * i) % 17 for i in range(33)]),
+    "packed_160": (35, 2, 16, 2, 160, 2721, 2721, 40, [(5 * i) % 41 for i in range(35)]),
+    "packed_256": (70, 1, 8, 1, 256, 5500, 5600, 64, [(7 * i) % 65 for i in range(70)]),
     "long": (2, 1, 8, 1, 256, 9001, 9001, 5000, [4999, 700]),
 }
 
@@ -185,6 +191,25 @@ def test_rows_of_very_different_scale(rt):
     check("mixed scales", got, exp, bound, P + 8, D)
 
 
+@pytest.mark.parametrize("B,P", [(3, 70), (1, 70), (40, 70), (70, 5500)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_seen_value_that_is_no_number_is_never_lost(rt, B, P, bad):
+    """It may leave NaN in all dims of the rows that see it, and a number only where float64 has the same."""
+    say(f"seen {bad}, batch {B}, prompt {P}")
+    D, cap = 256, 20
+    lengths = [(13 * i) % 20 + 1 for i in range(B)]
+    q, prefix, cache, n = make(3, "f32", B, 1, 8, 1, D, P, P, cap, lengths)
+    prefix.view(f32)[1, P // 3, 7] = bad
+    cache.view(f32).reshape(2, B, cap, D)[1, B - 1, 0, 100] = bad
+    exp, _, bound = ref.attention(q, prefix, P, cache, n, cap, 1, 0.0625, "f32")
+    got, _ = run(rt, "f32", q, prefix, P, cache, n, cap, 1, 0.0625)
+    assert not np.isfinite(got[..., 7]).any() and not np.isfinite(got[B - 1, ..., 100]).any()
+    same = np.isfinite(got)
+    assert np.isfinite(exp[same]).all()
+    got, exp = np.where(same, got, 0), np.where(same, exp, 0)
+    check(f"seen {bad} batch {B}", got, exp, (np.where(np.isfinite(bound[0]), bound[0], 0), bound[1]), P + cap, D)
+
+
 def test_offsets_past_32_bits(rt):
     """The third sequence's rows and the whole V plane lie more than 2^32 bytes into the cache."""
     say("long cache")
@@ -209,8 +234,8 @@ def test_offsets_past_32_bits(rt):
     rt.free(ws)
 
 
-def _program(rt, seed, B, shared_ws=None):
-    T, H, KH, D, P, cap = 2, 8, 1, 256, 600, 64
+def _program(rt, seed, B):
+    T, H, KH, D, P, cap = 2, 8, 1, 256, 2 * B + 600, 64
     q, prefix, cache, n = make(seed, "q8_0", B, T, H, KH, D, P, P, cap, [(i * 11) % 65 for i in range(B)])
     d = {"q": rt.upload(q), "prefix": rt.upload(prefix), "cache": rt.upload(cache), "n": rt.upload(n),
          "out": rt.empty(q.size), "w": rt.empty(B * cap)}
@@ -224,7 +249,7 @@ def _program(rt, seed, B, shared_ws=None):
     return d, call, q, B * cap
 
 
-@pytest.mark.parametrize("B", [2, 40])
+@pytest.mark.parametrize("B", [2, 40, 300])
 def test_graph_replays_equal_the_eager_call(rt, B):
     say(f"graph, batch {B}")
     d, call, q, weights = _program(rt, 31, B)
