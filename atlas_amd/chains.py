@@ -1,6 +1,6 @@
-"""Two more executor chains over the fused ops, beside the Gemma decode step
-(decode.py): the Llama resident decode token and the Gemma layer-major
-prefill chunk.  Each enqueues the path's ops in the reference executor's
+"""Three more chains over the fused ops, beside the Gemma decode step
+(decode.py): the Llama resident decode token, the Gemma layer-major prefill
+chunk, and a batch that decodes drafted tokens behind a shared prompt.  Each enqueues the path's ops in the reference executor's
 order, with seeded stand-in buffers for the GEMM, attention and matvec
 outputs between them (outside this path); per-step inputs (token ids,
 positions, RoPE tables) live in device buffers, so `capture()` records a
@@ -48,6 +48,23 @@ gemma4_executor.rs:3694-4121; chunk size GEMMA4_PREFILL_BATCH_CAPACITY,
   The stand-in GEMM outputs are written into `work` by a scale-by-one pass
   (exact for every finite value), as the GEMM writes it, because the
   residual epilogues normalise `work` in place.
+
+SharedPromptDecode -- no counterpart in the reference, whose executors decode
+one sequence: a batch continues one prompt, each sequence with the same number
+of drafted tokens behind its last one, with caches of a limited size:
+
+    for each layer:
+        QK-RMSNorm + RoPE                 qk_norm_rope
+        V RMSNorm + KV append             kv_append, sequence b at b * capacity
+        attention over prompt and cache   prefix_attention, adding up the
+                                          weights that each own row drew
+    logits soft cap                       softcap
+    drafts accepted, one token drawn      verify_draft
+  and, where the next step could pass a cache's capacity, for each layer
+    the cache cut to its budget           kv_evict, in place
+
+  Rows of rejected drafts stay behind the sequence's new length; the next
+  step's rows and weights (set to zero first) take their place.
 """
 from __future__ import annotations
 
@@ -277,6 +294,167 @@ class GemmaPrefillChunk:
         res = {k: o[k].download() for k in ("state", "ple", "residual", "work")}
         res.update({k: [b.download() for b in o[k]] for k in per_layer})
         res["kv"] = [b.download(self.cache_bytes, np.uint8) for b in o["kv"]]
+        return res
+
+
+@dataclass(frozen=True)
+class SharedPromptShape:
+    """A batch behind a shared prompt at the Gemma-4-E2B-like layer shape."""
+
+    sequences: int = 6
+    drafts: int = 3
+    layers: int = 3
+    q_heads: int = 8
+    head_dim: int = 256
+    prompt: int = 300
+    capacity: int = 48
+    budget: int = 24
+    recent: int = 8
+    vocab: int = 8192
+    eps: float = 1e-6
+    softcap: float = 30.0
+    temperature: float = 0.8
+
+
+class SharedPromptDecode:
+    def __init__(self, rt: HipRuntime, shape: SharedPromptShape = SharedPromptShape(), kv_format: str = "q8_0",
+                 seed: int = 17):
+        self.rt, self.S, self.kv_format = rt, shape, kv_format
+        S = shape
+        B, T, QH, D, V = S.sequences, S.drafts + 1, S.q_heads, S.head_dim, S.vocab
+        r = wl.rng(seed)
+        self.row_bytes = _kv_row_bytes(kv_format, D)
+        self.scale = 1.0 / wl.f32_sqrt(D)
+        self.positions = np.full(B, S.prompt, np.uint32)  # of each sequence's next token
+        self.lengths = np.zeros(B, np.uint32)             # rows of each sequence's cache
+        self.layers = [{"q": wl.normal(r, B * T * QH * D), "k": wl.normal(r, B * T * D), "v": wl.normal(r, B * T * D),
+                        "qw": wl.normal(r, D, 1.0, 0.1), "kw": wl.normal(r, D, 1.0, 0.1),
+                        "prompt_k": wl.normal(r, S.prompt * D), "prompt_v": wl.normal(r, S.prompt * D)}
+                       for _ in range(S.layers)]
+        self.dlayers = [{k: rt.upload(v) for k, v in lay.items()} for lay in self.layers]
+        self.dev = {"slots": rt.empty(B * T, np.uint32), "lengths": rt.empty(B, np.uint32),
+                    "cos": rt.empty(B * T * (D // 2)), "sin": rt.empty(B * T * (D // 2)),
+                    "logits": rt.empty(B * T * V), "draft_logits": rt.empty(max(B * S.drafts * V, 1)),
+                    "draft_tokens": rt.empty(max(B * S.drafts, 1), np.uint32), "accept": rt.empty(max(B * S.drafts, 1)),
+                    "sample": rt.empty(B)}
+        L = range(S.layers)
+        self.cache_bytes = 2 * B * S.capacity * self.row_bytes
+        self.prompt_bytes = 2 * S.prompt * self.row_bytes
+        self.out = {
+            "q_rot": [rt.empty(B * T * QH * D) for _ in L], "k_rot": [rt.empty(B * T * D) for _ in L],
+            "attention": [rt.empty(B * T * QH * D) for _ in L],
+            "kv": [rt.alloc(self.cache_bytes, np.uint8) for _ in L],
+            "prompt": [rt.alloc(self.prompt_bytes, np.uint8) for _ in L],
+            "weights": [rt.empty(B * S.capacity) for _ in L], "kept": [rt.empty(B * S.budget, np.uint32) for _ in L],
+            "cut_lengths": [rt.empty(B, np.uint32) for _ in L],
+            "capped": rt.empty(B * T * V), "accepted": rt.empty(B, np.uint32), "tokens": rt.empty(B * T, np.uint32),
+        }
+        # one workspace: the stream orders the calls that use it
+        self.attention_bytes = rt.prefix_attention_workspace(kv_format, B, T, QH, 1, D, S.prompt, S.capacity, True)
+        self.verify_bytes = rt.verify_draft_workspace(B, S.drafts, V)
+        self.workspace = rt.alloc(max(self.attention_bytes, self.verify_bytes))
+        slots = rt.upload(np.arange(S.prompt, dtype=np.uint32))
+        for layer, lay in enumerate(self.dlayers):
+            rt.memset(self.out["kv"][layer], 0, self.cache_bytes)
+            rt.memset(self.out["weights"][layer], 0, 4 * B * S.capacity)
+            rt.kv_append(kv_format, lay["prompt_k"], lay["prompt_v"], self.out["prompt"][layer], D, S.prompt, slots,
+                         S.prompt, True, S.eps)
+        rt.sync()
+        rt.free(slots)
+        self.graph = None
+
+    def set_step(self, draft_tokens, logits, draft_logits, accept, sample) -> None:
+        """The step's drafts [B, drafts], the logits that verify them [B, drafts + 1, vocab] and proposed them [B,
+        drafts, vocab], and the random numbers [B, drafts] and [B]."""
+        S, d = self.S, self.dev
+        B, T, D = S.sequences, S.drafts + 1, S.head_dim
+        if int(self.lengths.max()) + T > S.capacity:
+            raise ValueError("a cache has no room for the step: cut() first")
+        ahead = np.arange(T, dtype=np.uint32)
+        slots = (np.arange(B, dtype=np.uint32) * S.capacity + self.lengths)[:, None] + ahead
+        d["slots"].upload(slots.astype(np.uint32))
+        d["lengths"].upload((self.lengths + T).astype(np.uint32))
+        c, s = rope_tables_gemma4((self.positions[:, None] + ahead).reshape(-1).astype(np.uint32), D // 2, D, 1e4)
+        d["cos"].upload(c)
+        d["sin"].upload(s)
+        d["logits"].upload(logits)
+        d["sample"].upload(sample)
+        if S.drafts:
+            d["draft_tokens"].upload(draft_tokens)
+            d["draft_logits"].upload(draft_logits)
+            d["accept"].upload(accept)
+        zeros = np.zeros(T, np.float32)
+        for w in self.out["weights"]:
+            for b in range(B):
+                w.offset(4 * int(slots[b, 0])).upload(zeros)
+
+    def enqueue(self) -> None:
+        rt, S, d, o = self.rt, self.S, self.dev, self.out
+        B, T, QH, D = S.sequences, S.drafts + 1, S.q_heads, S.head_dim
+        for layer, lay in enumerate(self.dlayers):
+            rt.qk_norm_rope(lay["q"], lay["k"], lay["qw"], lay["kw"], d["cos"], d["sin"], o["q_rot"][layer],
+                            o["k_rot"][layer], B * T, QH, 1, D, D // 2, S.eps)
+            rt.kv_append(self.kv_format, o["k_rot"][layer], lay["v"], o["kv"][layer], D, B * S.capacity, d["slots"], B * T,
+                         True, S.eps)
+            w = o["weights"][layer]
+            rt.prefix_attention(self.kv_format, o["q_rot"][layer], o["prompt"][layer], S.prompt, S.prompt, o["kv"][layer],
+                                d["lengths"], S.capacity, o["attention"][layer], w, w, B, T, QH, 1, D, self.scale,
+                                self.workspace, self.attention_bytes)
+        rt.softcap(d["logits"], o["capped"], B * T * S.vocab, S.softcap)
+        some = S.drafts > 0
+        rt.verify_draft(o["capped"], d["draft_logits"] if some else None, d["draft_tokens"] if some else None, None,
+                        d["accept"] if some else None, d["sample"], o["accepted"], o["tokens"], B, S.drafts, S.vocab,
+                        1.0 / S.temperature, self.workspace, self.verify_bytes)
+
+    def advance(self) -> tuple[np.ndarray, np.ndarray]:
+        """(accepted, tokens) of the step that ran; the sequences grow by them."""
+        S = self.S
+        accepted = self.out["accepted"].download(S.sequences, np.uint32)
+        tokens = self.out["tokens"].download(S.sequences * (S.drafts + 1), np.uint32).reshape(S.sequences, -1)
+        # the rows of the last token and of the accepted drafts; the drawn token's comes with the next step
+        self.lengths = self.lengths + accepted + 1
+        self.positions = self.positions + accepted + 1
+        return accepted, tokens
+
+    @property
+    def full(self) -> bool:
+        return int(self.lengths.max()) + self.S.drafts + 1 > self.S.capacity
+
+    def cut(self) -> None:
+        """Every cache cut to the budget, by the weights of its own layer."""
+        S, o = self.S, self.out
+        self.dev["lengths"].upload(self.lengths.astype(np.uint32))
+        for layer in range(S.layers):
+            w = o["weights"][layer]
+            self.rt.kv_evict(self.kv_format, o["kv"][layer], o["kv"][layer], w, w, self.dev["lengths"],
+                             o["cut_lengths"][layer], o["kept"][layer], S.sequences, S.capacity, S.head_dim, S.budget, S.recent)
+        self.rt.sync()
+        self.lengths = o["cut_lengths"][0].download(S.sequences, np.uint32)
+
+    def capture(self) -> int:
+        if self.graph is not None:
+            self.rt.graph_destroy(self.graph)
+        self.rt.graph_begin()
+        try:
+            self.enqueue()
+        finally:
+            graph = self.rt.graph_end()
+        self.graph = graph
+        return graph
+
+    def replay(self) -> None:
+        self.rt.graph_launch(self.graph)
+
+    def close(self) -> None:
+        if self.graph is not None:
+            self.rt.graph_destroy(self.graph)
+            self.graph = None
+
+    def results(self) -> dict:
+        o = self.out
+        res = {k: [b.download() for b in o[k]] for k in ("q_rot", "k_rot", "attention", "weights")}
+        res["kv"] = [b.download(self.cache_bytes, np.uint8) for b in o["kv"]]
+        res["capped"], res["accepted"], res["tokens"] = (o[k].download() for k in ("capped", "accepted", "tokens"))
         return res
 
 

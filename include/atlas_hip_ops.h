@@ -409,7 +409,8 @@ int atlas_hip_kv_append_q4_0(atlas_hip_ctx *ctx, const float *key, const float *
  *
  * weights_out (NULL: none; [sequences, capacity]) is weights_in (NULL: zeros;
  * may be the same buffer) plus the attention that own row j got, summed over
- * tokens and heads; rows from len_b on are left untouched.
+ * tokens and heads; rows from len_b on are left untouched (weights added up
+ * over steps start at zero: a caller clears a row's when it appends the row).
  *
  * head_dim is at most 256 and a multiple of 4 (f32) or 32 (Q8_0, Q4_0);
  * kv_heads divides q_heads; q, output, f32 caches and the workspace are
