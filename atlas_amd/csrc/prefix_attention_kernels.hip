@@ -40,7 +40,7 @@ __device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const floa
         }
 }
 
-// One workgroup: 16 * NR query rows of one KV head against one segment of a
+// One workgroup: 16 query rows of one KV head against one segment of a
 // sequence's own rows (or of the prompt, for batches of up to 16 rows).  Its
 // bytes bound it: the wavefronts take its keys 16 at a time in turn, straight
 // from the cache into the operands' registers, with the next 16 loading while
@@ -48,11 +48,13 @@ __device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const floa
 // leaves lane l with query row l % 16 and keys 4 (l / 16) + r, which is the
 // operand that O^T = V^T P^T wants, so P never leaves its registers and a
 // row's statistics are the lane's own.  Queries wait in LDS.
-template <int FMT, int NB, int NR>
-__global__ __launch_bounds__(kAttnThreads, NB < 8 ? 2 : 1) void attn_rows_kernel(AttnParams a) {
+template <int FMT, int NB>
+__global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel(AttnParams a) {
     constexpr int NG = (NB + 1) / 2;  // groups of 64 dims
-    constexpr int kRoom = NR * NB * 2 > 2 * (NG * 4 + 1) ? NR * NB * 2 : 2 * (NG * 4 + 1);
-    // queries [row tile][step][half]; at the end two wavefronts' sums
+    constexpr int kSums = NG * 4 + 1;
+    constexpr int kRoom = kAttnWaves * kSums;
+    static_assert(kRoom >= NB * 2, "the queries fit");
+    // queries [step][half]; at the end the wavefronts' sums
     __shared__ f32x4 room[kRoom][kWave];
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
@@ -68,7 +70,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 2 : 1) void attn_rows_kernel
         item /= a.prefix_tiles;
         slot = item % a.prefix_slots;
         kv_head = __builtin_amdgcn_readfirstlane(item / a.prefix_slots);
-        row0 = tile * 16 * NR;
+        row0 = tile * 16;
         row_end = a.rows;
         const uint32_t part = ((a.prefix_length + a.prefix_slots - 1) / a.prefix_slots + 63) / 64 * 64;
         key_begin = min(slot * part, a.prefix_length);
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 2 : 1) void attn_rows_kernel
         kv_head = __builtin_amdgcn_readfirstlane(item % a.kv_heads);
         seq = __builtin_amdgcn_readfirstlane(item / a.kv_heads);
         slot = a.prefix_slots + part_index;
-        row0 = seq * a.seq_rows + tile * 16 * NR;
+        row0 = seq * a.seq_rows + tile * 16;
         row_end = (seq + 1) * a.seq_rows;
         length = min(a.lengths[seq], a.capacity);
         const uint32_t part = ((length + a.own_slots - 1) / a.own_slots + 63) / 64 * 64;
@@ -97,59 +99,63 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 2 : 1) void attn_rows_kernel
     key_begin = __builtin_amdgcn_readfirstlane(key_begin);
     key_end = __builtin_amdgcn_readfirstlane(key_end);
     row0 = __builtin_amdgcn_readfirstlane(row0);
+    const uint64_t line0 = (static_cast<uint64_t>(slot) * a.kv_heads + kv_head) * a.rows;
+    if (key_begin >= key_end) {
+        // an empty segment: the join takes no more of it than its maximum
+        const uint32_t i = row0 + threadIdx.x;
+        if (threadIdx.x < 16 && i < row_end) a.partial_ml[line0 + i] = make_float2(neg_inf(), 0.0f);
+        return;
+    }
     const uint32_t head_off = static_cast<uint32_t>(head_offset<FMT>(kv_head, a.head_dim));
     keys += head_off;
     values += head_off;
 
-    for (uint32_t i = wave; i < NR * NB; i += kAttnWaves) {
-        const uint32_t at = min(row0 + 16 * (i / NB) + n, row_end - 1);
+    for (uint32_t i = wave; i < NB; i += kAttnWaves) {
+        const uint32_t at = min(row0 + n, row_end - 1);
         float x[8];
         load_query8<FMT>(a.q + (static_cast<uint64_t>(at / a.group) * a.q_heads + kv_head * a.group + at % a.group) * a.head_dim,
-                         4 * (i % NB) + quarter, a.head_dim, a.scale, x);
+                         4 * i + quarter, a.head_dim, a.scale, x);
         room[2 * i][lane] = f32x4{x[0], x[1], x[2], x[3]};
         room[2 * i + 1][lane] = f32x4{x[4], x[5], x[6], x[7]};
     }
-    uint32_t seen[NR];  // keys below it are seen by the lane's row
-    float m[NR], l[NR];
-    f32x4 out[NR][NG * 4];
-#pragma unroll
-    for (int t = 0; t < NR; ++t) {
-        const uint32_t row = row0 + 16 * t + n;
-        seen[t] = key_end;
-        if (!shared) {
-            const uint32_t behind = a.tokens - 1 - (min(row, row_end - 1) - seq * a.seq_rows) / a.group;
-            seen[t] = min(length > behind ? length - behind : 0u, key_end);
-        }
-        if (row >= row_end) seen[t] = 0;
-        m[t] = neg_inf();
-        l[t] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NG * 4; ++i) out[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t seen = key_end;  // keys below it are seen by the lane's row
+    const uint32_t row = row0 + n;
+    if (!shared) {
+        const uint32_t behind = a.tokens - 1 - (min(row, row_end - 1) - seq * a.seq_rows) / a.group;
+        seen = min(length > behind ? length - behind : 0u, key_end);
     }
-    uint32_t key_off[NB][2], value_off[NG];
+    if (row >= row_end) seen = 0;
+    float m = neg_inf(), l = 0.0f;
+    f32x4 out[NG * 4];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) key_off[b][p] = RawKey<FMT>::offset(4 * b + quarter, a.head_dim, p);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) value_off[g] = RawValue<FMT>::offset(16 * g + n, a.head_dim);
+    for (int i = 0; i < NG * 4; ++i) out[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     RawKey<FMT> k[NB];
     RawValue<FMT> raw_v[4][NG];
     const auto rows_of = [&](const uint8_t* plane, uint32_t first) {
         const uint32_t there = first < key_end ? min(key_end - first, 16u) : 0u;
         return TileRows<FMT>(plane, there ? first : key_end - 1, there, a.row_bytes, head_off);
     };
+    // offsets are found anew for every tile: kept, they send other numbers to memory
     const auto load_k = [&](uint32_t first) {
         const TileRows<FMT> rows = rows_of(keys, first);
+        uint32_t unit = quarter;
+        asm volatile("" : "+v"(unit));
 #pragma unroll
-        for (int b = 0; b < NB; ++b) k[b].load(rows, n, 4 * b + quarter, key_off[b]);
+        for (int b = 0; b < NB; ++b) {
+            const uint32_t off[2] = {RawKey<FMT>::offset(4 * b + unit, a.head_dim, 0), RawKey<FMT>::offset(4 * b + unit, a.head_dim, 1)};
+            k[b].load(rows, n, 4 * b + unit, off);
+        }
     };
     const auto load_v = [&](uint32_t first) {
         const TileRows<FMT> rows = rows_of(values, first);
+        uint32_t quad = n;
+        asm volatile("" : "+v"(quad));
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int g = 0; g < NG; ++g) {
+            const uint32_t off = RawValue<FMT>::offset(16 * g + quad, a.head_dim);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) raw_v[r][g].load(rows, 4 * quarter + r, 16 * g + n, value_off[g]);
+            for (int r = 0; r < 4; ++r) raw_v[r][g].load(rows, 4 * quarter + r, 16 * g + quad, off);
+        }
     };
     const uint32_t first = key_begin + wave * 16;
     if (first < key_end) {
@@ -159,21 +165,16 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 2 : 1) void attn_rows_kernel
     __syncthreads();
 
     for (uint32_t key0 = first; key0 < key_end; key0 += kAttnWaves * 16) {
-        f32x4 s[NR][2];
-#pragma unroll
-        for (int t = 0; t < NR; ++t) s[t][0] = s[t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 s[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float x[8];
             raw_values(k[b], x);
+            const f32x4 q0 = room[2 * b][lane], q1 = room[2 * b + 1][lane];
 #pragma unroll
-            for (int t = 0; t < NR; ++t) {
-                const f32x4 q0 = room[2 * (t * NB + b)][lane], q1 = room[2 * (t * NB + b) + 1][lane];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[t][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], q0[j], s[t][0], 0, 0, 0);
-                    s[t][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[4 + j], q1[j], s[t][1], 0, 0, 0);
-                }
+            for (int j = 0; j < 4; ++j) {
+                s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], q0[j], s[0], 0, 0, 0);
+                s[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[4 + j], q1[j], s[1], 0, 0, 0);
             }
             // or every query read is moved up here and the loads in flight to memory
             if (b % 2) __builtin_amdgcn_sched_barrier(0);
@@ -202,87 +203,81 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 2 : 1) void attn_rows_kernel
                 for (int i = 0; i < NG * 4; ++i) any = __builtin_fmaf(v[r][i], 0.0f, any);
             stained = __builtin_amdgcn_ballot_w64(any != 0.0f) != 0;
         }
+        float p[4];
+        float top = neg_inf();
 #pragma unroll
-        for (int t = 0; t < NR; ++t) {
-            float p[4];
-            float top = neg_inf();
+        for (int r = 0; r < 4; ++r) {
+            p[r] = key0 + 4 * quarter + r < seen ? s[0][r] + s[1][r] : neg_inf();
+            top = fmaxf(top, p[r]);
+        }
+        if (!shared && a.scores && row < row_end && key0 + 4 * quarter < key_end) {
+            const uint64_t line = (static_cast<uint64_t>(seq) * a.kv_heads + kv_head) * a.seq_rows + row - seq * a.seq_rows;
+            *reinterpret_cast<f32x4*>(a.scores + line * a.score_pitch + key0 + 4 * quarter) = f32x4{p[0], p[1], p[2], p[3]};
+        }
+        top = max_xor32(max_xor16(top));
+        if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+            const float m_new = fmaxf(m, top);
+            const float fade = m == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+            m = m_new;
+            l *= fade;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                p[r] = key0 + 4 * quarter + r < seen[t] ? s[t][0][r] + s[t][1][r] : neg_inf();
-                top = fmaxf(top, p[r]);
-            }
-            if (!shared && a.scores) {
-                const uint32_t row = row0 + 16 * t + n;
-                if (row < row_end && key0 + 4 * quarter < key_end) {
-                    const uint64_t line = (static_cast<uint64_t>(seq) * a.kv_heads + kv_head) * a.seq_rows + row - seq * a.seq_rows;
-                    *reinterpret_cast<f32x4*>(a.scores + line * a.score_pitch + key0 + 4 * quarter) = f32x4{p[0], p[1], p[2], p[3]};
-                }
-            }
-            top = max_xor32(max_xor16(top));
-            if (__builtin_amdgcn_ballot_w64(top > m[t]) != 0) {
-                const float m_new = fmaxf(m[t], top);
-                const float fade = m[t] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m[t] - m_new);
-                m[t] = m_new;
-                l[t] *= fade;
+            for (int i = 0; i < NG * 4; ++i) out[i] *= fade;
+        }
+        const float base = m == neg_inf() ? 0.0f : m;
 #pragma unroll
-                for (int i = 0; i < NG * 4; ++i) out[t][i] *= fade;
-            }
-            const float base = m[t] == neg_inf() ? 0.0f : m[t];
+        for (int r = 0; r < 4; ++r) {
+            p[r] = __builtin_amdgcn_exp2f(p[r] - base);
+            l += p[r];
+        }
+        if (stained) {
+            add_seen<NG>(v, p, key0, seen, out);
+        } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                p[r] = __builtin_amdgcn_exp2f(p[r] - base);
-                l[t] += p[r];
-            }
-            if (stained) {
-                add_seen<NG>(v, p, key0, seen[t], out[t]);
-            } else {
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int i = 0; i < NG * 4; ++i)
-                        out[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i], p[r], out[t][i], 0, 0, 0);
-            }
+                for (int i = 0; i < NG * 4; ++i)
+                    out[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i], p[r], out[i], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         load_v(next);
     }
 
-    // join the wavefronts, two to two and one to one
+    // join the wavefronts: each takes a part of the dims
+    l = sum_xor32(sum_xor16(l));
+    __syncthreads();
+    f32x4(*mine)[kWave] = room + wave * kSums;
+    mine[NG * 4][lane] = f32x4{m, l, 0.0f, 0.0f};
 #pragma unroll
-    for (int t = 0; t < NR; ++t) {
-        l[t] = sum_xor32(sum_xor16(l[t]));
+    for (int i = 0; i < NG * 4; ++i) mine[i][lane] = out[i];
+    __syncthreads();
+    float top = neg_inf(), sum = 0.0f, f[kAttnWaves];
 #pragma unroll
-        for (uint32_t half = kAttnWaves / 2; half > 0; half /= 2) {
-            __syncthreads();
-            f32x4(*mine)[kWave] = room + (wave % half) * (NG * 4 + 1);
-            if (wave >= half && wave < 2 * half) {
-                mine[NG * 4][lane] = f32x4{m[t], l[t], 0.0f, 0.0f};
+    for (int w = 0; w < kAttnWaves; ++w) {
+        f[w] = room[w * kSums + NG * 4][lane].x;
+        top = fmaxf(top, f[w]);
+    }
 #pragma unroll
-                for (int i = 0; i < NG * 4; ++i) mine[i][lane] = out[t][i];
-            }
-            __syncthreads();
-            if (wave < half) {
-                const float m2 = mine[NG * 4][lane].x, l2 = mine[NG * 4][lane].y;
-                const float both = fmaxf(m[t], m2);
-                const float f1 = m[t] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m[t] - both);
-                const float f2 = m2 == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m2 - both);
-                m[t] = both;
-                l[t] = l[t] * f1 + l2 * f2;
+    for (int w = 0; w < kAttnWaves; ++w) {
+        f[w] = f[w] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(f[w] - top);
+        sum += f[w] * room[w * kSums + NG * 4][lane].y;
+    }
+    const uint64_t at = line0 + row;
+    if (wave == 0 && quarter == 0 && row < row_end) a.partial_ml[at] = make_float2(top, sum);
+    // group g of 64 dims, NG of the four quads that a lane has of it
+    const uint32_t g = wave % NG, quad0 = wave / NG * NG;
+    f32x4 o[4];
 #pragma unroll
-                for (int i = 0; i < NG * 4; ++i) out[t][i] = out[t][i] * f1 + mine[i][lane] * f2;
-            }
-        }
-        const uint32_t row = row0 + 16 * t + n;
-        if (wave == 0 && row < row_end) {
-            const uint64_t at = (static_cast<uint64_t>(slot) * a.kv_heads + kv_head) * a.rows + row;
-            if (quarter == 0) a.partial_ml[at] = make_float2(m[t], l[t]);
+    for (int j = 0; j < 4; ++j) {
+        o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int g = 0; g < NG; ++g)
+        for (int w = 0; w < kAttnWaves; ++w) o[j] += f[w] * room[w * kSums + 4 * g + j][lane];
+    }
+    if (row < row_end) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    store_quad<FMT>(a.partial_out + at * a.head_dim, 16 * g + 4 * quarter + i, a.head_dim,
-                                    f32x4{out[t][4 * g][i], out[t][4 * g + 1][i], out[t][4 * g + 2][i], out[t][4 * g + 3][i]});
-        }
+        for (int i = 0; i < 4; ++i)
+            if (i >= quad0 && i < quad0 + NG)
+                store_quad<FMT>(a.partial_out + at * a.head_dim, 16 * g + 4 * quarter + i, a.head_dim,
+                                f32x4{o[0][i], o[1][i], o[2][i], o[3][i]});
     }
 }
 
@@ -319,8 +314,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, f
         const f32x4 part = *reinterpret_cast<const f32x4*>(parts + s * all * a.head_dim);
         const float f = __builtin_amdgcn_exp2f(x.x - base);
         sum += f * x.y;
+        // an empty segment has left what was there
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] += f * part[j];
+        for (int j = 0; j < 4; ++j) o[j] += x.x == neg_inf() ? 0.0f : f * part[j];
     }
     sums[group][lane] = o;
     if (lane == 0) group_l[group] = sum;
@@ -381,7 +377,6 @@ __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a
 
 // How the work is laid out, and what of the workspace it takes.
 struct AttnPlan {
-    uint32_t row_tiles;  // of 16 rows a workgroup
     bool wide;           // the prompt goes by f16 pieces, not with the own rows
     uint32_t prefix_tiles, prefix_slots, own_tiles, own_slots;
     uint64_t out_bytes, ml_bytes, score_bytes, log_bytes, packed_bytes;
@@ -395,13 +390,12 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     AttnPlan p{};
     const uint32_t seq_rows = s.tokens * (s.q_heads / s.kv_heads);
     const uint64_t rows = static_cast<uint64_t>(s.sequences) * seq_rows;
-    p.row_tiles = seq_rows > 16 ? 2 : 1;
-    const uint32_t step = 16 * p.row_tiles;
-    // Workgroups of a launch: more parts cost their starts and their joins, fewer
-    // leave CUs idle.  256 x 512 own rows, 64 x 8192, 24 x 1024 with 5 drafts, us:
-    //   128  38 / 215 / 38    256  38 / 158 / 35    512  44 / 152 / 40
-    //   1024  59 / 152 / 49   2048  88 / 168 / 63
-    const uint32_t wanted = 512;
+    // Workgroups that the chip holds: one to a CU above 128 dims, three below.
+    // More parts cost their starts and their joins, fewer leave CUs idle.  Own
+    // rows of 256 x 512, 64 x 8192 (256 dims), 24 x 1024 with 5 drafts (128), us:
+    //   256  40 / 147 / 34    512  47 / 143 / 31    768  51 / 148 / 28
+    //   1024  61 / 143 / 30
+    const uint32_t wanted = s.head_dim > 128 ? 256 : 768;
     if (s.prefix_length && rows > 16) {
         p.wide = true;
         const uint32_t pad = s.head_dim <= 64 ? 64 : (s.head_dim <= 128 ? 128 : 256);
@@ -428,7 +422,7 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         if (want > 8) want = want / 8 * 8;
         p.prefix_slots = static_cast<uint32_t>(want);
     } else if (s.prefix_length) {
-        p.prefix_tiles = static_cast<uint32_t>((rows + step - 1) / step);
+        p.prefix_tiles = static_cast<uint32_t>((rows + 15) / 16);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         const uint32_t most = (s.prefix_length + 63) / 64;
         const uint64_t want = (wanted + units - 1) / units;
@@ -436,7 +430,7 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         if (p.prefix_slots > 64) p.prefix_slots = 64;
     }
     if (s.capacity) {
-        p.own_tiles = (seq_rows + step - 1) / step;
+        p.own_tiles = (seq_rows + 15) / 16;
         const uint64_t units = static_cast<uint64_t>(p.own_tiles) * s.kv_heads * s.sequences;
         const uint32_t most = (s.capacity + 63) / 64;
         const uint64_t want = (wanted + units - 1) / units;
@@ -454,27 +448,19 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     return p;
 }
 
-template <int FMT, int NB, int NR>
-void launch_rows(hipStream_t stream, uint32_t items, const AttnParams& a) {
-    hipLaunchKernelGGL((attn_rows_kernel<FMT, NB, NR>), dim3(items), dim3(kAttnThreads), 0, stream, a);
-}
-
 template <int FMT, int NB>
-void launch_rows(hipStream_t stream, uint32_t items, uint32_t row_tiles, const AttnParams& a) {
-    if (row_tiles == 1)
-        launch_rows<FMT, NB, 1>(stream, items, a);
-    else
-        launch_rows<FMT, NB, 2>(stream, items, a);
+void launch_rows(hipStream_t stream, uint32_t items, const AttnParams& a) {
+    hipLaunchKernelGGL((attn_rows_kernel<FMT, NB>), dim3(items), dim3(kAttnThreads), 0, stream, a);
 }
 
 template <int FMT>
-void launch_rows(hipStream_t stream, uint32_t items, uint32_t row_tiles, const AttnParams& a) {
+void launch_rows(hipStream_t stream, uint32_t items, const AttnParams& a) {
     if (a.head_dim <= 64)
-        launch_rows<FMT, 2>(stream, items, row_tiles, a);
+        launch_rows<FMT, 2>(stream, items, a);
     else if (a.head_dim <= 128)
-        launch_rows<FMT, 4>(stream, items, row_tiles, a);
+        launch_rows<FMT, 4>(stream, items, a);
     else
-        launch_rows<FMT, 8>(stream, items, row_tiles, a);
+        launch_rows<FMT, 8>(stream, items, a);
 }
 
 }  // namespace
@@ -520,11 +506,11 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
     if (p.wide && (e = launch_attn_wide(stream, s.format, prefix_items, a, packed)) != hipSuccess) return e;
     if (items) {
         if (s.format == kKvF32)
-            launch_rows<kKvF32>(stream, items, p.row_tiles, a);
+            launch_rows<kKvF32>(stream, items, a);
         else if (s.format == kKvQ8_0)
-            launch_rows<kKvQ8_0>(stream, items, p.row_tiles, a);
+            launch_rows<kKvQ8_0>(stream, items, a);
         else
-            launch_rows<kKvQ4_0>(stream, items, p.row_tiles, a);
+            launch_rows<kKvQ4_0>(stream, items, a);
         if ((e = hipGetLastError()) != hipSuccess) return e;
     }
     const uint64_t all = static_cast<uint64_t>(a.rows) * a.kv_heads;

@@ -484,7 +484,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_wide_kernel(AttnParams a
 #pragma unroll
         for (int b = 0; b < W::KT / 32; ++b) rows.add(tile, b, scores[2 * b], scores[2 * b + 1], left, lane);
     }
-    rows.finish(a, item, row, quarter);
+    // the row anew: kept through the loop, its registers were those that spilled
+    uint32_t id = threadIdx.x;
+    asm volatile("" : "+v"(id));
+    rows.finish(a, item, row0 + id % 16, id % kWave / 16);
 }
 
 // The prompt's tiles converted once, for batches whose rows would have every
