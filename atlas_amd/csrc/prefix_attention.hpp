@@ -252,6 +252,14 @@ __device__ __forceinline__ void store_quad(float* row, uint32_t q, uint32_t head
     }
 }
 
+// Part `i` of `parts` of `rows` rows, in whole units of `unit`: no two parts
+// differ by more than one (slots is at most 2^9 or so, units below 2^29).
+__device__ __forceinline__ void part_of(uint32_t rows, uint32_t unit, uint32_t i, uint32_t parts, uint32_t& begin, uint32_t& end) {
+    const uint32_t units = (rows + unit - 1) / unit, each = units / parts, more = units % parts;
+    begin = min((i * each + min(i, more)) * unit, rows);
+    end = min(begin + (each + (i < more ? 1u : 0u)) * unit, rows);
+}
+
 struct AttnParams {
     const float* q;
     const uint8_t* prefix;       // K plane; V plane prefix_plane bytes on

@@ -72,9 +72,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
         kv_head = __builtin_amdgcn_readfirstlane(item / a.prefix_slots);
         row0 = tile * 16;
         row_end = a.rows;
-        const uint32_t part = ((a.prefix_length + a.prefix_slots - 1) / a.prefix_slots + 63) / 64 * 64;
-        key_begin = min(slot * part, a.prefix_length);
-        key_end = min(key_begin + part, a.prefix_length);
+        part_of(a.prefix_length, 64, slot, a.prefix_slots, key_begin, key_end);
         keys = a.prefix;
         values = a.prefix + a.prefix_plane;
     } else {
@@ -89,9 +87,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
         row0 = seq * a.seq_rows + tile * 16;
         row_end = (seq + 1) * a.seq_rows;
         length = min(a.lengths[seq], a.capacity);
-        const uint32_t part = ((length + a.own_slots - 1) / a.own_slots + 63) / 64 * 64;
-        key_begin = min(part_index * part, length);
-        key_end = min(key_begin + part, length);
+        part_of(length, 64, part_index, a.own_slots, key_begin, key_end);
         const uint64_t base = static_cast<uint64_t>(seq) * a.capacity * a.row_bytes;
         keys = a.cache + base;
         values = a.cache + a.cache_plane + base;

@@ -321,9 +321,7 @@ struct WideItem {
         slot = __builtin_amdgcn_readfirstlane(slot);
         tile = __builtin_amdgcn_readfirstlane(tile);
         kv_head = __builtin_amdgcn_readfirstlane(kv_head);
-        const uint32_t part = ((a.prefix_length + a.prefix_slots - 1) / a.prefix_slots + kt - 1) / kt * kt;
-        begin = min(slot * part, a.prefix_length);
-        end = min(begin + part, a.prefix_length);
+        part_of(a.prefix_length, kt, slot, a.prefix_slots, begin, end);
     }
 };
 
