@@ -411,9 +411,7 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         if (packed) p.packed_bytes = round256(packed_bytes);
         p.prefix_tiles = static_cast<uint32_t>(packed ? (rows + 127) / 128 : row_tiles);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
-        // two workgroups to a CU, or one of eight wavefronts
-        const uint64_t whole = packed ? 256 : 512;
-        uint64_t want = units >= whole ? 1 : whole / units;
+        uint64_t want = units >= 256 ? 1 : 256 / units;  // one workgroup to a CU
         if (want > most) want = most;
         if (want > 8) want = want / 8 * 8;
         p.prefix_slots = static_cast<uint32_t>(want);

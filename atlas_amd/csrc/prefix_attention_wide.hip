@@ -430,62 +430,72 @@ struct WideRows {
     }
 };
 
+// Eight wavefronts: four convert a tile while the other four, 16 rows each,
+// multiply the one before it, so that the vector units and the matrix units of
+// every SIMD have a wavefront of their own.  One barrier a tile: behind it the
+// converted tile is there and the buffer of the one before is free.
+constexpr int kWideThreads = 512;
+
 template <int FMT, int D>
-__global__ __launch_bounds__(kAttnThreads, 2) void attn_wide_kernel(AttnParams a) {
+__global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a) {
     using W = Wide<D>;
-    __shared__ WideTile<D> tile;
+    __shared__ WideTile<D> buffers[2];
     const uint32_t lane = threadIdx.x % kWave, n = lane % 16, quarter = lane / 16;
     const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
     const WideItem item(a, W::KT);
-    const uint32_t head_off = static_cast<uint32_t>(head_offset<FMT>(item.kv_head, a.head_dim));
-    const uint8_t* keys = a.prefix + head_off;
-    const uint8_t* values = a.prefix + a.prefix_plane + head_off;
-    const uint32_t row0 = item.tile * 64 + wave * 16, row = row0 + n, end = item.end;
-    const bool busy = row0 < a.rows;  // the wavefront has rows
-    WideRows<FMT, D> rows(a, item.kv_head, row, quarter);
-    const WideLane<FMT, D> mine(lane, wave, a.head_dim);
-    RawKeys<FMT, D> raw_keys;
-    RawValues<FMT> raw_values;
-
-    // Two barriers a tile: the first stands between its keys' conversion and
-    // their use (and between the last tile's values' use and this one's
-    // conversion), the second likewise for its values.  Rows are loaded a whole
-    // tile ahead, or half a one where they would not fit the registers.
-    const auto rows_of = [&](const uint8_t* plane, uint32_t first) {
-        const uint32_t there = first < end ? min(end - first, static_cast<uint32_t>(W::KT)) : 0u;
-        return TileRows<FMT>(plane, there ? first : end - 1, there, a.row_bytes, head_off);
-    };
-    constexpr bool kAhead = FMT != kKvF32 || D < 256;
-    load_keys(raw_keys, mine, rows_of(keys, item.begin));
-    if (kAhead) load_values(raw_values, mine, rows_of(values, item.begin));
-    for (uint32_t first = item.begin; first < end; first += W::KT) {
-        const uint32_t left = end - first;
-        convert_keys(raw_keys, tile, lane, wave);
-        if (kAhead)
-            load_keys(raw_keys, mine, rows_of(keys, first + W::KT));
-        else
-            load_values(raw_values, mine, rows_of(values, first));
-        __syncthreads();
-        f32x4 scores[W::KT / 16];
-        if (busy) {
+    const uint32_t end = item.end;
+    uint32_t buffer = 0;
+    if (wave >= 4) {
+        const uint32_t head_off = static_cast<uint32_t>(head_offset<FMT>(item.kv_head, a.head_dim));
+        const uint8_t* keys = a.prefix + head_off;
+        const uint8_t* values = a.prefix + a.prefix_plane + head_off;
+        const WideLane<FMT, D> mine(lane, wave - 4, a.head_dim);
+        const auto rows_of = [&](const uint8_t* plane, uint32_t first) {
+            const uint32_t there = first < end ? min(end - first, static_cast<uint32_t>(W::KT)) : 0u;
+            return TileRows<FMT>(plane, there ? first : end - 1, there, a.row_bytes, head_off);
+        };
+        // a tile of f32 rows is enough in flight, of quantised ones two are
+        constexpr int kAhead = FMT == kKvF32 ? 1 : 2;
+        RawKeys<FMT, D> raw_keys[kAhead];
+        RawValues<FMT> raw_values[kAhead];
+        uint32_t first = item.begin;
+        if (first < end) {
 #pragma unroll
-            for (int t = 0; t < W::KT / 16; t += 2)
-                score_pair<D>(tile, t, lane, rows.q_hi, rows.q_lo, rows.q_exp, scores[t], scores[t + 1]);
+            for (int i = 0; i < kAhead; ++i) {
+                load_keys(raw_keys[i], mine, rows_of(keys, first + i * W::KT));
+                load_values(raw_values[i], mine, rows_of(values, first + i * W::KT));
+            }
         }
-        convert_values(raw_values, tile, lane, wave);
-        if (kAhead)
-            load_values(raw_values, mine, rows_of(values, first + W::KT));
-        else
-            load_keys(raw_keys, mine, rows_of(keys, first + W::KT));
+        while (first < end) {
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (first >= end) break;
+                convert_keys(raw_keys[i], buffers[buffer], lane, wave - 4);
+                load_keys(raw_keys[i], mine, rows_of(keys, first + kAhead * W::KT));
+                convert_values(raw_values[i], buffers[buffer], lane, wave - 4);
+                load_values(raw_values[i], mine, rows_of(values, first + kAhead * W::KT));
+                __syncthreads();
+                first += W::KT;
+                buffer ^= 1;
+            }
+        }
+        return;
+    }
+    const uint32_t row0 = item.tile * 64 + wave * 16;
+    const bool busy = row0 < a.rows;  // the wavefront has rows
+    WideRows<FMT, D> rows(a, item.kv_head, row0 + n, quarter);
+    for (uint32_t first = item.begin; first < end; first += W::KT, buffer ^= 1) {
         __syncthreads();
         if (!busy) continue;
+        const WideTile<D>& tile = buffers[buffer];
+        f32x4 scores[W::KT / 16];
 #pragma unroll
-        for (int b = 0; b < W::KT / 32; ++b) rows.add(tile, b, scores[2 * b], scores[2 * b + 1], left, lane);
+        for (int t = 0; t < W::KT / 16; t += 2)
+            score_pair<D>(tile, t, lane, rows.q_hi, rows.q_lo, rows.q_exp, scores[t], scores[t + 1]);
+#pragma unroll
+        for (int b = 0; b < W::KT / 32; ++b) rows.add(tile, b, scores[2 * b], scores[2 * b + 1], end - first, lane);
     }
-    // the row anew: kept through the loop, its registers were those that spilled
-    uint32_t id = threadIdx.x;
-    asm volatile("" : "+v"(id));
-    rows.finish(a, item, row0 + id % 16, id % kWave / 16);
+    rows.finish(a, item, row0 + n, quarter);
 }
 
 // The prompt's tiles converted once, for batches whose rows would have every
@@ -570,7 +580,7 @@ __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnPara
 template <int FMT, int D>
 hipError_t launch_wide(hipStream_t stream, uint32_t items, const AttnParams& a, void* room) {
     if (!room) {
-        hipLaunchKernelGGL((attn_wide_kernel<FMT, D>), dim3(items), dim3(kAttnThreads), 0, stream, a);
+        hipLaunchKernelGGL((attn_wide_kernel<FMT, D>), dim3(items), dim3(kWideThreads), 0, stream, a);
         return hipGetLastError();
     }
     WideTile<D>* packed = static_cast<WideTile<D>*>(room);
