@@ -51,11 +51,14 @@ __device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const floa
 template <int FMT, int NB>
 __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel(AttnParams a) {
     constexpr int NG = (NB + 1) / 2;  // groups of 64 dims
-    constexpr int kSums = NG * 4 + 1;
-    constexpr int kRoom = kAttnWaves * kSums;
-    static_assert(kRoom >= NB * 2, "the queries fit");
-    // queries [step][half]; at the end the wavefronts' sums
-    __shared__ f32x4 room[kRoom][kWave];
+    constexpr uint32_t kDims = 64 * NG, kPitch = kDims + 4;
+    static_assert(kAttnWaves * 16 * kPitch * sizeof(float) >= NB * 2 * kWave * sizeof(f32x4), "the queries fit");
+    // queries [step][half][lane]; at the end the wavefronts' sums, row by row
+    __shared__ union {
+        f32x4 queries[NB * 2][kWave];
+        float sums[kAttnWaves][16][kPitch];
+    } room;
+    __shared__ float2 room_ml[kAttnWaves][16];
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
     const uint32_t n = lane % 16, quarter = lane / 16;
@@ -111,8 +114,8 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
         float x[8];
         load_query8<FMT>(a.q + (static_cast<uint64_t>(at / a.group) * a.q_heads + kv_head * a.group + at % a.group) * a.head_dim,
                          4 * i + quarter, a.head_dim, a.scale, x);
-        room[2 * i][lane] = f32x4{x[0], x[1], x[2], x[3]};
-        room[2 * i + 1][lane] = f32x4{x[4], x[5], x[6], x[7]};
+        room.queries[2 * i][lane] = f32x4{x[0], x[1], x[2], x[3]};
+        room.queries[2 * i + 1][lane] = f32x4{x[4], x[5], x[6], x[7]};
     }
     uint32_t seen = key_end;  // keys below it are seen by the lane's row
     const uint32_t row = row0 + n;
@@ -165,8 +168,8 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float x[8];
-            raw_values(k[b], x);
-            const f32x4 q0 = room[2 * b][lane], q1 = room[2 * b + 1][lane];
+            raw_values(k[b], x, key0 + n < key_end && 32 * b + 8 * quarter < a.head_dim);
+            const f32x4 q0 = room.queries[2 * b][lane], q1 = room.queries[2 * b + 1][lane];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], q0[j], s[0], 0, 0, 0);
@@ -184,7 +187,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 float x[4];
-                raw_values(raw_v[r][g], x);
+                raw_values(raw_v[r][g], x, key0 + 4 * quarter + r < key_end && 64 * g + 4 * n < a.head_dim);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[r][4 * g + j] = x[j];
             }
@@ -238,42 +241,36 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
         load_v(next);
     }
 
-    // join the wavefronts: each takes a part of the dims
+    // join the wavefronts; by way of LDS whole rows are written
     l = sum_xor32(sum_xor16(l));
     __syncthreads();
-    f32x4(*mine)[kWave] = room + wave * kSums;
-    mine[NG * 4][lane] = f32x4{m, l, 0.0f, 0.0f};
+    if (quarter == 0) room_ml[wave][n] = make_float2(m, l);
 #pragma unroll
-    for (int i = 0; i < NG * 4; ++i) mine[i][lane] = out[i];
-    __syncthreads();
-    float top = neg_inf(), sum = 0.0f, f[kAttnWaves];
-#pragma unroll
-    for (int w = 0; w < kAttnWaves; ++w) {
-        f[w] = room[w * kSums + NG * 4][lane].x;
-        top = fmaxf(top, f[w]);
-    }
-#pragma unroll
-    for (int w = 0; w < kAttnWaves; ++w) {
-        f[w] = f[w] == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(f[w] - top);
-        sum += f[w] * room[w * kSums + NG * 4][lane].y;
-    }
-    const uint64_t at = line0 + row;
-    if (wave == 0 && quarter == 0 && row < row_end) a.partial_ml[at] = make_float2(top, sum);
-    // group g of 64 dims, NG of the four quads that a lane has of it
-    const uint32_t g = wave % NG, quad0 = wave / NG * NG;
-    f32x4 o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) o[j] += f[w] * room[w * kSums + 4 * g + j][lane];
-    }
-    if (row < row_end) {
+    for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (i >= quad0 && i < quad0 + NG)
-                store_quad<FMT>(a.partial_out + at * a.head_dim, 16 * g + 4 * quarter + i, a.head_dim,
-                                f32x4{o[0][i], o[1][i], o[2][i], o[3][i]});
+            put_quad<FMT>(room.sums[wave][n], 16 * g + 4 * quarter + i,
+                          f32x4{out[4 * g][i], out[4 * g + 1][i], out[4 * g + 2][i], out[4 * g + 3][i]});
+    __syncthreads();
+    constexpr uint32_t kQuads = kDims / 4;
+#pragma unroll
+    for (uint32_t i = threadIdx.x; i < 16 * kQuads; i += kAttnThreads) {
+        const uint32_t r = i / kQuads, quad = i % kQuads;
+        if (row0 + r >= row_end || 4 * quad >= a.head_dim) continue;
+        float top = neg_inf(), sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; ++w) top = fmaxf(top, room_ml[w][r].x);
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; ++w) {
+            const float2 ml = room_ml[w][r];
+            const float f = ml.x == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
+            sum += f * ml.y;
+            o += f * *reinterpret_cast<const f32x4*>(&room.sums[w][r][4 * quad]);
+        }
+        const uint64_t at = line0 + row0 + r;
+        if (quad == 0) a.partial_ml[at] = make_float2(top, sum);
+        *reinterpret_cast<f32x4*>(a.partial_out + at * a.head_dim + 4 * quad) = o;
     }
 }
 

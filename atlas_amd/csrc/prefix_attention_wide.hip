@@ -30,10 +30,16 @@ namespace atlas {
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float max_mag(float a, float b) { return fmaxf(__builtin_fabsf(a), __builtin_fabsf(b)); }
+
+// What a wavefront's lanes have written to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // The exponent e that brings a row of largest magnitude `top` to
 // [2^14, 2^15) as x 2^-e; rows below 2^-low are taken as 2^-low.
@@ -42,28 +48,35 @@ __device__ __forceinline__ int row_exponent(float top, int low) {
     return (e < -low ? -low : e) - 14;
 }
 
-// x 2^-e as two f16 vectors.
+// x times[i] as two f16 vectors, where the product is exact in f32: each piece
+// is one instruction, rounded from the exact difference.
 struct Pieces {
     half8 hi, lo;
 };
-__device__ __forceinline__ Pieces pieces(const float (&x)[8]) {
-    Pieces p;
+template <class Times>
+__device__ __forceinline__ Pieces pieces(const float (&x)[8], const Times& times) {
+    u32x4_t hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const f32x2_t y = {x[2 * i], x[2 * i + 1]};
-        const half2_t h = __builtin_convertvector(y, half2_t);
-        // y - h in one instruction each, exactly
-        f32x2_t rest;
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rest.x) : "v"(h), "v"(y.x));
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rest.y) : "v"(h), "v"(y.y));
-        const half2_t l = __builtin_convertvector(rest, half2_t);
-        p.hi[2 * i] = h.x;
-        p.hi[2 * i + 1] = h.y;
-        p.lo[2 * i] = l.x;
-        p.lo[2 * i + 1] = l.y;
+        const float x0 = x[2 * i], x1 = x[2 * i + 1], t0 = times(2 * i), t1 = times(2 * i + 1);
+        uint32_t h, l;
+        asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(x0), "v"(t0));
+        asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(x1), "v"(t1));
+        asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(l) : "v"(x0), "v"(t0), "v"(h));
+        asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(x1), "v"(t1), "v"(h));
+        hi[i] = h;
+        lo[i] = l;
     }
-    return p;
+    return {__builtin_bit_cast(half8, hi), __builtin_bit_cast(half8, lo)};
 }
+__device__ __forceinline__ Pieces pieces(const float (&x)[8], float times) {
+    return pieces(x, [=](int) { return times; });
+}
+
+// A quantised row's exponent is that of its largest block scale and code: the
+// pieces keep their bits wherever the row lies in f16's range.
+template <int FMT>
+constexpr float kMostCode = FMT == kKvQ8_0 ? 128.0f : 8.0f;
 
 // Sizes of a kernel: D the head_dim it is padded to.
 template <int D>
@@ -133,30 +146,31 @@ __device__ __forceinline__ void load_values(RawValues<FMT>& raw, const WideLane<
 }
 
 template <int FMT, int D>
-__device__ __forceinline__ void convert_keys(const RawKeys<FMT, D>& raw, WideTile<D>& tile, uint32_t lane, uint32_t wave) {
+__device__ __forceinline__ void convert_keys(const RawKeys<FMT, D>& raw, WideTile<D>& tile, uint32_t lane, uint32_t wave,
+                                             uint32_t left, uint32_t head_dim) {
     using W = Wide<D>;
 #pragma unroll
     for (int i = 0; i < W::KI; ++i) {
         float x[W::KU][8], times[W::KU];
         float top = 0.0f;
+        const uint32_t key = 32 * i + 8 * wave + lane % 8;
 #pragma unroll
         for (int u = 0; u < W::KU; ++u) {
-            times[u] = raw.at[i][u].codes(x[u]);
-            float most = 0.0f;
+            times[u] = raw.at[i][u].codes(x[u], key < left && 8 * (lane / 8 + 8 * u) < head_dim);
+            if (FMT == kKvF32) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) most = max_mag(most, x[u][j]);
-            top = max_mag(top, most * times[u]);
+                for (int j = 0; j < 8; ++j) top = max_mag(top, x[u][j]);
+            } else {
+                top = max_mag(top, times[u] * kMostCode<FMT>);
+            }
         }
         top = max_xor32(max_xor16(max_xor8(top)));
         const int e = row_exponent(top, 100);
         const float scale = pow2i(-e);
-        const uint32_t key = 32 * i + 8 * wave + lane % 8;
         if (lane < 8) tile.key_exp[key] = e;
 #pragma unroll
         for (int u = 0; u < W::KU; ++u) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[u][j] *= times[u] * scale;
-            const Pieces p = pieces(x[u]);
+            const Pieces p = pieces(x[u], times[u] * scale);
             const uint32_t unit = lane / 8 + 8 * u;
             const uint32_t frag = (key / 16 * W::KS + unit / 4) * 2, to = unit % 4 * 16 + key % 16;
             tile.key[frag][to] = p.hi;
@@ -166,7 +180,8 @@ __device__ __forceinline__ void convert_keys(const RawKeys<FMT, D>& raw, WideTil
 }
 
 template <int FMT, int D>
-__device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTile<D>& tile, uint32_t lane, uint32_t wave) {
+__device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTile<D>& tile, uint32_t lane, uint32_t wave,
+                                               uint32_t left, uint32_t head_dim) {
     using W = Wide<D>;
     constexpr uint32_t kQuads = D / 4;
     const uint32_t group = wave * (kWave / kQuads) + lane / kQuads, quad = lane % kQuads;
@@ -175,8 +190,8 @@ __device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTi
     float top[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        times[j] = raw.at[j].codes(x[j]);
-        top[j] = __builtin_fabsf(fmaxf(max_mag(x[j][0], x[j][1]), max_mag(x[j][2], x[j][3])) * times[j]);
+        times[j] = raw.at[j].codes(x[j], key0 + 16 * (j >> 2) + (j & 3) < left && 4 * quad < head_dim);
+        top[j] = FMT == kKvF32 ? fmaxf(max_mag(x[j][0], x[j][1]), max_mag(x[j][2], x[j][3])) : __builtin_fabsf(times[j] * kMostCode<FMT>);
     }
     // eight maxima over the group's lanes: each step halves what a lane keeps,
     // ending with key lane % 8
@@ -198,19 +213,15 @@ __device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTi
         // an infinity would leave the row's other values no bits: NaN, not a wrong number
         tile.value_scale[key] = m == __builtin_inff() ? __builtin_nanf("") : pow2i(-e);
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_lds_fence();
     const f32x4 s0 = *reinterpret_cast<const f32x4*>(&tile.value_scale[key0]);
     const f32x4 s1 = *reinterpret_cast<const f32x4*>(&tile.value_scale[key0 + 16]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) times[j] *= j < 4 ? s0[j & 3] : s1[j & 3];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[j][e] * times[j];
-        const Pieces p = pieces(y);
+        const float y[8] = {x[0][e], x[1][e], x[2][e], x[3][e], x[4][e], x[5][e], x[6][e], x[7][e]};
+        const Pieces p = pieces(y, [&](int j) { return times[j]; });
         // dim e of quad q: row q % 16 of block 4 (q / 16) + e
         const uint32_t frag = (group / 4 * W::DT + 4 * (quad / 16) + e) * 2, to = group % 4 * 16 + quad % 16;
         tile.value[frag][to] = p.hi;
@@ -353,9 +364,7 @@ struct WideRows {
         const float scale = pow2i(-q_exp);
 #pragma unroll
         for (int s = 0; s < Wide<D>::KS; ++s) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[s][j] *= scale;
-            const Pieces p = pieces(x[s]);
+            const Pieces p = pieces(x[s], scale);
             q_hi[s] = p.hi;
             q_lo[s] = p.lo;
         }
@@ -407,26 +416,44 @@ struct WideRows {
             l += w;
             s[j] = __builtin_ldexpf(w, ev[j / 4][j % 4] + shift);
         }
-        add_values<D>(tile, b, lane, pieces(s), out);
+        add_values<D>(tile, b, lane, pieces(s, 1.0f), out);
     }
 
-    // The segment's sums, relative to 2^m.
-    __device__ __forceinline__ void finish(const AttnParams& a, const WideItem& item, uint32_t row, uint32_t quarter) {
-        if (row >= a.rows) return;
+    // The segment's sums, relative to 2^m, by way of LDS (`room` of the
+    // wavefront, 8 rows at a time) so that whole rows are written: straight from
+    // the accumulators, 16 bytes here and there, it took 13 us.
+    static constexpr uint32_t kPitch = D + 4, kRoom = 8 * kPitch;
+    __device__ __forceinline__ void finish(const AttnParams& a, const WideItem& item, uint32_t row0, float* room, uint32_t lane) {
+        const uint32_t n = lane % 16, quarter = lane / 16;
         const float all = sum_xor32(sum_xor16(l));
         const int back = m == neg_inf() ? 0 : static_cast<int>(mv - m) - 6;
-        const uint64_t to = (static_cast<uint64_t>(item.slot) * a.kv_heads + item.kv_head) * a.rows + row;
-        if (quarter == 0) a.partial_ml[to] = make_float2(m, all);
-        float* p = a.partial_out + to * a.head_dim;
+        const uint64_t to = (static_cast<uint64_t>(item.slot) * a.kv_heads + item.kv_head) * a.rows + row0;
+        if (quarter == 0 && row0 + n < a.rows) a.partial_ml[to + n] = make_float2(m, all);
 #pragma unroll
-        for (int d = 0; d < Wide<D>::DT; d += 4)
+        for (uint32_t half = 0; half < 2; ++half) {
+            if (n / 8 == half) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f32x4 v;
+                for (int d = 0; d < Wide<D>::DT; d += 4)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(out[d + e][i], back);
-                store_quad<FMT>(p, 4 * d + 4 * quarter + i, a.head_dim, v);
+                    for (int i = 0; i < 4; ++i) {
+                        f32x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = __builtin_ldexpf(out[d + e][i], back);
+                        put_quad<FMT>(room + n % 8 * kPitch, 4 * d + 4 * quarter + i, v);
+                    }
             }
+            wave_lds_fence();
+            constexpr uint32_t kQuads = D / 4, kAtOnce = kWave / kQuads;
+            const uint32_t quad = lane % kQuads;
+#pragma unroll
+            for (uint32_t r0 = 0; r0 < 8; r0 += kAtOnce) {
+                const uint32_t r = r0 + lane / kQuads, row = 8 * half + r;
+                const f32x4 v = *reinterpret_cast<const f32x4*>(room + r * kPitch + 4 * quad);
+                if (row0 + row < a.rows && 4 * quad < a.head_dim)
+                    *reinterpret_cast<f32x4*>(a.partial_out + (to + row) * a.head_dim + 4 * quad) = v;
+            }
+            wave_lds_fence();
+        }
     }
 };
 
@@ -446,6 +473,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a
     const uint32_t end = item.end;
     uint32_t buffer = 0;
     if (wave >= 4) {
+        __builtin_amdgcn_s_setprio(2);  // converting takes longest: 43.2 us without (100003 keys, 64 rows)
         const uint32_t head_off = static_cast<uint32_t>(head_offset<FMT>(item.kv_head, a.head_dim));
         const uint8_t* keys = a.prefix + head_off;
         const uint8_t* values = a.prefix + a.prefix_plane + head_off;
@@ -470,9 +498,9 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
                 if (first >= end) break;
-                convert_keys(raw_keys[i], buffers[buffer], lane, wave - 4);
+                convert_keys(raw_keys[i], buffers[buffer], lane, wave - 4, end - first, a.head_dim);
                 load_keys(raw_keys[i], mine, rows_of(keys, first + kAhead * W::KT));
-                convert_values(raw_values[i], buffers[buffer], lane, wave - 4);
+                convert_values(raw_values[i], buffers[buffer], lane, wave - 4, end - first, a.head_dim);
                 load_values(raw_values[i], mine, rows_of(values, first + kAhead * W::KT));
                 __syncthreads();
                 first += W::KT;
@@ -484,6 +512,7 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a
     const uint32_t row0 = item.tile * 64 + wave * 16;
     const bool busy = row0 < a.rows;  // the wavefront has rows
     WideRows<FMT, D> rows(a, item.kv_head, row0 + n, quarter);
+    
     for (uint32_t first = item.begin; first < end; first += W::KT, buffer ^= 1) {
         __syncthreads();
         if (!busy) continue;
@@ -495,7 +524,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a
 #pragma unroll
         for (int b = 0; b < W::KT / 32; ++b) rows.add(tile, b, scores[2 * b], scores[2 * b + 1], end - first, lane);
     }
-    rows.finish(a, item, row0 + n, quarter);
+    // the buffer of the tile before the last is free
+    if (busy) rows.finish(a, item, row0, reinterpret_cast<float*>(&buffers[buffer]) + wave * rows.kRoom, lane);
 }
 
 // The prompt's tiles converted once, for batches whose rows would have every
@@ -515,8 +545,8 @@ __global__ __launch_bounds__(kAttnThreads) void attn_pack_kernel(AttnParams a, W
     const uint32_t there = min(a.prefix_length - first, static_cast<uint32_t>(W::KT));
     load_keys(raw_keys, mine, TileRows<FMT>(a.prefix + head_off, first, there, a.row_bytes, head_off));
     load_values(raw_values, mine, TileRows<FMT>(a.prefix + a.prefix_plane + head_off, first, there, a.row_bytes, head_off));
-    convert_keys(raw_keys, tile, lane, wave);
-    convert_values(raw_values, tile, lane, wave);
+    convert_keys(raw_keys, tile, lane, wave, there, a.head_dim);
+    convert_values(raw_values, tile, lane, wave, there, a.head_dim);
     __syncthreads();
     const f32x4* from = reinterpret_cast<const f32x4*>(&tile);
     f32x4* to = reinterpret_cast<f32x4*>(packed + blockIdx.x);
@@ -530,6 +560,7 @@ constexpr int kPackedThreads = 512;
 template <int FMT, int D>
 __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnParams a, const WideTile<D>* packed, uint32_t tiles) {
     using W = Wide<D>;
+    static_assert(sizeof(WideTile<D>) >= 8 * WideRows<FMT, D>::kRoom * sizeof(float), "eight wavefronts' rows fit a buffer");
     static_assert(sizeof(WideTile<D>) % 1024 == 0, "copied by whole KiB");
     constexpr uint32_t kChunks = sizeof(WideTile<D>) / 1024;
     __shared__ WideTile<D> buffers[2];
@@ -574,7 +605,8 @@ __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnPara
 #pragma unroll
         for (int b = 0; b < W::KT / 32; ++b) rows.add(tile, b, scores[2 * b], scores[2 * b + 1], left, lane);
     }
-    rows.finish(a, item, row, quarter);
+    // the buffer of the tile before the last is free
+    if (busy) rows.finish(a, item, row0, reinterpret_cast<float*>(&buffers[buffer]) + wave * rows.kRoom, lane);
 }
 
 template <int FMT, int D>
