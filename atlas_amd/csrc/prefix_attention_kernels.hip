@@ -396,15 +396,15 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         const uint32_t most = (s.prefix_length + tile - 1) / tile;
         // Packing converts a tile of keys once, not once for every 64 rows, for a
         // launch and a copy of the tiles: it pays from eight such row tiles and
-        // three tiles of keys a workgroup on.  Whole calls without and with it,
-        // us, rows x prompt, one KV head of 256 and four of 128:
-        //   256 x 4097   43 / 45   45 / 42     480 x 4097    48 / 49   (512) 56 / 50
-        //   256 x 32768  71 / 80  108 / 105    512 x 32768  100 / 100
-        //   512 x 1000   37 / 42   37 / 39     2048 x 4097   77 / 70   (1024) 82 / 70
+        // twelve tiles of keys a workgroup on.  Whole calls without and with it, us,
+        // rows x prompt, a KV head of 256 dims, four of 128, three of 64:
+        //   512 x 1000   32 / 39   29 / 37   20 / 24    512 x 4097  39 / 43   43 / 46   31 / 36
+        //   1024 x 4097  46 / 48   72 / 66   48 / 46    2048 x 4097 60 / 61  (64 dims) 78 / 67
+        //   256 x 32768  61 / 75  100 / 103  68 / 75    512 x 32768 90 / 94  (64 dims) 121 / 97
         // Tiles take as much as the prompt in f32, of which a caller may have none to
         // spare beside a very long one: 4 GiB at most.
         const uint64_t row_tiles = (rows + 63) / 64, packed_bytes = attn_packed_bytes(s.head_dim, s.kv_heads, s.prefix_length);
-        const bool packed = row_tiles >= 8 && row_tiles * most * s.kv_heads >= 3 * 512 && packed_bytes <= 1ull << 32;
+        const bool packed = row_tiles >= 8 && row_tiles * most * s.kv_heads >= 12 * 256 && packed_bytes <= 1ull << 32;
         if (packed) p.packed_bytes = round256(packed_bytes);
         p.prefix_tiles = static_cast<uint32_t>(packed ? (rows + 127) / 128 : row_tiles);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
