@@ -70,21 +70,34 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
     const uint32_t steps = KEYS ? KEYS : (n + kSelectThreads - 1) / kSelectThreads;
     const uint32_t first = wave * steps * kWave + lane;
     // how many of this lane's positions are old, and there: comparing k with
-    // them keeps 64 positions a lane out of the registers
-    const uint32_t mine_old = old > first ? (old - first + kWave - 1) / kWave : 0u;
-    const uint32_t mine_all = n > first ? (n - first + kWave - 1) / kWave : 0u;
+    // them keeps 64 positions a lane out of the registers, and each pass anew
+    // (the empty asm) the 64 masks of the comparisons
+    uint32_t mine_old = old > first ? (old - first + kWave - 1) / kWave : 0u;
+    uint32_t mine_all = n > first ? (n - first + kWave - 1) / kWave : 0u;
     const auto key_at = [&](uint32_t k) {
         if (k >= mine_old) return 0xffffffffu;  // recent: above every weight
         return weight_key(weights[first + k * kWave]);
     };
     uint32_t held[KEYS ? KEYS : 1];
     if (KEYS) {
+        // sixteen loads are on their way before the first key is made of them:
+        // one behind the other 64 of them took 35 us
+        constexpr int kAtOnce = KEYS && KEYS < 16 ? KEYS : 16;
 #pragma unroll
-        for (int k = 0; k < KEYS; ++k) held[k] = key_at(k);
+        for (int k0 = 0; k0 < KEYS; k0 += kAtOnce) {
+#pragma unroll
+            for (int k = k0; k < k0 + kAtOnce; ++k)
+                held[k] = __float_as_uint(weights[static_cast<uint32_t>(k) < mine_old ? first + k * kWave : 0u]);
+#pragma unroll
+            for (int k = k0; k < k0 + kAtOnce; ++k)
+                held[k] = static_cast<uint32_t>(k) < mine_old ? weight_key(__uint_as_float(held[k])) : 0xffffffffu;
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
     // f(k, key) for every position first + 64 k of this lane, in order
     const auto each = [&](auto&& f) {
         if constexpr (KEYS != 0) {
+            asm volatile("" : "+v"(mine_old), "+v"(mine_all));
 #pragma unroll
             for (uint32_t k = 0; k < KEYS; ++k) f(k, held[k]);
         } else {
