@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t waves_before(uint32_t mine, uint32_t (&room)
 // KEYS = 0: longer sequences, whose keys are read anew by every pass.
 // Histogram bins have 16 counters, one for every lane % 16: few exponents
 // share most weights, and lanes that add to one counter go one by one (a
-// sequence of 65536 in one counter a bin took 193 us).
+// sequence of 65536 in one counter a bin took 193 us; so 52, of 2048 6 us).
 template <int KEYS>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArgs a) {
     __shared__ uint32_t bins[256][16];
@@ -197,7 +197,9 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
 }
 
 // Rows to another cache, a thread a unit of T at a time, and the weights as
-// rows of one unit: blockIdx.y is a sequence and a plane, or its weights.
+// rows of one unit: blockIdx.y is a sequence and a plane, or its weights.  Bound
+// by its bytes: 256 sequences keeping up to 512 rows of 1 KiB, 0.5 GB, 91 us,
+// 5.5 TB/s read and written.
 constexpr int kMoveThreads = 256;
 
 template <typename T>
@@ -228,7 +230,9 @@ __global__ __launch_bounds__(kMoveThreads) void evict_copy_kernel(KvEvictArgs a,
 // Rows within their cache: a workgroup owns a column of units of one sequence
 // and plane and walks its rows from the front, eight to a thread a step, each
 // step's loads before its stores.  A row only moves towards the front, so what
-// a step loads lies behind all that earlier ones store.
+// a step loads lies behind all that earlier ones store.  The barrier of each
+// step bounds it: the 256 sequences above 55 us (a third of their rows stay
+// where they are).
 constexpr int kShiftThreads = 1024;
 constexpr int kShiftRows = 8;
 
@@ -294,8 +298,12 @@ hipError_t launch_move(hipStream_t stream, const KvEvictArgs& a, bool in_place) 
         b.weights_out = a.weights_out + positions;
         b.kept = a.kept + static_cast<uint64_t>(s0) * a.budget;
         if (in_place) {
-            // 256 bytes of a row at most: narrow columns leave more workgroups
-            const uint32_t column = units < 16 ? units : 16;
+            // 256 bytes of a row to a workgroup, or 64 where those are too few for
+            // the chip (8 sequences keeping 30000 rows of 1088 bytes 386 -> 277 us,
+            // one keeping 1024 of 768 bytes 8.4 -> 4.2)
+            uint32_t column = 256 / sizeof(T);
+            while (column > 64 / sizeof(T) && (units + column - 1) / column * 2 * count < 256) column /= 2;
+            if (column > units) column = units;
             hipLaunchKernelGGL((evict_shift_kernel<T>), dim3((units + column - 1) / column, 2 * count), dim3(kShiftThreads), 0,
                                stream, b, units, column);
         } else {

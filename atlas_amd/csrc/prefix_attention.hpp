@@ -261,7 +261,7 @@ __device__ __forceinline__ void put_quad(float* row, uint32_t q, f32x4 v) {
 }
 
 // Part `i` of `parts` of `rows` rows, in whole units of `unit`: no two parts
-// differ by more than one (slots is at most 2^9 or so, units below 2^29).
+// differ by more than one.
 __device__ __forceinline__ void part_of(uint32_t rows, uint32_t unit, uint32_t i, uint32_t parts, uint32_t& begin, uint32_t& end) {
     const uint32_t units = (rows + unit - 1) / unit, each = units / parts, more = units % parts;
     begin = min((i * each + min(i, more)) * unit, rows);

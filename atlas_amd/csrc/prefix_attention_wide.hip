@@ -15,15 +15,18 @@
 // that sum 2^x v = 2^{m'} sum p' v' keeps every row's precision whatever the
 // rows' scales.  m and m' are whole numbers: all these factors are exact.
 //
-// A workgroup of four wavefronts takes 64 query rows and walks one segment in
-// tiles of KT keys: the tile's rows come from the cache as they are stored and
-// are converted once, into the fragments that the matrix instructions read
-// (LDS, 16 bytes a lane, in lane order: no bank conflicts).  A wavefront holds
-// 16 rows' queries and accumulators in registers; S^T = K Q^T leaves lane l
-// with query row l % 16, so its maximum and sum are the lane's own up to two
-// exchanges, and P^T is the operand of O^T = V^T P^T without leaving its
-// registers.  Two workgroups share a CU: one converts or waits for rows while
-// the other multiplies.
+// A workgroup walks one segment in tiles of KT keys: the tile's rows come from
+// the cache as they are stored and are converted once, into the fragments that
+// the matrix instructions read (LDS, 16 bytes a lane, in lane order: no bank
+// conflicts).  A wavefront holds 16 rows' queries and accumulators in registers
+// (32 rows spilled); S^T = K Q^T leaves lane l with query row l % 16, so its
+// maximum and sum are the lane's own up to two exchanges, and P^T is the operand
+// of O^T = V^T P^T without leaving its registers.
+//
+// Measured: 64 rows x 100003 keys of 256 dims Q8_0 40 us, of which 12 are start
+// and segments; converting and multiplying take as long as each other (4500
+// cycles a tile).  2048 rows x 32768 f32, packed, 190 us: 1.08 PFLOP/s of f16,
+// what a large matrix product reaches here.
 #include "prefix_attention.hpp"
 
 namespace atlas {
@@ -459,8 +462,10 @@ struct WideRows {
 
 // Eight wavefronts: four convert a tile while the other four, 16 rows each,
 // multiply the one before it, so that the vector units and the matrix units of
-// every SIMD have a wavefront of their own.  One barrier a tile: behind it the
-// converted tile is there and the buffer of the one before is free.
+// every SIMD have a wavefront of their own (all eight doing both in turn, in two
+// workgroups, 48 us for 100003 keys and 64 rows; so 43).  One barrier a tile:
+// behind it the converted tile is there and the buffer of the one before is
+// free.
 constexpr int kWideThreads = 512;
 
 template <int FMT, int D>
@@ -529,7 +534,8 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a
 }
 
 // The prompt's tiles converted once, for batches whose rows would have every
-// one converted many times: a workgroup a tile of a KV head.
+// one converted many times: a workgroup a tile of a KV head.  Its bytes bound
+// it: 32768 keys of 256 dims f32 26 us, 5.2 TB/s read and written.
 template <int FMT, int D>
 __global__ __launch_bounds__(kAttnThreads) void attn_pack_kernel(AttnParams a, WideTile<D>* packed, uint32_t tiles) {
     using W = Wide<D>;
