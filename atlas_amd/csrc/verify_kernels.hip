@@ -38,34 +38,67 @@ typedef f32x4 f32x4_row __attribute__((aligned(4)));
 
 __device__ __forceinline__ float number_or_none(float x) { return x != x ? -__builtin_inff() : x; }
 
-// 2^y, y <= 0, by 2^(j / 32) from a table in LDS and the Taylor polynomial of
-// 2^r to the sixth degree, |r| <= 1 / 64: (r ln 2)^7 / 7! is below 2^-58.  With
-// the rounding of y and of the products, within 2^-51 (|y| + 2) of the true value.
-// About half the operations of the library's exp, whose time the first launch
-// then took: see verify_stats_kernel.
-__device__ __forceinline__ void exp_table(double* table) {
-    if (threadIdx.x < 32) table[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32.0));
-}
-__device__ __forceinline__ double exp2_table(double y, const double* table) {
-    const double yc = fmax(y, -1200.0);  // 0 there, and what is no number ends there too
-    const double n = __builtin_rint(yc * 32.0);
-    const double r = __builtin_fma(n, -1.0 / 32.0, yc);
-    const int k = static_cast<int>(n);
-    double p = 0x1.430912f86c787p-13;               // ln2^6 / 720
-    p = __builtin_fma(p, r, 0x1.5d87fe78a6731p-10);  // ln2^5 / 120
-    p = __builtin_fma(p, r, 0x1.3b2ab6fba4e77p-7);   // ln2^4 / 24
-    p = __builtin_fma(p, r, 0x1.c6b08d704a0c0p-5);   // ln2^3 / 6
-    p = __builtin_fma(p, r, 0x1.ebfbdff82c58fp-3);   // ln2^2 / 2
-    p = __builtin_fma(p, r, 0x1.62e42fefa39efp-1);   // ln2
-    p = __builtin_fma(p, r, 1.0);
-    return __builtin_ldexp(p * table[k & 31], k >> 5);
-}
+// 2^(y / 32), y <= 0, by 2^(j / 32) from a table in LDS and the Taylor
+// polynomial of 2^(r / 32) to the sixth degree, |r| <= 1 / 2: ((r / 32) ln 2)^7 / 7!
+// is below 2^-58.  With the rounding of y and of the products, within
+// 2^-51 (|y / 32| + 2) of the true value; zero from 2^-1023 down, and of a y that is
+// no number.
+//
+// Its instructions bound the first launch, so it has few (15 and a read; with
+// the library's exp that launch took 120 us, as written in C 105, so NEWFIG):
+// adding 1.5 2^52 leaves the nearest whole number of thirty-seconds in the low
+// bits of the sum, with 1023 of them in front; its upper part is added to the
+// exponent of a table entry, whose own is taken out; and the constants stay in
+// registers, one operand of an instruction a scalar one, which the compiler
+// would not hold them in by itself.
+struct Exp2 {
+    const uint2* table;
+    double first, c[5], shift, least;
 
-// e^{(x - top) * inv}, `scale` = inv log2(e): 1 at the top (also of an infinite
-// one), 0 in a row that has none.
-__device__ __forceinline__ double mass(float x, float top, double scale, const double* table) {
-    const double e = exp2_table((static_cast<double>(x) - static_cast<double>(top)) * scale, table);
-    return top == -__builtin_inff() ? 0.0 : (x == top ? 1.0 : e);
+    static __device__ void fill(uint2 (&table)[32]) {
+        if (threadIdx.x < 32) {
+            const uint64_t bits = __builtin_bit_cast(uint64_t, exp2(threadIdx.x * (1.0 / 32.0)));
+            table[threadIdx.x] = make_uint2(static_cast<uint32_t>(bits), static_cast<uint32_t>(bits >> 32) - (1023u << 20));
+        }
+    }
+    explicit __device__ Exp2(const uint2 (&table)[32])
+        : table(table),
+          first(0x1.430912f86c787p-13 * 0x1p-30),  // ln2^6 / 720, of 1 / 32 each
+          c{0x1.5d87fe78a6731p-10 * 0x1p-25,       // ln2^5 / 120
+            0x1.3b2ab6fba4e77p-7 * 0x1p-20,        // ln2^4 / 24
+            0x1.c6b08d704a0c0p-5 * 0x1p-15,        // ln2^3 / 6
+            0x1.ebfbdff82c58fp-3 * 0x1p-10,        // ln2^2 / 2
+            0x1.62e42fefa39efp-1 * 0x1p-5},        // ln2
+          shift(0x1.8p52 + 32 * 1023), least(-32.0 * 1023.0) {
+        asm("" : "+v"(first));
+#pragma unroll
+        for (int i = 0; i < 5; ++i) asm("" : "+s"(c[i]));
+        asm("" : "+s"(shift), "+s"(least));
+    }
+    __device__ __forceinline__ double operator()(double y) const {
+        y = fmax(y, least);
+        const double t = y + shift;
+        const double r = y - (t - shift);
+        const uint32_t k = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, t));
+        double p = first;
+#pragma unroll
+        for (int i = 0; i < 5; ++i) p = __builtin_fma(p, r, c[i]);
+        p = __builtin_fma(p, r, 1.0);
+        uint2 power = table[k & 31];
+        power.y += k >> 5 << 20;
+        return p * __builtin_bit_cast(double, static_cast<uint64_t>(power.y) << 32 | power.x);
+    }
+};
+
+// A row's masses are e^{(x - top) * inv}, `scale` = 32 inv log2(e): 1 at the top,
+// of an infinite one too, 0 in a row that has none.  With an infinite top that
+// is the same about zero, for 0 at the top and -inf elsewhere.
+__device__ __forceinline__ float about(float x, float top) {
+    return top == __builtin_inff() ? (x == top ? 0.0f : -__builtin_inff()) : x;
+}
+__device__ __forceinline__ double finite(float top) { return __builtin_isinf(top) ? 0.0 : static_cast<double>(top); }
+__device__ __forceinline__ double mass(float x, float top, double scale, const Exp2& exp2_of) {
+    return exp2_of((static_cast<double>(about(x, top)) - finite(top)) * scale);
 }
 
 template <int CTRL, int ROW_MASK, bool BOUND>
@@ -112,7 +145,7 @@ struct Decision {
 
 struct VerifyParams {
     VerifyDraftArgs s;
-    double scale;             // inv_temperature log2(e)
+    double scale;             // 32 inv_temperature log2(e)
     SliceStat* target_stats;  // [sequence][drafts + 1][slices]
     SliceStat* draft_stats;   // [sequence][drafts][slices]
     double* slice_sums;       // [sequence][slices]
@@ -148,7 +181,7 @@ __device__ __forceinline__ void load_slice(const float* logits, uint32_t first, 
 // bytes bound it, once the exponentials are short: 384 rows of 262144 logits
 // 105 us, 3.8 TB/s (120 us with the library's exp).
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyParams v) {
-    __shared__ double table[32];
+    __shared__ uint2 table[32];
     const VerifyDraftArgs& s = v.s;
     const uint32_t rows = s.drafts + 1 + (s.draft ? s.drafts : 0);
     const uint32_t seq = blockIdx.x / (v.blocks * rows);
@@ -163,16 +196,22 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyPara
                                     : s.draft + (static_cast<uint64_t>(seq) * s.drafts + row) * s.vocab;
     float x[kEach];
     load_slice(logits, min(slice, v.slices - 1) * kSlice, s.vocab, x);
-    exp_table(table);
+    Exp2::fill(table);
+    const Exp2 exp2_of(table);
     __syncthreads();
     if (slice >= v.slices) return;
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
     top = wave_max_tree_f32(top);
+    if (top == __builtin_inff()) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) x[i] = about(x[i], top);
+    }
+    const double zero = finite(top);
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += mass(x[i], top, v.scale, table);
+    for (int i = 0; i < kEach; ++i) sum += exp2_of((static_cast<double>(x[i]) - zero) * v.scale);
     sum = wave_sum_f64(sum);
     SliceStat* out = of_target ? v.target_stats + (static_cast<uint64_t>(seq) * (s.drafts + 1) + row) * v.slices
                                : v.draft_stats + (static_cast<uint64_t>(seq) * s.drafts + row) * v.slices;
@@ -186,13 +225,13 @@ __device__ __forceinline__ SliceStat first_stat(const SliceStat* slices, uint32_
     return lane < count ? slices[lane] : SliceStat{0.0, -__builtin_inff(), 0.0f};
 }
 __device__ __forceinline__ void row_stat(const SliceStat& first, const SliceStat* slices, uint32_t count, double scale,
-                                         const double* table, float& top, double& sum) {
+                                         const Exp2& exp2_of, float& top, double& sum) {
     const uint32_t lane = threadIdx.x % kWave;
     top = first.top;
     for (uint32_t i = lane + kWave; i < count; i += kWave) top = fmaxf(top, slices[i].top);
     top = wave_max_tree_f32(top);
-    sum = first.sum * mass(first.top, top, scale, table);
-    for (uint32_t i = lane + kWave; i < count; i += kWave) sum += slices[i].sum * mass(slices[i].top, top, scale, table);
+    sum = first.sum * mass(first.top, top, scale, exp2_of);
+    for (uint32_t i = lane + kWave; i < count; i += kWave) sum += slices[i].sum * mass(slices[i].top, top, scale, exp2_of);
     sum = wave_sum_f64(sum);
 }
 
@@ -200,7 +239,7 @@ __device__ __forceinline__ void row_stat(const SliceStat& first, const SliceStat
 // in turn, the drafts' tests by its threads.  The table is filled, and `d` can
 // be read, behind the barriers here.
 template <int THREADS, uint32_t MOST>
-__device__ void decide(const VerifyParams& v, uint32_t seq, const double* table, Decision& d) {
+__device__ void decide(const VerifyParams& v, uint32_t seq, const Exp2& exp2_of, Decision& d) {
     constexpr uint32_t kWaves = THREADS / kWave;
     __shared__ double sums[2][MOST + 1];
     __shared__ float tops[2][MOST + 1];
@@ -226,7 +265,7 @@ __device__ void decide(const VerifyParams& v, uint32_t seq, const double* table,
             if (r >= rows) break;
             float top;
             double sum;
-            row_stat(first[i], stats_of(r), v.slices, v.scale, table, top, sum);
+            row_stat(first[i], stats_of(r), v.slices, v.scale, exp2_of, top, sum);
             if (threadIdx.x % kWave == 0) {
                 sums[r > count][r <= count ? r : r - count - 1] = sum;
                 tops[r > count][r <= count ? r : r - count - 1] = top;
@@ -240,9 +279,9 @@ __device__ void decide(const VerifyParams& v, uint32_t seq, const double* table,
         double p = 0.0, q = s.draft ? 0.0 : 1.0;
         if (token < s.vocab) {
             const float x = number_or_none(s.target[(static_cast<uint64_t>(seq) * (s.drafts + 1) + t) * s.vocab + token]);
-            if (sums[0][t] > 0.0) p = mass(x, tops[0][t], v.scale, table) / sums[0][t];
+            if (sums[0][t] > 0.0) p = mass(x, tops[0][t], v.scale, exp2_of) / sums[0][t];
             if (s.draft && sums[1][t] > 0.0)
-                q = mass(number_or_none(s.draft[at * s.vocab + token]), tops[1][t], v.scale, table) / sums[1][t];
+                q = mass(number_or_none(s.draft[at * s.vocab + token]), tops[1][t], v.scale, exp2_of) / sums[1][t];
         }
         if (!(static_cast<double>(s.accept_uniform[at]) * q < p)) atomicMin(&first_rejected, t);
     }
@@ -256,10 +295,11 @@ __device__ void decide(const VerifyParams& v, uint32_t seq, const double* table,
 }
 
 __global__ __launch_bounds__(kPickThreads) void verify_decide_kernel(VerifyParams v) {
-    __shared__ double table[32];
-    exp_table(table);
+    __shared__ uint2 table[32];
+    Exp2::fill(table);
+    const Exp2 exp2_of(table);
     Decision d;
-    decide<kPickThreads, 1024>(v, blockIdx.x, table, d);
+    decide<kPickThreads, 1024>(v, blockIdx.x, exp2_of, d);
     if (threadIdx.x == 0) v.decisions[blockIdx.x] = d;
 }
 
@@ -284,10 +324,10 @@ struct Terms {
         target_scale = d.target_sum > 0.0 ? 1.0 / d.target_sum : 0.0;
         draft_scale = d.draft_sum > 0.0 ? 1.0 / d.draft_sum : 0.0;
     }
-    __device__ double term(float x, float y, uint32_t at, const double* table) const {
-        const double p = mass(x, target_top, scale, table) * target_scale;
+    __device__ double term(float x, float y, uint32_t at, const Exp2& exp2_of) const {
+        const double p = mass(x, target_top, scale, exp2_of) * target_scale;
         if (!draft) return at == token ? 0.0 : p;
-        const double q = mass(y, draft_top, scale, table) * draft_scale;
+        const double q = mass(y, draft_top, scale, exp2_of) * draft_scale;
         return p > q ? p - q : 0.0;
     }
 };
@@ -298,13 +338,14 @@ struct Terms {
 // decides for itself, and the first leaves the decision for the next launch.
 template <bool FUSED>
 __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyParams v) {
-    __shared__ double table[32];
+    __shared__ uint2 table[32];
     const uint32_t seq = blockIdx.x / v.blocks, block = blockIdx.x % v.blocks;
     const uint32_t slice = block * kVerifyWaves + threadIdx.x / kWave;
-    exp_table(table);
+    Exp2::fill(table);
+    const Exp2 exp2_of(table);
     Decision d;
     if (FUSED) {
-        decide<kVerifyThreads, kFusedDrafts>(v, seq, table, d);
+        decide<kVerifyThreads, kFusedDrafts>(v, seq, exp2_of, d);
         if (block == 0 && threadIdx.x == 0) v.decisions[seq] = d;
     } else {
         d = v.decisions[seq];
@@ -317,7 +358,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_residual_kernel(VerifyP
     load_slice(terms.draft, slice * kSlice, v.s.vocab, y);
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += terms.term(x[i], y[i], slice * kSlice + slice_at(i), table);
+    for (int i = 0; i < kEach; ++i) sum += terms.term(x[i], y[i], slice * kSlice + slice_at(i), exp2_of);
     sum = wave_sum_f64(sum);
     if (threadIdx.x % kWave == 0) v.slice_sums[static_cast<uint64_t>(seq) * v.slices + slice] = sum;
 }
@@ -360,7 +401,7 @@ __device__ __forceinline__ void first_and_last(bool hit, uint32_t at, bool mass,
 // running sum: the last item with mass is then the one.
 template <bool FUSED>
 __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams v) {
-    __shared__ double table[32];
+    __shared__ uint2 table[32];
     __shared__ uint32_t first_hit, last_mass;
     __shared__ double shared_before;
     const VerifyDraftArgs& s = v.s;
@@ -370,10 +411,11 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams 
     const double my_sum = s.draft && tid < v.slices ? sums[tid] : 0.0;
     const uint32_t my_token = tid < s.drafts ? s.draft_tokens[static_cast<uint64_t>(seq) * s.drafts + tid] : kNoToken;
     const double uniform = s.sample_uniform[seq];
-    exp_table(table);
+    Exp2::fill(table);
+    const Exp2 exp2_of(table);
     Decision d;
     if (FUSED) {
-        decide<kPickThreads, kFusedDrafts>(v, seq, table, d);
+        decide<kPickThreads, kFusedDrafts>(v, seq, exp2_of, d);
     } else {
         d = v.decisions[seq];
         __syncthreads();
@@ -386,7 +428,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams 
     const auto term_of = [&](const Terms& terms, uint32_t slice) {
         const uint32_t at = slice * kSlice + tid;
         if (at >= s.vocab) return 0.0;
-        return terms.term(number_or_none(terms.target[at]), terms.draft ? number_or_none(terms.draft[at]) : 0.0f, at, table);
+        return terms.term(number_or_none(terms.target[at]), terms.draft ? number_or_none(terms.draft[at]) : 0.0f, at, exp2_of);
     };
     // the slice that lost the token that was proposed with certainty
     uint32_t short_slice = kNoToken;
@@ -402,7 +444,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams 
     const auto part = [&](uint32_t i) {
         if (residual && d.rejected && s.draft) return i == tid ? my_sum : sums[i];
         if (residual && i == short_slice) return short_sum;
-        return stats[i].sum * mass(stats[i].top, d.target_top, v.scale, table) * target_scale;
+        return stats[i].sum * mass(stats[i].top, d.target_top, v.scale, exp2_of) * target_scale;
     };
     // slices [begin, end) are this thread's
     const uint32_t each = (v.slices + kPickThreads - 1) / kPickThreads;
@@ -501,7 +543,7 @@ hipError_t launch_verify_draft(hipStream_t stream, const VerifyDraftArgs& s) {
     const VerifyPlan p = verify_plan(s.sequences, s.drafts, s.vocab);
     uint8_t* ws = static_cast<uint8_t*>(s.workspace);
     VerifyParams v{s,
-                   s.inv_temperature * 0x1.71547652b82fep+0,
+                   s.inv_temperature * 0x1.71547652b82fep+5,
                    reinterpret_cast<SliceStat*>(ws),
                    reinterpret_cast<SliceStat*>(ws + p.target_bytes),
                    reinterpret_cast<double*>(ws + p.target_bytes + p.draft_bytes),
