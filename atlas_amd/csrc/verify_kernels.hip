@@ -44,9 +44,9 @@ __device__ __forceinline__ float number_or_none(float x) { return x != x ? -__bu
 // 2^-51 (|y / 32| + 2) of the true value; zero from 2^-1023 down, and of a y that is
 // no number.
 //
-// Its instructions bound the first launch, so it has few (15 and a read; with
-// the library's exp that launch took 120 us, as written in C 105, so NEWFIG):
-// adding 1.5 2^52 leaves the nearest whole number of thirty-seconds in the low
+// Its 64-bit instructions bound the first launch (384 rows of 262144 logits 68
+// us without them), so it has few: with the library's exp that launch took 120
+// us, as plain C 105, so 98.  Adding 1.5 2^52 leaves the nearest whole number of thirty-seconds in the low
 // bits of the sum, with 1023 of them in front; its upper part is added to the
 // exponent of a table entry, whose own is taken out; and the constants stay in
 // registers, one operand of an instruction a scalar one, which the compiler
@@ -177,9 +177,10 @@ __device__ __forceinline__ void load_slice(const float* logits, uint32_t first, 
     }
 }
 
-// A wavefront a slice of a row; rows of a sequence: targets, then drafts.  Its
-// bytes bound it, once the exponentials are short: 384 rows of 262144 logits
-// 105 us, 3.8 TB/s (120 us with the library's exp).
+// A wavefront a slice of a row; rows of a sequence: targets, then drafts.  Bytes
+// and exponentials take as long as each other: 384 rows of 262144 logits 98 us,
+// 4.1 TB/s.  Two to eight slices a wavefront, the next one's logits on their way:
+// 94 to 107 us, and 37 to 56 where one slice takes 34 (640 rows of 50257).
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyParams v) {
     __shared__ uint2 table[32];
     const VerifyDraftArgs& s = v.s;
