@@ -393,7 +393,10 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     // rows of 256 x 512, 64 x 8192 (256 dims), 24 x 1024 with 5 drafts (128), us:
     //   256  40 / 147 / 34    512  47 / 143 / 31    768  51 / 148 / 28
     //   1024  61 / 143 / 30
+    // One sequence behind 100003 rows of 256: 153 us with 32 parts, 87 with 64, 48
+    // with 256.
     const uint32_t wanted = s.head_dim > 128 ? 256 : 768;
+    uint32_t own_wanted = wanted;
     if (s.prefix_length && rows > 16) {
         p.wide = true;
         const uint32_t pad = s.head_dim <= 64 ? 64 : (s.head_dim <= 128 ? 128 : 256);
@@ -421,17 +424,18 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         p.prefix_tiles = static_cast<uint32_t>((rows + 15) / 16);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         const uint32_t most = (s.prefix_length + 63) / 64;
-        const uint64_t want = (wanted + units - 1) / units;
+        // one launch for both: shared by their lengths, so that all of it is at work at once
+        const uint32_t mine = static_cast<uint32_t>(static_cast<uint64_t>(wanted) * s.prefix_length / (static_cast<uint64_t>(s.prefix_length) + s.capacity));
+        own_wanted = wanted - mine;
+        const uint64_t want = mine < units ? 1 : mine / units;
         p.prefix_slots = static_cast<uint32_t>(want < most ? want : most);
-        if (p.prefix_slots > 64) p.prefix_slots = 64;
     }
     if (s.capacity) {
         p.own_tiles = (seq_rows + 15) / 16;
         const uint64_t units = static_cast<uint64_t>(p.own_tiles) * s.kv_heads * s.sequences;
         const uint32_t most = (s.capacity + 63) / 64;
-        const uint64_t want = (wanted + units - 1) / units;
+        const uint64_t want = own_wanted < units ? 1 : (own_wanted + units - 1) / units;
         p.own_slots = static_cast<uint32_t>(want < most ? want : most);
-        if (p.own_slots > 64) p.own_slots = 64;
     }
     const uint64_t lines = rows * s.kv_heads, parts = lines * (p.prefix_slots + p.own_slots);
     p.out_bytes = round256(parts * s.head_dim * 4);

@@ -41,16 +41,16 @@ __device__ __forceinline__ float number_or_none(float x) { return x != x ? -__bu
 // 2^(y / 32), y <= 0, by 2^(j / 32) from a table in LDS and the Taylor
 // polynomial of 2^(r / 32) to the sixth degree, |r| <= 1 / 2: ((r / 32) ln 2)^7 / 7!
 // is below 2^-58.  With the rounding of y and of the products, within
-// 2^-51 (|y / 32| + 2) of the true value; zero from 2^-1023 down, and of a y that is
-// no number.
+// 2^-51 (|y / 32| + 2) of the true value; below 2^-1022 no bits are kept, and from
+// 2^-1023 down, and of a y that is no number, it is zero.
 //
 // Its 64-bit instructions bound the first launch (384 rows of 262144 logits 68
 // us without them), so it has few: with the library's exp that launch took 120
-// us, as plain C 105, so 98.  Adding 1.5 2^52 leaves the nearest whole number of thirty-seconds in the low
-// bits of the sum, with 1023 of them in front; its upper part is added to the
-// exponent of a table entry, whose own is taken out; and the constants stay in
-// registers, one operand of an instruction a scalar one, which the compiler
-// would not hold them in by itself.
+// us, as plain C 105, so 98.  Adding 1.5 2^52 leaves the nearest whole number of
+// thirty-seconds in the low bits of the sum, with 1023 ones more in front; its
+// upper part is added to the exponent of a table entry, whose own is taken out;
+// and the constants stay in registers, one operand of an instruction a scalar
+// one, which the compiler would not hold them in by itself.
 struct Exp2 {
     const uint2* table;
     double first, c[5], shift, least;
