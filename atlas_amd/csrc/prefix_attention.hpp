@@ -47,6 +47,7 @@ __device__ __forceinline__ float sum_xor32(float x) {
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32_a2 __attribute__((aligned(2)));
 typedef u32x2_t u32x2_a2 __attribute__((aligned(2)));
+typedef u32x4_t u32x4_a2 __attribute__((aligned(2)));
 
 // The dims of unit 4 blk + a, j < 8.
 template <int FMT>
@@ -113,6 +114,11 @@ struct TileRows<kKvQ4_0> : QuantTileRows {
         : QuantTileRows(plane, first, rows, row_bytes) {}
 };
 
+// The low four bits of byte i, less 8: bytes convert in one instruction.
+__device__ __forceinline__ float nibble(uint32_t w, int i) {
+    return static_cast<float>((w & 0x0f0f0f0fu) >> (8 * i) & 255u) - 8.0f;
+}
+
 // 8 key dims as stored (unit c = 4 blk + a, the dims of key_dim); offset is
 // the first of them, for a quantised row its block's scale.  codes() leaves
 // the stored numbers and returns what they are times: nothing where the key or
@@ -172,7 +178,7 @@ struct RawKey<kKvQ4_0> {
         uint32_t c0 = c, scale = d;
         asm volatile("" : "+v"(c0), "+v"(scale));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((c0 >> (8 * (j & 3) + 4 * (j >> 2))) & 15u) - 8);
+        for (int j = 0; j < 8; ++j) v[j] = nibble(j < 4 ? c0 : c0 >> 4, j & 3);
         return there ? h2f(static_cast<uint16_t>(scale)) : 0.0f;
     }
 };
@@ -223,7 +229,7 @@ struct RawValue<kKvQ4_0> {
         uint32_t c0 = c, scale = d;
         asm volatile("" : "+v"(c0), "+v"(scale));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(static_cast<int>((c0 >> (8 * (j & 1) + 4 * (j >> 1))) & 15u) - 8);
+        for (int j = 0; j < 4; ++j) v[j] = nibble(j < 2 ? c0 : c0 >> 4, j & 1);
         return there ? h2f(static_cast<uint16_t>(scale)) : 0.0f;
     }
 };

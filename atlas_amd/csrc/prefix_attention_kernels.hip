@@ -40,6 +40,109 @@ __device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const floa
         }
 }
 
+// What a lane of the own rows' kernel holds of a key: NB units of 8 dims,
+// `quarter` of four lanes; and of a value: NG quads, lane n of 16.  Any order of
+// the dims will do that queries and outputs share.  Of f32 rows a load is 16 bytes
+// and neighbouring lanes have neighbouring units; of quantised rows a lane's
+// units are neighbours, so that a few wide loads bring them (by loads of 2 and 4
+// bytes 24 sequences with 5 drafts, Q4_0, took 27 us, so 23).
+template <int FMT, int NB>
+struct KeyRun {
+    static constexpr int kUnit = FMT == kKvQ8_0 ? 8 : 4, kBlock = FMT == kKvQ8_0 ? 34 : 18;  // bytes
+    static constexpr int kBlocks = NB < 4 ? 1 : NB / 4, kWords = NB * kUnit / 4 / kBlocks;    // words of each block
+    uint32_t c[kBlocks][kWords];
+    uint16_t d[kBlocks];
+    static __device__ uint32_t unit(uint32_t quarter, uint32_t b) { return NB * quarter + b; }
+    __device__ __forceinline__ void load(const TileRows<FMT>& t, uint32_t row, uint32_t quarter, uint32_t head_dim) {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+            const uint32_t block = unit(quarter, 0) / 4 + i, off = 32 * block < head_dim ? block * kBlock : 0u;
+            const uint32_t behind = 2 + (NB < 4 ? unit(quarter, 0) % 4 * kUnit : 0);
+            d[i] = t.template at<uint16_t>(row, off, 0);
+            if constexpr (kWords == 2) {
+                const u32x2_a2 w = t.template at<u32x2_a2>(row, off, behind);
+                c[i][0] = w.x;
+                c[i][1] = w.y;
+            } else {
+#pragma unroll
+                for (int k = 0; k < kWords; k += 4) {
+                    const u32x4_a2 w = t.template at<u32x4_a2>(row, off, behind + 4 * k);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) c[i][k + j] = w[j];
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void values(int b, uint32_t quarter, uint32_t head_dim, bool there, float (&v)[8]) const {
+        const int i = b / 4, w = b % 4 * (kUnit / 4);
+        RawKey<FMT> raw;
+        if constexpr (FMT == kKvQ8_0)
+            raw.c = u32x2_t{c[i][w], c[i][w + 1]};
+        else
+            raw.c = c[i][w];
+        raw.d = d[i];
+        raw_values(raw, v, there && 8 * unit(quarter, b) < head_dim);
+    }
+};
+template <int NB>
+struct KeyRun<kKvF32, NB> {
+    RawKey<kKvF32> k[NB];
+    static __device__ uint32_t unit(uint32_t quarter, uint32_t b) { return 4 * b + quarter; }
+    __device__ __forceinline__ void load(const TileRows<kKvF32>& t, uint32_t row, uint32_t quarter, uint32_t head_dim) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint32_t u = unit(quarter, b);
+            const uint32_t off[2] = {RawKey<kKvF32>::offset(u, head_dim, 0), RawKey<kKvF32>::offset(u, head_dim, 1)};
+            k[b].load(t, row, u, off);
+        }
+    }
+    __device__ __forceinline__ void values(int b, uint32_t, uint32_t, bool, float (&v)[8]) const { raw_values(k[b], v, true); }
+};
+template <int FMT, int NG>
+struct ValueRun {
+    static constexpr uint32_t kQuad = FMT == kKvQ8_0 ? 4 : 2, kBlock = FMT == kKvQ8_0 ? 34 : 18;  // bytes
+    static constexpr int kWords = NG * kQuad < 4 ? 1 : NG * kQuad / 4;
+    uint32_t c[kWords];
+    uint16_t d;
+    static __device__ uint32_t quad(uint32_t n, uint32_t g) { return NG * n + g; }
+    __device__ __forceinline__ void load(const TileRows<FMT>& t, uint32_t row, uint32_t n, uint32_t head_dim) {
+        const uint32_t q = quad(n, 0), off = 4 * q < head_dim ? q / 8 * kBlock : 0u, behind = 2 + q % 8 * kQuad;
+        d = t.template at<uint16_t>(row, off, 0);
+        if constexpr (NG * kQuad == 2) {
+            c[0] = t.template at<uint16_t>(row, off, behind);
+        } else if constexpr (kWords == 1) {
+            c[0] = t.template at<u32_a2>(row, off, behind);
+        } else if constexpr (kWords == 2) {
+            const u32x2_a2 w = t.template at<u32x2_a2>(row, off, behind);
+            c[0] = w.x;
+            c[1] = w.y;
+        } else {
+            const u32x4_a2 w = t.template at<u32x4_a2>(row, off, behind);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) c[j] = w[j];
+        }
+    }
+    __device__ __forceinline__ void values(int g, uint32_t n, uint32_t head_dim, bool there, float (&v)[4]) const {
+        RawValue<FMT> raw;
+        if constexpr (FMT == kKvQ8_0)
+            raw.c = c[g];
+        else
+            raw.c = static_cast<uint16_t>(c[g / 2] >> (16 * (g % 2)));
+        raw.d = d;
+        raw_values(raw, v, there && 4 * quad(n, g) < head_dim);
+    }
+};
+template <int NG>
+struct ValueRun<kKvF32, NG> {
+    RawValue<kKvF32> v4[NG];
+    static __device__ uint32_t quad(uint32_t n, uint32_t g) { return 16 * g + n; }
+    __device__ __forceinline__ void load(const TileRows<kKvF32>& t, uint32_t row, uint32_t n, uint32_t head_dim) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) v4[g].load(t, row, quad(n, g), RawValue<kKvF32>::offset(quad(n, g), head_dim));
+    }
+    __device__ __forceinline__ void values(int g, uint32_t, uint32_t, bool, float (&v)[4]) const { raw_values(v4[g], v, true); }
+};
+
 // One workgroup: 16 query rows of one KV head against one segment of a
 // sequence's own rows (or of the prompt, for batches of up to 16 rows).  Its
 // bytes bound it over long caches (64 sequences of up to 8192 rows of 256 dims,
@@ -117,7 +220,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
         const uint32_t at = min(row0 + n, row_end - 1);
         float x[8];
         load_query8<FMT>(a.q + (static_cast<uint64_t>(at / a.group) * a.q_heads + kv_head * a.group + at % a.group) * a.head_dim,
-                         4 * i + quarter, a.head_dim, a.scale, x);
+                         KeyRun<FMT, NB>::unit(quarter, i), a.head_dim, a.scale, x);
         room.queries[2 * i][lane] = f32x4{x[0], x[1], x[2], x[3]};
         room.queries[2 * i + 1][lane] = f32x4{x[4], x[5], x[6], x[7]};
     }
@@ -132,8 +235,8 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
     f32x4 out[NG * 4];
 #pragma unroll
     for (int i = 0; i < NG * 4; ++i) out[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    RawKey<FMT> k[NB];
-    RawValue<FMT> raw_v[4][NG];
+    KeyRun<FMT, NB> k;
+    ValueRun<FMT, NG> raw_v[4];
     const auto rows_of = [&](const uint8_t* plane, uint32_t first) {
         const uint32_t there = first < key_end ? min(key_end - first, 16u) : 0u;
         return TileRows<FMT>(plane, there ? first : key_end - 1, there, a.row_bytes, head_off);
@@ -141,24 +244,16 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
     // offsets are found anew for every tile: kept, they send other numbers to memory
     const auto load_k = [&](uint32_t first) {
         const TileRows<FMT> rows = rows_of(keys, first);
-        uint32_t unit = quarter;
-        asm volatile("" : "+v"(unit));
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const uint32_t off[2] = {RawKey<FMT>::offset(4 * b + unit, a.head_dim, 0), RawKey<FMT>::offset(4 * b + unit, a.head_dim, 1)};
-            k[b].load(rows, n, 4 * b + unit, off);
-        }
+        uint32_t lane4 = quarter;
+        asm volatile("" : "+v"(lane4));
+        k.load(rows, n, lane4, a.head_dim);
     };
     const auto load_v = [&](uint32_t first) {
         const TileRows<FMT> rows = rows_of(values, first);
-        uint32_t quad = n;
-        asm volatile("" : "+v"(quad));
+        uint32_t lane16 = n;
+        asm volatile("" : "+v"(lane16));
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const uint32_t off = RawValue<FMT>::offset(16 * g + quad, a.head_dim);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) raw_v[r][g].load(rows, 4 * quarter + r, 16 * g + quad, off);
-        }
+        for (int r = 0; r < 4; ++r) raw_v[r].load(rows, 4 * quarter + r, lane16, a.head_dim);
     };
     const uint32_t first = key_begin + wave * 16;
     if (first < key_end) {
@@ -172,7 +267,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             float x[8];
-            raw_values(k[b], x, key0 + n < key_end && 32 * b + 8 * quarter < a.head_dim);
+            k.values(b, quarter, a.head_dim, key0 + n < key_end, x);
             const f32x4 q0 = room.queries[2 * b][lane], q1 = room.queries[2 * b + 1][lane];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -191,7 +286,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 float x[4];
-                raw_values(raw_v[r][g], x, key0 + 4 * quarter + r < key_end && 64 * g + 4 * n < a.head_dim);
+                raw_v[r].values(g, n, a.head_dim, key0 + 4 * quarter + r < key_end, x);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[r][4 * g + j] = x[j];
             }
@@ -253,7 +348,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel
     for (int g = 0; g < NG; ++g)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            put_quad<FMT>(room.sums[wave][n], 16 * g + 4 * quarter + i,
+            put_quad<FMT>(room.sums[wave][n], ValueRun<FMT, NG>::quad(4 * quarter + i, g),
                           f32x4{out[4 * g][i], out[4 * g + 1][i], out[4 * g + 2][i], out[4 * g + 3][i]});
     __syncthreads();
     constexpr uint32_t kQuads = kDims / 4;
