@@ -511,10 +511,8 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         if (packed) p.packed_bytes = round256(packed_bytes);
         p.prefix_tiles = static_cast<uint32_t>(packed ? (rows + 127) / 128 : row_tiles);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
-        uint64_t want = units >= 256 ? 1 : 256 / units;  // one workgroup to a CU
-        if (want > most) want = most;
-        if (want > 8) want = want / 8 * 8;
-        p.prefix_slots = static_cast<uint32_t>(want);
+        const uint64_t want = units >= 256 ? 1 : 256 / units;  // one workgroup to a CU
+        p.prefix_slots = static_cast<uint32_t>(want < most ? want : most);
     } else if (s.prefix_length) {
         p.prefix_tiles = static_cast<uint32_t>((rows + 15) / 16);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
