@@ -11,8 +11,6 @@ inline constexpr int kAttnThreads = 256;
 inline constexpr int kAttnWaves = kAttnThreads / kWave;
 inline constexpr float kLog2e = 1.44269504088896340736f;
 
-typedef f32x4 f32x4_b4 __attribute__((aligned(4)));
-
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
 // The maximum over lanes that differ in bit 3 / 4 / 5 of their number.
@@ -64,7 +62,6 @@ __device__ __forceinline__ uint64_t head_offset(uint32_t head, uint32_t head_dim
 
 constexpr uint32_t kNowhere = 0x7ffffff0u;  // a buffer offset past every span: reads as zero
 
-
 // The dims that value quad q (of head_dim / 4) holds, e < 4.
 template <int FMT>
 __device__ __forceinline__ uint32_t quad_dim(uint32_t q, uint32_t e) {
@@ -73,11 +70,12 @@ __device__ __forceinline__ uint32_t quad_dim(uint32_t q, uint32_t e) {
 }
 
 // The rows of a plane that a tile covers, from `first` on: `rows` of them are
-// there (0: none, `first` is then some row that is), and what a lane asks for past them, or past the head's
-// dims (offset kNowhere), is zero.  f32 rows come through a buffer that ends
-// with them.  Quantised rows lie on 2-byte boundaries, where buffer loads of
-// more than 2 bytes have returned zeros inside the buffer: they come by plain
-// loads, from the last row there where there are no more.
+// there (0: none, `first` is then some row that is).  f32 rows come through a
+// buffer that ends with them: what a lane asks for past them, or past the head's
+// dims (offset kNowhere), is zero.  Quantised rows lie on 2-byte boundaries, where
+// buffer loads of more than 2 bytes have returned zeros inside the buffer: they
+// come by plain loads, from the last row or the head's first block where there
+// is nothing, and whoever unpacks them takes nothing of those.
 template <int FMT>
 struct TileRows;
 template <>
