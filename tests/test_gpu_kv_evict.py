@@ -116,6 +116,29 @@ def test_kv_evict_long_cache(rt, in_place):
         check(f"long {kind}", got, exp)
 
 
+@pytest.mark.parametrize("cap", [1024, 1025, 2049, 4096, 8000, 16384, 16385, 32768, 65536, 65537])
+def test_kv_evict_capacities(rt, cap):
+    """Every number of positions a lane of the selection holds, and the first that it reads anew."""
+    say(f"capacity {cap}")
+    r = np.random.default_rng(cap)
+    n = np.asarray([cap, cap - 1, cap // 2 + 3, 1], np.uint32)
+    cache = ref.make_cache(r, "f32", 4 * cap, 4)
+    for kind in ("plain", "ties", "odd"):
+        for budget, recent, in_place in ((cap // 2, cap // 8, True), (cap - 2, 1, False), (3, 3, True)):
+            got, exp = run(rt, "f32", cache, weights_of(r, kind, 4, cap), n, cap, 4, budget, recent, in_place)
+            check(f"{cap} {kind} {budget}", got, exp)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_kv_evict_more_sequences_than_a_launch_moves(rt, in_place):
+    say(f"22001 sequences, in place {in_place}")
+    r = np.random.default_rng(8)
+    n = r.integers(0, 5, 22001, dtype=np.uint32)
+    cache = ref.make_cache(r, "f32", 4 * 22001, 4)
+    got, exp = run(rt, "f32", cache, weights_of(r, "plain", 22001, 4), n, 4, 4, 2, 1, in_place)
+    check("22001 sequences", got, exp)
+
+
 def test_kv_evict_offsets_past_32_bits(rt):
     say("offsets past 32 bits")
     B, cap, width = 3, 1 << 21, 256

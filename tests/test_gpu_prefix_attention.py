@@ -95,6 +95,13 @@ SHAPES = {
     "packed_128": (33, 2, 32, 4, 128, 5441, 5442, 16, [(5 * i) % 17 for i in range(33)]),
     "packed_160": (35, 2, 16, 2, 160, 5441, 5441, 40, [(5 * i) % 41 for i in range(35)]),
     "packed_256": (70, 1, 8, 1, 256, 10915, 11000, 64, [(7 * i) % 65 for i in range(70)]),
+    "widest_rows": (2, 1, 128, 128, 256, 40, 41, 20, [20, 3]),
+    "widest_batch": (18, 1, 128, 128, 256, 40, 41, 3, [i % 4 for i in range(18)]),
+    "one_group": (1, 1, 128, 1, 128, 70, 70, 50, [50]),
+    "prefill": (1, 300, 4, 2, 64, 100, 100, 301, [300]),
+    "one_long_prompt": (1, 1, 8, 1, 256, 30001, 30001, 70, [70]),
+    "one_long_own": (1, 2, 16, 4, 128, 0, 0, 20001, [20001]),
+    "odd_segments": (37, 1, 28, 4, 128, 1500, 1500, 8, [i % 9 for i in range(37)]),
     "long": (2, 1, 8, 1, 256, 9001, 9001, 5000, [4999, 700]),
 }
 
@@ -126,6 +133,18 @@ def test_prefix_attention_matches_float64(rt, shape, fmt):
             tol = (np.expm1(2 * dx) + (P + cap + 32 + T * H) * 2.0 ** -24) * weights + 2.0 ** -23 * (before + weights) + 1e-30
             off = np.abs(w.astype(np.float64) - (before.astype(np.float64) + weights))
             assert (off[there] <= tol[there]).all(), f"{shape} {fmt}: weights off {float((off / tol)[there].max()):.2f} of the bound"
+
+
+def test_more_sequences_than_a_launch_has_rows_of_workgroups(rt):
+    say("70001 sequences")
+    B, D, cap = 70001, 4, 3
+    q, prefix, cache, n = make(2, "f32", B, 1, 1, 1, D, 5, 5, cap, [i % 4 for i in range(B)])
+    exp, weights, bound = ref.attention(q, prefix, 5, cache, n, cap, 1, 0.5, "f32")
+    w = np.full((B, cap), 2.0, f32)
+    got, w_got = run(rt, "f32", q, prefix, 5, cache, n, cap, 1, 0.5, w, w, alias=True)
+    check("70001 sequences", got, exp, bound, 5 + cap, D)
+    # one share of at most 1, off by under 16 roundings of 2^-24 (eight keys, exp2, log2), added to 2
+    assert np.allclose(w_got, w + weights, rtol=2e-6, atol=0)
 
 
 @pytest.mark.parametrize("D", [4, 20, 36, 68, 80, 132, 244])

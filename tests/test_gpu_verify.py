@@ -61,7 +61,8 @@ def make(seed, B, T, V, std=4.0, apart=1.0):
 
 @pytest.mark.parametrize("B,T,V", [(1, 1, 1), (3, 1, 2), (2, 4, 3), (5, 2, 63), (4, 3, 257), (6, 2, 4095), (6, 2, 4096),
                                    (6, 2, 4097), (3, 5, 8193), (40, 3, 1000), (2, 4, 50257), (1, 2, 151936),
-                                   (3, 16, 500), (4, 17, 500), (2, 70, 4097), (1, 3, 300000)])
+                                   (3, 16, 500), (4, 17, 500), (2, 70, 4097), (1, 3, 300000), (2, 1024, 7), (3000, 1, 5),
+                                   (300, 17, 40)])
 @pytest.mark.parametrize("certain", [False, True])
 def test_verify_matches_float64(rt, B, T, V, certain):
     r, target, draft, tokens, lengths, accept, sample = make(B * 31 + V, B, T, V)
