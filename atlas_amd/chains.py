@@ -78,8 +78,8 @@ from .runtime import HipRuntime, rope_tables_gemma4, rope_tables_llama
 
 class LlamaDecodeStep:
     """One decode token of the Llama resident executor at SmolLM2-135M shapes
-    (hidden 576, 9 Q heads, 3 KV heads, head_dim
-    64, FFN 1536, vocab 49152, eps 1e-5, theta 1e4)."""
+    (hidden 576, 9 Q heads, 3 KV heads, head_dim 64, FFN 1536, vocab 49152,
+    eps 1e-5, theta 1e4)."""
 
     def __init__(self, rt: HipRuntime, shape: wl.SmolShape = wl.SmolShape(), layers: int = 30,
                  capacity: int = 128, seed: int = 11):
