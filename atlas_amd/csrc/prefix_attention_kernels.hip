@@ -156,7 +156,7 @@ struct ValueRun<kKvF32, NG> {
 // so P never leaves its registers and a row's statistics are the lane's own.
 // Queries wait in LDS.
 template <int FMT, int NB>
-__global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : 1) void attn_rows_kernel(AttnParams a) {
+__global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : (FMT == kKvF32 ? 1 : 2)) void attn_rows_kernel(AttnParams a) {
     constexpr int NG = (NB + 1) / 2;  // groups of 64 dims
     constexpr uint32_t kDims = 64 * NG, kPitch = kDims + 4;
     static_assert(kAttnWaves * 16 * kPitch * sizeof(float) >= NB * 2 * kWave * sizeof(f32x4), "the queries fit");
@@ -483,14 +483,16 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     AttnPlan p{};
     const uint32_t seq_rows = s.tokens * (s.q_heads / s.kv_heads);
     const uint64_t rows = static_cast<uint64_t>(s.sequences) * seq_rows;
-    // Workgroups that the chip holds: one to a CU above 128 dims, three below.
-    // More parts cost their starts and their joins, fewer leave CUs idle.  Own
-    // rows of 256 x 512, 64 x 8192 (256 dims), 24 x 1024 with 5 drafts (128), us:
+    // Workgroups that the chip holds: three to a CU up to 128 dims (five or four
+    // fit, and take 0 to 20 % longer), above them two of quantised rows (64 x 4096
+    // Q4_0 141 -> 115 us) and one of f32 (two spill: 147 -> 268).  More parts cost
+    // their starts and their joins, fewer leave CUs idle.  Own rows of f32 256 x 512,
+    // 64 x 8192 (256 dims), Q4_0 24 x 1024 with 5 drafts (128), us:
     //   256  40 / 147 / 34    512  47 / 143 / 31    768  51 / 148 / 28
     //   1024  61 / 143 / 30
     // One sequence behind 100003 rows of 256: 153 us with 32 parts, 87 with 64, 48
     // with 256.
-    const uint32_t wanted = s.head_dim > 128 ? 256 : 768;
+    const uint32_t wanted = s.head_dim <= 128 ? 768 : (s.format == kKvF32 ? 256 : 512);
     uint32_t own_wanted = wanted;
     if (s.prefix_length && rows > 16) {
         p.wide = true;
