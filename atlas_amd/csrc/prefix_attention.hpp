@@ -292,6 +292,7 @@ struct AttnParams {
 // The prompt by f16 pieces (prefix_attention_wide.hip), items = prefix_tiles *
 // prefix_slots * kv_heads: 64 rows to a workgroup and tile, or 128 with the
 // prompt packed into `room` (attn_packed_bytes) first.
+inline constexpr uint32_t kMostPromptKeys = 1u << 16;  // of a segment
 hipError_t launch_attn_wide(hipStream_t stream, int format, uint32_t items, const AttnParams& a, void* room);
 uint64_t attn_packed_bytes(uint32_t head_dim, uint32_t kv_heads, uint32_t prefix_length);
 

@@ -479,6 +479,16 @@ struct AttnPlan {
 
 uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
 
+// Segments of `keys` keys for each of `units` workgroups: `want`, or more where a
+// segment's sums would be longer than `longest` keys; `most` at most, and no more
+// than a launch holds (2^22 workgroups of 512 threads).
+uint32_t segments(uint64_t want, uint32_t keys, uint32_t longest, uint32_t most, uint64_t units) {
+    const uint64_t least = (keys + longest - 1) / longest, launch = units < 1u << 22 ? (1u << 22) / units : 1;
+    uint64_t n = want < least ? least : want;
+    n = n < launch ? n : launch;
+    return static_cast<uint32_t>(n < most ? n : most);
+}
+
 AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     AttnPlan p{};
     const uint32_t seq_rows = s.tokens * (s.q_heads / s.kv_heads);
@@ -514,7 +524,7 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         p.prefix_tiles = static_cast<uint32_t>(packed ? (rows + 127) / 128 : row_tiles);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;
         const uint64_t want = units >= 256 ? 1 : 256 / units;  // one workgroup to a CU
-        p.prefix_slots = static_cast<uint32_t>(want < most ? want : most);
+        p.prefix_slots = segments(want, s.prefix_length, kMostPromptKeys, most, units);
     } else if (s.prefix_length) {
         p.prefix_tiles = static_cast<uint32_t>((rows + 15) / 16);
         const uint64_t units = static_cast<uint64_t>(p.prefix_tiles) * s.kv_heads;

@@ -339,7 +339,7 @@ struct WideItem {
 
 // 16 query rows of a wavefront as operands, lane (row n, quarter) holding the
 // dims of units 4 s + quarter, and what they have summed.
-template <int FMT, int D>
+template <int FMT, int D, bool RUNS>
 struct WideRows {
     half8 q_hi[Wide<D>::KS], q_lo[Wide<D>::KS];
     int q_exp;
@@ -347,6 +347,10 @@ struct WideRows {
     // whole numbers; every x <= m + 8 and x + ev <= mv + 8, so a weight
     // 2^(x - m) is at most 2^8 and p' = 2^(x + ev - mv + 6) at most 2^14
     float m, mv, l;
+    // sums of the runs that have ended, if any, relative to the m and mv of then
+    bool ended;
+    f32x4 out_before[Wide<D>::DT];
+    float m_before, mv_before, l_before;
 
     __device__ __forceinline__ WideRows(const AttnParams& a, uint32_t kv_head, uint32_t row, uint32_t quarter) {
         const uint32_t at = min(row, a.rows - 1);
@@ -373,6 +377,38 @@ struct WideRows {
         for (int d = 0; d < Wide<D>::DT; ++d) out[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         m = mv = neg_inf();
         l = 0.0f;
+        ended = false;
+    }
+
+    // The sums so far put aside.  Adding key after key to one f32 rounds every
+    // time, and with keys alike every time the same way: the results of 60001 equal
+    // keys came to 4e-4 too much.  From every 32 keys a lane's l takes one sum of eight
+    // weights and an accumulator three products; so a run of 512 keys rounds 16 and
+    // 48 times, a segment of kMostPromptKeys its runs 128 times: off by 5.2e-6 for
+    // equal keys.  A segment of at most kShort keys is one run (off by 6.8e-6) of a
+    // kernel without RUNS, whose registers and code they lengthen (100003 keys, 64
+    // rows: 51.3 us, without 50.5).
+    static constexpr uint32_t kRun = 512, kShort = 1024;
+    __device__ __forceinline__ void end_run() {
+        join_runs();
+        l_before = l;
+        l = 0.0f;
+        m_before = m;
+        mv_before = mv;
+#pragma unroll
+        for (int d = 0; d < Wide<D>::DT; ++d) {
+            out_before[d] = out[d];
+            out[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        ended = true;
+    }
+    __device__ __forceinline__ void join_runs() {
+        if (!RUNS || __builtin_expect(!ended, 1)) return;
+        const float fade = m_before == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m_before - m);
+        const float fade_v = mv_before == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(mv_before - mv);
+        l += l_before * fade;
+#pragma unroll
+        for (int d = 0; d < Wide<D>::DT; ++d) out[d] += out_before[d] * fade_v;
     }
 
     // Block b of 32 keys: scores to weights, and their values added.  Register
@@ -411,12 +447,13 @@ struct WideRows {
         }
         const float base = m == neg_inf() ? 0.0f : m;
         const int shift = m == neg_inf() ? 0 : static_cast<int>(m - mv) + 6;
+        float w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float w = __builtin_amdgcn_exp2f(s[j] - base);
-            l += w;
-            s[j] = __builtin_ldexpf(w, ev[j / 4][j % 4] + shift);
+            w[j] = __builtin_amdgcn_exp2f(s[j] - base);
+            s[j] = __builtin_ldexpf(w[j], ev[j / 4][j % 4] + shift);
         }
+        l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
         add_values<D>(tile, b, lane, pieces(s, 1.0f), out);
     }
 
@@ -426,6 +463,7 @@ struct WideRows {
     static constexpr uint32_t kPitch = D + 4, kRoom = 8 * kPitch;
     __device__ __forceinline__ void finish(const AttnParams& a, const WideItem& item, uint32_t row0, float* room, uint32_t lane) {
         const uint32_t n = lane % 16, quarter = lane / 16;
+        join_runs();
         const float all = sum_xor32(sum_xor16(l));
         const int back = m == neg_inf() ? 0 : static_cast<int>(mv - m) - 6;
         const uint64_t to = (static_cast<uint64_t>(item.slot) * a.kv_heads + item.kv_head) * a.rows + row0;
@@ -466,7 +504,7 @@ struct WideRows {
 // free.
 constexpr int kWideThreads = 512;
 
-template <int FMT, int D>
+template <int FMT, int D, bool RUNS>
 __global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a) {
     using W = Wide<D>;
     __shared__ WideTile<D> buffers[2];
@@ -515,11 +553,12 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a
     }
     const uint32_t row0 = item.tile * 64 + wave * 16;
     const bool busy = row0 < a.rows;  // the wavefront has rows
-    WideRows<FMT, D> rows(a, item.kv_head, row0 + n, quarter);
+    WideRows<FMT, D, RUNS> rows(a, item.kv_head, row0 + n, quarter);
     
     for (uint32_t first = item.begin; first < end; first += W::KT, buffer ^= 1) {
         __syncthreads();
         if (!busy) continue;
+        if (RUNS && __builtin_expect(first != item.begin && (first - item.begin) % rows.kRun == 0, 0)) rows.end_run();
         const WideTile<D>& tile = buffers[buffer];
         f32x4 scores[W::KT / 16];
 #pragma unroll
@@ -565,7 +604,7 @@ constexpr int kPackedThreads = 512;
 template <int FMT, int D>
 __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnParams a, const WideTile<D>* packed, uint32_t tiles) {
     using W = Wide<D>;
-    static_assert(sizeof(WideTile<D>) >= 8 * WideRows<FMT, D>::kRoom * sizeof(float), "eight wavefronts' rows fit a buffer");
+    static_assert(sizeof(WideTile<D>) >= 8 * WideRows<FMT, D, true>::kRoom * sizeof(float), "eight wavefronts' rows fit a buffer");
     static_assert(sizeof(WideTile<D>) % 1024 == 0, "copied by whole KiB");
     constexpr uint32_t kChunks = sizeof(WideTile<D>) / 1024;
     __shared__ WideTile<D> buffers[2];
@@ -594,7 +633,7 @@ __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnPara
         }
     };
     if (item.begin < end) copy(item.begin, 0);
-    WideRows<FMT, D> rows(a, item.kv_head, row, quarter);
+    WideRows<FMT, D, true> rows(a, item.kv_head, row, quarter);
     uint32_t buffer = 0;
     for (uint32_t first = item.begin; first < end; first += W::KT, buffer ^= 1) {
         // this tile has arrived, and every wavefront is done with the one before
@@ -602,6 +641,7 @@ __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnPara
         __syncthreads();
         if (first + W::KT < end) copy(first + W::KT, buffer ^ 1);
         if (!busy) continue;
+        if (__builtin_expect(first != item.begin && (first - item.begin) % rows.kRun == 0, 0)) rows.end_run();
         const uint32_t left = end - first;
         const WideTile<D>& tile = buffers[buffer];
         f32x4 scores[W::KT / 16];
@@ -618,7 +658,13 @@ __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnPara
 template <int FMT, int D>
 hipError_t launch_wide(hipStream_t stream, uint32_t items, const AttnParams& a, void* room) {
     if (!room) {
-        hipLaunchKernelGGL((attn_wide_kernel<FMT, D>), dim3(WideItem::grid(items)), dim3(kWideThreads), 0, stream, a);
+        const uint32_t tiles = (a.prefix_length + Wide<D>::KT - 1) / Wide<D>::KT;
+        const uint32_t longest = (tiles + a.prefix_slots - 1) / a.prefix_slots * Wide<D>::KT;
+        const dim3 grid(WideItem::grid(items)), block(kWideThreads);
+        if (longest <= WideRows<FMT, D, false>::kShort)
+            hipLaunchKernelGGL((attn_wide_kernel<FMT, D, false>), grid, block, 0, stream, a);
+        else
+            hipLaunchKernelGGL((attn_wide_kernel<FMT, D, true>), grid, block, 0, stream, a);
         return hipGetLastError();
     }
     WideTile<D>* packed = static_cast<WideTile<D>*>(room);

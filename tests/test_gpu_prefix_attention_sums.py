@@ -1,0 +1,69 @@
+"""GPU tests of the shared-prompt attention's sums over many keys that are all
+alike, whose roundings all fall to one side: the result is the one value that
+they hold."""
+import sys
+
+import numpy as np
+import pytest
+
+import decode_refs as ref
+
+pytestmark = pytest.mark.gpu
+f32 = np.float32
+
+
+def say(msg):
+    print(f"[gpu-prefix-sums] {msg}", flush=True)
+    sys.stdout.flush()
+
+
+# Every key alike and every value one number c: the result is c, and each sum adds equal terms.  Values are
+# written by memset: f32 0x3c3c3c3c = 0.0115; a block of Q8_0 or Q4_0 of bytes x has scale f16(0x3c3c) = 1.0586 and
+# codes x.  Batches of as many (head, row tile) units as fill the chip, so that segments are few and long.
+def constant(fmt, byte):
+    if fmt == "f32":
+        return float(np.full(4, byte, np.uint8).view(f32)[0])
+    d = float(np.full(2, byte, np.uint8).view(np.float16)[0])
+    # Q4_0: alternate dims hold the two nibbles; equal ones make one number
+    return d * (float(np.int8(byte)) if fmt == "q8_0" else (byte & 15) - 8)
+
+
+LONG = {  # sequences, heads, KV heads, head_dim, prompt, capacity
+    "prompt": (448, 32, 32, 32, 60001, 0),
+    "prompt_longer": (448, 32, 32, 4, 300001, 0),
+    "prompt_packed": (1024, 32, 32, 32, 60001, 0),
+    "prompt_packed_256": (2048, 16, 16, 256, 40001, 0),
+    "prompt_1024": (448, 32, 32, 32, 1024, 0),
+    "prompt_1025": (448, 32, 32, 32, 1025, 0),
+}
+
+
+@pytest.mark.parametrize("shape", list(LONG))
+@pytest.mark.parametrize("fmt,byte", [("f32", 0x3C), ("f32", 0x3B), ("f32", 0x3A), ("q8_0", 0x3C), ("q4_0", 0x33)])
+def test_long_sums_of_equal_terms(rt, shape, fmt, byte):
+    B, H, KH, D, P, cap = LONG[shape]
+    if fmt != "f32" and D % 32:
+        pytest.skip("quantised rows hold blocks of 32")
+    width = KH * D
+    c = constant(fmt, byte)
+    say(f"{shape} {fmt} {byte:#x}: {c}")
+    rows = max(P, B * cap)
+    nbytes = 2 * rows * ref.row_bytes(fmt, width)
+    data = rt.alloc(nbytes)
+    rt.memset(data, byte, nbytes)
+    # rows' scores differ, so that their weights, 2^(x - a whole number) in the prompt's kernels, take many values
+    r = np.random.default_rng(9)
+    q = np.repeat(r.uniform(0.0, 1.0, (B, 1, H, 1)), D, -1).astype(f32)
+    scale = float(f32(2.0 / (abs(c) * D)))
+    dq, out, n = rt.upload(q), rt.empty(q.size), rt.upload(np.full(B, cap, np.uint32))
+    size = rt.prefix_attention_workspace(fmt, B, 1, H, KH, D, P, cap, False)
+    ws = rt.alloc(size)
+    rt.prefix_attention(fmt, dq, data if P else None, P, P, data if cap else None, n if cap else None, cap, out, None, None,
+                        B, 1, H, KH, D, scale, ws, size)
+    rt.sync()
+    got = out.download(q.size).astype(np.float64)
+    for b in (data, dq, out, n, ws):
+        rt.free(b)
+    worst = float(np.abs(got / c - 1).max())
+    say(f"{shape} {fmt} {byte:#x}: off by {worst:.2e}")
+    assert worst <= 1e-5
