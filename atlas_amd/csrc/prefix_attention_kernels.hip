@@ -18,11 +18,14 @@
 namespace atlas {
 namespace {
 
-// out += the products of the keys that a row sees, key by key: for the tiles
-// where a key that only some rows see holds values that are no numbers.
+// The blocks of dims whose products with 16 keys are summed at once.
+constexpr int kAtOnce = 4;
+
+// sum += the products of the keys that a row sees, key by key, from block `block` on: for
+// the tiles where a key that only some rows see holds values that are no numbers.
 template <int NG>
-__device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const float (&p)[4], uint32_t key0, uint32_t seen,
-                                      f32x4 (&out)[NG * 4]) {
+__device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const float (&p)[4], int block, uint32_t key0,
+                                         uint32_t seen, f32x4 (&sum)[kAtOnce]) {
     const uint32_t lane = threadIdx.x % kWave, n = lane % 16, quarter = lane / 16;
     for (uint32_t from = 0; from < 4; ++from)
 #pragma unroll
@@ -30,11 +33,11 @@ __device__ __forceinline__ void add_seen(const float (&v)[4][NG * 4], const floa
             const bool sees = key0 + 4 * from + r < seen;
             const float weight = __shfl(p[r], static_cast<int>(n + 16 * from), kWave);
 #pragma unroll
-            for (int g = 0; g < NG * 4; ++g)
+            for (int g = 0; g < kAtOnce; ++g)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = __shfl(v[r][g], static_cast<int>(4 * quarter + i + 16 * from), kWave);
-                    out[g][i] = sees ? out[g][i] + weight * x : out[g][i];
+                    const float x = __shfl(v[r][block + g], static_cast<int>(4 * quarter + i + 16 * from), kWave);
+                    sum[g][i] = sees ? sum[g][i] + weight * x : sum[g][i];
                     __builtin_amdgcn_sched_barrier(0);
                 }
         }
@@ -323,18 +326,24 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : (FMT == kKvF32 ? 1 : 2))
         }
         const float base = m == neg_inf() ? 0.0f : m;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(p[r] - base);
-            l += p[r];
-        }
-        if (stained) {
-            add_seen<NG>(v, p, key0, seen, out);
-        } else {
+        for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(p[r] - base);
+        // One rounding of the long sums for every 16 keys, not one a key: with keys
+        // alike they all fall to one side (40001 keys a segment 1.4e-4).
+        l += (p[0] + p[1]) + (p[2] + p[3]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+        for (int block = 0; block < NG * 4; block += kAtOnce) {
+            f32x4 sixteen[kAtOnce] = {};
+            if (stained) {
+                add_seen<NG>(v, p, block, key0, seen, sixteen);
+            } else {
 #pragma unroll
-                for (int i = 0; i < NG * 4; ++i)
-                    out[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][i], p[r], out[i], 0, 0, 0);
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i)
+                        sixteen[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][block + i], p[r], sixteen[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) out[block + i] += sixteen[i];
         }
         __builtin_amdgcn_sched_barrier(0);
         load_v(next);
@@ -479,6 +488,9 @@ struct AttnPlan {
 
 uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
 
+// Keys of a segment of attn_rows_kernel: 128 roundings of a wavefront's sums.
+constexpr uint32_t kMostRowKeys = 8192;
+
 // Segments of `keys` keys for each of `units` workgroups: `want`, or more where a
 // segment's sums would be longer than `longest` keys; `most` at most, and no more
 // than a launch holds (2^22 workgroups of 512 threads).
@@ -532,15 +544,14 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
         // one launch for both: shared by their lengths, so that all of it is at work at once
         const uint32_t mine = static_cast<uint32_t>(static_cast<uint64_t>(wanted) * s.prefix_length / (static_cast<uint64_t>(s.prefix_length) + s.capacity));
         own_wanted = wanted - mine;
-        const uint64_t want = mine < units ? 1 : mine / units;
-        p.prefix_slots = static_cast<uint32_t>(want < most ? want : most);
+        p.prefix_slots = segments(mine < units ? 1 : mine / units, s.prefix_length, kMostRowKeys, most, units);
     }
     if (s.capacity) {
         p.own_tiles = (seq_rows + 15) / 16;
         const uint64_t units = static_cast<uint64_t>(p.own_tiles) * s.kv_heads * s.sequences;
         const uint32_t most = (s.capacity + 63) / 64;
         const uint64_t want = own_wanted < units ? 1 : (own_wanted + units - 1) / units;
-        p.own_slots = static_cast<uint32_t>(want < most ? want : most);
+        p.own_slots = segments(want, s.capacity, kMostRowKeys, most, units);
     }
     const uint64_t lines = rows * s.kv_heads, parts = lines * (p.prefix_slots + p.own_slots);
     p.out_bytes = round256(parts * s.head_dim * 4);

@@ -35,6 +35,11 @@ LONG = {  # sequences, heads, KV heads, head_dim, prompt, capacity
     "prompt_packed_256": (2048, 16, 16, 256, 40001, 0),
     "prompt_1024": (448, 32, 32, 32, 1024, 0),
     "prompt_1025": (448, 32, 32, 32, 1025, 0),
+    "prompt_few_rows": (1, 1, 1, 32, 3000001, 0),
+    "own": (768, 1, 1, 32, 0, 40001),
+    "own_128": (256, 1, 1, 128, 0, 40001),
+    "own_256": (256, 1, 1, 256, 0, 30001),
+    "own_longer": (8, 1, 1, 32, 0, 3000001),
 }
 
 
