@@ -408,24 +408,25 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, f
     const uint32_t dim = 4 * (blockIdx.y * LANES + lane);
     const bool holds = dim < a.head_dim;
     const float* parts = a.partial_out + row * a.head_dim + (holds ? dim : 0);
-    float sum = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    // in 64 bits: a cache of 2^29 positions has 65536 segments
+    double all_l = 0.0, all_o[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll 4
     for (uint32_t s = group; s < slots; s += kGroups) {
         const float2 x = ml[s * all];
         const f32x4 part = *reinterpret_cast<const f32x4*>(parts + s * all * a.head_dim);
         const float f = __builtin_amdgcn_exp2f(x.x - base);
-        sum += f * x.y;
+        all_l += static_cast<double>(f * x.y);
         // an empty segment has left what was there
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] += x.x == neg_inf() ? 0.0f : f * part[j];
+        for (int j = 0; j < 4; ++j) all_o[j] += static_cast<double>(x.x == neg_inf() ? 0.0f : f * part[j]);
     }
-    sums[group][lane] = o;
-    if (lane == 0) group_l[group] = sum;
+    sums[group][lane] = f32x4{static_cast<float>(all_o[0]), static_cast<float>(all_o[1]), static_cast<float>(all_o[2]),
+                              static_cast<float>(all_o[3])};
+    if (lane == 0) group_l[group] = static_cast<float>(all_l);
     __syncthreads();
     if (group) return;
-    sum = 0.0f;
-    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (uint32_t g = 0; g < kGroups; ++g) {
         sum += group_l[g];

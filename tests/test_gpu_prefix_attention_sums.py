@@ -40,6 +40,7 @@ LONG = {  # sequences, heads, KV heads, head_dim, prompt, capacity
     "own_128": (256, 1, 1, 128, 0, 40001),
     "own_256": (256, 1, 1, 256, 0, 30001),
     "own_longer": (8, 1, 1, 32, 0, 3000001),
+    "own_longest": (1, 1, 1, 4, 0, 1 << 29),
 }
 
 
