@@ -11,9 +11,10 @@
 // magnitude in [2^14, 2^15) (the exponents are added back to the score), and
 // each value row likewise, v' = v 2^{-ev}.  A weight 2^{x - m} (m about the
 // row's largest x) takes its value row's exponent before it is split,
-// p' = 2^{x - m} 2^{ev + m - m'} with m' about the row's largest x + ev, so
-// that sum 2^x v = 2^{m'} sum p' v' keeps every row's precision whatever the
-// rows' scales.  m and m' are whole numbers: all these factors are exact.
+// p' = 2^{x - m} 2^{ev - m'} with m' about the row's largest x - m + ev, so
+// that sum 2^{x - m} v = 2^{m'} sum p' v' keeps every row's precision whatever the
+// rows' scales (but a weight below 2^-126, which f32 does not hold, is zero).
+// m and m' are whole numbers: all these factors are exact.
 //
 // A workgroup walks one segment in tiles of KT keys: the tile's rows come from
 // the cache as they are stored and are converted once, into the fragments that
@@ -344,9 +345,13 @@ struct WideRows {
     half8 q_hi[Wide<D>::KS], q_lo[Wide<D>::KS];
     int q_exp;
     f32x4 out[Wide<D>::DT];
-    // whole numbers; every x <= m + 8 and x + ev <= mv + 8, so a weight
-    // 2^(x - m) is at most 2^8 and p' = 2^(x + ev - mv + 6) at most 2^14
+    // Whole numbers; every x <= m + 8 and x - m + ev <= mv + 8, so a weight
+    // 2^(x - m) is at most 2^8 and p' = 2^(x - m + ev - mv + 6) at most 2^14.  mv is
+    // counted from m: a score may be so large that its neighbours lie further
+    // apart than the exponents of values.
     float m, mv, l;
+    // below it a result is zero, whatever the values
+    static constexpr float kLeast = -200.0f;
     // sums of the runs that have ended, if any, relative to the m and mv of then
     bool ended;
     f32x4 out_before[Wide<D>::DT];
@@ -375,7 +380,8 @@ struct WideRows {
         }
 #pragma unroll
         for (int d = 0; d < Wide<D>::DT; ++d) out[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        m = mv = neg_inf();
+        m = -0x1.fffffep127f;  // the least number, so that differences of m are never NaN
+        mv = kLeast;
         l = 0.0f;
         ended = false;
     }
@@ -404,8 +410,8 @@ struct WideRows {
     }
     __device__ __forceinline__ void join_runs() {
         if (!RUNS || __builtin_expect(!ended, 1)) return;
-        const float fade = m_before == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m_before - m);
-        const float fade_v = mv_before == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(mv_before - mv);
+        const float down = m_before - m;
+        const float fade = __builtin_amdgcn_exp2f(down), fade_v = __builtin_amdgcn_exp2f(down + (mv_before - mv));
         l += l_before * fade;
 #pragma unroll
         for (int d = 0; d < Wide<D>::DT; ++d) out[d] += out_before[d] * fade_v;
@@ -418,43 +424,58 @@ struct WideRows {
                                         uint32_t lane) {
         const uint32_t quarter = lane / 16;
         float s[8];
+        f32x4 evf[2];
         i32x4 ev[2];
-        float top = neg_inf(), top_v = neg_inf();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const uint32_t key = 32 * b + 16 * t + 4 * quarter;
-            const f32x4 evf = *reinterpret_cast<const f32x4*>(&tile.value_expf[key]);
+            evf[t] = *reinterpret_cast<const f32x4*>(&tile.value_expf[key]);
             ev[t] = *reinterpret_cast<const i32x4*>(&tile.value_exp[key]);
+        }
+        const auto score = [&](int j) {
+            const float x = j < 4 ? s0[j] : s1[j - 4];
+            return left < Wide<D>::KT && 32 * b + 16 * (j / 4) + 4 * quarter + j % 4 >= left ? neg_inf() : x;
+        };
+        float top = neg_inf(), top_v = neg_inf();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float x = t ? s1[j] : s0[j];
-                if (left < Wide<D>::KT) x = key + j < left ? x : neg_inf();
-                s[4 * t + j] = x;
-                top = fmaxf(top, x);
-                top_v = fmaxf(top_v, x + evf[j]);
-            }
+        for (int j = 0; j < 8; ++j) {
+            s[j] = score(j) - m;
+            top = fmaxf(top, s[j]);
+            top_v = fmaxf(top_v, s[j] + evf[j / 4][j % 4]);
         }
         top = max_xor32(max_xor16(top));
         top_v = max_xor32(max_xor16(top_v));
-        if (__builtin_amdgcn_ballot_w64(top > m + 8.0f || top_v > mv + 8.0f) != 0) {
-            const float m_new = fmaxf(m, __builtin_ceilf(top)), mv_new = fmaxf(mv, __builtin_ceilf(top_v));
-            l *= m == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-            const float fade = mv == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(mv - mv_new);
-            m = m_new;
-            mv = mv_new;
-#pragma unroll
-            for (int d = 0; d < Wide<D>::DT; ++d) out[d] *= fade;
-        }
-        const float base = m == neg_inf() ? 0.0f : m;
-        const int shift = m == neg_inf() ? 0 : static_cast<int>(m - mv) + 6;
+        if (__builtin_amdgcn_ballot_w64(top > 8.0f || top_v > mv + 8.0f) != 0) raise(score, evf, s);
+        const int shift = 6 - static_cast<int>(mv);
         float w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            w[j] = __builtin_amdgcn_exp2f(s[j] - base);
+            w[j] = __builtin_amdgcn_exp2f(s[j]);
             s[j] = __builtin_ldexpf(w[j], ev[j / 4][j % 4] + shift);
         }
         l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
         add_values<D>(tile, b, lane, pieces(s, 1.0f), out);
+    }
+
+    // New m and mv, and the differences from the scores again.
+    template <class Score>
+    __device__ __forceinline__ void raise(const Score& score, const f32x4 (&evf)[2], float (&s)[8]) {
+        float top = neg_inf(), top_v = neg_inf();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, score(j));
+        const float m_new = fmaxf(m, __builtin_ceilf(max_xor32(max_xor16(top)))), down = m - m_new;
+        m = m_new;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            s[j] = score(j) - m;
+            top_v = fmaxf(top_v, s[j] + evf[j / 4][j % 4]);
+        }
+        const float mv_new = fmaxf(fmaxf(mv + down, __builtin_ceilf(max_xor32(max_xor16(top_v)))), kLeast);
+        const float fade = __builtin_amdgcn_exp2f(mv + down - mv_new);
+        l *= __builtin_amdgcn_exp2f(down);
+        mv = mv_new;
+#pragma unroll
+        for (int d = 0; d < Wide<D>::DT; ++d) out[d] *= fade;
     }
 
     // The segment's sums, relative to 2^m, by way of LDS (`room` of the
@@ -465,7 +486,7 @@ struct WideRows {
         const uint32_t n = lane % 16, quarter = lane / 16;
         join_runs();
         const float all = sum_xor32(sum_xor16(l));
-        const int back = m == neg_inf() ? 0 : static_cast<int>(mv - m) - 6;
+        const int back = static_cast<int>(mv) - 6;
         const uint64_t to = (static_cast<uint64_t>(item.slot) * a.kv_heads + item.kv_head) * a.rows + row0;
         if (quarter == 0 && row0 + n < a.rows) a.partial_ml[to + n] = make_float2(m, all);
 #pragma unroll

@@ -1,0 +1,56 @@
+"""GPU tests of the shared-prompt attention where finite inputs lie far from
+those of a model, against float64."""
+import sys
+
+import numpy as np
+import pytest
+
+import decode_refs as ref
+from test_gpu_prefix_attention import check, run
+
+pytestmark = pytest.mark.gpu
+f32 = np.float32
+
+
+def say(msg):
+    print(f"[gpu-prefix-range] {msg}", flush=True)
+    sys.stdout.flush()
+
+
+# sequences of 8 heads, prompt, head_dim: f32 products throughout, f16 pieces, f16 pieces of a packed prompt
+PATHS = {"few_rows": (1, 300, 128), "many_rows": (40, 300, 128), "packed": (70, 10915, 256)}
+
+
+def one_dim(B, P, D, cap, seed, value):
+    """A batch whose scores lie in dim 0 alone: q (dim 0 zero), prompt and own keys zero, values about N(0, value)."""
+    r = np.random.default_rng(seed)
+    q = np.zeros((B, 1, 8, D), f32)
+    prefix, cache = np.zeros((2, P, D), f32), np.zeros((2, B * cap, D), f32)
+    prefix[1] = r.standard_normal((P, D)) * value
+    cache[1] = r.standard_normal((B * cap, D)) * value
+    n = np.asarray([cap - i % (cap + 1) for i in range(B)], np.uint32)
+    return q, prefix, cache, n
+
+
+def as_bytes(a):
+    return a.view(np.uint8).reshape(*a.shape[:-1], -1)
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+@pytest.mark.parametrize("value", [1e-6, 1e-2, 1e3])
+@pytest.mark.parametrize("e", [10, 24, 27, 28, 29, 31, 100])
+def test_scores_of_any_size(rt, path, value, e):
+    """Keys alike but one or three, whose scores are the only large ones, or the only small ones: every weight is 1, a
+    third, or nothing, whatever the scores' spacing.  (Equal keys have equal scores: only the sums round.)"""
+    B, P, D = PATHS[path]
+    say(f"{path}, values {value}, scores of 2^{e}")
+    q, prefix, cache, n = one_dim(B, P, D, 8, 3, value)
+    q[..., 0] = 2.0 ** (e / 2)
+    hot = [P // 3, P // 2, P - 1]
+    for which, sign in (([P // 3], 1), (hot, 1), (hot, -1), (range(P), 1)):
+        prefix[0] = 0.0
+        prefix[0, list(which), 0] = sign * 2.0 ** (e / 2)
+        exp, _, bound = ref.attention(q, as_bytes(prefix), P, as_bytes(cache), n, 8, 1, 1.0, "f32")
+        got, _ = run(rt, "f32", q, as_bytes(prefix), P, as_bytes(cache), n, 8, 1, 1.0)
+        # the weights are exact, so the bound has no part of the scores' rounding
+        check(f"{path} {value} 2^{e} {len(list(which))} {sign}", got, exp, (bound[0], np.zeros_like(bound[1])), P + 8, D)
