@@ -212,8 +212,10 @@ __device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTi
     if (quad < 8) {
         const uint32_t key = key0 + 16 * (quad / 4) + quad % 4;
         const int e = row_exponent(m, 76);
-        tile.value_exp[key] = e;
-        tile.value_expf[key] = static_cast<float>(e);
+        // a row of zeros raises no m', or it could leave the other rows no bits
+        const bool zeros = m == 0.0f;
+        tile.value_exp[key] = zeros ? -1000 : e;
+        tile.value_expf[key] = zeros ? neg_inf() : static_cast<float>(e);
         // an infinity would leave the row's other values no bits: NaN, not a wrong number
         tile.value_scale[key] = m == __builtin_inff() ? __builtin_nanf("") : pow2i(-e);
     }

@@ -54,3 +54,20 @@ def test_scores_of_any_size(rt, path, value, e):
         got, _ = run(rt, "f32", q, as_bytes(prefix), P, as_bytes(cache), n, 8, 1, 1.0)
         # the weights are exact, so the bound has no part of the scores' rounding
         check(f"{path} {value} 2^{e} {len(list(which))} {sign}", got, exp, (bound[0], np.zeros_like(bound[1])), P + 8, D)
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+@pytest.mark.parametrize("score", [20.0, 60.0, 75.0])
+def test_a_row_of_zeros_that_draws_all_attention(rt, path, score):
+    """What the other rows add is small and keeps its bits.  (Scores in dim 0, 75 = 108 in base 2 and exact but for the
+    factor log2 e: 2^-24 of 108 moves a weight by 4.5e-6.)"""
+    B, P, D = PATHS[path]
+    say(f"{path}, score {score}")
+    q, prefix, cache, n = one_dim(B, P, D, 8, 5, 1.0)
+    q[..., 0] = 1.0
+    prefix[0, P // 2, 0] = score
+    prefix[1, P // 2] = 0.0
+    cache[1] = 0.0
+    exp, _, bound = ref.attention(q, as_bytes(prefix), P, as_bytes(cache), n, 8, 1, 1.0, "f32")
+    got, _ = run(rt, "f32", q, as_bytes(prefix), P, as_bytes(cache), n, 8, 1, 1.0)
+    check(f"{path} zeros {score}", got, exp, bound, P + 8, D)
