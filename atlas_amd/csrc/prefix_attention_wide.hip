@@ -46,10 +46,11 @@ __device__ __forceinline__ void wave_lds_fence() {
 }
 
 // The exponent e that brings a row of largest magnitude `top` to
-// [2^14, 2^15) as x 2^-e; rows below 2^-low are taken as 2^-low.
-__device__ __forceinline__ int row_exponent(float top, int low) {
+// [2^14, 2^15) as x 2^-e; rows below 2^-112, whose 2^-e f32 does not hold, only to
+// 1 and more, where the pieces have their 22 bits too.
+__device__ __forceinline__ int row_exponent(float top) {
     const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-    return (e < -low ? -low : e) - 14;
+    return (e < -112 ? -112 : e) - 14;
 }
 
 // x times[i] as two f16 vectors, where the product is exact in f32: each piece
@@ -169,7 +170,7 @@ __device__ __forceinline__ void convert_keys(const RawKeys<FMT, D>& raw, WideTil
             }
         }
         top = max_xor32(max_xor16(max_xor8(top)));
-        const int e = row_exponent(top, 100);
+        const int e = row_exponent(top);
         const float scale = pow2i(-e);
         if (lane < 8) tile.key_exp[key] = e;
 #pragma unroll
@@ -211,7 +212,7 @@ __device__ __forceinline__ void convert_values(const RawValues<FMT>& raw, WideTi
     if (kQuads >= 64) m = max_xor32(m);
     if (quad < 8) {
         const uint32_t key = key0 + 16 * (quad / 4) + quad % 4;
-        const int e = row_exponent(m, 76);
+        const int e = row_exponent(m);
         // a row of zeros raises no m', or it could leave the other rows no bits
         const bool zeros = m == 0.0f;
         tile.value_exp[key] = zeros ? -1000 : e;
@@ -372,7 +373,7 @@ struct WideRows {
             for (int j = 0; j < 8; ++j) top = max_mag(top, x[s][j]);
         }
         top = max_xor32(max_xor16(top));
-        q_exp = row_exponent(top, 100);
+        q_exp = row_exponent(top);
         const float scale = pow2i(-q_exp);
 #pragma unroll
         for (int s = 0; s < Wide<D>::KS; ++s) {

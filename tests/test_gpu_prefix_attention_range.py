@@ -71,3 +71,17 @@ def test_a_row_of_zeros_that_draws_all_attention(rt, path, score):
     exp, _, bound = ref.attention(q, as_bytes(prefix), P, as_bytes(cache), n, 8, 1, 1.0, "f32")
     got, _ = run(rt, "f32", q, as_bytes(prefix), P, as_bytes(cache), n, 8, 1, 1.0)
     check(f"{path} zeros {score}", got, exp, bound, P + 8, D)
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+@pytest.mark.parametrize("q_exp,k_exp,v_exp", [(0, 0, -100), (0, 0, -106), (116, -118, 0), (-118, 116, 0), (110, -112, -100)])
+def test_operands_at_the_ends_of_the_range(rt, path, q_exp, k_exp, v_exp):
+    B, P, D = PATHS[path]
+    say(f"{path}, q 2^{q_exp} k 2^{k_exp} v 2^{v_exp}")
+    r = np.random.default_rng(7)
+    q = np.ldexp(r.standard_normal((B, 1, 8, D)), q_exp).astype(f32)
+    prefix = np.stack([np.ldexp(r.standard_normal((P, D)), k_exp), np.ldexp(r.standard_normal((P, D)), v_exp)]).astype(f32)
+    n = np.zeros(B, np.uint32)
+    exp, _, bound = ref.attention(q, as_bytes(prefix), P, None, n, 0, 1, 0.25, "f32")
+    got, _ = run(rt, "f32", q, as_bytes(prefix), P, None, n, 0, 1, 0.25)
+    check(f"{path} {q_exp} {k_exp} {v_exp}", got, exp, bound, P, D)
