@@ -382,13 +382,15 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : (FMT == kKvF32 ? 1 : 2))
     }
 }
 
-// One workgroup a row, or 4 LANES dims of one: its segments joined, and the
-// base-2 logarithm of its sum (+inf where it saw nothing) for the weights.
+// One workgroup a row, or 4 LANES dims of one: its segments joined, and for the
+// weights its maximum and 1 / sum (0 where it saw nothing), apart: beside a large
+// maximum the sum's logarithm has few bits (three equal keys with scores of 2^10
+// had weights of 0.33337).
 // LANES lanes hold a segment's dims; as many segments as fit the workgroup are
 // taken at once, and their sums meet in LDS in the segments' order.  Bound by
 // the segments' bytes: 2048 rows of 256 dims with 17 of them 11 us, 3.3 TB/s.
 template <int LANES>
-__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, float* output, float* log_sum) {
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, float* output, float2* shares) {
     constexpr uint32_t kGroups = kAttnThreads / LANES;
     __shared__ float wave_top[kAttnWaves];
     __shared__ f32x4 sums[kGroups][LANES];
@@ -440,20 +442,21 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, f
         float* p = output + (static_cast<uint64_t>(r / a.group) * a.q_heads + kv_head * a.group + r % a.group) * a.head_dim;
         *reinterpret_cast<f32x4*>(p + dim) = y;
     }
-    if (log_sum && dim == 0) {
+    if (shares && dim == 0) {
         const uint64_t seq = r / a.seq_rows;
-        log_sum[(seq * a.kv_heads + kv_head) * a.seq_rows + r % a.seq_rows] =
-            sum == 0.0f ? __builtin_inff() : base + __builtin_log2f(sum);
+        shares[(seq * a.kv_heads + kv_head) * a.seq_rows + r % a.seq_rows] = make_float2(base, sum == 0.0f ? 0.0f : 1.0f / sum);
     }
 }
 
 // A lane a position: the weight it got from every row of its sequence.  A
 // workgroup's wavefronts take a quarter of the rows each, in row order, and
 // their sums meet in order (64 sequences of up to 8192 positions and 8 rows: 9 us).
-__global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a, const float* log_sum, const float* in,
+__global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a, const float2* shares, const float* in,
                                                                     float* out) {
     __shared__ float sums[kAttnWaves][kWave];
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t lane = threadIdx.x % kWave;
+    // known to be one for the wavefront, so that its rows' shares are scalar loads
+    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
     const uint32_t key = blockIdx.x * kWave + lane;
     const uint32_t lines = a.kv_heads * a.seq_rows, part = (lines + kAttnWaves - 1) / kAttnWaves;
     const uint32_t begin = min(wave * part, lines), end = min(begin + part, lines);
@@ -461,12 +464,22 @@ __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a
     for (uint32_t seq = blockIdx.y; seq < a.rows / a.seq_rows; seq += gridDim.y) {
         const uint32_t length = min(a.lengths[seq], a.capacity);
         if (blockIdx.x * kWave >= length) continue;
-        const float* logs = log_sum + static_cast<uint64_t>(seq) * lines;
+        const float2* share = shares + static_cast<uint64_t>(seq) * lines;
         const float* scores = a.scores + static_cast<uint64_t>(seq) * lines * a.score_pitch + min(key, length - 1);
         float sum = 0.0f;
-#pragma unroll 8
-        for (uint32_t i = begin; i < end; ++i)
-            sum += __builtin_amdgcn_exp2f(scores[static_cast<uint64_t>(i) * a.score_pitch] - logs[i]);
+        for (uint32_t i0 = begin; i0 < end; i0 += 4) {
+            // four rows' loads on their way, of the last row again where there are fewer
+            float x[4];
+            float2 of[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t line = min(i0 + i, end - 1);
+                x[i] = scores[static_cast<uint64_t>(line) * a.score_pitch];
+                of[i] = share[line];
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) sum += i0 + i < end ? __builtin_amdgcn_exp2f(x[i] - of[i].x) * of[i].y : 0.0f;
+        }
         sums[wave][lane] = sum;
         __syncthreads();
         if (wave == 0 && key < length) {
@@ -482,9 +495,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a
 struct AttnPlan {
     bool wide;           // the prompt goes by f16 pieces, not with the own rows
     uint32_t prefix_tiles, prefix_slots, own_tiles, own_slots;
-    uint64_t out_bytes, ml_bytes, score_bytes, log_bytes, packed_bytes;
+    uint64_t out_bytes, ml_bytes, score_bytes, share_bytes, packed_bytes;
     uint32_t score_pitch;
-    uint64_t total() const { return out_bytes + ml_bytes + score_bytes + log_bytes + packed_bytes; }
+    uint64_t total() const { return out_bytes + ml_bytes + score_bytes + share_bytes + packed_bytes; }
 };
 
 uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
@@ -560,7 +573,7 @@ AttnPlan attn_plan(const PrefixAttentionArgs& s) {
     if (s.weights_out) {
         p.score_pitch = (s.capacity + 3) / 4 * 4;
         p.score_bytes = round256(lines * p.score_pitch * 4);
-        p.log_bytes = round256(lines * 4);
+        p.share_bytes = round256(lines * sizeof(float2));
     }
     return p;
 }
@@ -595,7 +608,7 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
     a.partial_out = reinterpret_cast<float*>(ws);
     a.partial_ml = reinterpret_cast<float2*>(ws + p.out_bytes);
     a.scores = s.weights_out ? reinterpret_cast<float*>(ws + p.out_bytes + p.ml_bytes) : nullptr;
-    float* log_sum = s.weights_out ? reinterpret_cast<float*>(ws + p.out_bytes + p.ml_bytes + p.score_bytes) : nullptr;
+    float2* shares = s.weights_out ? reinterpret_cast<float2*>(ws + p.out_bytes + p.ml_bytes + p.score_bytes) : nullptr;
     const uint32_t width = s.kv_heads * s.head_dim;
     a.row_bytes = s.format == kKvF32 ? width * 4 : width / 32 * (s.format == kKvQ8_0 ? 34 : 18);
     a.prefix_plane = static_cast<uint64_t>(s.prefix_capacity) * a.row_bytes;
@@ -619,7 +632,7 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
     if (!p.wide) a.prefix_items = prefix_items;
     const uint32_t items = a.prefix_items + s.sequences * s.kv_heads * p.own_slots * p.own_tiles;
     hipError_t e = hipSuccess;
-    void* packed = p.packed_bytes ? ws + p.out_bytes + p.ml_bytes + p.score_bytes + p.log_bytes : nullptr;
+    void* packed = p.packed_bytes ? ws + p.out_bytes + p.ml_bytes + p.score_bytes + p.share_bytes : nullptr;
     if (p.wide && (e = launch_attn_wide(stream, s.format, prefix_items, a, packed)) != hipSuccess) return e;
     if (items) {
         if (s.format == kKvF32)
@@ -636,15 +649,15 @@ hipError_t launch_prefix_attention(hipStream_t stream, const PrefixAttentionArgs
     const uint32_t pieces = all < 512 ? (s.head_dim + 63) / 64 : 1;
     const dim3 join_grid(static_cast<uint32_t>(all), pieces), join_block(kAttnThreads);
     if (s.head_dim <= 64 * pieces)
-        hipLaunchKernelGGL(attn_join_kernel<16>, join_grid, join_block, 0, stream, a, s.output, log_sum);
+        hipLaunchKernelGGL(attn_join_kernel<16>, join_grid, join_block, 0, stream, a, s.output, shares);
     else if (s.head_dim <= 128)
-        hipLaunchKernelGGL(attn_join_kernel<32>, join_grid, join_block, 0, stream, a, s.output, log_sum);
+        hipLaunchKernelGGL(attn_join_kernel<32>, join_grid, join_block, 0, stream, a, s.output, shares);
     else
-        hipLaunchKernelGGL(attn_join_kernel<64>, join_grid, join_block, 0, stream, a, s.output, log_sum);
+        hipLaunchKernelGGL(attn_join_kernel<64>, join_grid, join_block, 0, stream, a, s.output, shares);
     e = hipGetLastError();
     if (e != hipSuccess || !s.weights_out) return e;
     hipLaunchKernelGGL(attn_weights_kernel, dim3((s.capacity + kWave - 1) / kWave, s.sequences < 65535 ? s.sequences : 65535),
-                       dim3(kAttnThreads), 0, stream, a, log_sum, s.weights_in, s.weights_out);
+                       dim3(kAttnThreads), 0, stream, a, shares, s.weights_in, s.weights_out);
     return hipGetLastError();
 }
 

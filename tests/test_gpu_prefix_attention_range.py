@@ -85,3 +85,19 @@ def test_operands_at_the_ends_of_the_range(rt, path, q_exp, k_exp, v_exp):
     exp, _, bound = ref.attention(q, as_bytes(prefix), P, None, n, 0, 1, 0.25, "f32")
     got, _ = run(rt, "f32", q, as_bytes(prefix), P, None, n, 0, 1, 0.25)
     check(f"{path} {q_exp} {k_exp} {v_exp}", got, exp, bound, P, D)
+
+
+def test_weights_of_equal_keys_at_any_score(rt):
+    """A third each, whatever the score's spacing: the rounding of a score shifts all three alike."""
+    B, H, D, cap = 3, 2, 64, 4
+    for e in (0, 10, 20, 24, 27, 60):
+        q, cache = np.zeros((B, 1, H, D), f32), np.zeros((2, B * cap, D), f32)
+        q[..., 0] = 1.375
+        cache[0, :, 0] = 2.0 ** e
+        cache[1] = 1.0
+        n = np.full(B, 3, np.uint32)
+        w = np.zeros((B, cap), f32)
+        _, got = run(rt, "f32", q, None, 0, as_bytes(cache), n, cap, 1, 1.0, None, w)
+        say(f"scores of 2^{e}: {got[0]}")
+        # H shares of a third, each off by under 16 roundings of 2^-24
+        assert np.allclose(got[:, :3], H / 3, rtol=16 * 2.0 ** -24, atol=0) and (got[:, 3] == 0).all()
