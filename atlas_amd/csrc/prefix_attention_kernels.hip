@@ -466,7 +466,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a
         if (blockIdx.x * kWave >= length) continue;
         const float2* share = shares + static_cast<uint64_t>(seq) * lines;
         const float* scores = a.scores + static_cast<uint64_t>(seq) * lines * a.score_pitch + min(key, length - 1);
-        float sum = 0.0f;
+        // what an addition rounds off goes into the next: a sequence has up to 2^23
+        // rows, whose shares may all round to one side (131072 of them 8.0e-5)
+        float sum = 0.0f, lost = 0.0f;
         for (uint32_t i0 = begin; i0 < end; i0 += 4) {
             // four rows' loads on their way, of the last row again where there are fewer
             float x[4];
@@ -478,7 +480,10 @@ __global__ __launch_bounds__(kAttnThreads) void attn_weights_kernel(AttnParams a
                 of[i] = share[line];
             }
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) sum += i0 + i < end ? __builtin_amdgcn_exp2f(x[i] - of[i].x) * of[i].y : 0.0f;
+            for (uint32_t i = 0; i < 4; ++i) x[i] = i0 + i < end ? __builtin_amdgcn_exp2f(x[i] - of[i].x) * of[i].y : 0.0f;
+            const float four = ((x[0] + x[1]) + (x[2] + x[3])) - lost, next = sum + four;
+            lost = (next - sum) - four;
+            sum = next;
         }
         sums[wave][lane] = sum;
         __syncthreads();

@@ -73,3 +73,27 @@ def test_long_sums_of_equal_terms(rt, shape, fmt, byte):
     worst = float(np.abs(got / c - 1).max())
     say(f"{shape} {fmt} {byte:#x}: off by {worst:.2e}")
     assert worst <= 1e-5
+
+
+def test_weights_of_many_rows(rt):
+    """131072 shares of about 1 / 60000 added up for each of a sequence's first rows."""
+    T, H, D, P, cap = 2048, 64, 4, 60000, 2112
+    say("131072 shares")
+    q = np.zeros((1, T, H, D), f32)
+    dq, zero, w = rt.upload(q), rt.alloc(2 * P * D * 4), rt.empty(cap)
+    rt.memset(zero, 0, 2 * P * D * 4)
+    out, n = rt.empty(q.size), rt.upload(np.asarray([cap], np.uint32))
+    size = rt.prefix_attention_workspace("f32", 1, T, H, 1, D, P, cap, True)
+    ws = rt.alloc(size)
+    rt.prefix_attention("f32", dq, zero, P, P, zero, n, cap, out, None, w, 1, T, H, 1, D, 1.0, ws, size)
+    rt.sync()
+    got = w.download(cap).astype(np.float64)
+    for b in (dq, zero, w, out, n, ws):
+        rt.free(b)
+    # token t sees the prompt and own rows below cap - (T - 1 - t), all with equal scores
+    sees = cap - (T - 1 - np.arange(T))
+    share = H / (P + sees.astype(np.float64))
+    exp = np.array([share[sees > j].sum() for j in range(cap)])
+    worst = float(np.abs(got / exp - 1).max())
+    say(f"off by {worst:.2e}")
+    assert worst <= 2e-6  # a share's sum of 62112 equal weights and under 32 roundings of 2^-24
