@@ -23,6 +23,9 @@
 #include "device_common.hpp"
 #include "launch.hpp"
 
+#include <algorithm>
+#include <limits>
+
 namespace atlas {
 namespace {
 
@@ -543,8 +546,10 @@ uint64_t verify_draft_workspace(uint32_t sequences, uint32_t drafts, uint32_t vo
 hipError_t launch_verify_draft(hipStream_t stream, const VerifyDraftArgs& s) {
     const VerifyPlan p = verify_plan(s.sequences, s.drafts, s.vocab);
     uint8_t* ws = static_cast<uint8_t*>(s.workspace);
+    // finite: 0 * inf at the largest logit would leave its row no mass
+    const double scale = std::min(s.inv_temperature * 0x1.71547652b82fep+5, std::numeric_limits<double>::max());
     VerifyParams v{s,
-                   s.inv_temperature * 0x1.71547652b82fep+5,
+                   scale,
                    reinterpret_cast<SliceStat*>(ws),
                    reinterpret_cast<SliceStat*>(ws + p.target_bytes),
                    reinterpret_cast<double*>(ws + p.target_bytes + p.draft_bytes),
