@@ -646,11 +646,12 @@ __global__ __launch_bounds__(kPackedThreads, 2) void attn_packed_kernel(AttnPara
 #pragma unroll
         for (uint32_t c = 0; c < (kChunks + 7) / 8; ++c) {
             const uint32_t chunk = c * 8 + wave;
-            // 64 lanes of 16 bytes to LDS at M0, which the compiler keeps nothing
-            // in; nothing comes back to a register
+            // 64 lanes of 16 bytes to LDS at M0, an output of the asm so that the
+            // compiler knows of its change; nothing comes back to a register
+            uint32_t m0;
             if (chunk < kChunks)
-                asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                             :
+                asm volatile("s_mov_b32 %0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3"
+                             : "={m0}"(m0)
                              : "s"(lds + buffer * static_cast<uint32_t>(sizeof(WideTile<D>)) + chunk * 1024),
                                "v"(lane * 16), "s"(from + chunk * 1024)
                              : "memory");
