@@ -142,15 +142,15 @@ class LlamaDecodeStep:
             rt.add_rms_norm(lay["ffn_out"], o["residual"], nxt, o["state"], o["norm"], 1, H, S.eps)
 
     def capture(self) -> int:
-        if self.graph is not None:
-            self.rt.graph_destroy(self.graph)
+        self.close()
         self.rt.graph_begin()
         try:
             self.enqueue()
-        finally:
-            graph = self.rt.graph_end()
-        self.graph = graph
-        return graph
+        except BaseException:
+            self.rt.graph_destroy(self.rt.graph_end())
+            raise
+        self.graph = self.rt.graph_end()
+        return self.graph
 
     def replay(self) -> None:
         self.rt.graph_launch(self.graph)
@@ -270,15 +270,15 @@ class GemmaPrefillChunk:
             rt.rms_norm_add_scale(o["work"], lay["post_norm_w"], o["state"], lay["scale"], T, H, S.eps)
 
     def capture(self) -> int:
-        if self.graph is not None:
-            self.rt.graph_destroy(self.graph)
+        self.close()
         self.rt.graph_begin()
         try:
             self.enqueue()
-        finally:
-            graph = self.rt.graph_end()
-        self.graph = graph
-        return graph
+        except BaseException:
+            self.rt.graph_destroy(self.rt.graph_end())
+            raise
+        self.graph = self.rt.graph_end()
+        return self.graph
 
     def replay(self) -> None:
         self.rt.graph_launch(self.graph)
@@ -432,15 +432,15 @@ class SharedPromptDecode:
         self.lengths = o["cut_lengths"][0].download(S.sequences, np.uint32)
 
     def capture(self) -> int:
-        if self.graph is not None:
-            self.rt.graph_destroy(self.graph)
+        self.close()
         self.rt.graph_begin()
         try:
             self.enqueue()
-        finally:
-            graph = self.rt.graph_end()
-        self.graph = graph
-        return graph
+        except BaseException:
+            self.rt.graph_destroy(self.rt.graph_end())
+            raise
+        self.graph = self.rt.graph_end()
+        return self.graph
 
     def replay(self) -> None:
         self.rt.graph_launch(self.graph)

@@ -151,15 +151,15 @@ class GemmaDecodeStep:
 
     def capture(self) -> int:
         """Record one step into a HIP graph (kept on the object)."""
-        if self.graph is not None:
-            self.rt.graph_destroy(self.graph)
+        self.close()
         self.rt.graph_begin()
         try:
             self.enqueue()
-        finally:
-            graph = self.rt.graph_end()
-        self.graph = graph
-        return graph
+        except BaseException:
+            self.rt.graph_destroy(self.rt.graph_end())
+            raise
+        self.graph = self.rt.graph_end()
+        return self.graph
 
     def replay(self) -> None:
         self.rt.graph_launch(self.graph)
