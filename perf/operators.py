@@ -250,7 +250,11 @@ def run(state):
 def _runtime():
     from atlas_amd import HipRuntime
 
-    return HipRuntime(0)
+    rt = HipRuntime(0)
+    # the tensors are torch's: the library's launches join its stream (1 names the legacy default stream, whose handle is 0
+    # and would ask for the context's own)
+    rt._check(rt.lib.atlas_hip_set_stream(rt.ctx, torch.cuda.current_stream().cuda_stream or 1))
+    return rt
 
 
 @functools.lru_cache(maxsize=None)
