@@ -1,12 +1,13 @@
-"""GPU tests of the shared-prompt attention's sums over many keys that are all
-alike, whose roundings all fall to one side: the result is the one value that
-they hold."""
+"""GPU tests of the shared-prompt attention's sums over many keys: alike, so that
+all roundings fall to one side and the result is the one value that they hold,
+and with maxima that move, against float64."""
 import sys
 
 import numpy as np
 import pytest
 
 import decode_refs as ref
+from test_gpu_prefix_attention import check, run
 
 pytestmark = pytest.mark.gpu
 f32 = np.float32
@@ -30,6 +31,8 @@ def constant(fmt, byte):
 
 LONG = {  # sequences, heads, KV heads, head_dim, prompt, capacity
     "prompt": (448, 32, 32, 32, 60001, 0),
+    "prompt_128": (448, 32, 32, 128, 30001, 0),
+    "prompt_256": (448, 32, 32, 256, 20001, 0),
     "prompt_longer": (448, 32, 32, 4, 300001, 0),
     "prompt_packed": (1024, 32, 32, 32, 60001, 0),
     "prompt_packed_256": (2048, 16, 16, 256, 40001, 0),
@@ -97,3 +100,30 @@ def test_weights_of_many_rows(rt):
     worst = float(np.abs(got / exp - 1).max())
     say(f"off by {worst:.2e}")
     assert worst <= 2e-6  # a share's sum of 62112 equal weights and under 32 roundings of 2^-24
+
+
+@pytest.mark.parametrize("fmt", ["f32", "q8_0", "q4_0"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("ramp", ["up", "down", "none"])
+@pytest.mark.parametrize("B", [112, 129])
+def test_segments_of_several_runs(rt, B, D, fmt, ramp):
+    """Maxima that rise from run to run, or fall away behind the first: 1500 or more keys to a segment, unpacked (448 rows
+    of each KV head) and packed (516)."""
+    H, KH, P = 64, 16, 3001
+    say(f"{B} {D} {fmt} {ramp}")
+    r = np.random.default_rng(D)
+    q = (r.standard_normal((B, 1, H, D)) * 2).astype(f32)
+    prefix = ref.make_cache(r, fmt, P, KH * D)
+    scale = np.ones(P) if ramp == "none" else np.linspace(0.1, 3.0, P)[:: 1 if ramp == "up" else -1]
+    if fmt == "f32":
+        prefix.view(f32).reshape(2, P, -1)[:] *= scale[None, :, None].astype(f32)
+    else:
+        size = {"q8_0": 34, "q4_0": 18}[fmt]
+        b = prefix.reshape(2, P, KH * D // 32, size)
+        d = np.ascontiguousarray(b[..., :2]).view(np.float16) * scale[None, :, None, None]
+        b[..., :2] = d.astype(np.float16).view(np.uint8)
+    lengths = np.zeros(B, np.uint32)
+    some = np.arange(0, B, 16)  # of whose rows float64 is asked
+    exp, _, bound = ref.attention(q[some], prefix, P, None, lengths[some], 0, KH, float(f32(D ** -0.5)), fmt)
+    got, _ = run(rt, fmt, q, prefix, P, None, lengths, 0, KH, float(f32(D ** -0.5)))
+    check(f"{B} {D} {fmt} {ramp}", got[some], exp, bound, P, D)
