@@ -47,7 +47,7 @@ __device__ __forceinline__ uint32_t waves_before(uint32_t mine, uint32_t (&room)
 // KEYS = 0: longer sequences, whose keys are read anew by every pass.
 // Histogram bins have 16 counters, one for every lane % 16: few exponents
 // share most weights, and lanes that add to one counter go one by one (a
-// sequence of 65536 in one counter a bin took 193 us; so 52, of 2048 4.4 us).
+// sequence of 65536 in one counter a bin took 193 us; so 52, of 2048 4.3 to 5.0 us).
 template <int KEYS>
 __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArgs a) {
     __shared__ uint32_t bins[256][16];
@@ -70,8 +70,8 @@ __global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(KvEvictArg
     const uint32_t steps = KEYS ? KEYS : (n + kSelectThreads - 1) / kSelectThreads;
     const uint32_t first = wave * steps * kWave + lane;
     // how many of this lane's positions are old, and there: comparing k with
-    // them keeps 64 positions a lane out of the registers, and each pass anew
-    // (the empty asm) the 64 masks of the comparisons
+    // them, each pass anew (the empty asm), keeps 64 positions and 64 masks out of
+    // the registers, which the 64 keys fill (128, and 11 more in scratch)
     uint32_t mine_old = old > first ? (old - first + kWave - 1) / kWave : 0u;
     uint32_t mine_all = n > first ? (n - first + kWave - 1) / kWave : 0u;
     const auto key_at = [&](uint32_t k) {
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_copy_kernel(KvEvictArgs a,
 // and plane and walks its rows from the front, eight to a thread a step, each
 // step's loads before its stores.  A row only moves towards the front, so what
 // a step loads lies behind all that earlier ones store.  The barrier of each
-// step bounds it: the 256 sequences above 55 us (a third of their rows stay
+// step bounds it: the 256 sequences above 59 us (a third of their rows stay
 // where they are).
 constexpr int kShiftThreads = 1024;
 constexpr int kShiftRows = 8;
@@ -301,8 +301,8 @@ hipError_t launch_move(hipStream_t stream, const KvEvictArgs& a, bool in_place) 
         b.kept = a.kept + static_cast<uint64_t>(s0) * a.budget;
         if (in_place) {
             // 256 bytes of a row to a workgroup, or 64 where those are too few for
-            // the chip (8 sequences keeping 30000 rows of 1088 bytes 386 -> 277 us,
-            // one keeping 1024 of 768 bytes 8.4 -> 4.2)
+            // the chip (8 sequences keeping 30000 rows of 1088 bytes 386 -> 279 us,
+            // one keeping 1024 of 768 bytes 8.4 -> 4.6)
             uint32_t column = 256 / sizeof(T);
             while (column > 64 / sizeof(T) && (units + column - 1) / column * 2 * count < 256) column /= 2;
             if (column > units) column = units;

@@ -149,7 +149,7 @@ struct ValueRun<kKvF32, NG> {
 // One workgroup: 16 query rows of one KV head against one segment of a
 // sequence's own rows (or of the prompt, for batches of up to 16 rows).  Its
 // bytes bound it over long caches (64 sequences of up to 8192 rows of 256 dims,
-// 0.6 GB: 146 us, 4.1 TB/s), start and join over short ones.  More rows go by
+// 0.6 GB: 147 us, 4.1 TB/s), start and join over short ones.  More rows go by
 // more workgroups: two tiles of 16 in one took 38 us where two workgroups take
 // 23 (64 sequences, 4 tokens of 8 heads, 256 dims).  The wavefronts take its
 // keys 16 at a time in turn, straight from the cache into the operands'
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(kAttnThreads, NB < 8 ? 3 : (FMT == kKvF32 ? 1 : 2))
 // had weights of 0.33337).
 // LANES lanes hold a segment's dims; as many segments as fit the workgroup are
 // taken at once, and their sums meet in LDS in the segments' order.  Bound by
-// the segments' bytes: 2048 rows of 256 dims with 17 of them 11 us, 3.3 TB/s.
+// the segments' bytes: 2048 rows of 256 dims with 17 of them 10 us, 3.6 TB/s.
 template <int LANES>
 __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(AttnParams a, float* output, float2* shares) {
     constexpr uint32_t kGroups = kAttnThreads / LANES;

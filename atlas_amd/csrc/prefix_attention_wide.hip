@@ -25,8 +25,8 @@
 // of O^T = V^T P^T without leaving its registers.
 //
 // Measured: 64 rows x 100003 keys of 256 dims Q8_0 40 us, of which 12 are start
-// and segments; converting and multiplying take as long as each other (4500
-// cycles a tile).  2048 rows x 32768 f32, packed, 190 us: 1.08 PFLOP/s of f16,
+// and segments; converting and multiplying take about as long as each other.
+// 2048 rows x 32768 f32, packed, 192 to 199 us: 1.04 to 1.07 PFLOP/s of f16,
 // what a large matrix product reaches here.
 #include "prefix_attention.hpp"
 
@@ -578,7 +578,6 @@ __global__ __launch_bounds__(kWideThreads, 2) void attn_wide_kernel(AttnParams a
     const uint32_t row0 = item.tile * 64 + wave * 16;
     const bool busy = row0 < a.rows;  // the wavefront has rows
     WideRows<FMT, D, RUNS> rows(a, item.kv_head, row0 + n, quarter);
-    
     for (uint32_t first = item.begin; first < end; first += W::KT, buffer ^= 1) {
         __syncthreads();
         if (!busy) continue;

@@ -49,7 +49,7 @@ __device__ __forceinline__ float number_or_none(float x) { return x != x ? -__bu
 //
 // Its 64-bit instructions bound the first launch (384 rows of 262144 logits 68
 // us without them), so it has few: with the library's exp that launch took 120
-// us, as plain C 105, so 98.  Adding 1.5 2^52 leaves the nearest whole number of
+// us, as plain C 105, so 98 (in the same runs; 101 to 107 in others).  Adding 1.5 2^52 leaves the nearest whole number of
 // thirty-seconds in the low bits of the sum, with 1023 ones more in front; its
 // upper part is added to the exponent of a table entry, whose own is taken out;
 // and the constants stay in registers, one operand of an instruction a scalar
@@ -181,8 +181,8 @@ __device__ __forceinline__ void load_slice(const float* logits, uint32_t first, 
 }
 
 // A wavefront a slice of a row; rows of a sequence: targets, then drafts.  Bytes
-// and exponentials take as long as each other: 384 rows of 262144 logits 98 us,
-// 4.1 TB/s.  Two to eight slices a wavefront, the next one's logits on their way:
+// and exponentials add up: 384 rows of 262144 logits 98 to 107 us, 3.8 to 4.1
+// TB/s.  Two to eight slices a wavefront, the next one's logits on their way:
 // 94 to 107 us, and 37 to 56 where one slice takes 34 (640 rows of 50257).
 __global__ __launch_bounds__(kVerifyThreads) void verify_stats_kernel(VerifyParams v) {
     __shared__ uint2 table[32];
@@ -400,7 +400,7 @@ __device__ __forceinline__ void first_and_last(bool hit, uint32_t at, bool mass,
 }
 
 // One workgroup a sequence: the slice that holds the draw, the token in it,
-// and the row of results (5 us for one sequence, 7 for 64: loads that wait for
+// and the row of results (5.5 us for one sequence, 7.4 for 64: loads that wait for
 // each other).  Rounding may leave the goal just past the last
 // running sum: the last item with mass is then the one.
 template <bool FUSED>
@@ -562,7 +562,7 @@ hipError_t launch_verify_draft(hipStream_t stream, const VerifyDraftArgs& s) {
     if (e != hipSuccess) return e;
     // Deciding in the launches that need it saves one; where those are many
     // workgroups, deciding so often costs more.  Residual of 1 x 12 slices fused
-    // 7 us, apart 5 + 5; of 64 x 64 slices fused 41, apart 5 + 27.
+    // 8 us, apart 5 + 5; of 64 x 64 slices fused 41, apart 8 + 30.
     const uint32_t blocks = v.blocks * s.sequences;
     const bool fused = s.drafts <= kFusedDrafts && (v.s.draft ? blocks : s.sequences) <= 256;
     if (!fused && (e = launch(stream, verify_decide_kernel, s.sequences, v, kPickThreads)) != hipSuccess) return e;

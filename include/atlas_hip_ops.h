@@ -101,7 +101,8 @@ void atlas_hip_destroy(atlas_hip_ctx *ctx);
 /* ResidentCommand::finish (lib.rs:743-755): wait for all enqueued work and
  * surface device-side failures as ATLAS_ERR_COMMAND_FAILED. */
 int atlas_hip_sync(atlas_hip_ctx *ctx);
-/* Enqueue on a caller-owned hipStream_t (NULL restores the context stream). */
+/* Enqueue on a caller-owned hipStream_t (NULL restores the context stream;
+ * hipStreamLegacy, handle 1, names the device's default stream). */
 int atlas_hip_set_stream(atlas_hip_ctx *ctx, void *hip_stream);
 void *atlas_hip_get_stream(atlas_hip_ctx *ctx);
 int atlas_hip_set_reduction(atlas_hip_ctx *ctx, int reduction);
@@ -419,8 +420,13 @@ int atlas_hip_kv_append_q4_0(atlas_hip_ctx *ctx, const float *key, const float *
  * sequences * capacity < 2^32, kv_heads * head_dim <= 32768.  What a row does
  * not see never reaches it, whatever it holds; what it sees has to be finite,
  * with sums of values below 2^119 (a row that sees anything else may be NaN in
- * every dim).  Scores, sums and accumulators are f32 (within 1e-5 of float64
- * normwise); a call's result does not depend on timing.  The workspace
+ * every dim).  Scores, weights and sums are f32; of more than 16 query rows of a
+ * KV head over the prompt, the products' operands are two f16 numbers each, 22
+ * bits together.  A score is off by up to (head_dim + 24) 2^-24 of
+ * |scale| sum_i |q_i k_i|, which moves its weight by a factor; apart from that a
+ * result is within 1e-5 of float64 normwise, at any number of keys.  A weight
+ * below 2^-126 of its row's largest is zero.  A call's result does not depend on
+ * timing.  The workspace
  * (atlas_hip_prefix_attention_workspace bytes at the call's own sizes; smaller
  * sizes can need more) is overwritten by every call and holds nothing between
  * calls: calls that can overlap, and graphs whose replays can, need one each.
@@ -539,8 +545,10 @@ int atlas_hip_softcap_argmax_f32_noalloc(atlas_hip_ctx *ctx, const float *logits
  * NaN and -inf logits have no mass, all of a row's mass lies on its +inf; a
  * row without mass rejects its draft and draws 0xffffffff; a drafted token >=
  * vocab is rejected.  At most 1024 drafts, 2^29 logits a row and 2^20
- * sequences.  Probabilities and sums are float64, so that the drawn
- * token does not depend on how the sums are split.  Workspace as for
+ * sequences.  Probabilities and sums are float64, summed in a fixed order:
+ * accepted drafts and drawn token are the rule's unless the two sides of a
+ * comparison lie within 2e-12 of each other, relative to the larger or, of
+ * running sums, to the row's mass.  Workspace as for
  * prefix_attention (16-byte aligned, one for each of overlapping calls).
  * accepted and tokens must not overlap the inputs. */
 int atlas_hip_verify_draft_workspace(atlas_hip_ctx *ctx, uint32_t sequences, uint32_t drafts, uint32_t vocab,
