@@ -101,3 +101,20 @@ def test_weights_of_equal_keys_at_any_score(rt):
         say(f"scores of 2^{e}: {got[0]}")
         # H shares of a third, each off by under 16 roundings of 2^-24
         assert np.allclose(got[:, :3], H / 3, rtol=16 * 2.0 ** -24, atol=0) and (got[:, 3] == 0).all()
+
+
+@pytest.mark.parametrize("path", list(PATHS))
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 1e38])
+def test_a_query_that_is_no_number_stays_alone(rt, path, bad):
+    """A padded row of a batch: its own result may be anything, the others' are theirs."""
+    B, P, D = PATHS[path]
+    say(f"{path}, query {bad}")
+    r = np.random.default_rng(13)
+    q = (r.standard_normal((B, 1, 8, D)) * 2).astype(f32)
+    prefix, cache = (as_bytes(r.standard_normal((2, rows, D)).astype(f32)) for rows in (P, B * 8))
+    n = np.asarray([8 - i % 9 for i in range(B)], np.uint32)
+    exp, _, bound = ref.attention(q, prefix, P, cache, n, 8, 1, 0.0625, "f32")
+    q[0, 0, 3] = bad
+    got, _ = run(rt, "f32", q, prefix, P, cache, n, 8, 1, 0.0625)
+    got[0, 0, 3] = exp[0, 0, 3]
+    check(f"{path} query {bad}", got, exp, bound, P + 8, D)
