@@ -49,6 +49,14 @@ class GgufTensor(ctypes.Structure):
                 ("offset", c_uint64), ("bytes", c_uint64)]
 
 
+class PagedCache(ctypes.Structure):
+    """atlas_paged_cache (include/atlas_hip_ops.h)."""
+
+    _fields_ = [("pages", c_void_p), ("page_table", c_void_p), ("page_count", c_uint32), ("page_size", c_uint32),
+                ("kv_heads", c_uint32), ("head_dim", c_uint32), ("sequences", c_uint32), ("table_width", c_uint32),
+                ("format", c_int)]
+
+
 P = c_void_p  # device or host pointer
 CTX = c_void_p
 F = c_float
@@ -56,6 +64,7 @@ U32 = c_uint32
 U64 = c_uint64
 SZ = c_size_t
 TIMING = POINTER(DispatchTiming)
+PAGED = POINTER(PagedCache)
 
 # name -> argtypes (all return int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -129,6 +138,13 @@ SIGNATURES = {
     "atlas_hip_kv_evict_q4_0": [CTX, P, P, P, P, P, P, P, U32, U32, U32, U32, U32],
     "atlas_hip_verify_draft_workspace": [CTX, U32, U32, U32, POINTER(c_uint64)],
     "atlas_hip_verify_draft_f32": [CTX, P, P, P, P, P, P, P, P, U32, U32, U32, c_double, P, U64],
+    "atlas_hip_paged_cache_bytes": [CTX, PAGED, POINTER(c_uint64)],
+    "atlas_hip_paged_append": [CTX, PAGED, P, P, P, P, P, P, U32, U32, P, P, U32, U32],
+    "atlas_hip_paged_read": [CTX, PAGED, P, P, U32, P, P],
+    "atlas_hip_paged_attention_workspace": [CTX, PAGED, U32, POINTER(c_uint64)],
+    "atlas_hip_paged_attention": [CTX, PAGED, P, P, P, U32, F, U32, P, U64],
+    "atlas_hip_token_logprobs_workspace": [CTX, U32, U32, U32, POINTER(c_uint64)],
+    "atlas_hip_token_logprobs_f32": [CTX, P, U64, P, U32, P, P, P, P, U32, U32, U32, c_double, P, U64],
     "atlas_hip_softcap_f32": [CTX, P, P, U64, F],
     "atlas_hip_argmax_f32": [CTX, P, P, U32, U32],
     "atlas_hip_softcap_argmax_f32": [CTX, P, P, P, U32, U32, F],

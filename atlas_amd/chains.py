@@ -1,7 +1,8 @@
-"""Three more chains over the fused ops, beside the Gemma decode step
+"""Four more chains over the fused ops, beside the Gemma decode step
 (decode.py): the Llama resident decode token, the Gemma layer-major prefill
-chunk, and a batch that decodes drafted tokens behind a shared prompt.  Each enqueues the path's ops in the reference executor's
-order, with seeded stand-in buffers for the GEMM, attention and matvec
+chunk, a batch that decodes drafted tokens behind a shared prompt, and a batch
+that decodes from a paged cache.  Each enqueues the path's ops in the reference
+executor's order, with seeded stand-in buffers for the GEMM, attention and matvec
 outputs between them (outside this path); per-step inputs (token ids,
 positions, RoPE tables) live in device buffers, so `capture()` records a
 step once and `replay()` recomputes it from new inputs.
@@ -65,6 +66,20 @@ of drafted tokens behind its last one, with caches of a limited size:
 
   Rows of rejected drafts stay behind the sequence's new length; the next
   step's rows and weights (set to zero first) take their place.
+
+PagedDecode -- no counterpart in the reference: a batch of sequences that come
+and go, their caches in pages of one pool a layer, one table for all layers:
+
+    prompts: for each layer, their keys rotated and stored    paged_append
+    for each layer:
+        RoPE on Q and K, K and V into their pages             paged_append
+        attention over the sequence's pages, of the last
+        `window` positions in four layers of five             paged_attention
+    the likeliest token of each sequence                      argmax
+    its log probability, the entropy, the alternatives        token_logprobs
+
+  A sequence takes a page when its length reaches one, and gives all back when it
+  ends; a place without a sequence has length 0 and its token is skipped.
 """
 from __future__ import annotations
 
@@ -455,6 +470,168 @@ class SharedPromptDecode:
         res = {k: [b.download() for b in o[k]] for k in ("q_rot", "k_rot", "attention", "weights")}
         res["kv"] = [b.download(self.cache_bytes, np.uint8) for b in o["kv"]]
         res["capped"], res["accepted"], res["tokens"] = (o[k].download() for k in ("capped", "accepted", "tokens"))
+        return res
+
+
+@dataclass(frozen=True)
+class PagedShape:
+    """A batch of Llama-like sequences over a paged cache (SmolLM2-135M heads)."""
+
+    sequences: int = 6
+    layers: int = 3
+    q_heads: int = 9
+    kv_heads: int = 3
+    head_dim: int = 64
+    page_size: int = 16
+    capacity: int = 128   # positions of a sequence
+    pages: int = 32       # of a layer's pool
+    window: int = 40
+    vocab: int = 8192
+    alternatives: int = 5
+    theta: float = 1e4
+    temperature: float = 0.8
+
+
+class PagedDecode:
+    NO_PAGE = 0xFFFFFFFF
+
+    def __init__(self, rt: HipRuntime, shape: PagedShape = PagedShape(), kv_format: str = "q8_0", seed: int = 19):
+        self.rt, self.S, self.kv_format = rt, shape, kv_format
+        S = shape
+        B, H, KH, D, V = S.sequences, S.q_heads, S.kv_heads, S.head_dim, S.vocab
+        r = wl.rng(seed)
+        self.scale = 1.0 / wl.f32_sqrt(D)
+        self.width = -(-S.capacity // S.page_size)
+        self.lengths = np.zeros(B, np.uint32)                       # 0: no sequence there
+        self.table = np.full((B, self.width), self.NO_PAGE, np.uint32)
+        self.free = list(range(S.pages - 1, -1, -1))
+        self.layers = [{"q": wl.normal(r, B * H * D), "k": wl.normal(r, B * KH * D), "v": wl.normal(r, B * KH * D)}
+                       for _ in range(S.layers)]
+        self.dlayers = [{k: rt.upload(v) for k, v in lay.items()} for lay in self.layers]
+        cos, sin = rope_tables_llama(np.arange(self.width * S.page_size, dtype=np.uint32), D, S.theta)
+        self.dev = {"table": rt.empty(B * self.width, np.uint32), "lengths": rt.empty(B, np.uint32),
+                    "positions": rt.empty(B, np.uint32), "cos": rt.upload(cos), "sin": rt.upload(sin),
+                    "logits": rt.empty(B * V)}
+        self.pool_bytes = rt.paged_cache_bytes(kv_format, S.pages, S.page_size, KH, D)
+        L = range(S.layers)
+        self.out = {"q_rot": [rt.empty(B * H * D) for _ in L], "attention": [rt.empty(B * H * D) for _ in L],
+                    "pool": [rt.alloc(self.pool_bytes, np.uint8) for _ in L],
+                    "tokens": rt.empty(B, np.uint32), "logprobs": rt.empty(B), "entropy": rt.empty(B),
+                    "top_ids": rt.empty(max(B * S.alternatives, 1), np.uint32),
+                    "top_logprobs": rt.empty(max(B * S.alternatives, 1))}
+        self.caches = [rt.paged_cache(kv_format, p, S.pages, S.page_size, KH, D, self.dev["table"], B, self.width)
+                       for p in self.out["pool"]]
+        # one workspace: the stream orders the calls that use it
+        self.attention_bytes = rt.paged_attention_workspace(self.caches[0], H)
+        self.logprobs_bytes = rt.token_logprobs_workspace(B, V, S.alternatives)
+        self.workspace = rt.alloc(max(self.attention_bytes, self.logprobs_bytes))
+        for p in self.out["pool"]:
+            rt.memset(p, 0, self.pool_bytes)
+        rt.sync()
+        self.graph = None
+
+    def window(self, layer: int) -> int:
+        return 0 if layer % 5 == 4 else self.S.window
+
+    def _grow(self, place: int, length: int) -> None:
+        """Pages for the first `length` positions of a sequence."""
+        if length > self.S.capacity:
+            raise ValueError("a sequence has no room for its next position: end() it first")
+        have = int((self.table[place] != self.NO_PAGE).sum())
+        need = -(-length // self.S.page_size) - have
+        if need > len(self.free):
+            raise ValueError("the pool has no page left: end() a sequence first")
+        for i in range(need):
+            self.table[place, have + i] = self.free.pop()
+
+    def begin(self, prompts) -> None:
+        """Sequences for free places: {place: per layer (keys, values) [tokens, kv_heads, head_dim]}."""
+        rt, S = self.rt, self.S
+        places, positions = [], []
+        for place, layers in prompts.items():
+            if self.lengths[place]:
+                raise ValueError(f"place {place} has a sequence")
+            n = layers[0][0].shape[0]
+            self._grow(place, n)
+            self.lengths[place] = n
+            places += [place] * n
+            positions += range(n)
+        if not places:
+            return
+        self.dev["table"].upload(self.table)
+        held = [rt.upload(np.array(places, np.uint32)), rt.upload(np.array(positions, np.uint32))]
+        for layer in range(S.layers):
+            k, v = (np.concatenate([p[layer][i].reshape(-1, S.kv_heads, S.head_dim) for p in prompts.values()]) for i in (0, 1))
+            held += [rt.upload(k), rt.upload(v)]
+            rt.paged_append(self.caches[layer], held[-2], held[-1], None, None, self.dev["cos"], self.dev["sin"],
+                            self.width * S.page_size, S.head_dim // 2, held[0], held[1], len(places), 0)
+        rt.sync()
+        for b in held:
+            rt.free(b)
+
+    def end(self, place: int) -> None:
+        """The sequence's pages go back to the pool."""
+        pages = self.table[place][self.table[place] != self.NO_PAGE]
+        self.free.extend(int(p) for p in pages[::-1])
+        self.table[place] = self.NO_PAGE
+        self.lengths[place] = 0
+
+    def set_step(self, logits) -> None:
+        """The step's logits [sequences, vocab]; pages for its positions."""
+        active = self.lengths > 0
+        for place in np.nonzero(active)[0]:
+            self._grow(int(place), int(self.lengths[place]) + 1)
+        d = self.dev
+        d["table"].upload(self.table)
+        d["positions"].upload(np.where(active, self.lengths, 0xFFFFFFFF).astype(np.uint32))
+        d["lengths"].upload(np.where(active, self.lengths + 1, 0).astype(np.uint32))
+        d["logits"].upload(logits)
+
+    def enqueue(self) -> None:
+        rt, S, d, o = self.rt, self.S, self.dev, self.out
+        B, H = S.sequences, S.q_heads
+        for layer, lay in enumerate(self.dlayers):
+            rt.paged_append(self.caches[layer], lay["k"], lay["v"], lay["q"], o["q_rot"][layer], d["cos"], d["sin"],
+                            self.width * S.page_size, S.head_dim // 2, None, d["positions"], B, H)
+            rt.paged_attention(self.caches[layer], o["q_rot"][layer], d["lengths"], o["attention"][layer], H, self.scale,
+                               self.window(layer), self.workspace, self.attention_bytes)
+        rt.argmax(d["logits"], o["tokens"], B, S.vocab)
+        some = S.alternatives > 0
+        rt.token_logprobs(d["logits"], S.vocab, o["tokens"], 1, o["logprobs"], o["entropy"], o["top_ids"] if some else None,
+                          o["top_logprobs"] if some else None, B, S.vocab, S.alternatives, 1.0 / S.temperature, self.workspace,
+                          self.logprobs_bytes)
+
+    def advance(self) -> np.ndarray:
+        """The tokens of the step that ran; the sequences grow by them."""
+        tokens = self.out["tokens"].download(self.S.sequences, np.uint32)
+        self.lengths = np.where(self.lengths > 0, self.lengths + 1, 0).astype(np.uint32)
+        return tokens
+
+    def capture(self) -> int:
+        self.close()
+        self.rt.graph_begin()
+        try:
+            self.enqueue()
+        except BaseException:
+            self.rt.graph_destroy(self.rt.graph_end())
+            raise
+        self.graph = self.rt.graph_end()
+        return self.graph
+
+    def replay(self) -> None:
+        self.rt.graph_launch(self.graph)
+
+    def close(self) -> None:
+        if self.graph is not None:
+            self.rt.graph_destroy(self.graph)
+            self.graph = None
+
+    def results(self) -> dict:
+        o, B, n = self.out, self.S.sequences, self.S.sequences * self.S.alternatives
+        res = {k: [b.download() for b in o[k]] for k in ("q_rot", "attention")}
+        res["pool"] = [b.download(self.pool_bytes, np.uint8) for b in o["pool"]]
+        res.update({k: o[k].download(B) for k in ("tokens", "logprobs", "entropy")})
+        res.update({k: o[k].download(n) for k in ("top_ids", "top_logprobs")})
         return res
 
 

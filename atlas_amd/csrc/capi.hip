@@ -1002,6 +1002,95 @@ int atlas_hip_verify_draft_f32(atlas_hip_ctx* ctx, const float* target_logits, c
 }
 
 // ---------------------------------------------------------------------------
+// decoding from a paged cache
+// ---------------------------------------------------------------------------
+
+static atlas::PagedCache paged_cache(const atlas_paged_cache& c) {
+    return {static_cast<uint8_t*>(c.pages), c.page_table, c.page_count, c.page_size, c.kv_heads, c.head_dim, c.sequences,
+            c.table_width, c.format};
+}
+
+int atlas_hip_paged_cache_bytes(atlas_hip_ctx* ctx, const atlas_paged_cache* cache, uint64_t* bytes) {
+    if (!ctx) return ATLAS_ERR_INVALID_INPUT;
+    if (!cache || !bytes) return invalid(ctx, "null paged cache or output pointer");
+    *bytes = 0;
+    const atlas::PagedCache c = paged_cache(*cache);
+    if (int rc = checked(ctx, atlas::paged_cache_sizes_error(c))) return rc;
+    *bytes = atlas::paged_pool_bytes(c);
+    return ATLAS_OK;
+}
+
+int atlas_hip_paged_append(atlas_hip_ctx* ctx, const atlas_paged_cache* cache, const float* key, const float* value,
+                           const float* query, float* query_out, const float* cosine, const float* sine, uint32_t rope_rows,
+                           uint32_t rope_stride, const uint32_t* sequence_ids, const uint32_t* positions, uint32_t tokens,
+                           uint32_t q_heads) {
+    int rc = enter(ctx);
+    if (rc) return rc;
+    if (!cache) return invalid(ctx, "null paged cache");
+    const atlas::PagedAppendArgs a{paged_cache(*cache), key, value, query, query_out, cosine, sine, sequence_ids, positions,
+                                   rope_rows, rope_stride, tokens, q_heads};
+    if ((rc = checked(ctx, atlas::paged_append_error(a)))) return rc;
+    return launched(ctx, atlas::launch_paged_append(ctx->stream, a), "paged_append");
+}
+
+int atlas_hip_paged_read(atlas_hip_ctx* ctx, const atlas_paged_cache* cache, const uint32_t* sequence_ids,
+                         const uint32_t* positions, uint32_t rows, float* key, float* value) {
+    int rc = enter(ctx);
+    if (rc) return rc;
+    if (!cache) return invalid(ctx, "null paged cache");
+    const atlas::PagedReadArgs a{paged_cache(*cache), sequence_ids, positions, key, value, rows};
+    if ((rc = checked(ctx, atlas::paged_read_error(a)))) return rc;
+    return launched(ctx, atlas::launch_paged_read(ctx->stream, a), "paged_read");
+}
+
+int atlas_hip_paged_attention_workspace(atlas_hip_ctx* ctx, const atlas_paged_cache* cache, uint32_t q_heads,
+                                        uint64_t* bytes) {
+    if (!ctx) return ATLAS_ERR_INVALID_INPUT;
+    if (!cache || !bytes) return invalid(ctx, "null paged cache or output pointer");
+    *bytes = 0;
+    const atlas::PagedCache c = paged_cache(*cache);
+    if (int rc = checked(ctx, atlas::paged_attention_sizes_error(c, q_heads))) return rc;
+    *bytes = atlas::paged_attention_workspace(c, q_heads);
+    return ATLAS_OK;
+}
+
+int atlas_hip_paged_attention(atlas_hip_ctx* ctx, const atlas_paged_cache* cache, const float* q, const uint32_t* lengths,
+                              float* output, uint32_t q_heads, float scale, uint32_t window, void* workspace,
+                              uint64_t workspace_bytes) {
+    int rc = enter(ctx);
+    if (rc) return rc;
+    if (!cache) return invalid(ctx, "null paged cache");
+    const atlas::PagedAttentionArgs a{paged_cache(*cache), q, lengths, output, q_heads, window, scale, workspace};
+    if ((rc = checked(ctx, atlas::paged_attention_error(a)))) return rc;
+    if (workspace_bytes < atlas::paged_attention_workspace(a.cache, q_heads))
+        return invalid(ctx, "paged attention workspace is too small");
+    return launched(ctx, atlas::launch_paged_attention(ctx->stream, a), "paged_attention");
+}
+
+int atlas_hip_token_logprobs_workspace(atlas_hip_ctx* ctx, uint32_t rows, uint32_t vocab, uint32_t top, uint64_t* bytes) {
+    if (!ctx) return ATLAS_ERR_INVALID_INPUT;
+    if (!bytes) return invalid(ctx, "null output pointer");
+    *bytes = 0;
+    if (int rc = checked(ctx, atlas::token_logprobs_sizes_error(rows, vocab, top))) return rc;
+    *bytes = atlas::token_logprobs_workspace(rows, vocab, top);
+    return ATLAS_OK;
+}
+
+int atlas_hip_token_logprobs_f32(atlas_hip_ctx* ctx, const float* logits, uint64_t row_stride, const uint32_t* tokens,
+                                 uint32_t given, float* logprobs, float* entropy, uint32_t* top_ids, float* top_logprobs,
+                                 uint32_t rows, uint32_t vocab, uint32_t top, double inv_temperature, void* workspace,
+                                 uint64_t workspace_bytes) {
+    int rc = enter(ctx);
+    if (rc) return rc;
+    const atlas::TokenLogprobsArgs a{logits, row_stride, tokens, logprobs, entropy, top_ids, top_logprobs, rows, vocab, given,
+                                     top, inv_temperature, workspace};
+    if ((rc = checked(ctx, atlas::token_logprobs_error(a)))) return rc;
+    if (workspace_bytes < atlas::token_logprobs_workspace(rows, vocab, top))
+        return invalid(ctx, "log probability workspace is too small");
+    return launched(ctx, atlas::launch_token_logprobs(ctx->stream, a), "token_logprobs_f32");
+}
+
+// ---------------------------------------------------------------------------
 // logits: soft cap and argmax
 // ---------------------------------------------------------------------------
 

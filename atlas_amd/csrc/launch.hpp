@@ -157,7 +157,7 @@ uint32_t ple_projection_max_groups();
 hipError_t launch_ple_projection_f16(hipStream_t stream, const PleProjArgs& a);
 
 // KV-cache append with optional fused V RMSNorm (kv_kernels.hip).
-enum KvFormat : int { kKvF32 = 0, kKvQ8_0 = 1, kKvQ4_0 = 2 };
+enum KvFormat : int { kKvF32 = 0, kKvQ8_0 = 1, kKvQ4_0 = 2, kKvF16 = 3 };  // f16: paged caches only
 struct KvAppendArgs {
     const float* key;           // [tokens, kv_width]
     const float* value;         // [tokens, kv_width]
@@ -222,6 +222,71 @@ struct VerifyDraftArgs {
 };
 uint64_t verify_draft_workspace(uint32_t sequences, uint32_t drafts, uint32_t vocab);
 hipError_t launch_verify_draft(hipStream_t stream, const VerifyDraftArgs& a);
+
+// A cache in pages (paged_layout.hpp), as atlas_paged_cache.
+struct PagedCache {
+    uint8_t* pages;         // [page_count] pages
+    const uint32_t* table;  // [sequences, table_width]: the page of positions [i page_size, (i + 1) page_size)
+    uint32_t page_count, page_size, kv_heads, head_dim, sequences, table_width;
+    int format;             // KvFormat
+};
+
+// Rotated keys and values into pages (paged_cache_kernels.hip).
+struct PagedAppendArgs {
+    PagedCache cache;
+    const float* key;           // [tokens, kv_heads, head_dim]
+    const float* value;
+    const float* query;         // [tokens, q_heads, head_dim], or null
+    float* query_out;           // may be query
+    const float* cosine;        // [rope_rows, rope_stride], or null: no rotation
+    const float* sine;
+    const uint32_t* sequences;  // [tokens], or null: token t is sequence t's
+    const uint32_t* positions;  // [tokens]
+    uint32_t rope_rows, rope_stride, tokens, q_heads;
+};
+hipError_t launch_paged_append(hipStream_t stream, const PagedAppendArgs& a);
+
+// Rows of pages as f32 (paged_cache_kernels.hip).
+struct PagedReadArgs {
+    PagedCache cache;
+    const uint32_t* sequences;  // [rows], or null: row r is sequence r's
+    const uint32_t* positions;  // [rows]
+    float* key;                 // [rows, kv_heads, head_dim], or null
+    float* value;               // or null
+    uint32_t rows;
+};
+hipError_t launch_paged_read(hipStream_t stream, const PagedReadArgs& a);
+
+// Attention of one token of each sequence over its pages (paged_attention_kernels.hip).
+struct PagedAttentionArgs {
+    PagedCache cache;
+    const float* q;           // [sequences, q_heads, head_dim]
+    const uint32_t* lengths;  // [sequences], device
+    float* output;            // as q
+    uint32_t q_heads;
+    uint32_t window;          // 0: none
+    float scale;
+    void* workspace;
+};
+uint64_t paged_attention_workspace(const PagedCache& c, uint32_t q_heads);
+hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& a);
+
+// Log probabilities, entropies and likeliest tokens of rows of logits (logprobs_kernels.hip).
+struct TokenLogprobsArgs {
+    const float* logits;     // [rows, row_stride], vocab of each row
+    uint64_t row_stride;
+    const uint32_t* tokens;  // [rows, given]
+    float* logprobs;         // [rows, given], or null
+    float* entropy;          // [rows], or null
+    uint32_t* top_ids;       // [rows, top], or null
+    float* top_logprobs;     // [rows, top], or null
+    uint32_t rows, vocab, given, top;
+    double inv_temperature;
+    void* workspace;
+};
+constexpr uint32_t kMostTop = 64;
+uint64_t token_logprobs_workspace(uint32_t rows, uint32_t vocab, uint32_t top);
+hipError_t launch_token_logprobs(hipStream_t stream, const TokenLogprobsArgs& a);
 
 // Logit soft cap and argmax (logits_kernels.hip).  The argmax of a row split
 // over several workgroups goes through a workspace owned by the context:

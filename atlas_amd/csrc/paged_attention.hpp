@@ -1,0 +1,843 @@
+// paged_attention.hpp -- attention of one new token of each sequence over the
+// sequence's pages (paged_layout.hpp), for the translation units of its formats.
+//
+// For query head h of sequence b, with KV head h / group:
+//   x_j = scale * (q . k_j) over positions lo <= j < length whose page is there,
+//         lo = max(0, length - window), or 0 without a window,
+//   out = sum_j e^{x_j} v_j / sum_j e^{x_j}, zero where nothing is seen.
+// One pass over the keys with the running maximum and sum.  The work is split
+// evenly, not row by row: a row is a sequence's KV head with up to 16 query
+// heads, its positions are counted in units of a workgroup's step, and of all
+// rows' units together every workgroup takes the same number, so that lengths do
+// not matter for the balance and a lone sequence keeps the whole chip.  Lengths
+// live on the device, so the workgroups find their parts there.  A part that ends
+// inside a row leaves its maximum m, sum l of 2^{x - m} and sum O of 2^{x - m} v,
+// which a second launch joins.
+#pragma once
+
+#include "attention_lanes.hpp"
+#include "paged_layout.hpp"
+
+namespace atlas {
+
+inline constexpr int kPagedAttnThreads = 256;
+inline constexpr int kPagedAttnWaves = kPagedAttnThreads / kWave;
+inline constexpr uint32_t kPagedHeads = 16;  // query heads of a row: the columns of a product
+
+struct PagedAttnParams {
+    const float* q;
+    const uint8_t* pages;
+    const uint32_t* table;
+    const uint32_t* lengths;
+    float* output;
+    float* partial_out;   // [2 parts][heads][head_dim]
+    float2* partial_ml;   // [2 parts][heads]
+    uint64_t page_bytes;
+    uint32_t part_bytes, page_count, page_shift, table_width, sequences, capacity;
+    uint32_t kv_heads, group, head_tiles, heads, q_heads, head_dim, window;
+    uint32_t few_parts, most_parts, part_units;  // parts of all work; units of a part where there are more than few_parts
+    float scale;                                 // with log2(e)
+};
+
+// Keys of a wavefront's step: two tiles of 16 where a product over keys takes 32.
+__host__ __device__ constexpr uint32_t paged_keys(int format) { return format == kKvF32 ? 16 : 32; }
+__host__ __device__ constexpr uint32_t paged_unit(int format) { return kPagedAttnWaves * paged_keys(format); }
+// Workgroups to a CU.
+__host__ __device__ constexpr uint32_t paged_occupancy(uint32_t head_dim) { return head_dim <= 64 ? 4 : (head_dim <= 128 ? 3 : 2); }
+
+// The positions that a sequence's token sees, and their units.
+struct SeenRange {
+    uint32_t lo, hi;
+};
+__device__ __forceinline__ SeenRange seen_of(const PagedAttnParams& a, uint32_t seq) {
+    const uint32_t length = min(a.lengths[seq], a.capacity);
+    return {a.window && length > a.window ? length - a.window : 0u, length};
+}
+__device__ __forceinline__ uint32_t units_of(SeenRange s, uint32_t unit) {
+    return s.hi > s.lo ? (s.hi + unit - 1) / unit - s.lo / unit : 0u;
+}
+__device__ __forceinline__ uint64_t parts_of(const PagedAttnParams& a, uint64_t total) {
+    uint64_t parts = (total + a.part_units - 1) / a.part_units;
+    parts = parts > a.few_parts ? parts : a.few_parts;
+    parts = parts < a.most_parts ? parts : a.most_parts;
+    return parts < total ? parts : total;
+}
+
+// Sums over the workgroup, the result in every thread.
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d, kWave);
+    return v;
+}
+__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t (&room)[kPagedAttnWaves]) {
+    v = wave_sum_u64(v);
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) room[threadIdx.x / kWave] = v;
+    __syncthreads();
+    return (room[0] + room[1]) + (room[2] + room[3]);
+}
+
+__device__ __forceinline__ uint64_t uniform_u64(uint64_t v) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32)))) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)));
+}
+__device__ __forceinline__ uint32_t uniform_u32(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(v)); }
+
+constexpr uint32_t kPastPage = 0x7ffffff0u;  // a buffer offset past every part: reads as zero
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ u32x4_t load16(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t base) {
+    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, off, base, 0));
+}
+__device__ __forceinline__ u32x2_t load8(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t base) {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(rs, off, base, 0));
+}
+__device__ __forceinline__ uint32_t load4(__amdgpu_buffer_rsrc_t rs, uint32_t off, uint32_t base) {
+    return __builtin_amdgcn_raw_buffer_load_b32(rs, off, base, 0);
+}
+
+// A head's rows of one page, from row `row` on: 16 keys.  A page that is not
+// there has no bytes, and every load of it is zero.
+struct PageRows {
+    __amdgpu_buffer_rsrc_t keys, values;
+    uint32_t row;
+    __device__ PageRows(const PagedAttnParams& a, uint32_t kv_head, uint32_t page, uint32_t row)
+        : keys(span_rsrc(base(a, page, kv_head), page < a.page_count ? a.part_bytes : 0u)),
+          values(span_rsrc(base(a, page, a.kv_heads + kv_head), page < a.page_count ? a.part_bytes : 0u)), row(row) {}
+    static __device__ const uint8_t* base(const PagedAttnParams& a, uint32_t page, uint32_t part) {
+        return a.pages + (page < a.page_count ? page : 0u) * a.page_bytes + static_cast<uint64_t>(part) * a.part_bytes;
+    }
+};
+
+// Blocks of a value row in runs of 8, 4, 2, 1 (paged_run), and the 32-bit words
+// in which a lane holds its codes: BLOCK bytes of each block.
+template <int NB, int BLOCK>
+struct ValueWords {
+    uint8_t first[NB] = {}, run[NB] = {}, word[NB] = {};
+    int words = 0;
+    constexpr ValueWords() {
+        int b = 0;
+        for (int r = 8; r; r /= 2)
+            if (NB & r) {
+                for (int i = 0; i < r; ++i) {
+                    first[b + i] = static_cast<uint8_t>(b);
+                    run[b + i] = static_cast<uint8_t>(r);
+                    word[b + i] = static_cast<uint8_t>(words);
+                }
+                words += r * BLOCK < 4 ? 1 : r * BLOCK / 4;
+                b += r;
+            }
+    }
+};
+
+// What a wavefront holds of its step's keys and values, lane c + 16 g: of a tile
+// of 16 keys, key c's dims of group g; of the values, 16 lanes' dims of the keys
+// 4 g + r.  Scores come out as S^T = K Q^T: lane (c, g) has the scores of head c
+// with keys 4 g + r of each tile, which is the operand that O^T = V^T P^T wants if
+// the order of its keys is (tile, r) for each g; so P never leaves its lane and
+// a head's statistics are the lane's own.
+template <int FMT, int NB>
+struct Step;
+
+// f32 throughout (v_mfma_f32_16x16x4): 20 TB/s of keys and values, whatever the
+// number of heads.
+template <int NB>
+struct Step<kKvF32, NB> {
+    static constexpr int kTiles = 1, kOut = 2 * NB, kQuads = NB / 2;
+    static constexpr float kUnscale = 1.0f;
+    f32x4 k[2 * NB];
+    f32x4 v[4][kQuads ? kQuads : 1];
+    f32x2_t v2[4];
+    __device__ __forceinline__ void load_keys(const PageRows (&p)[1], uint32_t c, uint32_t g, uint32_t head_dim) {
+#pragma unroll
+        for (int s = 0; s < 2 * NB; ++s) {
+            const uint32_t dim = 16 * s + 4 * g;
+            const uint32_t off = s < 2 * NB - 2 || dim < head_dim ? c * head_dim * 4 + dim * 4 : kPastPage;
+            k[s] = __builtin_bit_cast(f32x4, load16(p[0].keys, off, p[0].row * head_dim * 4));
+        }
+    }
+    __device__ __forceinline__ void load_values(const PageRows (&p)[1], uint32_t c, uint32_t g, uint32_t head_dim) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t line = (4 * g + r) * head_dim * 4;
+#pragma unroll
+            for (int u = 0; u < kQuads; ++u) {
+                const uint32_t dim = 64 * u + 4 * c;
+                v[r][u] = __builtin_bit_cast(f32x4, load16(p[0].values, dim < head_dim ? line + dim * 4 : kPastPage, p[0].row * head_dim * 4));
+            }
+            if constexpr (NB % 2) {
+                const uint32_t dim = 64 * kQuads + 2 * c;
+                v2[r] = __builtin_bit_cast(f32x2_t, load8(p[0].values, dim < head_dim ? line + dim * 4 : kPastPage, p[0].row * head_dim * 4));
+            }
+        }
+    }
+    template <class Room>
+    __device__ __forceinline__ void scores(const Room& room, uint32_t lane, float, f32x4 (&s)[1]) const {
+        f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+        s[0] = t;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i += 2) {
+            const f32x4 q0 = room.queries[i][lane], q1 = room.queries[i + 1][lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i][j], q0[j], s[0], 0, 0, 0);
+                t = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i + 1][j], q1[j], t, 0, 0, 0);
+            }
+            if (i % 4) __builtin_amdgcn_sched_barrier(0);
+        }
+        s[0] += t;
+    }
+    // values of keys that are not seen must not be numbers that are none
+    __device__ __forceinline__ void keep(const bool (&seen)[1][4]) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int u = 0; u < kQuads; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[r][u][j] = seen[0][r] ? v[r][u][j] : 0.0f;
+            if constexpr (NB % 2) v2[r] = f32x2_t{seen[0][r] ? v2[r].x : 0.0f, seen[0][r] ? v2[r].y : 0.0f};
+        }
+    }
+    __device__ __forceinline__ void add(const f32x4 (&p)[1], f32x4 (&out)[kOut]) const {
+        // one rounding of the long sums for the step's keys, not one for every four
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u) {
+            f32x4 sum[4] = {};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r][u][j], p[0][r], sum[j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[4 * u + j] += sum[j];
+        }
+        if constexpr (NB % 2) {
+            f32x4 sum[2] = {};
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) sum[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v2[r][j], p[0][r], sum[j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) out[4 * kQuads + j] += sum[j];
+        }
+    }
+    // O^T has dims in its rows: tile 4 u + j row i is dim 64 u + 4 i + j
+    static __device__ __forceinline__ void put(float* line, uint32_t g, const f32x4 (&out)[kOut]) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int u = 0; u < kQuads; ++u)
+                *reinterpret_cast<f32x4*>(line + 64 * u + 16 * g + 4 * r) =
+                    f32x4{out[4 * u][r], out[4 * u + 1][r], out[4 * u + 2][r], out[4 * u + 3][r]};
+            if constexpr (NB % 2)
+                *reinterpret_cast<f32x2_t*>(line + 64 * kQuads + 8 * g + 2 * r) = f32x2_t{out[4 * kQuads][r], out[4 * kQuads + 1][r]};
+        }
+    }
+    static __device__ constexpr uint32_t query_dim(uint32_t j) { return j; }
+};
+
+// Two f16 numbers that add up to x, each rounded to nearest: 2^-24 of x at most is
+// lost, or 2^-25 where the second one is below 2^-14.
+__device__ __forceinline__ void f16_pieces(float x, _Float16& hi, _Float16& lo) {
+    hi = static_cast<_Float16>(materialize(x));
+    lo = static_cast<_Float16>(materialize(x - static_cast<float>(hi)));
+}
+
+// Products of f16 (v_mfma_f32_16x16x32_f16): keys and values as they are, the
+// other factor as two f16 numbers, brought near f16's largest by a power of two
+// that the sums are divided by.  A query's pieces lose 2^-24 of each number, or
+// 2^-39 of the row's largest; a weight's 2^-24, or 2^-40.
+template <int NB>
+struct Step<kKvF16, NB> {
+    static constexpr int kTiles = 2, kOut = 2 * NB, kQuads = NB / 2;
+    static constexpr float kUnscale = 0x1p-15f;
+    u32x4_t k[2][NB];
+    u32x2_t v[8][kQuads ? kQuads : 1];
+    uint32_t v2[8];
+    __device__ __forceinline__ void load_keys(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t head_dim) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int s = 0; s < NB; ++s) {
+                const uint32_t dim = 32 * s + 8 * g;
+                const uint32_t off = s < NB - 1 || dim < head_dim ? (c * head_dim + dim) * 2 : kPastPage;
+                k[h][s] = load16(p[h].keys, off, p[h].row * head_dim * 2);
+            }
+    }
+    __device__ __forceinline__ void load_values(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t head_dim) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const PageRows& rows = p[j / 4];
+            const uint32_t line = (4 * g + j % 4) * head_dim * 2;
+#pragma unroll
+            for (int u = 0; u < kQuads; ++u) {
+                const uint32_t dim = 64 * u + 4 * c;
+                v[j][u] = load8(rows.values, dim < head_dim ? line + dim * 2 : kPastPage, rows.row * head_dim * 2);
+            }
+            if constexpr (NB % 2) {
+                const uint32_t dim = 64 * kQuads + 2 * c;
+                v2[j] = load4(rows.values, dim < head_dim ? line + dim * 2 : kPastPage, rows.row * head_dim * 2);
+            }
+        }
+    }
+    template <class Room>
+    __device__ __forceinline__ void scores(const Room& room, uint32_t lane, float unscale, f32x4 (&s)[2]) const {
+        s[0] = s[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const f16x8_t hi = __builtin_bit_cast(f16x8_t, room.queries[2 * b][lane]);
+            const f16x8_t lo = __builtin_bit_cast(f16x8_t, room.queries[2 * b + 1][lane]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, k[h][b]), hi, s[h], 0, 0, 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, k[h][b]), lo, s[h], 0, 0, 0);
+            if (b % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+        s[0] *= unscale;
+        s[1] *= unscale;
+    }
+    __device__ __forceinline__ void keep(const bool (&seen)[2][4]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t mask = seen[j / 4][j % 4] ? 0xffffffffu : 0u;
+#pragma unroll
+            for (int u = 0; u < kQuads; ++u) v[j][u] &= mask;
+            if constexpr (NB % 2) v2[j] &= mask;
+        }
+    }
+    // dims 2 pair + e of eight keys
+    template <int E>
+    static __device__ __forceinline__ f16x8_t column(const uint32_t (&w)[8]) {
+        u32x4_t x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], E ? 0x07060302u : 0x05040100u);
+        return __builtin_bit_cast(f16x8_t, x);
+    }
+    __device__ __forceinline__ void add(const f32x4 (&p)[2], f32x4 (&out)[kOut]) const {
+        f16x8_t hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            _Float16 a, b;
+            f16_pieces(p[j / 4][j % 4] * 0x1p15f, a, b);
+            hi[j] = a;
+            lo[j] = b;
+        }
+        const auto one = [&](f16x8_t x, f32x4& o) {
+            f32x4 sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, sum, 0, 0, 0);
+            o += sum;
+        };
+#pragma unroll
+        for (int u = 0; u < kQuads; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = v[j][u][i];
+                one(column<0>(w), out[4 * u + 2 * i]);
+                one(column<1>(w), out[4 * u + 2 * i + 1]);
+            }
+        if constexpr (NB % 2) {
+            one(column<0>(v2), out[4 * kQuads]);
+            one(column<1>(v2), out[4 * kQuads + 1]);
+        }
+    }
+    static __device__ __forceinline__ void put(float* line, uint32_t g, const f32x4 (&out)[kOut]) {
+        Step<kKvF32, NB>::put(line, g, out);
+    }
+    static __device__ constexpr uint32_t query_dim(uint32_t j) { return j; }
+};
+
+// Products of codes, which f16 and bf16 hold as they are, with two f16 numbers for
+// a query's (as above) and, for the weights times the values' scales, three bf16
+// numbers: the 24 bits of an f32, cut in three, over its whole range.  A key's
+// scale goes on the product of its block, a value's on the weight, so codes are
+// only unpacked.
+template <int FMT, int NB>
+struct Step {
+    static_assert(FMT == kKvQ8_0 || FMT == kKvQ4_0);
+    static constexpr bool kBytes = FMT == kKvQ8_0;
+    static constexpr int kTiles = 2, kOut = 2 * NB, kKeyWords = kBytes ? 2 : 1, kBlock = kBytes ? 2 : 1;
+    static constexpr ValueWords<NB, kBlock> kWords{};
+    // v_cvt_off_f32_i4 gives sixteenths
+    static constexpr float kUnscale = kBytes ? 1.0f : 16.0f;
+    uint32_t k[2][NB][kKeyWords];
+    u32x2_t ks[2][NB], vs[2][NB];  // scales of keys 4 g + r
+    uint32_t v[8][kWords.words];
+    static __device__ __forceinline__ uint32_t row_bytes(uint32_t head_dim) { return kBytes ? head_dim : head_dim / 2; }
+    static __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rs, const PagedAttnParams& a, uint32_t row, uint32_t g,
+                                                       u32x2_t (&s)[NB]) {
+        const uint32_t base = (row_bytes(NB * 32) << a.page_shift) + row / 4 * NB * 8, off = g * NB * 8;
+#pragma unroll
+        for (int b = 0; b + 1 < NB; b += 2) {
+            const u32x4_t x = load16(rs, off + b * 8, base);
+            s[b] = u32x2_t{x[0], x[1]};
+            s[b + 1] = u32x2_t{x[2], x[3]};
+        }
+        if constexpr (NB % 2) s[NB - 1] = load8(rs, off + (NB - 1) * 8, base);
+    }
+    __device__ __forceinline__ void load_keys(const PageRows (&p)[2], uint32_t c, uint32_t g, const PagedAttnParams& a) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const uint32_t base = p[h].row * row_bytes(NB * 32);
+                if constexpr (kBytes) {
+                    const u32x2_t x = load8(p[h].keys, c * NB * 32 + b * 32 + 8 * g, base);
+                    k[h][b][0] = x[0];
+                    k[h][b][1] = x[1];
+                } else {
+                    k[h][b][0] = load4(p[h].keys, c * NB * 16 + b * 16 + 4 * g, base);
+                }
+            }
+            load_scales(p[h].keys, a, p[h].row, g, ks[h]);
+        }
+    }
+    __device__ __forceinline__ void load_values(const PageRows (&p)[2], uint32_t c, uint32_t g, const PagedAttnParams& a) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const __amdgpu_buffer_rsrc_t rs = p[j / 4].values;
+            const uint32_t base = p[j / 4].row * row_bytes(NB * 32), line = (4 * g + j % 4) * row_bytes(NB * 32);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (kWords.first[b] != b) continue;  // a run starts here
+                const int bytes = kWords.run[b] * kBlock, w = kWords.word[b];
+                const uint32_t off = line + 16 * kBlock * b + c * bytes;
+                if (bytes == 16) {
+                    const u32x4_t x = load16(rs, off, base);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[j][(w + i) % kWords.words] = x[i];
+                } else if (bytes == 8) {
+                    const u32x2_t x = load8(rs, off, base);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) v[j][(w + i) % kWords.words] = x[i];
+                } else if (bytes == 4) {
+                    v[j][w] = load4(rs, off, base);
+                } else if (bytes == 2) {
+                    v[j][w] = static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(rs, off, base, 0));
+                } else {
+                    v[j][w] = static_cast<uint8_t>(__builtin_amdgcn_raw_buffer_load_b8(rs, off, base, 0));
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_scales(p[h].values, a, p[h].row, g, vs[h]);
+    }
+    // Eight codes of a key as f16: 1024 + (a code without its sign) has it in its low bits.
+    static __device__ __forceinline__ f16x8_t key_codes(const uint32_t (&w)[kKeyWords]) {
+        u32x4_t x;
+        _Float16 less;
+        if constexpr (kBytes) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                x[i] = __builtin_amdgcn_perm(0x64646464u, w[i / 2] ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u);
+            less = static_cast<_Float16>(-1152.0f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (w[0] >> (4 * i) & 0x000f000fu) | 0x64006400u;
+            less = static_cast<_Float16>(-1032.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, static_cast<uint32_t>(x[i])) + f16x2_t{less, less});
+        return __builtin_bit_cast(f16x8_t, x);
+    }
+    static __device__ __forceinline__ float scale_of(u32x2_t s, int r) { return h2f(static_cast<uint16_t>(s[r / 2] >> (16 * (r % 2)))); }
+    template <class Room>
+    __device__ __forceinline__ void scores(const Room& room, uint32_t lane, float unscale, f32x4 (&s)[2]) const {
+        s[0] = s[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const f16x8_t hi = __builtin_bit_cast(f16x8_t, room.queries[2 * b][lane]);
+            const f16x8_t lo = __builtin_bit_cast(f16x8_t, room.queries[2 * b + 1][lane]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const f16x8_t x = key_codes(k[h][b]);
+                f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, d, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[h][r] = __builtin_fmaf(d[r], scale_of(ks[h][b], r), s[h][r]);
+            }
+            if (b % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+        s[0] *= unscale;
+        s[1] *= unscale;
+    }
+    __device__ __forceinline__ void keep(const bool (&seen)[2][4]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t mask = (seen[h][2 * i] ? 0xffffu : 0u) | (seen[h][2 * i + 1] ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) vs[h][b][i] &= mask;
+            }
+    }
+    static __device__ __forceinline__ uint32_t upper(float odd, float even) {  // their upper halves
+        return __builtin_amdgcn_perm(__float_as_uint(odd), __float_as_uint(even), 0x07060302u);
+    }
+    static __device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+    // code e of block b of eight keys
+    __device__ __forceinline__ bf16x8_t value_codes(int b, int e) const {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int at = (b - kWords.first[b]) * kBlock + (kBytes ? e : 0);
+            const uint32_t w = v[j][kWords.word[b] + at / 4];
+            if constexpr (kBytes)
+                x[j] = static_cast<float>(static_cast<int8_t>(w >> (8 * (at % 4))));
+            else  // two's complement by the flip of bit 3
+                x[j] = __builtin_amdgcn_cvt_off_f32_i4(((e ? w >> 4 : w) ^ 0x08080808u) >> (8 * (at % 4)) & 255u);
+        }
+        u32x4_t y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = upper(x[2 * i + 1], x[2 * i]);
+        return __builtin_bit_cast(bf16x8_t, y);
+    }
+    __device__ __forceinline__ void add(const f32x4 (&p)[2], f32x4 (&out)[kOut]) const {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            u32x4_t piece[3];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float w[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) w[j] = p[i / 2][i % 2 * 2 + j] * scale_of(vs[i / 2][b], i % 2 * 2 + j);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) {
+                    piece[n][i] = upper(w[1], w[0]);
+                    if (n == 2) break;
+                    w[0] -= cut(w[0]);
+                    w[1] -= cut(w[1]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const bf16x8_t x = value_codes(b, e);
+                f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int n = 0; n < 3; ++n)
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8_t, piece[n]), sum, 0, 0, 0);
+                out[2 * b + e] += sum;
+            }
+        }
+    }
+    // tile 2 b + e row i is dim 32 b + 2 i + e
+    static __device__ __forceinline__ void put(float* line, uint32_t g, const f32x4 (&out)[kOut]) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<f32x2_t*>(line + 32 * b + 8 * g + 2 * r) = f32x2_t{out[2 * b][r], out[2 * b + 1][r]};
+    }
+    // the order in which key_codes gives a lane's eight dims
+    static __device__ constexpr uint32_t query_dim(uint32_t j) { return kBytes ? j : j / 2 + j % 2 * 4; }
+};
+
+template <int FMT, int NB>
+__global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void paged_attention_kernel(PagedAttnParams a) {
+    using S = Step<FMT, NB>;
+    constexpr int kTiles = S::kTiles;
+    constexpr uint32_t kKeys = paged_keys(FMT), kUnit = paged_unit(FMT), kDims = 32 * NB, kPitch = kDims + 4;
+    static_assert(kKeys == 16 * kTiles);
+    // queries in the products' order [part][lane]; at the end the wavefronts' sums
+    __shared__ union Room {
+        f32x4 queries[2 * NB][kWave];
+        float sums[kPagedAttnWaves][kPagedHeads][kPitch];
+    } room;
+    __shared__ float2 room_ml[kPagedAttnWaves][kPagedHeads];
+    __shared__ float room_unscale[kPagedHeads];
+    __shared__ uint64_t room_sum[kPagedAttnWaves];
+    __shared__ struct {
+        uint64_t before;
+        uint32_t seq;
+    } found;
+    const uint32_t lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
+    const uint32_t wave = uniform_u32(threadIdx.x / kWave);
+    const uint64_t rows = static_cast<uint64_t>(a.kv_heads) * a.head_tiles;  // of a sequence
+
+    // this workgroup's units of all sequences'
+    uint64_t mine = 0;
+    for (uint32_t b = threadIdx.x; b < a.sequences; b += kPagedAttnThreads) mine += units_of(seen_of(a, b), kUnit);
+    const uint64_t total = uniform_u64(block_sum_u64(mine, room_sum)) * rows;
+    const uint64_t parts = parts_of(a, total);
+    if (blockIdx.x >= parts) return;
+    const uint64_t begin = uniform_u64(total * blockIdx.x / parts), end = uniform_u64(total * (blockIdx.x + 1) / parts);
+    // the sequence that `begin` lies in
+    uint64_t before = 0;
+    for (uint32_t first = 0; first < a.sequences; first += kPagedAttnThreads) {
+        const uint32_t b = first + threadIdx.x;
+        const uint32_t units = b < a.sequences ? units_of(seen_of(a, b), kUnit) : 0u;
+        uint64_t upto = units;  // of this and the ones before
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) {
+            const uint64_t x = __shfl_up(upto, d, kWave);
+            if (lane >= static_cast<uint32_t>(d)) upto += x;
+        }
+        __syncthreads();
+        if (lane == kWave - 1) room_sum[wave] = upto;
+        __syncthreads();
+        uint64_t chunk = 0;
+        for (uint32_t w = 0; w < kPagedAttnWaves; ++w) {
+            if (w == wave) upto += chunk;
+            chunk += room_sum[w];
+        }
+        const uint64_t from = before + (upto - units) * rows;
+        if (units && begin >= from && begin < before + upto * rows) {
+            found.before = from;
+            found.seq = b;
+        }
+        before += chunk * rows;
+        if (before > begin) break;
+    }
+    __syncthreads();
+    before = uniform_u64(found.before);
+    uint32_t seq = uniform_u32(found.seq);
+
+    for (uint64_t at = begin; at < end;) {
+        // a segment: units [t0, t1) of a row's `units`
+        SeenRange seen = seen_of(a, seq);
+        uint32_t units = uniform_u32(units_of(seen, kUnit));
+        while (at >= before + units * rows) {
+            before += units * rows;
+            ++seq;
+            seen = seen_of(a, seq);
+            units = uniform_u32(units_of(seen, kUnit));
+        }
+        seen.lo = uniform_u32(seen.lo);
+        seen.hi = uniform_u32(seen.hi);
+        const uint32_t row = uniform_u32(static_cast<uint32_t>((at - before) / units));
+        const uint32_t t0 = uniform_u32(static_cast<uint32_t>((at - before) - static_cast<uint64_t>(row) * units));
+        const uint32_t t1 = uniform_u32(end - at < units - t0 ? t0 + static_cast<uint32_t>(end - at) : units);
+        at += t1 - t0;
+        const uint32_t kv_head = row / a.head_tiles, head0 = row % a.head_tiles * kPagedHeads;
+        const uint32_t heads = min(a.group - head0, kPagedHeads);
+        const uint64_t line0 = static_cast<uint64_t>(seq) * a.q_heads + kv_head * a.group + head0;
+
+        __syncthreads();  // the last segment's sums have been read
+        {
+            const uint32_t head = threadIdx.x / 16, sub = threadIdx.x % 16;
+            const float* q = a.q + (line0 + min(head, heads - 1)) * a.head_dim;
+            constexpr int kEach = FMT == kKvF32 ? 4 : 8, kItems = (kDims / kEach + 15) / 16;
+            f32x4 x[kItems][kEach / 4];
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kItems; ++i)
+#pragma unroll
+                for (int h = 0; h < kEach / 4; ++h) {
+                    const uint32_t dim = (sub + 16 * i) * kEach + 4 * h;
+                    const bool there = dim < a.head_dim && head < heads;
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(q + (dim < a.head_dim ? dim : 0));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[i][h][j] = there ? y[j] * a.scale : 0.0f;
+                        top = fmaxf(top, __builtin_fabsf(x[i][h][j]));
+                    }
+                }
+            if constexpr (FMT == kKvF32) {
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) {
+                    const uint32_t item = sub + 16 * i;
+                    if (item < kDims / 4) room.queries[item / 4][item % 4 * 16 + head] = x[i][0];
+                }
+            } else {
+                top = fmaxf(top, dpp_f32<0xb1, 0xf, false>(top));
+                top = fmaxf(top, dpp_f32<0x4e, 0xf, false>(top));
+                top = fmaxf(top, dpp_f32<0x141, 0xf, false>(top));
+                top = fmaxf(top, dpp_f32<0x140, 0xf, false>(top));
+                // the row's largest to 2^13 .. 2^14
+                int up = 0;
+                if (top > 0.0f && top < __builtin_inff()) up = min(14 - __builtin_amdgcn_frexp_expf(top), 126);
+                const float by = pow2i(up);
+                if (sub == 0) room_unscale[head] = pow2i(-up);
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) {
+                    const uint32_t item = sub + 16 * i;
+                    f16x8_t hi, lo;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        _Float16 p, r;
+                        const uint32_t d = S::query_dim(j);
+                        f16_pieces(x[i][d / 4][d % 4] * by, p, r);
+                        hi[j] = p;
+                        lo[j] = r;
+                    }
+                    if (item < kDims / 8) {
+                        room.queries[item / 4 * 2][item % 4 * 16 + head] = __builtin_bit_cast(f32x4, hi);
+                        room.queries[item / 4 * 2 + 1][item % 4 * 16 + head] = __builtin_bit_cast(f32x4, lo);
+                    }
+                }
+            }
+        }
+
+        // Unit t's keys of this wavefront start at (seen.lo / kUnit + t) * kUnit + wave * kKeys.
+        const uint32_t* table = a.table + static_cast<uint64_t>(seq) * a.table_width;
+        const uint32_t start = (seen.lo / kUnit) * kUnit + wave * kKeys;
+        constexpr uint32_t kAhead = kWave / kTiles;  // units whose pages a wavefront's lanes hold
+        uint32_t pages = 0, pages_from = t0;
+        const auto look_up = [&](uint32_t t) {
+            pages_from = t;
+            const uint32_t entry = (start + (t + lane / kTiles) * kUnit + lane % kTiles * 16) >> a.page_shift;
+            pages = entry < a.table_width ? table[entry] : 0xffffffffu;
+        };
+        const auto page_of = [&](uint32_t t, uint32_t tile) { return readlane_u32(pages, (t - pages_from) * kTiles + tile); };
+        S step;
+        uint32_t page[kTiles];
+        // which of the step's tiles have a page, for the one that is used and the one that is loaded
+        const auto load = [&](uint32_t t, bool keys) {
+            const bool some = t < t1;
+            const uint32_t key = start + (some ? t : t1 - 1) * kUnit;
+            const uint32_t mask = (1u << a.page_shift) - 1;
+            if constexpr (kTiles == 1) {
+                const PageRows p[1] = {PageRows(a, kv_head, some ? page[0] : 0xffffffffu, key & mask)};
+                if (keys)
+                    step.load_keys(p, c, g, a.head_dim);
+                else
+                    step.load_values(p, c, g, a.head_dim);
+            } else {
+                const PageRows p[2] = {PageRows(a, kv_head, some ? page[0] : 0xffffffffu, key & mask),
+                                       PageRows(a, kv_head, some ? page[1] : 0xffffffffu, (key + 16) & mask)};
+                if constexpr (FMT == kKvF16) {
+                    if (keys)
+                        step.load_keys(p, c, g, a.head_dim);
+                    else
+                        step.load_values(p, c, g, a.head_dim);
+                } else {
+                    if (keys)
+                        step.load_keys(p, c, g, a);
+                    else
+                        step.load_values(p, c, g, a);
+                }
+            }
+        };
+        const auto turn = [&](uint32_t t) {
+            if (t < t1 && t - pages_from >= kAhead) look_up(t);
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) page[i] = t < t1 ? page_of(t, i) : 0xffffffffu;
+        };
+        look_up(t0);
+        turn(t0);
+        load(t0, true);
+        load(t0, false);
+        __syncthreads();
+        const float unscale = FMT == kKvF32 ? 1.0f : room_unscale[c];
+
+        float m = neg_inf(), l = 0.0f;
+        f32x4 out[S::kOut];
+#pragma unroll
+        for (int i = 0; i < S::kOut; ++i) out[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t t = t0; t < t1; ++t) {
+            const uint32_t key0 = start + t * kUnit;
+            bool there[kTiles], whole = key0 >= seen.lo && key0 + kKeys <= seen.hi;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                there[i] = page[i] < a.page_count;
+                whole = whole && there[i];
+            }
+            f32x4 s[kTiles];
+            step.scores(room, lane, unscale, s);
+            turn(t + 1);
+            load(t + 1, true);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!whole) {
+                bool sees[kTiles][4];
+#pragma unroll
+                for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t key = key0 + 16 * i + 4 * g + r;
+                        sees[i][r] = there[i] && key >= seen.lo && key < seen.hi;
+                        s[i][r] = sees[i][r] ? s[i][r] : neg_inf();
+                    }
+                step.keep(sees);
+            }
+            float top = neg_inf();
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) top = fmaxf(top, fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3])));
+            top = max_xor32(max_xor16(top));
+            if (__builtin_amdgcn_ballot_w64(top > m) != 0) {
+                const float m_new = fmaxf(m, top);
+                const float fade = m == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+                m = m_new;
+                l *= fade;
+#pragma unroll
+                for (int i = 0; i < S::kOut; ++i) out[i] *= fade;
+            }
+            const float base = m == neg_inf() ? 0.0f : m;
+            float sum[kTiles];
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[i][r] = __builtin_amdgcn_exp2f(s[i][r] - base);
+                sum[i] = (s[i][0] + s[i][1]) + (s[i][2] + s[i][3]);
+            }
+            l += kTiles == 1 ? sum[0] : sum[0] + sum[kTiles - 1];
+            step.add(s, out);
+            __builtin_amdgcn_sched_barrier(0);
+            load(t + 1, false);
+        }
+
+        // join the wavefronts
+        l = sum_xor32(sum_xor16(l));
+        __syncthreads();
+        if (g == 0) room_ml[wave][c] = make_float2(m, l);
+#pragma unroll
+        for (int i = 0; i < S::kOut; ++i) out[i] *= S::kUnscale;
+        S::put(room.sums[wave][c], g, out);
+        __syncthreads();
+        const bool all = t0 == 0 && t1 == units;
+        const uint64_t slot = 2ull * blockIdx.x + (t0 == 0 ? 1 : 0);
+        constexpr uint32_t kQuads = kDims / 4;
+        for (uint32_t i = threadIdx.x; i < heads * kQuads; i += kPagedAttnThreads) {
+            const uint32_t r = i / kQuads, quad = i % kQuads;
+            if (4 * quad >= a.head_dim) continue;
+            float top = neg_inf(), sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kPagedAttnWaves; ++w) top = fmaxf(top, room_ml[w][r].x);
+            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kPagedAttnWaves; ++w) {
+                const float2 ml = room_ml[w][r];
+                const float f = ml.x == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
+                sum += f * ml.y;
+                o += f * *reinterpret_cast<const f32x4*>(&room.sums[w][r][4 * quad]);
+            }
+            if (all) {
+                f32x4 y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = sum == 0.0f ? 0.0f : o[j] / sum;
+                *reinterpret_cast<f32x4*>(a.output + (line0 + r) * a.head_dim + 4 * quad) = y;
+            } else {
+                if (quad == 0) a.partial_ml[slot * a.heads + r] = make_float2(top, sum);
+                *reinterpret_cast<f32x4*>(a.partial_out + (slot * a.heads + r) * a.head_dim + 4 * quad) = o;
+            }
+        }
+    }
+}
+
+hipError_t launch_paged_attention_f32(hipStream_t stream, const PagedAttnParams& a);
+hipError_t launch_paged_attention_f16(hipStream_t stream, const PagedAttnParams& a);
+hipError_t launch_paged_attention_q8_0(hipStream_t stream, const PagedAttnParams& a);
+hipError_t launch_paged_attention_q4_0(hipStream_t stream, const PagedAttnParams& a);
+
+template <int FMT, int NB>
+hipError_t launch_paged_blocks(hipStream_t stream, const PagedAttnParams& a) {
+    hipLaunchKernelGGL((paged_attention_kernel<FMT, NB>), dim3(a.most_parts), dim3(kPagedAttnThreads), 0, stream, a);
+    return hipGetLastError();
+}
+template <int FMT>
+hipError_t launch_paged_format(hipStream_t stream, const PagedAttnParams& a) {
+    switch ((a.head_dim + 31) / 32) {
+        case 1: return launch_paged_blocks<FMT, 1>(stream, a);
+        case 2: return launch_paged_blocks<FMT, 2>(stream, a);
+        case 3: return launch_paged_blocks<FMT, 3>(stream, a);
+        case 4: return launch_paged_blocks<FMT, 4>(stream, a);
+        case 5: return launch_paged_blocks<FMT, 5>(stream, a);
+        case 6: return launch_paged_blocks<FMT, 6>(stream, a);
+        case 7: return launch_paged_blocks<FMT, 7>(stream, a);
+        default: return launch_paged_blocks<FMT, 8>(stream, a);
+    }
+}
+
+}  // namespace atlas

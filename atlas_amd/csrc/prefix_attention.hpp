@@ -2,39 +2,13 @@
 // in common: how lanes read the rows of a cache, and a call's parameters.
 #pragma once
 
-#include "device_common.hpp"
+#include "attention_lanes.hpp"
 #include "launch.hpp"
 
 namespace atlas {
 
 inline constexpr int kAttnThreads = 256;
 inline constexpr int kAttnWaves = kAttnThreads / kWave;
-inline constexpr float kLog2e = 1.44269504088896340736f;
-
-__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
-
-// The maximum over lanes that differ in bit 3 / 4 / 5 of their number.
-__device__ __forceinline__ float max_xor8(float x) { return fmaxf(x, dpp_f32<0x128, 0xf, false>(x)); }  // row_ror:8
-__device__ __forceinline__ float max_xor16(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-__device__ __forceinline__ float max_xor32(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-__device__ __forceinline__ float sum_xor16(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto p = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
-__device__ __forceinline__ float sum_xor32(float x) {
-    const uint32_t u = __float_as_uint(x);
-    const auto p = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
 
 // ---------------------------------------------------------------------------
 // Rows of a cache as MFMA operands.  A product over dims may take them in any
@@ -42,7 +16,6 @@ __device__ __forceinline__ float sum_xor32(float x) {
 // format has the order in which a lane's values are contiguous in memory:
 // units of 8 key dims and quads of 4 value dims.
 // ---------------------------------------------------------------------------
-typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32_a2 __attribute__((aligned(2)));
 typedef u32x2_t u32x2_a2 __attribute__((aligned(2)));
 typedef u32x4_t u32x4_a2 __attribute__((aligned(2)));

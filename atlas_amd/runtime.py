@@ -348,6 +348,52 @@ class HipRuntime:
             _ptr(accept_uniform), _ptr(sample_uniform), _ptr(accepted), _ptr(tokens), sequences, drafts, vocab,
             inv_temperature, _ptr(workspace), workspace_bytes))
 
+    # Decoding from a paged cache (no counterpart in the reference).
+    _PAGED_FORMATS = {**_CACHE_FORMATS, "f16": 3}
+
+    def paged_cache(self, fmt, pages, page_count, page_size, kv_heads, head_dim, page_table, sequences, table_width):
+        """The pool `pages` and its table [sequences, table_width], as the paged ops take it; it keeps no buffer alive."""
+        return _lib.PagedCache(_ptr(pages), _ptr(page_table), page_count, page_size, kv_heads, head_dim, sequences, table_width,
+                               self._PAGED_FORMATS[fmt])
+
+    def paged_cache_bytes(self, fmt, page_count, page_size, kv_heads, head_dim) -> int:
+        """Bytes of a pool of page_count pages."""
+        n = c_uint64()
+        cache = self.paged_cache(fmt, None, page_count, page_size, kv_heads, head_dim, None, 1, 1)
+        self._check(self.lib.atlas_hip_paged_cache_bytes(self.ctx, byref(cache), byref(n)))
+        return n.value
+
+    def paged_append(self, cache, key, value, query, query_out, cosine, sine, rope_rows, rope_stride, sequence_ids, positions,
+                     tokens, q_heads):
+        self._check(self.lib.atlas_hip_paged_append(
+            self.ctx, byref(cache), _ptr(key), _ptr(value), _ptr(query), _ptr(query_out), _ptr(cosine), _ptr(sine), rope_rows,
+            rope_stride, _ptr(sequence_ids), _ptr(positions), tokens, q_heads))
+
+    def paged_read(self, cache, sequence_ids, positions, rows, key, value):
+        self._check(self.lib.atlas_hip_paged_read(self.ctx, byref(cache), _ptr(sequence_ids), _ptr(positions), rows, _ptr(key),
+                                                  _ptr(value)))
+
+    def paged_attention_workspace(self, cache, q_heads) -> int:
+        n = c_uint64()
+        self._check(self.lib.atlas_hip_paged_attention_workspace(self.ctx, byref(cache), q_heads, byref(n)))
+        return n.value
+
+    def paged_attention(self, cache, q, lengths, out, q_heads, scale, window, workspace, workspace_bytes):
+        self._check(self.lib.atlas_hip_paged_attention(self.ctx, byref(cache), _ptr(q), _ptr(lengths), _ptr(out), q_heads, scale,
+                                                       window, _ptr(workspace), workspace_bytes))
+
+    # Log probabilities of given tokens, entropies, likeliest tokens (no counterpart in the reference)
+    def token_logprobs_workspace(self, rows, vocab, top) -> int:
+        n = c_uint64()
+        self._check(self.lib.atlas_hip_token_logprobs_workspace(self.ctx, rows, vocab, top, byref(n)))
+        return n.value
+
+    def token_logprobs(self, logits, row_stride, tokens, given, logprobs, entropy, top_ids, top_logprobs, rows, vocab, top,
+                       inv_temperature, workspace, workspace_bytes):
+        self._check(self.lib.atlas_hip_token_logprobs_f32(
+            self.ctx, _ptr(logits), row_stride, _ptr(tokens), given, _ptr(logprobs), _ptr(entropy), _ptr(top_ids),
+            _ptr(top_logprobs), rows, vocab, top, inv_temperature, _ptr(workspace), workspace_bytes))
+
     # Decode tail: softcap_f32 / argmax_f32 (kernels.metal:931-934, 2033-2066)
     def softcap(self, x, y, n, cap):
         self._check(self.lib.atlas_hip_softcap_f32(self.ctx, _ptr(x), _ptr(y), n, cap))

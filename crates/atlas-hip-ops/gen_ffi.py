@@ -14,7 +14,8 @@ HEADERS = [os.path.join(ROOT, "include", h) for h in ("atlas_hip_ops.h", "atlas_
 SCALARS = {"int": "c_int", "float": "f32", "double": "f64", "size_t": "usize", "uint8_t": "u8", "uint16_t": "u16",
            "uint32_t": "u32", "uint64_t": "u64", "int64_t": "i64", "char": "c_char", "void": "c_void",
            "atlas_hip_ctx": "AtlasHipCtx", "atlas_gguf": "AtlasGguf", "atlas_gguf_tensor": "AtlasGgufTensor",
-           "atlas_dispatch_timing": "AtlasDispatchTiming", "atlas_hip_telemetry": "AtlasHipTelemetry"}
+           "atlas_dispatch_timing": "AtlasDispatchTiming", "atlas_hip_telemetry": "AtlasHipTelemetry",
+           "atlas_paged_cache": "AtlasPagedCache"}
 
 
 def declarations(path):
@@ -70,6 +71,11 @@ def render():
              "    pub dispatches: u64,", "    pub syncs: u64,", "    pub upload_bytes: u64,",
              "    pub readback_bytes: u64,", "    pub allocations: u64,", "    pub resident_bytes: u64,",
              "    pub peak_resident_bytes: u64,", "}", "",
+             "/// atlas_paged_cache (no counterpart in the reference).",
+             "#[repr(C)]", "#[derive(Debug, Clone, Copy)]", "pub struct AtlasPagedCache {",
+             "    pub pages: *mut c_void,", "    pub page_table: *const u32,", "    pub page_count: u32,",
+             "    pub page_size: u32,", "    pub kv_heads: u32,", "    pub head_dim: u32,", "    pub sequences: u32,",
+             "    pub table_width: u32,", "    pub format: c_int,", "}", "",
              "/// atlas_gguf_tensor (GgufTensor, crates/atlas-core/src/gguf.rs:80-87).",
              "#[repr(C)]", "#[derive(Debug, Clone, Copy)]", "pub struct AtlasGgufTensor {",
              "    pub name: *const c_char,", "    pub name_len: u64,", "    pub n_dims: u32,", "    pub dims: [u64; 4],",

@@ -37,6 +37,21 @@ pub struct AtlasHipTelemetry {
     pub peak_resident_bytes: u64,
 }
 
+/// atlas_paged_cache (no counterpart in the reference).
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct AtlasPagedCache {
+    pub pages: *mut c_void,
+    pub page_table: *const u32,
+    pub page_count: u32,
+    pub page_size: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub sequences: u32,
+    pub table_width: u32,
+    pub format: c_int,
+}
+
 /// atlas_gguf_tensor (GgufTensor, crates/atlas-core/src/gguf.rs:80-87).
 #[repr(C)]
 #[derive(Debug, Clone, Copy)]
@@ -137,12 +152,19 @@ extern "C" {
     pub fn atlas_hip_kv_evict_f32(ctx: *mut AtlasHipCtx, cache: *const f32, cache_out: *mut f32, weights: *const f32, weights_out: *mut f32, lengths: *const u32, lengths_out: *mut u32, kept: *mut u32, sequences: u32, capacity: u32, kv_width: u32, budget: u32, recent: u32) -> c_int;
     pub fn atlas_hip_kv_evict_q8_0(ctx: *mut AtlasHipCtx, cache: *const u8, cache_out: *mut u8, weights: *const f32, weights_out: *mut f32, lengths: *const u32, lengths_out: *mut u32, kept: *mut u32, sequences: u32, capacity: u32, kv_width: u32, budget: u32, recent: u32) -> c_int;
     pub fn atlas_hip_kv_evict_q4_0(ctx: *mut AtlasHipCtx, cache: *const u8, cache_out: *mut u8, weights: *const f32, weights_out: *mut f32, lengths: *const u32, lengths_out: *mut u32, kept: *mut u32, sequences: u32, capacity: u32, kv_width: u32, budget: u32, recent: u32) -> c_int;
+    pub fn atlas_hip_paged_cache_bytes(ctx: *mut AtlasHipCtx, cache: *const AtlasPagedCache, bytes: *mut u64) -> c_int;
+    pub fn atlas_hip_paged_append(ctx: *mut AtlasHipCtx, cache: *const AtlasPagedCache, key: *const f32, value: *const f32, query: *const f32, query_out: *mut f32, cosine: *const f32, sine: *const f32, rope_rows: u32, rope_stride: u32, sequence_ids: *const u32, positions: *const u32, tokens: u32, q_heads: u32) -> c_int;
+    pub fn atlas_hip_paged_read(ctx: *mut AtlasHipCtx, cache: *const AtlasPagedCache, sequence_ids: *const u32, positions: *const u32, rows: u32, key: *mut f32, value: *mut f32) -> c_int;
+    pub fn atlas_hip_paged_attention_workspace(ctx: *mut AtlasHipCtx, cache: *const AtlasPagedCache, q_heads: u32, bytes: *mut u64) -> c_int;
+    pub fn atlas_hip_paged_attention(ctx: *mut AtlasHipCtx, cache: *const AtlasPagedCache, q: *const f32, lengths: *const u32, output: *mut f32, q_heads: u32, scale: f32, window: u32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
     pub fn atlas_hip_softcap_f32(ctx: *mut AtlasHipCtx, input: *const f32, output: *mut f32, count: u64, cap: f32) -> c_int;
     pub fn atlas_hip_argmax_f32(ctx: *mut AtlasHipCtx, values: *const f32, selected: *mut u32, rows: u32, count: u32) -> c_int;
     pub fn atlas_hip_softcap_argmax_f32(ctx: *mut AtlasHipCtx, logits: *const f32, capped: *mut f32, selected: *mut u32, rows: u32, count: u32, cap: f32) -> c_int;
     pub fn atlas_hip_softcap_argmax_f32_noalloc(ctx: *mut AtlasHipCtx, logits: *const f32, capped: *mut f32, selected: *mut u32, rows: u32, count: u32, cap: f32) -> c_int;
     pub fn atlas_hip_verify_draft_workspace(ctx: *mut AtlasHipCtx, sequences: u32, drafts: u32, vocab: u32, bytes: *mut u64) -> c_int;
     pub fn atlas_hip_verify_draft_f32(ctx: *mut AtlasHipCtx, target_logits: *const f32, draft_logits: *const f32, draft_tokens: *const u32, draft_lengths: *const u32, accept_uniform: *const f32, sample_uniform: *const f32, accepted: *mut u32, tokens: *mut u32, sequences: u32, drafts: u32, vocab: u32, inv_temperature: f64, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn atlas_hip_token_logprobs_workspace(ctx: *mut AtlasHipCtx, rows: u32, vocab: u32, top: u32, bytes: *mut u64) -> c_int;
+    pub fn atlas_hip_token_logprobs_f32(ctx: *mut AtlasHipCtx, logits: *const f32, row_stride: u64, tokens: *const u32, given: u32, logprobs: *mut f32, entropy: *mut f32, top_ids: *mut u32, top_logprobs: *mut f32, rows: u32, vocab: u32, top: u32, inv_temperature: f64, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
     pub fn atlas_ops_embedding(ctx: *mut AtlasHipCtx, table: *const f32, table_len: usize, vocabulary: usize, hidden: usize, token_ids: *const u32, token_count: usize, output: *mut f32, output_len: usize, timing: *mut AtlasDispatchTiming) -> c_int;
     pub fn atlas_ops_embedding_q6_k(ctx: *mut AtlasHipCtx, weights: *const u8, weights_len: usize, vocabulary: usize, hidden: usize, token_ids: *const u32, token_count: usize, output: *mut f32, output_len: usize, timing: *mut AtlasDispatchTiming) -> c_int;
     pub fn atlas_ops_add(ctx: *mut AtlasHipCtx, lhs: *const f32, lhs_len: usize, rhs: *const f32, rhs_len: usize, output: *mut f32, output_len: usize, timing: *mut AtlasDispatchTiming) -> c_int;

@@ -451,10 +451,11 @@ int atlas_hip_prefix_attention_q4_0(atlas_hip_ctx *ctx, const float *q, const ui
                                     uint32_t sequences, uint32_t tokens, uint32_t q_heads, uint32_t kv_heads,
                                     uint32_t head_dim, float scale, void *workspace, uint64_t workspace_bytes);
 
-/* `format` of the workspace query. */
+/* `format` of the workspace query and of paged caches (F16: those alone). */
 #define ATLAS_CACHE_F32 0
 #define ATLAS_CACHE_Q8_0 1
 #define ATLAS_CACHE_Q4_0 2
+#define ATLAS_CACHE_F16 3
 
 /* No counterpart in the reference.  A batch's own caches (layout as above, a
  * row of kv_width values) cut to `budget` rows by the weights that
@@ -479,6 +480,91 @@ int atlas_hip_kv_evict_q8_0(atlas_hip_ctx *ctx, const uint8_t *cache, uint8_t *c
 int atlas_hip_kv_evict_q4_0(atlas_hip_ctx *ctx, const uint8_t *cache, uint8_t *cache_out, const float *weights,
                             float *weights_out, const uint32_t *lengths, uint32_t *lengths_out, uint32_t *kept,
                             uint32_t sequences, uint32_t capacity, uint32_t kv_width, uint32_t budget, uint32_t recent);
+
+/* ---- decoding from a paged cache ------------------------------------------ */
+
+/* No counterpart in the reference, whose caches are contiguous.
+ *
+ * A cache in pages: position p of sequence b is row p % page_size of page
+ * page_table[b, p / page_size] (device, [sequences, table_width]).  An entry that
+ * names no page (>= page_count; 0xffffffff by custom) holds nothing: its positions
+ * are not written, not seen, and read as zero -- pages behind a sliding window can
+ * be given back.  Sequences may share pages.  page_size is a power of two, 16 to
+ * 4096; head_dim at most 256 and a multiple of 4 (F32), 8 (F16) or 32 (Q8_0,
+ * Q4_0); kv_heads * head_dim <= 32768; table_width * page_size <= 2^29; at most
+ * 2^20 sequences.  The struct is read during the call; the table and whatever else
+ * is on the device when its work runs, so a replayed graph sees their new contents.
+ *
+ * pages: [page_count][K | V][kv_heads][part], 16-byte aligned; a part is one head's
+ * page_size rows of head_dim values.  F32 and F16: [row][head_dim].  Q8_0 and Q4_0:
+ * the codes, [row][head_dim or head_dim / 2 bytes], then the scales, f16
+ * [row / 4][block][row % 4], a block being 32 values (kv_append's encoders).  Q4_0
+ * has two codes a byte, the first one low; a value is (code - 8) * scale.  A key's
+ * codes are in the order of its dims; a value's blocks are taken in runs of 8, 4, 2
+ * and 1 (the binary digits of head_dim / 32, the largest first), a run being
+ * [16][block][2] codes: dims 32 block + 2 i + e of every block, for i = 0 .. 15. */
+typedef struct atlas_paged_cache {
+    void *pages;
+    const uint32_t *page_table;
+    uint32_t page_count;
+    uint32_t page_size;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t sequences;
+    uint32_t table_width;
+    int format; /* ATLAS_CACHE_* */
+} atlas_paged_cache;
+
+/* Bytes of a pool of cache->page_count pages (no pointer of the struct is read). */
+int atlas_hip_paged_cache_bytes(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, uint64_t *bytes);
+
+/* New tokens' keys and values into their pages, the keys rotated to their
+ * positions on the way, and with query the queries too (half-split RoPE, as
+ * rope_half_f32, with the tables' row `position`):
+ *   key, value [tokens, kv_heads, head_dim], query, query_out [tokens, q_heads,
+ *   head_dim] f32 (query_out may be query); cosine, sine [rope_rows, rope_stride],
+ *   rope_rows >= table_width * page_size, rope_stride >= head_dim / 2.
+ * cosine and sine NULL: nothing is rotated, and query is NULL.  sequence_ids NULL:
+ * token t is sequence t's (tokens <= sequences).  A token whose sequence or position
+ * (>= table_width * page_size) is out of range is skipped, query row and all:
+ * padding.  The rows of a call should be distinct: of two tokens at one position, the
+ * row has each value from either.  Rows are bit-equal to rope_half_f32's, rounded to
+ * nearest for F16, encoded block by block as kv_append does for Q8_0 and Q4_0.  key,
+ * value, query and query_out are 16-byte aligned; tokens * (q_heads + 2 kv_heads) <=
+ * 2^25. */
+int atlas_hip_paged_append(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, const float *key, const float *value,
+                           const float *query, float *query_out, const float *cosine, const float *sine,
+                           uint32_t rope_rows, uint32_t rope_stride, const uint32_t *sequence_ids,
+                           const uint32_t *positions, uint32_t tokens, uint32_t q_heads);
+
+/* Cached rows as f32: key and value [rows, kv_heads, head_dim] (either may be
+ * NULL), row r of sequence sequence_ids[r] (NULL: r) at positions[r]; zeros where
+ * there is no such row.  Outputs are 16-byte aligned. */
+int atlas_hip_paged_read(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, const uint32_t *sequence_ids,
+                         const uint32_t *positions, uint32_t rows, float *key, float *value);
+
+/* Attention of one new token of each sequence (append it first):
+ *   x_j    = scale * (q . k_j) over positions lo <= j < len_b whose page is there,
+ *            len_b = min(lengths[b], table_width * page_size), lo = window &&
+ *            len_b > window ? len_b - window : 0
+ *   output = sum_j e^{x_j} v_j / sum_j e^{x_j};  zero where nothing is seen
+ * q and output [sequences, q_heads, head_dim] f32; query head h reads KV head
+ * h / (q_heads / kv_heads).  What a token does not see never reaches it, whatever it
+ * holds; what it sees has to be finite.  Scores, weights and sums are f32; with F16,
+ * Q8_0 and Q4_0 rows the products' other operands are two f16 numbers or three bf16
+ * ones each, f32's bits.  A score is off by up to (head_dim + 24) 2^-24 of |scale|
+ * sum_i |q_i k_i|, which moves its weight by a factor; apart from that a result is
+ * within 1e-5 of float64 normwise, at any number of positions.  A call's result does
+ * not depend on timing.  q, output and the workspace are 16-byte aligned; output
+ * overlaps neither q nor the pages; sequences * q_heads <= 2^23.  The workspace
+ * (atlas_hip_paged_attention_workspace bytes; no pointer of the struct is read) is
+ * overwritten by every call and holds nothing between calls: calls that can overlap,
+ * and graphs whose replays can, need one each. */
+int atlas_hip_paged_attention_workspace(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, uint32_t q_heads,
+                                        uint64_t *bytes);
+int atlas_hip_paged_attention(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, const float *q,
+                              const uint32_t *lengths, float *output, uint32_t q_heads, float scale, uint32_t window,
+                              void *workspace, uint64_t workspace_bytes);
 
 /* ---- logits: soft cap and greedy argmax (decode tail) -------------------- */
 
@@ -558,6 +644,27 @@ int atlas_hip_verify_draft_f32(atlas_hip_ctx *ctx, const float *target_logits, c
                                const float *accept_uniform, const float *sample_uniform, uint32_t *accepted,
                                uint32_t *tokens, uint32_t sequences, uint32_t drafts, uint32_t vocab,
                                double inv_temperature, void *workspace, uint64_t workspace_bytes);
+
+/* No counterpart in the reference.  Log probabilities of p = softmax(logits[r] *
+ * inv_temperature) over `vocab` logits a row, rows `row_stride` values apart:
+ *   logprobs[r, g]     = log p of tokens[r, g], g < given (-inf for a token >= vocab)
+ *   entropy[r]         = -sum_i p_i log p_i (NULL: none)
+ *   top_ids[r, i], top_logprobs[r, i], i < top: the likeliest tokens, by logit, of
+ *                        equal logits the lowest token first; 0xffffffff and -inf
+ *                        behind the last token with a logit above -inf
+ * given and top may be 0, their buffers NULL then, but something is asked for.
+ * NaN and -inf logits have no mass and a log probability of -inf; all of a row's mass
+ * lies on its +inf; a row without mass has entropy 0.  Probabilities and sums are
+ * float64, in a fixed order; results are rounded to f32 once.  At most 2^29 logits a
+ * row, 64 likeliest tokens, and 2^23 times 4096 logits in all (a row counts in whole
+ * 4096s).  Outputs overlap neither inputs nor each other.  Workspace as for
+ * paged_attention. */
+int atlas_hip_token_logprobs_workspace(atlas_hip_ctx *ctx, uint32_t rows, uint32_t vocab, uint32_t top,
+                                       uint64_t *bytes);
+int atlas_hip_token_logprobs_f32(atlas_hip_ctx *ctx, const float *logits, uint64_t row_stride, const uint32_t *tokens,
+                                 uint32_t given, float *logprobs, float *entropy, uint32_t *top_ids,
+                                 float *top_logprobs, uint32_t rows, uint32_t vocab, uint32_t top,
+                                 double inv_temperature, void *workspace, uint64_t workspace_bytes);
 
 /* ---- host-slice operator API (atlas_ops::NeuralOps) --------------------- */
 

@@ -1,0 +1,147 @@
+"""CPU tests of the paged decode ops: which calls are refused and that the calls
+the documentation allows are not, and the layout of a page, compiled from their
+headers by the host compiler; no device."""
+import ctypes
+import math
+import os
+import subprocess
+from ctypes import c_char_p, c_double, c_float, c_int, c_uint32, c_uint64
+
+import numpy as np
+import pytest
+
+import paged_refs as ref
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+U32, U64 = c_uint32, c_uint64
+CACHE_TYPES = [c_int, U64, U64] + [U32] * 6
+
+
+@pytest.fixture(scope="module")
+def checks(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("checks") / "libpaged_checks.so")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-shared", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-I/opt/rocm/include",
+                    "-o", so, os.path.join(HERE, "cpp", "paged_checks.cpp")], check=True)
+    lib = ctypes.CDLL(so)
+    lib.paged_bytes.argtypes, lib.paged_bytes.restype = CACHE_TYPES, U64
+    lib.value_place.argtypes, lib.value_place.restype = [U32, U32], U32
+    lib.check_append.argtypes = CACHE_TYPES + [U64] * 8 + [U32] * 4
+    lib.check_read.argtypes = CACHE_TYPES + [U64] * 4 + [U32]
+    lib.check_attention.argtypes = CACHE_TYPES + [U64] * 3 + [U32, U32, c_float, U64]
+    lib.check_logprobs.argtypes = [U64] * 7 + [U32] * 4 + [c_double, U64]
+    for f in (lib.check_append, lib.check_read, lib.check_attention, lib.check_logprobs):
+        f.restype = c_char_p
+    return lib
+
+
+M = 1 << 40  # addresses far apart
+CACHE = dict(format=0, pages=M, table=2 * M, page_count=100, page_size=16, kv_heads=2, head_dim=128, sequences=4, table_width=20)
+APPEND = dict(CACHE, key=3 * M, value=4 * M, query=5 * M, query_out=6 * M, cosine=7 * M, sine=8 * M, ids=9 * M, positions=10 * M,
+              rope_rows=320, rope_stride=64, tokens=7, q_heads=8)
+READ = dict(CACHE, ids=3 * M, positions=4 * M, key=5 * M, value=6 * M, rows=9)
+ATTEND = dict(CACHE, q=3 * M, lengths=4 * M, output=5 * M, q_heads=8, window=0, scale=0.1, workspace=6 * M)
+LOGPROBS = dict(logits=M, row_stride=1000, tokens=2 * M, logprobs=3 * M, entropy=4 * M, top_ids=5 * M, top_logprobs=6 * M, rows=4,
+                vocab=1000, given=1, top=5, inv_temperature=1.0, workspace=7 * M)
+GOOD_CACHES = [{}, dict(format=3), dict(format=1), dict(format=2), dict(head_dim=4, rope_stride=2), dict(format=3, head_dim=8),
+               dict(format=1, head_dim=256, rope_stride=128), dict(format=2, head_dim=96), dict(page_size=4096, rope_rows=81920),
+               dict(kv_heads=1), dict(page_count=1), dict(page_count=1 << 20)]
+BAD_CACHES = [dict(format=4), dict(format=-1), dict(pages=0), dict(table=0), dict(page_count=0), dict(page_count=0xFFFFFFFF),
+              dict(page_size=0), dict(page_size=8), dict(page_size=48), dict(page_size=8192), dict(kv_heads=0),
+              dict(kv_heads=257), dict(head_dim=0), dict(head_dim=6), dict(head_dim=260), dict(format=3, head_dim=12),
+              dict(format=1, head_dim=48), dict(format=2, head_dim=16), dict(sequences=0), dict(sequences=(1 << 20) + 1),
+              dict(table_width=0), dict(table_width=(1 << 25) + 1), dict(pages=M + 8), dict(table=2 * M + 2)]
+
+
+def call(fn, base, change):
+    return fn(*{**base, **{k: v for k, v in change.items() if k in base}}.values())
+
+
+@pytest.mark.parametrize("change", GOOD_CACHES)
+def test_caches_that_are_allowed(checks, change):
+    assert call(checks.check_append, APPEND, change) is None
+    assert call(checks.check_read, READ, change) is None
+    assert call(checks.check_attention, ATTEND, change) is None
+
+
+@pytest.mark.parametrize("change", BAD_CACHES)
+def test_caches_that_are_refused(checks, change):
+    for fn, base in ((checks.check_append, APPEND), (checks.check_read, READ), (checks.check_attention, ATTEND)):
+        assert call(fn, base, change)
+
+
+@pytest.mark.parametrize("change", [
+    dict(query=0, query_out=0), dict(query=0, query_out=0, cosine=0, sine=0, rope_rows=0, rope_stride=0, q_heads=0),
+    dict(query_out=5 * M), dict(ids=0, tokens=4), dict(tokens=1), dict(rope_rows=400, rope_stride=100), dict(q_heads=1),
+    dict(cosine=7 * M + 4, sine=8 * M + 4), dict(tokens=(1 << 25) // 12),
+])
+def test_append_calls_that_are_allowed(checks, change):
+    assert call(checks.check_append, APPEND, change) is None
+
+
+@pytest.mark.parametrize("change", [
+    dict(key=0), dict(value=0), dict(positions=0), dict(tokens=0), dict(ids=0, tokens=5), dict(cosine=0), dict(sine=0),
+    dict(cosine=0, sine=0), dict(query_out=0), dict(query=0), dict(q_heads=0), dict(rope_rows=319), dict(rope_stride=63),
+    dict(key=3 * M + 4), dict(value=4 * M + 8), dict(query=5 * M + 4), dict(query_out=6 * M + 4), dict(cosine=7 * M + 2),
+    dict(positions=10 * M + 1), dict(ids=9 * M + 2), dict(query_out=5 * M + 16), dict(key=M + 1024), dict(value=M + 1024),
+    dict(query=M + 1024), dict(query_out=M + 1024), dict(query_out=3 * M), dict(query_out=4 * M), dict(tokens=(1 << 25) // 12 + 1),
+    dict(q_heads=0xFFFFFFFF),
+])
+def test_append_calls_that_are_refused(checks, change):
+    assert call(checks.check_append, APPEND, change)
+
+
+@pytest.mark.parametrize("change,fine", [
+    ({}, True), (dict(key=0), True), (dict(value=0), True), (dict(ids=0, rows=4), True), (dict(rows=(1 << 25) // 4), True),
+    (dict(key=0, value=0), False), (dict(positions=0), False), (dict(rows=0), False), (dict(ids=0, rows=5), False),
+    (dict(key=5 * M + 4), False), (dict(value=6 * M + 4), False), (dict(key=M + 16), False), (dict(value=M + 16), False),
+    (dict(value=5 * M), False), (dict(positions=4 * M + 2), False), (dict(ids=3 * M + 2), False), (dict(rows=(1 << 25) // 4 + 1), False),
+])
+def test_read_calls(checks, change, fine):
+    assert (call(checks.check_read, READ, change) is None) == fine
+
+
+@pytest.mark.parametrize("change,fine", [
+    ({}, True), (dict(window=1), True), (dict(window=0xFFFFFFFF), True), (dict(q_heads=2), True), (dict(q_heads=64), True),
+    (dict(scale=0.0), True), (dict(scale=-1.0), True), (dict(sequences=1 << 20, q_heads=8), True),
+    (dict(q=0), False), (dict(lengths=0), False), (dict(output=0), False), (dict(workspace=0), False), (dict(q_heads=0), False),
+    (dict(q_heads=7), False), (dict(scale=math.nan), False), (dict(scale=math.inf), False), (dict(q=3 * M + 4), False),
+    (dict(output=5 * M + 8), False), (dict(workspace=6 * M + 8), False), (dict(lengths=4 * M + 2), False), (dict(output=3 * M), False),
+    (dict(output=M + 16), False), (dict(sequences=1 << 20, q_heads=10), False),
+])
+def test_attention_calls(checks, change, fine):
+    assert (call(checks.check_attention, ATTEND, change) is None) == fine
+
+
+@pytest.mark.parametrize("change,fine", [
+    ({}, True), (dict(given=0, tokens=0, logprobs=0), True), (dict(entropy=0), True), (dict(top=0, top_ids=0, top_logprobs=0), True),
+    (dict(top=64), True), (dict(vocab=1), True), (dict(row_stride=1 << 40), True), (dict(vocab=1 << 29, row_stride=1 << 29), True),
+    (dict(inv_temperature=5e-324), True), (dict(inv_temperature=1.7e308), True), (dict(rows=1 << 23), True),
+    (dict(logits=0), False), (dict(workspace=0), False), (dict(tokens=0), False), (dict(logprobs=0), False), (dict(top_ids=0), False),
+    (dict(top_logprobs=0), False), (dict(rows=0), False), (dict(vocab=0), False), (dict(top=65), False), (dict(row_stride=999), False),
+    (dict(given=0, top=0, entropy=0), False), (dict(inv_temperature=0.0), False), (dict(inv_temperature=-1.0), False),
+    (dict(inv_temperature=math.nan), False), (dict(inv_temperature=math.inf), False), (dict(logits=M + 2), False),
+    (dict(tokens=2 * M + 2), False), (dict(workspace=7 * M + 8), False), (dict(rows=(1 << 23) + 1), False),
+    (dict(vocab=(1 << 29) + 1, row_stride=1 << 30), False),
+])
+def test_logprob_calls(checks, change, fine):
+    assert (call(checks.check_logprobs, LOGPROBS, change) is None) == fine
+
+
+def test_pages_have_their_bytes(checks):
+    for fmt, name in enumerate(("f32", "q8_0", "q4_0", "f16")):
+        for ps in (16, 64, 4096):
+            for D in (32, 96, 160, 224, 256):
+                got = call(checks.paged_bytes, CACHE, dict(format=fmt, page_size=ps, head_dim=D, kv_heads=3, page_count=7))
+                assert got == 7 * 2 * 3 * ref.part_bytes(name, ps, D)
+                assert ref.part_bytes(name, ps, D) % 16 == 0  # every part is as aligned as the pool
+    big = call(checks.paged_bytes, CACHE, dict(page_count=0xFFFFFFFE, page_size=4096, kv_heads=128, head_dim=256))
+    assert big == 0xFFFFFFFE * 2 * 128 * 4096 * 1024
+
+
+@pytest.mark.parametrize("D", range(32, 257, 32))
+def test_a_values_codes_are_where_the_layout_says(checks, D):
+    order = ref.value_order(D)
+    assert sorted(order) == list(range(D))
+    place = np.argsort(order)
+    for d in range(0, D, 2):
+        assert checks.value_place(D, d) == place[d] and place[d + 1] == place[d] + 1
