@@ -187,10 +187,15 @@ inline const char* paged_read_error(const PagedReadArgs& a) {
     return nullptr;
 }
 
+// Units of 16 positions are counted in 32 bits.
+constexpr uint64_t kMostPagedPositions = 1ull << 35;
+
 inline const char* paged_attention_sizes_error(const PagedCache& c, uint32_t q_heads) {
     if (const char* error = paged_cache_sizes_error(c)) return error;
     if (q_heads == 0 || q_heads % c.kv_heads != 0) return "paged attention needs q_heads a multiple of kv_heads";
     if (static_cast<uint64_t>(c.sequences) * q_heads > kMostGroups) return "paged attention has more than 2^23 query rows";
+    if (static_cast<uint64_t>(c.table_width) * c.page_size * c.sequences > kMostPagedPositions)
+        return "paged attention is limited to 2^35 positions of all sequences together";
     return nullptr;
 }
 

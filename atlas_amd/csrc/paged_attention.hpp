@@ -24,6 +24,11 @@ inline constexpr int kPagedAttnThreads = 256;
 inline constexpr int kPagedAttnWaves = kPagedAttnThreads / kWave;
 inline constexpr uint32_t kPagedHeads = 16;  // query heads of a row: the columns of a product
 
+// The first and last part of a row.
+struct PagedRow {
+    uint32_t first, last;
+};
+
 struct PagedAttnParams {
     const float* q;
     const uint8_t* pages;
@@ -32,6 +37,7 @@ struct PagedAttnParams {
     float* output;
     float* partial_out;   // [2 parts][heads][head_dim]
     float2* partial_ml;   // [2 parts][heads]
+    PagedRow* rows;       // [sequences][kv_heads][head_tiles], of rows that see something
     uint64_t page_bytes;
     uint32_t part_bytes, page_count, page_shift, table_width, sequences, capacity;
     uint32_t kv_heads, group, head_tiles, heads, q_heads, head_dim, window;
@@ -39,9 +45,9 @@ struct PagedAttnParams {
     float scale;                                 // with log2(e)
 };
 
-// Keys of a wavefront's step: two tiles of 16 where a product over keys takes 32.
+// Keys of a wavefront's step, the unit of the split: two tiles of 16 where a
+// product over keys takes 32.
 __host__ __device__ constexpr uint32_t paged_keys(int format) { return format == kKvF32 ? 16 : 32; }
-__host__ __device__ constexpr uint32_t paged_unit(int format) { return kPagedAttnWaves * paged_keys(format); }
 // Workgroups to a CU.
 __host__ __device__ constexpr uint32_t paged_occupancy(uint32_t head_dim) { return head_dim <= 64 ? 4 : (head_dim <= 128 ? 3 : 2); }
 
@@ -61,20 +67,6 @@ __device__ __forceinline__ uint64_t parts_of(const PagedAttnParams& a, uint64_t 
     parts = parts > a.few_parts ? parts : a.few_parts;
     parts = parts < a.most_parts ? parts : a.most_parts;
     return parts < total ? parts : total;
-}
-
-// Sums over the workgroup, the result in every thread.
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d, kWave);
-    return v;
-}
-__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, uint64_t (&room)[kPagedAttnWaves]) {
-    v = wave_sum_u64(v);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) room[threadIdx.x / kWave] = v;
-    __syncthreads();
-    return (room[0] + room[1]) + (room[2] + room[3]);
 }
 
 __device__ __forceinline__ uint64_t uniform_u64(uint64_t v) {
@@ -139,14 +131,14 @@ struct ValueWords {
 // with keys 4 g + r of each tile, which is the operand that O^T = V^T P^T wants if
 // the order of its keys is (tile, r) for each g; so P never leaves its lane and
 // a head's statistics are the lane's own.
-template <int FMT, int NB>
+template <int FMT, int NB, int HP>
 struct Step;
 
 // f32 throughout (v_mfma_f32_16x16x4): 20 TB/s of keys and values, whatever the
 // number of heads.
 template <int NB>
-struct Step<kKvF32, NB> {
-    static constexpr int kTiles = 1, kOut = 2 * NB, kQuads = NB / 2;
+struct Step<kKvF32, NB, 16> {
+    static constexpr int kTiles = 1, kOut = 2 * NB, kQuads = NB / 2, kQueryBytes = 2 * NB * kWave * 16;
     static constexpr float kUnscale = 1.0f;
     f32x4 k[2 * NB];
     f32x4 v[4][kQuads ? kQuads : 1];
@@ -174,13 +166,13 @@ struct Step<kKvF32, NB> {
             }
         }
     }
-    template <class Room>
-    __device__ __forceinline__ void scores(const Room& room, uint32_t lane, float, f32x4 (&s)[1]) const {
+    static __device__ __forceinline__ uint32_t query_lane(uint32_t c, uint32_t g) { return (c + 16 * g) * 16; }
+    __device__ __forceinline__ void scores(const uint8_t* queries, uint32_t, float, f32x4 (&s)[1]) const {
         f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
         s[0] = t;
 #pragma unroll
         for (int i = 0; i < 2 * NB; i += 2) {
-            const f32x4 q0 = room.queries[i][lane], q1 = room.queries[i + 1][lane];
+            const f32x4 q0 = *reinterpret_cast<const f32x4*>(queries + i * 1024), q1 = *reinterpret_cast<const f32x4*>(queries + i * 1024 + 1024);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i][j], q0[j], s[0], 0, 0, 0);
@@ -224,7 +216,7 @@ struct Step<kKvF32, NB> {
         }
     }
     // O^T has dims in its rows: tile 4 u + j row i is dim 64 u + 4 i + j
-    static __device__ __forceinline__ void put(float* line, uint32_t g, const f32x4 (&out)[kOut]) {
+    static __device__ __forceinline__ void put(float* line, uint32_t, uint32_t g, const f32x4 (&out)[kOut]) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
 #pragma unroll
@@ -250,9 +242,10 @@ __device__ __forceinline__ void f16_pieces(float x, _Float16& hi, _Float16& lo) 
 // that the sums are divided by.  A query's pieces lose 2^-24 of each number, or
 // 2^-39 of the row's largest; a weight's 2^-24, or 2^-40.
 template <int NB>
-struct Step<kKvF16, NB> {
-    static constexpr int kTiles = 2, kOut = 2 * NB, kQuads = NB / 2;
+struct Step<kKvF16, NB, 16> {
+    static constexpr int kTiles = 2, kOut = 2 * NB, kQuads = NB / 2, kQueryBytes = 2 * NB * kWave * 16;
     static constexpr float kUnscale = 0x1p-15f;
+    static constexpr uint32_t kHeadLines = kPagedHeads, kItemsPadded = 4 * NB;
     u32x4_t k[2][NB];
     u32x2_t v[8][kQuads ? kQuads : 1];
     uint32_t v2[8];
@@ -282,13 +275,18 @@ struct Step<kKvF16, NB> {
             }
         }
     }
-    template <class Room>
-    __device__ __forceinline__ void scores(const Room& room, uint32_t lane, float unscale, f32x4 (&s)[2]) const {
+    static __device__ __forceinline__ uint32_t query_lane(uint32_t c, uint32_t g) { return (c + 16 * g) * 16; }
+    static __device__ __forceinline__ void put_query(uint8_t* room, uint32_t head, uint32_t it, f16x8_t hi, f16x8_t lo) {
+        uint8_t* to = room + it / 4 * 2048 + (it % 4 * 16 + head) * 16;
+        *reinterpret_cast<f16x8_t*>(to) = hi;
+        *reinterpret_cast<f16x8_t*>(to + 1024) = lo;
+    }
+    __device__ __forceinline__ void scores(const uint8_t* queries, uint32_t, float unscale, f32x4 (&s)[2]) const {
         s[0] = s[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const f16x8_t hi = __builtin_bit_cast(f16x8_t, room.queries[2 * b][lane]);
-            const f16x8_t lo = __builtin_bit_cast(f16x8_t, room.queries[2 * b + 1][lane]);
+            const f16x8_t hi = *reinterpret_cast<const f16x8_t*>(queries + b * 2048);
+            const f16x8_t lo = *reinterpret_cast<const f16x8_t*>(queries + b * 2048 + 1024);
 #pragma unroll
             for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, k[h][b]), hi, s[h], 0, 0, 0);
 #pragma unroll
@@ -344,8 +342,8 @@ struct Step<kKvF16, NB> {
             one(column<1>(v2), out[4 * kQuads + 1]);
         }
     }
-    static __device__ __forceinline__ void put(float* line, uint32_t g, const f32x4 (&out)[kOut]) {
-        Step<kKvF32, NB>::put(line, g, out);
+    static __device__ __forceinline__ void put(float* line, uint32_t c, uint32_t g, const f32x4 (&out)[kOut]) {
+        Step<kKvF32, NB, 16>::put(line, c, g, out);
     }
     static __device__ constexpr uint32_t query_dim(uint32_t j) { return j; }
 };
@@ -355,51 +353,81 @@ struct Step<kKvF16, NB> {
 // numbers: the 24 bits of an f32, cut in three, over its whole range.  A key's
 // scale goes on the product of its block, a value's on the weight, so codes are
 // only unpacked.
-template <int FMT, int NB>
+//
+// A product has 16 columns and a row HP heads at most (4, 8 or 16): columns are
+// (block, head), not heads alone.  For the keys that lets a lane load 16 bytes of its
+// row at once, though they are another block than its neighbours': a column takes
+// one block (its query is zero for the others'), and one scale goes on its result.
+// (Loads of 8 or 4 bytes a lane, rows apart, keep the address unit busy for 64
+// cycles whatever they bring: 4.7 and 2.4 TB/s of the 6.2 that 16 bytes reach.)  For
+// the values a lane cuts the weights of one block in 16 / HP, not of all.
+template <int FMT, int NB, int HP>
 struct Step {
     static_assert(FMT == kKvQ8_0 || FMT == kKvQ4_0);
     static constexpr bool kBytes = FMT == kKvQ8_0;
-    static constexpr int kTiles = 2, kOut = 2 * NB, kKeyWords = kBytes ? 2 : 1, kBlock = kBytes ? 2 : 1;
+    static constexpr int kTiles = 2, kOut = 2 * NB, kBlock = kBytes ? 2 : 1, kRow = NB * (kBytes ? 32 : 16);
     static constexpr ValueWords<NB, kBlock> kWords{};
     // v_cvt_off_f32_i4 gives sixteenths
     static constexpr float kUnscale = kBytes ? 1.0f : 16.0f;
-    uint32_t k[2][NB][kKeyWords];
-    u32x2_t ks[2][NB], vs[2][NB];  // scales of keys 4 g + r
+    // keys: blocks to the columns, heads to a product, products for all heads; steps of kKeyBlocks blocks; chunks of
+    // 8 dims of a lane's 16 bytes
+    static constexpr int kKeyBlocks = kBytes ? 2 : 4, kKeyHeads = 16 / kKeyBlocks, kSets = HP > kKeyHeads ? HP / kKeyHeads : 1;
+    static constexpr int kKeySteps = (NB + kKeyBlocks - 1) / kKeyBlocks, kChunks = kBytes ? 2 : 4;
+    // values: blocks to the columns
+    static constexpr int kValueBlocks = 16 / HP, kValueSteps = (NB + kValueBlocks - 1) / kValueBlocks;
+    // queries in LDS: for each step, chunk, piece and set, the lanes that are not zero; then as much of zeros
+    static constexpr int kQueryLanes = 64 / kKeyBlocks, kQueries = kKeySteps * kChunks * 2 * kSets;
+    static constexpr int kQueryBytes = kQueries * kQueryLanes * 16;
+    static constexpr uint32_t kHeadLines = kSets * kKeyHeads, kItemsPadded = 4 * kKeySteps * kKeyBlocks;
+
+    u32x4_t k[2][kKeySteps];
+    u32x2_t ks[2][kKeySteps], vs[2][kValueSteps];  // scales of keys 4 g + r
     uint32_t v[8][kWords.words];
-    static __device__ __forceinline__ uint32_t row_bytes(uint32_t head_dim) { return kBytes ? head_dim : head_dim / 2; }
-    static __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rs, const PagedAttnParams& a, uint32_t row, uint32_t g,
-                                                       u32x2_t (&s)[NB]) {
-        const uint32_t base = (row_bytes(NB * 32) << a.page_shift) + row / 4 * NB * 8, off = g * NB * 8;
-#pragma unroll
-        for (int b = 0; b + 1 < NB; b += 2) {
-            const u32x4_t x = load16(rs, off + b * 8, base);
-            s[b] = u32x2_t{x[0], x[1]};
-            s[b + 1] = u32x2_t{x[2], x[3]};
-        }
-        if constexpr (NB % 2) s[NB - 1] = load8(rs, off + (NB - 1) * 8, base);
+
+    static __device__ __forceinline__ uint32_t key_block(uint32_t c) { return c / kKeyHeads; }
+    static __device__ __forceinline__ uint32_t query_at(int i, int m, int piece, int set) {
+        return (((i * kChunks + m) * 2 + piece) * kSets + set) * kQueryLanes * 16;
     }
-    __device__ __forceinline__ void load_keys(const PageRows (&p)[2], uint32_t c, uint32_t g, const PagedAttnParams& a) {
+    // Where a lane reads its query: block key_block(c) of a step is in lanes g (Q4_0) or 2 g, 2 g + 1 (Q8_0).
+    static __device__ __forceinline__ uint32_t query_lane(uint32_t c, uint32_t g) {
+        const bool mine = (kBytes ? g / 2 : g) == key_block(c);
+        return mine ? (c % kKeyHeads + kKeyHeads * g) * 16 : kQueryBytes;
+    }
+    // Item `it` of a head's query, 8 dims of block it / 4.
+    static __device__ __forceinline__ void put_query(uint8_t* room, uint32_t head, uint32_t it, f16x8_t hi, f16x8_t lo) {
+        const uint32_t block = it / 4, i = block / kKeyBlocks, set = head / kKeyHeads, h = head % kKeyHeads;
+        const uint32_t m = kBytes ? it % 2 : it % 4, g = kBytes ? block % 2 * 2 + it % 4 / 2 : block % 4;
+        uint8_t* to = room + query_at(i, m, 0, set) + (h + kKeyHeads * g) * 16;
+        *reinterpret_cast<f16x8_t*>(to) = hi;
+        *reinterpret_cast<f16x8_t*>(to + query_at(0, 0, 1, 0)) = lo;
+    }
+    template <int STEPS>
+    static __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rs, uint32_t page_shift, uint32_t row, uint32_t g,
+                                                       uint32_t block, int blocks, u32x2_t (&s)[STEPS]) {
+        const uint32_t base = (kRow << page_shift) + row / 4 * NB * 8, off = g * NB * 8 + block * 8;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            const bool there = (i + 1) * blocks <= NB || block + i * blocks < NB;
+            s[i] = load8(rs, there ? off + i * blocks * 8 : kPastPage, base);
+        }
+    }
+    __device__ __forceinline__ void load_keys(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t page_shift) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const uint32_t base = p[h].row * row_bytes(NB * 32);
-                if constexpr (kBytes) {
-                    const u32x2_t x = load8(p[h].keys, c * NB * 32 + b * 32 + 8 * g, base);
-                    k[h][b][0] = x[0];
-                    k[h][b][1] = x[1];
-                } else {
-                    k[h][b][0] = load4(p[h].keys, c * NB * 16 + b * 16 + 4 * g, base);
-                }
+            for (int i = 0; i < kKeySteps; ++i) {
+                const uint32_t in_row = i * 64 + 16 * g;
+                const uint32_t off = (i + 1) * 64 <= kRow || in_row < kRow ? c * kRow + in_row : kPastPage;
+                k[h][i] = load16(p[h].keys, off, p[h].row * kRow);
             }
-            load_scales(p[h].keys, a, p[h].row, g, ks[h]);
+            load_scales(p[h].keys, page_shift, p[h].row, g, key_block(c), kKeyBlocks, ks[h]);
         }
     }
-    __device__ __forceinline__ void load_values(const PageRows (&p)[2], uint32_t c, uint32_t g, const PagedAttnParams& a) {
+    __device__ __forceinline__ void load_values(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t page_shift) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const __amdgpu_buffer_rsrc_t rs = p[j / 4].values;
-            const uint32_t base = p[j / 4].row * row_bytes(NB * 32), line = (4 * g + j % 4) * row_bytes(NB * 32);
+            const uint32_t base = p[j / 4].row * kRow, line = (4 * g + j % 4) * kRow;
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (kWords.first[b] != b) continue;  // a run starts here
@@ -423,20 +451,20 @@ struct Step {
             }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) load_scales(p[h].values, a, p[h].row, g, vs[h]);
+        for (int h = 0; h < 2; ++h) load_scales(p[h].values, page_shift, p[h].row, g, c / HP, kValueBlocks, vs[h]);
     }
     // Eight codes of a key as f16: 1024 + (a code without its sign) has it in its low bits.
-    static __device__ __forceinline__ f16x8_t key_codes(const uint32_t (&w)[kKeyWords]) {
+    static __device__ __forceinline__ f16x8_t key_codes(u32x4_t w, int m) {
         u32x4_t x;
         _Float16 less;
         if constexpr (kBytes) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                x[i] = __builtin_amdgcn_perm(0x64646464u, w[i / 2] ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u);
+                x[i] = __builtin_amdgcn_perm(0x64646464u, w[2 * m + i / 2] ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u);
             less = static_cast<_Float16>(-1152.0f);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = (w[0] >> (4 * i) & 0x000f000fu) | 0x64006400u;
+            for (int i = 0; i < 4; ++i) x[i] = (w[m] >> (4 * i) & 0x000f000fu) | 0x64006400u;
             less = static_cast<_Float16>(-1032.0f);
         }
 #pragma unroll
@@ -444,25 +472,51 @@ struct Step {
         return __builtin_bit_cast(f16x8_t, x);
     }
     static __device__ __forceinline__ float scale_of(u32x2_t s, int r) { return h2f(static_cast<uint16_t>(s[r / 2] >> (16 * (r % 2)))); }
-    template <class Room>
-    __device__ __forceinline__ void scores(const Room& room, uint32_t lane, float unscale, f32x4 (&s)[2]) const {
-        s[0] = s[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    __device__ __forceinline__ void scores(const uint8_t* queries, uint32_t c, float unscale, f32x4 (&s)[2]) const {
+        f32x4 sum[kSets][2];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const f16x8_t hi = __builtin_bit_cast(f16x8_t, room.queries[2 * b][lane]);
-            const f16x8_t lo = __builtin_bit_cast(f16x8_t, room.queries[2 * b + 1][lane]);
+        for (int set = 0; set < kSets; ++set) sum[set][0] = sum[set][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const f16x8_t x = key_codes(k[h][b]);
-                f32x4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, hi, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, lo, d, 0, 0, 0);
+        for (int i = 0; i < kKeySteps; ++i) {
+            f32x4 d[kSets][2];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[h][r] = __builtin_fmaf(d[r], scale_of(ks[h][b], r), s[h][r]);
+            for (int set = 0; set < kSets; ++set) d[set][0] = d[set][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int m = 0; m < kChunks; ++m) {
+                const f16x8_t x[2] = {key_codes(k[0][i], m), key_codes(k[1][i], m)};
+#pragma unroll
+                for (int set = 0; set < kSets; ++set)
+#pragma unroll
+                    for (int piece = 0; piece < 2; ++piece) {
+                        const f16x8_t q = *reinterpret_cast<const f16x8_t*>(queries + query_at(i, m, piece, set));
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) d[set][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[h], q, d[set][h], 0, 0, 0);
+                    }
+                if (m % 2) __builtin_amdgcn_sched_barrier(0);
             }
-            if (b % 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int set = 0; set < kSets; ++set)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sum[set][h][r] = __builtin_fmaf(d[set][h][r], scale_of(ks[h][i], r), sum[set][h][r]);
         }
-        s[0] *= unscale;
-        s[1] *= unscale;
+        // a head's blocks from its columns; then every lane its own head, c % HP
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float x[kSets];
+#pragma unroll
+                for (int set = 0; set < kSets; ++set) {
+                    x[set] = sum[set][h][r] + dpp_f32<0x128, 0xf, false>(sum[set][h][r]);                    // row_ror:8
+                    if constexpr (!kBytes) x[set] = x[set] + dpp_f32<0x124, 0xf, false>(x[set]);  // row_ror:4
+                }
+                float y = x[0];
+                if constexpr (kSets == 2) y = c % HP >= kKeyHeads ? x[1] : x[0];
+                if constexpr (kSets == 4) y = c >= 8 ? (c >= 12 ? x[3] : x[2]) : (c >= 4 ? x[1] : x[0]);
+                s[h][r] = y * unscale;
+            }
     }
     __device__ __forceinline__ void keep(const bool (&seen)[2][4]) {
 #pragma unroll
@@ -471,7 +525,7 @@ struct Step {
             for (int i = 0; i < 2; ++i) {
                 const uint32_t mask = (seen[h][2 * i] ? 0xffffu : 0u) | (seen[h][2 * i + 1] ? 0xffff0000u : 0u);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) vs[h][b][i] &= mask;
+                for (int b = 0; b < kValueSteps; ++b) vs[h][b][i] &= mask;
             }
     }
     static __device__ __forceinline__ uint32_t upper(float odd, float even) {  // their upper halves
@@ -497,13 +551,13 @@ struct Step {
     }
     __device__ __forceinline__ void add(const f32x4 (&p)[2], f32x4 (&out)[kOut]) const {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
+        for (int step = 0; step < kValueSteps; ++step) {
             u32x4_t piece[3];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float w[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) w[j] = p[i / 2][i % 2 * 2 + j] * scale_of(vs[i / 2][b], i % 2 * 2 + j);
+                for (int j = 0; j < 2; ++j) w[j] = p[i / 2][i % 2 * 2 + j] * scale_of(vs[i / 2][step], i % 2 * 2 + j);
 #pragma unroll
                 for (int n = 0; n < 3; ++n) {
                     piece[n][i] = upper(w[1], w[0]);
@@ -512,113 +566,169 @@ struct Step {
                     w[1] -= cut(w[1]);
                 }
             }
+            // columns of other blocks hold what no one reads
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const bf16x8_t x = value_codes(b, e);
-                f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int b = step * kValueBlocks; b < (step + 1) * kValueBlocks && b < NB; ++b)
 #pragma unroll
-                for (int n = 0; n < 3; ++n)
-                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8_t, piece[n]), sum, 0, 0, 0);
-                out[2 * b + e] += sum;
-            }
+                for (int e = 0; e < 2; ++e) {
+                    const bf16x8_t x = value_codes(b, e);
+                    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int n = 0; n < 3; ++n)
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8_t, piece[n]), sum, 0, 0, 0);
+                    out[2 * b + e] += sum;
+                }
         }
     }
     // tile 2 b + e row i is dim 32 b + 2 i + e
-    static __device__ __forceinline__ void put(float* line, uint32_t g, const f32x4 (&out)[kOut]) {
+    static __device__ __forceinline__ void put(float* line, uint32_t c, uint32_t g, const f32x4 (&out)[kOut]) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
+            if (c / HP == b % kValueBlocks)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<f32x2_t*>(line + 32 * b + 8 * g + 2 * r) = f32x2_t{out[2 * b][r], out[2 * b + 1][r]};
+                for (int r = 0; r < 4; ++r)
+                    *reinterpret_cast<f32x2_t*>(line + 32 * b + 8 * g + 2 * r) = f32x2_t{out[2 * b][r], out[2 * b + 1][r]};
     }
     // the order in which key_codes gives a lane's eight dims
     static __device__ constexpr uint32_t query_dim(uint32_t j) { return kBytes ? j : j / 2 + j % 2 * 4; }
 };
 
-template <int FMT, int NB>
+template <int FMT, int NB, int HP>
 __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void paged_attention_kernel(PagedAttnParams a) {
-    using S = Step<FMT, NB>;
+    using S = Step<FMT, NB, HP>;
     constexpr int kTiles = S::kTiles;
-    constexpr uint32_t kKeys = paged_keys(FMT), kUnit = paged_unit(FMT), kDims = 32 * NB, kPitch = kDims + 4;
+    constexpr bool kQuantised = FMT == kKvQ8_0 || FMT == kKvQ4_0;
+    constexpr uint32_t kKeys = paged_keys(FMT), kDims = 32 * NB, kPitch = kDims + 4;
     static_assert(kKeys == 16 * kTiles);
-    // queries in the products' order [part][lane]; at the end the wavefronts' sums
+    // queries in the products' order; at the end the wavefronts' sums
     __shared__ union Room {
-        f32x4 queries[2 * NB][kWave];
-        float sums[kPagedAttnWaves][kPagedHeads][kPitch];
+        uint8_t queries[S::kQueryBytes * (kQuantised ? 2 : 1)];
+        float sums[kPagedAttnWaves][HP][kPitch];
     } room;
-    __shared__ float2 room_ml[kPagedAttnWaves][kPagedHeads];
+    __shared__ float2 room_ml[kPagedAttnWaves][HP];
     __shared__ float room_unscale[kPagedHeads];
-    __shared__ uint64_t room_sum[kPagedAttnWaves];
-    __shared__ struct {
-        uint64_t before;
-        uint32_t seq;
-    } found;
+    __shared__ uint32_t room_units[kPagedAttnWaves];
+    __shared__ uint32_t found_before, found_seq;
     const uint32_t lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
     const uint32_t wave = uniform_u32(threadIdx.x / kWave);
     const uint64_t rows = static_cast<uint64_t>(a.kv_heads) * a.head_tiles;  // of a sequence
 
-    // this workgroup's units of all sequences'
-    uint64_t mine = 0;
-    for (uint32_t b = threadIdx.x; b < a.sequences; b += kPagedAttnThreads) mine += units_of(seen_of(a, b), kUnit);
-    const uint64_t total = uniform_u64(block_sum_u64(mine, room_sum)) * rows;
+    // this workgroup's units of all sequences'; those of a chunk of sequences, one a thread, up to each
+    const auto scan = [&](uint32_t units, uint32_t& chunk) {
+        uint32_t upto = wave_inclusive_scan_u32(units);
+        __syncthreads();
+        if (lane == kWave - 1) room_units[wave] = upto;
+        __syncthreads();
+        chunk = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kPagedAttnWaves; ++w) {
+            if (w == wave) upto += chunk;
+            chunk += room_units[w];
+        }
+        return upto;
+    };
+    uint32_t mine = 0, first_units = 0;
+    for (uint32_t b = threadIdx.x; b < a.sequences; b += kPagedAttnThreads) {
+        const uint32_t units = units_of(seen_of(a, b), kKeys);
+        if (b < kPagedAttnThreads) first_units = units;
+        mine += units;
+    }
+    uint32_t all_units;
+    uint32_t upto = scan(mine, all_units);
+    const uint64_t total = uniform_u32(all_units) * rows;
     const uint64_t parts = parts_of(a, total);
     if (blockIdx.x >= parts) return;
     const uint64_t begin = uniform_u64(total * blockIdx.x / parts), end = uniform_u64(total * (blockIdx.x + 1) / parts);
     // the sequence that `begin` lies in
-    uint64_t before = 0;
+    const uint32_t wanted = static_cast<uint32_t>(begin / rows);
+    uint32_t ahead = 0;
     for (uint32_t first = 0; first < a.sequences; first += kPagedAttnThreads) {
         const uint32_t b = first + threadIdx.x;
-        const uint32_t units = b < a.sequences ? units_of(seen_of(a, b), kUnit) : 0u;
-        uint64_t upto = units;  // of this and the ones before
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const uint64_t x = __shfl_up(upto, d, kWave);
-            if (lane >= static_cast<uint32_t>(d)) upto += x;
+        uint32_t units = first_units, chunk = all_units;
+        if (a.sequences > kPagedAttnThreads) {
+            if (first) units = b < a.sequences ? units_of(seen_of(a, b), kKeys) : 0u;
+            upto = scan(units, chunk);
         }
-        __syncthreads();
-        if (lane == kWave - 1) room_sum[wave] = upto;
-        __syncthreads();
-        uint64_t chunk = 0;
-        for (uint32_t w = 0; w < kPagedAttnWaves; ++w) {
-            if (w == wave) upto += chunk;
-            chunk += room_sum[w];
+        const uint32_t from = ahead + upto - units;
+        if (wanted >= from && wanted - from < units) {
+            found_before = from;
+            found_seq = b;
         }
-        const uint64_t from = before + (upto - units) * rows;
-        if (units && begin >= from && begin < before + upto * rows) {
-            found.before = from;
-            found.seq = b;
-        }
-        before += chunk * rows;
-        if (before > begin) break;
+        ahead += chunk;
+        if (ahead > wanted) break;
     }
     __syncthreads();
-    before = uniform_u64(found.before);
-    uint32_t seq = uniform_u32(found.seq);
+    uint64_t before = uniform_u32(found_before) * rows;
+    uint32_t seq = uniform_u32(found_seq);
 
     for (uint64_t at = begin; at < end;) {
         // a segment: units [t0, t1) of a row's `units`
         SeenRange seen = seen_of(a, seq);
-        uint32_t units = uniform_u32(units_of(seen, kUnit));
+        uint32_t units = uniform_u32(units_of(seen, kKeys));
         while (at >= before + units * rows) {
             before += units * rows;
             ++seq;
             seen = seen_of(a, seq);
-            units = uniform_u32(units_of(seen, kUnit));
+            units = uniform_u32(units_of(seen, kKeys));
         }
         seen.lo = uniform_u32(seen.lo);
         seen.hi = uniform_u32(seen.hi);
         const uint32_t row = uniform_u32(static_cast<uint32_t>((at - before) / units));
         const uint32_t t0 = uniform_u32(static_cast<uint32_t>((at - before) - static_cast<uint64_t>(row) * units));
         const uint32_t t1 = uniform_u32(end - at < units - t0 ? t0 + static_cast<uint32_t>(end - at) : units);
+        if (t0 == 0 && threadIdx.x == 0)  // unit u is part ((u + 1) parts - 1) / total's
+            a.rows[seq * rows + row] = {blockIdx.x, static_cast<uint32_t>(((at + units) * parts - 1) / total)};
         at += t1 - t0;
         const uint32_t kv_head = row / a.head_tiles, head0 = row % a.head_tiles * kPagedHeads;
-        const uint32_t heads = min(a.group - head0, kPagedHeads);
+        const uint32_t heads = min(a.group - head0, static_cast<uint32_t>(HP));
         const uint64_t line0 = static_cast<uint64_t>(seq) * a.q_heads + kv_head * a.group + head0;
+
+        // Unit t's keys start at (seen.lo / kKeys + t) * kKeys; the wavefronts take units in turn.
+        const uint32_t* table = a.table + static_cast<uint64_t>(seq) * a.table_width;
+        const uint32_t start = seen.lo / kKeys * kKeys, tw = t0 + wave;
+        constexpr uint32_t kAhead = kWave / kTiles;  // units whose pages a wavefront's lanes hold
+        uint32_t pages = 0, pages_from = tw;
+        const auto look_up = [&](uint32_t t) {
+            pages_from = t;
+            const uint32_t entry = (start + (t + lane / kTiles * kPagedAttnWaves) * kKeys + lane % kTiles * 16) >> a.page_shift;
+            pages = entry < a.table_width ? table[entry] : 0xffffffffu;
+        };
+        S step;
+        uint32_t page[kTiles];  // of the step that is loaded
+        const auto load = [&](uint32_t t, bool keys) {
+            const uint32_t key = start + t * kKeys, mask = (1u << a.page_shift) - 1;
+            if constexpr (kTiles == 1) {
+                const PageRows p[1] = {PageRows(a, kv_head, page[0], key & mask)};
+                if (keys)
+                    step.load_keys(p, c, g, a.head_dim);
+                else
+                    step.load_values(p, c, g, a.head_dim);
+            } else {
+                const PageRows p[2] = {PageRows(a, kv_head, page[0], key & mask), PageRows(a, kv_head, page[1], (key + 16) & mask)};
+                const uint32_t size = kQuantised ? a.page_shift : a.head_dim;
+                if (keys)
+                    step.load_keys(p, c, g, size);
+                else
+                    step.load_values(p, c, g, size);
+            }
+        };
+        // the pages of unit t; none where nothing is seen, which loads nothing
+        const auto turn = [&](uint32_t t) {
+            if (t < t1 && t - pages_from >= kAhead * kPagedAttnWaves) look_up(t);
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i) {
+                const uint32_t key = start + t * kKeys + 16 * i;
+                const bool some = t < t1 && key < seen.hi && key + 16 > seen.lo;
+                page[i] = some ? readlane_u32(pages, (t - pages_from) / kPagedAttnWaves * kTiles + i) : 0xffffffffu;
+            }
+        };
+        look_up(tw);
 
         __syncthreads();  // the last segment's sums have been read
         {
             const uint32_t head = threadIdx.x / 16, sub = threadIdx.x % 16;
-            const float* q = a.q + (line0 + min(head, heads - 1)) * a.head_dim;
+            const uint32_t real = head % HP;
+            const float* q = a.q + (line0 + min(real, heads - 1)) * a.head_dim;
             constexpr int kEach = FMT == kKvF32 ? 4 : 8, kItems = (kDims / kEach + 15) / 16;
             f32x4 x[kItems][kEach / 4];
             float top = 0.0f;
@@ -627,7 +737,7 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
 #pragma unroll
                 for (int h = 0; h < kEach / 4; ++h) {
                     const uint32_t dim = (sub + 16 * i) * kEach + 4 * h;
-                    const bool there = dim < a.head_dim && head < heads;
+                    const bool there = dim < a.head_dim && real < heads;
                     const f32x4 y = *reinterpret_cast<const f32x4*>(q + (dim < a.head_dim ? dim : 0));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -639,7 +749,7 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
 #pragma unroll
                 for (int i = 0; i < kItems; ++i) {
                     const uint32_t item = sub + 16 * i;
-                    if (item < kDims / 4) room.queries[item / 4][item % 4 * 16 + head] = x[i][0];
+                    if (item < kDims / 4) *reinterpret_cast<f32x4*>(room.queries + item / 4 * 1024 + (item % 4 * 16 + head) * 16) = x[i][0];
                 }
             } else {
                 top = fmaxf(top, dpp_f32<0xb1, 0xf, false>(top));
@@ -651,84 +761,41 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
                 if (top > 0.0f && top < __builtin_inff()) up = min(14 - __builtin_amdgcn_frexp_expf(top), 126);
                 const float by = pow2i(up);
                 if (sub == 0) room_unscale[head] = pow2i(-up);
+                constexpr uint32_t kSlots = kQuantised ? S::kQueryBytes / 16 : 0;
+                if constexpr (kQuantised) {
+                    for (uint32_t i = threadIdx.x; i < kSlots; i += kPagedAttnThreads)
+                        reinterpret_cast<u32x4_t*>(room.queries)[kSlots + i] = u32x4_t{0, 0, 0, 0};
+                }
+                constexpr uint32_t kLines = S::kHeadLines, kLast = S::kItemsPadded;
 #pragma unroll
-                for (int i = 0; i < kItems; ++i) {
+                for (int i = 0; i < static_cast<int>((kLast + 15) / 16); ++i) {
                     const uint32_t item = sub + 16 * i;
                     f16x8_t hi, lo;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        _Float16 p, r;
+                        _Float16 p = static_cast<_Float16>(0.0f), r = p;
                         const uint32_t d = S::query_dim(j);
-                        f16_pieces(x[i][d / 4][d % 4] * by, p, r);
+                        if (i < kItems) f16_pieces(x[i < kItems ? i : 0][d / 4][d % 4] * by, p, r);
                         hi[j] = p;
                         lo[j] = r;
                     }
-                    if (item < kDims / 8) {
-                        room.queries[item / 4 * 2][item % 4 * 16 + head] = __builtin_bit_cast(f32x4, hi);
-                        room.queries[item / 4 * 2 + 1][item % 4 * 16 + head] = __builtin_bit_cast(f32x4, lo);
-                    }
+                    if (item < kLast && head < kLines) S::put_query(room.queries, head, item, hi, lo);
                 }
             }
         }
-
-        // Unit t's keys of this wavefront start at (seen.lo / kUnit + t) * kUnit + wave * kKeys.
-        const uint32_t* table = a.table + static_cast<uint64_t>(seq) * a.table_width;
-        const uint32_t start = (seen.lo / kUnit) * kUnit + wave * kKeys;
-        constexpr uint32_t kAhead = kWave / kTiles;  // units whose pages a wavefront's lanes hold
-        uint32_t pages = 0, pages_from = t0;
-        const auto look_up = [&](uint32_t t) {
-            pages_from = t;
-            const uint32_t entry = (start + (t + lane / kTiles) * kUnit + lane % kTiles * 16) >> a.page_shift;
-            pages = entry < a.table_width ? table[entry] : 0xffffffffu;
-        };
-        const auto page_of = [&](uint32_t t, uint32_t tile) { return readlane_u32(pages, (t - pages_from) * kTiles + tile); };
-        S step;
-        uint32_t page[kTiles];
-        // which of the step's tiles have a page, for the one that is used and the one that is loaded
-        const auto load = [&](uint32_t t, bool keys) {
-            const bool some = t < t1;
-            const uint32_t key = start + (some ? t : t1 - 1) * kUnit;
-            const uint32_t mask = (1u << a.page_shift) - 1;
-            if constexpr (kTiles == 1) {
-                const PageRows p[1] = {PageRows(a, kv_head, some ? page[0] : 0xffffffffu, key & mask)};
-                if (keys)
-                    step.load_keys(p, c, g, a.head_dim);
-                else
-                    step.load_values(p, c, g, a.head_dim);
-            } else {
-                const PageRows p[2] = {PageRows(a, kv_head, some ? page[0] : 0xffffffffu, key & mask),
-                                       PageRows(a, kv_head, some ? page[1] : 0xffffffffu, (key + 16) & mask)};
-                if constexpr (FMT == kKvF16) {
-                    if (keys)
-                        step.load_keys(p, c, g, a.head_dim);
-                    else
-                        step.load_values(p, c, g, a.head_dim);
-                } else {
-                    if (keys)
-                        step.load_keys(p, c, g, a);
-                    else
-                        step.load_values(p, c, g, a);
-                }
-            }
-        };
-        const auto turn = [&](uint32_t t) {
-            if (t < t1 && t - pages_from >= kAhead) look_up(t);
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) page[i] = t < t1 ? page_of(t, i) : 0xffffffffu;
-        };
-        look_up(t0);
-        turn(t0);
-        load(t0, true);
-        load(t0, false);
+        turn(tw);
+        load(tw, true);
+        load(tw, false);
         __syncthreads();
-        const float unscale = FMT == kKvF32 ? 1.0f : room_unscale[c];
+        const float unscale = FMT == kKvF32 ? 1.0f : room_unscale[c % HP];
+        const uint8_t* queries = room.queries + S::query_lane(c, g);
 
         float m = neg_inf(), l = 0.0f;
         f32x4 out[S::kOut];
 #pragma unroll
         for (int i = 0; i < S::kOut; ++i) out[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t t = t0; t < t1; ++t) {
-            const uint32_t key0 = start + t * kUnit;
+        for (uint32_t t = tw; t < t1; t += kPagedAttnWaves) {
+            const uint32_t key0 = start + t * kKeys;
             bool there[kTiles], whole = key0 >= seen.lo && key0 + kKeys <= seen.hi;
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
@@ -736,9 +803,9 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
                 whole = whole && there[i];
             }
             f32x4 s[kTiles];
-            step.scores(room, lane, unscale, s);
-            turn(t + 1);
-            load(t + 1, true);
+            step.scores(queries, c, unscale, s);
+            turn(t + kPagedAttnWaves);
+            load(t + kPagedAttnWaves, true);
             __builtin_amdgcn_sched_barrier(0);
             if (!whole) {
                 bool sees[kTiles][4];
@@ -775,16 +842,16 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
             l += kTiles == 1 ? sum[0] : sum[0] + sum[kTiles - 1];
             step.add(s, out);
             __builtin_amdgcn_sched_barrier(0);
-            load(t + 1, false);
+            load(t + kPagedAttnWaves, false);
         }
 
         // join the wavefronts
         l = sum_xor32(sum_xor16(l));
         __syncthreads();
-        if (g == 0) room_ml[wave][c] = make_float2(m, l);
+        if (g == 0 && c < HP) room_ml[wave][c] = make_float2(m, l);
 #pragma unroll
         for (int i = 0; i < S::kOut; ++i) out[i] *= S::kUnscale;
-        S::put(room.sums[wave][c], g, out);
+        S::put(room.sums[wave][c % HP], c, g, out);
         __syncthreads();
         const bool all = t0 == 0 && t1 == units;
         const uint64_t slot = 2ull * blockIdx.x + (t0 == 0 ? 1 : 0);
@@ -821,10 +888,18 @@ hipError_t launch_paged_attention_f16(hipStream_t stream, const PagedAttnParams&
 hipError_t launch_paged_attention_q8_0(hipStream_t stream, const PagedAttnParams& a);
 hipError_t launch_paged_attention_q4_0(hipStream_t stream, const PagedAttnParams& a);
 
+template <int FMT, int NB, int HP>
+hipError_t launch_paged_heads(hipStream_t stream, const PagedAttnParams& a) {
+    hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP>), dim3(a.most_parts), dim3(kPagedAttnThreads), 0, stream, a);
+    return hipGetLastError();
+}
 template <int FMT, int NB>
 hipError_t launch_paged_blocks(hipStream_t stream, const PagedAttnParams& a) {
-    hipLaunchKernelGGL((paged_attention_kernel<FMT, NB>), dim3(a.most_parts), dim3(kPagedAttnThreads), 0, stream, a);
-    return hipGetLastError();
+    if constexpr (FMT == kKvQ8_0 || FMT == kKvQ4_0) {
+        if (a.group <= 4) return launch_paged_heads<FMT, NB, 4>(stream, a);
+        if (a.group <= 8) return launch_paged_heads<FMT, NB, 8>(stream, a);
+    }
+    return launch_paged_heads<FMT, NB, 16>(stream, a);
 }
 template <int FMT>
 hipError_t launch_paged_format(hipStream_t stream, const PagedAttnParams& a) {

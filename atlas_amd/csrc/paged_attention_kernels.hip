@@ -11,37 +11,25 @@ namespace {
 // part's dims; as many parts as fit the workgroup are taken at once, and their
 // sums meet in LDS in the parts' order.
 template <int LANES>
-__global__ __launch_bounds__(kPagedAttnThreads) void paged_join_kernel(PagedAttnParams a, uint32_t unit) {
+__global__ __launch_bounds__(kPagedAttnThreads) void paged_join_kernel(PagedAttnParams a) {
     constexpr uint32_t kGroups = kPagedAttnThreads / LANES;
-    __shared__ uint64_t room_sum[kPagedAttnWaves];
     __shared__ float wave_top[kPagedAttnWaves];
     __shared__ f32x4 sums[kGroups][LANES];
     __shared__ float group_l[kGroups];
     const uint32_t seq = blockIdx.x / a.q_heads, q_head = blockIdx.x % a.q_heads;
-    const uint64_t rows = static_cast<uint64_t>(a.kv_heads) * a.head_tiles;
-    uint64_t all = 0, ahead = 0;
-    for (uint32_t b = threadIdx.x; b < a.sequences; b += kPagedAttnThreads) {
-        const uint32_t units = units_of(seen_of(a, b), unit);
-        all += units;
-        ahead += b < seq ? units : 0u;
-    }
-    const uint64_t total = block_sum_u64(all, room_sum) * rows;
-    ahead = block_sum_u64(ahead, room_sum) * rows;
-    const uint32_t units = units_of(seen_of(a, seq), unit);
+    const uint32_t kv_head = q_head / a.group, in_group = q_head % a.group;
+    const PagedRow row = a.rows[(static_cast<uint64_t>(seq) * a.kv_heads + kv_head) * a.head_tiles + in_group / kPagedHeads];
+    const SeenRange seen = seen_of(a, seq);
     const uint32_t group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const uint32_t dim = 4 * (blockIdx.y * LANES + lane);
     float* out = a.output + static_cast<uint64_t>(blockIdx.x) * a.head_dim + dim;
-    if (units == 0) {
+    if (seen.hi == seen.lo) {  // no part has the row
         if (group == 0 && dim < a.head_dim) *reinterpret_cast<f32x4*>(out) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         return;
     }
-    const uint64_t parts = parts_of(a, total);
-    const uint32_t kv_head = q_head / a.group, in_group = q_head % a.group;
-    const uint64_t first_unit = ahead + static_cast<uint64_t>(kv_head * a.head_tiles + in_group / kPagedHeads) * units;
-    // unit u is part ((u + 1) parts - 1) / total's
-    const uint64_t first = ((first_unit + 1) * parts - 1) / total, last = ((first_unit + units) * parts - 1) / total;
-    if (first == last) return;
-    const uint32_t count = static_cast<uint32_t>(last - first + 1), head = in_group % kPagedHeads;
+    if (row.first == row.last) return;
+    const uint64_t first = row.first;
+    const uint32_t count = row.last - row.first + 1, head = in_group % kPagedHeads;
     // a row begins in the second slot of its first part and goes on in the others' first
     const auto line_of = [&](uint32_t i) { return (2 * (first + i) + (i == 0 ? 1 : 0)) * a.heads + head; };
     float top = neg_inf();
@@ -82,34 +70,35 @@ __global__ __launch_bounds__(kPagedAttnThreads) void paged_join_kernel(PagedAttn
     *reinterpret_cast<f32x4*>(out) = y;
 }
 
-// Additions to a wavefront's sums in a part: with keys alike they all round to
+// Additions to a wavefront's sums in a part, a unit each: with keys alike they all round to
 // one side, 2^-25 of the sum at most each.
-constexpr uint32_t kMostAdditions = 256;
+constexpr uint32_t kPartUnits = 256 * kPagedAttnWaves;
 constexpr uint32_t kMostParts = 1u << 20;
 
 uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
 
 struct PagedPlan {
     uint32_t few_parts, most_parts, heads;
-    uint64_t out_bytes, ml_bytes;
+    uint64_t out_bytes, ml_bytes, row_bytes;
 };
 
 PagedPlan paged_plan(const PagedCache& c, uint32_t q_heads) {
     PagedPlan p{};
     const uint32_t group = q_heads / c.kv_heads;
     p.heads = group < kPagedHeads ? group : kPagedHeads;
-    const uint32_t unit = paged_unit(c.format);
+    const uint32_t unit = paged_keys(c.format);
     const uint64_t capacity = static_cast<uint64_t>(c.table_width) * c.page_size;
-    // a window may begin and end inside units: one more than its length has
-    const uint64_t units = (capacity + unit - 1) / unit * c.sequences * c.kv_heads * ((group + kPagedHeads - 1) / kPagedHeads);
+    const uint64_t rows = static_cast<uint64_t>(c.sequences) * c.kv_heads * ((group + kPagedHeads - 1) / kPagedHeads);
+    const uint64_t units = (capacity + unit - 1) / unit * rows;
     p.few_parts = 256 * paged_occupancy(c.head_dim);
-    const uint64_t long_parts = (units + kMostAdditions - 1) / kMostAdditions;
+    const uint64_t long_parts = (units + kPartUnits - 1) / kPartUnits;
     uint64_t most = long_parts > p.few_parts ? long_parts : p.few_parts;
     most = most < units ? most : units;
     p.most_parts = static_cast<uint32_t>(most < kMostParts ? most : kMostParts);
     const uint64_t lines = 2ull * p.most_parts * p.heads;
     p.out_bytes = round256(lines * c.head_dim * 4);
     p.ml_bytes = round256(lines * 8);
+    p.row_bytes = round256(rows * sizeof(PagedRow));
     return p;
 }
 
@@ -117,7 +106,7 @@ PagedPlan paged_plan(const PagedCache& c, uint32_t q_heads) {
 
 uint64_t paged_attention_workspace(const PagedCache& c, uint32_t q_heads) {
     const PagedPlan p = paged_plan(c, q_heads);
-    return p.out_bytes + p.ml_bytes;
+    return p.out_bytes + p.ml_bytes + p.row_bytes;
 }
 
 hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& s) {
@@ -131,6 +120,7 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
     a.output = s.output;
     a.partial_out = static_cast<float*>(s.workspace);
     a.partial_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(s.workspace) + p.out_bytes);
+    a.rows = reinterpret_cast<PagedRow*>(static_cast<uint8_t*>(s.workspace) + p.out_bytes + p.ml_bytes);
     a.page_bytes = paged_page_bytes(c);
     a.part_bytes = paged_part_bytes(c.format, c.page_size, c.head_dim);
     a.page_count = c.page_count;
@@ -147,7 +137,7 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
     a.window = s.window;
     a.few_parts = p.few_parts;
     a.most_parts = p.most_parts;
-    a.part_units = kMostAdditions;
+    a.part_units = kPartUnits;
     a.scale = s.scale * kLog2e;
     hipError_t e;
     switch (c.format) {
@@ -157,15 +147,15 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
         default: e = launch_paged_attention_q4_0(stream, a); break;
     }
     if (e != hipSuccess) return e;
-    const uint32_t lines = c.sequences * s.q_heads, unit = paged_unit(c.format);
+    const uint32_t lines = c.sequences * s.q_heads;
     const uint32_t pieces = lines < 512 ? (c.head_dim + 63) / 64 : 1;
     const dim3 grid(lines, pieces), block(kPagedAttnThreads);
     if (c.head_dim <= 64 * pieces)
-        hipLaunchKernelGGL(paged_join_kernel<16>, grid, block, 0, stream, a, unit);
+        hipLaunchKernelGGL(paged_join_kernel<16>, grid, block, 0, stream, a);
     else if (c.head_dim <= 128)
-        hipLaunchKernelGGL(paged_join_kernel<32>, grid, block, 0, stream, a, unit);
+        hipLaunchKernelGGL(paged_join_kernel<32>, grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL(paged_join_kernel<64>, grid, block, 0, stream, a, unit);
+        hipLaunchKernelGGL(paged_join_kernel<64>, grid, block, 0, stream, a);
     return hipGetLastError();
 }
 
