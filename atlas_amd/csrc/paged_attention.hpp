@@ -453,22 +453,36 @@ struct Step {
 #pragma unroll
         for (int h = 0; h < 2; ++h) load_scales(p[h].values, page_shift, p[h].row, g, c / HP, kValueBlocks, vs[h]);
     }
-    // Eight codes of a key as f16: 1024 + (a code without its sign) has it in its low bits.
+    // Eight codes of a key as f16: 1024 + (a code without its sign) has it in its low
+    // bits, or 16 times it four bits higher up.  Written out where the compiler makes
+    // two instructions of one.
+    static __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+        uint32_t y;
+        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(y) : "v"(x), "s"(mask), "v"(bits));
+        return y;
+    }
     static __device__ __forceinline__ f16x8_t key_codes(u32x4_t w, int m) {
         u32x4_t x;
-        _Float16 less;
+        const auto less = [](uint32_t y, float by) {
+            const f16x2_t z = {static_cast<_Float16>(by), static_cast<_Float16>(by)};
+            return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, y) - z);
+        };
         if constexpr (kBytes) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                x[i] = __builtin_amdgcn_perm(0x64646464u, w[2 * m + i / 2] ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u);
-            less = static_cast<_Float16>(-1152.0f);
+                x[i] = less(__builtin_amdgcn_perm(0x64646464u, w[2 * m + i / 2] ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u), 1152.0f);
         } else {
+            const f16x2_t sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+            const f16x2_t minus72 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = (w[m] >> (4 * i) & 0x000f000fu) | 0x64006400u;
-            less = static_cast<_Float16>(-1032.0f);
+            for (int i = 0; i < 4; i += 2) {
+                const uint32_t y = i ? w[m] >> 8 : w[m];
+                x[i] = less(and_or(y, 0x000f000fu, 0x64006400u), 1032.0f);
+                // (1024 + 16 n) / 16 - 72 = n - 8
+                x[i + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, and_or(y, 0x00f000f0u, 0x64006400u)),
+                                                                                  sixteenth, minus72));
+            }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, static_cast<uint32_t>(x[i])) + f16x2_t{less, less});
         return __builtin_bit_cast(f16x8_t, x);
     }
     static __device__ __forceinline__ float scale_of(u32x2_t s, int r) { return h2f(static_cast<uint16_t>(s[r / 2] >> (16 * (r % 2)))); }
@@ -532,6 +546,19 @@ struct Step {
         return __builtin_amdgcn_perm(__float_as_uint(odd), __float_as_uint(even), 0x07060302u);
     }
     static __device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+    // The low four bits of byte i, in one instruction.
+    static __device__ __forceinline__ float nibble(uint32_t w, int i) {
+        float x;
+        if (i == 0)
+            asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(x) : "v"(w));
+        else if (i == 1)
+            asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(x) : "v"(w));
+        else if (i == 2)
+            asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(x) : "v"(w));
+        else
+            asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(x) : "v"(w));
+        return x;
+    }
     // code e of block b of eight keys
     __device__ __forceinline__ bf16x8_t value_codes(int b, int e) const {
         float x[8];
@@ -542,7 +569,7 @@ struct Step {
             if constexpr (kBytes)
                 x[j] = static_cast<float>(static_cast<int8_t>(w >> (8 * (at % 4))));
             else  // two's complement by the flip of bit 3
-                x[j] = __builtin_amdgcn_cvt_off_f32_i4(((e ? w >> 4 : w) ^ 0x08080808u) >> (8 * (at % 4)) & 255u);
+                x[j] = nibble(e ? (w ^ 0x88888888u) >> 4 : w ^ 0x88888888u, at % 4);
         }
         u32x4_t y;
 #pragma unroll
@@ -692,6 +719,8 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
             pages_from = t;
             const uint32_t entry = (start + (t + lane / kTiles * kPagedAttnWaves) * kKeys + lane % kTiles * 16) >> a.page_shift;
             pages = entry < a.table_width ? table[entry] : 0xffffffffu;
+            // waited for here, and not by whoever reads it: that wait would be for every load of every step
+            asm volatile("" : "+v"(pages));
         };
         S step;
         uint32_t page[kTiles];  // of the step that is loaded
@@ -722,26 +751,35 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
                 page[i] = some ? readlane_u32(pages, (t - pages_from) / kPagedAttnWaves * kTiles + i) : 0xffffffffu;
             }
         };
-        look_up(tw);
-
-        __syncthreads();  // the last segment's sums have been read
+        // the query's loads, the step's behind them, and then what is done with the query
+        const uint32_t head = threadIdx.x / 16, sub = threadIdx.x % 16, real = head % HP;
+        constexpr int kEach = FMT == kKvF32 ? 4 : 8, kItems = (kDims / kEach + 15) / 16;
+        f32x4 x[kItems][kEach / 4];
         {
-            const uint32_t head = threadIdx.x / 16, sub = threadIdx.x % 16;
-            const uint32_t real = head % HP;
             const float* q = a.q + (line0 + min(real, heads - 1)) * a.head_dim;
-            constexpr int kEach = FMT == kKvF32 ? 4 : 8, kItems = (kDims / kEach + 15) / 16;
-            f32x4 x[kItems][kEach / 4];
-            float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < kItems; ++i)
 #pragma unroll
                 for (int h = 0; h < kEach / 4; ++h) {
                     const uint32_t dim = (sub + 16 * i) * kEach + 4 * h;
-                    const bool there = dim < a.head_dim && real < heads;
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(q + (dim < a.head_dim ? dim : 0));
+                    x[i][h] = *reinterpret_cast<const f32x4*>(q + (dim < a.head_dim ? dim : 0));
+                }
+        }
+        look_up(tw);
+        turn(tw);
+        load(tw, true);
+        load(tw, false);
+        __syncthreads();  // the last segment's sums have been read
+        {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kItems; ++i)
+#pragma unroll
+                for (int h = 0; h < kEach / 4; ++h) {
+                    const bool there = (sub + 16 * i) * kEach + 4 * h < a.head_dim && real < heads;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        x[i][h][j] = there ? y[j] * a.scale : 0.0f;
+                        x[i][h][j] = there ? x[i][h][j] * a.scale : 0.0f;
                         top = fmaxf(top, __builtin_fabsf(x[i][h][j]));
                     }
                 }
@@ -783,9 +821,6 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
                 }
             }
         }
-        turn(tw);
-        load(tw, true);
-        load(tw, false);
         __syncthreads();
         const float unscale = FMT == kKvF32 ? 1.0f : room_unscale[c % HP];
         const uint8_t* queries = room.queries + S::query_lane(c, g);

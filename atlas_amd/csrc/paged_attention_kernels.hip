@@ -9,11 +9,12 @@ namespace {
 // One workgroup a query row, or 4 LANES dims of one: its parts joined, where
 // there is more than one, or zero where nothing was seen.  LANES lanes hold a
 // part's dims; as many parts as fit the workgroup are taken at once, and their
-// sums meet in LDS in the parts' order.
-template <int LANES>
-__global__ __launch_bounds__(kPagedAttnThreads) void paged_join_kernel(PagedAttnParams a) {
-    constexpr uint32_t kGroups = kPagedAttnThreads / LANES;
-    __shared__ float wave_top[kPagedAttnWaves];
+// sums meet in LDS in the parts' order.  The loads' latency is its time: a
+// group's first parts are on their way before the row's maximum is known.
+template <int LANES, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnParams a) {
+    constexpr uint32_t kGroups = THREADS / LANES, kWaves = THREADS / kWave, kAtOnce = 4;
+    __shared__ float wave_top[kWaves];
     __shared__ f32x4 sums[kGroups][LANES];
     __shared__ float group_l[kGroups];
     const uint32_t seq = blockIdx.x / a.q_heads, q_head = blockIdx.x % a.q_heads;
@@ -22,35 +23,47 @@ __global__ __launch_bounds__(kPagedAttnThreads) void paged_join_kernel(PagedAttn
     const SeenRange seen = seen_of(a, seq);
     const uint32_t group = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const uint32_t dim = 4 * (blockIdx.y * LANES + lane);
+    const bool holds = dim < a.head_dim;
     float* out = a.output + static_cast<uint64_t>(blockIdx.x) * a.head_dim + dim;
     if (seen.hi == seen.lo) {  // no part has the row
-        if (group == 0 && dim < a.head_dim) *reinterpret_cast<f32x4*>(out) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (group == 0 && holds) *reinterpret_cast<f32x4*>(out) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         return;
     }
     if (row.first == row.last) return;
-    const uint64_t first = row.first;
     const uint32_t count = row.last - row.first + 1, head = in_group % kPagedHeads;
     // a row begins in the second slot of its first part and goes on in the others' first
-    const auto line_of = [&](uint32_t i) { return (2 * (first + i) + (i == 0 ? 1 : 0)) * a.heads + head; };
+    const auto line_of = [&](uint32_t i) { return (2ull * (row.first + i) + (i == 0 ? 1 : 0)) * a.heads + head; };
+    float2 ml[kAtOnce];
+    f32x4 part[kAtOnce];
+    const auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t j = 0; j < kAtOnce; ++j) {
+            const uint64_t line = line_of(min(i0 + j * kGroups, count - 1));
+            ml[j] = a.partial_ml[line];
+            part[j] = *reinterpret_cast<const f32x4*>(a.partial_out + line * a.head_dim + (holds ? dim : 0));
+        }
+    };
+    load(group);
     float top = neg_inf();
-    for (uint32_t i = threadIdx.x; i < count; i += kPagedAttnThreads) top = fmaxf(top, a.partial_ml[line_of(i)].x);
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS) top = fmaxf(top, a.partial_ml[line_of(i)].x);
     top = wave_max_tree_f32(top);
     if (threadIdx.x % kWave == 0) wave_top[threadIdx.x / kWave] = top;
     __syncthreads();
-    top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
+    top = wave_top[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kWaves; ++w) top = fmaxf(top, wave_top[w]);
     const float base = top == neg_inf() ? 0.0f : top;
-    const bool holds = dim < a.head_dim;
     // in 64 bits: a row has up to 2^20 parts
     double all_l = 0.0, all_o[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll 4
-    for (uint32_t i = group; i < count; i += kGroups) {
-        const uint64_t line = line_of(i);
-        const float2 x = a.partial_ml[line];
-        const f32x4 part = *reinterpret_cast<const f32x4*>(a.partial_out + line * a.head_dim + (holds ? dim : 0));
-        const float f = __builtin_amdgcn_exp2f(x.x - base);
-        all_l += static_cast<double>(f * x.y);
+    for (uint32_t i0 = group; i0 < count; i0 += kAtOnce * kGroups) {
+        if (i0 != group) load(i0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) all_o[j] += static_cast<double>(f * part[j]);
+        for (uint32_t j = 0; j < kAtOnce; ++j) {
+            const float f = i0 + j * kGroups < count ? __builtin_amdgcn_exp2f(ml[j].x - base) : 0.0f;
+            all_l += static_cast<double>(f * ml[j].y);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) all_o[k] += static_cast<double>(f * part[j][k]);
+        }
     }
     sums[group][lane] = f32x4{static_cast<float>(all_o[0]), static_cast<float>(all_o[1]), static_cast<float>(all_o[2]),
                               static_cast<float>(all_o[3])};
@@ -59,8 +72,7 @@ __global__ __launch_bounds__(kPagedAttnThreads) void paged_join_kernel(PagedAttn
     if (group || !holds) return;
     float sum = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (uint32_t i = 0; i < kGroups; ++i) {
+    for (uint32_t i = 0; i < min(kGroups, count); ++i) {
         sum += group_l[i];
         o += sums[i][lane];
     }
@@ -148,14 +160,18 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
     }
     if (e != hipSuccess) return e;
     const uint32_t lines = c.sequences * s.q_heads;
-    const uint32_t pieces = lines < 512 ? (c.head_dim + 63) / 64 : 1;
-    const dim3 grid(lines, pieces), block(kPagedAttnThreads);
-    if (c.head_dim <= 64 * pieces)
-        hipLaunchKernelGGL(paged_join_kernel<16>, grid, block, 0, stream, a);
+    // Few rows have many parts: a workgroup for every 64 dims of one, and of 16 wavefronts.
+    if (lines < 512) {
+        hipLaunchKernelGGL((paged_join_kernel<16, 1024>), dim3(lines, (c.head_dim + 63) / 64), dim3(1024), 0, stream, a);
+        return hipGetLastError();
+    }
+    const dim3 grid(lines), block(kPagedAttnThreads);
+    if (c.head_dim <= 64)
+        hipLaunchKernelGGL((paged_join_kernel<16, kPagedAttnThreads>), grid, block, 0, stream, a);
     else if (c.head_dim <= 128)
-        hipLaunchKernelGGL(paged_join_kernel<32>, grid, block, 0, stream, a);
+        hipLaunchKernelGGL((paged_join_kernel<32, kPagedAttnThreads>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL(paged_join_kernel<64>, grid, block, 0, stream, a);
+        hipLaunchKernelGGL((paged_join_kernel<64, kPagedAttnThreads>), grid, block, 0, stream, a);
     return hipGetLastError();
 }
 
