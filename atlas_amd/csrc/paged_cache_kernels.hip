@@ -12,10 +12,11 @@
 // are rounded one by one, as everywhere here.
 //
 // A row (a head's query, key or value) is LANES lanes of four dims, so a block of
-// 32 is eight lanes and a wavefront holds 64 / LANES rows.  A rotating lane loads
-// its partners' dims too: the line is there, and nothing is exchanged.  Bound by
-// bytes, and below a few hundred tokens by the chain of its loads (position,
-// table, store).
+// 32 is eight lanes, and a wavefront holds 64 / LANES rows at once, all of one
+// token: where the token goes is known to the wavefront by scalar loads, and a
+// lane's angles serve all of its rows.  A rotating lane loads its partners' dims
+// too: the line is there, and nothing is exchanged.  Bound by bytes, and below a few
+// hundred tokens by the chain of its loads (position, table, store).
 #include "device_common.hpp"
 #include "paged_layout.hpp"
 
@@ -24,19 +25,44 @@ namespace {
 
 constexpr uint32_t kPagedThreads = 256;
 constexpr uint32_t kPagedWaves = kPagedThreads / kWave;
-constexpr uint32_t kNoPlace = 0xffffffffu;
 
 typedef f32x4 f32x4_row __attribute__((aligned(4)));
 
+// Where a token's rows are: known to the whole wavefront.
 struct Place {
-    uint32_t page, row;  // page kNoPlace: the position has none
+    uint32_t page, row;
+    bool in_range, there;  // the position is one of the table's; it has a page
 };
 
 __device__ __forceinline__ Place place_of(const PagedCache& c, uint32_t shift, uint32_t sequence, uint32_t position) {
     const uint32_t entry = position >> shift;
-    if (sequence >= c.sequences || entry >= c.table_width) return {kNoPlace, 0};
-    const uint32_t page = c.table[static_cast<uint64_t>(sequence) * c.table_width + entry];
-    return {page < c.page_count ? page : kNoPlace, position & (c.page_size - 1)};
+    Place p{0, position & (c.page_size - 1), sequence < c.sequences && entry < c.table_width, false};
+    if (p.in_range) {
+        p.page = c.table[static_cast<uint64_t>(sequence) * c.table_width + entry];
+        p.there = p.page < c.page_count;
+    }
+    return p;
+}
+
+// A wavefront's token and its share of the token's rows, 2^chunks shares.
+struct Share {
+    uint32_t token, first;
+};
+__device__ __forceinline__ Share share_of(uint32_t chunks, uint32_t steps) {
+    const uint32_t wave = blockIdx.x * kPagedWaves + static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+    return {wave >> chunks, (wave & ((1u << chunks) - 1)) * steps};
+}
+constexpr int kAtOnce = 4;  // rows of a lane on their way
+
+// The codes of a row, four to a lane, from the order of the dims to a value's or
+// back: through LDS, so that memory sees whole rows (two loads of two codes a lane
+// keep the address unit busy for as long as the rows of 32768 positions take, 83 us).
+// A wavefront's room has a word for every lane of every step.
+typedef uint32_t CodeRoom[kAtOnce][kWave];
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 __device__ __forceinline__ uint8_t* part_of_page(const PagedCache& c, uint32_t page, uint32_t plane, uint32_t head, uint32_t part_bytes) {
@@ -88,67 +114,12 @@ __device__ __forceinline__ void encode(const float (&v)[4], uint32_t (&code)[4],
     }
 }
 
-template <int FMT, int LANES>
-__global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppendArgs a, uint32_t shift) {
-    constexpr uint32_t kRows = kWave / LANES;  // of a wavefront
-    const PagedCache& c = a.cache;
-    const uint32_t hd = c.head_dim, heads = a.query ? a.q_heads : 0, each = heads + 2 * c.kv_heads;
-    const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * kPagedWaves + threadIdx.x / kWave) * kRows + threadIdx.x % kWave / LANES;
-    const uint32_t token = static_cast<uint32_t>(row / each);
-    const uint32_t head = static_cast<uint32_t>(row % each);  // queries, keys, values
-    if (token >= a.tokens) return;
-    const uint32_t dim = threadIdx.x % LANES * 4;
-    const bool holds = dim < hd;
-    const uint32_t sequence = a.sequences ? a.sequences[token] : token, position = a.positions[token];
-    if (sequence >= c.sequences || position >> shift >= c.table_width) return;
-    const bool is_query = head < heads, is_key = !is_query && head < heads + c.kv_heads;
-    const uint32_t kv_head = is_query ? 0 : (head - heads) % c.kv_heads;
-    const float* in = is_query ? a.query + (static_cast<uint64_t>(token) * heads + head) * hd
-                               : (is_key ? a.key : a.value) + (static_cast<uint64_t>(token) * c.kv_heads + kv_head) * hd;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (holds) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(in + dim);
-        if ((is_query || is_key) && a.cosine) {
-            const uint32_t half = hd / 2;
-            const float* cosine = a.cosine + static_cast<uint64_t>(position) * a.rope_stride;
-            const float* sine = a.sine + static_cast<uint64_t>(position) * a.rope_stride;
-            f32x4 y, cs, sn;  // the partners; the lane's angles
-            if (half % 4 == 0) {
-                const uint32_t at = dim < half ? dim : dim - half;
-                y = *reinterpret_cast<const f32x4*>(in + (dim < half ? dim + half : at));
-                cs = *reinterpret_cast<const f32x4_row*>(cosine + at);
-                sn = *reinterpret_cast<const f32x4_row*>(sine + at);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t d = dim + j, at = d < half ? d : d - half;
-                    y[j] = in[d < half ? d + half : at];
-                    cs[j] = cosine[at];
-                    sn[j] = sine[at];
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float turned = y[j] * sn[j], kept = x[j] * cs[j];
-                v[j] = dim + j < half ? kept - turned : turned + kept;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = x[j];
-        }
-    }
-    if (is_query) {
-        // query_out may be query: the row has been read by its wavefront, whose stores follow
-        if (holds)
-            *reinterpret_cast<f32x4*>(a.query_out + (static_cast<uint64_t>(token) * heads + head) * hd + dim) =
-                f32x4{v[0], v[1], v[2], v[3]};
-        return;
-    }
-    const Place at = place_of(c, shift, sequence, position);
-    if (at.page == kNoPlace) return;
-    uint8_t* part = part_of_page(c, at.page, is_key ? 0 : 1, kv_head, paged_part_bytes(FMT, c.page_size, hd));
-    const uint32_t row_bytes = paged_row_code_bytes(FMT, hd);
-    uint8_t* to = part + at.row * row_bytes;
+// One head's row of four dims a lane, stored: `to` is the page's part.
+template <int FMT>
+__device__ __forceinline__ void store_row(uint8_t* part, const PagedCache& c, uint32_t row, uint32_t dim, bool is_key, bool holds,
+                                          uint32_t p0, uint32_t p1, uint8_t* room, const float (&v)[4]) {
+    const uint32_t hd = c.head_dim, row_bytes = paged_row_code_bytes(FMT, hd);
+    uint8_t* to = part + row * row_bytes;
     if constexpr (FMT == kKvF32) {
         if (holds) *reinterpret_cast<f32x4*>(to + 4 * dim) = f32x4{v[0], v[1], v[2], v[3]};
     } else if constexpr (FMT == kKvF16) {
@@ -160,97 +131,214 @@ __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppend
         float scale;
         encode<FMT>(v, code, scale);
         if (!holds) return;  // head_dim is a multiple of 32: whole blocks
-        if (is_key) {
-            if constexpr (FMT == kKvQ8_0)
-                *reinterpret_cast<uint32_t*>(to + dim) = code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24;
-            else
-                *reinterpret_cast<uint16_t*>(to + dim / 2) =
-                    static_cast<uint16_t>(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
+        const uint32_t q0 = is_key ? dim : p0, q1 = is_key ? dim + 2 : p1;
+        if constexpr (FMT == kKvQ8_0) {
+            *reinterpret_cast<uint16_t*>(room + q0) = static_cast<uint16_t>(code[0] | code[1] << 8);
+            *reinterpret_cast<uint16_t*>(room + q1) = static_cast<uint16_t>(code[2] | code[3] << 8);
+            wave_lds_fence();
+            *reinterpret_cast<uint32_t*>(to + dim) = *reinterpret_cast<const uint32_t*>(room + dim);
         } else {
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-                const uint32_t place = paged_value_place(hd, dim + j);
-                if constexpr (FMT == kKvQ8_0)
-                    *reinterpret_cast<uint16_t*>(to + place) = static_cast<uint16_t>(code[j] | code[j + 1] << 8);
-                else
-                    to[place / 2] = static_cast<uint8_t>(code[j] | code[j + 1] << 4);
-            }
+            room[q0 / 2] = static_cast<uint8_t>(code[0] | code[1] << 4);
+            room[q1 / 2] = static_cast<uint8_t>(code[2] | code[3] << 4);
+            wave_lds_fence();
+            *reinterpret_cast<uint16_t*>(to + dim / 2) = *reinterpret_cast<const uint16_t*>(room + dim / 2);
         }
         if (threadIdx.x % 8 == 0)
-            *reinterpret_cast<uint16_t*>(part + c.page_size * row_bytes +
-                                         2 * ((at.row / 4 * (hd / 32) + dim / 32) * 4 + at.row % 4)) = f2h(scale);
+            *reinterpret_cast<uint16_t*>(part + c.page_size * row_bytes + 2 * ((row / 4 * (hd / 32) + dim / 32) * 4 + row % 4)) =
+                f2h(scale);
+    }
+}
+
+template <int FMT, int LANES>
+__global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppendArgs a, uint32_t shift, uint32_t chunks, uint32_t steps) {
+    constexpr uint32_t kRows = kWave / LANES;  // of a wavefront at once
+    const PagedCache& c = a.cache;
+    const uint32_t hd = c.head_dim, half = hd / 2, heads = a.query ? a.q_heads : 0, each = heads + 2 * c.kv_heads;
+    const Share share = share_of(chunks, steps);
+    if (share.token >= a.tokens) return;
+    const uint32_t sequence = a.sequences ? a.sequences[share.token] : share.token, position = a.positions[share.token];
+    const Place at = place_of(c, shift, sequence, position);
+    if (!at.in_range) return;
+    const uint32_t dim = threadIdx.x % LANES * 4;
+    const bool holds = dim < hd, turns = a.cosine != nullptr, whole = half % 4 == 0;
+    const uint32_t at_dim = holds ? dim : 0, partner = at_dim < half ? at_dim + half : at_dim - half;
+    f32x4 cs = {1.0f, 1.0f, 1.0f, 1.0f}, sn = {0.0f, 0.0f, 0.0f, 0.0f};  // the lane's angles
+    if (turns) {
+        const float* cosine = a.cosine + static_cast<uint64_t>(position) * a.rope_stride;
+        const float* sine = a.sine + static_cast<uint64_t>(position) * a.rope_stride;
+        if (whole) {
+            cs = *reinterpret_cast<const f32x4_row*>(cosine + (at_dim < half ? at_dim : partner));
+            sn = *reinterpret_cast<const f32x4_row*>(sine + (at_dim < half ? at_dim : partner));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t d = at_dim + j, i = d < half ? d : d - half;
+                cs[j] = cosine[i];
+                sn[j] = sine[i];
+            }
+        }
+    }
+    const uint32_t part_bytes = paged_part_bytes(FMT, c.page_size, hd);
+    __shared__ CodeRoom rooms[paged_quantised(FMT) ? kPagedWaves : 1];
+    const uint32_t p0 = paged_quantised(FMT) ? paged_value_place(hd, at_dim) : 0, p1 = paged_quantised(FMT) ? paged_value_place(hd, at_dim + 2) : 0;
+    for (uint32_t s0 = 0; s0 < steps; s0 += kAtOnce) {
+        f32x4 x[kAtOnce], y[kAtOnce];  // the lane's dims and their partners
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s) {
+            if (s0 + s >= steps) break;
+            const uint32_t row = min((share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES, each - 1);
+            const float* in = row < heads ? a.query + (static_cast<uint64_t>(share.token) * heads + row) * hd
+                                          : (row < heads + c.kv_heads ? a.key : a.value) +
+                                                (static_cast<uint64_t>(share.token) * c.kv_heads + (row - heads) % c.kv_heads) * hd;
+            x[s] = *reinterpret_cast<const f32x4*>(in + at_dim);
+            if (!turns) {
+                y[s] = x[s];
+            } else if (whole) {
+                y[s] = *reinterpret_cast<const f32x4*>(in + partner);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[s][j] = in[at_dim + j < half ? at_dim + j + half : at_dim + j - half];
+            }
+        }
+        // query_out may be query: a row has been read by its wavefront, and is no other's
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s) {
+            const uint32_t row = (share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES;
+            if (s0 + s >= steps) break;
+            if (row >= each) continue;
+            const bool is_query = row < heads, is_key = !is_query && row < heads + c.kv_heads;
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float turned = y[s][j] * sn[j], kept = x[s][j] * cs[j];
+                v[j] = !turns || !(is_query || is_key) ? x[s][j] : (dim + j < half ? kept - turned : turned + kept);
+                if (!holds) v[j] = 0.0f;
+            }
+            if (is_query) {
+                if (holds)
+                    *reinterpret_cast<f32x4*>(a.query_out + (static_cast<uint64_t>(share.token) * heads + row) * hd + dim) =
+                        f32x4{v[0], v[1], v[2], v[3]};
+            } else if (at.there) {
+                store_row<FMT>(part_of_page(c, at.page, is_key ? 0 : 1, (row - heads) % c.kv_heads, part_bytes), c, at.row, dim, is_key,
+                               holds, p0, p1, reinterpret_cast<uint8_t*>(rooms[paged_quantised(FMT) ? threadIdx.x / kWave : 0][s]) +
+                                                  threadIdx.x % kWave / LANES * LANES * 4, v);
+            }
+        }
     }
 }
 
 // Bound by what it writes, 4 bytes a value.
 template <int FMT, int LANES>
-__global__ __launch_bounds__(kPagedThreads) void paged_read_kernel(PagedReadArgs a, uint32_t shift) {
+__global__ __launch_bounds__(kPagedThreads) void paged_read_kernel(PagedReadArgs a, uint32_t shift, uint32_t chunks, uint32_t steps) {
     constexpr uint32_t kRows = kWave / LANES;
     const PagedCache& c = a.cache;
     const uint32_t hd = c.head_dim, each = 2 * c.kv_heads;
-    const uint64_t row = (static_cast<uint64_t>(blockIdx.x) * kPagedWaves + threadIdx.x / kWave) * kRows + threadIdx.x % kWave / LANES;
-    const uint32_t token = static_cast<uint32_t>(row / each);
-    const uint32_t head = static_cast<uint32_t>(row % each);  // keys, values
+    const Share share = share_of(chunks, steps);
+    if (share.token >= a.rows) return;
+    const Place at = place_of(c, shift, a.sequences ? a.sequences[share.token] : share.token, a.positions[share.token]);
     const uint32_t dim = threadIdx.x % LANES * 4;
-    if (token >= a.rows || dim >= hd) return;
-    const uint32_t plane = head / c.kv_heads, kv_head = head % c.kv_heads;
-    float* out = plane ? a.value : a.key;
-    if (!out) return;
-    const Place at = place_of(c, shift, a.sequences ? a.sequences[token] : token, a.positions[token]);
-    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (at.page != kNoPlace) {
-        const uint8_t* part = part_of_page(c, at.page, plane, kv_head, paged_part_bytes(FMT, c.page_size, hd));
-        const uint32_t row_bytes = paged_row_code_bytes(FMT, hd);
-        const uint8_t* from = part + at.row * row_bytes;
-        if constexpr (FMT == kKvF32) {
-            v = *reinterpret_cast<const f32x4*>(from + 4 * dim);
-        } else if constexpr (FMT == kKvF16) {
-            const u32x2_t w = *reinterpret_cast<const u32x2_t*>(from + 2 * dim);
+    if (dim >= hd) return;
+    const uint32_t part_bytes = paged_part_bytes(FMT, c.page_size, hd), row_bytes = paged_row_code_bytes(FMT, hd);
+    const uint32_t p0 = paged_quantised(FMT) ? paged_value_place(hd, dim) : 0, p1 = paged_quantised(FMT) ? paged_value_place(hd, dim + 2) : 0;
+    __shared__ CodeRoom rooms[paged_quantised(FMT) ? kPagedWaves : 1];
+    const uint32_t scale_at = c.page_size * row_bytes + 2 * ((at.row / 4 * (hd / 32) + dim / 32) * 4 + at.row % 4);
+    for (uint32_t s0 = 0; s0 < steps; s0 += kAtOnce) {
+        u32x4_t w[kAtOnce];
+        uint32_t scale[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = h2f(static_cast<uint16_t>(w[j / 2] >> (16 * (j % 2))));
-        } else {
-            const float scale = h2f(*reinterpret_cast<const uint16_t*>(
-                part + c.page_size * row_bytes + 2 * ((at.row / 4 * (hd / 32) + dim / 32) * 4 + at.row % 4)));
-            uint32_t w;
-            if (plane == 0) {
-                w = FMT == kKvQ8_0 ? *reinterpret_cast<const uint32_t*>(from + dim) : *reinterpret_cast<const uint16_t*>(from + dim / 2);
+        for (int s = 0; s < kAtOnce; ++s) {
+            const uint32_t row = min((share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES, each - 1);
+            const uint32_t plane = row < c.kv_heads ? 0 : 1;
+            w[s] = u32x4_t{0, 0, 0, 0};
+            scale[s] = 0;
+            if (!at.there || s0 + s >= steps) continue;
+            const uint8_t* part = part_of_page(c, at.page, plane, row - plane * c.kv_heads, part_bytes);
+            const uint8_t* from = part + at.row * row_bytes;
+            if constexpr (FMT == kKvF32) {
+                w[s] = *reinterpret_cast<const u32x4_t*>(from + 4 * dim);
+            } else if constexpr (FMT == kKvF16) {
+                const u32x2_t x = *reinterpret_cast<const u32x2_t*>(from + 2 * dim);
+                w[s][0] = x[0];
+                w[s][1] = x[1];
             } else {
-                const uint32_t p0 = paged_value_place(hd, dim), p1 = paged_value_place(hd, dim + 2);
-                w = FMT == kKvQ8_0 ? *reinterpret_cast<const uint16_t*>(from + p0) |
-                                         static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(from + p1)) << 16
-                                   : from[p0 / 2] | static_cast<uint32_t>(from[p1 / 2]) << 8;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float code = FMT == kKvQ8_0 ? static_cast<float>(static_cast<int8_t>(w >> (8 * j)))
-                                                  : static_cast<float>(w >> (4 * j) & 15u) - 8.0f;
-                v[j] = code * scale;
+                scale[s] = *reinterpret_cast<const uint16_t*>(part + scale_at);
+                w[s][0] = FMT == kKvQ8_0 ? *reinterpret_cast<const uint32_t*>(from + dim) : *reinterpret_cast<const uint16_t*>(from + dim / 2);
             }
         }
+        if constexpr (paged_quantised(FMT)) {
+#pragma unroll
+            for (int s = 0; s < kAtOnce; ++s) {
+                const uint32_t row = (share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES;
+                uint8_t* codes = reinterpret_cast<uint8_t*>(rooms[threadIdx.x / kWave][s]) + threadIdx.x % kWave / LANES * LANES * 4;
+                // a key's four codes lie together, a value's two by two
+                const uint32_t q0 = row < c.kv_heads ? dim : p0, q1 = row < c.kv_heads ? dim + 2 : p1;
+                if constexpr (FMT == kKvQ8_0) {
+                    *reinterpret_cast<uint32_t*>(codes + dim) = w[s][0];
+                    wave_lds_fence();
+                    w[s][0] = *reinterpret_cast<const uint16_t*>(codes + q0);
+                    w[s][1] = *reinterpret_cast<const uint16_t*>(codes + q1);
+                } else {
+                    *reinterpret_cast<uint16_t*>(codes + dim / 2) = static_cast<uint16_t>(w[s][0]);
+                    wave_lds_fence();
+                    w[s][0] = codes[q0 / 2];
+                    w[s][1] = codes[q1 / 2];
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < kAtOnce; ++s) {
+            const uint32_t row = (share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES;
+            if (s0 + s >= steps || row >= each) continue;
+            const uint32_t plane = row < c.kv_heads ? 0 : 1;
+            float* out = plane ? a.value : a.key;
+            if (!out) continue;
+            f32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (FMT == kKvF32) {
+                    v[j] = __uint_as_float(w[s][j]);
+                } else if constexpr (FMT == kKvF16) {
+                    v[j] = h2f(static_cast<uint16_t>(w[s][j / 2] >> (16 * (j % 2))));
+                } else {
+                    const uint32_t two = w[s][j / 2];
+                    const float code = FMT == kKvQ8_0 ? static_cast<float>(static_cast<int8_t>(two >> (8 * (j % 2))))
+                                                      : static_cast<float>(two >> (4 * (j % 2)) & 15u) - 8.0f;
+                    v[j] = code * h2f(static_cast<uint16_t>(scale[s]));
+                }
+                if (paged_quantised(FMT) && !at.there) v[j] = 0.0f;  // not -0
+            }
+            __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(out + (static_cast<uint64_t>(share.token) * c.kv_heads + (row - plane * c.kv_heads)) * hd + dim));
+        }
     }
-    *reinterpret_cast<f32x4*>(out + (static_cast<uint64_t>(token) * c.kv_heads + kv_head) * hd + dim) = v;
 }
 
 uint32_t shift_of(uint32_t page_size) { return static_cast<uint32_t>(__builtin_ctz(page_size)); }
 
-template <int LANES>
-uint32_t groups_for(uint64_t rows) {
-    constexpr uint32_t kEach = kPagedThreads / LANES;
-    return static_cast<uint32_t>((rows + kEach - 1) / kEach);
-}
+// How a token's rows are shared out: few tokens go to many wavefronts, for their
+// loads' latency, and many have eight rows a lane, whose loads overlap.
+struct Shares {
+    uint32_t chunks, steps, groups;
+    Shares(uint64_t tokens, uint32_t rows, uint32_t at_once) {
+        const uint32_t all = (rows + at_once - 1) / at_once;  // steps of a token
+        chunks = 0;
+        while ((1u << chunks) < all && (((all + (1u << chunks) - 1) >> chunks) > 8 || tokens << chunks < 4096)) ++chunks;
+        steps = (all + (1u << chunks) - 1) >> chunks;
+        groups = static_cast<uint32_t>(((tokens << chunks) + kPagedWaves - 1) / kPagedWaves);
+    }
+};
 
 template <int FMT, int LANES>
 hipError_t launch_append(hipStream_t stream, const PagedAppendArgs& a) {
-    const uint64_t rows = static_cast<uint64_t>(a.tokens) * ((a.query ? a.q_heads : 0) + 2 * a.cache.kv_heads);
-    hipLaunchKernelGGL((paged_append_kernel<FMT, LANES>), dim3(groups_for<LANES>(rows)), dim3(kPagedThreads), 0, stream, a,
-                       shift_of(a.cache.page_size));
+    const Shares s(a.tokens, (a.query ? a.q_heads : 0) + 2 * a.cache.kv_heads, kWave / LANES);
+    hipLaunchKernelGGL((paged_append_kernel<FMT, LANES>), dim3(s.groups), dim3(kPagedThreads), 0, stream, a,
+                       shift_of(a.cache.page_size), s.chunks, s.steps);
     return hipGetLastError();
 }
 template <int FMT, int LANES>
 hipError_t launch_read(hipStream_t stream, const PagedReadArgs& a) {
-    const uint64_t rows = static_cast<uint64_t>(a.rows) * 2 * a.cache.kv_heads;
-    hipLaunchKernelGGL((paged_read_kernel<FMT, LANES>), dim3(groups_for<LANES>(rows)), dim3(kPagedThreads), 0, stream, a,
-                       shift_of(a.cache.page_size));
+    const Shares s(a.rows, 2 * a.cache.kv_heads, kWave / LANES);
+    hipLaunchKernelGGL((paged_read_kernel<FMT, LANES>), dim3(s.groups), dim3(kPagedThreads), 0, stream, a,
+                       shift_of(a.cache.page_size), s.chunks, s.steps);
     return hipGetLastError();
 }
 

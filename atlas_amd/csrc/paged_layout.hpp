@@ -29,7 +29,7 @@ __host__ __device__ inline uint32_t paged_row_code_bytes(int format, uint32_t he
         default: return head_dim / 2;
     }
 }
-__host__ __device__ inline bool paged_quantised(int format) { return format == kKvQ8_0 || format == kKvQ4_0; }
+__host__ __device__ constexpr bool paged_quantised(int format) { return format == kKvQ8_0 || format == kKvQ4_0; }
 // A head's rows of K or V in a page.
 __host__ __device__ inline uint32_t paged_part_bytes(int format, uint32_t page_size, uint32_t head_dim) {
     return page_size * (paged_row_code_bytes(format, head_dim) + (paged_quantised(format) ? head_dim / 32 * 2 : 0));
