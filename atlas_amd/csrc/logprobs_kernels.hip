@@ -11,9 +11,9 @@
 //
 // Launches: a wavefront a slice of 1024 logits leaves the slice's sums and the
 // maxima of its cells, 128 logits each; one workgroup a row joins them.  The
-// likeliest tokens cost the first launch nothing: of 64 groups of cells the k-th
+// likeliest tokens cost the first launch nothing: of 256 groups of cells the k-th
 // largest maximum is a border that k tokens reach, so only cells that reach it are
-// read again (a few hundred of 2048) and what reaches it in them is ranked.
+// read again (some 25 of 2048 for 20 tokens) and what reaches it in them is ranked.
 #include "exp2_f64.hpp"
 #include "launch.hpp"
 
@@ -33,16 +33,17 @@ constexpr uint32_t kCellList = 1024, kTokenList = 512;
 
 typedef f32x4 f32x4_row __attribute__((aligned(4)));
 
-// Sums of e^{y} and of e^{y} (-y), relative to the slice's top; the cells' maxima.
+// A slice's sums of e^{y} and of e^{y} (-y), relative to its top, y in thirty-seconds
+// of powers of two.
 struct SliceSums {
     double sum, spread;
-    float cells[kCells];
 };
 
 struct LogprobParams {
     TokenLogprobsArgs s;
-    double scale;      // 32 inv_temperature log2(e)
-    SliceSums* slices; // [row][slices]
+    double scale;            // 32 inv_temperature log2(e)
+    SliceSums* slices;       // [row][slices]
+    float* cells;            // [row][slices][kCells]: their maxima
     uint32_t count, blocks;  // slices of a row; workgroups of kLogWaves slices
 };
 
@@ -60,56 +61,118 @@ __device__ __forceinline__ void load_lane(const float* logits, uint32_t first, u
         for (int i = 0; i < kEach / 4; ++i) {
             const f32x4 y = *reinterpret_cast<const f32x4_row*>(logits + first + slice_at(lane, 4 * i));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[4 * i + j] = number_or_none(y[j]);
+            for (int j = 0; j < 4; ++j) x[4 * i + j] = y[j];
         }
     } else {
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const uint32_t at = first + slice_at(lane, i);
-            x[i] = at < vocab ? number_or_none(logits[at]) : -__builtin_inff();
+            x[i] = at < vocab ? logits[at] : -__builtin_inff();
         }
     }
 }
 
+// 2^(y / 1024), y <= 0, as Exp2 has 2^(y / 32): of a table of 1024 the polynomial
+// needs three degrees, ((ln 2 / 2048)^4 / 24 is below 2^-50).
+struct FineExp2 {
+    static constexpr uint32_t kSize = 1024;
+    const uint2* table;
+    double c[3], shift, least;
+
+    static __device__ void fill(uint2 (&table)[kSize]) {
+        for (uint32_t i = threadIdx.x; i < kSize; i += kLogThreads) {
+            const uint64_t bits = __builtin_bit_cast(uint64_t, exp2(i * (1.0 / kSize)));
+            table[i] = make_uint2(static_cast<uint32_t>(bits), static_cast<uint32_t>(bits >> 32) - (1023u << 20));
+        }
+    }
+    explicit __device__ FineExp2(const uint2 (&table)[kSize])
+        : table(table),
+          c{0x1.c6b08d704a0c0p-5 * 0x1p-30,  // ln2^3 / 6, of 1 / 1024 each
+            0x1.ebfbdff82c58fp-3 * 0x1p-20,  // ln2^2 / 2
+            0x1.62e42fefa39efp-1 * 0x1p-10}, // ln2
+          shift(0x1.8p52 + kSize * 1023.0), least(-1022.0 * kSize) {
+        asm("" : "+v"(c[0]));
+#pragma unroll
+        for (int i = 1; i < 3; ++i) asm("" : "+s"(c[i]));
+        asm("" : "+s"(shift));
+    }
+    __device__ __forceinline__ double operator()(double y) const {  // y >= least
+        const double t = y + shift;
+        const double r = y - (t - shift);
+        const uint32_t k = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, t));
+        double p = __builtin_fma(c[0], r, c[1]);
+        p = __builtin_fma(p, r, c[2]);
+        p = __builtin_fma(p, r, 1.0);
+        uint2 power = table[k % kSize];
+        power.y += k >> 10 << 20;
+        return p * __builtin_bit_cast(double, static_cast<uint64_t>(power.y) << 32 | power.x);
+    }
+};
+
+// Workgroups that stay: eight to a CU, and the table's filling, behind the first
+// logits' loads, once for all of a workgroup's slices.  Bound by the bytes and the
+// 64-bit instructions together, so a logit takes as few as there are: one that is no
+// number, and one too far below the top to have mass, become the lowest that has
+// hardly any in an instruction of 32 bits (where the top and the temperature let 32
+// bits tell them apart).
 template <bool SPREAD>
 __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams v) {
-    __shared__ uint2 table[32];
-    const uint32_t row = blockIdx.x / v.blocks, lane = threadIdx.x % kWave;
-    const uint32_t slice = blockIdx.x % v.blocks * kLogWaves + threadIdx.x / kWave;
+    __shared__ uint2 table[FineExp2::kSize];
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t items = v.s.rows * v.blocks;
+    uint32_t row = blockIdx.x / v.blocks, block = blockIdx.x % v.blocks;
+    const uint32_t row_step = gridDim.x / v.blocks, block_step = gridDim.x % v.blocks;
     float x[kEach];
-    load_lane(v.s.logits + row * v.s.row_stride, min(slice, v.count - 1) * kSlice, lane, v.s.vocab, x);
-    Exp2::fill(table);
-    const Exp2 exp2_of(table);
+    const auto load = [&] {
+        load_lane(v.s.logits + row * v.s.row_stride, min(block * kLogWaves + wave, v.count - 1) * kSlice, lane, v.s.vocab, x);
+    };
+    load();
+    FineExp2::fill(table);
+    const FineExp2 exp2_of(table);
+    const double scale = fmin(v.scale * 32.0, 0x1.fffffffffffffp1023), reach = 708.0 / v.s.inv_temperature;
     __syncthreads();
-    if (slice >= v.count) return;
-    float cell = -__builtin_inff();
+    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t slice = block * kLogWaves + wave;
+        const uint64_t at = static_cast<uint64_t>(row) * v.count + slice;
+        const bool there = slice < v.count;
+        float cell = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) cell = fmaxf(cell, x[i]);
-    cell = fmaxf(cell, dpp_f32<0xb1, 0xf, false>(cell));
-    cell = fmaxf(cell, dpp_f32<0x4e, 0xf, false>(cell));
-    cell = fmaxf(cell, dpp_f32<0x141, 0xf, false>(cell));
-    const float top = wave_max_tree_f32(cell);
-    if (top == __builtin_inff()) {
+        for (int i = 0; i < kEach; ++i) cell = fmaxf(cell, x[i]);
+        cell = fmaxf(cell, dpp_f32<0xb1, 0xf, false>(cell));
+        cell = fmaxf(cell, dpp_f32<0x4e, 0xf, false>(cell));
+        cell = fmaxf(cell, dpp_f32<0x141, 0xf, false>(cell));
+        const float top = wave_max_tree_f32(cell);
+        const double zero = finite(top);
+        double sum = 0.0, spread = 0.0;
+        const auto add = [&](double y) {
+            const double e = exp2_of(y);
+            sum += e;
+            if (SPREAD) spread = __builtin_fma(e, -y, spread);
+        };
+        // |top| within 2^20 temperatures: its neighbours are nearer than `reach`
+        if (__builtin_fabs(zero) * v.s.inv_temperature < 0x1p20 && v.s.inv_temperature > 0x1p-60 && !__builtin_isinf(top)) {
+            const float lowest = static_cast<float>(zero - reach);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) x[i] = about(x[i], top);
-    }
-    const double zero = finite(top);
-    double sum = 0.0, spread = 0.0;
+            for (int i = 0; i < kEach; ++i) add((static_cast<double>(fmaxf(x[i], lowest)) - zero) * scale);
+        } else {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const double y = fmax((static_cast<double>(x[i]) - zero) * v.scale, exp2_of.least);
-        const double e = exp2_of(y);
-        sum += e;
-        if (SPREAD) spread = __builtin_fma(e, -y, spread);
+            for (int i = 0; i < kEach; ++i) {
+                const double y = (static_cast<double>(about(number_or_none(x[i]), top)) - zero) * scale;
+                if (y >= exp2_of.least) add(y);
+            }
+        }
+        row += row_step;
+        block += block_step;
+        if (block >= v.blocks) {
+            block -= v.blocks;
+            ++row;
+        }
+        if (item + gridDim.x < items) load();
+        sum = wave_sum_f64(sum);
+        if (SPREAD) spread = wave_sum_f64(spread);
+        if (there && lane == 0) v.slices[at] = SliceSums{sum, spread * (1.0 / 32.0)};
+        if (there && lane % 8 == 0) v.cells[at * kCells + lane / 8] = cell;
     }
-    sum = wave_sum_f64(sum);
-    if (SPREAD) spread = wave_sum_f64(spread);
-    SliceSums* out = v.slices + static_cast<uint64_t>(row) * v.count + slice;
-    if (lane == 0) {
-        out->sum = sum;
-        out->spread = spread;
-    }
-    if (lane % 8 == 0) out->cells[lane / 8] = cell;
 }
 
 // A logit's place among all: larger first, of equal ones the lower index; 0: none.
@@ -135,19 +198,21 @@ __device__ __forceinline__ void for_cell(const float* logits, uint32_t cell, uin
 }
 
 // The place that exactly `k` tokens reach, by eight bits a pass over the cells
-// that reach `border`: for rows where too many tokens are level for a list.
-__device__ uint64_t exact_border(const LogprobParams& v, const float* logits, const SliceSums* slices, uint32_t border, uint32_t k,
+// that reach `border`: for rows where too many tokens are level for a list.  1
+// where there are fewer than k.
+template <int THREADS>
+__device__ uint64_t exact_border(const LogprobParams& v, const float* logits, const float* cells, uint32_t border, uint32_t k,
                                  uint32_t (&bins)[256], uint64_t& state, uint32_t& left) {
     if (threadIdx.x == 0) {
         state = 0;
         left = k;
     }
     for (int shift = 56; shift >= 0; shift -= 8) {
-        bins[threadIdx.x] = 0;
+        if (threadIdx.x < 256) bins[threadIdx.x] = 0;
         __syncthreads();
         const uint64_t above = state;
-        for (uint32_t cell = threadIdx.x / 8; cell < v.count * kCells; cell += kLogThreads / 8) {
-            if (ordered(slices[cell / kCells].cells[cell % kCells]) < border) continue;
+        for (uint32_t cell = threadIdx.x / 8; cell < v.count * kCells; cell += THREADS / 8) {
+            if (ordered(cells[cell]) < border) continue;
             for_cell(logits, cell, v.s.vocab, [&](float x, uint32_t index) {
                 const uint64_t place = place_of(x, index);
                 if (place && (shift == 56 || place >> (shift + 8) == above >> (shift + 8))) atomicAdd(&bins[place >> shift & 255], 1u);
@@ -157,8 +222,7 @@ __device__ uint64_t exact_border(const LogprobParams& v, const float* logits, co
         if (threadIdx.x == 0) {
             uint32_t need = left, bin = 256;
             while (bin-- > 0 && bins[bin] < need) need -= bins[bin];
-            // fewer than k in all: the first pass ends below its lowest bin, and every token counts
-            if (bin == 0xffffffffu) {
+            if (bin == 0xffffffffu) {  // fewer than k in all, known after the first pass
                 left = 0;
             } else {
                 state = above | static_cast<uint64_t>(bin) << shift;
@@ -171,11 +235,15 @@ __device__ uint64_t exact_border(const LogprobParams& v, const float* logits, co
     return state;
 }
 
-// One workgroup a row.
-__global__ __launch_bounds__(kLogThreads) void logprob_rows_kernel(LogprobParams v) {
+// One workgroup a row, of 1024 threads where the rows do not fill the chip by
+// themselves: its steps wait for one another and for memory (256 rows of 262144
+// logits, 20 tokens each, 10 us with 256 threads).
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) {
+    constexpr uint32_t kWaves = THREADS / kWave, kBorderGroups = 256;
     __shared__ uint2 table[32];
-    __shared__ double wave_sum[kLogWaves], wave_spread[kLogWaves];
-    __shared__ float wave_top[kLogWaves];
+    __shared__ double wave_sum[kWaves], wave_spread[kWaves];
+    __shared__ float wave_top[kWaves], group_top[THREADS];
     __shared__ uint32_t border_room, cell_count, token_count, left_room;
     __shared__ uint64_t state_room;
     __shared__ union {
@@ -186,55 +254,72 @@ __global__ __launch_bounds__(kLogThreads) void logprob_rows_kernel(LogprobParams
         uint32_t bins[256];
     } room;
     const TokenLogprobsArgs& s = v.s;
-    const uint32_t row = blockIdx.x, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const uint32_t row = blockIdx.x, lane = threadIdx.x % kWave;
+    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
     const float* logits = s.logits + row * s.row_stride;
     const SliceSums* slices = v.slices + static_cast<uint64_t>(row) * v.count;
+    const float* cells = v.cells + static_cast<uint64_t>(row) * v.count * kCells;
+    const uint32_t cells_of_row = v.count * kCells;
     Exp2::fill(table);
     const Exp2 exp2_of(table);
 
-    // the row's top, and with it the border: the k-th largest of 64 groups' maxima
-    const uint32_t cells = v.count * kCells;
     float mine = -__builtin_inff();
-    for (uint32_t i = threadIdx.x; i < cells; i += kLogThreads) mine = fmaxf(mine, slices[i / kCells].cells[i % kCells]);
+    for (uint32_t i = threadIdx.x; i < cells_of_row; i += THREADS) mine = fmaxf(mine, cells[i]);
     const float wtop = wave_max_tree_f32(mine);
     if (lane == 0) wave_top[wave] = wtop;
-    __shared__ float group_top[kLogThreads];
     group_top[threadIdx.x] = mine;
     if (threadIdx.x == 0) cell_count = token_count = 0;
     __syncthreads();
-    const float top = fmaxf(fmaxf(wave_top[0], wave_top[1]), fmaxf(wave_top[2], wave_top[3]));
-    if (s.top && wave == 0) {
-        uint32_t group = 0;
-        for (int w = 0; w < kLogWaves; ++w) group = max(group, ordered(group_top[w * kWave + lane]));
-        uint32_t border = 0;
+    float top = wave_top[0];
 #pragma unroll
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t with = border | 1u << bit;
-            if (static_cast<uint32_t>(__builtin_popcountll(__builtin_amdgcn_ballot_w64(group >= with))) >= s.top) border = with;
+    for (uint32_t w = 1; w < kWaves; ++w) top = fmaxf(top, wave_top[w]);
+
+    // one wavefront finds the border, to 21 bits of its place, while the others sum
+    const bool finds = s.top && wave == 0;
+    double sum = 0.0, spread = 0.0;
+    if (finds) {
+        uint32_t group[kBorderGroups / kWave];
+#pragma unroll
+        for (uint32_t j = 0; j < kBorderGroups / kWave; ++j) {
+            float x = -__builtin_inff();
+#pragma unroll
+            for (uint32_t i = 0; i < THREADS / kBorderGroups; ++i) x = fmaxf(x, group_top[i * kBorderGroups + j * kWave + lane]);
+            group[j] = ordered(x);
+        }
+        uint32_t border = 0;
+        for (uint32_t bit = 1u << 31; bit >= 1u << 11; bit >>= 1) {
+            const uint32_t with = border | bit;
+            uint32_t reached = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < kBorderGroups / kWave; ++j)
+                reached += static_cast<uint32_t>(__builtin_popcountll(__builtin_amdgcn_ballot_w64(group[j] >= with)));
+            if (reached >= s.top) border = with;
         }
         if (lane == 0) border_room = max(border, 1u);
+    } else {
+        const uint32_t summing = s.top ? THREADS - kWave : THREADS;
+        for (uint32_t i = threadIdx.x - (THREADS - summing); i < v.count; i += summing) {
+            const SliceSums x = slices[i];
+            const f32x4 c0 = *reinterpret_cast<const f32x4*>(cells + i * kCells), c1 = *reinterpret_cast<const f32x4*>(cells + i * kCells + 4);
+            const float slice_top = fmaxf(fmaxf(fmaxf(c0.x, c0.y), fmaxf(c0.z, c0.w)), fmaxf(fmaxf(c1.x, c1.y), fmaxf(c1.z, c1.w)));
+            const double y = fmax((static_cast<double>(about(slice_top, top)) - finite(top)) * v.scale, exp2_of.least);
+            const double f = exp2_of(y);
+            sum = __builtin_fma(f, x.sum, sum);
+            spread = __builtin_fma(f, __builtin_fma(-y, x.sum, x.spread), spread);
+        }
+        sum = wave_sum_f64(sum);
+        spread = wave_sum_f64(spread);
     }
-
-    double sum = 0.0, spread = 0.0;
-    for (uint32_t i = threadIdx.x; i < v.count; i += kLogThreads) {
-        const SliceSums x = slices[i];
-        float slice_top = x.cells[0];
-#pragma unroll
-        for (uint32_t j = 1; j < kCells; ++j) slice_top = fmaxf(slice_top, x.cells[j]);
-        const double y = fmax((static_cast<double>(about(slice_top, top)) - finite(top)) * v.scale, exp2_of.least);
-        const double f = exp2_of(y);
-        sum = __builtin_fma(f, x.sum, sum);
-        spread = __builtin_fma(f, __builtin_fma(-y, x.sum, x.spread), spread);
-    }
-    sum = wave_sum_f64(sum);
-    spread = wave_sum_f64(spread);
     if (lane == 0) {
         wave_sum[wave] = sum;
         wave_spread[wave] = spread;
     }
     __syncthreads();
-    sum = (wave_sum[0] + wave_sum[1]) + (wave_sum[2] + wave_sum[3]);
-    spread = (wave_spread[0] + wave_spread[1]) + (wave_spread[2] + wave_spread[3]);
+    sum = spread = 0.0;
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        sum += wave_sum[w];
+        spread += wave_spread[w];
+    }
     const bool any = top > -__builtin_inff();
     const double log_sum = any ? log(sum) : 0.0;
     const auto logprob = [&](float x) {
@@ -244,7 +329,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_rows_kernel(LogprobParams
     if (s.entropy && threadIdx.x == 0)
         // thirty-seconds of powers of two to natural units
         s.entropy[row] = any ? static_cast<float>(log_sum + spread / sum * (0x1.62e42fefa39efp-1 / 32.0)) : 0.0f;
-    for (uint32_t i = threadIdx.x; i < s.given; i += kLogThreads) {
+    for (uint32_t i = threadIdx.x; i < s.given; i += THREADS) {
         const uint64_t at = static_cast<uint64_t>(row) * s.given + i;
         const uint32_t token = s.tokens[at];
         s.logprobs[at] = token < s.vocab ? logprob(logits[token]) : -__builtin_inff();
@@ -252,8 +337,8 @@ __global__ __launch_bounds__(kLogThreads) void logprob_rows_kernel(LogprobParams
     if (!s.top) return;
 
     const uint32_t border = border_room;
-    for (uint32_t i = threadIdx.x; i < cells; i += kLogThreads)
-        if (ordered(slices[i / kCells].cells[i % kCells]) >= border) {
+    for (uint32_t i = threadIdx.x; i < cells_of_row; i += THREADS)
+        if (ordered(cells[i]) >= border) {
             const uint32_t at = atomicAdd(&cell_count, 1u);
             if (at < kCellList) room.list.cells[at] = i;
         }
@@ -267,19 +352,19 @@ __global__ __launch_bounds__(kLogThreads) void logprob_rows_kernel(LogprobParams
         }
     };
     if (cell_count <= kCellList)
-        for (uint32_t i = threadIdx.x / 8; i < cell_count; i += kLogThreads / 8) for_cell(logits, room.list.cells[i], s.vocab, push);
+        for (uint32_t i = threadIdx.x / 8; i < cell_count; i += THREADS / 8) for_cell(logits, room.list.cells[i], s.vocab, push);
     __syncthreads();
     if (cell_count > kCellList || token_count > kTokenList) {
         __syncthreads();
         if (threadIdx.x == 0) token_count = 0;
-        reach = exact_border(v, logits, slices, border, s.top, room.bins, state_room, left_room);
+        reach = exact_border<THREADS>(v, logits, cells, border, s.top, room.bins, state_room, left_room);
         __syncthreads();
-        for (uint32_t i = threadIdx.x / 8; i < cells; i += kLogThreads / 8)
-            if (ordered(slices[i / kCells].cells[i % kCells]) >= border) for_cell(logits, i, s.vocab, push);
+        for (uint32_t i = threadIdx.x / 8; i < cells_of_row; i += THREADS / 8)
+            if (ordered(cells[i]) >= border) for_cell(logits, i, s.vocab, push);
         __syncthreads();
     }
     const uint32_t count = token_count;
-    for (uint32_t i = threadIdx.x; i < count; i += kLogThreads) {
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
         const uint64_t place = room.list.tokens[i];
         uint32_t rank = 0;
         for (uint32_t j = 0; j < count; ++j) rank += room.list.tokens[j] > place;
@@ -288,18 +373,20 @@ __global__ __launch_bounds__(kLogThreads) void logprob_rows_kernel(LogprobParams
             s.top_logprobs[static_cast<uint64_t>(row) * s.top + rank] = logprob(value_of(static_cast<uint32_t>(place >> 32)));
         }
     }
-    for (uint32_t i = count + threadIdx.x; i < s.top; i += kLogThreads) {
+    for (uint32_t i = count + threadIdx.x; i < s.top; i += THREADS) {
         s.top_ids[static_cast<uint64_t>(row) * s.top + i] = kNoToken;
         s.top_logprobs[static_cast<uint64_t>(row) * s.top + i] = -__builtin_inff();
     }
 }
+
+constexpr uint32_t kGroups = 256 * 8;
 
 uint32_t slices_of(uint32_t vocab) { return (vocab + kSlice - 1) / kSlice; }
 
 }  // namespace
 
 uint64_t token_logprobs_workspace(uint32_t rows, uint32_t vocab, uint32_t) {
-    return static_cast<uint64_t>(rows) * slices_of(vocab) * sizeof(SliceSums);
+    return static_cast<uint64_t>(rows) * slices_of(vocab) * (sizeof(SliceSums) + kCells * sizeof(float));
 }
 
 hipError_t launch_token_logprobs(hipStream_t stream, const TokenLogprobsArgs& s) {
@@ -309,15 +396,20 @@ hipError_t launch_token_logprobs(hipStream_t stream, const TokenLogprobsArgs& s)
     v.scale = std::min(32.0 * 1.4426950408889634074 * s.inv_temperature, std::numeric_limits<double>::max());
     v.slices = static_cast<SliceSums*>(s.workspace);
     v.count = slices_of(s.vocab);
+    v.cells = reinterpret_cast<float*>(v.slices + static_cast<uint64_t>(s.rows) * v.count);
     v.blocks = (v.count + kLogWaves - 1) / kLogWaves;
-    const dim3 grid(s.rows * v.blocks), block(kLogThreads);
+    const uint64_t items = static_cast<uint64_t>(s.rows) * v.blocks;
+    const dim3 grid(static_cast<uint32_t>(items < kGroups ? items : kGroups)), block(kLogThreads);
     if (s.entropy)
         hipLaunchKernelGGL(logprob_sums_kernel<true>, grid, block, 0, stream, v);
     else
         hipLaunchKernelGGL(logprob_sums_kernel<false>, grid, block, 0, stream, v);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(logprob_rows_kernel, dim3(s.rows), block, 0, stream, v);
+    if (s.rows <= 512)
+        hipLaunchKernelGGL(logprob_rows_kernel<1024>, dim3(s.rows), dim3(1024), 0, stream, v);
+    else
+        hipLaunchKernelGGL(logprob_rows_kernel<256>, dim3(s.rows), dim3(256), 0, stream, v);
     return hipGetLastError();
 }
 
