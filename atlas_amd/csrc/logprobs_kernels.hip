@@ -9,9 +9,9 @@
 // 64 bits, so a likely token's small log probability keeps its digits.  NaN and
 // -inf logits have no mass; all of a row's mass lies on its +inf.
 //
-// Launches: a wavefront a slice of 1024 logits leaves the slice's sums and the
+// Launches: a wavefront a slice of one or two strips of 1024 logits leaves the slice's sums and the
 // maxima of its cells, 128 logits each; one workgroup a row joins them.  The
-// likeliest tokens cost the first launch nothing: of 256 groups of cells the k-th
+// likeliest tokens cost the first launch nothing: of 64 or 256 groups of cells the k-th
 // largest maximum is a border that k tokens reach, so only cells that reach it are
 // read again (some 25 of 2048 for 20 tokens) and what reaches it in them is ranked.
 #include "exp2_f64.hpp"
@@ -25,9 +25,9 @@ namespace {
 
 constexpr int kLogThreads = 256;
 constexpr int kLogWaves = kLogThreads / kWave;
-constexpr uint32_t kSlice = 1024;  // a wavefront's, 16 logits a lane
-constexpr int kEach = kSlice / kWave;
-constexpr uint32_t kCells = 8;     // of a slice: the logits of eight lanes
+constexpr uint32_t kStrip = 1024;  // 16 logits a lane
+constexpr uint32_t kCells = 8;     // of a strip: the logits of eight lanes
+constexpr int kEach = kStrip / kWave;
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr uint32_t kCellList = 1024, kTokenList = 512;
 
@@ -43,8 +43,9 @@ struct LogprobParams {
     TokenLogprobsArgs s;
     double scale;            // 32 inv_temperature log2(e)
     SliceSums* slices;       // [row][slices]
-    float* cells;            // [row][slices][kCells]: their maxima
-    uint32_t count, blocks;  // slices of a row; workgroups of kLogWaves slices
+    float* cells;            // [row][strips][kCells]: their maxima
+    uint32_t strips, count;  // strips and slices of a row
+    uint32_t each;           // strips of a slice
 };
 
 __device__ __forceinline__ float about(float x, float top) {
@@ -52,11 +53,11 @@ __device__ __forceinline__ float about(float x, float top) {
 }
 __device__ __forceinline__ double finite(float top) { return __builtin_isinf(top) ? 0.0 : static_cast<double>(top); }
 
-// Logit i of a lane's, four at a time; lanes 8 r .. 8 r + 7 have cell r.
+// Logit i of a lane's in a strip, four at a time; lanes 8 r .. 8 r + 7 have cell r.
 __device__ __forceinline__ uint32_t slice_at(uint32_t lane, int i) { return (i / 4 * kWave + lane) * 4 + i % 4; }
 
 __device__ __forceinline__ void load_lane(const float* logits, uint32_t first, uint32_t lane, uint32_t vocab, float (&x)[kEach]) {
-    if (first + kSlice <= vocab) {
+    if (first + kStrip <= vocab) {
 #pragma unroll
         for (int i = 0; i < kEach / 4; ++i) {
             const f32x4 y = *reinterpret_cast<const f32x4_row*>(logits + first + slice_at(lane, 4 * i));
@@ -104,7 +105,7 @@ struct FineExp2 {
         p = __builtin_fma(p, r, c[2]);
         p = __builtin_fma(p, r, 1.0);
         uint2 power = table[k % kSize];
-        power.y += k >> 10 << 20;
+        power.y += (k & ~(kSize - 1)) << 10;
         return p * __builtin_bit_cast(double, static_cast<uint64_t>(power.y) << 32 | power.x);
     }
 };
@@ -115,33 +116,41 @@ struct FineExp2 {
 // number, and one too far below the top to have mass, become the lowest that has
 // hardly any in an instruction of 32 bits (where the top and the temperature let 32
 // bits tell them apart).
-template <bool SPREAD>
+template <bool SPREAD, int STRIPS>
 __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams v) {
     __shared__ uint2 table[FineExp2::kSize];
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const uint32_t items = v.s.rows * v.blocks;
-    uint32_t row = blockIdx.x / v.blocks, block = blockIdx.x % v.blocks;
-    const uint32_t row_step = gridDim.x / v.blocks, block_step = gridDim.x % v.blocks;
-    float x[kEach];
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
+    // a wavefront's slices of all rows', every `step`-th
+    const uint64_t items = static_cast<uint64_t>(v.s.rows) * v.count;
+    const uint32_t step = gridDim.x * kLogWaves, first = min(blockIdx.x * kLogWaves + wave, static_cast<uint32_t>(items - 1));
+    uint32_t row = first / v.count, slice = first % v.count;
+    const uint32_t row_step = step / v.count, slice_step = step % v.count;
+    float x[STRIPS][kEach];
     const auto load = [&] {
-        load_lane(v.s.logits + row * v.s.row_stride, min(block * kLogWaves + wave, v.count - 1) * kSlice, lane, v.s.vocab, x);
+        const float* logits = v.s.logits + row * v.s.row_stride;
+#pragma unroll
+        for (int i = 0; i < STRIPS; ++i) load_lane(logits, (slice * STRIPS + i) * kStrip, lane, v.s.vocab, x[i]);
     };
     load();
     FineExp2::fill(table);
     const FineExp2 exp2_of(table);
     const double scale = fmin(v.scale * 32.0, 0x1.fffffffffffffp1023), reach = 708.0 / v.s.inv_temperature;
     __syncthreads();
-    for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const uint32_t slice = block * kLogWaves + wave;
+    for (uint64_t item = blockIdx.x * kLogWaves + wave; item < items; item += step) {
         const uint64_t at = static_cast<uint64_t>(row) * v.count + slice;
-        const bool there = slice < v.count;
-        float cell = -__builtin_inff();
+        float cell[STRIPS], most = -__builtin_inff();
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) cell = fmaxf(cell, x[i]);
-        cell = fmaxf(cell, dpp_f32<0xb1, 0xf, false>(cell));
-        cell = fmaxf(cell, dpp_f32<0x4e, 0xf, false>(cell));
-        cell = fmaxf(cell, dpp_f32<0x141, 0xf, false>(cell));
-        const float top = wave_max_tree_f32(cell);
+        for (int i = 0; i < STRIPS; ++i) {
+            cell[i] = -__builtin_inff();
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) cell[i] = fmaxf(cell[i], x[i][j]);
+            cell[i] = fmaxf(cell[i], dpp_f32<0xb1, 0xf, false>(cell[i]));
+            cell[i] = fmaxf(cell[i], dpp_f32<0x4e, 0xf, false>(cell[i]));
+            cell[i] = fmaxf(cell[i], dpp_f32<0x141, 0xf, false>(cell[i]));
+            most = fmaxf(most, cell[i]);
+        }
+        const float top = wave_max_tree_f32(most);
         const double zero = finite(top);
         double sum = 0.0, spread = 0.0;
         const auto add = [&](double y) {
@@ -153,25 +162,34 @@ __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams
         if (__builtin_fabs(zero) * v.s.inv_temperature < 0x1p20 && v.s.inv_temperature > 0x1p-60 && !__builtin_isinf(top)) {
             const float lowest = static_cast<float>(zero - reach);
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) add((static_cast<double>(fmaxf(x[i], lowest)) - zero) * scale);
+            for (int i = 0; i < STRIPS; ++i)
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) add((static_cast<double>(fmaxf(x[i][j], lowest)) - zero) * scale);
         } else {
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const double y = (static_cast<double>(about(number_or_none(x[i]), top)) - zero) * scale;
-                if (y >= exp2_of.least) add(y);
-            }
+            for (int i = 0; i < STRIPS; ++i)
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) {
+                    const double y = (static_cast<double>(about(number_or_none(x[i][j]), top)) - zero) * scale;
+                    if (y >= exp2_of.least) add(y);
+                }
         }
+        float* cells = v.cells + static_cast<uint64_t>(row) * v.strips * kCells;
+        const uint32_t strip = slice * STRIPS;
         row += row_step;
-        block += block_step;
-        if (block >= v.blocks) {
-            block -= v.blocks;
+        slice += slice_step;
+        if (slice >= v.count) {
+            slice -= v.count;
             ++row;
         }
-        if (item + gridDim.x < items) load();
+        if (item + step < items) load();
         sum = wave_sum_f64(sum);
         if (SPREAD) spread = wave_sum_f64(spread);
-        if (there && lane == 0) v.slices[at] = SliceSums{sum, spread * (1.0 / 32.0)};
-        if (there && lane % 8 == 0) v.cells[at * kCells + lane / 8] = cell;
+        if (lane == 0) v.slices[at] = SliceSums{sum, spread * (1.0 / 32.0)};
+        if (lane % 8 == 0)
+#pragma unroll
+            for (uint32_t i = 0; i < STRIPS; ++i)
+                if (strip + i < v.strips) cells[static_cast<uint64_t>(strip + i) * kCells + lane / 8] = cell[i];
     }
 }
 
@@ -190,7 +208,7 @@ __device__ __forceinline__ float value_of(uint32_t u) { return __uint_as_float(u
 // Every logit of the cells that reach `border`, by eight lanes a cell.
 template <class F>
 __device__ __forceinline__ void for_cell(const float* logits, uint32_t cell, uint32_t vocab, F&& f) {
-    const uint32_t lane = threadIdx.x % 8 + cell % kCells * 8, first = cell / kCells * kSlice;
+    const uint32_t lane = threadIdx.x % 8 + cell % kCells * 8, first = cell / kCells * kStrip;
     float x[kEach];
     load_lane(logits, first, lane, vocab, x);
 #pragma unroll
@@ -211,7 +229,7 @@ __device__ uint64_t exact_border(const LogprobParams& v, const float* logits, co
         if (threadIdx.x < 256) bins[threadIdx.x] = 0;
         __syncthreads();
         const uint64_t above = state;
-        for (uint32_t cell = threadIdx.x / 8; cell < v.count * kCells; cell += THREADS / 8) {
+        for (uint32_t cell = threadIdx.x / 8; cell < v.strips * kCells; cell += THREADS / 8) {
             if (ordered(cells[cell]) < border) continue;
             for_cell(logits, cell, v.s.vocab, [&](float x, uint32_t index) {
                 const uint64_t place = place_of(x, index);
@@ -235,12 +253,36 @@ __device__ uint64_t exact_border(const LogprobParams& v, const float* logits, co
     return state;
 }
 
+// The s.top-th largest of 64 EACH groups' maxima, to 21 bits of its place, by one wavefront.
+template <int EACH, int THREADS>
+__device__ __forceinline__ uint32_t border_of(const float (&maxima)[THREADS], uint32_t lane, uint32_t k) {
+    uint32_t group[EACH];
+#pragma unroll
+    for (uint32_t j = 0; j < EACH; ++j) {
+        float x = -__builtin_inff();
+#pragma unroll
+        for (uint32_t i = 0; i < THREADS / (EACH * kWave); ++i) x = fmaxf(x, maxima[(i * EACH + j) * kWave + lane]);
+        group[j] = ordered(x);
+    }
+    uint32_t border = 0;
+#pragma unroll
+    for (uint32_t bit = 1u << 31; bit >= 1u << 11; bit >>= 1) {
+        const uint32_t with = border | bit;
+        uint32_t reached = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < EACH; ++j)
+            reached += static_cast<uint32_t>(__builtin_popcountll(__builtin_amdgcn_ballot_w64(group[j] >= with)));
+        if (reached >= k) border = with;
+    }
+    return border;
+}
+
 // One workgroup a row, of 1024 threads where the rows do not fill the chip by
 // themselves: its steps wait for one another and for memory (256 rows of 262144
 // logits, 20 tokens each, 10 us with 256 threads).
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) {
-    constexpr uint32_t kWaves = THREADS / kWave, kBorderGroups = 256;
+    constexpr uint32_t kWaves = THREADS / kWave;
     __shared__ uint2 table[32];
     __shared__ double wave_sum[kWaves], wave_spread[kWaves];
     __shared__ float wave_top[kWaves], group_top[THREADS];
@@ -258,13 +300,14 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
     const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
     const float* logits = s.logits + row * s.row_stride;
     const SliceSums* slices = v.slices + static_cast<uint64_t>(row) * v.count;
-    const float* cells = v.cells + static_cast<uint64_t>(row) * v.count * kCells;
-    const uint32_t cells_of_row = v.count * kCells;
+    const float* cells = v.cells + static_cast<uint64_t>(row) * v.strips * kCells;
+    const uint32_t cells_of_row = v.strips * kCells;
     Exp2::fill(table);
     const Exp2 exp2_of(table);
 
-    float mine = -__builtin_inff();
-    for (uint32_t i = threadIdx.x; i < cells_of_row; i += THREADS) mine = fmaxf(mine, cells[i]);
+    const float first_cell = threadIdx.x < cells_of_row ? cells[threadIdx.x] : -__builtin_inff();
+    float mine = first_cell;
+    for (uint32_t i = threadIdx.x + THREADS; i < cells_of_row; i += THREADS) mine = fmaxf(mine, cells[i]);
     const float wtop = wave_max_tree_f32(mine);
     if (lane == 0) wave_top[wave] = wtop;
     group_top[threadIdx.x] = mine;
@@ -274,34 +317,23 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
 #pragma unroll
     for (uint32_t w = 1; w < kWaves; ++w) top = fmaxf(top, wave_top[w]);
 
-    // one wavefront finds the border, to 21 bits of its place, while the others sum
+    // one wavefront finds the border while the others sum
     const bool finds = s.top && wave == 0;
     double sum = 0.0, spread = 0.0;
     if (finds) {
-        uint32_t group[kBorderGroups / kWave];
-#pragma unroll
-        for (uint32_t j = 0; j < kBorderGroups / kWave; ++j) {
-            float x = -__builtin_inff();
-#pragma unroll
-            for (uint32_t i = 0; i < THREADS / kBorderGroups; ++i) x = fmaxf(x, group_top[i * kBorderGroups + j * kWave + lane]);
-            group[j] = ordered(x);
-        }
-        uint32_t border = 0;
-        for (uint32_t bit = 1u << 31; bit >= 1u << 11; bit >>= 1) {
-            const uint32_t with = border | bit;
-            uint32_t reached = 0;
-#pragma unroll
-            for (uint32_t j = 0; j < kBorderGroups / kWave; ++j)
-                reached += static_cast<uint32_t>(__builtin_popcountll(__builtin_amdgcn_ballot_w64(group[j] >= with)));
-            if (reached >= s.top) border = with;
-        }
+        // 64 groups do for few tokens: 20 of them leave some 24 above the border
+        const uint32_t border = s.top <= 24 ? border_of<1, THREADS>(group_top, lane, s.top) : border_of<4, THREADS>(group_top, lane, s.top);
         if (lane == 0) border_room = max(border, 1u);
     } else {
         const uint32_t summing = s.top ? THREADS - kWave : THREADS;
         for (uint32_t i = threadIdx.x - (THREADS - summing); i < v.count; i += summing) {
             const SliceSums x = slices[i];
-            const f32x4 c0 = *reinterpret_cast<const f32x4*>(cells + i * kCells), c1 = *reinterpret_cast<const f32x4*>(cells + i * kCells + 4);
-            const float slice_top = fmaxf(fmaxf(fmaxf(c0.x, c0.y), fmaxf(c0.z, c0.w)), fmaxf(fmaxf(c1.x, c1.y), fmaxf(c1.z, c1.w)));
+            float slice_top = -__builtin_inff();
+            // the last slice may have a strip less
+            for (uint32_t j = i * v.each * kCells; j < min((i + 1) * v.each * kCells, cells_of_row); j += 4) {
+                const f32x4 c = *reinterpret_cast<const f32x4*>(cells + j);
+                slice_top = fmaxf(slice_top, fmaxf(fmaxf(c.x, c.y), fmaxf(c.z, c.w)));
+            }
             const double y = fmax((static_cast<double>(about(slice_top, top)) - finite(top)) * v.scale, exp2_of.least);
             const double f = exp2_of(y);
             sum = __builtin_fma(f, x.sum, sum);
@@ -338,7 +370,7 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
 
     const uint32_t border = border_room;
     for (uint32_t i = threadIdx.x; i < cells_of_row; i += THREADS)
-        if (ordered(cells[i]) >= border) {
+        if (ordered(i < THREADS ? first_cell : cells[i]) >= border) {
             const uint32_t at = atomicAdd(&cell_count, 1u);
             if (at < kCellList) room.list.cells[at] = i;
         }
@@ -381,12 +413,19 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
 
 constexpr uint32_t kGroups = 256 * 8;
 
-uint32_t slices_of(uint32_t vocab) { return (vocab + kSlice - 1) / kSlice; }
+uint32_t strips_of(uint32_t vocab) { return (vocab + kStrip - 1) / kStrip; }
+// Two strips to a slice halve what a slice costs beside its logits; one where that
+// leaves CUs idle (one row of 49152 logits 4.7 -> 4.0 us).
+uint32_t strips_each(uint32_t rows, uint32_t vocab) { return static_cast<uint64_t>(rows) * strips_of(vocab) >= 256 * 32 ? 2 : 1; }
+uint32_t slices_of(uint32_t rows, uint32_t vocab) {
+    const uint32_t each = strips_each(rows, vocab);
+    return (strips_of(vocab) + each - 1) / each;
+}
 
 }  // namespace
 
 uint64_t token_logprobs_workspace(uint32_t rows, uint32_t vocab, uint32_t) {
-    return static_cast<uint64_t>(rows) * slices_of(vocab) * (sizeof(SliceSums) + kCells * sizeof(float));
+    return static_cast<uint64_t>(rows) * (slices_of(rows, vocab) * sizeof(SliceSums) + strips_of(vocab) * kCells * sizeof(float));
 }
 
 hipError_t launch_token_logprobs(hipStream_t stream, const TokenLogprobsArgs& s) {
@@ -395,15 +434,15 @@ hipError_t launch_token_logprobs(hipStream_t stream, const TokenLogprobsArgs& s)
     // finite, or the top itself would be 0 times infinity
     v.scale = std::min(32.0 * 1.4426950408889634074 * s.inv_temperature, std::numeric_limits<double>::max());
     v.slices = static_cast<SliceSums*>(s.workspace);
-    v.count = slices_of(s.vocab);
+    v.strips = strips_of(s.vocab);
+    v.count = slices_of(s.rows, s.vocab);
+    v.each = strips_each(s.rows, s.vocab);
     v.cells = reinterpret_cast<float*>(v.slices + static_cast<uint64_t>(s.rows) * v.count);
-    v.blocks = (v.count + kLogWaves - 1) / kLogWaves;
-    const uint64_t items = static_cast<uint64_t>(s.rows) * v.blocks;
+    const uint64_t items = (static_cast<uint64_t>(s.rows) * v.count + kLogWaves - 1) / kLogWaves;
     const dim3 grid(static_cast<uint32_t>(items < kGroups ? items : kGroups)), block(kLogThreads);
-    if (s.entropy)
-        hipLaunchKernelGGL(logprob_sums_kernel<true>, grid, block, 0, stream, v);
-    else
-        hipLaunchKernelGGL(logprob_sums_kernel<false>, grid, block, 0, stream, v);
+    const auto sums = s.entropy ? (v.each == 2 ? logprob_sums_kernel<true, 2> : logprob_sums_kernel<true, 1>)
+                                : (v.each == 2 ? logprob_sums_kernel<false, 2> : logprob_sums_kernel<false, 1>);
+    hipLaunchKernelGGL(sums, grid, block, 0, stream, v);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (s.rows <= 512)
