@@ -20,8 +20,7 @@
 
 namespace atlas {
 
-inline constexpr int kPagedAttnThreads = 256;
-inline constexpr int kPagedAttnWaves = kPagedAttnThreads / kWave;
+inline constexpr uint32_t kPagedAttnWaves = 4;  // of a workgroup that takes a part
 inline constexpr uint32_t kPagedHeads = 16;  // query heads of a row: the columns of a product
 
 // The first and last part of a row.
@@ -41,6 +40,7 @@ struct PagedAttnParams {
     uint64_t page_bytes;
     uint32_t part_bytes, page_count, page_shift, table_width, sequences, capacity;
     uint32_t kv_heads, group, head_tiles, heads, q_heads, head_dim, window;
+    uint32_t row_units;                          // rows are not split, and have as many units at most; 0: they are
     uint32_t few_parts, most_parts, part_units;  // parts of all work; units of a part where there are more than few_parts
     float scale;                                 // with log2(e)
 };
@@ -620,9 +620,12 @@ struct Step {
     static __device__ constexpr uint32_t query_dim(uint32_t j) { return kBytes ? j : j / 2 + j % 2 * 4; }
 };
 
-template <int FMT, int NB, int HP>
-__global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void paged_attention_kernel(PagedAttnParams a) {
+// A workgroup a part of the work, or a whole row: then no other sequence's length
+// is asked for and nothing is left to join.
+template <int FMT, int NB, int HP, int WAVES, bool WHOLE>
+__global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? paged_occupancy(32 * NB) : WAVES / 4) void paged_attention_kernel(PagedAttnParams a) {
     using S = Step<FMT, NB, HP>;
+    constexpr uint32_t kThreads = WAVES * kWave;
     constexpr int kTiles = S::kTiles;
     constexpr bool kQuantised = FMT == kKvQ8_0 || FMT == kKvQ4_0;
     constexpr uint32_t kKeys = paged_keys(FMT), kDims = 32 * NB, kPitch = kDims + 4;
@@ -630,63 +633,80 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
     // queries in the products' order; at the end the wavefronts' sums
     __shared__ union Room {
         uint8_t queries[S::kQueryBytes * (kQuantised ? 2 : 1)];
-        float sums[kPagedAttnWaves][HP][kPitch];
+        float sums[WAVES][HP][kPitch];
     } room;
-    __shared__ float2 room_ml[kPagedAttnWaves][HP];
+    __shared__ float2 room_ml[WAVES][HP];
     __shared__ float room_unscale[kPagedHeads];
-    __shared__ uint32_t room_units[kPagedAttnWaves];
+    __shared__ uint32_t room_units[WAVES];
     __shared__ uint32_t found_before, found_seq;
     const uint32_t lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
     const uint32_t wave = uniform_u32(threadIdx.x / kWave);
     const uint64_t rows = static_cast<uint64_t>(a.kv_heads) * a.head_tiles;  // of a sequence
 
-    // this workgroup's units of all sequences'; those of a chunk of sequences, one a thread, up to each
-    const auto scan = [&](uint32_t units, uint32_t& chunk) {
-        uint32_t upto = wave_inclusive_scan_u32(units);
-        __syncthreads();
-        if (lane == kWave - 1) room_units[wave] = upto;
-        __syncthreads();
-        chunk = 0;
+    uint64_t begin, end, before = 0, total = 0, parts = 0;
+    uint32_t seq;
+    if constexpr (WHOLE) {
+        seq = static_cast<uint32_t>(blockIdx.x / rows);
+        const uint32_t units = uniform_u32(units_of(seen_of(a, seq), kKeys));
+        begin = blockIdx.x % rows * units;
+        end = begin + units;
+        if (units == 0) {
+            const uint32_t row = static_cast<uint32_t>(blockIdx.x % rows), head0 = row % a.head_tiles * kPagedHeads;
+            const uint32_t heads = min(a.group - head0, static_cast<uint32_t>(HP));
+            float* to = a.output + (static_cast<uint64_t>(seq) * a.q_heads + row / a.head_tiles * a.group + head0) * a.head_dim;
+            for (uint32_t i = threadIdx.x; i < heads * a.head_dim; i += kThreads) to[i] = 0.0f;
+            return;
+        }
+    } else {
+        // this workgroup's units of all sequences'; those of a chunk of sequences, one a thread, up to each
+        const auto scan = [&](uint32_t units, uint32_t& chunk) {
+            uint32_t upto = wave_inclusive_scan_u32(units);
+            __syncthreads();
+            if (lane == kWave - 1) room_units[wave] = upto;
+            __syncthreads();
+            chunk = 0;
 #pragma unroll
-        for (uint32_t w = 0; w < kPagedAttnWaves; ++w) {
-            if (w == wave) upto += chunk;
-            chunk += room_units[w];
+            for (uint32_t w = 0; w < WAVES; ++w) {
+                if (w == wave) upto += chunk;
+                chunk += room_units[w];
+            }
+            return upto;
+        };
+        uint32_t mine = 0, first_units = 0;
+        for (uint32_t b = threadIdx.x; b < a.sequences; b += kThreads) {
+            const uint32_t units = units_of(seen_of(a, b), kKeys);
+            if (b < kThreads) first_units = units;
+            mine += units;
         }
-        return upto;
-    };
-    uint32_t mine = 0, first_units = 0;
-    for (uint32_t b = threadIdx.x; b < a.sequences; b += kPagedAttnThreads) {
-        const uint32_t units = units_of(seen_of(a, b), kKeys);
-        if (b < kPagedAttnThreads) first_units = units;
-        mine += units;
+        uint32_t all_units;
+        uint32_t upto = scan(mine, all_units);
+        total = uniform_u32(all_units) * rows;
+        parts = parts_of(a, total);
+        if (blockIdx.x >= parts) return;
+        begin = uniform_u64(total * blockIdx.x / parts);
+        end = uniform_u64(total * (blockIdx.x + 1) / parts);
+        // the sequence that `begin` lies in
+        const uint32_t wanted = static_cast<uint32_t>(begin / rows);
+        uint32_t ahead = 0;
+        for (uint32_t first = 0; first < a.sequences; first += kThreads) {
+            const uint32_t b = first + threadIdx.x;
+            uint32_t units = first_units, chunk = all_units;
+            if (a.sequences > kThreads) {
+                if (first) units = b < a.sequences ? units_of(seen_of(a, b), kKeys) : 0u;
+                upto = scan(units, chunk);
+            }
+            const uint32_t from = ahead + upto - units;
+            if (wanted >= from && wanted - from < units) {
+                found_before = from;
+                found_seq = b;
+            }
+            ahead += chunk;
+            if (ahead > wanted) break;
+        }
+        __syncthreads();
+        before = uniform_u32(found_before) * rows;
+        seq = uniform_u32(found_seq);
     }
-    uint32_t all_units;
-    uint32_t upto = scan(mine, all_units);
-    const uint64_t total = uniform_u32(all_units) * rows;
-    const uint64_t parts = parts_of(a, total);
-    if (blockIdx.x >= parts) return;
-    const uint64_t begin = uniform_u64(total * blockIdx.x / parts), end = uniform_u64(total * (blockIdx.x + 1) / parts);
-    // the sequence that `begin` lies in
-    const uint32_t wanted = static_cast<uint32_t>(begin / rows);
-    uint32_t ahead = 0;
-    for (uint32_t first = 0; first < a.sequences; first += kPagedAttnThreads) {
-        const uint32_t b = first + threadIdx.x;
-        uint32_t units = first_units, chunk = all_units;
-        if (a.sequences > kPagedAttnThreads) {
-            if (first) units = b < a.sequences ? units_of(seen_of(a, b), kKeys) : 0u;
-            upto = scan(units, chunk);
-        }
-        const uint32_t from = ahead + upto - units;
-        if (wanted >= from && wanted - from < units) {
-            found_before = from;
-            found_seq = b;
-        }
-        ahead += chunk;
-        if (ahead > wanted) break;
-    }
-    __syncthreads();
-    uint64_t before = uniform_u32(found_before) * rows;
-    uint32_t seq = uniform_u32(found_seq);
 
     for (uint64_t at = begin; at < end;) {
         // a segment: units [t0, t1) of a row's `units`
@@ -703,7 +723,7 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
         const uint32_t row = uniform_u32(static_cast<uint32_t>((at - before) / units));
         const uint32_t t0 = uniform_u32(static_cast<uint32_t>((at - before) - static_cast<uint64_t>(row) * units));
         const uint32_t t1 = uniform_u32(end - at < units - t0 ? t0 + static_cast<uint32_t>(end - at) : units);
-        if (t0 == 0 && threadIdx.x == 0)  // unit u is part ((u + 1) parts - 1) / total's
+        if (!WHOLE && t0 == 0 && threadIdx.x == 0)  // unit u is part ((u + 1) parts - 1) / total's
             a.rows[seq * rows + row] = {blockIdx.x, static_cast<uint32_t>(((at + units) * parts - 1) / total)};
         at += t1 - t0;
         const uint32_t kv_head = row / a.head_tiles, head0 = row % a.head_tiles * kPagedHeads;
@@ -717,7 +737,7 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
         uint32_t pages = 0, pages_from = tw;
         const auto look_up = [&](uint32_t t) {
             pages_from = t;
-            const uint32_t entry = (start + (t + lane / kTiles * kPagedAttnWaves) * kKeys + lane % kTiles * 16) >> a.page_shift;
+            const uint32_t entry = (start + (t + lane / kTiles * WAVES) * kKeys + lane % kTiles * 16) >> a.page_shift;
             pages = entry < a.table_width ? table[entry] : 0xffffffffu;
             // waited for here, and not by whoever reads it: that wait would be for every load of every step
             asm volatile("" : "+v"(pages));
@@ -743,16 +763,16 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
         };
         // the pages of unit t; none where nothing is seen, which loads nothing
         const auto turn = [&](uint32_t t) {
-            if (t < t1 && t - pages_from >= kAhead * kPagedAttnWaves) look_up(t);
+            if (t < t1 && t - pages_from >= kAhead * WAVES) look_up(t);
 #pragma unroll
             for (uint32_t i = 0; i < kTiles; ++i) {
                 const uint32_t key = start + t * kKeys + 16 * i;
                 const bool some = t < t1 && key < seen.hi && key + 16 > seen.lo;
-                page[i] = some ? readlane_u32(pages, (t - pages_from) / kPagedAttnWaves * kTiles + i) : 0xffffffffu;
+                page[i] = some ? readlane_u32(pages, (t - pages_from) / WAVES * kTiles + i) : 0xffffffffu;
             }
         };
         // the query's loads, the step's behind them, and then what is done with the query
-        const uint32_t head = threadIdx.x / 16, sub = threadIdx.x % 16, real = head % HP;
+        const uint32_t head = threadIdx.x / 16 % 16, sub = threadIdx.x % 16, real = head % HP;  // by the first four wavefronts
         constexpr int kEach = FMT == kKvF32 ? 4 : 8, kItems = (kDims / kEach + 15) / 16;
         f32x4 x[kItems][kEach / 4];
         {
@@ -770,7 +790,7 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
         load(tw, true);
         load(tw, false);
         __syncthreads();  // the last segment's sums have been read
-        {
+        if (WAVES == 4 || wave < 4) {
             float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < kItems; ++i)
@@ -801,7 +821,7 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
                 if (sub == 0) room_unscale[head] = pow2i(-up);
                 constexpr uint32_t kSlots = kQuantised ? S::kQueryBytes / 16 : 0;
                 if constexpr (kQuantised) {
-                    for (uint32_t i = threadIdx.x; i < kSlots; i += kPagedAttnThreads)
+                    for (uint32_t i = threadIdx.x; i < kSlots; i += 4 * kWave)
                         reinterpret_cast<u32x4_t*>(room.queries)[kSlots + i] = u32x4_t{0, 0, 0, 0};
                 }
                 constexpr uint32_t kLines = S::kHeadLines, kLast = S::kItemsPadded;
@@ -829,7 +849,7 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
         f32x4 out[S::kOut];
 #pragma unroll
         for (int i = 0; i < S::kOut; ++i) out[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t t = tw; t < t1; t += kPagedAttnWaves) {
+        for (uint32_t t = tw; t < t1; t += WAVES) {
             const uint32_t key0 = start + t * kKeys;
             bool there[kTiles], whole = key0 >= seen.lo && key0 + kKeys <= seen.hi;
 #pragma unroll
@@ -839,8 +859,8 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
             }
             f32x4 s[kTiles];
             step.scores(queries, c, unscale, s);
-            turn(t + kPagedAttnWaves);
-            load(t + kPagedAttnWaves, true);
+            turn(t + WAVES);
+            load(t + WAVES, true);
             __builtin_amdgcn_sched_barrier(0);
             if (!whole) {
                 bool sees[kTiles][4];
@@ -877,7 +897,7 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
             l += kTiles == 1 ? sum[0] : sum[0] + sum[kTiles - 1];
             step.add(s, out);
             __builtin_amdgcn_sched_barrier(0);
-            load(t + kPagedAttnWaves, false);
+            load(t + WAVES, false);
         }
 
         // join the wavefronts
@@ -891,15 +911,15 @@ __global__ __launch_bounds__(kPagedAttnThreads, paged_occupancy(32 * NB)) void p
         const bool all = t0 == 0 && t1 == units;
         const uint64_t slot = 2ull * blockIdx.x + (t0 == 0 ? 1 : 0);
         constexpr uint32_t kQuads = kDims / 4;
-        for (uint32_t i = threadIdx.x; i < heads * kQuads; i += kPagedAttnThreads) {
+        for (uint32_t i = threadIdx.x; i < heads * kQuads; i += kThreads) {
             const uint32_t r = i / kQuads, quad = i % kQuads;
             if (4 * quad >= a.head_dim) continue;
             float top = neg_inf(), sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kPagedAttnWaves; ++w) top = fmaxf(top, room_ml[w][r].x);
+            for (int w = 0; w < WAVES; ++w) top = fmaxf(top, room_ml[w][r].x);
             f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < kPagedAttnWaves; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 const float2 ml = room_ml[w][r];
                 const float f = ml.x == neg_inf() ? 0.0f : __builtin_amdgcn_exp2f(ml.x - top);
                 sum += f * ml.y;
@@ -923,9 +943,20 @@ hipError_t launch_paged_attention_f16(hipStream_t stream, const PagedAttnParams&
 hipError_t launch_paged_attention_q8_0(hipStream_t stream, const PagedAttnParams& a);
 hipError_t launch_paged_attention_q4_0(hipStream_t stream, const PagedAttnParams& a);
 
+// Wavefronts of a workgroup that takes a whole row of more than two steps for four.
+template <int NB>
+inline constexpr int kPagedRowWaves = NB <= 2 ? 16 : 8;
+
 template <int FMT, int NB, int HP>
 hipError_t launch_paged_heads(hipStream_t stream, const PagedAttnParams& a) {
-    hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP>), dim3(a.most_parts), dim3(kPagedAttnThreads), 0, stream, a);
+    const uint32_t rows = a.sequences * a.kv_heads * a.head_tiles;
+    if (a.row_units == 0)
+        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, 4, false>), dim3(a.most_parts), dim3(4 * kWave), 0, stream, a);
+    else if (a.row_units <= 8)
+        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, 4, true>), dim3(rows), dim3(4 * kWave), 0, stream, a);
+    else
+        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, kPagedRowWaves<NB>, true>), dim3(rows),
+                           dim3(kPagedRowWaves<NB> * kWave), 0, stream, a);
     return hipGetLastError();
 }
 template <int FMT, int NB>

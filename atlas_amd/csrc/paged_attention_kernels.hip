@@ -82,6 +82,8 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnParams a) 
     *reinterpret_cast<f32x4*>(out) = y;
 }
 
+constexpr uint32_t kJoinThreads = 256;
+
 // Additions to a wavefront's sums in a part, a unit each: with keys alike they all round to
 // one side, 2^-25 of the sum at most each.
 constexpr uint32_t kPartUnits = 256 * kPagedAttnWaves;
@@ -112,6 +114,27 @@ PagedPlan paged_plan(const PagedCache& c, uint32_t q_heads) {
     p.ml_bytes = round256(lines * 8);
     p.row_bytes = round256(rows * sizeof(PagedRow));
     return p;
+}
+
+// The units that a row has at most, where a workgroup a row is sooner done than
+// parts and their join; 0 where it is not.  Both by what was measured, in KB and us:
+// a workgroup takes 48 KB/us, or its share of the chip's 5500; parts have the whole
+// chip whatever the rows, but cost 4 us more with the join, and 8 more where they are
+// small and many.  Whole / parts, us: 256 windows of 512 f16 (256 dims) 33 / 52, f32 65
+// / 81, Q8_0 22 / 38; 64 of them f16 24 / 30; 2048 rows of up to 500 f16 (128 dims) 88 /
+// 114; 2000 of up to 100 Q8_0 (64) 15 / 39; 64 rows of up to 1024 f16 (128) 17 / 21, of
+// 4096 49 / 31; one of 64 f32 (128) 6 / 10; 3 of 2048 f32 (64) 25 / 11; one of 1024 Q8_0
+// (256) 24 / 13.  Long rows end at different times and are always split.
+uint32_t whole_row_units(const PagedCache& c, uint32_t window, uint64_t rows) {
+    const uint32_t unit = paged_keys(c.format);
+    uint64_t positions = static_cast<uint64_t>(c.table_width) * c.page_size;
+    if (window && window < positions) positions = window + unit;  // it may begin and end inside units
+    const double row_kb = 2e-3 * positions * paged_part_bytes(c.format, c.page_size, c.head_dim) / c.page_size;
+    if (row_kb > 1500.0) return 0;
+    const double busy = rows < 256 ? static_cast<double>(rows) : 256.0, share = 5500.0 / busy;
+    const double whole = static_cast<double>((rows + 255) / 256) * row_kb / (share < 48.0 ? share : 48.0);
+    const double parts = 4.0 + 8.0 * (rows < 64 ? rows / 64.0 : 1.0) + rows * row_kb / 5500.0;
+    return whole < parts ? static_cast<uint32_t>((positions + unit - 1) / unit) : 0;
 }
 
 }  // namespace
@@ -150,6 +173,7 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
     a.few_parts = p.few_parts;
     a.most_parts = p.most_parts;
     a.part_units = kPartUnits;
+    a.row_units = whole_row_units(c, s.window, c.sequences * c.kv_heads * a.head_tiles);
     a.scale = s.scale * kLog2e;
     hipError_t e;
     switch (c.format) {
@@ -158,20 +182,20 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
         case kKvQ8_0: e = launch_paged_attention_q8_0(stream, a); break;
         default: e = launch_paged_attention_q4_0(stream, a); break;
     }
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || a.row_units) return e;
     const uint32_t lines = c.sequences * s.q_heads;
     // Few rows have many parts: a workgroup for every 64 dims of one, and of 16 wavefronts.
     if (lines < 512) {
         hipLaunchKernelGGL((paged_join_kernel<16, 1024>), dim3(lines, (c.head_dim + 63) / 64), dim3(1024), 0, stream, a);
         return hipGetLastError();
     }
-    const dim3 grid(lines), block(kPagedAttnThreads);
+    const dim3 grid(lines), block(kJoinThreads);
     if (c.head_dim <= 64)
-        hipLaunchKernelGGL((paged_join_kernel<16, kPagedAttnThreads>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((paged_join_kernel<16, kJoinThreads>), grid, block, 0, stream, a);
     else if (c.head_dim <= 128)
-        hipLaunchKernelGGL((paged_join_kernel<32, kPagedAttnThreads>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((paged_join_kernel<32, kJoinThreads>), grid, block, 0, stream, a);
     else
-        hipLaunchKernelGGL((paged_join_kernel<64, kPagedAttnThreads>), grid, block, 0, stream, a);
+        hipLaunchKernelGGL((paged_join_kernel<64, kJoinThreads>), grid, block, 0, stream, a);
     return hipGetLastError();
 }
 

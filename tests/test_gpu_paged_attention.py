@@ -286,6 +286,46 @@ def test_refusals(rt):
     rt.sync()
 
 
+def spread(seed, fmt, H, KH, D, ps, width, lengths):
+    """Tables of `width` entries, of which the lengths need the first."""
+    r = np.random.default_rng(seed)
+    need = [-(-n // ps) for n in lengths]
+    pool = ref.Pool(fmt, sum(need) + 2, ps, KH, D).random(r)
+    order = iter(r.permutation(len(pool.bytes)))
+    table = np.full((len(lengths), width), ref.NO, u32)
+    for b, n in enumerate(need):
+        table[b, :n] = [next(order) for _ in range(n)]
+    return pool, table, (r.standard_normal((len(lengths), H, D)) * 2).astype(f32), np.asarray(lengths, u32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", range(32, 257, 32))
+@pytest.mark.parametrize("how", ["split", "whole", "short"])
+def test_rows_split_and_whole(rt, fmt, D, how):
+    """Rows that may be long are split over workgroups and joined; many of some length, and short ones, are not.  Of 3, 8 and
+    more than 16 query heads to a KV head, in each of the products' widths."""
+    for group, KH in ((3, 2), (8, 1), (19, 1)):
+        if how == "split":
+            args = spread(D + group, fmt, group * KH, KH, D, 64, 800, [700, 33, 0, 129])
+        elif how == "whole":
+            args = spread(D + group, fmt, group * KH, KH, D, 16, 20, [(53 * i) % 321 for i in range(80 // KH)])
+        else:
+            args = spread(D + group, fmt, group * KH, KH, D, 16, 7, [112, 0, 17, 1, 64])
+        for window in (0, 37) if how == "short" else (0,):
+            say(f"{how} {fmt} {D} group {group} window {window}")
+            got = run(rt, fmt, *args, window, D ** -0.5)
+            assert (got[args[3] == 0] == 0).all()
+            check(f"{how} {fmt} {D}", fmt, *args, window, D ** -0.5, got)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_windows_of_many_rows(rt, fmt):
+    """A window bounds a row where the capacity does not: such rows are whole."""
+    args = spread(3, fmt, 8, 2, 128, 16, 4000, [(211 * i) % 2001 for i in range(40)])
+    got = run(rt, fmt, *args, 200, 0.09)
+    check(f"{fmt}", fmt, *args, 200, 0.09, got)
+
+
 def test_two_graphs_with_a_workspace_each():
     """Recorded calls of two contexts replayed together, with other lengths and tables from replay to replay."""
     rts = [HipRuntime(0), HipRuntime(0)]

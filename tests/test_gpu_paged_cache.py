@@ -229,6 +229,37 @@ def test_rows_behind_four_gigabytes(rt):
     rt.free(dp)
 
 
+@pytest.mark.parametrize("fmt", ["f32", "q4_0"])
+def test_more_rows_than_the_caches_hold(rt, fmt):
+    """Rotated queries of 39 MB in a call, and rows of 39 MB read back: the same as a few."""
+    r = np.random.default_rng(4)
+    KH, D, H, T = 1, 64, 16, 9500
+    pool = ref.Pool(fmt, 20, 1024, KH, D)
+    table = make_table(r, 2, 5, 20)
+    table[1, 2] = ref.NO
+    cos, sin = angles(r, 5120, D)
+    ids, positions = np.repeat(np.arange(2, dtype=u32), T // 2), np.tile(np.arange(T // 2, dtype=u32), 2)
+    key, value = r.standard_normal((2, T, KH, D)).astype(f32)
+    query = r.standard_normal((T, H, D)).astype(f32)
+    got, q, q_exp = run_append(rt, fmt, pool, table, key, value, query, cos, sin, ids, positions)
+    same("queries", q.view(u32), q_exp.view(u32))
+    same("pool", got, pool.bytes)
+
+    dp, dt, cache = device(rt, fmt, pool, table)
+    n = 76000
+    ids, positions = r.integers(0, 2, n).astype(u32), r.integers(0, 5120, n).astype(u32)
+    di, dn, k, v = rt.upload(ids), rt.upload(positions), rt.empty(n * D), rt.empty(n * D)
+    rt.paged_read(cache, di, dn, n, k, v)
+    rt.sync()
+    held = np.stack([np.concatenate([pool.values(int(p), plane, 0) if p != ref.NO else np.zeros((1024, D)) for p in table.reshape(-1)])
+                     for plane in range(2)]).astype(f32)
+    rows = ids.astype(np.int64) * 5120 + positions
+    same("keys", k.download().reshape(n, D), held[0, rows])
+    same("values", v.download().reshape(n, D), held[1, rows])
+    for b in (dp, dt, di, dn, k, v):
+        rt.free(b)
+
+
 def test_refusals(rt):
     pool = ref.Pool("f32", 2, 16, 1, 64)
     dp, dt, cache = device(rt, "f32", pool, np.zeros((2, 1), u32))

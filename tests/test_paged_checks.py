@@ -11,6 +11,7 @@ import numpy as np
 import pytest
 
 import paged_refs as ref
+from atlas_amd.chains import PagedDecode
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 U32, U64 = c_uint32, c_uint64
@@ -107,6 +108,7 @@ def test_read_calls(checks, change, fine):
     (dict(q_heads=7), False), (dict(scale=math.nan), False), (dict(scale=math.inf), False), (dict(q=3 * M + 4), False),
     (dict(output=5 * M + 8), False), (dict(workspace=6 * M + 8), False), (dict(lengths=4 * M + 2), False), (dict(output=3 * M), False),
     (dict(output=M + 16), False), (dict(sequences=1 << 20, q_heads=10), False),
+    (dict(sequences=1 << 20, table_width=2048), True), (dict(sequences=1 << 20, table_width=2049), False),
 ])
 def test_attention_calls(checks, change, fine):
     assert (call(checks.check_attention, ATTEND, change) is None) == fine
@@ -145,3 +147,34 @@ def test_a_values_codes_are_where_the_layout_says(checks, D):
     place = np.argsort(order)
     for d in range(0, D, 2):
         assert checks.value_place(D, d) == place[d] and place[d + 1] == place[d] + 1
+
+
+def test_a_failed_recording_leaves_no_graph_behind():
+    """PagedDecode keeps no handle of the graph that a failed recording destroyed."""
+    class Runtime:
+        live, next = set(), 1
+
+        def graph_begin(self):
+            pass
+
+        def graph_end(self):
+            self.next += 1
+            self.live.add(self.next)
+            return self.next
+
+        def graph_destroy(self, graph):
+            self.live.remove(graph)  # KeyError: destroyed twice
+
+    chain = object.__new__(PagedDecode)
+    chain.rt, chain.graph = Runtime(), None
+    chain.enqueue = lambda: None
+    first = chain.capture()
+    assert chain.graph == first and chain.rt.live == {first}
+
+    def fails():
+        raise ValueError("no")
+
+    chain.enqueue = fails
+    with pytest.raises(ValueError, match="no"):
+        chain.capture()
+    assert chain.graph is None and not chain.rt.live
