@@ -245,7 +245,7 @@ template <int NB>
 struct Step<kKvF16, NB, 16> {
     static constexpr int kTiles = 2, kOut = 2 * NB, kQuads = NB / 2, kQueryBytes = 2 * NB * kWave * 16;
     static constexpr float kUnscale = 0x1p-15f;
-    static constexpr uint32_t kHeadLines = kPagedHeads, kItemsPadded = 4 * NB;
+    static constexpr uint32_t kItemsPadded = 4 * NB;
     u32x4_t k[2][NB];
     u32x2_t v[8][kQuads ? kQuads : 1];
     uint32_t v2[8];
@@ -354,13 +354,16 @@ struct Step<kKvF16, NB, 16> {
 // scale goes on the product of its block, a value's on the weight, so codes are
 // only unpacked.
 //
-// A product has 16 columns and a row HP heads at most (4, 8 or 16): columns are
-// (block, head), not heads alone.  For the keys that lets a lane load 16 bytes of its
-// row at once, though they are another block than its neighbours': a column takes
-// one block (its query is zero for the others'), and one scale goes on its result.
-// (Loads of 8 or 4 bytes a lane, rows apart, keep the address unit busy for 64
-// cycles whatever they bring: 4.7 and 2.4 TB/s of the 6.2 that 16 bytes reach.)  For
-// the values a lane cuts the weights of one block in 16 / HP, not of all.
+// A lane loads 16 bytes of a key at once: loads of 8 or 4 bytes a lane, rows apart,
+// keep the address unit busy for 64 cycles whatever they bring (4.7 and 2.4 TB/s of
+// the 6.2 that 16 bytes reach).  They are another block than its neighbours'.  So
+// lanes exchange words until a product has one block's dims, whose scale goes on the
+// result; or, of Q8_0's two blocks and 8 heads at most, each column takes one (its
+// query is zero for the other's), with twice the products and half the scales (256
+// dims, 8 heads: 88 us for 95; Q4_0 the other way, 71 for 77).  A product has 16
+// columns and a row HP heads at most (4, 8 or 16): for the keys columns are (piece of
+// the query or block, head), for the values (block, head), so that a lane cuts the
+// weights of one block in 16 / HP, not of all.
 template <int FMT, int NB, int HP>
 struct Step {
     static_assert(FMT == kKvQ8_0 || FMT == kKvQ4_0);
@@ -369,46 +372,35 @@ struct Step {
     static constexpr ValueWords<NB, kBlock> kWords{};
     // v_cvt_off_f32_i4 gives sixteenths
     static constexpr float kUnscale = kBytes ? 1.0f : 16.0f;
-    // keys: blocks to the columns, heads to a product, products for all heads; steps of kKeyBlocks blocks; chunks of
-    // 8 dims of a lane's 16 bytes
-    static constexpr int kKeyBlocks = kBytes ? 2 : 4, kKeyHeads = 16 / kKeyBlocks, kSets = HP > kKeyHeads ? HP / kKeyHeads : 1;
-    static constexpr int kKeySteps = (NB + kKeyBlocks - 1) / kKeyBlocks, kChunks = kBytes ? 2 : 4;
+    // keys: blocks of the 64 bytes that lanes g load at once, and of a product; products that the query's pieces make;
+    // in LDS a query's 64 lanes for each product
+    static constexpr int kKeyBlocks = kBytes ? 2 : 4, kKeySteps = (NB + kKeyBlocks - 1) / kKeyBlocks;
+    static constexpr bool kExchanged = !kBytes || HP == 16;
+    static constexpr int kSpan = kExchanged ? 1 : 2, kSpans = (NB + kSpan - 1) / kSpan, kPieces = kExchanged && HP < 16 ? 1 : 2;
     // values: blocks to the columns
     static constexpr int kValueBlocks = 16 / HP, kValueSteps = (NB + kValueBlocks - 1) / kValueBlocks;
-    // queries in LDS: for each step, chunk, piece and set, the lanes that are not zero; then as much of zeros
-    static constexpr int kQueryLanes = 64 / kKeyBlocks, kQueries = kKeySteps * kChunks * 2 * kSets;
-    static constexpr int kQueryBytes = kQueries * kQueryLanes * 16;
-    static constexpr uint32_t kHeadLines = kSets * kKeyHeads, kItemsPadded = 4 * kKeySteps * kKeyBlocks;
+    static constexpr int kQueryBytes = kSpans * kSpan * kPieces * 1024;
+    static constexpr uint32_t kItemsPadded = 4 * kSpans * kSpan;
 
     u32x4_t k[2][kKeySteps];
-    u32x2_t ks[2][kKeySteps], vs[2][kValueSteps];  // scales of keys 4 g + r
+    u32x2_t ks[2][kSpans], vs[2][kValueSteps];  // scales of keys 4 g + r
     uint32_t v[8][kWords.words];
 
-    static __device__ __forceinline__ uint32_t key_block(uint32_t c) { return c / kKeyHeads; }
-    static __device__ __forceinline__ uint32_t query_at(int i, int m, int piece, int set) {
-        return (((i * kChunks + m) * 2 + piece) * kSets + set) * kQueryLanes * 16;
-    }
-    // Where a lane reads its query: block key_block(c) of a step is in lanes g (Q4_0) or 2 g, 2 g + 1 (Q8_0).
-    static __device__ __forceinline__ uint32_t query_lane(uint32_t c, uint32_t g) {
-        const bool mine = (kBytes ? g / 2 : g) == key_block(c);
-        return mine ? (c % kKeyHeads + kKeyHeads * g) * 16 : kQueryBytes;
-    }
-    // Item `it` of a head's query, 8 dims of block it / 4.
+    static __device__ __forceinline__ uint32_t query_lane(uint32_t c, uint32_t g) { return (c + 16 * g) * 16; }
+    // Item `it` of a head's query, 8 dims of block it / 4, for the lane that has their codes.
     static __device__ __forceinline__ void put_query(uint8_t* room, uint32_t head, uint32_t it, f16x8_t hi, f16x8_t lo) {
-        const uint32_t block = it / 4, i = block / kKeyBlocks, set = head / kKeyHeads, h = head % kKeyHeads;
-        const uint32_t m = kBytes ? it % 2 : it % 4, g = kBytes ? block % 2 * 2 + it % 4 / 2 : block % 4;
-        uint8_t* to = room + query_at(i, m, 0, set) + (h + kKeyHeads * g) * 16;
-        *reinterpret_cast<f16x8_t*>(to) = hi;
-        *reinterpret_cast<f16x8_t*>(to + query_at(0, 0, 1, 0)) = lo;
-    }
-    template <int STEPS>
-    static __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rs, uint32_t page_shift, uint32_t row, uint32_t g,
-                                                       uint32_t block, int blocks, u32x2_t (&s)[STEPS]) {
-        const uint32_t base = (kRow << page_shift) + row / 4 * NB * 8, off = g * NB * 8 + block * 8;
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-            const bool there = (i + 1) * blocks <= NB || block + i * blocks < NB;
-            s[i] = load8(rs, there ? off + i * blocks * 8 : kPastPage, base);
+        const uint32_t block = it / 4, quarter = it % 4;
+        f16x8_t* to = reinterpret_cast<f16x8_t*>(room);
+        if constexpr (kExchanged) {
+            to += block * kPieces * 64 + (kBytes ? quarter % 2 * 2 + quarter / 2 : quarter) * 16 + head;
+            *to = HP < 16 && head / HP % 2 ? lo : hi;
+            if constexpr (HP == 16) to[64] = lo;
+        } else if (head < 8) {
+            to += (block / 2 * 2 + quarter % 2) * 128 + (block % 2 * 2 + quarter / 2) * 16 + head;
+            const uint32_t mine = block % 2 * 8, others = 8 - mine;
+            to[mine] = hi;
+            to[mine + 64] = lo;
+            to[others] = to[others + 64] = f16x8_t{};
         }
     }
     __device__ __forceinline__ void load_keys(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t page_shift) {
@@ -420,7 +412,22 @@ struct Step {
                 const uint32_t off = (i + 1) * 64 <= kRow || in_row < kRow ? c * kRow + in_row : kPastPage;
                 k[h][i] = load16(p[h].keys, off, p[h].row * kRow);
             }
-            load_scales(p[h].keys, page_shift, p[h].row, g, key_block(c), kKeyBlocks, ks[h]);
+            const uint32_t base = (kRow << page_shift) + p[h].row / 4 * NB * 8, off = g * NB * 8;
+            if constexpr (kExchanged) {
+#pragma unroll
+                for (int b = 0; b + 1 < NB; b += 2) {
+                    const u32x4_t x = load16(p[h].keys, off + 8 * b, base);
+                    ks[h][b] = u32x2_t{x[0], x[1]};
+                    ks[h][b + 1] = u32x2_t{x[2], x[3]};
+                }
+                if constexpr (NB % 2) ks[h][NB - 1] = load8(p[h].keys, off + 8 * (NB - 1), base);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kSpans; ++i) {
+                    const uint32_t b = 2 * i + c / 8;
+                    ks[h][i] = load8(p[h].keys, 2 * (i + 1) <= NB || b < NB ? off + 8 * b : kPastPage, base);
+                }
+            }
         }
     }
     __device__ __forceinline__ void load_values(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t page_shift) {
@@ -451,7 +458,14 @@ struct Step {
             }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) load_scales(p[h].values, page_shift, p[h].row, g, c / HP, kValueBlocks, vs[h]);
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t base = (kRow << page_shift) + p[h].row / 4 * NB * 8, block = c / HP;
+#pragma unroll
+            for (int i = 0; i < kValueSteps; ++i) {
+                const bool there = (i + 1) * kValueBlocks <= NB || block + i * kValueBlocks < NB;
+                vs[h][i] = load8(p[h].values, there ? (g * NB + block + i * kValueBlocks) * 8 : kPastPage, base);
+            }
+        }
     }
     // Eight codes of a key as f16: 1024 + (a code without its sign) has it in its low
     // bits, or 16 times it four bits higher up.  Written out where the compiler makes
@@ -461,7 +475,7 @@ struct Step {
         asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(y) : "v"(x), "s"(mask), "v"(bits));
         return y;
     }
-    static __device__ __forceinline__ f16x8_t key_codes(u32x4_t w, int m) {
+    static __device__ __forceinline__ f16x8_t key_codes(u32x2_t w) {
         u32x4_t x;
         const auto less = [](uint32_t y, float by) {
             const f16x2_t z = {static_cast<_Float16>(by), static_cast<_Float16>(by)};
@@ -470,13 +484,13 @@ struct Step {
         if constexpr (kBytes) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                x[i] = less(__builtin_amdgcn_perm(0x64646464u, w[2 * m + i / 2] ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u), 1152.0f);
+                x[i] = less(__builtin_amdgcn_perm(0x64646464u, w[i / 2] ^ 0x80808080u, i % 2 ? 0x04030402u : 0x04010400u), 1152.0f);
         } else {
             const f16x2_t sixteenth = {static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
             const f16x2_t minus72 = {static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-                const uint32_t y = i ? w[m] >> 8 : w[m];
+                const uint32_t y = i ? w[0] >> 8 : w[0];
                 x[i] = less(and_or(y, 0x000f000fu, 0x64006400u), 1032.0f);
                 // (1024 + 16 n) / 16 - 72 = n - 8
                 x[i + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(f16x2_t, and_or(y, 0x00f000f0u, 0x64006400u)),
@@ -486,50 +500,66 @@ struct Step {
         return __builtin_bit_cast(f16x8_t, x);
     }
     static __device__ __forceinline__ float scale_of(u32x2_t s, int r) { return h2f(static_cast<uint16_t>(s[r / 2] >> (16 * (r % 2)))); }
-    __device__ __forceinline__ void scores(const uint8_t* queries, uint32_t c, float unscale, f32x4 (&s)[2]) const {
-        f32x4 sum[kSets][2];
-#pragma unroll
-        for (int set = 0; set < kSets; ++set) sum[set][0] = sum[set][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // Words i, j of lanes g and of lanes g ^ 2 or g ^ 1 change places where they are off the diagonal.
+    static __device__ __forceinline__ void exchange32(u32x4_t& w, int i, int j) {
+        const auto p = __builtin_amdgcn_permlane32_swap(w[i], w[j], false, false);
+        w[i] = p[0];
+        w[j] = p[1];
+    }
+    static __device__ __forceinline__ void exchange16(u32x4_t& w, int i, int j) {
+        const auto p = __builtin_amdgcn_permlane16_swap(w[i], w[j], false, false);
+        w[i] = p[0];
+        w[j] = p[1];
+    }
+    // From a lane's 16 bytes of one block its eight dims of each: of Q4_0's block b in word b, the dims of word g; of
+    // Q8_0's in words 2 b and 2 b + 1, those of the half g % 2, quarter g / 2.
+    static __device__ __forceinline__ u32x4_t exchange(u32x4_t w) {
+        exchange32(w, 0, 2);
+        exchange32(w, 1, 3);
+        if constexpr (!kBytes) {
+            exchange16(w, 0, 1);
+            exchange16(w, 2, 3);
+        }
+        return w;
+    }
+    __device__ __forceinline__ void scores(const uint8_t* queries, uint32_t, float unscale, f32x4 (&s)[2]) const {
+        s[0] = s[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kKeySteps; ++i) {
-            f32x4 d[kSets][2];
+            const u32x4_t w[2] = {kExchanged ? exchange(k[0][i]) : k[0][i], kExchanged ? exchange(k[1][i]) : k[1][i]};
 #pragma unroll
-            for (int set = 0; set < kSets; ++set) d[set][0] = d[set][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = 0; j < kKeyBlocks / kSpan; ++j) {
+                const int b = i * kKeyBlocks / kSpan + j;
+                if (b >= kSpans) break;
+                f32x4 d[2] = {};
 #pragma unroll
-            for (int m = 0; m < kChunks; ++m) {
-                const f16x8_t x[2] = {key_codes(k[0][i], m), key_codes(k[1][i], m)};
+                for (int m = 0; m < kSpan; ++m) {
+                    f16x8_t x[2];
 #pragma unroll
-                for (int set = 0; set < kSets; ++set)
+                    for (int h = 0; h < 2; ++h)
+                        x[h] = key_codes(kBytes ? u32x2_t{w[h][2 * (j + m) % 4], w[h][(2 * (j + m) + 1) % 4]} : u32x2_t{w[h][j], 0});
 #pragma unroll
-                    for (int piece = 0; piece < 2; ++piece) {
-                        const f16x8_t q = *reinterpret_cast<const f16x8_t*>(queries + query_at(i, m, piece, set));
+                    for (int n = 0; n < kPieces; ++n) {
+                        const f16x8_t q = *reinterpret_cast<const f16x8_t*>(queries + ((b * kSpan + m) * kPieces + n) * 1024);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) d[set][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[h], q, d[set][h], 0, 0, 0);
+                        for (int h = 0; h < 2; ++h) d[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[h], q, d[h], 0, 0, 0);
                     }
-                if (m % 2) __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int set = 0; set < kSets; ++set)
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sum[set][h][r] = __builtin_fmaf(d[set][h][r], scale_of(ks[h][i], r), sum[set][h][r]);
+                    for (int r = 0; r < 4; ++r) s[h][r] = __builtin_fmaf(d[h][r], scale_of(ks[h][b], r), s[h][r]);
+                if (kSpan == 2 || j % 2) __builtin_amdgcn_sched_barrier(0);
+            }
         }
-        // a head's blocks from its columns; then every lane its own head, c % HP
+        // the sums of a head's columns; every lane has its own head, c % HP
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float x[kSets];
-#pragma unroll
-                for (int set = 0; set < kSets; ++set) {
-                    x[set] = sum[set][h][r] + dpp_f32<0x128, 0xf, false>(sum[set][h][r]);                    // row_ror:8
-                    if constexpr (!kBytes) x[set] = x[set] + dpp_f32<0x124, 0xf, false>(x[set]);  // row_ror:4
-                }
-                float y = x[0];
-                if constexpr (kSets == 2) y = c % HP >= kKeyHeads ? x[1] : x[0];
-                if constexpr (kSets == 4) y = c >= 8 ? (c >= 12 ? x[3] : x[2]) : (c >= 4 ? x[1] : x[0]);
-                s[h][r] = y * unscale;
+                if constexpr (HP == 8 || !kExchanged) s[h][r] += dpp_f32<0x128, 0xf, false>(s[h][r]);  // row_ror:8
+                else if constexpr (HP == 4) s[h][r] += dpp_f32<0x124, 0xf, false>(s[h][r]);            // row_ror:4
+                s[h][r] *= unscale;
             }
     }
     __device__ __forceinline__ void keep(const bool (&seen)[2][4]) {
@@ -632,7 +662,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? paged_occupancy(32 * NB
     static_assert(kKeys == 16 * kTiles);
     // queries in the products' order; at the end the wavefronts' sums
     __shared__ union Room {
-        uint8_t queries[S::kQueryBytes * (kQuantised ? 2 : 1)];
+        uint8_t queries[S::kQueryBytes];
         float sums[WAVES][HP][kPitch];
     } room;
     __shared__ float2 room_ml[WAVES][HP];
@@ -819,12 +849,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? paged_occupancy(32 * NB
                 if (top > 0.0f && top < __builtin_inff()) up = min(14 - __builtin_amdgcn_frexp_expf(top), 126);
                 const float by = pow2i(up);
                 if (sub == 0) room_unscale[head] = pow2i(-up);
-                constexpr uint32_t kSlots = kQuantised ? S::kQueryBytes / 16 : 0;
-                if constexpr (kQuantised) {
-                    for (uint32_t i = threadIdx.x; i < kSlots; i += 4 * kWave)
-                        reinterpret_cast<u32x4_t*>(room.queries)[kSlots + i] = u32x4_t{0, 0, 0, 0};
-                }
-                constexpr uint32_t kLines = S::kHeadLines, kLast = S::kItemsPadded;
+                constexpr uint32_t kLast = S::kItemsPadded;
 #pragma unroll
                 for (int i = 0; i < static_cast<int>((kLast + 15) / 16); ++i) {
                     const uint32_t item = sub + 16 * i;
@@ -837,7 +862,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? paged_occupancy(32 * NB
                         hi[j] = p;
                         lo[j] = r;
                     }
-                    if (item < kLast && head < kLines) S::put_query(room.queries, head, item, hi, lo);
+                    if (item < kLast) S::put_query(room.queries, head, item, hi, lo);
                 }
             }
         }

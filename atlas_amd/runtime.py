@@ -36,10 +36,10 @@ class OperatorError(RuntimeError):
 
 
 def _ptr(a) -> int:
+    if a is None or type(a) is int:  # first: small calls are bound by the host
+        return a
     if isinstance(a, DeviceBuffer):
         return a.ptr
-    if a is None:
-        return None
     if isinstance(a, int):
         return a
     return a.ctypes.data
