@@ -9,14 +9,14 @@ namespace {
 // One workgroup a query row, or 4 LANES dims of one: its parts joined, where
 // there is more than one, or zero where nothing was seen.  LANES lanes hold a
 // part's dims; as many parts as fit the workgroup are taken at once, and their
-// sums meet in LDS in the parts' order.  The loads' latency is its time: a
+// sums meet in the wavefront and then in LDS, in an order of their own.  The loads' latency is its time: a
 // group's first parts are on their way before the row's maximum is known.
 template <int LANES, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnParams a) {
     constexpr uint32_t kGroups = THREADS / LANES, kWaves = THREADS / kWave, kAtOnce = 4;
     __shared__ float wave_top[kWaves];
-    __shared__ f32x4 sums[kGroups][LANES];
-    __shared__ float group_l[kGroups];
+    __shared__ f32x4 sums[kWaves][LANES];
+    __shared__ float wave_l[kWaves];
     const uint32_t seq = blockIdx.x / a.q_heads, q_head = blockIdx.x % a.q_heads;
     const uint32_t kv_head = q_head / a.group, in_group = q_head % a.group;
     const PagedRow row = a.rows[(static_cast<uint64_t>(seq) * a.kv_heads + kv_head) * a.head_tiles + in_group / kPagedHeads];
@@ -65,15 +65,25 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnParams a) 
             for (int k = 0; k < 4; ++k) all_o[k] += static_cast<double>(f * part[j][k]);
         }
     }
-    sums[group][lane] = f32x4{static_cast<float>(all_o[0]), static_cast<float>(all_o[1]), static_cast<float>(all_o[2]),
-                              static_cast<float>(all_o[3])};
-    if (lane == 0) group_l[group] = static_cast<float>(all_l);
+    // the groups of a wavefront, then the wavefronts
+    const auto join = [&](double all) {
+        float x = static_cast<float>(all);
+        if constexpr (LANES <= 8) x += dpp_f32<0x128, 0xf, false>(x);  // row_ror:8
+        if constexpr (LANES <= 16) x = sum_xor16(x);
+        if constexpr (LANES <= 32) x = sum_xor32(x);
+        return x;
+    };
+    const f32x4 mine = {join(all_o[0]), join(all_o[1]), join(all_o[2]), join(all_o[3])};
+    const float mine_l = join(all_l);
+    if (threadIdx.x % kWave < LANES) sums[threadIdx.x / kWave][lane] = mine;
+    if (threadIdx.x % kWave == 0) wave_l[threadIdx.x / kWave] = mine_l;
     __syncthreads();
     if (group || !holds) return;
     float sum = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t i = 0; i < min(kGroups, count); ++i) {
-        sum += group_l[i];
+#pragma unroll
+    for (uint32_t i = 0; i < kWaves; ++i) {
+        sum += wave_l[i];
         o += sums[i][lane];
     }
     f32x4 y;
@@ -184,7 +194,12 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
     }
     if (e != hipSuccess || a.row_units) return e;
     const uint32_t lines = c.sequences * s.q_heads;
-    // Few rows have many parts: a workgroup for every 64 dims of one, and of 16 wavefronts.
+    // Few rows have many parts: a workgroup for every 64 dims of one, and of 16 wavefronts; for every 32 where they
+    // have 128 and more (8 heads of 256 dims, 512 parts 34.1 us for 35.0; 32 parts the other way, 13.5 for 13.9).
+    if (lines < 64 && p.most_parts / (c.sequences * c.kv_heads * a.head_tiles) >= 128) {
+        hipLaunchKernelGGL((paged_join_kernel<8, 1024>), dim3(lines, (c.head_dim + 31) / 32), dim3(1024), 0, stream, a);
+        return hipGetLastError();
+    }
     if (lines < 512) {
         hipLaunchKernelGGL((paged_join_kernel<16, 1024>), dim3(lines, (c.head_dim + 63) / 64), dim3(1024), 0, stream, a);
         return hipGetLastError();
