@@ -7,12 +7,18 @@
 //   out = sum_j e^{x_j} v_j / sum_j e^{x_j}, zero where nothing is seen.
 // One pass over the keys with the running maximum and sum.  The work is split
 // evenly, not row by row: a row is a sequence's KV head with up to 16 query
-// heads, its positions are counted in units of a workgroup's step, and of all
+// heads, its positions are counted in units of a wavefront's step, and of all
 // rows' units together every workgroup takes the same number, so that lengths do
 // not matter for the balance and a lone sequence keeps the whole chip.  Lengths
 // live on the device, so the workgroups find their parts there.  A part that ends
 // inside a row leaves its maximum m, sum l of 2^{x - m} and sum O of 2^{x - m} v,
-// which a second launch joins.
+// which a second launch joins.  (Short rows are not cut: whole_row_units.)
+//
+// Bound by how fast a CU loads, some 18 KB/us: 24 sequences of 1000 to 30001 Q8_0
+// positions, 8 KV heads of 128 dims and 32 heads 172 us, 4.7 TB/s of 6.2 that a
+// plain load of all CUs reaches; 131072 f16 positions of 256 dims 39 us with the join,
+// 3.4 TB/s.  Q4_0 is bound by its unpacking: 261001 positions of 256 dims 28 us, 1000
+// vector instructions of a wavefront for 32 positions.
 #pragma once
 
 #include "attention_lanes.hpp"
@@ -134,8 +140,8 @@ struct ValueWords {
 template <int FMT, int NB, int HP>
 struct Step;
 
-// f32 throughout (v_mfma_f32_16x16x4): 20 TB/s of keys and values, whatever the
-// number of heads.
+// f32 throughout (v_mfma_f32_16x16x4): at the 151 TFLOP/s of a large product 19 TB/s
+// of keys and values, whatever the number of heads.
 template <int NB>
 struct Step<kKvF32, NB, 16> {
     static constexpr int kTiles = 1, kOut = 2 * NB, kQuads = NB / 2, kQueryBytes = 2 * NB * kWave * 16;

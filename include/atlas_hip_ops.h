@@ -554,11 +554,11 @@ int atlas_hip_paged_read(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, con
  * Q8_0 and Q4_0 rows the products' other operands are two f16 numbers or three bf16
  * ones each, f32's bits.  A score is off by up to (head_dim + 24) 2^-24 of |scale|
  * sum_i |q_i k_i|, with those formats and 2^-38 of |scale| max_i |q_i| sum_i |k_i|,
- * which moves its weight by a factor; apart from that a result is within 1e-5 of
- * float64 normwise, at any number of positions.  A call's result does not depend on
- * timing.  q, output and the workspace are 16-byte aligned; output
- * overlaps neither q nor the pages; sequences * q_heads <= 2^23, sequences *
- * table_width * page_size <= 2^35.  The workspace
+ * which moves its weight by a factor; with F16 a weight is off by up to 2^-40 of its
+ * row's largest; apart from that a result is within 1e-5 of float64 normwise, at any
+ * number of positions.  A call's result does not depend on timing.  q, output and the
+ * workspace are 16-byte aligned; output overlaps neither q nor the pages; sequences *
+ * q_heads <= 2^23, sequences * table_width * page_size <= 2^35.  The workspace
  * (atlas_hip_paged_attention_workspace bytes; no pointer of the struct is read) is
  * overwritten by every call and holds nothing between calls: calls that can overlap,
  * and graphs whose replays can, need one each. */
