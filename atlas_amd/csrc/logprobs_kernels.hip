@@ -160,8 +160,9 @@ __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams
             sum += e;
             if (SPREAD) spread = __builtin_fma(e, -y, spread);
         };
-        // |top| within 2^20 temperatures: its neighbours are nearer than `reach`
-        if (__builtin_fabs(zero) * v.s.inv_temperature < 0x1p20 && v.s.inv_temperature > 0x1p-60 && !__builtin_isinf(top)) {
+        // |top| within 2^20 temperatures, and the least of numbers far below one: its neighbours are nearer than `reach`
+        if (__builtin_fabs(zero) * v.s.inv_temperature < 0x1p20 && v.s.inv_temperature > 0x1p-60 && v.s.inv_temperature < 0x1p100 &&
+            !__builtin_isinf(top)) {
             const float lowest = static_cast<float>(zero - reach);
 #pragma unroll
             for (int i = 0; i < STRIPS; ++i)

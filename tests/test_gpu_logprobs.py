@@ -142,6 +142,28 @@ def test_temperatures(rt, inv):
     assert np.array_equal(got[2], exp[2])
 
 
+@pytest.mark.parametrize("inv", [1e20, 1e30, 1e39, 1e46, 1e60, 1e300])
+def test_cold_rows_around_zero(rt, inv):
+    """A largest logit of zero or hardly more, and others nearer to it than a number of its size could tell, and farther."""
+    x = np.zeros((5, 1500), f32)
+    away = np.random.default_rng(6).uniform(0, 30, (5, 1500)) / inv
+    x[0] = -away[0].astype(f32)
+    x[0, 7] = 0.0
+    x[1] = -1.0
+    x[1, 700] = 0.0
+    x[2] = -np.arange(1500, dtype=f32) * f32(2.0 ** -149)
+    x[3] = -1e-30
+    x[3, 3:40:9] = 1e-41
+    x[4] = np.where(np.arange(1500) % 2, -1e-40, -2.0)
+    tokens = np.argsort(-x, 1, kind="stable")[:, :5].astype(u32)
+    got = run(rt, x, 1500, tokens, inv, 5)
+    exp = ref.logprobs(x, tokens, inv, 5)
+    assert np.array_equal(got[2], exp[2])
+    with np.errstate(over="ignore"):
+        for g, e in ((got[0], exp[0]), (got[1], exp[1]), (got[3], exp[3])):
+            close(f"inv {inv}", g, np.where(np.isinf(e.astype(f32)), e.astype(f32), e))
+
+
 def test_likely_tokens_keep_their_digits(rt):
     """Log probabilities down to -1e-30: the others' mass, not 1 less a sum."""
     x = np.zeros((4, 3000), f32)
