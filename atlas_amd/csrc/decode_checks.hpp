@@ -187,15 +187,16 @@ inline const char* paged_read_error(const PagedReadArgs& a) {
     return nullptr;
 }
 
-// Units of 16 positions are counted in 32 bits.
-constexpr uint64_t kMostPagedPositions = 1ull << 35;
+// Of all rows of up to 16 query heads: a part has 1024 units of 16 positions, and there are 2^20 parts.
+constexpr uint64_t kMostPagedPositions = 1ull << 34;
 
 inline const char* paged_attention_sizes_error(const PagedCache& c, uint32_t q_heads) {
     if (const char* error = paged_cache_sizes_error(c)) return error;
     if (q_heads == 0 || q_heads % c.kv_heads != 0) return "paged attention needs q_heads a multiple of kv_heads";
     if (static_cast<uint64_t>(c.sequences) * q_heads > kMostGroups) return "paged attention has more than 2^23 query rows";
-    if (static_cast<uint64_t>(c.table_width) * c.page_size * c.sequences > kMostPagedPositions)
-        return "paged attention is limited to 2^35 positions of all sequences together";
+    const uint64_t rows = static_cast<uint64_t>(c.sequences) * c.kv_heads * ((q_heads / c.kv_heads + 15) / 16);
+    if (static_cast<uint64_t>(c.table_width) * c.page_size * rows > kMostPagedPositions)
+        return "paged attention is limited to 2^34 positions of all sequences and KV heads together";
     return nullptr;
 }
 

@@ -138,6 +138,8 @@ __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams
     FineExp2::fill(table);
     const FineExp2 exp2_of(table);
     const double scale = fmin(v.scale * 32.0, 0x1.fffffffffffffp1023), reach = 708.0 / v.s.inv_temperature;
+    // a top within 2^20 temperatures, and the least of numbers far below one: its neighbours are nearer than `reach`
+    const double near = v.s.inv_temperature > 0x1p-60 && v.s.inv_temperature < 0x1p100 ? 0x1p20 / v.s.inv_temperature : 0.0;
     __syncthreads();
     for (uint64_t item = blockIdx.x * kLogWaves + wave; item < items; item += step) {
         const uint64_t at = static_cast<uint64_t>(row) * v.count + slice;
@@ -160,9 +162,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams
             sum += e;
             if (SPREAD) spread = __builtin_fma(e, -y, spread);
         };
-        // |top| within 2^20 temperatures, and the least of numbers far below one: its neighbours are nearer than `reach`
-        if (__builtin_fabs(zero) * v.s.inv_temperature < 0x1p20 && v.s.inv_temperature > 0x1p-60 && v.s.inv_temperature < 0x1p100 &&
-            !__builtin_isinf(top)) {
+        if (__builtin_fabs(static_cast<double>(top)) < near) {
             const float lowest = static_cast<float>(zero - reach);
 #pragma unroll
             for (int i = 0; i < STRIPS; ++i)

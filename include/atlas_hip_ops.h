@@ -527,11 +527,11 @@ int atlas_hip_paged_cache_bytes(atlas_hip_ctx *ctx, const atlas_paged_cache *cac
  * cosine and sine NULL: nothing is rotated, and query is NULL.  sequence_ids NULL:
  * token t is sequence t's (tokens <= sequences).  A token whose sequence or position
  * (>= table_width * page_size) is out of range is skipped, query row and all:
- * padding.  The rows of a call should be distinct: of two tokens at one position, the
- * row has each value from either.  Rows are bit-equal to rope_half_f32's, rounded to
- * nearest for F16, encoded block by block as kv_append does for Q8_0 and Q4_0.  key,
- * value, query and query_out are 16-byte aligned; tokens * (q_heads + 2 kv_heads) <=
- * 2^25. */
+ * padding.  The rows of a call have to be distinct: one that two tokens write (their
+ * positions are the same, or their sequences share the page) holds codes and scales of
+ * either.  Rows are bit-equal to rope_half_f32's, rounded to nearest for F16, encoded
+ * block by block as kv_append does for Q8_0 and Q4_0.  key, value, query and query_out
+ * are 16-byte aligned; tokens * (q_heads + 2 kv_heads) <= 2^25. */
 int atlas_hip_paged_append(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, const float *key, const float *value,
                            const float *query, float *query_out, const float *cosine, const float *sine,
                            uint32_t rope_rows, uint32_t rope_stride, const uint32_t *sequence_ids,
@@ -558,7 +558,8 @@ int atlas_hip_paged_read(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, con
  * row's largest; apart from that a result is within 1e-5 of float64 normwise, at any
  * number of positions.  A call's result does not depend on timing.  q, output and the
  * workspace are 16-byte aligned; output overlaps neither q nor the pages; sequences *
- * q_heads <= 2^23, sequences * table_width * page_size <= 2^35.  The workspace
+ * q_heads <= 2^23, sequences * kv_heads * table_width * page_size <= 2^34, a KV head of
+ * more than 16 query heads counting once for every 16.  The workspace
  * (atlas_hip_paged_attention_workspace bytes; no pointer of the struct is read) is
  * overwritten by every call and holds nothing between calls: calls that can overlap,
  * and graphs whose replays can, need one each. */

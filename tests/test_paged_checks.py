@@ -108,7 +108,9 @@ def test_read_calls(checks, change, fine):
     (dict(q_heads=7), False), (dict(scale=math.nan), False), (dict(scale=math.inf), False), (dict(q=3 * M + 4), False),
     (dict(output=5 * M + 8), False), (dict(workspace=6 * M + 8), False), (dict(lengths=4 * M + 2), False), (dict(output=3 * M), False),
     (dict(output=M + 16), False), (dict(sequences=1 << 20, q_heads=10), False),
-    (dict(sequences=1 << 20, table_width=2048), True), (dict(sequences=1 << 20, table_width=2049), False),
+    (dict(sequences=1 << 20, table_width=512), True), (dict(sequences=1 << 20, table_width=513), False),
+    (dict(sequences=1 << 17, q_heads=64, table_width=2048), True), (dict(sequences=1 << 17, q_heads=64, table_width=2049), False),
+    (dict(table_width=1 << 25), True), (dict(sequences=17, table_width=1 << 25), False),
 ])
 def test_attention_calls(checks, change, fine):
     assert (call(checks.check_attention, ATTEND, change) is None) == fine
