@@ -533,31 +533,35 @@ class PagedDecode:
     def window(self, layer: int) -> int:
         return 0 if layer % 5 == 4 else self.S.window
 
-    def _grow(self, place: int, length: int) -> None:
-        """Pages for the first `length` positions of a sequence."""
-        if length > self.S.capacity:
+    def _grow(self, lengths: dict) -> None:
+        """Pages for the first positions of sequences, {place: positions}: of all or of none."""
+        if any(n > self.S.capacity for n in lengths.values()):
             raise ValueError("a sequence has no room for its next position: end() it first")
-        have = int((self.table[place] != self.NO_PAGE).sum())
-        need = -(-length // self.S.page_size) - have
-        if need > len(self.free):
+        have = {place: int((self.table[place] != self.NO_PAGE).sum()) for place in lengths}
+        need = {place: -(-n // self.S.page_size) - have[place] for place, n in lengths.items()}
+        if sum(need.values()) > len(self.free):
             raise ValueError("the pool has no page left: end() a sequence first")
-        for i in range(need):
-            self.table[place, have + i] = self.free.pop()
+        for place, n in need.items():
+            for i in range(n):
+                self.table[place, have[place] + i] = self.free.pop()
 
     def begin(self, prompts) -> None:
         """Sequences for free places: {place: per layer (keys, values) [tokens, kv_heads, head_dim]}."""
         rt, S = self.rt, self.S
-        places, positions = [], []
-        for place, layers in prompts.items():
+        tokens = {place: layers[0][0].shape[0] for place, layers in prompts.items()}
+        for place, n in tokens.items():
             if self.lengths[place]:
                 raise ValueError(f"place {place} has a sequence")
-            n = layers[0][0].shape[0]
-            self._grow(place, n)
+            if not n:
+                raise ValueError("a prompt has no token")
+        if not tokens:
+            return
+        self._grow(tokens)
+        places, positions = [], []
+        for place, n in tokens.items():
             self.lengths[place] = n
             places += [place] * n
             positions += range(n)
-        if not places:
-            return
         self.dev["table"].upload(self.table)
         held = [rt.upload(np.array(places, np.uint32)), rt.upload(np.array(positions, np.uint32))]
         for layer in range(S.layers):
@@ -579,8 +583,7 @@ class PagedDecode:
     def set_step(self, logits) -> None:
         """The step's logits [sequences, vocab]; pages for its positions."""
         active = self.lengths > 0
-        for place in np.nonzero(active)[0]:
-            self._grow(int(place), int(self.lengths[place]) + 1)
+        self._grow({int(place): int(self.lengths[place]) + 1 for place in np.nonzero(active)[0]})
         d = self.dev
         d["table"].upload(self.table)
         d["positions"].upload(np.where(active, self.lengths, 0xFFFFFFFF).astype(np.uint32))

@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 import paged_refs as ref
-from atlas_amd.chains import PagedDecode
+from atlas_amd.chains import PagedDecode, PagedShape
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 U32, U64 = c_uint32, c_uint64
@@ -149,6 +149,32 @@ def test_a_values_codes_are_where_the_layout_says(checks, D):
     place = np.argsort(order)
     for d in range(0, D, 2):
         assert checks.value_place(D, d) == place[d] and place[d + 1] == place[d] + 1
+
+
+def test_sequences_that_do_not_fit_change_nothing():
+    """PagedDecode.begin takes all of its prompts or none, and set_step pages for all of the sequences."""
+    class Runtime:
+        def __getattr__(self, name):
+            raise AssertionError(f"{name} was called")
+
+    chain = object.__new__(PagedDecode)
+    chain.rt, chain.S = Runtime(), PagedShape(sequences=4, capacity=64, pages=6, page_size=16)
+    chain.lengths, chain.table = np.array([16, 0, 0, 16], np.uint32), np.full((4, 4), PagedDecode.NO_PAGE, np.uint32)
+    chain.table[0, 0], chain.table[3, 0] = 0, 1
+    chain.free = [5]
+    before = chain.lengths.copy(), chain.table.copy(), list(chain.free)
+
+    def prompt(n):
+        return [(np.zeros((n, 3, 64), np.float32),) * 2] * 3
+
+    for prompts, what in (({1: prompt(16), 2: prompt(17)}, "no page left"), ({1: prompt(3), 0: prompt(1)}, "has a sequence"),
+                          ({1: prompt(3), 2: prompt(65)}, "no room"), ({1: prompt(3), 2: prompt(0)}, "no token")):
+        with pytest.raises(ValueError, match=what):
+            chain.begin(prompts)
+        assert (chain.lengths == before[0]).all() and (chain.table == before[1]).all() and chain.free == before[2], what
+    with pytest.raises(ValueError, match="no page left"):
+        chain.set_step(None)
+    assert (chain.table == before[1]).all() and chain.free == before[2]
 
 
 def test_a_failed_recording_leaves_no_graph_behind():
