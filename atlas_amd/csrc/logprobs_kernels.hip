@@ -14,8 +14,9 @@
 // likeliest tokens cost the first launch nothing: of 64 or 256 groups of cells the k-th
 // largest maximum is a border that k tokens reach, so only cells that reach it are
 // read again (some 25 of 2048 for 20 tokens) and what reaches it in them is ranked.
-// Bound by the 64-bit sums: 256 rows of 262144 logits 56 to 62 us in the first launch,
-// 4.5 TB/s, and 8.5 in the second; 2048 of 50257 88 and 7.
+// Bound by the bytes and nearly as much by the 64-bit instructions: 256 rows of 262144
+// logits 52 to 54 us in the first launch, 5.0 TB/s (random numbers are read at 5.8 at
+// best), and 8.5 in the second; 2048 of 50257 82 to 84 and 7.
 #include "exp2_f64.hpp"
 #include "launch.hpp"
 
@@ -32,8 +33,6 @@ constexpr uint32_t kCells = 8;     // of a strip: the logits of eight lanes
 constexpr int kEach = kStrip / kWave;
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr uint32_t kCellList = 1024, kTokenList = 512;
-
-typedef f32x4 f32x4_row __attribute__((aligned(4)));
 
 // A slice's sums of e^{y} and of e^{y} (-y), relative to its top, y in thirty-seconds
 // of powers of two.
@@ -58,41 +57,42 @@ __device__ __forceinline__ double finite(float top) { return __builtin_isinf(top
 // Logit i of a lane's in a strip, four at a time; lanes 8 r .. 8 r + 7 have cell r.
 __device__ __forceinline__ uint32_t slice_at(uint32_t lane, int i) { return (i / 4 * kWave + lane) * 4 + i % 4; }
 
-__device__ __forceinline__ void load_lane(const float* logits, uint32_t first, uint32_t lane, uint32_t vocab, float (&x)[kEach]) {
-    if (first + kStrip <= vocab) {
+// Behind a row's end a load brings zeros, which are no logits of it.
+__device__ __forceinline__ void load_lane(__amdgpu_buffer_rsrc_t logits, uint32_t first, uint32_t lane, float (&x)[kEach]) {
 #pragma unroll
-        for (int i = 0; i < kEach / 4; ++i) {
-            const f32x4 y = *reinterpret_cast<const f32x4_row*>(logits + first + slice_at(lane, 4 * i));
+    for (int i = 0; i < kEach / 4; ++i) {
+        const f32x4 y = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(logits, (first + slice_at(lane, 4 * i)) * 4, 0, 0));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[4 * i + j] = y[j];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const uint32_t at = first + slice_at(lane, i);
-            x[i] = at < vocab ? logits[at] : -__builtin_inff();
-        }
+        for (int j = 0; j < 4; ++j) x[4 * i + j] = y[j];
     }
 }
+__device__ __forceinline__ void end_lane(uint32_t first, uint32_t lane, uint32_t vocab, float (&x)[kEach]) {
+    if (first + kStrip > vocab)
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (first + slice_at(lane, i) >= vocab) x[i] = -__builtin_inff();
+}
 
-// 2^(y / 1024), y <= 0, as Exp2 has 2^(y / 32): of a table of 1024 the polynomial
-// needs three degrees, ((ln 2 / 2048)^4 / 24 is below 2^-50).
+// 2^(y / 256), y <= 0, as Exp2 has 2^(y / 32): of a table of 256 the polynomial needs
+// three degrees: of r^4, |r| <= 1 / 2, the second one takes a r^2, which leaves least at
+// a = (sqrt 2 - 1) / 2, and the whole within 2^-45.  A table's place is a byte of the
+// sum; its bits come along with the exponent, so a table entry has them taken out.
 struct FineExp2 {
-    static constexpr uint32_t kSize = 1024;
+    static constexpr uint32_t kSize = 256;
     const uint2* table;
     double c[3], shift, least;
 
     static __device__ void fill(uint2 (&table)[kSize]) {
-        for (uint32_t i = threadIdx.x; i < kSize; i += kLogThreads) {
-            const uint64_t bits = __builtin_bit_cast(uint64_t, exp2(i * (1.0 / kSize)));
-            table[i] = make_uint2(static_cast<uint32_t>(bits), static_cast<uint32_t>(bits >> 32) - (1023u << 20));
-        }
+        static_assert(kSize == kLogThreads);
+        const uint32_t i = threadIdx.x;
+        const uint64_t bits = __builtin_bit_cast(uint64_t, exp2(i * (1.0 / kSize)));
+        table[i] = make_uint2(static_cast<uint32_t>(bits), static_cast<uint32_t>(bits >> 32) - (1023u << 20) - (i << 12));
     }
     explicit __device__ FineExp2(const uint2 (&table)[kSize])
         : table(table),
-          c{0x1.c6b08d704a0c0p-5 * 0x1p-30,  // ln2^3 / 6, of 1 / 1024 each
-            0x1.ebfbdff82c58fp-3 * 0x1p-20,  // ln2^2 / 2
-            0x1.62e42fefa39efp-1 * 0x1p-10}, // ln2
+          c{0x1.c6b08d704a0c0p-5 * 0x1p-24,  // ln2^3 / 6, of 1 / 256 each
+            0x1.ebfbe40c8b585p-3 * 0x1p-16,  // ln2^2 / 2 + a ln2^4 / 24 / 256^2
+            0x1.62e42fefa39efp-1 * 0x1p-8},  // ln2
           shift(0x1.8p52 + kSize * 1023.0), least(-1022.0 * kSize) {
         asm("" : "+v"(c[0]));
 #pragma unroll
@@ -107,7 +107,7 @@ struct FineExp2 {
         p = __builtin_fma(p, r, c[2]);
         p = __builtin_fma(p, r, 1.0);
         uint2 power = table[k % kSize];
-        power.y += (k & ~(kSize - 1)) << 10;
+        power.y += k << 12;
         return p * __builtin_bit_cast(double, static_cast<uint64_t>(power.y) << 32 | power.x);
     }
 };
@@ -115,11 +115,10 @@ struct FineExp2 {
 // Workgroups that stay: eight to a CU, and the table's filling, behind the first
 // logits' loads, once for all of a workgroup's slices.  Bound by the bytes and the
 // 64-bit instructions together, so a logit takes as few as there are: one that is no
-// number, and one too far below the top to have mass, become the lowest that has
-// hardly any in an instruction of 32 bits (where the top and the temperature let 32
-// bits tell them apart).
+// number, and one too far below the top to have mass, become in one instruction the
+// lowest that has hardly any.
 template <bool SPREAD, int STRIPS>
-__global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams v) {
+__global__ __launch_bounds__(kLogThreads, 8) void logprob_sums_kernel(LogprobParams v) {
     __shared__ uint2 table[FineExp2::kSize];
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(threadIdx.x / kWave));
@@ -130,22 +129,21 @@ __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams
     const uint32_t row_step = step / v.count, slice_step = step % v.count;
     float x[STRIPS][kEach];
     const auto load = [&] {
-        const float* logits = v.s.logits + row * v.s.row_stride;
+        const auto logits = span_rsrc(v.s.logits + row * v.s.row_stride, v.s.vocab * 4);
 #pragma unroll
-        for (int i = 0; i < STRIPS; ++i) load_lane(logits, (slice * STRIPS + i) * kStrip, lane, v.s.vocab, x[i]);
+        for (int i = 0; i < STRIPS; ++i) load_lane(logits, (slice * STRIPS + i) * kStrip, lane, x[i]);
     };
     load();
     FineExp2::fill(table);
     const FineExp2 exp2_of(table);
-    const double scale = fmin(v.scale * 32.0, 0x1.fffffffffffffp1023), reach = 708.0 / v.s.inv_temperature;
-    // a top within 2^20 temperatures, and the least of numbers far below one: its neighbours are nearer than `reach`
-    const double near = v.s.inv_temperature > 0x1p-60 && v.s.inv_temperature < 0x1p100 ? 0x1p20 / v.s.inv_temperature : 0.0;
+    const double scale = fmin(v.scale * 8.0, 0x1.fffffffffffffp1023);
     __syncthreads();
     for (uint64_t item = blockIdx.x * kLogWaves + wave; item < items; item += step) {
         const uint64_t at = static_cast<uint64_t>(row) * v.count + slice;
         float cell[STRIPS], most = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < STRIPS; ++i) {
+            end_lane((slice * STRIPS + i) * kStrip, lane, v.s.vocab, x[i]);
             cell[i] = -__builtin_inff();
 #pragma unroll
             for (int j = 0; j < kEach; ++j) cell[i] = fmaxf(cell[i], x[i][j]);
@@ -157,26 +155,21 @@ __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams
         const float top = wave_max_tree_f32(most);
         const double zero = finite(top);
         double sum = 0.0, spread = 0.0;
-        const auto add = [&](double y) {
-            const double e = exp2_of(y);
-            sum += e;
-            if (SPREAD) spread = __builtin_fma(e, -y, spread);
-        };
-        if (__builtin_fabs(static_cast<double>(top)) < near) {
-            const float lowest = static_cast<float>(zero - reach);
+        if (top == __builtin_inff())
 #pragma unroll
             for (int i = 0; i < STRIPS; ++i)
 #pragma unroll
-                for (int j = 0; j < kEach; ++j) add((static_cast<double>(fmaxf(x[i][j], lowest)) - zero) * scale);
-        } else {
+                for (int j = 0; j < kEach; ++j) x[i][j] = about(x[i][j], top);
 #pragma unroll
-            for (int i = 0; i < STRIPS; ++i)
+        for (int i = 0; i < STRIPS; ++i)
 #pragma unroll
-                for (int j = 0; j < kEach; ++j) {
-                    const double y = (static_cast<double>(about(number_or_none(x[i][j]), top)) - zero) * scale;
-                    if (y >= exp2_of.least) add(y);
-                }
-        }
+            for (int j = 0; j < kEach; ++j) {
+                const double y = fmax((static_cast<double>(x[i][j]) - zero) * scale, exp2_of.least), e = exp2_of(y);
+                sum += e;
+                if (SPREAD) spread = __builtin_fma(e, -y, spread);
+            }
+        // here, and not behind the next logits' loads, beside which these would have to be kept
+        asm volatile("" : "+v"(sum), "+v"(spread));
         float* cells = v.cells + static_cast<uint64_t>(row) * v.strips * kCells;
         const uint32_t strip = slice * STRIPS;
         row += row_step;
@@ -188,7 +181,7 @@ __global__ __launch_bounds__(kLogThreads) void logprob_sums_kernel(LogprobParams
         if (item + step < items) load();
         sum = wave_sum_f64(sum);
         if (SPREAD) spread = wave_sum_f64(spread);
-        if (lane == 0) v.slices[at] = SliceSums{sum, spread * (1.0 / 32.0)};
+        if (lane == 0) v.slices[at] = SliceSums{sum, spread * (1.0 / 8.0)};
         if (lane % 8 == 0)
 #pragma unroll
             for (uint32_t i = 0; i < STRIPS; ++i)
@@ -213,7 +206,8 @@ template <class F>
 __device__ __forceinline__ void for_cell(const float* logits, uint32_t cell, uint32_t vocab, F&& f) {
     const uint32_t lane = threadIdx.x % 8 + cell % kCells * 8, first = cell / kCells * kStrip;
     float x[kEach];
-    load_lane(logits, first, lane, vocab, x);
+    load_lane(span_rsrc(logits, vocab * 4), first, lane, x);
+    end_lane(first, lane, vocab, x);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) f(x[i], first + slice_at(lane, i));
 }
