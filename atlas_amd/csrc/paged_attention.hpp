@@ -604,15 +604,24 @@ struct Step {
             const uint32_t w = v[j][kWords.word[b] + at / 4];
             if constexpr (kBytes)
                 x[j] = static_cast<float>(static_cast<int8_t>(w >> (8 * (at % 4))));
-            else  // two's complement by the flip of bit 3
-                x[j] = nibble(e ? (w ^ 0x88888888u) >> 4 : w ^ 0x88888888u, at % 4);
+            else
+                x[j] = nibble(e ? w >> 4 : w, at % 4);
         }
         u32x4_t y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = upper(x[2 * i + 1], x[2 * i]);
         return __builtin_bit_cast(bf16x8_t, y);
     }
-    __device__ __forceinline__ void add(const f32x4 (&p)[2], f32x4 (&out)[kOut]) const {
+    __device__ __forceinline__ void add(const f32x4 (&p)[2], f32x4 (&out)[kOut]) {
+        if constexpr (!kBytes) {  // two's complement by the flip of bit 3, here for both codes of a byte
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < kWords.words; ++i) {
+                    v[j][i] ^= 0x88888888u;
+                    asm("" : "+v"(v[j][i]));
+                }
+        }
 #pragma unroll
         for (int step = 0; step < kValueSteps; ++step) {
             u32x4_t piece[3];
@@ -620,7 +629,8 @@ struct Step {
             for (int i = 0; i < 4; ++i) {
                 float w[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) w[j] = p[i / 2][i % 2 * 2 + j] * scale_of(vs[i / 2][step], i % 2 * 2 + j);
+                for (int j = 0; j < 2; ++j)  // a multiply-add takes the f16 scale as it is
+                    w[j] = __builtin_fmaf(p[i / 2][i % 2 * 2 + j], scale_of(vs[i / 2][step], i % 2 * 2 + j), 0.0f);
 #pragma unroll
                 for (int n = 0; n < 3; ++n) {
                     piece[n][i] = upper(w[1], w[0]);
