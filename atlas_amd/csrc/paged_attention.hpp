@@ -68,17 +68,14 @@ __device__ __forceinline__ SeenRange seen_of(const PagedAttnParams& a, uint32_t 
 __device__ __forceinline__ uint32_t units_of(SeenRange s, uint32_t unit) {
     return s.hi > s.lo ? (s.hi + unit - 1) / unit - s.lo / unit : 0u;
 }
-__device__ __forceinline__ uint64_t parts_of(const PagedAttnParams& a, uint64_t total) {
-    uint64_t parts = (total + a.part_units - 1) / a.part_units;
+// Of at most 2^30 units, and one more for a row whose window begins and ends inside units.
+__device__ __forceinline__ uint32_t parts_of(const PagedAttnParams& a, uint32_t total) {
+    uint32_t parts = (total + a.part_units - 1) / a.part_units;
     parts = parts > a.few_parts ? parts : a.few_parts;
     parts = parts < a.most_parts ? parts : a.most_parts;
     return parts < total ? parts : total;
 }
 
-__device__ __forceinline__ uint64_t uniform_u64(uint64_t v) {
-    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32)))) << 32 |
-           static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v)));
-}
 __device__ __forceinline__ uint32_t uniform_u32(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(v)); }
 
 constexpr uint32_t kPastPage = 0x7ffffff0u;  // a buffer offset past every part: reads as zero
@@ -687,77 +684,96 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? paged_occupancy(32 * NB
     __shared__ uint32_t found_before, found_seq;
     const uint32_t lane = threadIdx.x % kWave, c = lane % 16, g = lane / 16;
     const uint32_t wave = uniform_u32(threadIdx.x / kWave);
-    const uint64_t rows = static_cast<uint64_t>(a.kv_heads) * a.head_tiles;  // of a sequence
+    const uint32_t rows = a.kv_heads * a.head_tiles;  // of a sequence
 
-    uint64_t begin, end, before = 0, total = 0, parts = 0;
-    uint32_t seq;
+    uint32_t begin, end, before = 0, seq, units, each = 0, longer = 0;
+    SeenRange seen;
     if constexpr (WHOLE) {
-        seq = static_cast<uint32_t>(blockIdx.x / rows);
-        const uint32_t units = uniform_u32(units_of(seen_of(a, seq), kKeys));
+        seq = blockIdx.x / rows;
+        seen = seen_of(a, seq);
+        units = uniform_u32(units_of(seen, kKeys));
         begin = blockIdx.x % rows * units;
         end = begin + units;
         if (units == 0) {
-            const uint32_t row = static_cast<uint32_t>(blockIdx.x % rows), head0 = row % a.head_tiles * kPagedHeads;
+            const uint32_t row = blockIdx.x % rows, head0 = row % a.head_tiles * kPagedHeads;
             const uint32_t heads = min(a.group - head0, static_cast<uint32_t>(HP));
             float* to = a.output + (static_cast<uint64_t>(seq) * a.q_heads + row / a.head_tiles * a.group + head0) * a.head_dim;
             for (uint32_t i = threadIdx.x; i < heads * a.head_dim; i += kThreads) to[i] = 0.0f;
             return;
         }
     } else {
-        // this workgroup's units of all sequences'; those of a chunk of sequences, one a thread, up to each
-        const auto scan = [&](uint32_t units, uint32_t& chunk) {
-            uint32_t upto = wave_inclusive_scan_u32(units);
-            __syncthreads();
-            if (lane == kWave - 1) room_units[wave] = upto;
-            __syncthreads();
-            chunk = 0;
-#pragma unroll
-            for (uint32_t w = 0; w < WAVES; ++w) {
-                if (w == wave) upto += chunk;
-                chunk += room_units[w];
-            }
-            return upto;
+        // this workgroup's units of all sequences', and the sequence that the first lies in; parts have `each` units,
+        // the first `longer` one more
+        const auto share = [&](uint32_t all_units) {
+            const uint32_t total = uniform_u32(all_units) * rows, parts = uniform_u32(parts_of(a, total));
+            if (blockIdx.x >= parts) return false;
+            each = uniform_u32(total / parts);
+            longer = total - each * parts;
+            begin = blockIdx.x * each + min(blockIdx.x, longer);
+            end = begin + each + (blockIdx.x < longer ? 1 : 0);
+            return true;
         };
-        uint32_t mine = 0, first_units = 0;
-        for (uint32_t b = threadIdx.x; b < a.sequences; b += kThreads) {
-            const uint32_t units = units_of(seen_of(a, b), kKeys);
-            if (b < kThreads) first_units = units;
-            mine += units;
-        }
-        uint32_t all_units;
-        uint32_t upto = scan(mine, all_units);
-        total = uniform_u32(all_units) * rows;
-        parts = parts_of(a, total);
-        if (blockIdx.x >= parts) return;
-        begin = uniform_u64(total * blockIdx.x / parts);
-        end = uniform_u64(total * (blockIdx.x + 1) / parts);
-        // the sequence that `begin` lies in
-        const uint32_t wanted = static_cast<uint32_t>(begin / rows);
-        uint32_t ahead = 0;
-        for (uint32_t first = 0; first < a.sequences; first += kThreads) {
-            const uint32_t b = first + threadIdx.x;
-            uint32_t units = first_units, chunk = all_units;
-            if (a.sequences > kThreads) {
-                if (first) units = b < a.sequences ? units_of(seen_of(a, b), kKeys) : 0u;
-                upto = scan(units, chunk);
+        if (a.sequences <= kWave) {  // each wavefront for itself: one sequence 9.7 -> 9.0 us with the shares' 32 bits
+            SeenRange of_lane = {0, 0};
+            if (lane < a.sequences) of_lane = seen_of(a, lane);
+            const uint32_t own = units_of(of_lane, kKeys), upto = wave_inclusive_scan_u32(own);
+            if (!share(readlane_u32(upto, kWave - 1))) return;
+            const uint32_t wanted = uniform_u32(begin / rows), from = upto - own;
+            seq = static_cast<uint32_t>(__builtin_ctzll(__builtin_amdgcn_ballot_w64(wanted >= from && wanted - from < own)));
+            before = readlane_u32(from, seq) * rows;
+            seen = {readlane_u32(of_lane.lo, seq), readlane_u32(of_lane.hi, seq)};
+            units = readlane_u32(own, seq);
+        } else {
+            // a chunk of sequences, one a thread: units up to each
+            const auto scan = [&](uint32_t units, uint32_t& chunk) {
+                uint32_t upto = wave_inclusive_scan_u32(units);
+                __syncthreads();
+                if (lane == kWave - 1) room_units[wave] = upto;
+                __syncthreads();
+                chunk = 0;
+#pragma unroll
+                for (uint32_t w = 0; w < WAVES; ++w) {
+                    if (w == wave) upto += chunk;
+                    chunk += room_units[w];
+                }
+                return upto;
+            };
+            uint32_t mine = 0, first_units = 0;
+            for (uint32_t b = threadIdx.x; b < a.sequences; b += kThreads) {
+                const uint32_t own = units_of(seen_of(a, b), kKeys);
+                if (b < kThreads) first_units = own;
+                mine += own;
             }
-            const uint32_t from = ahead + upto - units;
-            if (wanted >= from && wanted - from < units) {
-                found_before = from;
-                found_seq = b;
+            uint32_t all_units;
+            uint32_t upto = scan(mine, all_units);
+            if (!share(all_units)) return;
+            const uint32_t wanted = uniform_u32(begin / rows);
+            uint32_t ahead = 0;
+            for (uint32_t first = 0; first < a.sequences; first += kThreads) {
+                const uint32_t b = first + threadIdx.x;
+                uint32_t own = first_units, chunk = all_units;
+                if (a.sequences > kThreads) {
+                    if (first) own = b < a.sequences ? units_of(seen_of(a, b), kKeys) : 0u;
+                    upto = scan(own, chunk);
+                }
+                const uint32_t from = ahead + upto - own;
+                if (wanted >= from && wanted - from < own) {
+                    found_before = from;
+                    found_seq = b;
+                }
+                ahead += chunk;
+                if (ahead > wanted) break;
             }
-            ahead += chunk;
-            if (ahead > wanted) break;
+            __syncthreads();
+            before = uniform_u32(found_before) * rows;
+            seq = uniform_u32(found_seq);
+            seen = seen_of(a, seq);
+            units = uniform_u32(units_of(seen, kKeys));
         }
-        __syncthreads();
-        before = uniform_u32(found_before) * rows;
-        seq = uniform_u32(found_seq);
     }
 
-    for (uint64_t at = begin; at < end;) {
+    for (uint32_t at = begin; at < end;) {
         // a segment: units [t0, t1) of a row's `units`
-        SeenRange seen = seen_of(a, seq);
-        uint32_t units = uniform_u32(units_of(seen, kKeys));
         while (at >= before + units * rows) {
             before += units * rows;
             ++seq;
@@ -766,11 +782,12 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? paged_occupancy(32 * NB
         }
         seen.lo = uniform_u32(seen.lo);
         seen.hi = uniform_u32(seen.hi);
-        const uint32_t row = uniform_u32(static_cast<uint32_t>((at - before) / units));
-        const uint32_t t0 = uniform_u32(static_cast<uint32_t>((at - before) - static_cast<uint64_t>(row) * units));
-        const uint32_t t1 = uniform_u32(end - at < units - t0 ? t0 + static_cast<uint32_t>(end - at) : units);
-        if (!WHOLE && t0 == 0 && threadIdx.x == 0)  // unit u is part ((u + 1) parts - 1) / total's
-            a.rows[seq * rows + row] = {blockIdx.x, static_cast<uint32_t>(((at + units) * parts - 1) / total)};
+        const uint32_t row = uniform_u32((at - before) / units);
+        const uint32_t t0 = at - before - row * units, t1 = min(units, t0 + (end - at));
+        if (!WHOLE && t0 == 0 && threadIdx.x == 0) {
+            const uint32_t last = at + units - 1, short_from = longer * (each + 1);  // the row's last unit
+            a.rows[seq * rows + row] = {blockIdx.x, last < short_from ? last / (each + 1) : longer + (last - short_from) / each};
+        }
         at += t1 - t0;
         const uint32_t kv_head = row / a.head_tiles, head0 = row % a.head_tiles * kPagedHeads;
         const uint32_t heads = min(a.group - head0, static_cast<uint32_t>(HP));
