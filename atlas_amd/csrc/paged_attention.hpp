@@ -666,7 +666,7 @@ struct Step {
 // A workgroup a part of the work, or a whole row: then no other sequence's length
 // is asked for and nothing is left to join.
 template <int FMT, int NB, int HP, int WAVES, bool WHOLE>
-__global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? paged_occupancy(32 * NB) : WAVES / 4) void paged_attention_kernel(PagedAttnParams a) {
+__global__ __launch_bounds__(WAVES * kWave, WAVES == 4 ? paged_occupancy(32 * NB) : (WAVES + 3) / 4) void paged_attention_kernel(PagedAttnParams a) {
     using S = Step<FMT, NB, HP>;
     constexpr uint32_t kThreads = WAVES * kWave;
     constexpr int kTiles = S::kTiles;
@@ -1001,9 +1001,12 @@ hipError_t launch_paged_attention_f16(hipStream_t stream, const PagedAttnParams&
 hipError_t launch_paged_attention_q8_0(hipStream_t stream, const PagedAttnParams& a);
 hipError_t launch_paged_attention_q4_0(hipStream_t stream, const PagedAttnParams& a);
 
-// Wavefronts of a workgroup that takes a whole row of more than two steps for four.
-template <int NB>
-inline constexpr int kPagedRowWaves = NB <= 2 ? 16 : 8;
+// Wavefronts of a workgroup that takes a whole row of more than two steps for four:
+// as many as the registers let stay, but six of f16 rows, whose 32 positions are twice
+// the bytes (256 rows of up to 500 of 128 dims 24 us for 27 with eight; 100 Q8_0 rows of
+// up to 1500 the other way, 23 for 20).
+template <int FMT, int NB>
+inline constexpr int kPagedRowWaves = NB <= 2 ? 16 : FMT == kKvF16 ? 6 : 8;
 
 template <int FMT, int NB, int HP>
 hipError_t launch_paged_heads(hipStream_t stream, const PagedAttnParams& a) {
@@ -1013,8 +1016,8 @@ hipError_t launch_paged_heads(hipStream_t stream, const PagedAttnParams& a) {
     else if (a.row_units <= 8)
         hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, 4, true>), dim3(rows), dim3(4 * kWave), 0, stream, a);
     else
-        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, kPagedRowWaves<NB>, true>), dim3(rows),
-                           dim3(kPagedRowWaves<NB> * kWave), 0, stream, a);
+        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, kPagedRowWaves<FMT, NB>, true>), dim3(rows),
+                           dim3(kPagedRowWaves<FMT, NB> * kWave), 0, stream, a);
     return hipGetLastError();
 }
 template <int FMT, int NB>
