@@ -1001,9 +1001,10 @@ hipError_t launch_paged_attention_f16(hipStream_t stream, const PagedAttnParams&
 hipError_t launch_paged_attention_q8_0(hipStream_t stream, const PagedAttnParams& a);
 hipError_t launch_paged_attention_q4_0(hipStream_t stream, const PagedAttnParams& a);
 
-// Wavefronts of a workgroup that takes a whole row of more than two steps for four:
+inline constexpr uint32_t kFewRows = 256;  // a workgroup a CU
+// Wavefronts of a workgroup that takes one of few rows whole, of more than two steps for four:
 // as many as the registers let stay, but six of f16 rows, whose 32 positions are twice
-// the bytes (256 rows of up to 500 of 128 dims 24 us for 27 with eight; 100 Q8_0 rows of
+// the bytes (256 rows of up to 500 of 256 dims 24 us for 27 with eight; 100 Q8_0 rows of
 // up to 1500 the other way, 23 for 20).
 template <int FMT, int NB>
 inline constexpr int kPagedRowWaves = NB <= 2 ? 16 : FMT == kKvF16 ? 6 : 8;
@@ -1013,7 +1014,7 @@ hipError_t launch_paged_heads(hipStream_t stream, const PagedAttnParams& a) {
     const uint32_t rows = a.sequences * a.kv_heads * a.head_tiles;
     if (a.row_units == 0)
         hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, 4, false>), dim3(a.most_parts), dim3(4 * kWave), 0, stream, a);
-    else if (a.row_units <= 8)
+    else if (a.row_units <= 8 || rows > kFewRows)
         hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, 4, true>), dim3(rows), dim3(4 * kWave), 0, stream, a);
     else
         hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, kPagedRowWaves<FMT, NB>, true>), dim3(rows),

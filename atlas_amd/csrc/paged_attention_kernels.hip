@@ -127,24 +127,32 @@ PagedPlan paged_plan(const PagedCache& c, uint32_t q_heads) {
 }
 
 // The units that a row has at most, where a workgroup a row is sooner done than
-// parts and their join; 0 where it is not.  Both by what was measured, in KB and us:
-// a workgroup takes 48 KB/us, or its share of the chip's 5500; parts have the whole
-// chip whatever the rows, but cost 4 us more with the join, and 8 more where they are
-// small and many.  Whole / parts, us: 256 windows of 512 f16 (256 dims) 33 / 52, f32 65
-// / 81, Q8_0 22 / 38; 64 of them f16 24 / 30; 2048 rows of up to 500 f16 (128 dims) 88 /
-// 114; 2000 of up to 100 Q8_0 (64) 15 / 39; 64 rows of up to 1024 f16 (128) 17 / 21, of
-// 4096 49 / 31; one of 64 f32 (128) 6 / 10; 3 of 2048 f32 (64) 25 / 11; one of 1024 Q8_0
-// (256) 24 / 13.  Long rows end at different times and are always split.
+// parts and their join; 0 where it is not.
+//
+// Of up to 256 rows by what was measured, in KB and us: a workgroup takes 48 KB/us, or
+// its share of the chip's 5500; parts have the whole chip whatever the rows, but cost 4
+// us more with the join, and 8 more where they are small and many.  Whole / parts, us:
+// 256 windows of 512 f16 (256 dims) 32 / 52, f32 65 / 81, Q8_0 22 / 38; 64 of them f16 24
+// / 30; 64 rows of up to 1024 f16 (128) 17 / 21, of 4096 49 / 31; one of 64 f32 (128) 6 /
+// 10; 3 of 2048 f32 (64) 25 / 11; one of 1024 Q8_0 (256) 24 / 13.
+//
+// More rows are many workgroups of four wavefronts, which hide one another's beginnings
+// and ends, up to 700 KB a row (400 of up to 600 f16 (256 dims) 42 / 58, 2000 of up to
+// 100 Q8_0 (64) 15 / 39); the longest of longer ones ends alone (300 of up to 2000 Q8_0
+// (256) 70 / 59, 512 of up to 1400 f16 110 / 108).
 uint32_t whole_row_units(const PagedCache& c, uint32_t window, uint64_t rows) {
     const uint32_t unit = paged_keys(c.format);
     uint64_t positions = static_cast<uint64_t>(c.table_width) * c.page_size;
     if (window && window < positions) positions = window + unit;  // it may begin and end inside units
     const double row_kb = 2e-3 * positions * paged_part_bytes(c.format, c.page_size, c.head_dim) / c.page_size;
-    if (row_kb > 1500.0) return 0;
-    const double busy = rows < 256 ? static_cast<double>(rows) : 256.0, share = 5500.0 / busy;
-    const double whole = static_cast<double>((rows + 255) / 256) * row_kb / (share < 48.0 ? share : 48.0);
-    const double parts = 4.0 + 8.0 * (rows < 64 ? rows / 64.0 : 1.0) + rows * row_kb / 5500.0;
-    return whole < parts ? static_cast<uint32_t>((positions + unit - 1) / unit) : 0;
+    bool whole = row_kb <= 700.0;
+    if (rows <= kFewRows) {
+        const double share = 5500.0 / rows;
+        whole = row_kb / (share < 48.0 ? share : 48.0) < 4.0 + 8.0 * (rows < 64 ? rows / 64.0 : 1.0) + rows * row_kb / 5500.0;
+        whole = whole && row_kb <= 1500.0;
+    }
+    whole = whole && positions <= static_cast<uint64_t>(unit) * kPartUnits;  // as many additions as in a part
+    return whole ? static_cast<uint32_t>((positions + unit - 1) / unit) : 0;
 }
 
 }  // namespace

@@ -361,3 +361,30 @@ def test_two_graphs_with_a_workspace_each():
     finally:
         for rt in rts:
             rt.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D", range(32, 257, 32))
+def test_more_rows_than_workgroups_at_once(rt, fmt, D):
+    """More than 256 rows, whole and of several steps each, empty ones among them."""
+    for group, KH in ((2, 3), (8, 2), (20, 1)):
+        B = 320 // KH if group < 16 else 140  # 20 heads are two rows
+        args = spread(D + group, fmt, group * KH, KH, D, 16, 20, [(53 * i) % 321 for i in range(B)])
+        say(f"{fmt} {D} group {group}")
+        got = run(rt, fmt, *args, 0, D ** -0.5)
+        assert (got[args[3] == 0] == 0).all()
+        check(f"{fmt} {D}", fmt, *args, 0, D ** -0.5, got)
+
+
+def test_many_long_rows_of_small_heads(rt):
+    """Rows of few bytes and many positions are cut where a wavefront would add too many of them up."""
+    H, KH, D, ps, n = 257, 257, 4, 4096, 20000
+    pool = ref.Pool("f32", 1, ps, KH, D)
+    row = np.random.default_rng(1).standard_normal((2, KH, 1, D)).astype(f32)
+    pool.bytes = np.ascontiguousarray(np.broadcast_to(row, (2, KH, ps, D))).view(np.uint8).reshape(pool.bytes.shape)
+    table = np.zeros((1, -(-n // ps)), u32)
+    q = np.random.default_rng(2).standard_normal((1, H, D)).astype(f32)
+    got = run(rt, "f32", pool, table, q, np.array([n], u32), 0, 0.5).astype(np.float64)
+    off = np.abs(got[0] - row[1, :, 0]) / np.abs(row[1, :, 0])
+    say(f"{off.max():.2e} of each value")
+    assert off.max() <= 3.5e-5 and np.linalg.norm(got[0] - row[1, :, 0]) <= 1e-5 * np.linalg.norm(row[1])
