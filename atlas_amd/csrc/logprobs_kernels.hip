@@ -299,10 +299,14 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
     const SliceSums* slices = v.slices + static_cast<uint64_t>(row) * v.count;
     const float* cells = v.cells + static_cast<uint64_t>(row) * v.strips * kCells;
     const uint32_t cells_of_row = v.strips * kCells;
+    // the table is filled while the first loads are on their way
+    const float first_cell = threadIdx.x < cells_of_row ? cells[threadIdx.x] : -__builtin_inff();
+    const uint32_t idle = s.top ? kWave : 0;  // threads that look for the border instead
+    SliceSums first_slice{0.0, 0.0};
+    if (threadIdx.x >= idle && threadIdx.x - idle < v.count) first_slice = slices[threadIdx.x - idle];
+    __builtin_amdgcn_sched_barrier(0);
     Exp2::fill(table);
     const Exp2 exp2_of(table);
-
-    const float first_cell = threadIdx.x < cells_of_row ? cells[threadIdx.x] : -__builtin_inff();
     float mine = first_cell;
     for (uint32_t i = threadIdx.x + THREADS; i < cells_of_row; i += THREADS) mine = fmaxf(mine, cells[i]);
     const float wtop = wave_max_tree_f32(mine);
@@ -322,9 +326,8 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
         const uint32_t border = s.top <= 24 ? border_of<1, THREADS>(group_top, lane, s.top) : border_of<4, THREADS>(group_top, lane, s.top);
         if (lane == 0) border_room = max(border, 1u);
     } else {
-        const uint32_t summing = s.top ? THREADS - kWave : THREADS;
-        for (uint32_t i = threadIdx.x - (THREADS - summing); i < v.count; i += summing) {
-            const SliceSums x = slices[i];
+        for (uint32_t i = threadIdx.x - idle; i < v.count; i += THREADS - idle) {
+            const SliceSums x = i + idle < THREADS ? first_slice : slices[i];
             float slice_top = -__builtin_inff();
             // the last slice may have a strip less
             for (uint32_t j = i * v.each * kCells; j < min((i + 1) * v.each * kCells, cells_of_row); j += 4) {
