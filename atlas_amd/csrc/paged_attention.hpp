@@ -243,14 +243,17 @@ __device__ __forceinline__ void f16_pieces(float x, _Float16& hi, _Float16& lo) 
 // Products of f16 (v_mfma_f32_16x16x32_f16): keys and values as they are, the
 // other factor as two f16 numbers, brought near f16's largest by a power of two
 // that the sums are divided by.  A query's pieces lose 2^-24 of each number, or
-// 2^-39 of the row's largest; a weight's 2^-24, or 2^-40.
+// 2^-39 of the row's largest; a weight's 2^-24, or 2^-40.  A value's load has 16 bytes a
+// lane: the address unit takes 17 cycles for any of whole rows (65 for a key's), and
+// twice the loads of 8 took 32.2 us for 30.2 (256 windows of 512 of 256 dims).
 template <int NB>
 struct Step<kKvF16, NB, 16> {
-    static constexpr int kTiles = 2, kOut = 2 * NB, kQuads = NB / 2, kQueryBytes = 2 * NB * kWave * 16;
+    static constexpr int kTiles = 2, kOut = 2 * NB, kEights = NB / 4, kFours = NB % 4 / 2, kQueryBytes = 2 * NB * kWave * 16;
     static constexpr float kUnscale = 0x1p-15f;
     static constexpr uint32_t kItemsPadded = 4 * NB;
     u32x4_t k[2][NB];
-    u32x2_t v[8][kQuads ? kQuads : 1];
+    u32x4_t v[8][kEights ? kEights : 1];  // eight dims a lane of runs of 128, then four of one of 64, two of one of 32
+    u32x2_t v4[8];
     uint32_t v2[8];
     __device__ __forceinline__ void load_keys(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t head_dim) {
 #pragma unroll
@@ -268,12 +271,16 @@ struct Step<kKvF16, NB, 16> {
             const PageRows& rows = p[j / 4];
             const uint32_t line = (4 * g + j % 4) * head_dim * 2;
 #pragma unroll
-            for (int u = 0; u < kQuads; ++u) {
-                const uint32_t dim = 64 * u + 4 * c;
-                v[j][u] = load8(rows.values, dim < head_dim ? line + dim * 2 : kPastPage, rows.row * head_dim * 2);
+            for (int u = 0; u < kEights; ++u) {
+                const uint32_t dim = 128 * u + 8 * c;
+                v[j][u] = load16(rows.values, dim < head_dim ? line + dim * 2 : kPastPage, rows.row * head_dim * 2);
+            }
+            if constexpr (kFours) {
+                const uint32_t dim = 128 * kEights + 4 * c;
+                v4[j] = load8(rows.values, dim < head_dim ? line + dim * 2 : kPastPage, rows.row * head_dim * 2);
             }
             if constexpr (NB % 2) {
-                const uint32_t dim = 64 * kQuads + 2 * c;
+                const uint32_t dim = 32 * (NB - 1) + 2 * c;
                 v2[j] = load4(rows.values, dim < head_dim ? line + dim * 2 : kPastPage, rows.row * head_dim * 2);
             }
         }
@@ -304,7 +311,8 @@ struct Step<kKvF16, NB, 16> {
         for (int j = 0; j < 8; ++j) {
             const uint32_t mask = seen[j / 4][j % 4] ? 0xffffffffu : 0u;
 #pragma unroll
-            for (int u = 0; u < kQuads; ++u) v[j][u] &= mask;
+            for (int u = 0; u < kEights; ++u) v[j][u] &= mask;
+            if constexpr (kFours) v4[j] &= mask;
             if constexpr (NB % 2) v2[j] &= mask;
         }
     }
@@ -331,22 +339,29 @@ struct Step<kKvF16, NB, 16> {
             o += sum;
         };
 #pragma unroll
-        for (int u = 0; u < kQuads; ++u)
+        for (int i = 0; i < NB; ++i) {  // the words that a lane holds of a row
+            uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = v[j][u][i];
-                one(column<0>(w), out[4 * u + 2 * i]);
-                one(column<1>(w), out[4 * u + 2 * i + 1]);
-            }
-        if constexpr (NB % 2) {
-            one(column<0>(v2), out[4 * kQuads]);
-            one(column<1>(v2), out[4 * kQuads + 1]);
+            for (int j = 0; j < 8; ++j)
+                w[j] = i < 4 * kEights ? v[j][i / 4 % (kEights ? kEights : 1)][i % 4] : i < 4 * kEights + 2 * kFours ? v4[j][i % 2] : v2[j];
+            one(column<0>(w), out[2 * i]);
+            one(column<1>(w), out[2 * i + 1]);
         }
     }
-    static __device__ __forceinline__ void put(float* line, uint32_t c, uint32_t g, const f32x4 (&out)[kOut]) {
-        Step<kKvF32, NB, 16>::put(line, c, g, out);
+    // O^T has dims in its rows: tile 2 i + e row k is dim 2 i + e of the lane's run k
+    static __device__ __forceinline__ void put(float* line, uint32_t, uint32_t g, const f32x4 (&out)[kOut]) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t k = 4 * g + r;
+#pragma unroll
+            for (int i = 0; i < 4 * kEights; i += 2)
+                *reinterpret_cast<f32x4*>(line + i / 4 * 128 + 8 * k + i % 4 * 2) = f32x4{out[2 * i][r], out[2 * i + 1][r], out[2 * i + 2][r], out[2 * i + 3][r]};
+            if constexpr (kFours) {
+                constexpr int i = 4 * kEights;
+                *reinterpret_cast<f32x4*>(line + 32 * i + 4 * k) = f32x4{out[2 * i][r], out[2 * i + 1][r], out[2 * i + 2][r], out[2 * i + 3][r]};
+            }
+            if constexpr (NB % 2) *reinterpret_cast<f32x2_t*>(line + 32 * (NB - 1) + 2 * k) = f32x2_t{out[2 * NB - 2][r], out[2 * NB - 1][r]};
+        }
     }
     static __device__ constexpr uint32_t query_dim(uint32_t j) { return j; }
 };
