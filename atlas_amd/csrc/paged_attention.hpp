@@ -414,38 +414,37 @@ struct Step {
             *to = HP < 16 && head / HP % 2 ? lo : hi;
             if constexpr (HP == 16) to[64] = lo;
         } else if (head < 8) {
-            to += (block / 2 * 2 + quarter % 2) * 128 + (block % 2 * 2 + quarter / 2) * 16 + head;
-            const uint32_t mine = block % 2 * 8, others = 8 - mine;
+            to += (block % kSpans * 2 + quarter % 2) * 128 + (block / kSpans * 2 + quarter / 2) * 16 + head;
+            const uint32_t mine = block / kSpans * 8, others = 8 - mine;
             to[mine] = hi;
             to[mine + 64] = lo;
             to[others] = to[others + 64] = f16x8_t{};
         }
+    }
+    // Of a lane's blocks, one behind the other, two at a time.  Behind a row's blocks lie other rows', or nothing: the
+    // columns that take those are no block's, and no one reads them.
+    template <int BLOCKS>
+    static __device__ __forceinline__ void load_scales(__amdgpu_buffer_rsrc_t rs, uint32_t page_shift, uint32_t row, uint32_t g,
+                                                       uint32_t block, u32x2_t (&s)[BLOCKS]) {
+        const uint32_t base = (kRow << page_shift) + row / 4 * NB * 8, off = (g * NB + block) * 8;
+#pragma unroll
+        for (int i = 0; i + 1 < BLOCKS; i += 2) {
+            const u32x4_t x = load16(rs, off + 8 * i, base);
+            s[i] = u32x2_t{x[0], x[1]};
+            s[i + 1] = u32x2_t{x[2], x[3]};
+        }
+        if constexpr (BLOCKS % 2) s[BLOCKS - 1] = load8(rs, off + 8 * (BLOCKS - 1), base);
     }
     __device__ __forceinline__ void load_keys(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t page_shift) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int i = 0; i < kKeySteps; ++i) {
-                const uint32_t in_row = i * 64 + 16 * g;
-                const uint32_t off = (i + 1) * 64 <= kRow || in_row < kRow ? c * kRow + in_row : kPastPage;
+                const uint32_t in_row = kExchanged ? i * 64 + 16 * g : (g / 2 * kSpans + i) * 32 + g % 2 * 16;
+                const uint32_t off = (kExchanged ? (i + 1) * 64 <= kRow : NB % 2 == 0) || in_row < kRow ? c * kRow + in_row : kPastPage;
                 k[h][i] = load16(p[h].keys, off, p[h].row * kRow);
             }
-            const uint32_t base = (kRow << page_shift) + p[h].row / 4 * NB * 8, off = g * NB * 8;
-            if constexpr (kExchanged) {
-#pragma unroll
-                for (int b = 0; b + 1 < NB; b += 2) {
-                    const u32x4_t x = load16(p[h].keys, off + 8 * b, base);
-                    ks[h][b] = u32x2_t{x[0], x[1]};
-                    ks[h][b + 1] = u32x2_t{x[2], x[3]};
-                }
-                if constexpr (NB % 2) ks[h][NB - 1] = load8(p[h].keys, off + 8 * (NB - 1), base);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kSpans; ++i) {
-                    const uint32_t b = 2 * i + c / 8;
-                    ks[h][i] = load8(p[h].keys, 2 * (i + 1) <= NB || b < NB ? off + 8 * b : kPastPage, base);
-                }
-            }
+            load_scales(p[h].keys, page_shift, p[h].row, g, kExchanged ? 0 : c / 8 * kSpans, ks[h]);
         }
     }
     __device__ __forceinline__ void load_values(const PageRows (&p)[2], uint32_t c, uint32_t g, uint32_t page_shift) {
@@ -476,14 +475,7 @@ struct Step {
             }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t base = (kRow << page_shift) + p[h].row / 4 * NB * 8, block = c / HP;
-#pragma unroll
-            for (int i = 0; i < kValueSteps; ++i) {
-                const bool there = (i + 1) * kValueBlocks <= NB || block + i * kValueBlocks < NB;
-                vs[h][i] = load8(p[h].values, there ? (g * NB + block + i * kValueBlocks) * 8 : kPastPage, base);
-            }
-        }
+        for (int h = 0; h < 2; ++h) load_scales(p[h].values, page_shift, p[h].row, g, c / HP * kValueSteps, vs[h]);
     }
     // Eight codes of a key as f16: 1024 + (a code without its sign) has it in its low
     // bits, or 16 times it four bits higher up.  Written out where the compiler makes
@@ -540,7 +532,7 @@ struct Step {
         }
         return w;
     }
-    __device__ __forceinline__ void scores(const uint8_t* queries, uint32_t, float unscale, f32x4 (&s)[2]) const {
+    __device__ __forceinline__ void scores(const uint8_t* queries, uint32_t c, float unscale, f32x4 (&s)[2]) const {
         s[0] = s[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < kKeySteps; ++i) {
@@ -565,8 +557,12 @@ struct Step {
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
+                {
+                    u32x2_t scale = ks[h][b];
+                    if (kSpan == 2 && NB % 2 && b == kSpans - 1 && c >= 8) scale = u32x2_t{0, 0};  // no block's
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[h][r] = __builtin_fmaf(d[h][r], scale_of(ks[h][b], r), s[h][r]);
+                    for (int r = 0; r < 4; ++r) s[h][r] = __builtin_fmaf(d[h][r], scale_of(scale, r), s[h][r]);
+                }
                 if (kSpan == 2 || j % 2) __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -653,7 +649,7 @@ struct Step {
             }
             // columns of other blocks hold what no one reads
 #pragma unroll
-            for (int b = step * kValueBlocks; b < (step + 1) * kValueBlocks && b < NB; ++b)
+            for (int b = step; b < NB; b += kValueSteps)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const bf16x8_t x = value_codes(b, e);
@@ -669,7 +665,7 @@ struct Step {
     static __device__ __forceinline__ void put(float* line, uint32_t c, uint32_t g, const f32x4 (&out)[kOut]) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
-            if (c / HP == b % kValueBlocks)
+            if (c / HP == b / kValueSteps)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     *reinterpret_cast<f32x2_t*>(line + 32 * b + 8 * g + 2 * r) = f32x2_t{out[2 * b][r], out[2 * b + 1][r]};

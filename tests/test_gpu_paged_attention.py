@@ -388,3 +388,24 @@ def test_many_long_rows_of_small_heads(rt):
     off = np.abs(got[0] - row[1, :, 0]) / np.abs(row[1, :, 0])
     say(f"{off.max():.2e} of each value")
     assert off.max() <= 3.5e-5 and np.linalg.norm(got[0] - row[1, :, 0]) <= 1e-5 * np.linalg.norm(row[1])
+
+
+@pytest.mark.parametrize("fmt", ["q8_0", "q4_0"])
+@pytest.mark.parametrize("D", range(32, 257, 32))
+def test_scales_of_rows_behind_the_last(rt, fmt, D):
+    """Whatever lies in a page behind a sequence's last row, scales that are no numbers too: any number of blocks, of 3, 8
+    and 16 heads."""
+    for group in (3, 8, 16):
+        for n in (1, 5, 16, 20, 28):
+            pool, table, q, lengths = spread(D + n, fmt, group * 2, 2, D, 16, 4, [n, 3])
+            rows, clean = ref.Pool(fmt, len(pool.bytes), 16, 2, D), pool.bytes
+            rows.bytes = np.full_like(clean, 0xFF)
+            for b, length in enumerate(lengths):
+                for p in range(int(length)):
+                    for part, src in zip(rows.bytes[table[b, p // 16]].reshape(4, -1), clean[table[b, p // 16]].reshape(4, -1)):
+                        at, scales = rows._spots(p % 16)
+                        part[at] = src[at]
+                        for s in scales:
+                            part[s:s + 2] = src[s:s + 2]
+            got = run(rt, fmt, rows, table, q, lengths, 0, D ** -0.5)
+            assert np.array_equal(got, run(rt, fmt, pool, table, q, lengths, 0, D ** -0.5)), (group, n)
