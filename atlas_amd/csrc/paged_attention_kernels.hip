@@ -132,12 +132,12 @@ PagedPlan paged_plan(const PagedCache& c, uint32_t q_heads) {
 // Of up to 256 rows by what was measured, in KB and us: a workgroup takes 48 KB/us, or
 // its share of the chip's 5500; parts have the whole chip whatever the rows, but cost 4
 // us more with the join, and 8 more where they are small and many.  Whole / parts, us:
-// 256 windows of 512 f16 (256 dims) 32 / 52, f32 65 / 81, Q8_0 22 / 38; 64 of them f16 24
-// / 30; 64 rows of up to 1024 f16 (128) 17 / 21, of 4096 49 / 31; one of 64 f32 (128) 6 /
+// 256 windows of 512 f16 (256 dims) 30 / 52, f32 65 / 81, Q8_0 22 / 38; 64 of them f16 21
+// / 30; 64 rows of up to 1024 f16 (128) 15 / 21, of 4096 49 / 31; one of 64 f32 (128) 6 /
 // 10; 3 of 2048 f32 (64) 25 / 11; one of 1024 Q8_0 (256) 24 / 13.
 //
 // More rows are many workgroups of four wavefronts, which hide one another's beginnings
-// and ends, up to 700 KB a row (400 of up to 600 f16 (256 dims) 42 / 58, 2000 of up to
+// and ends, up to 700 KB a row (400 of up to 600 f16 (256 dims) 38 / 58, 2000 of up to
 // 100 Q8_0 (64) 15 / 39); the longest of longer ones ends alone (300 of up to 2000 Q8_0
 // (256) 70 / 59, 512 of up to 1400 f16 110 / 108).
 uint32_t whole_row_units(const PagedCache& c, uint32_t window, uint64_t rows) {
