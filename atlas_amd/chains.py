@@ -545,15 +545,28 @@ class PagedDecode:
             for i in range(n):
                 self.table[place, have[place] + i] = self.free.pop()
 
+    def _rows(self, layers) -> list:
+        """A prompt's keys and values as f32 rows, of as many tokens in every layer."""
+        S = self.S
+        rows = [[np.asarray(x, np.float32) for x in pair] for pair in layers]
+        tokens = rows[0][0].shape[:1] if rows and rows[0] else ()
+        if len(rows) != S.layers or any(len(pair) != 2 for pair in rows) or any(
+                x.shape[:1] != tokens or x.size != len(x) * S.kv_heads * S.head_dim for pair in rows for x in pair):
+            raise ValueError("a prompt has keys and values [tokens, kv_heads, head_dim] for every layer")
+        return [[x.reshape(len(x), S.kv_heads, S.head_dim) for x in pair] for pair in rows]
+
     def begin(self, prompts) -> None:
         """Sequences for free places: {place: per layer (keys, values) [tokens, kv_heads, head_dim]}."""
         rt, S = self.rt, self.S
-        tokens = {place: layers[0][0].shape[0] for place, layers in prompts.items()}
-        for place, n in tokens.items():
+        for place in prompts:
+            if not 0 <= place < S.sequences:
+                raise ValueError(f"there is no place {place}")
             if self.lengths[place]:
                 raise ValueError(f"place {place} has a sequence")
-            if not n:
-                raise ValueError("a prompt has no token")
+        rows = {place: self._rows(layers) for place, layers in prompts.items()}
+        tokens = {place: len(layers[0][0]) for place, layers in rows.items()}
+        if not all(tokens.values()):
+            raise ValueError("a prompt has no token")
         if not tokens:
             return
         self._grow(tokens)
@@ -565,7 +578,7 @@ class PagedDecode:
         self.dev["table"].upload(self.table)
         held = [rt.upload(np.array(places, np.uint32)), rt.upload(np.array(positions, np.uint32))]
         for layer in range(S.layers):
-            k, v = (np.concatenate([p[layer][i].reshape(-1, S.kv_heads, S.head_dim) for p in prompts.values()]) for i in (0, 1))
+            k, v = (np.concatenate([p[layer][i] for p in rows.values()]) for i in (0, 1))
             held += [rt.upload(k), rt.upload(v)]
             rt.paged_append(self.caches[layer], held[-2], held[-1], None, None, self.dev["cos"], self.dev["sin"],
                             self.width * S.page_size, S.head_dim // 2, held[0], held[1], len(places), 0)

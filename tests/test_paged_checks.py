@@ -206,3 +206,80 @@ def test_a_failed_recording_leaves_no_graph_behind():
     with pytest.raises(ValueError, match="no"):
         chain.capture()
     assert chain.graph is None and not chain.rt.live
+
+
+class Nothing:
+    """A runtime that no one may call."""
+
+    def __getattr__(self, name):
+        raise AssertionError(f"{name} was called")
+
+
+def chain_of(rt, lengths, table, free, **shape):
+    """A chain without a device: its sequences, their pages and the pool's."""
+    chain = object.__new__(PagedDecode)
+    chain.rt, chain.S = rt, PagedShape(sequences=len(lengths), **shape)
+    chain.lengths, chain.table, chain.free = np.array(lengths, np.uint32), np.array(table, np.uint32), list(free)
+    return chain
+
+
+def rows_of(n, heads=3, dim=64, dtype=np.float32):
+    return np.zeros((n, heads, dim), dtype)
+
+
+@pytest.mark.parametrize("prompts,what", [
+    ({0: [(rows_of(9), rows_of(9)), (rows_of(9), rows_of(8))]}, "every layer"),        # values of fewer tokens
+    ({0: [(rows_of(9), rows_of(9)), (rows_of(8), rows_of(9))]}, "every layer"),        # keys of fewer
+    ({0: [(rows_of(9), rows_of(9)), (rows_of(10), rows_of(10))]}, "every layer"),      # a layer of more
+    ({0: [(rows_of(9), rows_of(9))]}, "every layer"),                                  # a layer less
+    ({0: [(rows_of(9), rows_of(9))] * 3}, "every layer"),
+    ({0: []}, "every layer"),
+    ({0: [(rows_of(9),)] * 2}, "every layer"),
+    ({0: [(rows_of(9, heads=2), rows_of(9, heads=2))] * 2}, "every layer"),
+    ({0: [(rows_of(9, dim=32), rows_of(9, dim=32))] * 2}, "every layer"),
+    # one prompt's more make up for the other's less
+    ({0: [(rows_of(9), rows_of(9)), (rows_of(8), rows_of(8))], 1: [(rows_of(9), rows_of(9)), (rows_of(10), rows_of(10))]}, "every layer"),
+    ({-1: [(rows_of(9), rows_of(9))] * 2}, "no place"),
+    ({2: [(rows_of(9), rows_of(9))] * 2}, "no place"),
+])
+def test_prompts_that_do_not_match_are_refused(prompts, what):
+    """What would be read behind a layer's rows, or stored for another sequence, changes nothing."""
+    chain = chain_of(Nothing(), [0, 0], [[ref.NO] * 4] * 2, [3, 2, 1, 0], layers=2, capacity=64, pages=4)
+    with pytest.raises(ValueError, match=what):
+        chain.begin(prompts)
+    assert not chain.lengths.any() and (chain.table == ref.NO).all() and chain.free == [3, 2, 1, 0]
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32, np.float64])
+def test_prompts_go_up_as_f32_rows(dtype):
+    """Every buffer of an append has the bytes that the call reads, whatever the prompt's type."""
+    class Runtime:
+        def __init__(self):
+            self.appended = []
+
+        def upload(self, host):
+            return np.ascontiguousarray(host)
+
+        def paged_append(self, cache, key, value, query, query_out, cos, sin, rope_rows, rope_stride, ids, positions, tokens, heads):
+            assert key.nbytes == value.nbytes == 4 * tokens * 3 * 64 and ids.nbytes == positions.nbytes == 4 * tokens
+            self.appended.append((key, value))
+
+        def sync(self):
+            pass
+
+        def free(self, buf):
+            pass
+
+    rt = Runtime()
+    chain = chain_of(rt, [0, 0, 0], [[ref.NO] * 4] * 3, [5, 4, 3, 2, 1, 0], layers=2, capacity=64, pages=6)
+    chain.width, chain.caches = 4, [None, None]
+    chain.dev = {"table": type("Table", (), {"upload": lambda self, host: None})(), "cos": None, "sin": None}
+    r = np.random.default_rng(1)
+    first, second = ([tuple(r.integers(-9, 9, (n, 3, 64)).astype(dtype) for _ in range(2)) for _ in range(2)] for n in (17, 5))
+    second = [tuple(x.reshape(5, 192) for x in pair) for pair in second]  # heads side by side
+    chain.begin({2: first, 0: second})
+    assert chain.lengths.tolist() == [5, 0, 17] and len(chain.free) == 3
+    for layer, pair in enumerate(rt.appended):
+        for i in range(2):
+            exp = np.concatenate([first[layer][i], second[layer][i].reshape(5, 3, 64)])
+            assert pair[i].dtype == np.float32 and np.array_equal(pair[i], exp.astype(np.float32))
