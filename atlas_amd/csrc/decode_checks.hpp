@@ -225,6 +225,8 @@ inline const char* token_logprobs_error(const TokenLogprobsArgs& a) {
     if (!a.logits || !a.workspace || (a.given && (!a.tokens || !a.logprobs)) || (a.top && (!a.top_ids || !a.top_logprobs)))
         return "log probability buffer is null";
     if (a.given == 0 && a.top == 0 && !a.entropy) return "no log probabilities asked for";
+    // a thread counts to `given` and a workgroup further, in 32 bits
+    if (a.given > kMostPositions) return "log probabilities are limited to 2^29 given tokens a row";
     if (a.row_stride < a.vocab) return "rows of logits overlap";
     if (!std::isfinite(a.inv_temperature) || !(a.inv_temperature > 0.0)) return "inv_temperature must be finite and positive";
     if (misaligned(a.logits, 4) || misaligned(a.tokens, 4) || misaligned(a.logprobs, 4) || misaligned(a.entropy, 4) ||

@@ -283,3 +283,9 @@ def test_prompts_go_up_as_f32_rows(dtype):
         for i in range(2):
             exp = np.concatenate([first[layer][i], second[layer][i].reshape(5, 3, 64)])
             assert pair[i].dtype == np.float32 and np.array_equal(pair[i], exp.astype(np.float32))
+
+
+@pytest.mark.parametrize("given,fine", [(1, True), (1 << 29, True), ((1 << 29) + 1, False), (0xFFFFFC00, False), (0xFFFFFFFF, False)])
+def test_given_tokens_that_a_thread_can_count(checks, given, fine):
+    """A count past 2^32 begins again at zero, and a loop up to a larger number never ends."""
+    assert (call(checks.check_logprobs, LOGPROBS, dict(given=given)) is None) == fine
