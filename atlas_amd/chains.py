@@ -503,6 +503,7 @@ class PagedDecode:
         self.scale = 1.0 / wl.f32_sqrt(D)
         self.width = -(-S.capacity // S.page_size)
         self.lengths = np.zeros(B, np.uint32)                       # 0: no sequence there
+        self.stepped = np.zeros(B, bool)                            # whose next position the step has
         self.table = np.full((B, self.width), self.NO_PAGE, np.uint32)
         self.free = list(range(S.pages - 1, -1, -1))
         self.layers = [{"q": wl.normal(r, B * H * D), "k": wl.normal(r, B * KH * D), "v": wl.normal(r, B * KH * D)}
@@ -592,6 +593,7 @@ class PagedDecode:
         self.free.extend(int(p) for p in pages[::-1])
         self.table[place] = self.NO_PAGE
         self.lengths[place] = 0
+        self.stepped[place] = False
 
     def set_step(self, logits) -> None:
         """The step's logits [sequences, vocab]; pages for its positions."""
@@ -602,6 +604,7 @@ class PagedDecode:
         d["positions"].upload(np.where(active, self.lengths, 0xFFFFFFFF).astype(np.uint32))
         d["lengths"].upload(np.where(active, self.lengths + 1, 0).astype(np.uint32))
         d["logits"].upload(logits)
+        self.stepped = active
 
     def enqueue(self) -> None:
         rt, S, d, o = self.rt, self.S, self.dev, self.out
@@ -618,9 +621,10 @@ class PagedDecode:
                           self.logprobs_bytes)
 
     def advance(self) -> np.ndarray:
-        """The tokens of the step that ran; the sequences grow by them."""
+        """The tokens of the step that ran; its sequences grow by them, those that began behind set_step() do not."""
         tokens = self.out["tokens"].download(self.S.sequences, np.uint32)
-        self.lengths = np.where(self.lengths > 0, self.lengths + 1, 0).astype(np.uint32)
+        self.lengths = self.lengths + self.stepped.astype(np.uint32)
+        self.stepped = np.zeros(self.S.sequences, bool)
         return tokens
 
     def capture(self) -> int:

@@ -289,3 +289,39 @@ def test_prompts_go_up_as_f32_rows(dtype):
 def test_given_tokens_that_a_thread_can_count(checks, given, fine):
     """A count past 2^32 begins again at zero, and a loop up to a larger number never ends."""
     assert (call(checks.check_logprobs, LOGPROBS, dict(given=given)) is None) == fine
+
+
+class Buffer:
+    def upload(self, host):
+        self.host = np.array(host)
+
+    def download(self, count, dtype):
+        return np.zeros(count, dtype)
+
+
+def stepping_chain(lengths):
+    chain = chain_of(Nothing(), lengths, [[i] + [ref.NO] * 3 if n else [ref.NO] * 4 for i, n in enumerate(lengths)], [9, 8, 7, 6, 5],
+                     capacity=64, pages=10, vocab=10)
+    chain.stepped = np.zeros(len(lengths), bool)
+    chain.dev = {k: Buffer() for k in ("table", "positions", "lengths", "logits")}
+    chain.out = {"tokens": Buffer()}
+    return chain
+
+
+def test_sequences_grow_by_the_steps_that_they_were_in():
+    """A sequence that begins between set_step and advance has no row of that step, nor has one whose place another took; a
+    second advance is of no step."""
+    chain = stepping_chain([3, 0, 15, 7])
+    chain.set_step(np.zeros((4, 10), np.float32))
+    assert chain.dev["positions"].host.tolist() == [3, ref.NO, 15, 7] and chain.dev["lengths"].host.tolist() == [4, 0, 16, 8]
+    chain.end(3)
+    chain.lengths[1], chain.lengths[3] = 4, 6  # begun: prompts of 4 and 6
+    chain.advance()
+    assert chain.lengths.tolist() == [4, 4, 16, 6]
+    chain.advance()
+    assert chain.lengths.tolist() == [4, 4, 16, 6]
+    chain.table[1, 0], chain.table[3, 0] = chain.free.pop(), chain.free.pop()
+    chain.set_step(np.zeros((4, 10), np.float32))
+    assert chain.dev["positions"].host.tolist() == [4, 4, 16, 6]
+    chain.advance()
+    assert chain.lengths.tolist() == [5, 5, 17, 7] and chain.lengths.dtype == np.uint32
