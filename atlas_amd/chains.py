@@ -534,14 +534,19 @@ class PagedDecode:
     def window(self, layer: int) -> int:
         return 0 if layer % 5 == 4 else self.S.window
 
-    def _grow(self, lengths: dict) -> None:
-        """Pages for the first positions of sequences, {place: positions}: of all or of none."""
+    def _need(self, lengths: dict) -> tuple[dict, dict]:
+        """The pages that sequences have and lack for their first positions, {place: positions}."""
         if any(n > self.S.capacity for n in lengths.values()):
             raise ValueError("a sequence has no room for its next position: end() it first")
         have = {place: int((self.table[place] != self.NO_PAGE).sum()) for place in lengths}
         need = {place: -(-n // self.S.page_size) - have[place] for place, n in lengths.items()}
         if sum(need.values()) > len(self.free):
             raise ValueError("the pool has no page left: end() a sequence first")
+        return have, need
+
+    def _grow(self, lengths: dict) -> None:
+        """Pages for the first positions of sequences: of all or of none."""
+        have, need = self._need(lengths)
         for place, n in need.items():
             for i in range(n):
                 self.table[place, have[place] + i] = self.free.pop()
@@ -598,7 +603,12 @@ class PagedDecode:
     def set_step(self, logits) -> None:
         """The step's logits [sequences, vocab]; pages for its positions."""
         active = self.lengths > 0
-        self._grow({int(place): int(self.lengths[place]) + 1 for place in np.nonzero(active)[0]})
+        lengths = {int(place): int(self.lengths[place]) + 1 for place in np.nonzero(active)[0]}
+        self._need(lengths)
+        logits = np.asarray(logits, np.float32)
+        if logits.size != self.S.sequences * self.S.vocab:
+            raise ValueError("a step has logits [sequences, vocab]")
+        self._grow(lengths)
         d = self.dev
         d["table"].upload(self.table)
         d["positions"].upload(np.where(active, self.lengths, 0xFFFFFFFF).astype(np.uint32))

@@ -325,3 +325,22 @@ def test_sequences_grow_by_the_steps_that_they_were_in():
     assert chain.dev["positions"].host.tolist() == [4, 4, 16, 6]
     chain.advance()
     assert chain.lengths.tolist() == [5, 5, 17, 7] and chain.lengths.dtype == np.uint32
+
+
+@pytest.mark.parametrize("logits", [np.zeros((3, 10)), np.zeros((4, 9), np.float32), np.zeros((2, 4, 10), np.float32), np.zeros(0), None])
+def test_a_step_without_its_logits_changes_nothing(logits):
+    """Fewer numbers than the step has would leave the last step's logits of other sequences in their place."""
+    chain = stepping_chain([16, 0, 5, 0])
+    table = chain.table.copy()
+    with pytest.raises(ValueError, match="logits"):
+        chain.set_step(logits)
+    assert (chain.table == table).all() and chain.free == [9, 8, 7, 6, 5] and not hasattr(chain.dev["table"], "host")
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32, np.float64])
+def test_a_steps_logits_go_up_as_f32(dtype):
+    chain = stepping_chain([16, 0, 5, 0])
+    x = (np.arange(40).reshape(4, 10) - 20).astype(dtype)
+    chain.set_step(x)
+    assert chain.dev["logits"].host.dtype == np.float32 and np.array_equal(chain.dev["logits"].host, x.astype(np.float32))
+    assert chain.table[0].tolist() == [0, 5, ref.NO, ref.NO] and chain.free == [9, 8, 7, 6]
