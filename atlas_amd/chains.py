@@ -581,16 +581,27 @@ class PagedDecode:
             self.lengths[place] = n
             places += [place] * n
             positions += range(n)
-        self.dev["table"].upload(self.table)
-        held = [rt.upload(np.array(places, np.uint32)), rt.upload(np.array(positions, np.uint32))]
-        for layer in range(S.layers):
-            k, v = (np.concatenate([p[layer][i] for p in rows.values()]) for i in (0, 1))
-            held += [rt.upload(k), rt.upload(v)]
-            rt.paged_append(self.caches[layer], held[-2], held[-1], None, None, self.dev["cos"], self.dev["sin"],
-                            self.width * S.page_size, S.head_dim // 2, held[0], held[1], len(places), 0)
-        rt.sync()
-        for b in held:
-            rt.free(b)
+        held = []
+
+        def up(x):
+            held.append(rt.upload(x))
+            return held[-1]
+
+        try:
+            self.dev["table"].upload(self.table)
+            ids, at = up(np.array(places, np.uint32)), up(np.array(positions, np.uint32))
+            for layer in range(S.layers):
+                k, v = (up(np.concatenate([p[layer][i] for p in rows.values()])) for i in (0, 1))
+                rt.paged_append(self.caches[layer], k, v, None, None, self.dev["cos"], self.dev["sin"], self.width * S.page_size,
+                                S.head_dim // 2, ids, at, len(places), 0)
+            rt.sync()
+        except BaseException:
+            for place in tokens:  # rows of some layers are no sequence
+                self.end(place)
+            raise
+        finally:
+            for b in held:  # a free waits for the appends
+                rt.free(b)
 
     def end(self, place: int) -> None:
         """The sequence's pages go back to the pool."""

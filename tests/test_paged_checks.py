@@ -344,3 +344,39 @@ def test_a_steps_logits_go_up_as_f32(dtype):
     chain.set_step(x)
     assert chain.dev["logits"].host.dtype == np.float32 and np.array_equal(chain.dev["logits"].host, x.astype(np.float32))
     assert chain.table[0].tolist() == [0, 5, ref.NO, ref.NO] and chain.free == [9, 8, 7, 6]
+
+
+@pytest.mark.parametrize("call_that_fails", range(1, 10))
+def test_prompts_that_could_not_be_stored_leave_no_sequence(call_that_fails):
+    """A device without memory, or a call that fails half-way through the layers: pages and buffers come back."""
+    class Runtime:
+        calls, live = 0, 0
+
+        def step(self):
+            self.calls += 1
+            if self.calls == call_that_fails:
+                raise RuntimeError("no memory")
+
+        def upload(self, host):
+            self.step()
+            self.live += 1
+            return object()
+
+        def paged_append(self, *args):
+            self.step()
+
+        def sync(self):
+            self.step()
+
+        def free(self, buf):
+            self.live -= 1
+
+    chain = chain_of(Runtime(), [0, 3, 0], [[ref.NO] * 4, [9, ref.NO, ref.NO, ref.NO], [ref.NO] * 4], [5, 4, 3, 2, 1, 0], layers=2,
+                     capacity=64, pages=10)
+    chain.width, chain.caches, chain.stepped = 4, [None, None], np.array([False, True, False])
+    chain.dev = {"table": Buffer(), "cos": None, "sin": None}
+    with pytest.raises(RuntimeError, match="no memory"):
+        chain.begin({2: [(rows_of(17), rows_of(17))] * 2, 0: [(rows_of(5), rows_of(5))] * 2})
+    assert chain.rt.live == 0 and chain.lengths.tolist() == [0, 3, 0] and sorted(chain.free) == list(range(6))
+    assert chain.table[1].tolist() == [9] + [ref.NO] * 3 and (chain.table[[0, 2]] == ref.NO).all()
+    assert chain.stepped.tolist() == [False, True, False]
