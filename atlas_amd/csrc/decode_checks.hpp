@@ -28,6 +28,11 @@ constexpr uint32_t kMostSequences = 1u << 20;
 // A launch has less than 2^32 threads: 256 of them to each of these.
 constexpr uint32_t kMostGroups = 1u << 23;
 
+// The kernels take a scale with log2(e) in it, which has to be a number of f32 still.
+inline const char* attention_scale_error(float scale) {
+    return std::isfinite(scale * 1.44269504f) ? nullptr : "attention scale must be finite, and at most 2.3e38";
+}
+
 inline const char* prefix_attention_sizes_error(const PrefixAttentionArgs& a) {
     if (a.format != kKvF32 && a.format != kKvQ8_0 && a.format != kKvQ4_0) return "unknown cache format";
     if (a.sequences == 0 || a.tokens == 0 || a.q_heads == 0 || a.kv_heads == 0 || a.q_heads % a.kv_heads != 0)
@@ -52,7 +57,7 @@ inline const char* prefix_attention_error(const PrefixAttentionArgs& a) {
     if (a.capacity && (!a.cache || !a.lengths)) return "prefix attention own cache or lengths are null";
     if (a.weights_out && !a.capacity) return "attention weights need own rows";
     if (a.weights_in && !a.weights_out) return "weights_in without weights_out";
-    if (!std::isfinite(a.scale)) return "attention scale must be finite";
+    if (const char* error = attention_scale_error(a.scale)) return error;
     if (misaligned(a.q, 16) || misaligned(a.output, 16) || misaligned(a.workspace, 16))
         return "prefix attention q, output and workspace must be 16-byte aligned";
     const uintptr_t to = a.format == kKvF32 ? 16 : 2;
@@ -204,7 +209,7 @@ inline const char* paged_attention_error(const PagedAttentionArgs& a) {
     if (const char* error = paged_cache_error(a.cache)) return error;
     if (const char* error = paged_attention_sizes_error(a.cache, a.q_heads)) return error;
     if (!a.q || !a.lengths || !a.output || !a.workspace) return "paged attention buffer is null";
-    if (!std::isfinite(a.scale)) return "attention scale must be finite";
+    if (const char* error = attention_scale_error(a.scale)) return error;
     if (misaligned(a.q, 16) || misaligned(a.output, 16) || misaligned(a.workspace, 16) || misaligned(a.lengths, 4))
         return "paged attention q, output and workspace must be 16-byte aligned, lengths 4-byte";
     const uint64_t bytes = 4ull * a.cache.sequences * a.q_heads * a.cache.head_dim;

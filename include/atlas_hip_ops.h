@@ -415,7 +415,7 @@ int atlas_hip_kv_append_q4_0(atlas_hip_ctx *ctx, const float *key, const float *
  *
  * head_dim is at most 256 and a multiple of 4 (f32) or 32 (Q8_0, Q4_0);
  * kv_heads divides q_heads; q, output, f32 caches and the workspace are
- * 16-byte aligned, quantised caches 2-byte; output does not overlap q.
+ * 16-byte aligned, quantised caches 2-byte; output does not overlap q; |scale| <= 2.3e38.
  * sequences * tokens * q_heads <= 2^23, prefix_length and capacity <= 2^29,
  * sequences * capacity < 2^32, kv_heads * head_dim <= 32768.  What a row does
  * not see never reaches it, whatever it holds; what it sees has to be finite,
@@ -557,8 +557,8 @@ int atlas_hip_paged_read(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, con
  * which moves its weight by a factor; with F16 a weight is off by up to 2^-40 of its
  * row's largest; apart from that a result is within 1e-5 of float64 normwise, at any
  * number of positions.  A call's result does not depend on timing.  q, output and the
- * workspace are 16-byte aligned; output overlaps neither q nor the pages; sequences *
- * q_heads <= 2^23, sequences * kv_heads * table_width * page_size <= 2^34, a KV head of
+ * workspace are 16-byte aligned; output overlaps neither q nor the pages; |scale| <=
+ * 2.3e38; sequences * q_heads <= 2^23, sequences * kv_heads * table_width * page_size <= 2^34, a KV head of
  * more than 16 query heads counting once for every 16.  The workspace
  * (atlas_hip_paged_attention_workspace bytes; no pointer of the struct is read) is
  * overwritten by every call and holds nothing between calls: calls that can overlap,

@@ -102,3 +102,8 @@ def test_verify_calls_that_are_allowed(checks, change):
     dict(sequences=1 << 20, drafts=1024, vocab=4096)])
 def test_verify_calls_that_are_refused(checks, change):
     assert call(checks.check_verify_draft, VERIFY, change)
+
+
+@pytest.mark.parametrize("scale,fine", [(2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False)])
+def test_scales_that_are_no_number_with_their_logarithm(checks, scale, fine):
+    assert (call(checks.check_prefix_attention, ATTEND, dict(scale=scale)) is None) == fine

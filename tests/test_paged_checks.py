@@ -380,3 +380,9 @@ def test_prompts_that_could_not_be_stored_leave_no_sequence(call_that_fails):
     assert chain.rt.live == 0 and chain.lengths.tolist() == [0, 3, 0] and sorted(chain.free) == list(range(6))
     assert chain.table[1].tolist() == [9] + [ref.NO] * 3 and (chain.table[[0, 2]] == ref.NO).all()
     assert chain.stepped.tolist() == [False, True, False]
+
+
+@pytest.mark.parametrize("scale,fine", [(2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False)])
+def test_scales_that_are_no_number_with_their_logarithm(checks, scale, fine):
+    """f32's largest number over log2(e) is 2.36e38: what is larger made infinities of every query and NaN of every zero."""
+    assert (call(checks.check_attention, ATTEND, dict(scale=scale)) is None) == fine
