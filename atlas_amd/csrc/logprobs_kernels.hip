@@ -6,8 +6,9 @@
 //   S = sum_i e^{y_i},  log p_i = y_i - log S,
 //   entropy = -sum_i p_i log p_i = log S + sum_i e^{y_i} (-y_i) / S,
 // where every term is positive: nothing cancels.  Probabilities and sums are in
-// 64 bits, so a likely token's small log probability keeps its digits.  NaN and
-// -inf logits have no mass; all of a row's mass lies on its +inf.
+// 64 bits, and S is kept as what it has beside the top's own 1: of a likely token
+// that is its log probability, which so keeps its digits however small it is.  NaN
+// and -inf logits have no mass; all of a row's mass lies on its +inf.
 //
 // Launches: a wavefront a slice of one or two strips of 1024 logits leaves the slice's sums and the
 // maxima of its cells, 128 logits each; one workgroup a row joins them.  The
@@ -34,11 +35,15 @@ constexpr int kEach = kStrip / kWave;
 constexpr uint32_t kNoToken = 0xffffffffu;
 constexpr uint32_t kCellList = 1024, kTokenList = 512;
 
-// A slice's sums of e^{y} and of e^{y} (-y), relative to its top, y in thirty-seconds
-// of powers of two.
+// A slice's sums of e^{y}, less its top's own 1, and of e^{y} (-y), relative to its
+// top, y in thirty-seconds of powers of two.
 struct SliceSums {
-    double sum, spread;
+    double rest, spread;
 };
+// Sums that hold a 1 lose what is below its last bit, which matters where there is
+// little else: less than this in every lane, the top's apart.  (More of it in the sum,
+// and 45 additions move it by 2^-39 at most.)
+constexpr double kLittle = 0x1p-8;
 
 struct LogprobParams {
     TokenLogprobsArgs s;
@@ -170,6 +175,22 @@ __global__ __launch_bounds__(kLogThreads, 8) void logprob_sums_kernel(LogprobPar
             }
         // here, and not behind the next logits' loads, beside which these would have to be kept
         asm volatile("" : "+v"(sum), "+v"(spread));
+        const bool has_top = sum >= 1.0;
+        const bool little = __builtin_popcountll(__builtin_amdgcn_ballot_w64(has_top)) == 1 &&
+                            __builtin_amdgcn_ballot_w64((has_top ? sum - 1.0 : sum) > kLittle) == 0;
+        if (little) {  // the top's lane again, without it
+            double rest = 0.0;
+#pragma unroll
+            for (int i = 0; i < STRIPS; ++i)
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) {
+                    asm volatile("" : "+v"(x[i][j]), "+v"(rest));  // one by one, and no power kept from above
+                    const double y = fmax((static_cast<double>(x[i][j]) - zero) * scale, exp2_of.least), e = exp2_of(y);
+                    rest += y == 0.0 ? 0.0 : e;
+                }
+            asm volatile("" : "+v"(rest));
+            if (has_top) sum = rest;
+        }
         float* cells = v.cells + static_cast<uint64_t>(row) * v.strips * kCells;
         const uint32_t strip = slice * STRIPS;
         row += row_step;
@@ -181,7 +202,7 @@ __global__ __launch_bounds__(kLogThreads, 8) void logprob_sums_kernel(LogprobPar
         if (item + step < items) load();
         sum = wave_sum_f64(sum);
         if (SPREAD) spread = wave_sum_f64(spread);
-        if (lane == 0) v.slices[at] = SliceSums{sum, spread * (1.0 / 8.0)};
+        if (lane == 0) v.slices[at] = SliceSums{little ? sum : sum - 1.0, spread * (1.0 / 8.0)};
         if (lane % 8 == 0)
 #pragma unroll
             for (uint32_t i = 0; i < STRIPS; ++i)
@@ -250,6 +271,13 @@ __device__ uint64_t exact_border(const LogprobParams& v, const float* logits, co
     return state;
 }
 
+// log(1 + r), r >= 0, to 2^-42 of it: where 1 + r would lose more, five terms of its series.
+// (The library's log1p takes 0.3 us more of a row.)
+__device__ __forceinline__ double log_one_and(double r) {
+    if (r >= kLittle) return log(1.0 + r);
+    return r * __builtin_fma(r, __builtin_fma(r, __builtin_fma(r, __builtin_fma(r, 1.0 / 5.0, -1.0 / 4.0), 1.0 / 3.0), -1.0 / 2.0), 1.0);
+}
+
 // The s.top-th largest of 64 EACH groups' maxima, to 21 bits of its place, by one wavefront.
 template <int EACH, int THREADS>
 __device__ __forceinline__ uint32_t border_of(const float (&maxima)[THREADS], uint32_t lane, uint32_t k) {
@@ -281,9 +309,9 @@ template <int THREADS>
 __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) {
     constexpr uint32_t kWaves = THREADS / kWave;
     __shared__ uint2 table[32];
-    __shared__ double wave_sum[kWaves], wave_spread[kWaves];
+    __shared__ double wave_rest[kWaves], wave_spread[kWaves];
     __shared__ float wave_top[kWaves], group_top[THREADS];
-    __shared__ uint32_t border_room, cell_count, token_count, left_room;
+    __shared__ uint32_t border_room, cell_count, token_count, top_count, left_room;
     __shared__ uint64_t state_room;
     __shared__ union {
         struct {
@@ -312,7 +340,7 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
     const float wtop = wave_max_tree_f32(mine);
     if (lane == 0) wave_top[wave] = wtop;
     group_top[threadIdx.x] = mine;
-    if (threadIdx.x == 0) cell_count = token_count = 0;
+    if (threadIdx.x == 0) cell_count = token_count = top_count = 0;
     __syncthreads();
     float top = wave_top[0];
 #pragma unroll
@@ -320,7 +348,7 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
 
     // one wavefront finds the border while the others sum
     const bool finds = s.top && wave == 0;
-    double sum = 0.0, spread = 0.0;
+    double rest = 0.0, spread = 0.0;
     if (finds) {
         // 64 groups do for few tokens: 20 of them leave some 24 above the border
         const uint32_t border = s.top <= 24 ? border_of<1, THREADS>(group_top, lane, s.top) : border_of<4, THREADS>(group_top, lane, s.top);
@@ -336,31 +364,36 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
             }
             const double y = fmax((static_cast<double>(about(slice_top, top)) - finite(top)) * v.scale, exp2_of.least);
             const double f = exp2_of(y);
-            sum = __builtin_fma(f, x.sum, sum);
-            spread = __builtin_fma(f, __builtin_fma(-y, x.sum, x.spread), spread);
+            rest = __builtin_fma(f, x.rest, rest);
+            if (f == 1.0)
+                atomicAdd(&top_count, 1u);  // a slice with the row's top, or as good as it
+            else
+                rest += f;
+            spread = __builtin_fma(f, __builtin_fma(-y, 1.0 + x.rest, x.spread), spread);
         }
-        sum = wave_sum_f64(sum);
+        rest = wave_sum_f64(rest);
         spread = wave_sum_f64(spread);
     }
     if (lane == 0) {
-        wave_sum[wave] = sum;
+        wave_rest[wave] = rest;
         wave_spread[wave] = spread;
     }
     __syncthreads();
-    sum = spread = 0.0;
+    rest = spread = 0.0;
     for (uint32_t w = 0; w < kWaves; ++w) {
-        sum += wave_sum[w];
+        rest += wave_rest[w];
         spread += wave_spread[w];
     }
+    rest += static_cast<double>(top_count) - 1.0;
     const bool any = top > -__builtin_inff();
-    const double log_sum = any ? log(sum) : 0.0;
+    const double log_sum = any ? log_one_and(rest) : 0.0;
     const auto logprob = [&](float x) {
         const double y = (static_cast<double>(about(number_or_none(x), top)) - finite(top)) * s.inv_temperature - log_sum;
-        return any ? static_cast<float>(y) : -__builtin_inff();
+        return any ? static_cast<float>(y) + 0.0f : -__builtin_inff();  // not -0
     };
     if (s.entropy && threadIdx.x == 0)
         // thirty-seconds of powers of two to natural units
-        s.entropy[row] = any ? static_cast<float>(log_sum + spread / sum * (0x1.62e42fefa39efp-1 / 32.0)) : 0.0f;
+        s.entropy[row] = any ? static_cast<float>(log_sum + spread / (1.0 + rest) * (0x1.62e42fefa39efp-1 / 32.0)) : 0.0f;
     for (uint32_t i = threadIdx.x; i < s.given; i += THREADS) {
         const uint64_t at = static_cast<uint64_t>(row) * s.given + i;
         const uint32_t token = s.tokens[at];

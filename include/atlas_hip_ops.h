@@ -658,10 +658,11 @@ int atlas_hip_verify_draft_f32(atlas_hip_ctx *ctx, const float *target_logits, c
  * given and top may be 0, their buffers NULL then, but something is asked for.
  * NaN and -inf logits have no mass and a log probability of -inf; all of a row's mass
  * lies on its +inf; a row without mass has entropy 0.  Probabilities and sums are
- * float64, in a fixed order; results are rounded to f32 once.  At most 2^29 logits a
- * row, 2^29 given and 64 likeliest tokens, and 2^23 times 4096 logits in all (a row
- * counts in whole 4096s).  Outputs overlap neither inputs nor each other.  Workspace as for
- * paged_attention. */
+ * float64, in a fixed order, within 2^-38 of themselves, those that are all but 0
+ * (a token of nearly all the mass, and the entropy of its row) too; results are
+ * rounded to f32 once.  At most 2^29 logits a row, 2^29 given and 64 likeliest
+ * tokens, and 2^23 times 4096 logits in all (a row counts in whole 4096s).  Outputs
+ * overlap neither inputs nor each other.  Workspace as for paged_attention. */
 int atlas_hip_token_logprobs_workspace(atlas_hip_ctx *ctx, uint32_t rows, uint32_t vocab, uint32_t top,
                                        uint64_t *bytes);
 int atlas_hip_token_logprobs_f32(atlas_hip_ctx *ctx, const float *logits, uint64_t row_stride, const uint32_t *tokens,

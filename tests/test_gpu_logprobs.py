@@ -226,3 +226,32 @@ def test_replays(rt):
         rt.argmax(dl, dt, R, V)
         rt.sync()
     rt.graph_destroy(graph)
+
+
+@pytest.mark.parametrize("vocab,R", [(1, 3), (2, 3), (60, 3), (1000, 3), (3000, 3), (50257, 2), (16385, 600)])
+@pytest.mark.parametrize("ahead", [0.5, 5.5, 9.0, 12.0, 25.0, 40.0, 70.0, 100.0])
+def test_log_probabilities_near_zero(rt, vocab, R, ahead):
+    """A token so likely that the others' mass is far below the last bit of 1: its log probability is that mass, of its own
+    size, and so is the entropy.  f32's half a step; masses and sums are within 2^-38 (2^-45 a power, 2^-52 |y| its
+    argument, 45 additions of 2^-53 each of sums 2^8 times as large as what is left)."""
+    say(f"{R} x {vocab}, {ahead} ahead")
+    x = rows(vocab, R, vocab, std=1.0)
+    best = np.random.default_rng(int(ahead)).integers(0, vocab, R)
+    best[0], best[-1] = 0, vocab - 1
+    x[np.arange(R), best] = x.max(1) + f32(ahead)
+    x[:, 7::50] = -np.inf
+    x[np.arange(R), best] = np.where(np.isinf(x[np.arange(R), best]), f32(5 + ahead), x[np.arange(R), best])
+    if R > 3:
+        x[5, :] = -np.inf
+        x[5, best[5]] = 3.0  # alone
+        x[6, (best[6] + 1) % vocab] = x[6, best[6]]  # two of them
+    tokens = best.reshape(R, 1).astype(u32)
+    for inv in (1.0, 1.0 / 0.7):
+        got, exp = run(rt, x, vocab, tokens, inv, 2), ref.logprobs(x, tokens, inv, 2)
+        assert np.array_equal(got[2], exp[2])
+        for what, g, e in (("logprobs", got[0], exp[0]), ("entropy", got[1], exp[1]), ("tops", got[3], exp[3])):
+            same = np.isinf(e) | np.isinf(g)
+            assert np.array_equal(g[same], e[same].astype(f32)), what
+            assert not np.signbit(g[g == 0]).any(), f"{what}: -0"
+            off, tol = np.abs(g[~same] - e[~same]), np.abs(e[~same]) * (2.0 ** -24 + 2.0 ** -38) + 2.0 ** -149
+            assert (off <= tol).all(), f"{what}: {float((off / tol).max()):.3g} of the tolerance"
