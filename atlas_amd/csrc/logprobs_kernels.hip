@@ -19,7 +19,7 @@
 // logits 52 to 54 us in the first launch, 5.0 TB/s (random numbers are read at 5.8 at
 // best), and 8.5 in the second; 2048 of 50257 82 to 84 and 7.
 #include "exp2_f64.hpp"
-#include "launch.hpp"
+#include "logprobs_plan.hpp"
 
 #include <algorithm>
 #include <limits>
@@ -27,9 +27,6 @@
 namespace atlas {
 namespace {
 
-constexpr int kLogThreads = 256;
-constexpr int kLogWaves = kLogThreads / kWave;
-constexpr uint32_t kStrip = 1024;  // 16 logits a lane
 constexpr uint32_t kCells = 8;     // of a strip: the logits of eight lanes
 constexpr int kEach = kStrip / kWave;
 constexpr uint32_t kNoToken = 0xffffffffu;
@@ -302,9 +299,7 @@ __device__ __forceinline__ uint32_t border_of(const float (&maxima)[THREADS], ui
     return border;
 }
 
-// One workgroup a row, of 1024 threads where the rows do not fill the chip by
-// themselves: its steps wait for one another and for memory (256 rows of 262144
-// logits, 20 tokens each, 10 us with 256 threads).
+// One workgroup a row (row_threads).
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) {
     constexpr uint32_t kWaves = THREADS / kWave;
@@ -444,17 +439,6 @@ __global__ __launch_bounds__(THREADS) void logprob_rows_kernel(LogprobParams v) 
     }
 }
 
-constexpr uint32_t kGroups = 256 * 8;
-
-uint32_t strips_of(uint32_t vocab) { return (vocab + kStrip - 1) / kStrip; }
-// Two strips to a slice halve what a slice costs beside its logits; one where that
-// leaves CUs idle (one row of 49152 logits 4.7 -> 4.0 us).
-uint32_t strips_each(uint32_t rows, uint32_t vocab) { return static_cast<uint64_t>(rows) * strips_of(vocab) >= 256 * 32 ? 2 : 1; }
-uint32_t slices_of(uint32_t rows, uint32_t vocab) {
-    const uint32_t each = strips_each(rows, vocab);
-    return (strips_of(vocab) + each - 1) / each;
-}
-
 }  // namespace
 
 uint64_t token_logprobs_workspace(uint32_t rows, uint32_t vocab, uint32_t) {
@@ -471,14 +455,13 @@ hipError_t launch_token_logprobs(hipStream_t stream, const TokenLogprobsArgs& s)
     v.count = slices_of(s.rows, s.vocab);
     v.each = strips_each(s.rows, s.vocab);
     v.cells = reinterpret_cast<float*>(v.slices + static_cast<uint64_t>(s.rows) * v.count);
-    const uint64_t items = (static_cast<uint64_t>(s.rows) * v.count + kLogWaves - 1) / kLogWaves;
-    const dim3 grid(static_cast<uint32_t>(items < kGroups ? items : kGroups)), block(kLogThreads);
+    const dim3 grid(sum_groups(s.rows, s.vocab)), block(kLogThreads);
     const auto sums = s.entropy ? (v.each == 2 ? logprob_sums_kernel<true, 2> : logprob_sums_kernel<true, 1>)
                                 : (v.each == 2 ? logprob_sums_kernel<false, 2> : logprob_sums_kernel<false, 1>);
     hipLaunchKernelGGL(sums, grid, block, 0, stream, v);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (s.rows <= 512)
+    if (row_threads(s.rows) == 1024)
         hipLaunchKernelGGL(logprob_rows_kernel<1024>, dim3(s.rows), dim3(1024), 0, stream, v);
     else
         hipLaunchKernelGGL(logprob_rows_kernel<256>, dim3(s.rows), dim3(256), 0, stream, v);

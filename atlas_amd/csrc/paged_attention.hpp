@@ -22,17 +22,9 @@
 #pragma once
 
 #include "attention_lanes.hpp"
-#include "paged_layout.hpp"
+#include "paged_plan.hpp"
 
 namespace atlas {
-
-inline constexpr uint32_t kPagedAttnWaves = 4;  // of a workgroup that takes a part
-inline constexpr uint32_t kPagedHeads = 16;  // query heads of a row: the columns of a product
-
-// The first and last part of a row.
-struct PagedRow {
-    uint32_t first, last;
-};
 
 struct PagedAttnParams {
     const float* q;
@@ -50,12 +42,6 @@ struct PagedAttnParams {
     uint32_t few_parts, most_parts, part_units;  // parts of all work; units of a part where there are more than few_parts
     float scale;                                 // with log2(e)
 };
-
-// Keys of a wavefront's step, the unit of the split: two tiles of 16 where a
-// product over keys takes 32.
-__host__ __device__ constexpr uint32_t paged_keys(int format) { return format == kKvF32 ? 16 : 32; }
-// Workgroups to a CU.
-__host__ __device__ constexpr uint32_t paged_occupancy(uint32_t head_dim) { return head_dim <= 64 ? 4 : (head_dim <= 128 ? 3 : 2); }
 
 // The positions that a sequence's token sees, and their units.
 struct SeenRange {
@@ -1012,24 +998,18 @@ hipError_t launch_paged_attention_f16(hipStream_t stream, const PagedAttnParams&
 hipError_t launch_paged_attention_q8_0(hipStream_t stream, const PagedAttnParams& a);
 hipError_t launch_paged_attention_q4_0(hipStream_t stream, const PagedAttnParams& a);
 
-inline constexpr uint32_t kFewRows = 256;  // a workgroup a CU
-// Wavefronts of a workgroup that takes one of few rows whole, of more than two steps for four:
-// as many as the registers let stay, but six of f16 rows, whose 32 positions are twice
-// the bytes (256 rows of up to 500 of 256 dims 24 us for 27 with eight; 100 Q8_0 rows of
-// up to 1500 the other way, 23 for 20).
-template <int FMT, int NB>
-inline constexpr int kPagedRowWaves = NB <= 2 ? 16 : FMT == kKvF16 ? 6 : 8;
-
 template <int FMT, int NB, int HP>
 hipError_t launch_paged_heads(hipStream_t stream, const PagedAttnParams& a) {
     const uint32_t rows = a.sequences * a.kv_heads * a.head_tiles;
     if (a.row_units == 0)
-        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, 4, false>), dim3(a.most_parts), dim3(4 * kWave), 0, stream, a);
-    else if (a.row_units <= 8 || rows > kFewRows)
-        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, 4, true>), dim3(rows), dim3(4 * kWave), 0, stream, a);
+        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, kPagedAttnWaves, false>), dim3(a.most_parts),
+                           dim3(kPagedAttnWaves * kWave), 0, stream, a);
+    else if (paged_waves(FMT, NB, a.row_units, rows) == kPagedAttnWaves)
+        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, kPagedAttnWaves, true>), dim3(rows), dim3(kPagedAttnWaves * kWave),
+                           0, stream, a);
     else
-        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, kPagedRowWaves<FMT, NB>, true>), dim3(rows),
-                           dim3(kPagedRowWaves<FMT, NB> * kWave), 0, stream, a);
+        hipLaunchKernelGGL((paged_attention_kernel<FMT, NB, HP, paged_row_waves(FMT, NB), true>), dim3(rows),
+                           dim3(paged_row_waves(FMT, NB) * kWave), 0, stream, a);
     return hipGetLastError();
 }
 template <int FMT, int NB>

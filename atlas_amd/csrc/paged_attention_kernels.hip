@@ -1,6 +1,6 @@
-// paged_attention_kernels.hip -- attention over a cache in pages: how the work
-// is split, and the join of rows that were.  No counterpart in the reference,
-// whose executors decode one sequence from a contiguous cache.
+// paged_attention_kernels.hip -- attention over a cache in pages: its launches,
+// and the join of rows that were split.  No counterpart in the reference, whose
+// executors decode one sequence from a contiguous cache.
 #include "paged_attention.hpp"
 
 namespace atlas {
@@ -92,69 +92,6 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnParams a) 
     *reinterpret_cast<f32x4*>(out) = y;
 }
 
-constexpr uint32_t kJoinThreads = 256;
-
-// Additions to a wavefront's sums in a part, a unit each: with keys alike they all round to
-// one side, 2^-25 of the sum at most each.
-constexpr uint32_t kPartUnits = 256 * kPagedAttnWaves;
-constexpr uint32_t kMostParts = 1u << 20;
-
-uint64_t round256(uint64_t v) { return (v + 255) / 256 * 256; }
-
-struct PagedPlan {
-    uint32_t few_parts, most_parts, heads;
-    uint64_t out_bytes, ml_bytes, row_bytes;
-};
-
-PagedPlan paged_plan(const PagedCache& c, uint32_t q_heads) {
-    PagedPlan p{};
-    const uint32_t group = q_heads / c.kv_heads;
-    p.heads = group < kPagedHeads ? group : kPagedHeads;
-    const uint32_t unit = paged_keys(c.format);
-    const uint64_t capacity = static_cast<uint64_t>(c.table_width) * c.page_size;
-    const uint64_t rows = static_cast<uint64_t>(c.sequences) * c.kv_heads * ((group + kPagedHeads - 1) / kPagedHeads);
-    const uint64_t units = (capacity + unit - 1) / unit * rows;
-    p.few_parts = 256 * paged_occupancy(c.head_dim);
-    const uint64_t long_parts = (units + kPartUnits - 1) / kPartUnits;
-    uint64_t most = long_parts > p.few_parts ? long_parts : p.few_parts;
-    most = most < units ? most : units;
-    p.most_parts = static_cast<uint32_t>(most < kMostParts ? most : kMostParts);
-    const uint64_t lines = 2ull * p.most_parts * p.heads;
-    p.out_bytes = round256(lines * c.head_dim * 4);
-    p.ml_bytes = round256(lines * 8);
-    p.row_bytes = round256(rows * sizeof(PagedRow));
-    return p;
-}
-
-// The units that a row has at most, where a workgroup a row is sooner done than
-// parts and their join; 0 where it is not.
-//
-// Of up to 256 rows by what was measured, in KB and us: a workgroup takes 48 KB/us, or
-// its share of the chip's 5500; parts have the whole chip whatever the rows, but cost 4
-// us more with the join, and 8 more where they are small and many.  Whole / parts, us:
-// 256 windows of 512 f16 (256 dims) 30 / 52, f32 65 / 81, Q8_0 22 / 38; 64 of them f16 21
-// / 30; 64 rows of up to 1024 f16 (128) 15 / 21, of 4096 49 / 31; one of 64 f32 (128) 6 /
-// 10; 3 of 2048 f32 (64) 25 / 11; one of 1024 Q8_0 (256) 24 / 13.
-//
-// More rows are many workgroups of four wavefronts, which hide one another's beginnings
-// and ends, up to 700 KB a row (400 of up to 600 f16 (256 dims) 38 / 58, 2000 of up to
-// 100 Q8_0 (64) 15 / 39); the longest of longer ones ends alone (300 of up to 2000 Q8_0
-// (256) 70 / 59, 512 of up to 1400 f16 110 / 108).
-uint32_t whole_row_units(const PagedCache& c, uint32_t window, uint64_t rows) {
-    const uint32_t unit = paged_keys(c.format);
-    uint64_t positions = static_cast<uint64_t>(c.table_width) * c.page_size;
-    if (window && window < positions) positions = window + unit;  // it may begin and end inside units
-    const double row_kb = 2e-3 * positions * paged_part_bytes(c.format, c.page_size, c.head_dim) / c.page_size;
-    bool whole = row_kb <= 700.0;
-    if (rows <= kFewRows) {
-        const double share = 5500.0 / rows;
-        whole = row_kb / (share < 48.0 ? share : 48.0) < 4.0 + 8.0 * (rows < 64 ? rows / 64.0 : 1.0) + rows * row_kb / 5500.0;
-        whole = whole && row_kb <= 1500.0;
-    }
-    whole = whole && positions <= static_cast<uint64_t>(unit) * kPartUnits;  // as many additions as in a part
-    return whole ? static_cast<uint32_t>((positions + unit - 1) / unit) : 0;
-}
-
 }  // namespace
 
 uint64_t paged_attention_workspace(const PagedCache& c, uint32_t q_heads) {
@@ -183,7 +120,7 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
     a.capacity = c.table_width * c.page_size;
     a.kv_heads = c.kv_heads;
     a.group = s.q_heads / c.kv_heads;
-    a.head_tiles = (a.group + kPagedHeads - 1) / kPagedHeads;
+    a.head_tiles = paged_head_tiles(c, s.q_heads);
     a.heads = p.heads;
     a.q_heads = s.q_heads;
     a.head_dim = c.head_dim;
@@ -191,7 +128,7 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
     a.few_parts = p.few_parts;
     a.most_parts = p.most_parts;
     a.part_units = kPartUnits;
-    a.row_units = whole_row_units(c, s.window, c.sequences * c.kv_heads * a.head_tiles);
+    a.row_units = whole_row_units(c, s.window, paged_rows(c, s.q_heads));
     a.scale = s.scale * kLog2e;
     hipError_t e;
     switch (c.format) {
@@ -201,21 +138,15 @@ hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& 
         default: e = launch_paged_attention_q4_0(stream, a); break;
     }
     if (e != hipSuccess || a.row_units) return e;
-    const uint32_t lines = c.sequences * s.q_heads;
-    // Few rows have many parts: a workgroup for every 64 dims of one, and of 16 wavefronts; for every 32 where they
-    // have 128 and more (8 heads of 256 dims, 512 parts 34.1 us for 35.0; 32 parts the other way, 13.5 for 13.9).
-    if (lines < 64 && p.most_parts / (c.sequences * c.kv_heads * a.head_tiles) >= 128) {
-        hipLaunchKernelGGL((paged_join_kernel<8, 1024>), dim3(lines, (c.head_dim + 31) / 32), dim3(1024), 0, stream, a);
-        return hipGetLastError();
-    }
-    if (lines < 512) {
-        hipLaunchKernelGGL((paged_join_kernel<16, 1024>), dim3(lines, (c.head_dim + 63) / 64), dim3(1024), 0, stream, a);
-        return hipGetLastError();
-    }
-    const dim3 grid(lines), block(kJoinThreads);
-    if (c.head_dim <= 64)
+    const PagedJoin j = paged_join(c, s.q_heads, p.most_parts);
+    const dim3 grid(c.sequences * s.q_heads, j.groups), block(j.threads);
+    if (j.lanes == 8)
+        hipLaunchKernelGGL((paged_join_kernel<8, kFewThreads>), grid, block, 0, stream, a);
+    else if (j.threads == kFewThreads)
+        hipLaunchKernelGGL((paged_join_kernel<16, kFewThreads>), grid, block, 0, stream, a);
+    else if (j.lanes == 16)
         hipLaunchKernelGGL((paged_join_kernel<16, kJoinThreads>), grid, block, 0, stream, a);
-    else if (c.head_dim <= 128)
+    else if (j.lanes == 32)
         hipLaunchKernelGGL((paged_join_kernel<32, kJoinThreads>), grid, block, 0, stream, a);
     else
         hipLaunchKernelGGL((paged_join_kernel<64, kJoinThreads>), grid, block, 0, stream, a);
