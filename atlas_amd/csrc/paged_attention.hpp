@@ -229,7 +229,9 @@ __device__ __forceinline__ void f16_pieces(float x, _Float16& hi, _Float16& lo) 
 // Products of f16 (v_mfma_f32_16x16x32_f16): keys and values as they are, the
 // other factor as two f16 numbers, brought near f16's largest by a power of two
 // that the sums are divided by.  A query's pieces lose 2^-24 of each number, or
-// 2^-39 of the row's largest; a weight's 2^-24, or 2^-40.  A value's load has 16 bytes a
+// 2^-39 of the row's largest; a weight's 2^-24, or 2^-40.  (A product lines its terms up by
+// their operands' exponents, 2^-14 for all f16 numbers below it: of a weight of 2^15 such a
+// value loses what is below 2^-23, of a query's largest number such a key 2^-37.)  A value's load has 16 bytes a
 // lane: the address unit takes 17 cycles for any of whole rows (65 for a key's), and
 // twice the loads of 8 took 32.2 us for 30.2 (256 windows of 512 of 256 dims).
 template <int NB>

@@ -550,19 +550,29 @@ int atlas_hip_paged_read(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, con
  *   output = sum_j e^{x_j} v_j / sum_j e^{x_j};  zero where nothing is seen
  * q and output [sequences, q_heads, head_dim] f32; query head h reads KV head
  * h / (q_heads / kv_heads).  What a token does not see never reaches it, whatever it
- * holds; what it sees has to be finite.  Scores, weights and sums are f32; with F16,
- * Q8_0 and Q4_0 rows the products' other operands are two f16 numbers or three bf16
- * ones each, f32's bits.  A score is off by up to (head_dim + 24) 2^-24 of |scale|
- * sum_i |q_i k_i|, with those formats and 2^-38 of |scale| max_i |q_i| sum_i |k_i|,
- * which moves its weight by a factor; with F16 a weight is off by up to 2^-40 of its
- * row's largest; apart from that a result is within 1e-5 of float64 normwise, at any
- * number of positions.  A call's result does not depend on timing.  q, output and the
- * workspace are 16-byte aligned; output overlaps neither q nor the pages; |scale| <=
- * 2.3e38; sequences * q_heads <= 2^23, sequences * kv_heads * table_width * page_size <= 2^34, a KV head of
- * more than 16 query heads counting once for every 16.  The workspace
+ * holds; what it sees has to be finite, with scale * q, scores and sums of values below
+ * 2^126 (a row that sees anything else may be NaN in every dim).  Scores, weights and
+ * sums are f32; with F16, Q8_0 and Q4_0 rows the products' other operands are two f16
+ * numbers or three bf16 ones each, f32's bits.  A score is off by up to (head_dim + 24)
+ * 2^-24 of |scale| sum_i |q_i k_i|, with those formats and 2^-38 of |scale| max_i |q_i|
+ * sum_i |k_i|, which moves its weight by a factor; with F16 a weight is off by up to
+ * 2^-40 of its row's largest; apart from that a result is within 1e-5 of float64
+ * normwise, at any number of positions.  Of F16 rows with numbers below 2^-14 (their
+ * products are added with the digits of larger ones) a score is besides off by up to
+ * head_dim 2^-37 of |scale| max_i |q_i|, a result by up to 2^-33.  A weight below 2^-126
+ * of its row's largest is zero.  A call's result does not depend on timing.
+ *
+ * q, output and the workspace are 16-byte aligned; output overlaps neither q nor the
+ * pages; |scale| <= 2.3e38; sequences * q_heads <= 2^23, sequences * kv_heads *
+ * table_width * page_size <= 2^34, a KV head of more than 16 query heads counting once
+ * for every 16 -- and its rows are read once for every 16.  The workspace
  * (atlas_hip_paged_attention_workspace bytes; no pointer of the struct is read) is
  * overwritten by every call and holds nothing between calls: calls that can overlap,
- * and graphs whose replays can, need one each. */
+ * and graphs whose replays can, need one each.
+ *
+ * Whether rows are taken whole or cut, and into how many parts, goes by table_width *
+ * page_size and the window, not by the lengths, which are the device's: a batch of short
+ * sequences under a table as wide as a long context is cut. */
 int atlas_hip_paged_attention_workspace(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, uint32_t q_heads,
                                         uint64_t *bytes);
 int atlas_hip_paged_attention(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, const float *q,

@@ -409,3 +409,34 @@ def test_scales_of_rows_behind_the_last(rt, fmt, D):
                             part[s:s + 2] = src[s:s + 2]
             got = run(rt, fmt, rows, table, q, lengths, 0, D ** -0.5)
             assert np.array_equal(got, run(rt, fmt, pool, table, q, lengths, 0, D ** -0.5)), (group, n)
+
+
+@pytest.mark.parametrize("n", [2, 32, 64, 700])
+@pytest.mark.parametrize("most", [1, 60, 1023])
+def test_f16_numbers_below_the_normal_ones(rt, n, most):
+    """The matrix unit lines products up by their operands' exponents, which are 2^-14 for all f16 numbers below it, and
+    drops what is 2^-24 below the largest: of a weight of 1, held as 2^15, and such a value 2^(15 - 14 - 24) = 2^-23, which
+    is 2^-38 of the result for each of a step's 32 keys; of a query's largest number, held below 2^14, and such a key 2^-37
+    of it for each dim."""
+    r = np.random.default_rng(n + most)
+    pool, table, q, lengths = make(n, "f16", 8, 2, 64, 16, max(16, n), [n] * 3)
+    x = pool.bytes.view(np.float16).reshape(len(pool.bytes), 2, -1)
+    small = lambda shape: (r.integers(-most, most + 1, shape) * 2.0 ** -24).astype(np.float16)  # noqa: E731
+    keys = x[:, 0].copy()
+    x[:, 1] = small(keys.shape)
+    got = run(rt, "f16", pool, table, q, lengths, 0, 0.125)
+    exp = ref.attention(pool, table, q, lengths, 0, 0.125)
+    tol = ref.attention_bound("f16", pool, table, q, lengths, 0, 0.125, exp) + 2.0 ** -33
+    off = np.abs(got.astype(np.float64) - exp[0])
+    say(f"values {n} {most}: {float((off / tol).max()):.3f} of the bound, 2^{np.log2(off.max() + 1e-99):.1f}")
+    assert (off <= tol).all()
+    x[:, 0] = small(keys.shape)
+    x[:, 1] = keys
+    q *= f32(2.0 ** 14)
+    got = run(rt, "f16", pool, table, q, lengths, 0, 0.125)
+    exp = ref.attention(pool, table, q, lengths, 0, 0.125)
+    dx = 64 * 2.0 ** -37 * 0.125 * np.abs(q.astype(np.float64)).max(2)[..., None]
+    tol = ref.attention_bound("f16", pool, table, q, lengths, 0, 0.125, exp) + np.expm1(2 * dx) * exp[1]
+    off = np.abs(got.astype(np.float64) - exp[0])
+    say(f"keys {n} {most}: {float((off / tol).max()):.3f} of the bound")
+    assert (off <= tol).all()
