@@ -239,13 +239,17 @@ __global__ __launch_bounds__(kPagedThreads) void paged_append_kernel(PagedAppend
     }
 }
 
+// The rows that are asked for: of one output that is null neither is read.
+__host__ __device__ inline uint32_t read_begin(const PagedReadArgs& a) { return a.key ? 0 : a.cache.kv_heads; }
+__host__ __device__ inline uint32_t read_end(const PagedReadArgs& a) { return a.value ? 2 * a.cache.kv_heads : a.cache.kv_heads; }
+
 // Bound by what it writes, 4 bytes a value: 32768 rows of 8 heads of 128 dims from
 // Q4_0 48 us, 6.3 TB/s.
 template <int FMT, int LANES, bool PAST>
 __global__ __launch_bounds__(kPagedThreads) void paged_read_kernel(PagedReadArgs a, uint32_t shift, uint32_t chunks, uint32_t steps) {
     constexpr uint32_t kRows = kWave / LANES;
     const PagedCache& c = a.cache;
-    const uint32_t hd = c.head_dim, each = 2 * c.kv_heads;
+    const uint32_t hd = c.head_dim, begin = read_begin(a), end = read_end(a);  // of a token's rows, keys and then values
     const Share share = share_of(chunks, steps);
     if (share.token >= a.rows) return;
     const Place at = place_of(c, shift, a.sequences ? a.sequences[share.token] : share.token, a.positions[share.token]);
@@ -260,7 +264,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_read_kernel(PagedReadArgs
         uint32_t scale[kAtOnce];
 #pragma unroll
         for (int s = 0; s < kAtOnce; ++s) {
-            const uint32_t row = min((share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES, each - 1);
+            const uint32_t row = min(begin + (share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES, end - 1);
             const uint32_t plane = row < c.kv_heads ? 0 : 1;
             w[s] = u32x4_t{0, 0, 0, 0};
             scale[s] = 0;
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_read_kernel(PagedReadArgs
         if constexpr (paged_quantised(FMT)) {
 #pragma unroll
             for (int s = 0; s < kAtOnce; ++s) {
-                const uint32_t row = (share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES;
+                const uint32_t row = begin + (share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES;
                 uint8_t* codes = reinterpret_cast<uint8_t*>(rooms[threadIdx.x / kWave][s]) + threadIdx.x % kWave / LANES * LANES * 4;
                 // a key's four codes lie together, a value's two by two
                 const uint32_t q0 = row < c.kv_heads ? dim : p0, q1 = row < c.kv_heads ? dim + 2 : p1;
@@ -300,11 +304,10 @@ __global__ __launch_bounds__(kPagedThreads) void paged_read_kernel(PagedReadArgs
         }
 #pragma unroll
         for (int s = 0; s < kAtOnce; ++s) {
-            const uint32_t row = (share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES;
-            if (s0 + s >= steps || row >= each) continue;
+            const uint32_t row = begin + (share.first + s0 + s) * kRows + threadIdx.x % kWave / LANES;
+            if (s0 + s >= steps || row >= end) continue;
             const uint32_t plane = row < c.kv_heads ? 0 : 1;
             float* out = plane ? a.value : a.key;
-            if (!out) continue;
             f32x4 v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -350,7 +353,7 @@ hipError_t launch_append(hipStream_t stream, const PagedAppendArgs& a) {
 }
 template <int FMT, int LANES>
 hipError_t launch_read(hipStream_t stream, const PagedReadArgs& a) {
-    const uint32_t each = 2 * a.cache.kv_heads;
+    const uint32_t each = read_end(a) - read_begin(a);
     const Shares s(a.rows, each, kWave / LANES);
     const bool past = 4ull * a.rows * each * a.cache.head_dim > kCachedBytes;
     const auto kernel = past ? paged_read_kernel<FMT, LANES, true> : paged_read_kernel<FMT, LANES, false>;
