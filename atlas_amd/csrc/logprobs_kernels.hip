@@ -16,8 +16,8 @@
 // largest maximum is a border that k tokens reach, so only cells that reach it are
 // read again (some 25 of 2048 for 20 tokens) and what reaches it in them is ranked.
 // Bound by the bytes and nearly as much by the 64-bit instructions: 256 rows of 262144
-// logits 52 to 54 us in the first launch, 5.0 TB/s (random numbers are read at 5.8 at
-// best), and 8.5 in the second; 2048 of 50257 82 to 84 and 7.
+// logits 55 to 56 us in the first launch, 4.8 TB/s (random numbers are read at 5.8 at
+// best), and 8.3 in the second; 2048 of 50257 84 to 87 and 7.
 #include "exp2_f64.hpp"
 #include "logprobs_plan.hpp"
 

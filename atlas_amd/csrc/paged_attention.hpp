@@ -16,8 +16,8 @@
 //
 // Bound by its loads and, behind which they do not wholly hide, a step's chain of
 // products and conversions: 24 sequences of 1000 to 30001 Q8_0 positions, 8 KV heads of
-// 128 dims and 32 heads 172 us, 4.7 TB/s (the loads alone 5.8); 131072 f16 positions
-// of 256 dims 35 us with the join, 3.9 TB/s.  Q4_0 is bound by its unpacking: 261001
+// 128 dims and 32 heads 173 to 176 us, 4.6 TB/s (the loads alone 5.8); 131072 f16
+// positions of 256 dims 34 us with the join, 4.0 TB/s.  Q4_0 is bound by its unpacking: 261001
 // positions of 256 dims 28 us, 940 vector instructions of a wavefront for 32 positions.
 #pragma once
 

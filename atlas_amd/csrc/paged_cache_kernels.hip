@@ -16,7 +16,8 @@
 // token: where the token goes is known to the wavefront by scalar loads, and a
 // lane's angles serve all of its rows.  A rotating lane loads its partners' dims
 // too: the line is there, and nothing is exchanged.  Bound by bytes (4096 tokens of
-// 32 + 8 heads of 128 dims to f16 31 to 33 us, 5.7 TB/s read and written), and below a
+// 32 + 8 heads of 128 dims to f16 31 to 33 us, 5.7 TB/s read and written, to Q8_0 and Q4_0
+// 34, 5.2), and below a
 // few hundred tokens by the chain of its loads (position, table, store): 3 to 5 us.
 #include "device_common.hpp"
 #include "paged_layout.hpp"

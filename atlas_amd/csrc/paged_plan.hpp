@@ -90,8 +90,8 @@ inline uint32_t whole_row_units(const PagedCache& c, uint32_t window, uint64_t r
 
 // Wavefronts of a workgroup that takes one of few rows whole, of more than two steps for four:
 // as many as the registers let stay, but six of f16 rows, whose 32 positions are twice
-// the bytes (256 rows of up to 500 of 256 dims 24 us for 27 with eight; 100 Q8_0 rows of
-// up to 1500 the other way, 23 for 20).
+// the bytes (256 rows of up to 500 of 256 dims 22.6 us for 24.1 with eight, of 128 dims 11.5
+// for 12.3; 100 Q8_0 rows of up to 1500 the other way, 23 for 20).
 constexpr uint32_t paged_row_waves(int format, uint32_t blocks) { return blocks <= 2 ? 16 : format == kKvF16 ? 6 : 8; }
 inline uint32_t paged_waves(int format, uint32_t blocks, uint32_t row_units, uint64_t rows) {
     return row_units <= 2 * kPagedAttnWaves || rows > kFewRows ? kPagedAttnWaves : paged_row_waves(format, blocks);
