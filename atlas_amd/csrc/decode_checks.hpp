@@ -3,7 +3,7 @@
 #pragma once
 
 #include "launch.hpp"
-#include "paged_layout.hpp"
+#include "paged_plan.hpp"
 
 #include <cmath>
 #include <limits>
@@ -215,6 +215,19 @@ inline const char* paged_attention_error(const PagedAttentionArgs& a) {
     const uint64_t bytes = 4ull * a.cache.sequences * a.q_heads * a.cache.head_dim;
     if (spans_overlap(a.q, bytes, a.output, bytes) || spans_overlap(a.cache.pages, paged_pool_bytes(a.cache), a.output, bytes))
         return "paged attention output overlaps q or the pages";
+    // the second launch goes by what the first left in the workspace, and by the lengths that it went by
+    const struct {
+        const void* at;
+        uint64_t bytes;
+    } inputs[] = {{a.q, bytes},
+                  {a.cache.pages, paged_pool_bytes(a.cache)},
+                  {a.lengths, 4ull * a.cache.sequences},
+                  {a.cache.table, 4ull * a.cache.sequences * a.cache.table_width}};
+    const uint64_t room = paged_attention_workspace(a.cache, a.q_heads);
+    if (spans_overlap(a.output, bytes, a.workspace, room)) return "paged attention output overlaps the workspace";
+    for (const auto& x : inputs)
+        if (spans_overlap(x.at, x.bytes, a.workspace, room) || spans_overlap(x.at, x.bytes, a.output, bytes))
+            return "paged attention output or workspace overlaps its inputs";
     return nullptr;
 }
 

@@ -268,7 +268,6 @@ struct PagedAttentionArgs {
     float scale;
     void* workspace;
 };
-uint64_t paged_attention_workspace(const PagedCache& c, uint32_t q_heads);
 hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& a);
 
 // Log probabilities, entropies and likeliest tokens of rows of logits (logprobs_kernels.hip).

@@ -17,6 +17,7 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnParams a) 
     __shared__ float wave_top[kWaves];
     __shared__ f32x4 sums[kWaves][LANES];
     __shared__ float wave_l[kWaves];
+    const uint32_t last_part = a.most_parts - 1;
     const uint32_t seq = blockIdx.x / a.q_heads, q_head = blockIdx.x % a.q_heads;
     const uint32_t kv_head = q_head / a.group, in_group = q_head % a.group;
     const PagedRow row = a.rows[(static_cast<uint64_t>(seq) * a.kv_heads + kv_head) * a.head_tiles + in_group / kPagedHeads];
@@ -30,9 +31,11 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnParams a) 
         return;
     }
     if (row.first == row.last) return;
-    const uint32_t count = row.last - row.first + 1, head = in_group % kPagedHeads;
+    // of a length that changed between the launches whatever lies there: no other parts than there are
+    const uint32_t first = min(row.first, last_part);
+    const uint32_t count = min(row.last - row.first, last_part - first) + 1, head = in_group % kPagedHeads;
     // a row begins in the second slot of its first part and goes on in the others' first
-    const auto line_of = [&](uint32_t i) { return (2ull * (row.first + i) + (i == 0 ? 1 : 0)) * a.heads + head; };
+    const auto line_of = [&](uint32_t i) { return (2ull * (first + i) + (i == 0 ? 1 : 0)) * a.heads + head; };
     float2 ml[kAtOnce];
     f32x4 part[kAtOnce];
     const auto load = [&](uint32_t i0) {
@@ -93,11 +96,6 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedAttnParams a) 
 }
 
 }  // namespace
-
-uint64_t paged_attention_workspace(const PagedCache& c, uint32_t q_heads) {
-    const PagedPlan p = paged_plan(c, q_heads);
-    return p.out_bytes + p.ml_bytes + p.row_bytes;
-}
 
 hipError_t launch_paged_attention(hipStream_t stream, const PagedAttentionArgs& s) {
     const PagedCache& c = s.cache;

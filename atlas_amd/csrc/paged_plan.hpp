@@ -57,6 +57,11 @@ inline PagedPlan paged_plan(const PagedCache& c, uint32_t q_heads) {
     return p;
 }
 
+inline uint64_t paged_attention_workspace(const PagedCache& c, uint32_t q_heads) {
+    const PagedPlan p = paged_plan(c, q_heads);
+    return p.out_bytes + p.ml_bytes + p.row_bytes;
+}
+
 inline constexpr uint32_t kFewRows = 256;  // a workgroup a CU
 
 // The units that a row has at most, where a workgroup a row is sooner done than

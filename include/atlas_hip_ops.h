@@ -562,8 +562,8 @@ int atlas_hip_paged_read(atlas_hip_ctx *ctx, const atlas_paged_cache *cache, con
  * head_dim 2^-37 of |scale| max_i |q_i|, a result by up to 2^-33.  A weight below 2^-126
  * of its row's largest is zero.  A call's result does not depend on timing.
  *
- * q, output and the workspace are 16-byte aligned; output overlaps neither q nor the
- * pages; |scale| <= 2.3e38; sequences * q_heads <= 2^23, sequences * kv_heads *
+ * q, output and the workspace are 16-byte aligned; output and workspace overlap nothing
+ * else of the call's; |scale| <= 2.3e38; sequences * q_heads <= 2^23, sequences * kv_heads *
  * table_width * page_size <= 2^34, a KV head of more than 16 query heads counting once
  * for every 16 -- and its rows are read once for every 16.  The workspace
  * (atlas_hip_paged_attention_workspace bytes; no pointer of the struct is read) is

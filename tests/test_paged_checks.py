@@ -386,3 +386,13 @@ def test_prompts_that_could_not_be_stored_leave_no_sequence(call_that_fails):
 def test_scales_that_are_no_number_with_their_logarithm(checks, scale, fine):
     """f32's largest number over log2(e) is 2.36e38: what is larger made infinities of every query and NaN of every zero."""
     assert (call(checks.check_attention, ATTEND, dict(scale=scale)) is None) == fine
+
+
+@pytest.mark.parametrize("change", [
+    dict(workspace=5 * M), dict(workspace=5 * M + 4096), dict(output=6 * M + 256), dict(output=4 * M), dict(output=2 * M),
+    dict(workspace=3 * M), dict(workspace=4 * M), dict(workspace=2 * M), dict(workspace=M + 4096), dict(lengths=5 * M + 16),
+    dict(table=6 * M), dict(workspace=2 * M - 16),
+])
+def test_attention_outputs_and_workspaces_lie_apart(checks, change):
+    """The join takes its parts' numbers from the workspace: nothing else may write there, nor change the lengths."""
+    assert call(checks.check_attention, ATTEND, change)
