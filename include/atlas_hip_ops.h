@@ -493,7 +493,8 @@ int atlas_hip_kv_evict_q4_0(atlas_hip_ctx *ctx, const uint8_t *cache, uint8_t *c
  * 4096; head_dim at most 256 and a multiple of 4 (F32), 8 (F16) or 32 (Q8_0,
  * Q4_0); kv_heads * head_dim <= 32768; table_width * page_size <= 2^29; at most
  * 2^20 sequences.  The struct is read during the call; the table and whatever else
- * is on the device when its work runs, so a replayed graph sees their new contents.
+ * is on the device when its work runs, so a replayed graph sees their new contents; none
+ * of it may change meanwhile.
  *
  * pages: [page_count][K | V][kv_heads][part], 16-byte aligned; a part is one head's
  * page_size rows of head_dim values.  F32 and F16: [row][head_dim].  Q8_0 and Q4_0:
